@@ -7,6 +7,7 @@
 #include <vector>
 
 #include "ntc_hip.h"
+#include "ntc_ops.h"
 #include "jit.hpp"
 #include "trainer_impl.hpp"
 
@@ -170,6 +171,11 @@ size_t ntc_abi_sizeof(const char* name) {
     if (n == "ntc_dct_desc") return sizeof(ntc_dct_desc);
     if (n == "ntc_level_desc") return sizeof(ntc_level_desc);
     if (n == "ntc_print_stats") return sizeof(ntc_print_stats);
+    if (n == "ntc_logprobs_desc") return sizeof(ntc_logprobs_desc);
+    if (n == "ntc_adamw_desc") return sizeof(ntc_adamw_desc);
+    if (n == "ntc_adamw_tensor") return sizeof(ntc_adamw_tensor);
+    if (n == "ntc_fp8_quantize_desc") return sizeof(ntc_fp8_quantize_desc);
+    if (n == "ntc_fp8_matmul_desc") return sizeof(ntc_fp8_matmul_desc);
     return 0;
 }
 long long ntc_trainer_nparams(const ntc_trainer* t) { return t->t.im->P; }

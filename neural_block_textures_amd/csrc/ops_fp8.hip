@@ -177,7 +177,7 @@ extern "C" int64_t ntc_op_fp8_matmul_float_rows(void) { return 0; }
 extern "C" int ntc_op_fp8_matmul(const ntc_fp8_matmul_desc* d, void* stream, char* why, size_t cap) {
     if (!d) return refuse(why, cap, "no description");
     if (d->M < 0 || d->N < 0 || d->K < 0) return refuse(why, cap, "sizes are not negative");
-    if (d->a_type != NTC_FP8) return refuse(why, cap, "A in 8 bits only");
+    if (d->a_type != NTC_FP8) return refuse(why, cap, "A is a matrix in 8 bits");
     if (d->c_type < 0 || d->c_type > 2) return refuse(why, cap, "C is 32-bit floats, bfloat16 or float16");
     if ((d->a_block_rows != 1 && d->a_block_rows != 128) || (d->b_block_rows != 1 && d->b_block_rows != 128)) return refuse(why, cap, "blocks are 1 x 128 or 128 x 128");
     if (d->ldc < d->N) return refuse(why, cap, "C's rows overlap");

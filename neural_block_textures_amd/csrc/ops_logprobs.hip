@@ -27,6 +27,9 @@ __device__ __forceinline__ void soft_join(Soft& a, Soft b, float k) {
     a.t += b.t;
 }
 
+// log p of one value, in nats: not through (x - m) k, which overflows for a mask of the lowest value
+__device__ __forceinline__ float log_prob(float x, float m, float inv_t, float log_s) { return (x - m) * inv_t - kLn2 * log_s; }
+
 __device__ __forceinline__ long long token_of(const ntc_logprobs_desc& d, long long outer, long long inner) {
     const long long at = outer * d.token_outer_stride + inner * d.token_inner_stride;
     return d.token_bytes == 8 ? ((const long long*)d.tokens)[at] : ((const int*)d.tokens)[at];
@@ -39,7 +42,7 @@ __device__ __forceinline__ float order_of(float x) { return x != x ? -NTC_INF : 
 template <class T> __global__ void __launch_bounds__(256) k_logprobs_row(ntc_logprobs_desc d) {
     const long long row = blockIdx.x, outer = row / d.inner_rows, inner = row % d.inner_rows;
     const T* x = (const T*)d.logits + outer * d.outer_stride + inner * d.inner_stride;
-    const float k = kLog2e / d.temperature;
+    const float inv_t = 1.0f / d.temperature, k = kLog2e / d.temperature;
     __shared__ Soft part[256];
     __shared__ float bv[256];
     __shared__ long long bi[256];
@@ -61,7 +64,7 @@ template <class T> __global__ void __launch_bounds__(256) k_logprobs_row(ntc_log
     if (threadIdx.x == 0) {
         const long long t = token_of(d, outer, inner);
         float lp = 0.0f;
-        if (t != d.ignore_index) lp = t < 0 || t >= d.V ? __builtin_nanf("") : none ? -NTC_INF : kLn2 * (((float)x[t] - a.m) * k - log_s);
+        if (t != d.ignore_index) lp = t < 0 || t >= d.V ? __builtin_nanf("") : none ? -NTC_INF : log_prob((float)x[t], a.m, inv_t, log_s);
         d.logprob[row] = lp;
         d.entropy[row] = none ? 0.0f : kLn2 * (log_s - a.t / a.s);
         d.stats[2 * row] = none ? -NTC_INF : a.m;
@@ -91,7 +94,7 @@ template <class T> __global__ void __launch_bounds__(256) k_logprobs_row(ntc_log
         __syncthreads();
         if (threadIdx.x == 0) {
             d.top_ids[row * d.top + r] = pi;
-            d.top_logprobs[row * d.top + r] = none ? -NTC_INF : kLn2 * ((pv - a.m) * k - log_s);
+            d.top_logprobs[row * d.top + r] = none ? -NTC_INF : log_prob(pv, a.m, inv_t, log_s);
         }
     }
 }

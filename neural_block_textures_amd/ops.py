@@ -11,6 +11,7 @@ take raise ValueError, errors of the runtime RuntimeError. There is no fallback:
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import NamedTuple, Optional
 
 import numpy as np
@@ -194,6 +195,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
         raise ValueError(f"top is 0 to {min(MAX_TOP, V)}, not {top}")
     if not 0 < temperature < 3e38:
         raise ValueError(f"temperature must be positive and finite, not {temperature}")
+    if tokens.dim() > 2:
+        tokens = tokens.contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*_TokenLogprobsGrad.apply(logits, tokens, top, temperature, ignore_index))
     return TokenLogprobs(*_logprobs_forward(logits, tokens, top, temperature, ignore_index)[:4])
@@ -486,7 +489,7 @@ def fp8_linear(x: torch.Tensor, w) -> torch.Tensor:
             raise ValueError(f"x {tuple(shape)} must have w's {w.shape[1]} columns, on its device")
         if x.requires_grad and torch.is_grad_enabled():
             raise ValueError("w in 8 bits is for inference: give the weights themselves for a gradient")
-        x = x.reshape(-1, shape[-1])
+        x = x.reshape(math.prod(shape[:-1]), shape[-1])
         if 0 < x.shape[0] <= library().ntc_op_fp8_matmul_float_rows() and shape[-1]:
             y = _matmul(x if x.stride(1) == 1 or shape[-1] == 1 else x.contiguous(), w, x.dtype)
         else:
@@ -495,5 +498,5 @@ def fp8_linear(x: torch.Tensor, w) -> torch.Tensor:
         _on_gpu("w", w, tuple(_CODE))
         if w.dim() != 2 or w.shape[1] != shape[-1] or w.device != x.device:
             raise ValueError(f"w {tuple(w.shape)} must be a matrix with x's {shape[-1]} columns, on its device")
-        y = _Fp8Linear.apply(x.reshape(-1, shape[-1]), w)
+        y = _Fp8Linear.apply(x.reshape(math.prod(shape[:-1]), shape[-1]), w)
     return y.view(*shape[:-1], y.shape[1])
