@@ -28,6 +28,9 @@ ARCH = "gfx950"
 # off, v_max_f32 needs no canonicalising copies of its operands.
 EXTRA = {"kernels_pop.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"]}
 
+# The 8-bit products keep 256 sums a lane, more than the VGPRs hold beside their operands: these go to the accumulation registers.
+ACC_REGISTERS = {"ops_fp8.hip"}
+
 
 def hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
@@ -41,9 +44,10 @@ def flags(src: str) -> list[str]:
          "-Wno-unused-result", "-Wno-unknown-pragmas"]
     if src.endswith(".hip"):
         f += [f"--offload-arch={ARCH}", "-x", "hip", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-              "-munsafe-fp-atomics",
-              # matrix-core results straight into VGPRs: no AGPR copies between a layer and its activation
-              "-mllvm", "-amdgpu-mfma-vgpr-form"]
+              "-munsafe-fp-atomics"]
+        if src not in ACC_REGISTERS:
+            # matrix-core results straight into VGPRs: no AGPR copies between a layer and its activation
+            f += ["-mllvm", "-amdgpu-mfma-vgpr-form"]
     else:
         f += ["-D__HIP_PLATFORM_AMD__"]
     return f + EXTRA.get(src, [])

@@ -1,10 +1,12 @@
 // Matrices in 8-bit floating point with a power-of-two scale for each block of 128, and their products (include/ntc_ops.h).
+#include <type_traits>
+
 #include "ops_common.hpp"
 
 namespace ntc_ops {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
-typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ float power_of(int b) { return __uint_as_float(b > 0 ? (uint32_t)b << 23 : 1u << 22); }   // 2^(b - 127), b from 0 to 254
 // The bits of |x|, 0 where x is not finite.
@@ -118,37 +120,230 @@ template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_qua
 }
 
 // ---------------------------------------------------------------- products
-// v_mfma_scale_f32_16x16x128: lane l holds 32 bytes of row l % 16 at k = 32 (l / 16) of each operand and that row's exponent; the
-// result's element i of lane l is (first operand's row 4 (l / 16) + i, second's row l % 16). The first operand is B here, so
-// that a lane's four results are neighbours in C's row.
-template <class C> __global__ void __launch_bounds__(256) k_fp8_matmul(ntc_fp8_matmul_desc d) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-    const long long m0 = (long long)blockIdx.y * 64 + 32 * (wave >> 1), n0 = (long long)blockIdx.x * 64 + 32 * (wave & 1);
-    const long long code_stride = ntc_fp8_code_stride(d.K), exp_stride = ntc_fp8_exp_stride(d.K);
-    long long am[2], bn[2];
-    for (int i = 0; i < 2; i++) {
-        am[i] = m0 + 16 * i + r < d.M ? m0 + 16 * i + r : d.M - 1;
-        bn[i] = n0 + 16 * i + r < d.N ? n0 + 16 * i + r : d.N - 1;
+// v_mfma_scale_f32_32x32x64: lane l holds 32 bytes of row l % 32 at k = 32 (l / 32) of each operand, and that row's exponent byte;
+// the result's element i of lane l is (first operand's row 8 (i / 4) + 4 (l / 32) + i % 4, second's row l % 32). The first operand is B
+// here, so that four of a lane's results are neighbours in C's row.
+//
+// A block of four waves makes a TM x TN tile of C, a quarter each. The tiles of A and B come 64 columns at a time straight
+// into LDS (a stage; four of them in turn), two stages ahead of the registers that the products are fed from, which are themselves
+// one stage ahead of the products: one barrier a stage, and no product waits for a load of its own stage. In LDS a row is 64 bytes, and the 16-byte
+// piece c of row r lies at c ^ swizzle(r), which spreads any 8 or 16 rows' pieces over all banks.
+constexpr int kStages = 4;
+__device__ __forceinline__ int swizzle(int r) { return ((r >> 1) & 3) ^ ((r >> 3) & 1); }
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
+// 16 (4) bytes a lane from base + off to LDS at `to` + 16 (4) lane: `to` is the same in all lanes. Nothing waits for it but a vmcnt
+// of the caller's; the compiler's own waits only become stricter by loads that it does not count.
+__device__ __forceinline__ void to_lds16(uint32_t to, uint32_t off, const uint8_t* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(to), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void to_lds4(uint32_t to, uint32_t off, const uint8_t* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(to), "v"(off), "s"(base) : "memory");
+}
+
+struct MatmulArgs {
+    const uint8_t *a, *ae, *b, *be;
+    void* c;
+    long long M, N, ldc;
+    int stride, estride;      // bytes of a row of codes and of exponents
+    int blocks;               // of 128 columns
+    int a_shift, b_shift;     // log2 of the rows of a block
+    int tiles_m, tiles_n;
+    int split_blocks;         // blocks of one part of the sum, a multiple of 4
+};
+
+template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) k_fp8_matmul(MatmulArgs d) {
+    constexpr int RM = TM / 64, RN = TN / 64;              // 32-row tiles of a wave
+    constexpr int kLoads = (TM + TN) / 64;                 // 1 KiB loads a wave and stage
+    constexpr int kStage = (TM + TN) * 64;
+    __shared__ alignas(16) uint8_t lds[kStages * kStage + 2 * 4 * (TM + TN)];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Blocks are dealt to the 8 XCDs in turn, each with an L2 of its own: every XCD takes a run of tiles, which it walks in
+    // columns of up to 8 rows, so that neighbours share their operands there.
+    int tile = blockIdx.x;
+    const int tiles = d.tiles_m * d.tiles_n;
+    {
+        const int each = tiles / 8, rest = tiles % 8, x = tile % 8;
+        tile = x * each + (x < rest ? x : rest) + tile / 8;
     }
-    v4f acc[2][2] = {};
-    for (long long k = 0; k < d.K; k += 128) {
-        v8i a[2], b[2];
-        int ea[2], eb[2];
-        for (int i = 0; i < 2; i++) {
-            a[i] = *(const v8i*)((const uint8_t*)d.a + am[i] * code_stride + k + 32 * g);
-            b[i] = *(const v8i*)(d.b + bn[i] * code_stride + k + 32 * g);
-            ea[i] = d.a_exps[am[i] / d.a_block_rows * exp_stride + k / 128];
-            eb[i] = d.b_exps[bn[i] / d.b_block_rows * exp_stride + k / 128];
-        }
-        for (int i = 0; i < 2; i++)
-            for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a[i], acc[i][j], 0, 0, 0, eb[j], 0, ea[i]);
+    const int group = tile / (8 * d.tiles_n), first = group * 8, high = d.tiles_m - first < 8 ? d.tiles_m - first : 8;
+    const int tm = first + (tile - group * 8 * d.tiles_n) % high, tn = (tile - group * 8 * d.tiles_n) / high;
+    const long long m0 = (long long)tm * TM, n0 = (long long)tn * TN;
+    const int rows_m = d.M - m0 < TM ? (int)(d.M - m0) : TM, rows_n = d.N - n0 < TN ? (int)(d.N - n0) : TN;   // rows past the end read the last one
+    const int block0 = kParts ? blockIdx.y * d.split_blocks : 0;
+    const int blocks = kParts && d.blocks - block0 > d.split_blocks ? d.split_blocks : d.blocks - block0;
+
+    // what this lane loads: pieces of rows of A (the first TM / 64 loads of a wave) and of B
+    const uint8_t* base_a = d.a + m0 * d.stride + block0 * 128;
+    const uint8_t* base_b = d.b + n0 * d.stride + block0 * 128;
+    uint32_t off[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+        const bool is_a = i < TM / 64;
+        const int r = 16 * (4 * (is_a ? i : i - TM / 64) + wave) + (lane >> 2), rows = is_a ? rows_m : rows_n;
+        off[i] = (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)d.stride + 16 * ((lane & 3) ^ swizzle(r));
     }
-    for (int i = 0; i < 2; i++)
-        for (int j = 0; j < 2; j++) {
-            const long long m = m0 + 16 * i + r, n = n0 + 16 * j + 4 * g;
-            if (m >= d.M) continue;
-            for (int q = 0; q < 4; q++) if (n + q < d.N) ((C*)d.c)[m * d.ldc + n + q] = (C)acc[i][j][q];
+    const uint8_t* ebase_a = d.ae + (m0 >> d.a_shift) * d.estride + block0;
+    const uint8_t* ebase_b = d.be + (n0 >> d.b_shift) * d.estride + block0;
+    uint32_t eoff[kLoads / 4];
+#pragma unroll
+    for (int i = 0; i < kLoads / 4; i++) {                 // exponents of 64 rows: the blocks' words of A, then of B
+        const int at = 64 * (4 * i + wave), r = at < TM ? at + lane : at - TM + lane, rows = at < TM ? rows_m : rows_n;
+        eoff[i] = (uint32_t)((r < rows ? r : rows - 1) >> (at < TM ? d.a_shift : d.b_shift)) * (uint32_t)d.estride;
+    }
+    const uint32_t lds0 = lds_address(lds);
+    const int stages = 2 * blocks;
+    const auto load = [&](int s, int i) {                  // load i of stage s; past the end the last stage again, so that every stage has as many
+        const int k = 64 * (s < stages ? s : stages - 1);
+        to_lds16(lds0 + (s % kStages) * kStage + 1024 * wave + 4096 * i, off[i], (i < TM / 64 ? base_a : base_b) + k);
+    };
+    const auto load_exps = [&](int g) {                    // a word of four blocks' exponents for each row, two groups in turn
+        const int b = 4 * g < blocks ? 4 * g : 4 * ((blocks - 1) / 4);
+#pragma unroll
+        for (int i = 0; i < kLoads / 4; i++) {
+            const int at = 64 * (4 * i + wave);
+            to_lds4(lds0 + kStages * kStage + (g & 1) * 4 * (TM + TN) + 4 * at, eoff[i], (at < TM ? ebase_a : ebase_b) + b);
         }
+    };
+
+    const int wm = (wave >> 1) * (TM / 2), wn = (wave & 1) * (TN / 2), r32 = lane & 31, half = lane >> 5;
+    v8i fa[2][RM], fb[2][RN];
+    int ea[RM], eb[RN], na[RM], nb[RN];                    // exponents of this group of four blocks and of the next
+    // Half an operand: the 2 (RM + RN) pieces of a stage in the order in which its products need them (A's first tile, B's, A's others).
+    const auto fetch = [&](int s, int set, int p) {
+        const bool is_a = p < 2 || p >= 2 * RN + 2;
+        const int i = p < 2 ? 0 : is_a ? (p - 2 * RN) >> 1 : (p - 2) >> 1, r = (is_a ? wm : TM + wn) + 32 * i + r32, h = p & 1;
+        const int4 x = *(const int4*)(lds + (s % kStages) * kStage + 64 * r + 16 * ((2 * half + h) ^ swizzle(r)));
+        v8i& to = is_a ? fa[set][i] : fb[set][i];
+        to[4 * h] = x.x; to[4 * h + 1] = x.y; to[4 * h + 2] = x.z; to[4 * h + 3] = x.w;
+    };
+    const auto fetch_exps = [&](int g) {
+        const int* at = (const int*)(lds + kStages * kStage) + (g & 1) * (TM + TN);
+#pragma unroll
+        for (int i = 0; i < RM; i++) na[i] = at[wm + 32 * i + r32];
+#pragma unroll
+        for (int i = 0; i < RN; i++) nb[i] = at[TM + wn + 32 * i + r32];
+    };
+    v16f acc[RM][RN] = {};
+    // All but the newest stage's loads have landed, in every wave; and every wave has its operands of the stage before (their products
+    // have been issued), so that the buffer they came from is free.
+    const auto arrive = [&] {
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0x0f70 | (kLoads & 15) | ((kLoads >> 4) << 14));
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    // A stage: its RM RN products and, spread evenly between them, the reads of the next stage and the loads of the third after. A wave has
+    // its SIMD to itself and issues in order: what is not spread holds the products up. kByte: the block's byte of the exponents' words.
+    const auto stage = [&](int s, auto set_, auto byte_, auto&& first, auto&& last) {
+        constexpr int n = RM * RN, reads = 2 * (RM + RN), set = set_.value, kByte = byte_.value;
+        arrive();
+#pragma unroll
+        for (int q = 0; q < n; q++) {
+            const int i = q / RN, j = q % RN;
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[set][j], fa[set][i], acc[i][j], 0, 0, kByte, eb[j], kByte, ea[i]);
+            if (q == 0) first();
+#pragma unroll
+            for (int p = q * reads / n; p < (q + 1) * reads / n; p++) fetch(s + 1, set ^ 1, p);
+#pragma unroll
+            for (int p = q * kLoads / n; p < (q + 1) * kLoads / n; p++) load(s + 3, p);
+            if (q == n - 1) last();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    const auto none = [] {};
+    const auto next_exps = [&] {
+#pragma unroll
+        for (int i = 0; i < RM; i++) ea[i] = na[i];
+#pragma unroll
+        for (int i = 0; i < RN; i++) eb[i] = nb[i];
+    };
+
+    load_exps(0);
+#pragma unroll
+    for (int i = 0; i < 3 * kLoads; i++) load(i / kLoads, i % kLoads);
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    arrive();
+#pragma unroll
+    for (int p = 0; p < 2 * (RM + RN); p++) fetch(0, 0, p);
+    fetch_exps(0);
+    using std::integral_constant;
+    const integral_constant<int, 0> c0;
+    const integral_constant<int, 1> c1;
+    const integral_constant<int, 2> c2;
+    const integral_constant<int, 3> c3;
+    int b = 0;
+    for (; b + 4 <= blocks; b += 4) {                      // the loads of group b / 4 + 1 have 7 stages until they are read
+        next_exps();
+        stage(2 * b, c0, c0, [&] { load_exps((b >> 2) + 1); }, none);
+        stage(2 * b + 1, c1, c0, none, none);
+        stage(2 * b + 2, c0, c1, none, none);
+        stage(2 * b + 3, c1, c1, none, none);
+        stage(2 * b + 4, c0, c2, none, none);
+        stage(2 * b + 5, c1, c2, none, none);
+        stage(2 * b + 6, c0, c3, none, none);
+        stage(2 * b + 7, c1, c3, none, [&] { fetch_exps((b >> 2) + 1); });
+    }
+    next_exps();
+    for (; b < blocks; b++) {                              // one to three blocks more
+        stage(2 * b, c0, c0, none, none);
+        stage(2 * b + 1, c1, c0, none, none);
+#pragma unroll
+        for (int i = 0; i < RM; i++) ea[i] = (unsigned)ea[i] >> 8;
+#pragma unroll
+        for (int i = 0; i < RN; i++) eb[i] = (unsigned)eb[i] >> 8;
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);                    // loads past the end must not land after the block has gone
+
+    if (kParts) d.c = (float*)d.c + blockIdx.y * d.M * d.N;
+    const bool whole = (d.ldc & 3) == 0 && ((uintptr_t)d.c & (4 * sizeof(C) - 1)) == 0;
+#pragma unroll
+    for (int i = 0; i < RM; i++) {
+        const long long m = m0 + wm + 32 * i + r32;
+        if (m >= d.M) continue;
+#pragma unroll
+        for (int j = 0; j < RN; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const long long n = n0 + wn + 32 * j + 8 * q + 4 * half;
+                C* to = (C*)d.c + m * d.ldc + n;
+                if (whole && n + 4 <= d.N) {
+                    Run<C, 4> o;
+                    for (int k = 0; k < 4; k++) o.v[k] = (C)acc[i][j][4 * q + k];
+                    *(Run<C, 4>*)to = o;
+                } else {
+                    for (int k = 0; k < 4; k++) if (n + k < d.N) to[k] = (C)acc[i][j][4 * q + k];
+                }
+            }
+    }
+}
+
+// The parts of a split sum, added in order.
+template <class C> __global__ void __launch_bounds__(256) k_fp8_join(const float* parts, int n_parts, long long M, long long N, long long ldc, C* c) {
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x), size = M * N;
+    if (i >= size) return;
+    float s = 0.0f;
+    for (int p = 0; p < n_parts; p++) s += parts[p * size + i];
+    c[i / N * ldc + i % N] = (C)s;
+}
+
+// How a product is divided.
+struct Plan { int tile, parts, split_blocks; };
+static Plan plan_of(int64_t M, int64_t N, int64_t K) {
+    const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    const int64_t blocks = up(K, 128);
+    Plan p = { 256, 1, (int)blocks };
+    if (up(M, 256) * up(N, 256) < 200) p.tile = 128;
+    const int64_t tiles = up(M, p.tile) * up(N, p.tile);
+    if (p.tile == 128 && tiles < 256 && blocks > 8) {
+        int64_t parts = up(512, tiles);
+        if (parts > blocks / 4) parts = blocks / 4;
+        p.split_blocks = (int)(up(up(blocks, parts), 4) * 4);
+        p.parts = (int)up(blocks, p.split_blocks);
+    }
+    return p;
 }
 
 }  // namespace ntc_ops
@@ -171,8 +366,42 @@ extern "C" int ntc_op_fp8_quantize(const ntc_fp8_quantize_desc* d, void* stream,
     return launched(why, cap);
 }
 
-extern "C" size_t ntc_op_fp8_matmul_workspace(int64_t, int64_t, int64_t) { return 0; }
+extern "C" size_t ntc_op_fp8_matmul_workspace(int64_t M, int64_t N, int64_t K) {
+    if (M < 1 || N < 1 || K < 1) return 0;
+    const Plan p = plan_of(M, N, K);
+    return p.parts > 1 ? (size_t)p.parts * M * N * 4 : 0;
+}
 extern "C" int64_t ntc_op_fp8_matmul_float_rows(void) { return 0; }
+
+template <int T, class C> static void launch_matmul(const MatmulArgs& A, int parts, hipStream_t s) {
+    const unsigned tiles = (unsigned)(A.tiles_m * A.tiles_n);
+    if (parts > 1) k_fp8_matmul<T, T, float, true><<<dim3(tiles, parts), 256, 0, s>>>(A);
+    else k_fp8_matmul<T, T, C, false><<<tiles, 256, 0, s>>>(A);
+}
+
+template <class C> static void run_matmul(const ntc_fp8_matmul_desc* d, hipStream_t s) {
+    const Plan p = plan_of(d->M, d->N, d->K);
+    MatmulArgs A;
+    A.a = (const uint8_t*)d->a;
+    A.ae = d->a_exps;
+    A.b = d->b;
+    A.be = d->b_exps;
+    A.M = d->M;
+    A.N = d->N;
+    A.stride = (int)ntc_fp8_code_stride(d->K);
+    A.estride = (int)ntc_fp8_exp_stride(d->K);
+    A.blocks = (int)((d->K + 127) / 128);
+    A.a_shift = d->a_block_rows == 128 ? 7 : 0;
+    A.b_shift = d->b_block_rows == 128 ? 7 : 0;
+    A.tiles_m = (int)((d->M + p.tile - 1) / p.tile);
+    A.tiles_n = (int)((d->N + p.tile - 1) / p.tile);
+    A.split_blocks = p.split_blocks;
+    A.c = p.parts > 1 ? d->workspace : d->c;
+    A.ldc = p.parts > 1 ? d->N : d->ldc;
+    if (p.tile == 256) launch_matmul<256, C>(A, p.parts, s);
+    else launch_matmul<128, C>(A, p.parts, s);
+    if (p.parts > 1) k_fp8_join<C><<<(unsigned)((d->M * d->N + 255) / 256), 256, 0, s>>>((const float*)d->workspace, p.parts, d->M, d->N, d->ldc, (C*)d->c);
+}
 
 extern "C" int ntc_op_fp8_matmul(const ntc_fp8_matmul_desc* d, void* stream, char* why, size_t cap) {
     if (!d) return refuse(why, cap, "no description");
@@ -181,11 +410,14 @@ extern "C" int ntc_op_fp8_matmul(const ntc_fp8_matmul_desc* d, void* stream, cha
     if (d->c_type < 0 || d->c_type > 2) return refuse(why, cap, "C is 32-bit floats, bfloat16 or float16");
     if ((d->a_block_rows != 1 && d->a_block_rows != 128) || (d->b_block_rows != 1 && d->b_block_rows != 128)) return refuse(why, cap, "blocks are 1 x 128 or 128 x 128");
     if (d->ldc < d->N) return refuse(why, cap, "C's rows overlap");
-    const int64_t gy = (d->M + 63) / 64, gx = (d->N + 63) / 64;
-    if (gy > 65535 || gx > 0x7fffffff) return refuse(why, cap, "at most 65535 * 64 rows");
-    if (!gx || !gy) return 0;
-    if (!d->c || (d->K && (!d->a || !d->a_exps || !d->b || !d->b_exps))) return refuse(why, cap, "a null pointer");
-    const auto go = [&](auto kernel) { kernel<<<dim3((unsigned)gx, (unsigned)gy), 256, 0, (hipStream_t)stream>>>(*d); };
-    d->c_type == NTC_F32 ? go(k_fp8_matmul<f32>) : d->c_type == NTC_BF16 ? go(k_fp8_matmul<bf16>) : go(k_fp8_matmul<f16>);
+    if (d->K > 1 << 23 || d->M > (int64_t)1 << 36 || d->N > (int64_t)1 << 36 || (d->M + 127) / 128 * ((d->N + 127) / 128) > 0x7fffffff)
+        return refuse(why, cap, "K at most 2^23, and fewer than 2^31 tiles of 128 x 128");
+    if (!d->M || !d->N) return 0;
+    if (!d->K) return refuse(why, cap, "K is at least 1");
+    if (!d->c || !d->a || !d->a_exps || !d->b || !d->b_exps) return refuse(why, cap, "a null pointer");
+    if ((((uintptr_t)d->a | (uintptr_t)d->b) & 15) || (((uintptr_t)d->a_exps | (uintptr_t)d->b_exps) & 3)) return refuse(why, cap, "codes start at multiples of 16 bytes, exponents of 4");
+    if (!d->workspace && ntc_op_fp8_matmul_workspace(d->M, d->N, d->K)) return refuse(why, cap, "a null workspace");
+    const hipStream_t s = (hipStream_t)stream;
+    d->c_type == NTC_F32 ? run_matmul<f32>(d, s) : d->c_type == NTC_BF16 ? run_matmul<bf16>(d, s) : run_matmul<f16>(d, s);
     return launched(why, cap);
 }

@@ -415,8 +415,8 @@ def _check_fp8(name: str, t) -> None:
     want = ((R, -(-K // 128) * 128), (-(-R // t.block_rows) if t.block_rows in (1, 128) else -1, -(-K // 512) * 4))
     for what, x, shape in zip(("codes", "exps"), (t.codes, t.exps), want):
         _on_gpu(f"{name}.{what}", x, (torch.uint8,))
-        if tuple(x.shape) != shape or not x.is_contiguous() or x.device != t.codes.device:
-            raise ValueError(f"{name}.{what} must be contiguous and {shape} for a matrix {tuple(t.shape)} in blocks of {t.block_rows} x 128")
+        if tuple(x.shape) != shape or not x.is_contiguous() or x.device != t.codes.device or x.data_ptr() % 16:
+            raise ValueError(f"{name}.{what} must be contiguous, start at a multiple of 16 bytes and be {shape} for a matrix {tuple(t.shape)} in blocks of {t.block_rows} x 128")
 
 
 def _matmul(a, b: Fp8Tensor, dtype: torch.dtype) -> torch.Tensor:
