@@ -21,6 +21,8 @@ template <> inline constexpr int type_code<bf16> = NTC_BF16;
 template <> inline constexpr int type_code<f16> = NTC_F16;
 
 template <class T, int N> struct alignas(sizeof(T) * N) Run { T v[N]; };
+// A run at any element's address: one wide access all the same (the hardware takes unaligned ones, at the cost of the lines it crosses).
+template <class T, int N> struct __attribute__((packed, aligned(sizeof(T)))) LooseRun { T v[N]; };
 
 inline size_t type_size(int t) { return t == NTC_F32 ? 4 : 2; }
 

@@ -9,11 +9,6 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ float power_of(int b) { return __uint_as_float(b > 0 ? (uint32_t)b << 23 : 1u << 22); }   // 2^(b - 127), b from 0 to 254
-// The bits of |x|, 0 where x is not finite.
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-    const uint32_t a = __float_as_uint(x) & 0x7fffffffu;
-    return a < 0x7f800000u ? a : 0u;
-}
 // The exponent byte of a block whose largest finite magnitude has these bits: amax <= 448 * 2^(E - 127).
 __device__ __forceinline__ int exp_byte(uint32_t most) {
     const int e = (int)(most >> 23) - 8 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0);
@@ -26,96 +21,149 @@ __device__ __forceinline__ uint32_t to_fp8x4(float a, float b, float c, float d)
     return r;
 }
 
+// Largest magnitudes of finite values, as integers that order like them: 16-bit types two to a word, so that one instruction
+// takes two; of_max() gives the bits of the 32-bit float.
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, a), __builtin_bit_cast(us2, b)));
+}
+__device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) { return a > b ? a : b; }
+template <class T> struct Magnitude {                       // bf16 and f16
+    static constexpr uint32_t kInf = type_code<T> == NTC_BF16 ? 0x7f80u : 0x7c00u;
+    static __device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b) { return max_pair(a, b); }
+    // of eight values; non-finite ones count as 0 (seldom there: looked for once all eight are joined)
+    static __device__ __forceinline__ uint32_t of(const Run<T, 8>& x) {
+        const uint4 w = __builtin_bit_cast(uint4, x);
+        const uint32_t v[4] = { w.x & 0x7fff7fffu, w.y & 0x7fff7fffu, w.z & 0x7fff7fffu, w.w & 0x7fff7fffu };
+        uint32_t m = max_pair(max_pair(v[0], v[1]), max_pair(v[2], v[3]));
+        if (max_word(m & 0xffffu, m >> 16) >= kInf) {
+            m = 0;
+            for (int i = 0; i < 4; i++) m = max_pair(m, ((v[i] & 0xffffu) >= kInf ? 0u : v[i] & 0xffffu) | (v[i] >> 16 >= kInf ? 0u : v[i] & 0xffff0000u));
+        }
+        return m;
+    }
+    static __device__ __forceinline__ uint32_t float_bits(uint32_t m) {
+        const uint16_t h = (uint16_t)max_word(m & 0xffffu, m >> 16);
+        return __float_as_uint((float)__builtin_bit_cast(T, h));
+    }
+    // of one value
+    static __device__ __forceinline__ uint32_t one(T x) {
+        const uint32_t a = __builtin_bit_cast(uint16_t, x) & 0x7fffu;
+        return a >= kInf ? 0u : a;
+    }
+};
+template <> struct Magnitude<f32> {
+    static __device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b) { return max_word(a, b); }
+    static __device__ __forceinline__ uint32_t one(float x) {
+        const uint32_t a = __float_as_uint(x) & 0x7fffffffu;
+        return a < 0x7f800000u ? a : 0u;
+    }
+    static __device__ __forceinline__ uint32_t of(const Run<float, 8>& x) {
+        uint32_t m = 0;
+        for (int j = 0; j < 8; j++) m = max_word(m, one(x.v[j]));
+        return m;
+    }
+    static __device__ __forceinline__ uint32_t float_bits(uint32_t m) { return m; }
+};
+
 // ---------------------------------------------------------------- to 8 bits
 // A block of 256 threads takes a 128 x 128 tile: thread t holds 8 columns (8 (t % 16) ..) of the 8 rows 8 (t / 16) .., so that a
-// row's largest is a reduction over 16 lanes, and a column's codes of 8 rows are one 8-byte word of the transposed tile.
+// row's largest is a reduction over 16 lanes, and a column's codes of 8 rows are one 8-byte word of the transposed tile. x is
+// read once for both orders. Bound by memory.
 template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_quantize(ntc_fp8_quantize_desc d) {
+    using Mag = Magnitude<T>;
     __shared__ uint32_t most[4][128];
-    __shared__ alignas(16) uint8_t tile[128][144];
+    __shared__ alignas(16) uint8_t tile[128 * 128];        // transposed; word w of 8 rows of column c at w ^ (c / 8)
     const long long r0 = (long long)blockIdx.y * 128, c0 = (long long)blockIdx.x * 128;
     const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4, wave = threadIdx.x >> 6;
-    const long long c = c0 + 8 * cg, r = r0 + 8 * rg;
-    float x[8][8];
-    for (int i = 0; i < 8; i++)
-        for (int j = 0; j < 8; j++) x[i][j] = r + i < d.R && c + j < d.K ? (float)((const T*)d.x)[(r + i) * d.row_stride + c + j] : 0.0f;
-    const long long code_stride = ntc_fp8_code_stride(d.K), exp_stride = ntc_fp8_exp_stride(d.K), blocks = (d.K + 127) / 128;
-    const long long code_stride_t = ntc_fp8_code_stride(d.R), exp_stride_t = ntc_fp8_exp_stride(d.R), blocks_t = (d.R + 127) / 128;
+    const int rows = d.R - r0 < 128 ? (int)(d.R - r0) : 128, cols = d.K - c0 < 128 ? (int)(d.K - c0) : 128;   // of this tile
+    const T* from = (const T*)d.x + (r0 + 8 * rg) * d.row_stride + c0 + 8 * cg;
+    Run<T, 8> x[8];
+    if (rows == 128 && cols == 128) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) { const auto v = *(const LooseRun<T, 8>*)(from + i * d.row_stride); for (int j = 0; j < 8; j++) x[i].v[j] = v.v[j]; }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (8 * rg + i < rows && 8 * cg + 8 <= cols) { const auto v = *(const LooseRun<T, 8>*)(from + i * d.row_stride); for (int j = 0; j < 8; j++) x[i].v[j] = v.v[j]; }
+            else for (int j = 0; j < 8; j++) x[i].v[j] = 8 * rg + i < rows && 8 * cg + j < cols ? from[i * d.row_stride + j] : (T)0.0f;
+        }
+    }
+    const long long code_stride = ntc_fp8_code_stride(d.K), exp_stride = ntc_fp8_exp_stride(d.K), code_stride_t = ntc_fp8_code_stride(d.R), exp_stride_t = ntc_fp8_exp_stride(d.R);
+    // a row of exponents is written by the tile that has its block; the last one also clears what follows
+    const auto put_exp = [](uint8_t* row, long long at, int byte, bool last, long long stride) {
+        row[at] = (uint8_t)byte;
+        if (last) for (long long k = at + 1; k < stride; k++) row[k] = 0;
+    };
+    const bool last_c = c0 + 128 >= d.K, last_r = r0 + 128 >= d.R;
     int block_byte = 0;
     if (kBlock) {
         uint32_t b = 0;
-        for (int i = 0; i < 8; i++) for (int j = 0; j < 8; j++) { const uint32_t a = finite_bits(x[i][j]); b = a > b ? a : b; }
-        for (int w = 1; w < 64; w <<= 1) { const uint32_t o = __shfl_xor(b, w); b = o > b ? o : b; }
+#pragma unroll
+        for (int i = 0; i < 8; i++) b = Mag::join(b, Mag::of(x[i]));
+#pragma unroll
+        for (int w = 1; w < 64; w <<= 1) b = Mag::join(b, __shfl_xor(b, w));
         if ((threadIdx.x & 63) == 0) most[wave][0] = b;
         __syncthreads();
-        for (int w = 0; w < 4; w++) b = most[w][0] > b ? most[w][0] : b;
-        block_byte = exp_byte(b);
+        b = Mag::join(Mag::join(most[0][0], most[1][0]), Mag::join(most[2][0], most[3][0]));
+        block_byte = exp_byte(Mag::float_bits(b));
         if (threadIdx.x == 0) {
-            if (d.codes) {
-                uint8_t* e = d.exps + blockIdx.y * exp_stride;
-                e[blockIdx.x] = (uint8_t)block_byte;
-                if (blockIdx.x == blocks - 1) for (long long k = blocks; k < exp_stride; k++) e[k] = 0;
-            }
-            if (d.codes_t) {
-                uint8_t* e = d.exps_t + blockIdx.x * exp_stride_t;
-                e[blockIdx.y] = (uint8_t)block_byte;
-                if (blockIdx.y == blocks_t - 1) for (long long k = blocks_t; k < exp_stride_t; k++) e[k] = 0;
-            }
+            if (d.codes) put_exp(d.exps + blockIdx.y * exp_stride, blockIdx.x, block_byte, last_c, exp_stride);
+            if (d.codes_t) put_exp(d.exps_t + blockIdx.x * exp_stride_t, blockIdx.y, block_byte, last_r, exp_stride_t);
         }
     }
     if (d.codes) {
+        uint8_t* to = d.codes + (r0 + 8 * rg) * code_stride + c0 + 8 * cg;
+#pragma unroll
         for (int i = 0; i < 8; i++) {
             int byte = block_byte;
             if (!kBlock) {
-                uint32_t b = 0;
-                for (int j = 0; j < 8; j++) { const uint32_t a = finite_bits(x[i][j]); b = a > b ? a : b; }
-                for (int w = 1; w < 16; w <<= 1) { const uint32_t o = __shfl_xor(b, w); b = o > b ? o : b; }
-                byte = exp_byte(b);
-                if (cg == 0 && r + i < d.R) {
-                    uint8_t* e = d.exps + (r + i) * exp_stride;
-                    e[blockIdx.x] = (uint8_t)byte;
-                    if (blockIdx.x == blocks - 1) for (long long k = blocks; k < exp_stride; k++) e[k] = 0;
-                }
+                uint32_t b = Mag::of(x[i]);
+#pragma unroll
+                for (int w = 1; w < 16; w <<= 1) b = Mag::join(b, __shfl_xor(b, w));
+                byte = exp_byte(Mag::float_bits(b));
+                if (cg == 0 && 8 * rg + i < rows) put_exp(d.exps + (r0 + 8 * rg + i) * exp_stride, blockIdx.x, byte, last_c, exp_stride);
             }
-            if (r + i >= d.R) continue;
             const float s = power_of(254 - byte);
             uint2 o;
-            o.x = to_fp8x4(x[i][0] * s, x[i][1] * s, x[i][2] * s, x[i][3] * s);
-            o.y = to_fp8x4(x[i][4] * s, x[i][5] * s, x[i][6] * s, x[i][7] * s);
-            *(uint2*)(d.codes + (r + i) * code_stride + c) = o;
+            o.x = to_fp8x4((float)x[i].v[0] * s, (float)x[i].v[1] * s, (float)x[i].v[2] * s, (float)x[i].v[3] * s);
+            o.y = to_fp8x4((float)x[i].v[4] * s, (float)x[i].v[5] * s, (float)x[i].v[6] * s, (float)x[i].v[7] * s);
+            if (8 * rg + i < rows) *(uint2*)(to + i * code_stride) = o;
         }
     }
     if (!d.codes_t) return;
     if (!kBlock) {
+#pragma unroll
         for (int j = 0; j < 8; j++) {
             uint32_t b = 0;
-            for (int i = 0; i < 8; i++) { const uint32_t a = finite_bits(x[i][j]); b = a > b ? a : b; }
-            for (int w = 16; w < 64; w <<= 1) { const uint32_t o = __shfl_xor(b, w); b = o > b ? o : b; }
+#pragma unroll
+            for (int i = 0; i < 8; i++) b = max_word(b, Mag::one(x[i].v[j]));
+            b = max_word(b, __shfl_xor(b, 16));
+            b = max_word(b, __shfl_xor(b, 32));
             if ((threadIdx.x & 48) == 0) most[wave][8 * cg + j] = b;
         }
         __syncthreads();
     }
+#pragma unroll
     for (int j = 0; j < 8; j++) {
         int byte = block_byte;
         if (!kBlock) {
-            uint32_t b = 0;
-            for (int w = 0; w < 4; w++) b = most[w][8 * cg + j] > b ? most[w][8 * cg + j] : b;
-            byte = exp_byte(b);
-            if (rg == 0 && c + j < d.K) {
-                uint8_t* e = d.exps_t + (c + j) * exp_stride_t;
-                e[blockIdx.y] = (uint8_t)byte;
-                if (blockIdx.y == blocks_t - 1) for (long long k = blocks_t; k < exp_stride_t; k++) e[k] = 0;
-            }
+            const int c = 8 * cg + j;
+            byte = exp_byte(Mag::float_bits(max_word(max_word(most[0][c], most[1][c]), max_word(most[2][c], most[3][c]))));
+            if (rg == 0 && c < cols) put_exp(d.exps_t + (c0 + c) * exp_stride_t, blockIdx.y, byte, last_r, exp_stride_t);
         }
         const float s = power_of(254 - byte);
         uint2 o;
-        o.x = to_fp8x4(x[0][j] * s, x[1][j] * s, x[2][j] * s, x[3][j] * s);
-        o.y = to_fp8x4(x[4][j] * s, x[5][j] * s, x[6][j] * s, x[7][j] * s);
-        *(uint2*)&tile[8 * cg + j][8 * rg] = o;
+        o.x = to_fp8x4((float)x[0].v[j] * s, (float)x[1].v[j] * s, (float)x[2].v[j] * s, (float)x[3].v[j] * s);
+        o.y = to_fp8x4((float)x[4].v[j] * s, (float)x[5].v[j] * s, (float)x[6].v[j] * s, (float)x[7].v[j] * s);
+        *(uint2*)(tile + 128 * (8 * cg + j) + 8 * (rg ^ cg)) = o;
     }
     __syncthreads();
+#pragma unroll
     for (int p = 0; p < 4; p++) {
-        const int col = 32 * p + (threadIdx.x >> 3), part = threadIdx.x & 7;
-        if (c0 + col < d.K) *(uint4*)(d.codes_t + (c0 + col) * code_stride_t + r0 + 16 * part) = *(const uint4*)&tile[col][16 * part];
+        const int c = 32 * p + (threadIdx.x >> 3), part = threadIdx.x & 7, g = c >> 3;
+        const uint4 v = *(const uint4*)(tile + 128 * c + 8 * ((2 * part) ^ (g & 14)));
+        if (c < cols) *(uint4*)(d.codes_t + (c0 + c) * code_stride_t + r0 + 16 * part) = g & 1 ? uint4{ v.z, v.w, v.x, v.y } : v;
     }
 }
 
@@ -297,27 +345,56 @@ template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds_
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);                    // loads past the end must not land after the block has gone
 
-    if (kParts) d.c = (float*)d.c + blockIdx.y * d.M * d.N;
-    const bool whole = (d.ldc & 3) == 0 && ((uintptr_t)d.c & (4 * sizeof(C) - 1)) == 0;
+    C* const quarter = (C*)d.c + (kParts ? (long long)blockIdx.y * d.M * d.N : 0) + (m0 + wm) * d.ldc + n0 + wn;
+    const int left_m = rows_m - wm, left_n = rows_n - wn;
+    const auto put = [&](C* to, const auto& run, int m, int n, auto guard) {
+        constexpr int R = sizeof(run) / sizeof(C);
+        if (!guard.value) { *(LooseRun<C, R>*)to = *(const LooseRun<C, R>*)&run; return; }
+        if (m >= left_m) return;
+        if (n + R <= left_n) *(LooseRun<C, R>*)to = *(const LooseRun<C, R>*)&run;
+        else for (int k = 0; k < R; k++) if (n + k < left_n) to[k] = run.v[k];
+    };
+    const auto store = [&](auto guard) {
+    if constexpr (sizeof(C) == 2) {
+        // Four results a lane are 8 bytes of a row: 32 rows of the wave's quarter at a time go through LDS, so that rows are stored whole.
+        constexpr int kRow = TN, kPieces = kRow / 16;       // bytes of a row of the quarter, and its 16-byte pieces
+        __builtin_amdgcn_s_barrier();                       // every wave has its last operands
+        asm volatile("" ::: "memory");
+        uint8_t* own = lds + wave * 32 * kRow;
 #pragma unroll
-    for (int i = 0; i < RM; i++) {
-        const long long m = m0 + wm + 32 * i + r32;
-        if (m >= d.M) continue;
+        for (int i = 0; i < RM; i++) {
 #pragma unroll
-        for (int j = 0; j < RN; j++)
+            for (int j = 0; j < RN; j++)
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const long long n = n0 + wn + 32 * j + 8 * q + 4 * half;
-                C* to = (C*)d.c + m * d.ldc + n;
-                if (whole && n + 4 <= d.N) {
+                for (int q = 0; q < 4; q++) {
                     Run<C, 4> o;
                     for (int k = 0; k < 4; k++) o.v[k] = (C)acc[i][j][4 * q + k];
-                    *(Run<C, 4>*)to = o;
-                } else {
-                    for (int k = 0; k < 4; k++) if (n + k < d.N) to[k] = (C)acc[i][j][4 * q + k];
+                    *(Run<C, 4>*)(own + r32 * kRow + 16 * ((4 * j + q) ^ (r32 & (kPieces - 1))) + 8 * half) = o;
                 }
+#pragma unroll
+            for (int p = 0; p < 32 * kPieces / 64; p++) {
+                const int r = p * (64 / kPieces) + lane / kPieces, piece = lane % kPieces;
+                const Run<C, 8> x = *(const Run<C, 8>*)(own + r * kRow + 16 * (piece ^ (r & (kPieces - 1))));
+                put(quarter + (32 * i + r) * d.ldc + 8 * piece, x, 32 * i + r, 8 * piece, guard);
             }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < RM; i++)
+#pragma unroll
+            for (int j = 0; j < RN; j++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int m = 32 * i + r32, n = 32 * j + 8 * q + 4 * half;
+                    Run<C, 4> o;
+                    for (int k = 0; k < 4; k++) o.v[k] = (C)acc[i][j][4 * q + k];
+                    put(quarter + m * d.ldc + n, o, m, n, guard);
+                }
     }
+    };
+    // (one branch for the whole tile: a guard at every store of a full one is 5% of the largest product)
+    if (rows_m == TM && rows_n == TN) store(std::false_type());
+    else store(std::true_type());
 }
 
 // The parts of a split sum, added in order.
