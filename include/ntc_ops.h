@@ -27,8 +27,8 @@ enum { NTC_STATE_BLOCK = 256 };                      /* values that share one sc
  * A token equal to ignore_index has logprob 0; another token outside [0, V) has logprob NaN. A row of only -inf has
  * logprob and top_logprob -inf and entropy 0; a NaN or +inf makes a row's results NaN.
  * stats (2 floats a row) is what the backward pass needs: the largest x (-inf for a row of only -inf) and the log2
- * of the sum of exp(y - its largest). workspace: ntc_op_token_logprobs_workspace() bytes, zero at its first use
- * (a call leaves it zero where it has to be), not shared by calls that may overlap. */
+ * of the sum of exp(y - its largest). workspace: ntc_op_token_logprobs_workspace() bytes of any contents, not shared by calls
+ * that may overlap (null where that is 0). */
 typedef struct ntc_logprobs_desc {
     const void* logits;
     const void* tokens;
@@ -52,7 +52,7 @@ typedef struct ntc_logprobs_desc {
     void* dlogits;        /* [rows][V], contiguous, of `dtype` */
 } ntc_logprobs_desc;
 
-size_t ntc_op_token_logprobs_workspace(int64_t rows, int64_t V, int32_t top);
+size_t ntc_op_token_logprobs_workspace(int64_t rows, int64_t V, int32_t dtype, int32_t top);
 int ntc_op_token_logprobs(const ntc_logprobs_desc* d, void* stream, char* why, size_t why_cap);
 /* dlogits from logits, tokens, stats, entropy, top_ids and the gradients of the outputs:
  *   dx_v = 1/T [ g_lp (v == token) + sum_k g_top_k (v == id_k) - p_v (g_lp + sum_k g_top_k + g_H (log p_v + H)) ]

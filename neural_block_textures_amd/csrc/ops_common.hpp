@@ -4,6 +4,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "ntc_ops.h"
 
 namespace ntc_ops {
@@ -31,6 +33,31 @@ __device__ __forceinline__ int lane_id() { return (int)__builtin_amdgcn_mbcnt_hi
 __device__ __forceinline__ float read_lane(float x, int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l)); }
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }   // one instruction, 1 ulp; 2^-inf = 0
 __device__ __forceinline__ float fast_log2(float x) { return __builtin_amdgcn_logf(x); }
+
+// Reductions over aligned groups of 16 lanes (rotations within a row of the vector registers) and of 64 (rows swapped on the
+// way): every lane gets the result, and no shared memory is used.
+template <int kRor> __device__ __forceinline__ uint32_t rotate16(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + kRor, 0xf, 0xf, false); }
+template <class V, class F> __device__ __forceinline__ V reduce16(V x, F f) {
+    const auto turn = [](V v, auto n) { return __builtin_bit_cast(V, rotate16<n.value>(__builtin_bit_cast(uint32_t, v))); };
+    x = f(x, turn(x, std::integral_constant<int, 8>()));
+    x = f(x, turn(x, std::integral_constant<int, 4>()));
+    x = f(x, turn(x, std::integral_constant<int, 2>()));
+    return f(x, turn(x, std::integral_constant<int, 1>()));
+}
+// of lanes l and l ^ 16, then l ^ 32
+template <class V, class F> __device__ __forceinline__ V reduce_rows(V x, F f) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto p = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    x = f(__builtin_bit_cast(V, (uint32_t)p[0]), __builtin_bit_cast(V, (uint32_t)p[1]));
+    const uint32_t c = __builtin_bit_cast(uint32_t, x);
+    const auto q = __builtin_amdgcn_permlane32_swap(c, c, false, false);
+    return f(__builtin_bit_cast(V, (uint32_t)q[0]), __builtin_bit_cast(V, (uint32_t)q[1]));
+}
+template <class V, class F> __device__ __forceinline__ V reduce64(V x, F f) { return reduce_rows(reduce16(x, f), f); }
+template <int kGroup, class V, class F> __device__ __forceinline__ V reduce(V x, F f) {
+    if constexpr (kGroup == 16) return reduce16(x, f);
+    else return reduce64(x, f);
+}
 
 // ---------------------------------------------------------------- refusals
 inline int refuse(char* why, size_t cap, const char* text) {

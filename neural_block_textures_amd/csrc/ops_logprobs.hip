@@ -35,73 +35,359 @@ __device__ __forceinline__ long long token_of(const ntc_logprobs_desc& d, long l
     return d.token_bytes == 8 ? ((const long long*)d.tokens)[at] : ((const int*)d.tokens)[at];
 }
 
-// (v, i) comes before (w, j): larger value, then lower index
-__device__ __forceinline__ bool before(float v, long long i, float w, long long j) { return v > w || (v == w && i < j); }
-__device__ __forceinline__ float order_of(float x) { return x != x ? -NTC_INF : x; }
+template <class T> __device__ __forceinline__ const T* row_of(const ntc_logprobs_desc& d, long long row, long long& outer, long long& inner) {
+    outer = row / d.inner_rows;
+    inner = row % d.inner_rows;
+    return (const T*)d.logits + outer * d.outer_stride + inner * d.inner_stride;
+}
+// The results of a row but its alternatives, from its softmax with the largest value m (kLowest or less: see none).
+template <class T> __device__ __forceinline__ void write_row(const ntc_logprobs_desc& d, long long row, const T* x, long long t, float m, float log_s, float ratio, bool none, float inv_t) {
+    float lp = 0.0f;
+    if (t != d.ignore_index) lp = t < 0 || t >= d.V ? __builtin_nanf("") : none ? -NTC_INF : log_prob((float)x[t], m, inv_t, log_s);
+    d.logprob[row] = lp;
+    d.entropy[row] = none ? 0.0f : kLn2 * (log_s - ratio);
+    d.stats[2 * row] = none ? -NTC_INF : m;
+    d.stats[2 * row + 1] = log_s;
+}
 
-template <class T> __global__ void __launch_bounds__(256) k_logprobs_row(ntc_logprobs_desc d) {
-    const long long row = blockIdx.x, outer = row / d.inner_rows, inner = row % d.inner_rows;
-    const T* x = (const T*)d.logits + outer * d.outer_stride + inner * d.inner_stride;
-    const float inv_t = 1.0f / d.temperature, k = kLog2e / d.temperature;
-    __shared__ Soft part[256];
-    __shared__ float bv[256];
-    __shared__ long long bi[256];
-    Soft a = { kLowest, 0.0f, 0.0f };
-    for (long long i = threadIdx.x; i < d.V; i += 256) {
-        const float v = (float)x[i];
-        if (v > a.m) soft_raise(a, v, k);
-        soft_add(a, v, k);
+// ---------------------------------------------------------------- short rows
+// A group of kGroup lanes holds a row in registers, kEach values a lane (vectors of 16 bytes, dealt in turn): the largest, then the
+// sums, then the alternatives one by one, each the largest key below the last. Keys are integers that order as the values do, larger for
+// the lower of equal ones' indices: 16-bit types in one word; a 32-bit one's index is found in a second reduction.
+template <class T> __device__ __forceinline__ uint32_t order_key(T x) {
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t h = __builtin_bit_cast(uint16_t, x), a = h & 0x7fffu, inf = type_code<T> == NTC_BF16 ? 0x7f80u : 0x7c00u;
+        if (a > inf) return 0x8000u - inf;                  // NaN as -inf
+        return h & 0x8000u ? 0x8000u - a : 0x8000u + a;     // (-0 as 0)
+    } else {
+        const uint32_t h = __float_as_uint(x), a = h & 0x7fffffffu;
+        if (a > 0x7f800000u) return 0x80000000u - 0x7f800000u;
+        return h & 0x80000000u ? 0x80000000u - a : 0x80000000u + a;
     }
-    part[threadIdx.x] = a;
-    __syncthreads();
-    for (int w = 128; w; w >>= 1) {
-        if (threadIdx.x < w) { Soft b = part[threadIdx.x]; soft_join(b, part[threadIdx.x + w], k); part[threadIdx.x] = b; }
-        __syncthreads();
-    }
-    a = part[0];
-    const bool none = a.s == 0.0f;
-    const float log_s = fast_log2(a.s);
-    if (threadIdx.x == 0) {
-        const long long t = token_of(d, outer, inner);
-        float lp = 0.0f;
-        if (t != d.ignore_index) lp = t < 0 || t >= d.V ? __builtin_nanf("") : none ? -NTC_INF : log_prob((float)x[t], a.m, inv_t, log_s);
-        d.logprob[row] = lp;
-        d.entropy[row] = none ? 0.0f : kLn2 * (log_s - a.t / a.s);
-        d.stats[2 * row] = none ? -NTC_INF : a.m;
-        d.stats[2 * row + 1] = log_s;
-    }
-    float pv = NTC_INF;
-    long long pi = -1;
-    for (int r = 0; r < d.top; r++) {
-        float v = -NTC_INF;
-        long long at = d.V;
-        for (long long i = threadIdx.x; i < d.V; i += 256) {
-            const float w = order_of((float)x[i]);
-            if (before(pv, pi, w, i) && before(w, i, v, at)) { v = w; at = i; }
-        }
-        bv[threadIdx.x] = v;
-        bi[threadIdx.x] = at;
-        __syncthreads();
-        for (int w = 128; w; w >>= 1) {
-            if (threadIdx.x < w && before(bv[threadIdx.x + w], bi[threadIdx.x + w], bv[threadIdx.x], bi[threadIdx.x])) {
-                bv[threadIdx.x] = bv[threadIdx.x + w];
-                bi[threadIdx.x] = bi[threadIdx.x + w];
-            }
-            __syncthreads();
-        }
-        pv = bv[0];
-        pi = bi[0];
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            d.top_ids[row * d.top + r] = pi;
-            d.top_logprobs[row * d.top + r] = none ? -NTC_INF : log_prob(pv, a.m, inv_t, log_s);
-        }
+}
+template <class T> __device__ __forceinline__ float key_value(uint32_t key) {
+    if constexpr (sizeof(T) == 2) {
+        const uint16_t h = key >= 0x8000u ? (uint16_t)(key - 0x8000u) : (uint16_t)(0x8000u | (0x8000u - key));
+        return (float)__builtin_bit_cast(T, h);
+    } else {
+        return __uint_as_float(key >= 0x80000000u ? key - 0x80000000u : 0x80000000u | (0x80000000u - key));
     }
 }
 
-template <class T> __global__ void __launch_bounds__(256) k_logprobs_grad(ntc_logprobs_desc d) {
-    const long long row = blockIdx.x, outer = row / d.inner_rows, inner = row % d.inner_rows;
-    const T* x = (const T*)d.logits + outer * d.outer_stride + inner * d.inner_stride;
+template <class T, int kGroup, int kEach> __global__ void __launch_bounds__(256) k_logprobs_short(ntc_logprobs_desc d) {
+    constexpr int kVec = 16 / (int)sizeof(T), kVecs = kEach / kVec > 0 ? kEach / kVec : 1, kE = kEach < kVec ? kEach : kVec;   // values a vector
+    const int in = threadIdx.x % kGroup;
+    const long long row = (long long)blockIdx.x * (256 / kGroup) + threadIdx.x / kGroup;
+    if (row >= d.rows) return;                              // whole groups
+    long long outer, inner;
+    const T* x = row_of<T>(d, row, outer, inner);
+    const int V = (int)d.V;
+    const float inv_t = 1.0f / d.temperature, k = kLog2e / d.temperature;
+    T v[kVecs][kE];
+    float m = -NTC_INF;
+#pragma unroll
+    for (int i = 0; i < kVecs; i++) {
+        const int at = (i * kGroup + in) * kE;
+        if (at + kE <= V) { const auto r = *(const LooseRun<T, kE>*)(x + at); for (int j = 0; j < kE; j++) v[i][j] = r.v[j]; }
+        else for (int j = 0; j < kE; j++) v[i][j] = at + j < V ? x[at + j] : (T)-NTC_INF;
+        for (int j = 0; j < kE; j++) m = fmaxf(m, (float)v[i][j]);
+    }
+    const auto larger = [](float a, float b) { return fmaxf(a, b); };
+    const auto sum = [](float a, float b) { return a + b; };
+    m = reduce<kGroup>(m, larger);
+    const float mm = m == -NTC_INF ? 0.0f : m;              // nothing left: every exponential is 0
+    float s = 0.0f, t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kVecs; i++)
+#pragma unroll
+        for (int j = 0; j < kE; j++) {
+            const float q = ((float)v[i][j] - mm) * k, e = fast_exp2(q);
+            s += e;
+            t = __builtin_fmaf(e, fmaxf(q, -1e30f), t);
+        }
+    s = reduce<kGroup>(s, sum);
+    t = reduce<kGroup>(t, sum);
+    const bool none = s == 0.0f;
+    const float log_s = fast_log2(s);
+    if (in == 0) write_row(d, row, x, token_of(d, outer, inner), mm, log_s, t / s, none, inv_t);
+    if (!d.top) return;
+    uint32_t key[kVecs][kE];
+#pragma unroll
+    for (int i = 0; i < kVecs; i++)
+#pragma unroll
+        for (int j = 0; j < kE; j++) {
+            const int at = (i * kGroup + in) * kE + j;
+            key[i][j] = order_key<T>(v[i][j]);
+            if constexpr (sizeof(T) == 2) key[i][j] = key[i][j] << 16 | (uint32_t)(0xffff - at);
+            if (at >= V) key[i][j] = 0;
+        }
+    const auto above = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    const auto below = [](uint32_t a, uint32_t b) { return a < b ? a : b; };
+    uint32_t mine = 0, mine_at = 0, last = 0, last_at = 0;
+    for (int r = 0; r < d.top; r++) {
+        uint32_t best = 0;
+        if constexpr (sizeof(T) == 2) {
+            // the largest below the last: key - last wraps to the top of the range for just those
+#pragma unroll
+            for (int i = 0; i < kVecs; i++)
+#pragma unroll
+                for (int j = 0; j < kE; j++) best = above(best, key[i][j] - last);
+            last = reduce<kGroup>(best, above) + last;
+            last_at = 0xffffu - (last & 0xffffu);
+        } else {
+            // the taken ones are those above the last, and those equal to it up to its index
+            uint32_t at = 0xffffffffu;
+#pragma unroll
+            for (int i = 0; i < kVecs; i++)
+#pragma unroll
+                for (int j = 0; j < kE; j++) {
+                    const uint32_t c = (uint32_t)((i * kGroup + in) * kE + j);
+                    const bool open = r == 0 || key[i][j] < last || (key[i][j] == last && c > last_at);
+                    if (open && (int)c < V && (key[i][j] > best || at == 0xffffffffu)) { best = key[i][j]; at = c; }   // ascending c: the first of equals stays
+                }
+            const uint32_t top = reduce<kGroup>(at == 0xffffffffu ? 0u : best, above);
+            last_at = reduce<kGroup>(best == top ? at : 0xffffffffu, below);
+            last = top;
+        }
+        if (in == r) { mine = last; mine_at = last_at; }
+    }
+    if (in < d.top) {
+        if constexpr (sizeof(T) == 2) mine >>= 16;
+        d.top_ids[row * d.top + in] = mine_at;
+        // (a NaN anywhere has made log_s NaN; its own place reads -inf here, which NaN swallows)
+        d.top_logprobs[row * d.top + in] = none ? -NTC_INF : log_prob(key_value<T>(mine), mm, inv_t, log_s);
+    }
+}
+
+// ---------------------------------------------------------------- long rows
+// The best K values of what a wave has read, in its lanes 0 to K - 1: value and index, in order; empty places are (-inf, kNoIndex).
+constexpr int kNoIndex = 0x7fffffff;
+struct Best {
+    float v;
+    int i;
+    __device__ __forceinline__ void clear() { v = -NTC_INF; i = kNoIndex; }
+    // (w, j), the same in all lanes, to its place
+    __device__ __forceinline__ void insert(float w, int j) {
+        const bool keeps = v > w || (v == w && i < j);
+        const int at = __builtin_popcountll(__ballot(keeps));
+        const float uv = __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x138, 0xf, 0xf, false));   // lane l gets lane l - 1's
+        const int ui = __builtin_amdgcn_update_dpp(0, i, 0x138, 0xf, 0xf, false);
+        const int l = lane_id();
+        v = l < at ? v : l == at ? w : uv;
+        i = l < at ? i : l == at ? j : ui;
+    }
+};
+
+// What a lane reads at a time: kRun values in vectors of 16 bytes.
+template <class T> struct Long { static constexpr int kVec = 16 / (int)sizeof(T), kVecs = 2, kRun = kVec * kVecs, kChunk = 64 * kRun; };
+
+// A wave's share of a row: chunks first, first + step, .. below `end` (chunks of kChunk values, the last one ragged).
+// The sums are each lane's own, on a floor that only rises: exp2(x k - m k) is one fused operation and an exponential, with m held
+// within lim so that neither product overflows. A row whose values all lie below -lim, or reach past lim, or hold NaN ends with s = 0, infinite or
+// NaN and is read again by scan_again(). Values enter the list of the best only where their lane's largest of a chunk passes the list's last.
+template <class T> __device__ __forceinline__ void scan(const T* x, int V, int first, int step, int end, float k, float lim, int top, Soft& a, Best& best) {
+    using L = Long<T>;
+    const int lane = lane_id();
+    a = { -lim, 0.0f, 0.0f };
+    best.clear();
+    float mk = -lim * k, last = -NTC_INF;
+    bool fresh = true;
+    for (int c = first; c < end; c += step) {
+        float v[L::kRun];
+        const int base = c * L::kChunk;
+        const int at0 = base + lane * L::kVec;
+        if (base + L::kChunk <= V) {
+#pragma unroll
+            for (int i = 0; i < L::kVecs; i++) {
+                const auto r = *(const LooseRun<T, L::kVec>*)(x + at0 + i * 64 * L::kVec);
+#pragma unroll
+                for (int j = 0; j < L::kVec; j++) v[i * L::kVec + j] = (float)r.v[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < L::kVecs; i++)
+#pragma unroll
+                for (int j = 0; j < L::kVec; j++) { const int p = at0 + i * 64 * L::kVec + j; v[i * L::kVec + j] = p < V ? (float)x[p] : -NTC_INF; }
+        }
+        float cm = v[0];
+#pragma unroll
+        for (int j = 1; j < L::kRun; j++) cm = fmaxf(cm, v[j]);
+        if (cm > a.m) {
+            a.m = fminf(cm, lim);
+            const float was = mk, f = fast_exp2(was - a.m * k);   // between the rounded products, which the exponents are taken on
+            mk = a.m * k;
+            a.t = f * __builtin_fmaf(a.s, was - mk, a.t);
+            a.s *= f;
+        }
+#pragma unroll
+        for (int j = 0; j < L::kRun; j++) {
+            const float d = __builtin_fmaf(v[j], k, -mk), e = fast_exp2(d);
+            a.s += e;
+            a.t = __builtin_fmaf(e, fmaxf(d, -1e30f), a.t);
+        }
+        if (!top) continue;
+        float least = last;                                  // the list's last value; only larger ones can pass it later in the row
+        if (fresh) {
+            // the first chunk would enter the list value by value: start from the K-th largest of the lanes' largest, which K values reach
+            float w = cm;
+            for (int r = 0; r < top; r++) {
+                least = reduce64(w, [](float p, float q) { return fmaxf(p, q); });
+                const int who = __builtin_ctzll(__ballot(w == least) | 1ull << 63);
+                w = lane == who ? -NTC_INF : w;
+            }
+        }
+        if (__ballot(fresh ? cm >= least : cm > least)) {
+#pragma unroll
+            for (int j = 0; j < L::kRun; j++) {
+                unsigned long long ask = __ballot(v[j] >= least && v[j] > -NTC_INF);
+                while (ask) {
+                    const int l = __builtin_ctzll(ask);
+                    best.insert(read_lane(v[j], l), base + (j / L::kVec) * 64 * L::kVec + l * L::kVec + j % L::kVec);
+                    least = fmaxf(least, read_lane(best.v, top - 1));
+                    ask &= ask - 1;
+                    ask &= __ballot(v[j] >= least);
+                }
+            }
+            last = read_lane(best.v, top - 1);
+        }
+        fresh = false;
+    }
+    // the sums were taken on the rounded m k: to those on m itself
+    const float off = __builtin_fmaf(a.m, k, -mk);           // m k - fl(m k): every exponent was that much too large
+    a.t -= a.s * off;
+    const float f = fast_exp2(-off);
+    a.t *= f;
+    a.s *= f;
+}
+
+// The same sums for any values: on differences, which do not overflow where the values do not differ that much. One wave, whole row.
+template <class T> __device__ __forceinline__ Soft scan_again(const T* x, int V, float k) {
+    float m = kLowest;
+    for (int i = lane_id(); i < V; i += 64) m = fmaxf(m, (float)x[i]);
+    m = reduce64(m, [](float p, float q) { return fmaxf(p, q); });
+    Soft a = { m, 0.0f, 0.0f };
+    for (int i = lane_id(); i < V; i += 64) soft_add(a, (float)x[i], k);
+    const auto sum = [](float p, float q) { return p + q; };
+    a.s = reduce64(a.s, sum);
+    a.t = reduce64(a.t, sum);
+    return a;
+}
+__device__ __forceinline__ bool plain_sum(float s) { return s > 0.0f && s < NTC_INF; }
+
+__device__ __forceinline__ Soft join_lanes(Soft a, float k) {
+    const auto sum = [](float p, float q) { return p + q; };
+    const float m = reduce64(a.m, [](float p, float q) { return fmaxf(p, q); });
+    soft_raise(a, m, k);
+    a.s = reduce64(a.s, sum);
+    a.t = reduce64(a.t, sum);
+    return a;
+}
+
+// The rest of a row, by one wave that has its joined sums and best values: odd rows read again, places of the list that no number above -inf
+// took filled with the first indices that hold -inf or NaN, and everything written.
+template <class T> __device__ __forceinline__ void finish(const ntc_logprobs_desc& d, long long row, const T* x, long long t, Soft a, Best best) {
+    const int lane = lane_id(), V = (int)d.V;
+    const float inv_t = 1.0f / d.temperature, k = kLog2e / d.temperature;
+    if (!plain_sum(a.s)) a = scan_again(x, V, k);
+    const bool none = a.s == 0.0f;
+    const float log_s = fast_log2(a.s);
+    if (lane == 0) write_row(d, row, x, t, a.m, log_s, a.t / a.s, none, inv_t);
+    if (!d.top) return;
+    int have = __builtin_popcountll(__ballot(lane < d.top && best.i != kNoIndex));
+    for (int i = 0; have < d.top; i += 64) {                 // (ends: top <= V, and each value is a number above -inf or not)
+        const bool low = i + lane < V && !((float)x[i + lane < V ? i + lane : 0] > -NTC_INF);
+        unsigned long long ask = __ballot(low);
+        while (ask && have < d.top) {
+            const int l = __builtin_ctzll(ask);
+            ask &= ask - 1;
+            if (lane == have) { best.v = -NTC_INF; best.i = i + l; }
+            have++;
+        }
+    }
+    if (lane < d.top) {
+        d.top_ids[row * d.top + lane] = best.i;
+        d.top_logprobs[row * d.top + lane] = none ? -NTC_INF : log_prob(best.v, a.m, inv_t, log_s);
+    }
+}
+
+// kWaves waves (of a block of 4) read a row; with kParts a block reads the part blockIdx.y of a row and leaves its sums and list in the workspace.
+template <class T, int kWaves, bool kParts> __global__ void __launch_bounds__(256) k_logprobs_long(ntc_logprobs_desc d, float lim, int part_chunks) {
+    __shared__ Soft soft[4];
+    __shared__ float list_v[4][NTC_MAX_TOP];
+    __shared__ int list_i[4][NTC_MAX_TOP];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id();
+    const long long row = (long long)blockIdx.x * (4 / kWaves) + wave / kWaves;
+    if (row >= d.rows) return;                               // (kWaves 1: a wave on its own; else whole blocks)
+    long long outer, inner;
+    const T* x = row_of<T>(d, row, outer, inner);
+    const float k = kLog2e / d.temperature;
+    const int V = (int)d.V, chunks = (V + Long<T>::kChunk - 1) / Long<T>::kChunk;
+    const int begin = kParts ? (int)blockIdx.y * part_chunks : 0, end = kParts && begin + part_chunks < chunks ? begin + part_chunks : chunks;
+    Soft a;
+    Best best;
+    scan(x, V, begin + wave % kWaves, kWaves, end, k, lim, d.top, a, best);
+    a = join_lanes(a, k);
+    if (kWaves > 1) {
+        if (lane == 0) soft[wave] = a;
+        if (lane < d.top) { list_v[wave][lane] = best.v; list_i[wave][lane] = best.i; }
+        __syncthreads();
+        if (wave) return;
+        for (int w = 1; w < kWaves; w++) {
+            soft_join(a, soft[w], k);
+            for (int r = 0; r < d.top; r++) {                // in order: the first that does not pass the list's last ends it
+                const float v = list_v[w][r];
+                const int i = list_i[w][r];
+                if (!(i != kNoIndex) || !(v > read_lane(best.v, d.top - 1) || (v == read_lane(best.v, d.top - 1) && i < __builtin_amdgcn_readlane(best.i, d.top - 1)))) break;
+                best.insert(v, i);
+            }
+        }
+    }
+    if (!kParts) { finish(d, row, x, token_of(d, outer, inner), a, best); return; }
+    const int parts = gridDim.y;
+    float* to = (float*)d.workspace + (row * parts + blockIdx.y) * (4 + 2 * d.top);
+    if (lane == 0) { to[0] = a.m; to[1] = a.s; to[2] = a.t; }
+    if (lane < d.top) { to[4 + lane] = best.v; ((int*)to)[4 + d.top + lane] = best.i; }
+}
+
+// Joins a row's parts: a wave a row, part p's sums in lane p % 64. The lists go through LDS, since they are walked one value at a time.
+constexpr int kMostParts = 64;
+template <class T> __global__ void __launch_bounds__(64) k_logprobs_join(ntc_logprobs_desc d, int parts) {
+    __shared__ float list[kMostParts * 2 * NTC_MAX_TOP];
+    const long long row = blockIdx.x;
+    const int lane = lane_id(), size = 4 + 2 * d.top;
+    long long outer, inner;
+    const T* x = row_of<T>(d, row, outer, inner);
+    const float k = kLog2e / d.temperature;
+    const float* from = (const float*)d.workspace + row * parts * size;
+    Soft a = { kLowest, 0.0f, 0.0f };
+    if (lane < parts) a = { from[lane * size], from[lane * size + 1], from[lane * size + 2] };
+    for (int p = 0; p < parts; p++) if (lane < 2 * d.top) list[p * 2 * d.top + lane] = from[p * size + 4 + lane];
+    __syncthreads();
+    a = join_lanes(a, k);
+    Best best;
+    best.clear();
+    for (int p = 0; p < parts; p++)
+        for (int r = 0; r < d.top; r++) {
+            const float v = list[p * 2 * d.top + r];
+            const int i = __float_as_int(list[p * 2 * d.top + d.top + r]);
+            if (i == kNoIndex || !(v > read_lane(best.v, d.top - 1) || (v == read_lane(best.v, d.top - 1) && i < __builtin_amdgcn_readlane(best.i, d.top - 1)))) break;
+            best.insert(v, i);
+        }
+    finish(d, row, x, token_of(d, outer, inner), a, best);
+}
+
+// ---------------------------------------------------------------- gradient
+// A wave takes kGradRun vectors a lane of one row. The few places that get more than -p a (the token, the alternatives) are held one a lane
+// and looked for a chunk at a time.
+constexpr int kGradVecs = 2;
+template <class T> __global__ void __launch_bounds__(256) k_logprobs_grad(ntc_logprobs_desc d, int row_chunks) {
+    constexpr int kVec = 16 / (int)sizeof(T), kChunk = 64 * kVec;
+    const int lane = lane_id();
+    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), row = unit / row_chunks;
+    if (row >= d.rows) return;
+    const int V = (int)d.V, begin = (int)(unit % row_chunks) * (kGradVecs * kChunk);
+    long long outer, inner;
+    const T* x = row_of<T>(d, row, outer, inner);
     T* dx = (T*)d.dlogits + row * d.V;
     const float k = kLog2e / d.temperature, inv_t = 1.0f / d.temperature;
     const float m = d.stats[2 * row], log_s = d.stats[2 * row + 1], H = d.entropy[row];
@@ -109,16 +395,86 @@ template <class T> __global__ void __launch_bounds__(256) k_logprobs_grad(ntc_lo
     const bool none = m == -NTC_INF, out = t != d.ignore_index && (t < 0 || t >= d.V);
     const float glp = d.g_logprob && t != d.ignore_index ? d.g_logprob[row] : 0.0f;
     const float gh = d.g_entropy ? d.g_entropy[row] : 0.0f;
-    float all = glp;
-    if (d.g_top) for (int r = 0; r < d.top; r++) all += d.g_top[row * d.top + r];
+    const bool tops = d.g_top != nullptr;
+    // lane 0: the token; lanes 1 to top: the alternatives
+    int place = -1;
+    float extra = 0.0f;
+    if (lane == 0 && !out && t != d.ignore_index) { place = (int)t; extra = glp; }
+    if (tops && lane >= 1 && lane <= d.top) { place = (int)d.top_ids[row * d.top + lane - 1]; extra = d.g_top[row * d.top + lane - 1]; }
+    float all = reduce64(extra, [](float p, float q) { return p + q; });
     if (out) all = __builtin_nanf("");
-    for (long long i = threadIdx.x; i < d.V; i += 256) {
-        const float lp = ((float)x[i] - m) * k - log_s, p = fast_exp2(lp);
-        float g = i == t ? glp : 0.0f;
-        if (d.g_top) for (int r = 0; r < d.top; r++) g += d.top_ids[row * d.top + r] == i ? d.g_top[row * d.top + r] : 0.0f;
-        g -= p * (all + gh * __builtin_fmaf(kLn2, fmaxf(lp, -160.0f), H));
-        dx[i] = (T)(none ? 0.0f : g * inv_t);
+    extra *= inv_t;
+    const float na = -all * inv_t, nh = -gh * inv_t;
+#pragma unroll
+    for (int c = 0; c < kGradVecs; c++) {
+        const int base = begin + c * kChunk, at = base + lane * kVec;
+        if (base >= V) break;
+        T r[kVec];
+        const bool full = at + kVec <= V;
+        if (full) { const auto q = *(const LooseRun<T, kVec>*)(x + at); for (int j = 0; j < kVec; j++) r[j] = q.v[j]; }
+        else for (int j = 0; j < kVec; j++) r[j] = at + j < V ? x[at + j] : (T)0.0f;
+        float g[kVec];
+#pragma unroll
+        for (int j = 0; j < kVec; j++) {
+            const float lp = ((float)r[j] - m) * k - log_s, p = fast_exp2(lp);
+            g[j] = p * __builtin_fmaf(nh, __builtin_fmaf(kLn2, fmaxf(lp, -160.0f), H), na);
+        }
+        unsigned long long here = __ballot(place >= base && place < base + kChunk);
+        while (here) {
+            const int l = __builtin_ctzll(here);
+            here &= here - 1;
+            const int off = __builtin_amdgcn_readlane(place, l) - at;
+            const float e = read_lane(extra, l);
+#pragma unroll
+            for (int j = 0; j < kVec; j++) g[j] += off == j ? e : 0.0f;
+        }
+        LooseRun<T, kVec> o;
+#pragma unroll
+        for (int j = 0; j < kVec; j++) o.v[j] = (T)(none ? 0.0f : g[j]);
+        if (full) *(LooseRun<T, kVec>*)(dx + at) = o;
+        else for (int j = 0; j < kVec; j++) if (at + j < V) dx[at + j] = o.v[j];
     }
+}
+
+// How long rows are read: waves a row, and blocks a row where there are few rows.
+struct Reading { int waves, parts, part_chunks; };
+template <class T> static Reading reading(int64_t rows, int64_t V) {
+    const int64_t chunks = (V + Long<T>::kChunk - 1) / Long<T>::kChunk;
+    Reading r = { rows >= 2048 && chunks <= 8 ? 1 : 4, 1, (int)chunks };
+    if (r.waves == 4 && rows < 512 && chunks > 8) {
+        int64_t parts = 1024 / rows;
+        if (parts > kMostParts) parts = kMostParts;
+        if (parts > chunks / 4) parts = chunks / 4;
+        r.part_chunks = (int)((chunks + parts - 1) / parts);
+        r.parts = (int)((chunks + r.part_chunks - 1) / r.part_chunks);
+    }
+    return r;
+}
+constexpr int kShort = 1024;                                 // the longest row that a wave holds in registers
+
+template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s) {
+    const auto blocks = [&](int per) { return (unsigned)((d.rows + per - 1) / per); };
+    if (d.V <= 64 && d.top <= 16) { k_logprobs_short<T, 16, 4><<<blocks(16), 256, 0, s>>>(d); return; }
+    if (d.V <= 256 && d.top <= 16) { k_logprobs_short<T, 16, 16><<<blocks(16), 256, 0, s>>>(d); return; }
+    if (d.V <= kShort) { k_logprobs_short<T, 64, 16><<<blocks(4), 256, 0, s>>>(d); return; }
+    const Reading r = reading<T>(d.rows, d.V);
+    const float k = kLog2e / d.temperature, lim = 1e30f / (k > 1.0f ? k : 1.0f);
+    if (r.waves == 1) k_logprobs_long<T, 1, false><<<blocks(4), 256, 0, s>>>(d, lim, 0);
+    else if (r.parts == 1) k_logprobs_long<T, 4, false><<<blocks(1), 256, 0, s>>>(d, lim, 0);
+    else {
+        k_logprobs_long<T, 4, true><<<dim3((unsigned)d.rows, r.parts), 256, 0, s>>>(d, lim, r.part_chunks);
+        k_logprobs_join<T><<<(unsigned)d.rows, 64, 0, s>>>(d, r.parts);
+    }
+}
+template <class T> static size_t workspace(int64_t rows, int64_t V, int top) {
+    if (V <= kShort) return 0;
+    const Reading r = reading<T>(rows, V);
+    return r.parts == 1 ? 0 : (size_t)rows * r.parts * (4 + 2 * top) * 4;
+}
+template <class T> static void backward(const ntc_logprobs_desc& d, hipStream_t s) {
+    constexpr int kVec = 16 / (int)sizeof(T);
+    const int64_t row_chunks = (d.V + 64 * kVec * kGradVecs - 1) / (64 * kVec * kGradVecs);
+    k_logprobs_grad<T><<<(unsigned)((d.rows * row_chunks + 3) / 4), 256, 0, s>>>(d, (int)row_chunks);
 }
 
 static int check(const ntc_logprobs_desc* d, bool backward, char* why, size_t cap) {
@@ -140,20 +496,24 @@ static int check(const ntc_logprobs_desc* d, bool backward, char* why, size_t ca
 
 using namespace ntc_ops;
 
-extern "C" size_t ntc_op_token_logprobs_workspace(int64_t, int64_t, int32_t) { return 0; }
+extern "C" size_t ntc_op_token_logprobs_workspace(int64_t rows, int64_t V, int32_t dtype, int32_t top) {
+    if (rows < 1 || V < 1 || top < 0 || top > NTC_MAX_TOP) return 0;
+    return dtype == NTC_F32 ? workspace<f32>(rows, V, top) : workspace<bf16>(rows, V, top);
+}
 
 extern "C" int ntc_op_token_logprobs(const ntc_logprobs_desc* d, void* stream, char* why, size_t cap) {
     if (const int r = check(d, false, why, cap)) return r;
     if (!d->rows) return 0;
-    const auto go = [&](auto kernel) { kernel<<<(unsigned)d->rows, 256, 0, (hipStream_t)stream>>>(*d); };
-    d->dtype == NTC_F32 ? go(k_logprobs_row<f32>) : d->dtype == NTC_BF16 ? go(k_logprobs_row<bf16>) : go(k_logprobs_row<f16>);
+    if (!d->workspace && ntc_op_token_logprobs_workspace(d->rows, d->V, d->dtype, d->top)) return refuse(why, cap, "a null workspace");
+    const hipStream_t s = (hipStream_t)stream;
+    d->dtype == NTC_F32 ? forward<f32>(*d, s) : d->dtype == NTC_BF16 ? forward<bf16>(*d, s) : forward<f16>(*d, s);
     return launched(why, cap);
 }
 
 extern "C" int ntc_op_token_logprobs_backward(const ntc_logprobs_desc* d, void* stream, char* why, size_t cap) {
     if (const int r = check(d, true, why, cap)) return r;
     if (!d->rows) return 0;
-    const auto go = [&](auto kernel) { kernel<<<(unsigned)d->rows, 256, 0, (hipStream_t)stream>>>(*d); };
-    d->dtype == NTC_F32 ? go(k_logprobs_grad<f32>) : d->dtype == NTC_BF16 ? go(k_logprobs_grad<bf16>) : go(k_logprobs_grad<f16>);
+    const hipStream_t s = (hipStream_t)stream;
+    d->dtype == NTC_F32 ? backward<f32>(*d, s) : d->dtype == NTC_BF16 ? backward<bf16>(*d, s) : backward<f16>(*d, s);
     return launched(why, cap);
 }

@@ -59,7 +59,7 @@ def library() -> C.CDLL:
         lib = trainer.library()
         tail = [_P, C.c_char_p, C.c_size_t]
         sig = {
-            "ntc_op_token_logprobs_workspace": (C.c_size_t, [_L, _L, _I]),
+            "ntc_op_token_logprobs_workspace": (C.c_size_t, [_L, _L, _I, _I]),
             "ntc_op_token_logprobs": (C.c_int, [_P] + tail),
             "ntc_op_token_logprobs_backward": (C.c_int, [_P] + tail),
             "ntc_op_adamw": (C.c_int, [_P] + tail),
@@ -143,6 +143,9 @@ def _logprobs_forward(logits, tokens, top, temperature, ignore_index):
     if top:
         ids, top_logprobs = new((*shape, top), dtype=torch.int64), new((*shape, top), dtype=torch.float32)
         d.top_ids, d.top_logprobs = ids.data_ptr(), top_logprobs.data_ptr()
+    size = library().ntc_op_token_logprobs_workspace(d.rows, d.V, d.dtype, top)
+    work = new(size, dtype=torch.uint8) if size else None
+    d.workspace = None if work is None else work.data_ptr()
     _call(logits.device, library().ntc_op_token_logprobs, C.byref(d))
     return logprob, entropy, ids, top_logprobs, stats
 
