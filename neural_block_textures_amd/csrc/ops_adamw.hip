@@ -66,23 +66,17 @@ __device__ __forceinline__ bool aligned4(const void* p, int type) { return ((uin
 __device__ __forceinline__ float power_of(int b) { return __uint_as_float(b > 0 ? (uint32_t)b << 23 : 1u << 22); }
 
 // ---------------------------------------------------------------- 8-bit states
-// The value of a code without its sign (kTop: the exponent that stands for [1, 2)); exact, and `scale` is a power of two.
-template <int kTop> __device__ __forceinline__ float decode8(uint32_t c, float scale) {
-    const float normal = __uint_as_float((c + 8u * (127 - kTop)) << 20);
-    const float small = (float)c * __uint_as_float((uint32_t)(127 - 2 - kTop) << 23);
-    return (c >= 8 ? normal : small) * scale;
+// A code's bits are the top bits of a 32-bit float whose exponents are 2^(127 - kTop) too small (kTop: the exponent that stands for
+// [1, 2)), the smallest codes being that float's own subnormals: two exact products by powers of two are the whole conversion.
+template <int kTop> __device__ __forceinline__ float decode8(uint32_t c20, float scale) {   // c20: the code without sign, at bit 20
+    return __uint_as_float(c20) * __uint_as_float((uint32_t)(254 - kTop) << 23) * scale;
 }
-// a >= 0, at most 1.875, to its code: the 16 bits r are added below the last kept bit
-template <int kTop> __device__ __forceinline__ uint32_t encode8(float a, uint32_t r) {
-    const uint32_t normal = ((__float_as_uint(a) + (r << 4)) >> 20) - 8u * (127 - kTop);
-    const float small = a * __uint_as_float((uint32_t)(127 + kTop + 2) << 23) + (float)r * 0x1p-16f;
-    return a >= __uint_as_float((uint32_t)(127 + 1 - kTop) << 23) ? normal : (uint32_t)small;
+// 0 <= a * scale <= 1.875 to its code: 16 random bits r are added below the last kept bit. (Below the smallest power the product is
+// rounded 20 bits below the last kept one.)
+template <int kTop> __device__ __forceinline__ uint32_t encode8(float a, float scale, uint32_t r) {
+    return (__float_as_uint(a * scale * __uint_as_float((uint32_t)kTop << 23)) + (r << 4)) >> 20;
 }
-// The largest of 64 lanes' a >= 0 (NaN counts as the largest: bit patterns are compared), and the block's exponent byte from it.
-__device__ __forceinline__ uint32_t wave_max_bits(uint32_t b) {
-    for (int w = 1; w < 64; w <<= 1) { const uint32_t o = __shfl_xor(b, w); b = o > b ? o : b; }
-    return b;
-}
+// the block's exponent byte from the bits of its largest magnitude (NaN counts as the largest)
 __device__ __forceinline__ int exponent_byte(uint32_t most) {
     const int e = (int)(most >> 23) + ((most & 0x7fffffu) > 0x700000u ? 1 : 0);
     return (most >> 23) >= 254u ? 255 : e;
@@ -91,33 +85,131 @@ __device__ __forceinline__ int exponent_byte(uint32_t most) {
 // four values a lane of one block, to codes
 struct Codes { uint32_t m, v; int me, ve; };
 __device__ __forceinline__ Codes encode_block(const float (&m)[4], const float (&v)[4], const uint32_t (&rm)[4], const uint32_t (&rv)[4]) {
+    const auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
     uint32_t bm = 0, bv = 0;
     for (int j = 0; j < 4; j++) {
-        const uint32_t a = __float_as_uint(m[j]) & 0x7fffffffu, b = __float_as_uint(v[j]) & 0x7fffffffu;
-        bm = a > bm ? a : bm;
-        bv = b > bv ? b : bv;
+        bm = larger(bm, __float_as_uint(m[j]) & 0x7fffffffu);
+        bv = larger(bv, __float_as_uint(v[j]) & 0x7fffffffu);
     }
-    Codes c = { 0, 0, exponent_byte(wave_max_bits(bm)), exponent_byte(wave_max_bits(bv)) };
-    const float sm = power_of(254 - (c.me == 255 ? 254 : c.me)), sv = power_of(254 - (c.ve == 255 ? 254 : c.ve));
+    bm = __builtin_amdgcn_readfirstlane(reduce64(bm, larger));
+    bv = __builtin_amdgcn_readfirstlane(reduce64(bv, larger));
+    Codes c = { 0, 0, exponent_byte(bm), exponent_byte(bv) };
+    const float sm = power_of(254 - c.me), sv = power_of(254 - c.ve);
     for (int j = 0; j < 4; j++) {
-        const uint32_t sign = m[j] < 0.0f ? 128u : 0u;
-        uint32_t a = encode8<15>(fabsf(m[j]) * sm, rm[j]) | sign, b = encode8<31>(v[j] * sv, rv[j]);
-        b = b == 0 && v[j] * sv > 0.0f ? 1u : b;
-        c.m |= (c.me == 255 ? 0u : a) << (8 * j);
-        c.v |= (c.ve == 255 ? 0u : b) << (8 * j);
+        const uint32_t a = encode8<15>(fabsf(m[j]), sm, rm[j]) | (__float_as_uint(m[j]) >> 24 & 128u);
+        uint32_t b = encode8<31>(v[j], sv, rv[j]);
+        const uint32_t least = __float_as_uint(v[j]) < 1u ? 0u : 1u;     // v > 0 is not rounded to 0
+        b = b > least ? b : least;
+        c.m |= a << (8 * j);
+        c.v |= b << (8 * j);
     }
+    if (c.me == 255) c.m = 0;
+    if (c.ve == 255) c.v = 0;
     return c;
 }
 __device__ __forceinline__ void decode_block(uint32_t cm, uint32_t cv, int me, int ve, float (&m)[4], float (&v)[4]) {
     const float sm = me == 255 ? __builtin_nanf("") : power_of(me), sv = ve == 255 ? __builtin_nanf("") : power_of(ve);
     for (int j = 0; j < 4; j++) {
-        const uint32_t a = (cm >> (8 * j)) & 255u, b = (cv >> (8 * j)) & 255u;
-        const float x = decode8<15>(a & 127u, sm);
-        m[j] = a & 128u ? -x : x;
-        v[j] = decode8<31>(b, sv);
+        const uint32_t a = cm >> (8 * j), b = cv >> (8 * j);
+        m[j] = __uint_as_float(__float_as_uint(decode8<15>((a & 127u) << 20, sm)) | (a & 128u) << 24);
+        v[j] = decode8<31>((b & 255u) << 20, sv);
     }
 }
 
+// ---------------------------------------------------------------- the step
+// Four values of one tensor. The division and the root are the hardware's, an ulp each: a 2^-22 of the update, where p keeps 2^-24 of itself.
+__device__ __forceinline__ void update(const AdamArgs& A, float rate, float root, const float (&g)[4], float (&p)[4], float (&m)[4], float (&v)[4]) {
+    for (int j = 0; j < 4; j++) {
+        m[j] = m[j] * A.b1 + g[j] * A.nb1;
+        v[j] = v[j] * A.b2 + (g[j] * g[j]) * A.nb2;
+        p[j] = p[j] * A.keep - rate * (m[j] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[j]) * root + A.eps));
+    }
+}
+__device__ __forceinline__ void random16(uint64_t at, uint32_t (&rm)[4], uint32_t (&rv)[4]) {   // at: head + (position / 2) phi
+    for (int j = 0; j < 4; j += 2) {
+        const uint64_t h = ntc_hip::mix64(at + (j ? ntc_hip::kPhi64 : 0));
+        rm[j] = (uint32_t)h & 0xffffu;
+        rv[j] = (uint32_t)h >> 16;
+        rm[j + 1] = (uint32_t)(h >> 32) & 0xffffu;
+        rv[j + 1] = (uint32_t)(h >> 48);
+    }
+}
+
+// A wave's blocks of a chunk that lies whole in its tensor and on aligned addresses: everything is read first, so that the memory has
+// four blocks' requests at once; kG32, kP32: the gradient and the tensor are 32-bit.
+struct __attribute__((packed)) LooseWord { uint32_t v; };
+template <bool k32> struct Raw { using type = std::conditional_t<k32, uint4, uint2>; };
+template <bool k32> __device__ __forceinline__ void widen(float (&o)[4], const typename Raw<k32>::type& r, int type) {
+    if constexpr (k32) { const auto f = __builtin_bit_cast(Run<float, 4>, r); for (int j = 0; j < 4; j++) o[j] = f.v[j]; }
+    else if (type == NTC_BF16) { const auto f = __builtin_bit_cast(Run<bf16, 4>, r); for (int j = 0; j < 4; j++) o[j] = (float)f.v[j]; }
+    else { const auto f = __builtin_bit_cast(Run<f16, 4>, r); for (int j = 0; j < 4; j++) o[j] = (float)f.v[j]; }
+}
+template <bool k32> __device__ __forceinline__ typename Raw<k32>::type narrow(const float (&p)[4], int type) {
+    if constexpr (k32) { Run<float, 4> f; for (int j = 0; j < 4; j++) f.v[j] = p[j]; return __builtin_bit_cast(uint4, f); }
+    else if (type == NTC_BF16) { Run<bf16, 4> f; for (int j = 0; j < 4; j++) f.v[j] = (bf16)p[j]; return __builtin_bit_cast(uint2, f); }
+    else { Run<f16, 4> f; for (int j = 0; j < 4; j++) f.v[j] = (f16)p[j]; return __builtin_bit_cast(uint2, f); }
+}
+template <int kBits, bool kMaster, bool kG32, bool kP32> __device__ __forceinline__ void whole_chunk(const AdamArgs& A, const ntc_adamw_tensor& T, const void* g_ptr, int gt, float rate,
+                                                                                                     float root, long long i0) {
+    using GR = typename Raw<kG32>::type;
+    using PR = typename Raw<kP32>::type;
+    using SR = std::conditional_t<kBits == 8, uint32_t, float4>;
+    const GR* gp = (const GR*)((const uint8_t*)g_ptr + i0 * (kG32 ? 4 : 2));
+    PR* pp = (PR*)((uint8_t*)T.param + i0 * (kP32 ? 4 : 2));
+    const long long at = T.state_offset + i0;
+    SR* mp = (SR*)((uint8_t*)A.m + at * (kBits / 8));
+    SR* vp = (SR*)((uint8_t*)A.v + at * (kBits / 8));
+    float4* wp = (float4*)(A.master + at);
+    GR g[kWaveBlocks];
+    PR p[kWaveBlocks];
+    SR m[kWaveBlocks], v[kWaveBlocks];
+    float4 w[kWaveBlocks];
+    uint32_t me = 0, ve = 0;
+#pragma unroll
+    for (int u = 0; u < kWaveBlocks; u++) {
+        g[u] = gp[64 * u];
+        if (kMaster) w[u] = wp[64 * u];
+        else p[u] = pp[64 * u];
+        m[u] = mp[64 * u];
+        v[u] = vp[64 * u];
+    }
+    if constexpr (kBits == 8) {                              // a wave's four blocks' exponents are a word, at any byte
+        me = __builtin_amdgcn_readfirstlane(((const LooseWord*)(A.me + (at >> 8)))->v);
+        ve = __builtin_amdgcn_readfirstlane(((const LooseWord*)(A.ve + (at >> 8)))->v);
+    }
+    uint32_t new_me = 0, new_ve = 0;
+    uint64_t noise = A.head + (uint64_t)(at >> 1) * ntc_hip::kPhi64;
+#pragma unroll
+    for (int u = 0; u < kWaveBlocks; u++) {
+        float gf[4], pf[4], mf[4], vf[4];
+        widen<kG32>(gf, g[u], gt);
+        if (kMaster) { pf[0] = w[u].x; pf[1] = w[u].y; pf[2] = w[u].z; pf[3] = w[u].w; }
+        else widen<kP32>(pf, p[u], T.param_type);
+        if constexpr (kBits == 8) decode_block(m[u], v[u], (me >> (8 * u)) & 255, (ve >> (8 * u)) & 255, mf, vf);
+        else { mf[0] = m[u].x; mf[1] = m[u].y; mf[2] = m[u].z; mf[3] = m[u].w; vf[0] = v[u].x; vf[1] = v[u].y; vf[2] = v[u].z; vf[3] = v[u].w; }
+        update(A, rate, root, gf, pf, mf, vf);
+        if constexpr (kBits == 8) {
+            uint32_t rm[4], rv[4];
+            random16(noise + (uint64_t)(128 * u) * ntc_hip::kPhi64, rm, rv);
+            const Codes c = encode_block(mf, vf, rm, rv);
+            mp[64 * u] = c.m;
+            vp[64 * u] = c.v;
+            new_me |= (uint32_t)c.me << (8 * u);
+            new_ve |= (uint32_t)c.ve << (8 * u);
+        } else {
+            mp[64 * u] = float4{ mf[0], mf[1], mf[2], mf[3] };
+            vp[64 * u] = float4{ vf[0], vf[1], vf[2], vf[3] };
+        }
+        if (kMaster) wp[64 * u] = float4{ pf[0], pf[1], pf[2], pf[3] };
+        pp[64 * u] = narrow<kP32>(pf, T.param_type);
+    }
+    if (kBits == 8 && (threadIdx.x & 63) == 0) {
+        ((LooseWord*)(A.me + (at >> 8)))->v = new_me;
+        ((LooseWord*)(A.ve + (at >> 8)))->v = new_ve;
+    }
+}
+
+// Memory bounds it. A block takes 4096 values of one tensor, a wave 1024 of them, 256 (a block of an 8-bit state) at a time.
 template <int kBits, bool kMaster> __global__ void __launch_bounds__(kAdamTPB) k_adamw(AdamArgs A, AdamGrads G) {
     const long long chunk = A.chunk0 + blockIdx.x;
     const int ti = A.chunk_tensor[chunk], gi = ti - A.tensor0;
@@ -129,10 +221,16 @@ template <int kBits, bool kMaster> __global__ void __launch_bounds__(kAdamTPB) k
     const bool g_al = aligned4(g_ptr, gt), p_al = aligned4(T.param, T.param_type);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const long long base = (chunk - T.first_chunk) * NTC_ADAMW_CHUNK + wave * (kWaveBlocks * NTC_STATE_BLOCK) + lane * kLane;
-#pragma unroll
+    if ((chunk - T.first_chunk + 1) * NTC_ADAMW_CHUNK <= T.numel && g_al && p_al) {
+        const bool g32 = gt == NTC_F32, p32 = T.param_type == NTC_F32;
+        if (g32) p32 ? whole_chunk<kBits, kMaster, true, true>(A, T, g_ptr, gt, rate, root, base) : whole_chunk<kBits, kMaster, true, false>(A, T, g_ptr, gt, rate, root, base);
+        else p32 ? whole_chunk<kBits, kMaster, false, true>(A, T, g_ptr, gt, rate, root, base) : whole_chunk<kBits, kMaster, false, false>(A, T, g_ptr, gt, rate, root, base);
+        return;
+    }
+#pragma unroll 1
     for (int u = 0; u < kWaveBlocks; u++) {
         const long long i = base + u * NTC_STATE_BLOCK, at = T.state_offset + i;
-        if (i - lane * kLane >= T.numel) break;      // the whole block lies past the end
+        if (i - lane * kLane >= T.numel) break;              // the whole block lies past the end
         float g[4], p[4], m[4], v[4];
         load4(g, g_ptr, gt, i, T.numel, g_al);
         if (kMaster) { const auto r = *(const Run<float, 4>*)(A.master + at); for (int j = 0; j < 4; j++) p[j] = r.v[j]; }
@@ -143,20 +241,10 @@ template <int kBits, bool kMaster> __global__ void __launch_bounds__(kAdamTPB) k
             const auto r = *(const Run<float, 4>*)((const float*)A.m + at), q = *(const Run<float, 4>*)((const float*)A.v + at);
             for (int j = 0; j < 4; j++) { m[j] = r.v[j]; v[j] = q.v[j]; }
         }
-        for (int j = 0; j < 4; j++) {
-            m[j] = m[j] * A.b1 + g[j] * A.nb1;
-            v[j] = v[j] * A.b2 + (g[j] * g[j]) * A.nb2;
-            p[j] = p[j] * A.keep - rate * (m[j] / (sqrtf(v[j]) * root + A.eps));
-        }
+        update(A, rate, root, g, p, m, v);
         if (kBits == 8) {
             uint32_t rm[4], rv[4];
-            for (int j = 0; j < 4; j += 2) {
-                const uint64_t h = ntc_hip::noise_bits(A.head, (uint64_t)(at + j) >> 1);
-                rm[j] = (uint32_t)h & 0xffffu;
-                rv[j] = (uint32_t)(h >> 16) & 0xffffu;
-                rm[j + 1] = (uint32_t)(h >> 32) & 0xffffu;
-                rv[j + 1] = (uint32_t)(h >> 48);
-            }
+            random16(A.head + (uint64_t)(at >> 1) * ntc_hip::kPhi64, rm, rv);
             const Codes c = encode_block(m, v, rm, rv);
             *(uint32_t*)((uint8_t*)A.m + at) = c.m;
             *(uint32_t*)((uint8_t*)A.v + at) = c.v;
