@@ -149,9 +149,9 @@ typedef struct ntc_fp8_matmul_desc {
     int64_t a_stride, ldc;
     int32_t a_type, a_block_rows, b_block_rows, c_type;
 } ntc_fp8_matmul_desc;
-size_t ntc_op_fp8_matmul_workspace(int64_t M, int64_t N, int64_t K);
+size_t ntc_op_fp8_matmul_workspace(int64_t M, int64_t N, int64_t K, int32_t a_type);
 int ntc_op_fp8_matmul(const ntc_fp8_matmul_desc* d, void* stream, char* why, size_t why_cap);
-/* The rows up to which A is better given as floats. */
+/* The rows of A up to which it may be given as floats. */
 int64_t ntc_op_fp8_matmul_float_rows(void);
 
 #ifdef __cplusplus

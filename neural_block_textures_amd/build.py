@@ -20,6 +20,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libntc_hip.so")
+TORCH_LIB = os.path.join(PKG, "_ops.so")
 SOURCES = ["kernels_pop.hip", "kernels_mlp.hip", "kernels_latent.hip", "kernels_quant.hip", "kernels_stats.hip", "noalloc.hip", "trainer.cpp",
            "noise_fix.cpp", "capi.cpp", "jit.cpp", "ops_logprobs.hip", "ops_adamw.hip", "ops_fp8.hip"]
 ARCH = "gfx950"
@@ -80,7 +81,27 @@ def build(verbose: bool = False, jobs: int = 4) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"linking libntc_hip.so failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    build_torch(verbose)
     return LIB
+
+
+def build_torch(verbose: bool = False) -> str:
+    """The operators' torch binding (host code only), against the libntc_hip.so beside it."""
+    from torch.utils import cpp_extension as ext
+    import sysconfig
+    tmp = TORCH_LIB + ".tmp"
+    inc = [INCLUDE, *ext.include_paths(), "/opt/rocm/include", sysconfig.get_paths()["include"]]
+    torch_lib = ext.library_paths()[0]
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wno-deprecated-declarations", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           "-DTORCH_EXTENSION_NAME=_ops", *[f"-isystem{d}" for d in inc], os.path.join(CSRC, "torch_ops.cpp"), "-o", tmp, f"-L{PKG}", "-lntc_hip", "-Wl,-rpath,$ORIGIN",
+           f"-L{torch_lib}", f"-Wl,-rpath,{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compiling torch_ops.cpp failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
 
 
 if __name__ == "__main__":

@@ -443,7 +443,7 @@ extern "C" int ntc_op_fp8_quantize(const ntc_fp8_quantize_desc* d, void* stream,
     return launched(why, cap);
 }
 
-extern "C" size_t ntc_op_fp8_matmul_workspace(int64_t M, int64_t N, int64_t K) {
+extern "C" size_t ntc_op_fp8_matmul_workspace(int64_t M, int64_t N, int64_t K, int32_t) {
     if (M < 1 || N < 1 || K < 1) return 0;
     const Plan p = plan_of(M, N, K);
     return p.parts > 1 ? (size_t)p.parts * M * N * 4 : 0;
@@ -493,7 +493,7 @@ extern "C" int ntc_op_fp8_matmul(const ntc_fp8_matmul_desc* d, void* stream, cha
     if (!d->K) return refuse(why, cap, "K is at least 1");
     if (!d->c || !d->a || !d->a_exps || !d->b || !d->b_exps) return refuse(why, cap, "a null pointer");
     if ((((uintptr_t)d->a | (uintptr_t)d->b) & 15) || (((uintptr_t)d->a_exps | (uintptr_t)d->b_exps) & 3)) return refuse(why, cap, "codes start at multiples of 16 bytes, exponents of 4");
-    if (!d->workspace && ntc_op_fp8_matmul_workspace(d->M, d->N, d->K)) return refuse(why, cap, "a null workspace");
+    if (!d->workspace && ntc_op_fp8_matmul_workspace(d->M, d->N, d->K, d->a_type)) return refuse(why, cap, "a null workspace");
     const hipStream_t s = (hipStream_t)stream;
     d->c_type == NTC_F32 ? run_matmul<f32>(d, s) : d->c_type == NTC_BF16 ? run_matmul<bf16>(d, s) : run_matmul<f16>(d, s);
     return launched(why, cap);

@@ -1,0 +1,451 @@
+// The operators of include/ntc_ops.h on torch tensors: checks of arguments, allocation of results and workspaces on the current
+// stream, and the autograd nodes. In C++ because a call's cost is otherwise the interpreter's: a layer forward and backward 224 us of
+// host work from Python nodes against the kernels' 60 to 100.
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/extension.h>
+
+#include <cmath>
+#include <optional>
+#include <vector>
+
+#include "ntc_ops.h"
+
+using at::Tensor;
+using std::optional;
+namespace py = pybind11;
+
+namespace {
+
+int type_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? NTC_F32 : t.scalar_type() == at::kBFloat16 ? NTC_BF16 : t.scalar_type() == at::kHalf ? NTC_F16 : -1; }
+int type_of(at::ScalarType t) { return t == at::kFloat ? NTC_F32 : t == at::kBFloat16 ? NTC_BF16 : t == at::kHalf ? NTC_F16 : -1; }
+
+void on_gpu(const char* name, const Tensor& t) { TORCH_CHECK_VALUE(t.defined() && t.is_cuda(), name, " must be a tensor on the GPU"); }
+void floats(const char* name, const Tensor& t) {
+    on_gpu(name, t);
+    TORCH_CHECK_VALUE(type_of(t) >= 0, name, " is ", t.scalar_type(), "; it can be float32, bfloat16, float16");
+}
+
+// One entry point on a device's current stream: a refusal is a ValueError, an error of the runtime a RuntimeError.
+template <class F> void call(const c10::Device& device, F entry) {
+    const c10::DeviceGuard guard(device);
+    char why[256] = "";
+    const int rc = entry((void*)c10::hip::getCurrentHIPStream(device.index()).stream(), why, sizeof(why));
+    TORCH_CHECK_VALUE(rc != 1, why);
+    TORCH_CHECK(rc == 0, why);
+}
+
+Tensor bytes(int64_t n, const Tensor& like) { return at::empty({ n }, like.options().dtype(at::kByte).requires_grad(false)); }
+
+// Gradients of gradients are not there: asked for, they raise instead of counting as zero.
+Tensor once(const Tensor& grad, const char* op) {
+    if (!grad.defined() || !at::GradMode::is_enabled()) return grad;
+    auto error = std::make_shared<torch::autograd::DelayedError>(std::string(op) + " is differentiable once", 1);
+    Tensor g = grad.detach();
+    g.requires_grad_(true);
+    return (*error)({ g })[0];
+}
+
+// ---------------------------------------------------------------- token log probabilities
+struct Rows { int64_t rows, inner, outer_stride, inner_stride; };
+Rows rows_of(const Tensor& t, int64_t lead, const char* name) {
+    if (lead == 0) return { 1, 1, 0, 0 };
+    if (lead == 1) return { t.size(0), std::max<int64_t>(1, t.size(0)), 0, t.stride(0) };
+    // axes but the last one joined into one stride
+    int64_t outer = 1, stride = 0;
+    for (int64_t a = lead - 2; a >= 0; a--) {
+        if (t.size(a) != 1) {
+            TORCH_CHECK_VALUE(outer == 1 || t.stride(a) == stride * outer, "the rows of ", name, " must lie at two strides at most");
+            if (outer == 1) stride = t.stride(a);
+        }
+        outer *= t.size(a);
+    }
+    return { outer * t.size(lead - 1), std::max<int64_t>(1, t.size(lead - 1)), stride, t.stride(lead - 1) };
+}
+
+ntc_logprobs_desc logprobs_desc(const Tensor& logits, const Tensor& tokens, int64_t top, double temperature, int64_t ignore) {
+    const int64_t lead = logits.dim() - 1;
+    const Rows a = rows_of(logits, lead, "logits"), b = rows_of(tokens, lead, "tokens");
+    ntc_logprobs_desc d = {};
+    d.logits = logits.const_data_ptr();
+    d.tokens = tokens.const_data_ptr();
+    d.rows = a.rows;
+    d.inner_rows = a.inner;
+    d.V = logits.size(-1);
+    d.outer_stride = a.outer_stride;
+    d.inner_stride = a.inner_stride;
+    d.token_outer_stride = b.outer_stride;
+    d.token_inner_stride = b.inner_stride;
+    d.ignore_index = ignore;
+    d.dtype = type_of(logits);
+    d.token_bytes = (int32_t)tokens.element_size();
+    d.top = (int32_t)top;
+    d.temperature = (float)temperature;
+    return d;
+}
+
+struct Logprobs { Tensor logprob, entropy, ids, top, stats; };
+Logprobs logprobs_forward(const Tensor& logits, const Tensor& tokens, int64_t top, double temperature, int64_t ignore) {
+    ntc_logprobs_desc d = logprobs_desc(logits, tokens, top, temperature, ignore);
+    const auto f = logits.options().dtype(at::kFloat).requires_grad(false);
+    Logprobs r;
+    r.logprob = at::empty(tokens.sizes(), f);
+    r.entropy = at::empty(tokens.sizes(), f);
+    r.stats = at::empty({ d.rows, 2 }, f);
+    d.logprob = r.logprob.mutable_data_ptr<float>();
+    d.entropy = r.entropy.mutable_data_ptr<float>();
+    d.stats = r.stats.mutable_data_ptr<float>();
+    if (top) {
+        std::vector<int64_t> shape = tokens.sizes().vec();
+        shape.push_back(top);
+        r.ids = at::empty(shape, f.dtype(at::kLong));
+        r.top = at::empty(shape, f);
+        d.top_ids = r.ids.mutable_data_ptr<int64_t>();
+        d.top_logprobs = r.top.mutable_data_ptr<float>();
+    }
+    const size_t size = ntc_op_token_logprobs_workspace(d.rows, d.V, d.dtype, d.top);
+    const Tensor work = size ? bytes((int64_t)size, logits) : Tensor();
+    d.workspace = size ? work.mutable_data_ptr() : nullptr;
+    call(logits.device(), [&](void* s, char* why, size_t cap) { return ntc_op_token_logprobs(&d, s, why, cap); });
+    return r;
+}
+
+struct LogprobsNode : torch::autograd::Function<LogprobsNode> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, int64_t top, double temperature, int64_t ignore) {
+        const Logprobs r = logprobs_forward(logits, tokens, top, temperature, ignore);
+        ctx->save_for_backward({ logits, tokens, r.entropy, r.stats, r.ids });
+        ctx->saved_data["top"] = top;
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["ignore"] = ignore;
+        ctx->set_materialize_grads(false);
+        if (!top) return { r.logprob, r.entropy };
+        ctx->mark_non_differentiable({ r.ids });
+        return { r.logprob, r.entropy, r.ids, r.top };
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &logits = saved[0], &tokens = saved[1];
+        const int64_t top = ctx->saved_data["top"].toInt();
+        Tensor grads[3] = { g[0], g[1], top ? g[3] : Tensor() };
+        Tensor dlogits;
+        if (grads[0].defined() || grads[1].defined() || grads[2].defined()) {
+            ntc_logprobs_desc d = logprobs_desc(logits, tokens, top, ctx->saved_data["temperature"].toDouble(), ctx->saved_data["ignore"].toInt());
+            const float* p[3];
+            for (int i = 0; i < 3; i++) {
+                if (grads[i].defined()) grads[i] = grads[i].contiguous();
+                p[i] = grads[i].defined() ? grads[i].const_data_ptr<float>() : nullptr;
+            }
+            dlogits = at::empty(logits.sizes(), logits.options().requires_grad(false));
+            d.entropy = saved[2].data_ptr<float>();
+            d.stats = saved[3].data_ptr<float>();
+            d.top_ids = top ? saved[4].data_ptr<int64_t>() : nullptr;
+            d.g_logprob = p[0];
+            d.g_entropy = p[1];
+            d.g_top = p[2];
+            d.dlogits = dlogits.mutable_data_ptr();
+            call(logits.device(), [&](void* s, char* why, size_t cap) { return ntc_op_token_logprobs_backward(&d, s, why, cap); });
+        }
+        return { once(dlogits, "token_logprobs"), Tensor(), Tensor(), Tensor(), Tensor() };
+    }
+};
+
+py::tuple token_logprobs(const Tensor& logits, Tensor tokens, int64_t top, double temperature, int64_t ignore) {
+    floats("logits", logits);
+    on_gpu("tokens", tokens);
+    TORCH_CHECK_VALUE(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt, "tokens is ", tokens.scalar_type(), "; it can be int64, int32");
+    TORCH_CHECK_VALUE(logits.dim() >= 1 && tokens.sizes() == logits.sizes().slice(0, logits.dim() - 1) && tokens.device() == logits.device(),
+                      "tokens ", tokens.sizes(), " must have the shape of logits ", logits.sizes(), " without its last axis, on its device");
+    const int64_t V = logits.size(-1);
+    TORCH_CHECK_VALUE(V >= 1 && (V == 1 || logits.stride(-1) == 1), "a row of logits must hold at least one value, contiguous");
+    TORCH_CHECK_VALUE(top >= 0 && top <= std::min<int64_t>(NTC_MAX_TOP, V), "top is 0 to ", std::min<int64_t>(NTC_MAX_TOP, V), ", not ", top);
+    TORCH_CHECK_VALUE(temperature > 0 && temperature < 3e38, "temperature must be positive and finite, not ", temperature);
+    if (tokens.dim() > 2) tokens = tokens.contiguous();
+    if (logits.requires_grad() && at::GradMode::is_enabled()) {
+        auto r = LogprobsNode::apply(logits, tokens, top, temperature, ignore);
+        return top ? py::make_tuple(r[0], r[1], r[2], r[3]) : py::make_tuple(r[0], r[1], py::none(), py::none());
+    }
+    const Logprobs r = logprobs_forward(logits, tokens, top, temperature, ignore);
+    return top ? py::make_tuple(r.logprob, r.entropy, r.ids, r.top) : py::make_tuple(r.logprob, r.entropy, py::none(), py::none());
+}
+
+// ---------------------------------------------------------------- 8-bit floating point in blocks
+int64_t blocks_of(int64_t n, int64_t b) { return (n + b - 1) / b; }
+
+// A matrix in 8 bits inside one buffer: codes, then exponents.
+struct Held {
+    Tensor buffer;
+    int64_t R = 0, K = 0, block = 1;
+    uint8_t* codes() const { return (uint8_t*)buffer.data_ptr(); }
+    uint8_t* exps() const { return codes() + R * ntc_fp8_code_stride(K); }
+    Held() = default;
+    Held(int64_t r, int64_t k, int64_t b, const Tensor& like) : R(r), K(k), block(b) { buffer = bytes(r * ntc_fp8_code_stride(k) + blocks_of(r, b) * ntc_fp8_exp_stride(k), like); }
+};
+
+void run_quantize(const Tensor& x, int64_t block, uint8_t* codes, uint8_t* exps, uint8_t* codes_t, uint8_t* exps_t) {
+    if (!x.numel()) return;
+    const ntc_fp8_quantize_desc d = { x.const_data_ptr(), x.size(0), x.size(1), x.stride(0), type_of(x), (int32_t)block, codes, exps, codes_t, exps_t };
+    call(x.device(), [&](void* s, char* why, size_t cap) { return ntc_op_fp8_quantize(&d, s, why, cap); });
+}
+Tensor rows_contiguous(const Tensor& x) { return (x.size(1) > 1 && x.stride(1) != 1) || x.stride(0) < 0 ? x.contiguous() : x; }
+
+struct Operand { const void* p; const uint8_t* exps; int64_t rows, stride; int type, block; };
+Operand operand(const Held& h) { return { h.codes(), h.exps(), h.R, 0, NTC_FP8, (int)h.block }; }
+void run_matmul(const Operand& a, const Operand& b, int64_t K, const Tensor& c) {
+    if (!a.rows || !b.rows) return;
+    if (!K) { c.zero_(); return; }
+    const size_t size = ntc_op_fp8_matmul_workspace(a.rows, b.rows, K, a.type);
+    const Tensor work = size ? bytes((int64_t)size, c) : Tensor();
+    const ntc_fp8_matmul_desc d = { a.p, a.exps, (const uint8_t*)b.p, b.exps, c.mutable_data_ptr(), size ? work.mutable_data_ptr() : nullptr, a.rows, b.rows, K, a.stride, c.stride(0),
+                                    a.type, a.block, b.block, type_of(c) };
+    call(c.device(), [&](void* s, char* why, size_t cap) { return ntc_op_fp8_matmul(&d, s, why, cap); });
+}
+Tensor matrix(int64_t m, int64_t n, at::ScalarType t, const Tensor& like) { return at::empty({ m, n }, like.options().dtype(t).requires_grad(false)); }
+
+py::tuple quantize(const Tensor& x_, int64_t block, bool plain, bool transposed) {
+    floats("x", x_);
+    TORCH_CHECK_VALUE(x_.dim() == 2, "a matrix is needed, not ", x_.sizes());
+    TORCH_CHECK_VALUE(block == 1 || block == 128, "blocks have 1 or 128 rows, not ", block);
+    const Tensor x = rows_contiguous(x_);
+    const int64_t R = x.size(0), K = x.size(1);
+    const auto o = x.options().dtype(at::kByte).requires_grad(false);
+    const auto make = [&](int64_t r, int64_t k) { return std::make_pair(at::empty({ r, ntc_fp8_code_stride(k) }, o), at::empty({ blocks_of(r, block), ntc_fp8_exp_stride(k) }, o)); };
+    std::pair<Tensor, Tensor> q, t;
+    if (plain) q = make(R, K);
+    if (transposed) t = make(K, R);
+    const auto at_ = [](const Tensor& b) { return b.defined() ? (uint8_t*)b.data_ptr() : nullptr; };
+    run_quantize(x, block, at_(q.first), at_(q.second), at_(t.first), at_(t.second));
+    return py::make_tuple(plain ? py::cast(q) : py::none(), transposed ? py::cast(t) : py::none());
+}
+
+Operand given(const char* name, const Tensor& codes, const Tensor& exps, int64_t R, int64_t K, int64_t block) {
+    on_gpu(name, codes);
+    on_gpu(name, exps);
+    const bool ok = (block == 1 || block == 128) && codes.scalar_type() == at::kByte && exps.scalar_type() == at::kByte && codes.is_contiguous() && exps.is_contiguous() &&
+                    codes.device() == exps.device() && R >= 0 && K >= 0;
+    TORCH_CHECK_VALUE(ok && codes.sizes() == at::IntArrayRef({ R, ntc_fp8_code_stride(K) }) && (uintptr_t)codes.const_data_ptr() % 16 == 0, name, ".codes must be uint8, contiguous, start at a multiple of 16 bytes and be [",
+                      R, ", ", ntc_fp8_code_stride(K), "]");
+    TORCH_CHECK_VALUE(exps.sizes() == at::IntArrayRef({ blocks_of(R, block), ntc_fp8_exp_stride(K) }) && (uintptr_t)exps.const_data_ptr() % 4 == 0, name,
+                      ".exps must be uint8, contiguous, start at a multiple of 4 bytes and be [", blocks_of(R, block), ", ", ntc_fp8_exp_stride(K), "]");
+    return { codes.const_data_ptr(), (const uint8_t*)exps.const_data_ptr(), R, 0, NTC_FP8, (int)block };
+}
+
+Tensor matmul(const Tensor& ac, const Tensor& ae, int64_t M, int64_t ka, int64_t a_block, const Tensor& bc, const Tensor& be, int64_t N, int64_t kb, int64_t b_block, at::ScalarType type) {
+    const Operand a = given("a", ac, ae, M, ka, a_block), b = given("b", bc, be, N, kb, b_block);
+    TORCH_CHECK_VALUE(ka == kb && ac.device() == bc.device(), "a [", M, ", ", ka, "] and b [", N, ", ", kb, "] must have as many columns, on one device");
+    TORCH_CHECK_VALUE(type_of(type) >= 0, "products are float32, bfloat16 or float16, not ", type);
+    const Tensor c = matrix(M, N, type, ac);
+    run_matmul(a, b, ka, c);
+    return c;
+}
+
+struct LinearNode : torch::autograd::Function<LinearNode> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w) {
+        const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+        const bool need_x = x.requires_grad(), need_w = w.requires_grad();
+        const Held xq(M, K, 1, x), wq(N, K, 128, x);
+        const Held xt = need_w ? Held(K, M, 1, x) : Held(), wt = need_x ? Held(K, N, 128, x) : Held();
+        run_quantize(x, 1, xq.codes(), xq.exps(), need_w ? xt.codes() : nullptr, need_w ? xt.exps() : nullptr);
+        run_quantize(w, 128, wq.codes(), wq.exps(), need_x ? wt.codes() : nullptr, need_x ? wt.exps() : nullptr);
+        const Tensor y = matrix(M, N, x.scalar_type(), x);
+        run_matmul(operand(xq), operand(wq), K, y);
+        ctx->save_for_backward({ xt.buffer, wt.buffer });
+        ctx->saved_data["M"] = M;
+        ctx->saved_data["N"] = N;
+        ctx->saved_data["K"] = K;
+        ctx->saved_data["x"] = (int64_t)x.scalar_type();
+        ctx->saved_data["w"] = (int64_t)w.scalar_type();
+        ctx->set_materialize_grads(false);
+        return y;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+        if (!g[0].defined()) return { Tensor(), Tensor() };
+        const auto saved = ctx->get_saved_variables();
+        const int64_t M = ctx->saved_data["M"].toInt(), N = ctx->saved_data["N"].toInt(), K = ctx->saved_data["K"].toInt();
+        const bool need_x = saved[1].defined(), need_w = saved[0].defined();
+        const Tensor dy = rows_contiguous(g[0]);
+        const Held dq = need_x ? Held(M, N, 1, dy) : Held(), dt = need_w ? Held(N, M, 1, dy) : Held();
+        run_quantize(dy, 1, need_x ? dq.codes() : nullptr, need_x ? dq.exps() : nullptr, need_w ? dt.codes() : nullptr, need_w ? dt.exps() : nullptr);
+        Tensor dx, dw;
+        const auto held = [](const Tensor& b, int64_t r, int64_t k, int64_t block) { Held h; h.buffer = b; h.R = r; h.K = k; h.block = block; return h; };
+        if (need_x) {
+            dx = matrix(M, K, (at::ScalarType)ctx->saved_data["x"].toInt(), dy);
+            run_matmul(operand(dq), operand(held(saved[1], K, N, 128)), N, dx);
+        }
+        if (need_w) {
+            dw = matrix(N, K, (at::ScalarType)ctx->saved_data["w"].toInt(), dy);
+            run_matmul(operand(dt), operand(held(saved[0], K, M, 1)), M, dw);
+        }
+        return { once(dx, "fp8_linear"), once(dw, "fp8_linear") };
+    }
+};
+
+Tensor as_rows(const Tensor& x) {
+    int64_t rows = 1;
+    for (int64_t a = 0; a + 1 < x.dim(); a++) rows *= x.size(a);
+    return x.dim() == 2 ? x : x.reshape({ rows, x.size(-1) });
+}
+Tensor like_rows(const Tensor& y, const Tensor& x) {
+    if (x.dim() == 2) return y;
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = y.size(1);
+    return y.view(shape);
+}
+
+Tensor linear(const Tensor& x, const Tensor& w) {
+    floats("x", x);
+    floats("w", w);
+    TORCH_CHECK_VALUE(x.dim() >= 1, "x must have at least one axis");
+    TORCH_CHECK_VALUE(w.dim() == 2 && w.size(1) == x.size(-1) && w.device() == x.device(), "w ", w.sizes(), " must be a matrix with x's ", x.size(-1), " columns, on its device");
+    const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad());
+    const Tensor x2 = rows_contiguous(as_rows(x)), w2 = rows_contiguous(w);
+    if (grad) return like_rows(LinearNode::apply(x2, w2), x);
+    const Held xq(x2.size(0), x2.size(1), 1, x2), wq(w2.size(0), w2.size(1), 128, x2);
+    run_quantize(x2, 1, xq.codes(), xq.exps(), nullptr, nullptr);
+    run_quantize(w2, 128, wq.codes(), wq.exps(), nullptr, nullptr);
+    const Tensor y = matrix(x2.size(0), w2.size(0), x.scalar_type(), x2);
+    run_matmul(operand(xq), operand(wq), x2.size(1), y);
+    return like_rows(y, x);
+}
+
+Tensor linear_fp8(const Tensor& x, const Tensor& codes, const Tensor& exps, int64_t N, int64_t K, int64_t block) {
+    floats("x", x);
+    const Operand b = given("w", codes, exps, N, K, block);
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == K && x.device() == codes.device(), "x ", x.sizes(), " must have w's ", K, " columns, on its device");
+    TORCH_CHECK_VALUE(!(x.requires_grad() && at::GradMode::is_enabled()), "w in 8 bits is for inference: give the weights themselves for a gradient");
+    const Tensor x2 = rows_contiguous(as_rows(x));
+    const int64_t M = x2.size(0);
+    const Tensor y = matrix(M, N, x.scalar_type(), x2);
+    if (M <= ntc_op_fp8_matmul_float_rows()) {
+        run_matmul({ x2.const_data_ptr(), nullptr, M, x2.stride(0), type_of(x2), 1 }, b, K, y);
+    } else {
+        const Held xq(M, K, 1, x2);
+        run_quantize(x2, 1, xq.codes(), xq.exps(), nullptr, nullptr);
+        run_matmul(operand(xq), b, K, y);
+    }
+    return like_rows(y, x);
+}
+
+// ---------------------------------------------------------------- AdamW
+// The tensors of an optimizer, and what their step needs beside its state.
+struct AdamwPlan {
+    std::vector<Tensor> params;
+    std::vector<const void*> pointers;
+    Tensor table, chunk_tensor;
+    std::vector<int64_t> first_chunk, offsets;
+    std::vector<int32_t> steps;
+    int64_t size = 0, calls = 0;
+
+    explicit AdamwPlan(std::vector<Tensor> p) : params(std::move(p)) {
+        TORCH_CHECK_VALUE(!params.empty(), "no parameters");
+        std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+        std::vector<ntc_adamw_tensor> rows;
+        std::vector<int32_t> of_chunk;
+        first_chunk.push_back(0);
+        for (const Tensor& t : params) {
+            floats("a parameter", t);
+            TORCH_CHECK_VALUE(t.is_contiguous() && t.device() == params[0].device(), "parameters are contiguous and on one device");
+            const int64_t n = t.numel(), chunks = blocks_of(n, NTC_ADAMW_CHUNK);
+            const uintptr_t at = (uintptr_t)t.const_data_ptr();
+            if (n) spans.push_back({ at, at + (uintptr_t)(n * t.element_size()) });
+            TORCH_CHECK_VALUE(first_chunk.back() + chunks < (int64_t)1 << 31, "too many weights");
+            rows.push_back({ (void*)at, n, size, type_of(t), (int32_t)first_chunk.back() });
+            of_chunk.insert(of_chunk.end(), (size_t)chunks, (int32_t)pointers.size());
+            pointers.push_back((const void*)at);
+            offsets.push_back(size);
+            size += blocks_of(n, NTC_STATE_BLOCK) * NTC_STATE_BLOCK;
+            first_chunk.push_back(first_chunk.back() + chunks);
+        }
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); i++) TORCH_CHECK_VALUE(spans[i - 1].second <= spans[i].first, "parameters overlap");
+        const c10::DeviceGuard guard(params[0].device());
+        const auto up = [&](void* p, size_t n) { return at::from_blob(p, { (int64_t)n }, at::kByte).to(params[0].device()); };
+        table = up(rows.data(), rows.size() * sizeof(rows[0]));
+        chunk_tensor = up(of_chunk.data(), of_chunk.size() * sizeof(of_chunk[0]));
+        steps.resize(params.size());
+    }
+
+    // one gradient or None a parameter; None for all: the parameters' own
+    void step(const optional<std::vector<optional<Tensor>>>& given, const Tensor& m, const Tensor& v, const optional<Tensor>& me, const optional<Tensor>& ve, const optional<Tensor>& master, int64_t bits,
+              double lr, double b1, double b2, double eps, double decay, uint64_t seed) {
+        const size_t n = params.size();
+        TORCH_CHECK_VALUE(!given || given->size() == n, given ? given->size() : 0, " gradients for ", n, " parameters");
+        std::vector<Tensor> keep;                           // copies of gradients that are not contiguous, until their launch
+        std::vector<const void*> g(n, nullptr);
+        std::vector<int32_t> types(n, 0), next(steps);
+        const auto device = params[0].device();
+        for (size_t i = 0; i < n; i++) {
+            TORCH_CHECK_VALUE(params[i].const_data_ptr() == pointers[i], "a parameter has moved to other memory since the optimizer was made");
+            const Tensor& t = given ? ((*given)[i] ? *(*given)[i] : undefined) : params[i].grad();
+            if (!t.defined()) continue;
+            types[i] = type_of(t);
+            TORCH_CHECK_VALUE(types[i] >= 0 && t.device() == device && t.sizes() == params[i].sizes(), "gradient ", i, " must have its parameter's shape ", params[i].sizes(),
+                              ", be on its device, and be float32, bfloat16 or float16");
+            if (t.is_contiguous()) g[i] = t.const_data_ptr();
+            else { keep.push_back(t.contiguous()); g[i] = keep.back().const_data_ptr(); }
+            next[i]++;
+        }
+        const auto at_ = [](const optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; };
+        ntc_adamw_desc d = {};
+        d.tensors = (const ntc_adamw_tensor*)table.const_data_ptr();
+        d.chunk_tensor = (const int32_t*)chunk_tensor.const_data_ptr();
+        d.first_chunk = first_chunk.data();
+        d.grads = g.data();
+        d.grad_types = types.data();
+        d.steps = next.data();
+        d.n = (int64_t)n;
+        d.exp_avg = m.data_ptr();
+        d.exp_avg_sq = v.data_ptr();
+        d.exp_avg_exp = (uint8_t*)at_(me);
+        d.exp_avg_sq_exp = (uint8_t*)at_(ve);
+        d.master = (float*)at_(master);
+        d.lr = lr;
+        d.beta1 = b1;
+        d.beta2 = b2;
+        d.eps = eps;
+        d.weight_decay = decay;
+        d.seed = seed;
+        d.calls = (uint32_t)(calls + 1);
+        d.state_bits = (int32_t)bits;
+        call(device, [&](void* s, char* why, size_t cap) { return ntc_op_adamw(&d, s, why, cap); });
+        for (Tensor& t : params) if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();     // (changed in place, behind autograd's back)
+        steps = next;
+        calls++;
+    }
+    const Tensor undefined;
+};
+
+std::pair<Tensor, Tensor> adamw_moments(const Tensor& m, const Tensor& v, const Tensor& me, const Tensor& ve) {
+    const Tensor a = at::empty(m.sizes(), m.options().dtype(at::kFloat)), b = at::empty(m.sizes(), m.options().dtype(at::kFloat));
+    call(m.device(), [&](void* s, char* why, size_t cap) {
+        return ntc_op_adamw_moments(m.const_data_ptr(), v.const_data_ptr(), (const uint8_t*)me.const_data_ptr(), (const uint8_t*)ve.const_data_ptr(), m.numel(), a.mutable_data_ptr<float>(),
+                                    b.mutable_data_ptr<float>(), s, why, cap);
+    });
+    return { a, b };
+}
+void adamw_encode(const Tensor& m, const Tensor& v, const Tensor& cm, const Tensor& cv, const Tensor& me, const Tensor& ve) {
+    call(m.device(), [&](void* s, char* why, size_t cap) {
+        return ntc_op_adamw_encode(m.const_data_ptr<float>(), v.const_data_ptr<float>(), m.numel(), cm.data_ptr(), cv.data_ptr(), (uint8_t*)me.data_ptr(), (uint8_t*)ve.data_ptr(), s, why, cap);
+    });
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_ops, m) {
+    m.doc() = "The operators of ops.py on torch tensors";
+    m.def("token_logprobs", &token_logprobs);
+    m.def("quantize", &quantize);
+    m.def("matmul", [](const Tensor& ac, const Tensor& ae, int64_t M, int64_t ka, int64_t a_block, const Tensor& bc, const Tensor& be, int64_t N, int64_t kb, int64_t b_block, py::object type) {
+        return matmul(ac, ae, M, ka, a_block, bc, be, N, kb, b_block, torch::python::detail::py_object_to_dtype(type));
+    });
+    m.def("linear", &linear);
+    m.def("linear_fp8", &linear_fp8);
+    m.def("adamw_moments", &adamw_moments);
+    m.def("adamw_encode", &adamw_encode);
+    py::class_<AdamwPlan>(m, "AdamwPlan")
+        .def(py::init<std::vector<Tensor>>())
+        .def("step", &AdamwPlan::step)
+        .def_readonly("offsets", &AdamwPlan::offsets)
+        .def_readonly("size", &AdamwPlan::size)
+        .def_readwrite("calls", &AdamwPlan::calls)
+        .def_readwrite("steps", &AdamwPlan::steps);
+}
