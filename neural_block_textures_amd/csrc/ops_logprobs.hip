@@ -36,8 +36,12 @@ __device__ __forceinline__ long long token_of(const ntc_logprobs_desc& d, long l
 }
 
 template <class T> __device__ __forceinline__ const T* row_of(const ntc_logprobs_desc& d, long long row, long long& outer, long long& inner) {
-    outer = row / d.inner_rows;
-    inner = row % d.inner_rows;
+    outer = 0;
+    inner = row;
+    if (d.inner_rows < d.rows) {                            // (fewer than 2^31 rows: a 64-bit division is a tenth of a short row's work)
+        outer = (uint32_t)row / (uint32_t)d.inner_rows;
+        inner = (uint32_t)row % (uint32_t)d.inner_rows;
+    }
     return (const T*)d.logits + outer * d.outer_stride + inner * d.inner_stride;
 }
 // The results of a row but its alternatives, from its softmax with the largest value m (kLowest or less: see none).
@@ -51,76 +55,69 @@ template <class T> __device__ __forceinline__ void write_row(const ntc_logprobs_
 }
 
 // ---------------------------------------------------------------- short rows
-// A group of kGroup lanes holds a row in registers, kEach values a lane (vectors of 16 bytes, dealt in turn): the largest, then the
-// sums, then the alternatives one by one, each the largest key below the last. Keys are integers that order as the values do, larger for
-// the lower of equal ones' indices: 16-bit types in one word; a 32-bit one's index is found in a second reduction.
-template <class T> __device__ __forceinline__ uint32_t order_key(T x) {
-    if constexpr (sizeof(T) == 2) {
-        const uint32_t h = __builtin_bit_cast(uint16_t, x), a = h & 0x7fffu, inf = type_code<T> == NTC_BF16 ? 0x7f80u : 0x7c00u;
-        if (a > inf) return 0x8000u - inf;                  // NaN as -inf
-        return h & 0x8000u ? 0x8000u - a : 0x8000u + a;     // (-0 as 0)
-    } else {
-        const uint32_t h = __float_as_uint(x), a = h & 0x7fffffffu;
-        if (a > 0x7f800000u) return 0x80000000u - 0x7f800000u;
-        return h & 0x80000000u ? 0x80000000u - a : 0x80000000u + a;
-    }
+// Integers that order as floats do (-0 as 0), and back.
+__device__ __forceinline__ uint32_t order_key(float x) {
+    const uint32_t h = __float_as_uint(x + 0.0f);
+    return h ^ ((uint32_t)((int)h >> 31) | 0x80000000u);
 }
-template <class T> __device__ __forceinline__ float key_value(uint32_t key) {
-    if constexpr (sizeof(T) == 2) {
-        const uint16_t h = key >= 0x8000u ? (uint16_t)(key - 0x8000u) : (uint16_t)(0x8000u | (0x8000u - key));
-        return (float)__builtin_bit_cast(T, h);
-    } else {
-        return __uint_as_float(key >= 0x80000000u ? key - 0x80000000u : 0x80000000u | (0x80000000u - key));
-    }
-}
+__device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 
+// A group of kGroup lanes holds a row in registers, kEach neighbouring values a lane: the largest, then the sums, then the alternatives one by
+// one, each the largest key below the last. A 16-bit type's float has 13 low bits to spare, which take the index (of a row of at most
+// 1024, from the top down): one word orders values and indices both. A 32-bit value's index is found in a second reduction.
+// Bound by instructions: 262144 rows of 256 bf16 values with 4 alternatives take twice what their bytes do.
+constexpr int kShort = 1024;                                 // the longest such row
 template <class T, int kGroup, int kEach> __global__ void __launch_bounds__(256) k_logprobs_short(ntc_logprobs_desc d) {
-    constexpr int kVec = 16 / (int)sizeof(T), kVecs = kEach / kVec > 0 ? kEach / kVec : 1, kE = kEach < kVec ? kEach : kVec;   // values a vector
+    constexpr int kVec = 16 / (int)sizeof(T) < kEach ? 16 / (int)sizeof(T) : kEach;
+    constexpr uint32_t kMask = ~0x1fffu;
+    static_assert(kGroup * kEach <= kShort, "indices of 10 bits");
     const int in = threadIdx.x % kGroup;
     const long long row = (long long)blockIdx.x * (256 / kGroup) + threadIdx.x / kGroup;
     if (row >= d.rows) return;                              // whole groups
     long long outer, inner;
     const T* x = row_of<T>(d, row, outer, inner);
-    const int V = (int)d.V;
+    const int V = (int)d.V, at = in * kEach;
     const float inv_t = 1.0f / d.temperature, k = kLog2e / d.temperature;
-    T v[kVecs][kE];
-    float m = -NTC_INF;
+    float v[kEach];
 #pragma unroll
-    for (int i = 0; i < kVecs; i++) {
-        const int at = (i * kGroup + in) * kE;
-        if (at + kE <= V) { const auto r = *(const LooseRun<T, kE>*)(x + at); for (int j = 0; j < kE; j++) v[i][j] = r.v[j]; }
-        else for (int j = 0; j < kE; j++) v[i][j] = at + j < V ? x[at + j] : (T)-NTC_INF;
-        for (int j = 0; j < kE; j++) m = fmaxf(m, (float)v[i][j]);
+    for (int i = 0; i < kEach; i += kVec) {
+        if (at + i + kVec <= V) { const auto r = *(const LooseRun<T, kVec>*)(x + at + i); for (int j = 0; j < kVec; j++) v[i + j] = (float)r.v[j]; }
+        else for (int j = 0; j < kVec; j++) v[i + j] = at + i + j < V ? (float)x[at + i + j] : -NTC_INF;
     }
     const auto larger = [](float a, float b) { return fmaxf(a, b); };
     const auto sum = [](float a, float b) { return a + b; };
+    float m = v[0];
+#pragma unroll
+    for (int j = 1; j < kEach; j++) m = fmaxf(m, v[j]);
     m = reduce<kGroup>(m, larger);
     const float mm = m == -NTC_INF ? 0.0f : m;              // nothing left: every exponential is 0
     float s = 0.0f, t = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kVecs; i++)
-#pragma unroll
-        for (int j = 0; j < kE; j++) {
-            const float q = ((float)v[i][j] - mm) * k, e = fast_exp2(q);
-            s += e;
-            t = __builtin_fmaf(e, fmaxf(q, -1e30f), t);
-        }
+    for (int j = 0; j < kEach; j++) {
+        const float q = (v[j] - mm) * k, e = fast_exp2(q);
+        s += e;
+        t = __builtin_fmaf(e, fmaxf(q, -1e30f), t);
+    }
     s = reduce<kGroup>(s, sum);
     t = reduce<kGroup>(t, sum);
     const bool none = s == 0.0f;
     const float log_s = fast_log2(s);
     if (in == 0) write_row(d, row, x, token_of(d, outer, inner), mm, log_s, t / s, none, inv_t);
     if (!d.top) return;
-    uint32_t key[kVecs][kE];
+    if (__ballot(s != s)) {                                  // a NaN somewhere (or +inf): in the order it counts as -inf
 #pragma unroll
-    for (int i = 0; i < kVecs; i++)
+        for (int j = 0; j < kEach; j++) v[j] = v[j] != v[j] ? -NTC_INF : v[j];
+    }
+    uint32_t key[kEach];
 #pragma unroll
-        for (int j = 0; j < kE; j++) {
-            const int at = (i * kGroup + in) * kE + j;
-            key[i][j] = order_key<T>(v[i][j]);
-            if constexpr (sizeof(T) == 2) key[i][j] = key[i][j] << 16 | (uint32_t)(0xffff - at);
-            if (at >= V) key[i][j] = 0;
-        }
+    for (int j = 0; j < kEach; j++) {
+        key[j] = order_key(v[j]);
+        if constexpr (sizeof(T) == 2) key[j] = (key[j] & kMask) | (uint32_t)(kShort - 1 - at - j);
+    }
+    if (V < kGroup * kEach) {
+#pragma unroll
+        for (int j = 0; j < kEach; j++) key[j] = at + j < V ? key[j] : 0;   // below every key of a value
+    }
     const auto above = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
     const auto below = [](uint32_t a, uint32_t b) { return a < b ? a : b; };
     uint32_t mine = 0, mine_at = 0, last = 0, last_at = 0;
@@ -129,33 +126,28 @@ template <class T, int kGroup, int kEach> __global__ void __launch_bounds__(256)
         if constexpr (sizeof(T) == 2) {
             // the largest below the last: key - last wraps to the top of the range for just those
 #pragma unroll
-            for (int i = 0; i < kVecs; i++)
-#pragma unroll
-                for (int j = 0; j < kE; j++) best = above(best, key[i][j] - last);
+            for (int j = 0; j < kEach; j++) best = above(best, key[j] - last);
             last = reduce<kGroup>(best, above) + last;
-            last_at = 0xffffu - (last & 0xffffu);
         } else {
-            // the taken ones are those above the last, and those equal to it up to its index
-            uint32_t at = 0xffffffffu;
+            // open are those below the last, and those equal to it past its index; ascending j: the first of equals stays
+            uint32_t place = 0xffffffffu;
 #pragma unroll
-            for (int i = 0; i < kVecs; i++)
-#pragma unroll
-                for (int j = 0; j < kE; j++) {
-                    const uint32_t c = (uint32_t)((i * kGroup + in) * kE + j);
-                    const bool open = r == 0 || key[i][j] < last || (key[i][j] == last && c > last_at);
-                    if (open && (int)c < V && (key[i][j] > best || at == 0xffffffffu)) { best = key[i][j]; at = c; }   // ascending c: the first of equals stays
-                }
-            const uint32_t top = reduce<kGroup>(at == 0xffffffffu ? 0u : best, above);
-            last_at = reduce<kGroup>(best == top ? at : 0xffffffffu, below);
-            last = top;
+            for (int j = 0; j < kEach; j++) {
+                const bool open = r == 0 || key[j] < last || (key[j] == last && (uint32_t)(at + j) > last_at);
+                if (open && at + j < V && (key[j] > best || place == 0xffffffffu)) { best = key[j]; place = (uint32_t)(at + j); }
+            }
+            last = reduce<kGroup>(place == 0xffffffffu ? 0u : best, above);
+            last_at = reduce<kGroup>(best == last ? place : 0xffffffffu, below);
         }
         if (in == r) { mine = last; mine_at = last_at; }
     }
     if (in < d.top) {
-        if constexpr (sizeof(T) == 2) mine >>= 16;
+        if constexpr (sizeof(T) == 2) {
+            mine_at = kShort - 1 - (mine & (kShort - 1));
+            mine = mine & 0x80000000u ? mine & kMask : mine | ~kMask;
+        }
         d.top_ids[row * d.top + in] = mine_at;
-        // (a NaN anywhere has made log_s NaN; its own place reads -inf here, which NaN swallows)
-        d.top_logprobs[row * d.top + in] = none ? -NTC_INF : log_prob(key_value<T>(mine), mm, inv_t, log_s);
+        d.top_logprobs[row * d.top + in] = none ? -NTC_INF : log_prob(key_value(mine), mm, inv_t, log_s);
     }
 }
 
@@ -177,6 +169,29 @@ struct Best {
         i = l < at ? i : l == at ? j : ui;
     }
 };
+
+// The best of up to 64 lists in LDS (list p's values at v + p stride, indices at i + p stride): each lane holds the head of one, the
+// best head of all is taken and its lane moves on.
+__device__ __forceinline__ Best merge(const float* v, const int* i, int stride, int lists, int top) {
+    const int lane = lane_id();
+    int at = lane * stride, left = lane < lists ? top : 0;
+    float hv = left ? v[at] : -NTC_INF;
+    int hi = left ? i[at] : kNoIndex;
+    Best best;
+    best.clear();
+    for (int r = 0; r < top; r++) {
+        const float bv = reduce64(hv, [](float p, float q) { return fmaxf(p, q); });
+        const int bi = (int)reduce64((uint32_t)(hv == bv ? hi : kNoIndex), [](uint32_t p, uint32_t q) { return p < q ? p : q; });
+        if (lane == r) { best.v = bv; best.i = bi; }
+        if (hv == bv && hi == bi && left) {
+            at++;
+            left--;
+            hv = left ? v[at] : -NTC_INF;
+            hi = left ? i[at] : kNoIndex;
+        }
+    }
+    return best;
+}
 
 // What a lane reads at a time: kRun values in vectors of 16 bytes.
 template <class T> struct Long { static constexpr int kVec = 16 / (int)sizeof(T), kVecs = 2, kRun = kVec * kVecs, kChunk = 64 * kRun; };
@@ -252,6 +267,7 @@ template <class T> __device__ __forceinline__ void scan(const T* x, int V, int f
         }
         fresh = false;
     }
+    if (a.s == 0.0f) return;                                 // (nothing above the floor: its m k has no meaning)
     // the sums were taken on the rounded m k: to those on m itself
     const float off = __builtin_fmaf(a.m, k, -mk);           // m k - fl(m k): every exponent was that much too large
     a.t -= a.s * off;
@@ -294,7 +310,7 @@ template <class T> __device__ __forceinline__ void finish(const ntc_logprobs_des
     if (lane == 0) write_row(d, row, x, t, a.m, log_s, a.t / a.s, none, inv_t);
     if (!d.top) return;
     int have = __builtin_popcountll(__ballot(lane < d.top && best.i != kNoIndex));
-    for (int i = 0; have < d.top; i += 64) {                 // (ends: top <= V, and each value is a number above -inf or not)
+    for (int i = 0; have < d.top && i < V; i += 64) {
         const bool low = i + lane < V && !((float)x[i + lane < V ? i + lane : 0] > -NTC_INF);
         unsigned long long ask = __ballot(low);
         while (ask && have < d.top) {
@@ -332,15 +348,8 @@ template <class T, int kWaves, bool kParts> __global__ void __launch_bounds__(25
         if (lane < d.top) { list_v[wave][lane] = best.v; list_i[wave][lane] = best.i; }
         __syncthreads();
         if (wave) return;
-        for (int w = 1; w < kWaves; w++) {
-            soft_join(a, soft[w], k);
-            for (int r = 0; r < d.top; r++) {                // in order: the first that does not pass the list's last ends it
-                const float v = list_v[w][r];
-                const int i = list_i[w][r];
-                if (!(i != kNoIndex) || !(v > read_lane(best.v, d.top - 1) || (v == read_lane(best.v, d.top - 1) && i < __builtin_amdgcn_readlane(best.i, d.top - 1)))) break;
-                best.insert(v, i);
-            }
-        }
+        for (int w = 1; w < kWaves; w++) soft_join(a, soft[w], k);
+        if (d.top) best = merge(list_v[0], list_i[0], NTC_MAX_TOP, kWaves, d.top);
     }
     if (!kParts) { finish(d, row, x, token_of(d, outer, inner), a, best); return; }
     const int parts = gridDim.y;
@@ -349,30 +358,25 @@ template <class T, int kWaves, bool kParts> __global__ void __launch_bounds__(25
     if (lane < d.top) { to[4 + lane] = best.v; ((int*)to)[4 + d.top + lane] = best.i; }
 }
 
-// Joins a row's parts: a wave a row, part p's sums in lane p % 64. The lists go through LDS, since they are walked one value at a time.
+// Joins a row's parts: part p's sums and list in lane p.
 constexpr int kMostParts = 64;
-template <class T> __global__ void __launch_bounds__(64) k_logprobs_join(ntc_logprobs_desc d, int parts) {
-    __shared__ float list[kMostParts * 2 * NTC_MAX_TOP];
+template <class T> __global__ void __launch_bounds__(256) k_logprobs_join(ntc_logprobs_desc d, int parts) {
+    __shared__ float all[kMostParts * (4 + 2 * NTC_MAX_TOP)];
     const long long row = blockIdx.x;
     const int lane = lane_id(), size = 4 + 2 * d.top;
+    const float* from = (const float*)d.workspace + row * parts * size;
+    for (int i = threadIdx.x; i < parts * size; i += 256) all[i] = from[i];
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
     long long outer, inner;
     const T* x = row_of<T>(d, row, outer, inner);
     const float k = kLog2e / d.temperature;
-    const float* from = (const float*)d.workspace + row * parts * size;
     Soft a = { kLowest, 0.0f, 0.0f };
-    if (lane < parts) a = { from[lane * size], from[lane * size + 1], from[lane * size + 2] };
-    for (int p = 0; p < parts; p++) if (lane < 2 * d.top) list[p * 2 * d.top + lane] = from[p * size + 4 + lane];
-    __syncthreads();
+    if (lane < parts) a = { all[lane * size], all[lane * size + 1], all[lane * size + 2] };
     a = join_lanes(a, k);
     Best best;
     best.clear();
-    for (int p = 0; p < parts; p++)
-        for (int r = 0; r < d.top; r++) {
-            const float v = list[p * 2 * d.top + r];
-            const int i = __float_as_int(list[p * 2 * d.top + d.top + r]);
-            if (i == kNoIndex || !(v > read_lane(best.v, d.top - 1) || (v == read_lane(best.v, d.top - 1) && i < __builtin_amdgcn_readlane(best.i, d.top - 1)))) break;
-            best.insert(v, i);
-        }
+    if (d.top) best = merge(all + 4, (const int*)all + 4 + d.top, size, parts, d.top);
     finish(d, row, x, token_of(d, outer, inner), a, best);
 }
 
@@ -450,7 +454,6 @@ template <class T> static Reading reading(int64_t rows, int64_t V) {
     }
     return r;
 }
-constexpr int kShort = 1024;                                 // the longest row that a wave holds in registers
 
 template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s) {
     const auto blocks = [&](int per) { return (unsigned)((d.rows + per - 1) / per); };
@@ -463,7 +466,7 @@ template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s
     else if (r.parts == 1) k_logprobs_long<T, 4, false><<<blocks(1), 256, 0, s>>>(d, lim, 0);
     else {
         k_logprobs_long<T, 4, true><<<dim3((unsigned)d.rows, r.parts), 256, 0, s>>>(d, lim, r.part_chunks);
-        k_logprobs_join<T><<<(unsigned)d.rows, 64, 0, s>>>(d, r.parts);
+        k_logprobs_join<T><<<(unsigned)d.rows, 256, 0, s>>>(d, r.parts);
     }
 }
 template <class T> static size_t workspace(int64_t rows, int64_t V, int top) {
