@@ -6,6 +6,7 @@
 namespace ntc_ops {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ float power_of(int b) { return __uint_as_float(b > 0 ? (uint32_t)b << 23 : 1u << 22); }   // 2^(b - 127), b from 0 to 254
@@ -101,8 +102,7 @@ template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_qua
         uint32_t b = 0;
 #pragma unroll
         for (int i = 0; i < 8; i++) b = Mag::join(b, Mag::of(x[i]));
-#pragma unroll
-        for (int w = 1; w < 64; w <<= 1) b = Mag::join(b, __shfl_xor(b, w));
+        b = reduce64(b, Mag::join);
         if ((threadIdx.x & 63) == 0) most[wave][0] = b;
         __syncthreads();
         b = Mag::join(Mag::join(most[0][0], most[1][0]), Mag::join(most[2][0], most[3][0]));
@@ -119,8 +119,7 @@ template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_qua
             int byte = block_byte;
             if (!kBlock) {
                 uint32_t b = Mag::of(x[i]);
-#pragma unroll
-                for (int w = 1; w < 16; w <<= 1) b = Mag::join(b, __shfl_xor(b, w));
+                b = reduce16(b, Mag::join);
                 byte = exp_byte(Mag::float_bits(b));
                 if (cg == 0 && 8 * rg + i < rows) put_exp(d.exps + (r0 + 8 * rg + i) * exp_stride, blockIdx.x, byte, last_c, exp_stride);
             }
@@ -138,8 +137,7 @@ template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_qua
             uint32_t b = 0;
 #pragma unroll
             for (int i = 0; i < 8; i++) b = max_word(b, Mag::one(x[i].v[j]));
-            b = max_word(b, __shfl_xor(b, 16));
-            b = max_word(b, __shfl_xor(b, 32));
+            b = reduce_rows(b, max_word);
             if ((threadIdx.x & 48) == 0) most[wave][8 * cg + j] = b;
         }
         __syncthreads();
@@ -397,6 +395,106 @@ template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds_
     else store(std::true_type());
 }
 
+// Few rows of A: bound by the bytes of B. A block takes 16 rows of B, its waves a share of the columns each, straight from memory into the
+// operands' registers (v_mfma_scale_f32_16x16x128: lane l holds 32 bytes of row l % 16 at k = 32 (l / 16); result i is (first operand's row
+// 4 (l / 16) + i, second's row l % 16)), and the waves' sums are added in LDS, in order. A's rows are kM tiles of 16 (past the end the last row
+// again); floats are taken to 8 bits here, each wave what it needs, which saves a launch: a row's block is 32 values in each of 4 lanes.
+struct FewArgs {
+    const void* a;
+    const uint8_t *ae, *b, *be;
+    void* c;
+    long long N, a_stride, ldc;
+    int M, K, blocks, stride, estride, a_shift, b_shift;
+};
+template <class A> __device__ __forceinline__ v8i to_codes(const Run<A, 8> (&x)[4], int& byte) {
+    using Mag = Magnitude<A>;
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) m = Mag::join(m, Mag::of(x[i]));
+    byte = exp_byte(reduce_rows(Mag::float_bits(m), [](uint32_t p, uint32_t q) { return p > q ? p : q; }));
+    const float s = power_of(254 - byte);
+    v8i r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        r[2 * i] = (int)to_fp8x4((float)x[i].v[0] * s, (float)x[i].v[1] * s, (float)x[i].v[2] * s, (float)x[i].v[3] * s);
+        r[2 * i + 1] = (int)to_fp8x4((float)x[i].v[4] * s, (float)x[i].v[5] * s, (float)x[i].v[6] * s, (float)x[i].v[7] * s);
+    }
+    return r;
+}
+constexpr int kFewWaves = 8;
+template <class A, int kM, class C> __global__ void __launch_bounds__(64 * kFewWaves) k_fp8_few(FewArgs d) {
+    constexpr bool kFp8 = std::is_same_v<A, uint8_t>;
+    constexpr int kAhead = kM == 1 ? (sizeof(A) == 4 ? 2 : 4) : kM == 2 && sizeof(A) < 4 ? 2 : 1;    // blocks of columns in flight: as many as the registers hold
+    __shared__ float sums[kFewWaves][kM][16][17];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const long long n0 = (long long)blockIdx.x * 16, n = n0 + r < d.N ? n0 + r : d.N - 1;
+    const uint8_t* b = d.b + n * d.stride + 32 * g;
+    const uint8_t* be = d.be + (n >> d.b_shift) * d.estride;
+    const A* a[kM];
+    const uint8_t* ae[kM];
+#pragma unroll
+    for (int i = 0; i < kM; i++) {
+        const int m = 16 * i + r < d.M ? 16 * i + r : d.M - 1;
+        a[i] = (const A*)d.a + (long long)m * (kFp8 ? d.stride : d.a_stride) + 32 * g;
+        ae[i] = kFp8 ? d.ae + (long long)(m >> d.a_shift) * d.estride : nullptr;
+    }
+    v4f acc[kM] = {};
+    for (int k0 = wave; k0 < d.blocks; k0 += kFewWaves * kAhead) {
+        v8i w[kAhead];
+        int we[kAhead];
+        std::conditional_t<kFp8, v8i, Run<A, 8>[4]> x[kAhead][kM];
+        int xe[kAhead][kM];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            const int k = k0 + kFewWaves * u;
+            if (k >= d.blocks) break;
+            const uint4 p = *(const uint4*)(b + 128ll * k), q = *(const uint4*)(b + 128ll * k + 16);
+            w[u] = v8i{ (int)p.x, (int)p.y, (int)p.z, (int)p.w, (int)q.x, (int)q.y, (int)q.z, (int)q.w };
+            we[u] = be[k];
+#pragma unroll
+            for (int i = 0; i < kM; i++) {
+                if constexpr (kFp8) {
+                    const uint4 s = *(const uint4*)(a[i] + 128ll * k), t = *(const uint4*)(a[i] + 128ll * k + 16);
+                    x[u][i] = v8i{ (int)s.x, (int)s.y, (int)s.z, (int)s.w, (int)t.x, (int)t.y, (int)t.z, (int)t.w };
+                    xe[u][i] = ae[i][k];
+                } else {
+                    const int left = d.K - 128 * k - 32 * g;   // values of this lane's 32 that are there
+                    const A* from = a[i] + 128ll * k;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (8 * j + 8 <= left) { const auto v = *(const LooseRun<A, 8>*)(from + 8 * j); for (int e = 0; e < 8; e++) x[u][i][j].v[e] = v.v[e]; }
+                        else for (int e = 0; e < 8; e++) x[u][i][j].v[e] = 8 * j + e < left ? from[8 * j + e] : (A)0.0f;
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            if (k0 + kFewWaves * u >= d.blocks) break;
+#pragma unroll
+            for (int i = 0; i < kM; i++) {
+                v8i code;
+                if constexpr (kFp8) code = x[u][i];
+                else code = to_codes<A>(x[u][i], xe[u][i]);
+                acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[u], code, acc[i], 0, 0, 0, we[u], 0, xe[u][i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kM; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) sums[wave][i][r][4 * g + j] = acc[i][j];
+    __syncthreads();
+    for (int at = threadIdx.x; at < kM * 256; at += 64 * kFewWaves) {
+        const int m = at >> 4, c = at & 15;
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kFewWaves; w++) s += sums[w][m >> 4][m & 15][c];
+        if (m < d.M && n0 + c < d.N) ((C*)d.c)[m * d.ldc + n0 + c] = (C)s;
+    }
+}
+constexpr int kFewRows = 64;
+
 // The parts of a split sum, added in order.
 template <class C> __global__ void __launch_bounds__(256) k_fp8_join(const float* parts, int n_parts, long long M, long long N, long long ldc, C* c) {
     const long long i = ((long long)blockIdx.x * 256 + threadIdx.x), size = M * N;
@@ -444,11 +542,26 @@ extern "C" int ntc_op_fp8_quantize(const ntc_fp8_quantize_desc* d, void* stream,
 }
 
 extern "C" size_t ntc_op_fp8_matmul_workspace(int64_t M, int64_t N, int64_t K, int32_t) {
-    if (M < 1 || N < 1 || K < 1) return 0;
+    if (M <= kFewRows || N < 1 || K < 1) return 0;
     const Plan p = plan_of(M, N, K);
     return p.parts > 1 ? (size_t)p.parts * M * N * 4 : 0;
 }
-extern "C" int64_t ntc_op_fp8_matmul_float_rows(void) { return 0; }
+extern "C" int64_t ntc_op_fp8_matmul_float_rows(void) { return kFewRows; }
+
+template <class A, class C> static void launch_few(const FewArgs& F, hipStream_t s) {
+    const unsigned blocks = (unsigned)((F.N + 15) / 16);
+    if (F.M <= 16) k_fp8_few<A, 1, C><<<blocks, 64 * kFewWaves, 0, s>>>(F);
+    else if (F.M <= 32) k_fp8_few<A, 2, C><<<blocks, 64 * kFewWaves, 0, s>>>(F);
+    else k_fp8_few<A, 4, C><<<blocks, 64 * kFewWaves, 0, s>>>(F);
+}
+template <class C> static void run_few(const ntc_fp8_matmul_desc* d, hipStream_t s) {
+    const FewArgs F = { d->a, d->a_exps, d->b, d->b_exps, d->c, d->N, d->a_stride, d->ldc, (int)d->M, (int)d->K, (int)((d->K + 127) / 128), (int)ntc_fp8_code_stride(d->K),
+                        (int)ntc_fp8_exp_stride(d->K), d->a_block_rows == 128 ? 7 : 0, d->b_block_rows == 128 ? 7 : 0 };
+    if (d->a_type == NTC_FP8) launch_few<uint8_t, C>(F, s);
+    else if (d->a_type == NTC_F32) launch_few<f32, C>(F, s);
+    else if (d->a_type == NTC_BF16) launch_few<bf16, C>(F, s);
+    else launch_few<f16, C>(F, s);
+}
 
 template <int T, class C> static void launch_matmul(const MatmulArgs& A, int parts, hipStream_t s) {
     const unsigned tiles = (unsigned)(A.tiles_m * A.tiles_n);
@@ -483,7 +596,9 @@ template <class C> static void run_matmul(const ntc_fp8_matmul_desc* d, hipStrea
 extern "C" int ntc_op_fp8_matmul(const ntc_fp8_matmul_desc* d, void* stream, char* why, size_t cap) {
     if (!d) return refuse(why, cap, "no description");
     if (d->M < 0 || d->N < 0 || d->K < 0) return refuse(why, cap, "sizes are not negative");
-    if (d->a_type != NTC_FP8) return refuse(why, cap, "A is a matrix in 8 bits");
+    if (d->a_type < 0 || d->a_type > NTC_FP8) return refuse(why, cap, "A is 8-bit codes, or 32-bit floats, bfloat16 or float16");
+    if (d->a_type != NTC_FP8 && d->M > kFewRows) return refuse(why, cap, "A of more than 64 rows is given in 8 bits");
+    if (d->a_type != NTC_FP8 && d->a_stride < 0) return refuse(why, cap, "strides are not negative");
     if (d->c_type < 0 || d->c_type > 2) return refuse(why, cap, "C is 32-bit floats, bfloat16 or float16");
     if ((d->a_block_rows != 1 && d->a_block_rows != 128) || (d->b_block_rows != 1 && d->b_block_rows != 128)) return refuse(why, cap, "blocks are 1 x 128 or 128 x 128");
     if (d->ldc < d->N) return refuse(why, cap, "C's rows overlap");
@@ -491,10 +606,16 @@ extern "C" int ntc_op_fp8_matmul(const ntc_fp8_matmul_desc* d, void* stream, cha
         return refuse(why, cap, "K at most 2^23, and fewer than 2^31 tiles of 128 x 128");
     if (!d->M || !d->N) return 0;
     if (!d->K) return refuse(why, cap, "K is at least 1");
-    if (!d->c || !d->a || !d->a_exps || !d->b || !d->b_exps) return refuse(why, cap, "a null pointer");
-    if ((((uintptr_t)d->a | (uintptr_t)d->b) & 15) || (((uintptr_t)d->a_exps | (uintptr_t)d->b_exps) & 3)) return refuse(why, cap, "codes start at multiples of 16 bytes, exponents of 4");
+    const bool codes = d->a_type == NTC_FP8;
+    if (!d->c || !d->a || (codes && !d->a_exps) || !d->b || !d->b_exps) return refuse(why, cap, "a null pointer");
+    if ((((codes ? (uintptr_t)d->a : 0) | (uintptr_t)d->b) & 15) || (((codes ? (uintptr_t)d->a_exps : 0) | (uintptr_t)d->b_exps) & 3))
+        return refuse(why, cap, "codes start at multiples of 16 bytes, exponents of 4");
     if (!d->workspace && ntc_op_fp8_matmul_workspace(d->M, d->N, d->K, d->a_type)) return refuse(why, cap, "a null workspace");
     const hipStream_t s = (hipStream_t)stream;
+    if (d->M <= kFewRows) {
+        d->c_type == NTC_F32 ? run_few<f32>(d, s) : d->c_type == NTC_BF16 ? run_few<bf16>(d, s) : run_few<f16>(d, s);
+        return launched(why, cap);
+    }
     d->c_type == NTC_F32 ? run_matmul<f32>(d, s) : d->c_type == NTC_BF16 ? run_matmul<bf16>(d, s) : run_matmul<f16>(d, s);
     return launched(why, cap);
 }
