@@ -37,7 +37,7 @@ template <class T> struct Magnitude {                       // bf16 and f16
         const uint4 w = __builtin_bit_cast(uint4, x);
         const uint32_t v[4] = { w.x & 0x7fff7fffu, w.y & 0x7fff7fffu, w.z & 0x7fff7fffu, w.w & 0x7fff7fffu };
         uint32_t m = max_pair(max_pair(v[0], v[1]), max_pair(v[2], v[3]));
-        if (max_word(m & 0xffffu, m >> 16) >= kInf) {
+        if (__builtin_expect(__ballot(max_word(m & 0xffffu, m >> 16) >= kInf) != 0, 0)) {   // (a branch of the whole wave: else it would be computed always)
             m = 0;
             for (int i = 0; i < 4; i++) m = max_pair(m, ((v[i] & 0xffffu) >= kInf ? 0u : v[i] & 0xffffu) | (v[i] >> 16 >= kInf ? 0u : v[i] & 0xffff0000u));
         }
@@ -84,11 +84,28 @@ template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_qua
 #pragma unroll
         for (int i = 0; i < 8; i++) { const auto v = *(const LooseRun<T, 8>*)(from + i * d.row_stride); for (int j = 0; j < 8; j++) x[i].v[j] = v.v[j]; }
     } else {
+        // at the edges what is past them reads the last row or column instead (no branch between the loads) and counts as 0
+        const T* const tile0 = (const T*)d.x + r0 * d.row_stride + c0;
+        if (8 * cg + 8 <= cols) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (8 * rg + i < rows && 8 * cg + 8 <= cols) { const auto v = *(const LooseRun<T, 8>*)(from + i * d.row_stride); for (int j = 0; j < 8; j++) x[i].v[j] = v.v[j]; }
-            else for (int j = 0; j < 8; j++) x[i].v[j] = 8 * rg + i < rows && 8 * cg + j < cols ? from[i * d.row_stride + j] : (T)0.0f;
+            for (int i = 0; i < 8; i++) {
+                const int r = 8 * rg + i < rows ? 8 * rg + i : rows - 1;
+                const auto v = *(const LooseRun<T, 8>*)(tile0 + r * d.row_stride + 8 * cg);
+                for (int j = 0; j < 8; j++) x[i].v[j] = v.v[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int r = 8 * rg + i < rows ? 8 * rg + i : rows - 1, c = 8 * cg + j < cols ? 8 * cg + j : cols - 1;
+                    x[i].v[j] = tile0[r * d.row_stride + c];
+                }
         }
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[i].v[j] = 8 * rg + i < rows && 8 * cg + j < cols ? x[i].v[j] : (T)0.0f;
     }
     const long long code_stride = ntc_fp8_code_stride(d.K), exp_stride = ntc_fp8_exp_stride(d.K), code_stride_t = ntc_fp8_code_stride(d.R), exp_stride_t = ntc_fp8_exp_stride(d.R);
     // a row of exponents is written by the tile that has its block; the last one also clears what follows
@@ -444,13 +461,11 @@ template <class A, int kM, class C> __global__ void __launch_bounds__(64 * kFewW
         int we[kAhead];
         std::conditional_t<kFp8, v8i, Run<A, 8>[4]> x[kAhead][kM];
         int xe[kAhead][kM];
+        // A's first, so that they are converted while B's are on the way
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
             const int k = k0 + kFewWaves * u;
             if (k >= d.blocks) break;
-            const uint4 p = *(const uint4*)(b + 128ll * k), q = *(const uint4*)(b + 128ll * k + 16);
-            w[u] = v8i{ (int)p.x, (int)p.y, (int)p.z, (int)p.w, (int)q.x, (int)q.y, (int)q.z, (int)q.w };
-            we[u] = be[k];
 #pragma unroll
             for (int i = 0; i < kM; i++) {
                 if constexpr (kFp8) {
@@ -460,13 +475,23 @@ template <class A, int kM, class C> __global__ void __launch_bounds__(64 * kFewW
                 } else {
                     const int left = d.K - 128 * k - 32 * g;   // values of this lane's 32 that are there
                     const A* from = a[i] + 128ll * k;
+                    if (128 * k + 128 <= d.K) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if (8 * j + 8 <= left) { const auto v = *(const LooseRun<A, 8>*)(from + 8 * j); for (int e = 0; e < 8; e++) x[u][i][j].v[e] = v.v[e]; }
-                        else for (int e = 0; e < 8; e++) x[u][i][j].v[e] = 8 * j + e < left ? from[8 * j + e] : (A)0.0f;
+                        for (int j = 0; j < 4; j++) { const auto v = *(const LooseRun<A, 8>*)(from + 8 * j); for (int e = 0; e < 8; e++) x[u][i][j].v[e] = v.v[e]; }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) for (int e = 0; e < 8; e++) x[u][i][j].v[e] = 8 * j + e < left ? from[8 * j + e] : (A)0.0f;
                     }
                 }
             }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            const int k = k0 + kFewWaves * u;
+            if (k >= d.blocks) break;
+            const uint4 p = *(const uint4*)(b + 128ll * k), q = *(const uint4*)(b + 128ll * k + 16);
+            w[u] = v8i{ (int)p.x, (int)p.y, (int)p.z, (int)p.w, (int)q.x, (int)q.y, (int)q.z, (int)q.w };
+            we[u] = be[k];
         }
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
@@ -495,16 +520,38 @@ template <class A, int kM, class C> __global__ void __launch_bounds__(64 * kFewW
 }
 constexpr int kFewRows = 64;
 
-// The parts of a split sum, added in order.
-template <class C> __global__ void __launch_bounds__(256) k_fp8_join(const float* parts, int n_parts, long long M, long long N, long long ldc, C* c) {
-    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x), size = M * N;
-    if (i >= size) return;
-    float s = 0.0f;
-    for (int p = 0; p < n_parts; p++) s += parts[p * size + i];
-    c[i / N * ldc + i % N] = (C)s;
+// The parts of a split sum, added in a fixed order: a block takes 256 results, four a lane, each of its four waves every fourth part.
+template <class C> __global__ void __launch_bounds__(256) k_fp8_join(const float* parts, int n_parts, long long size, long long N, long long ldc, C* c) {
+    __shared__ float4 sums[3][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long at = ((long long)blockIdx.x * 64 + lane) * 4;
+    float4 s = { 0, 0, 0, 0 };
+    if (at + 4 <= size) {
+#pragma unroll 8
+        for (int p = wave; p < n_parts; p += 4) {
+            const auto v = *(const LooseRun<float, 4>*)(parts + p * size + at);
+            s.x += v.v[0]; s.y += v.v[1]; s.z += v.v[2]; s.w += v.v[3];
+        }
+    } else if (at < size) {
+        for (int p = wave; p < n_parts; p += 4) {
+            const float* v = parts + p * size + at;
+            s.x += v[0];
+            if (at + 1 < size) s.y += v[1];
+            if (at + 2 < size) s.z += v[2];
+        }
+    }
+    if (wave) sums[wave - 1][lane] = s;
+    __syncthreads();
+    if (wave) return;
+    for (int w = 0; w < 3; w++) { const float4 o = sums[w][lane]; s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w; }
+    Run<C, 4> o;
+    o.v[0] = (C)s.x; o.v[1] = (C)s.y; o.v[2] = (C)s.z; o.v[3] = (C)s.w;
+    if (ldc == N && at + 4 <= size) { *(LooseRun<C, 4>*)(c + at) = *(const LooseRun<C, 4>*)&o; return; }
+    for (int k = 0; k < 4; k++) if (at + k < size) c[(at + k) / N * ldc + (at + k) % N] = o.v[k];
 }
 
-// How a product is divided.
+// How a product is divided: tiles of 256 x 256 where they fill the chip (256 CUs, one each), else of 128 x 128 (two to a CU); and the sum into parts
+// of at least 8 blocks of columns where even those leave CUs idle.
 struct Plan { int tile, parts, split_blocks; };
 static Plan plan_of(int64_t M, int64_t N, int64_t K) {
     const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
@@ -512,9 +559,9 @@ static Plan plan_of(int64_t M, int64_t N, int64_t K) {
     Plan p = { 256, 1, (int)blocks };
     if (up(M, 256) * up(N, 256) < 200) p.tile = 128;
     const int64_t tiles = up(M, p.tile) * up(N, p.tile);
-    if (p.tile == 128 && tiles < 256 && blocks > 8) {
-        int64_t parts = up(512, tiles);
-        if (parts > blocks / 4) parts = blocks / 4;
+    if (p.tile == 128 && tiles <= 128 && blocks >= 16) {
+        int64_t parts = 256 / tiles;
+        if (parts > blocks / 8) parts = blocks / 8;
         p.split_blocks = (int)(up(up(blocks, parts), 4) * 4);
         p.parts = (int)up(blocks, p.split_blocks);
     }
@@ -590,7 +637,7 @@ template <class C> static void run_matmul(const ntc_fp8_matmul_desc* d, hipStrea
     A.ldc = p.parts > 1 ? d->N : d->ldc;
     if (p.tile == 256) launch_matmul<256, C>(A, p.parts, s);
     else launch_matmul<128, C>(A, p.parts, s);
-    if (p.parts > 1) k_fp8_join<C><<<(unsigned)((d->M * d->N + 255) / 256), 256, 0, s>>>((const float*)d->workspace, p.parts, d->M, d->N, d->ldc, (C*)d->c);
+    if (p.parts > 1) k_fp8_join<C><<<(unsigned)((d->M * d->N + 255) / 256), 256, 0, s>>>((const float*)d->workspace, p.parts, d->M * d->N, d->N, d->ldc, (C*)d->c);
 }
 
 extern "C" int ntc_op_fp8_matmul(const ntc_fp8_matmul_desc* d, void* stream, char* why, size_t cap) {
