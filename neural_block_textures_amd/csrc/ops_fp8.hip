@@ -47,11 +47,31 @@ template <class T> struct Magnitude {                       // bf16 and f16
         const uint16_t h = (uint16_t)max_word(m & 0xffffu, m >> 16);
         return __float_as_uint((float)__builtin_bit_cast(T, h));
     }
-    // of one value
-    static __device__ __forceinline__ uint32_t one(T x) {
-        const uint32_t a = __builtin_bit_cast(uint16_t, x) & 0x7fffu;
-        return a >= kInf ? 0u : a;
+    // of eight columns over eight rows, two columns to a word; and the float bits of column j of them
+    static constexpr int kWords = 4;
+    static __device__ __forceinline__ void columns(const Run<T, 8> (&x)[8], uint32_t (&m)[kWords]) {
+        uint32_t w[8][4], any = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint4 v = __builtin_bit_cast(uint4, x[i]);
+            w[i][0] = v.x & 0x7fff7fffu; w[i][1] = v.y & 0x7fff7fffu; w[i][2] = v.z & 0x7fff7fffu; w[i][3] = v.w & 0x7fff7fffu;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            m[q] = w[0][q];
+#pragma unroll
+            for (int i = 1; i < 8; i++) m[q] = max_pair(m[q], w[i][q]);
+            any = max_pair(any, m[q]);
+        }
+        if (__builtin_expect(__ballot(max_word(any & 0xffffu, any >> 16) >= kInf) != 0, 0)) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                m[q] = 0;
+                for (int i = 0; i < 8; i++) m[q] = max_pair(m[q], ((w[i][q] & 0xffffu) >= kInf ? 0u : w[i][q] & 0xffffu) | (w[i][q] >> 16 >= kInf ? 0u : w[i][q] & 0xffff0000u));
+            }
+        }
     }
+    static __device__ __forceinline__ uint32_t column_bits(const uint32_t (&m)[kWords], int j) { return float_bits(j & 1 ? m[j >> 1] >> 16 : m[j >> 1] & 0xffffu); }
 };
 template <> struct Magnitude<f32> {
     static __device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b) { return max_word(a, b); }
@@ -65,6 +85,15 @@ template <> struct Magnitude<f32> {
         return m;
     }
     static __device__ __forceinline__ uint32_t float_bits(uint32_t m) { return m; }
+    static constexpr int kWords = 8;
+    static __device__ __forceinline__ void columns(const Run<float, 8> (&x)[8], uint32_t (&m)[kWords]) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            m[j] = 0;
+            for (int i = 0; i < 8; i++) m[j] = max_word(m[j], one(x[i].v[j]));
+        }
+    }
+    static __device__ __forceinline__ uint32_t column_bits(const uint32_t (&m)[kWords], int j) { return m[j]; }
 };
 
 // ---------------------------------------------------------------- to 8 bits
@@ -73,7 +102,7 @@ template <> struct Magnitude<f32> {
 // read once for both orders. Bound by memory.
 template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_quantize(ntc_fp8_quantize_desc d) {
     using Mag = Magnitude<T>;
-    __shared__ uint32_t most[4][128];
+    __shared__ alignas(16) uint32_t most[4][16 * Mag::kWords];
     __shared__ alignas(16) uint8_t tile[128 * 128];        // transposed; word w of 8 rows of column c at w ^ (c / 8)
     const long long r0 = (long long)blockIdx.y * 128, c0 = (long long)blockIdx.x * 128;
     const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4, wave = threadIdx.x >> 6;
@@ -84,28 +113,28 @@ template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_qua
 #pragma unroll
         for (int i = 0; i < 8; i++) { const auto v = *(const LooseRun<T, 8>*)(from + i * d.row_stride); for (int j = 0; j < 8; j++) x[i].v[j] = v.v[j]; }
     } else {
-        // at the edges what is past them reads the last row or column instead (no branch between the loads) and counts as 0
+        // At the edges what is past them counts as 0; rows past the end read the last one instead, so that no branch is between the loads.
         const T* const tile0 = (const T*)d.x + r0 * d.row_stride + c0;
-        if (8 * cg + 8 <= cols) {
+        const int left = cols - 8 * cg;                     // of this lane's eight columns
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = Run<T, 8>{};
+        if (left >= 8) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const int r = 8 * rg + i < rows ? 8 * rg + i : rows - 1;
-                const auto v = *(const LooseRun<T, 8>*)(tile0 + r * d.row_stride + 8 * cg);
+                const auto v = *(const LooseRun<T, 8>*)(tile0 + (8 * rg + i < rows ? 8 * rg + i : rows - 1) * d.row_stride + 8 * cg);
                 for (int j = 0; j < 8; j++) x[i].v[j] = v.v[j];
             }
-        } else {
+        } else if (left > 0) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const int r = 8 * rg + i < rows ? 8 * rg + i : rows - 1, c = 8 * cg + j < cols ? 8 * cg + j : cols - 1;
-                    x[i].v[j] = tile0[r * d.row_stride + c];
+                    const T v = tile0[(8 * rg + i < rows ? 8 * rg + i : rows - 1) * d.row_stride + 8 * cg + (j < left ? j : 0)];
+                    x[i].v[j] = j < left ? v : (T)0.0f;
                 }
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[i].v[j] = 8 * rg + i < rows && 8 * cg + j < cols ? x[i].v[j] : (T)0.0f;
+        for (int i = 0; i < 8; i++) if (8 * rg + i >= rows) x[i] = Run<T, 8>{};
     }
     const long long code_stride = ntc_fp8_code_stride(d.K), exp_stride = ntc_fp8_exp_stride(d.K), code_stride_t = ntc_fp8_code_stride(d.R), exp_stride_t = ntc_fp8_exp_stride(d.R);
     // a row of exponents is written by the tile that has its block; the last one also clears what follows
@@ -148,23 +177,26 @@ template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_qua
         }
     }
     if (!d.codes_t) return;
+    uint32_t col[Mag::kWords];
     if (!kBlock) {
+        Mag::columns(x, col);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            uint32_t b = 0;
+        for (int q = 0; q < Mag::kWords; q++) col[q] = reduce_rows(col[q], Mag::join);
+        if ((threadIdx.x & 48) == 0)
 #pragma unroll
-            for (int i = 0; i < 8; i++) b = max_word(b, Mag::one(x[i].v[j]));
-            b = reduce_rows(b, max_word);
-            if ((threadIdx.x & 48) == 0) most[wave][8 * cg + j] = b;
-        }
+            for (int q = 0; q < Mag::kWords; q++) most[wave][Mag::kWords * cg + q] = col[q];
         __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+#pragma unroll
+            for (int q = 0; q < Mag::kWords; q++) col[q] = Mag::join(col[q], most[w][Mag::kWords * cg + q]);
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         int byte = block_byte;
         if (!kBlock) {
             const int c = 8 * cg + j;
-            byte = exp_byte(Mag::float_bits(max_word(max_word(most[0][c], most[1][c]), max_word(most[2][c], most[3][c]))));
+            byte = exp_byte(Mag::column_bits(col, j));
             if (rg == 0 && c < cols) put_exp(d.exps_t + (c0 + c) * exp_stride_t, blockIdx.y, byte, last_r, exp_stride_t);
         }
         const float s = power_of(254 - byte);
