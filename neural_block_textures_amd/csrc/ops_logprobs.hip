@@ -62,12 +62,21 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 __device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 
+__device__ __forceinline__ uint32_t above(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t below(uint32_t a, uint32_t b) { return a < b ? a : b; }
+// A lane's three largest keys, in order (0: none).
+struct Three {
+    uint32_t a, b, c;
+    __device__ __forceinline__ static uint32_t middle(uint32_t x, uint32_t y, uint32_t z) { return above(below(x, y), below(above(x, y), z)); }   // one instruction
+    __device__ __forceinline__ void add(uint32_t k) { c = middle(b, c, k); b = middle(a, b, k); a = above(a, k); }
+};
+
 // A group of kGroup lanes holds a row in registers, kEach neighbouring values a lane: the largest, then the sums, then the alternatives one by
-// one, each the largest key below the last. A 16-bit type's float has 13 low bits to spare, which take the index (of a row of at most
+// one, from the lanes' three largest. A 16-bit type's float has 13 low bits to spare, which take the index (of a row of at most
 // 1024, from the top down): one word orders values and indices both. A 32-bit value's index is found in a second reduction.
 // Bound by instructions: 262144 rows of 256 bf16 values with 4 alternatives take twice what their bytes do.
 constexpr int kShort = 1024;                                 // the longest such row
-template <class T, int kGroup, int kEach> __global__ void __launch_bounds__(256) k_logprobs_short(ntc_logprobs_desc d) {
+template <class T, int kGroup, int kEach> __global__ void __launch_bounds__(256) k_logprobs_short(ntc_logprobs_desc d, float lim) {
     constexpr int kVec = 16 / (int)sizeof(T) < kEach ? 16 / (int)sizeof(T) : kEach;
     constexpr uint32_t kMask = ~0x1fffu;
     static_assert(kGroup * kEach <= kShort, "indices of 10 bits");
@@ -92,11 +101,24 @@ template <class T, int kGroup, int kEach> __global__ void __launch_bounds__(256)
     m = reduce<kGroup>(m, larger);
     const float mm = m == -NTC_INF ? 0.0f : m;              // nothing left: every exponential is 0
     float s = 0.0f, t = 0.0f;
+    if (__ballot(!(fabsf(mm) <= lim)) == 0) {               // on products, which do not overflow here: one operation fewer a value
+        const float mk = mm * k, off = __builtin_fmaf(mm, k, -mk);   // (the exponents are this much too large)
 #pragma unroll
-    for (int j = 0; j < kEach; j++) {
-        const float q = (v[j] - mm) * k, e = fast_exp2(q);
-        s += e;
-        t = __builtin_fmaf(e, fmaxf(q, -1e30f), t);
+        for (int j = 0; j < kEach; j++) {
+            const float q = __builtin_fmaf(v[j], k, -mk), e = fast_exp2(q);
+            s += e;
+            t = __builtin_fmaf(e, fmaxf(q, -1e30f), t);
+        }
+        const float f = fast_exp2(-off);
+        t = f * __builtin_fmaf(-s, off, t);
+        s *= f;
+    } else {
+#pragma unroll
+        for (int j = 0; j < kEach; j++) {
+            const float q = (v[j] - mm) * k, e = fast_exp2(q);
+            s += e;
+            t = __builtin_fmaf(e, fmaxf(q, -1e30f), t);
+        }
     }
     s = reduce<kGroup>(s, sum);
     t = reduce<kGroup>(t, sum);
@@ -112,32 +134,40 @@ template <class T, int kGroup, int kEach> __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int j = 0; j < kEach; j++) {
         key[j] = order_key(v[j]);
-        if constexpr (sizeof(T) == 2) key[j] = (key[j] & kMask) | (uint32_t)(kShort - 1 - at - j);
+        if constexpr (sizeof(T) == 2) key[j] = ((key[j] & kMask) | (uint32_t)(kShort - 1 - at)) - j;   // (at is a multiple of kEach: no borrow)
     }
     if (V < kGroup * kEach) {
+        asm volatile("");                                    // (a branch, not selections that every row would make)
 #pragma unroll
         for (int j = 0; j < kEach; j++) key[j] = at + j < V ? key[j] : 0;   // below every key of a value
     }
-    const auto above = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
-    const auto below = [](uint32_t a, uint32_t b) { return a < b ? a : b; };
     uint32_t mine = 0, mine_at = 0, last = 0, last_at = 0;
-    for (int r = 0; r < d.top; r++) {
-        uint32_t best = 0;
-        if constexpr (sizeof(T) == 2) {
-            // the largest below the last: key - last wraps to the top of the range for just those
+    Three best = { 0, 0, 0 };
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-            for (int j = 0; j < kEach; j++) best = above(best, key[j] - last);
-            last = reduce<kGroup>(best, above) + last;
+        for (int j = 0; j < kEach; j++) best.add(key[j]);
+    }
+    for (int r = 0; r < d.top; r++) {
+        if constexpr (sizeof(T) == 2) {
+            last = reduce<kGroup>(best.a, above);
+            const bool took = best.a == last;
+            best = { took ? best.b : best.a, took ? best.c : best.b, took ? 0 : best.c };
+            if (__ballot(took && best.a == 0 && r + 1 < d.top)) {   // a lane has given its three: again from those below the last
+                asm volatile("");
+                best = { 0, 0, 0 };
+#pragma unroll
+                for (int j = 0; j < kEach; j++) best.add(key[j] < last ? key[j] : 0);
+            }
         } else {
             // open are those below the last, and those equal to it past its index; ascending j: the first of equals stays
-            uint32_t place = 0xffffffffu;
+            uint32_t high = 0, place = 0xffffffffu;
 #pragma unroll
             for (int j = 0; j < kEach; j++) {
                 const bool open = r == 0 || key[j] < last || (key[j] == last && (uint32_t)(at + j) > last_at);
-                if (open && at + j < V && (key[j] > best || place == 0xffffffffu)) { best = key[j]; place = (uint32_t)(at + j); }
+                if (open && at + j < V && (key[j] > high || place == 0xffffffffu)) { high = key[j]; place = (uint32_t)(at + j); }
             }
-            last = reduce<kGroup>(place == 0xffffffffu ? 0u : best, above);
-            last_at = reduce<kGroup>(best == last ? place : 0xffffffffu, below);
+            last = reduce<kGroup>(place == 0xffffffffu ? 0u : high, above);
+            last_at = reduce<kGroup>(high == last ? place : 0xffffffffu, below);
         }
         if (in == r) { mine = last; mine_at = last_at; }
     }
@@ -457,11 +487,11 @@ template <class T> static Reading reading(int64_t rows, int64_t V) {
 
 template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s) {
     const auto blocks = [&](int per) { return (unsigned)((d.rows + per - 1) / per); };
-    if (d.V <= 64 && d.top <= 16) { k_logprobs_short<T, 16, 4><<<blocks(16), 256, 0, s>>>(d); return; }
-    if (d.V <= 256 && d.top <= 16) { k_logprobs_short<T, 16, 16><<<blocks(16), 256, 0, s>>>(d); return; }
-    if (d.V <= kShort) { k_logprobs_short<T, 64, 16><<<blocks(4), 256, 0, s>>>(d); return; }
+    const float k = kLog2e / d.temperature, lim = 1e30f / (k > 1.0f ? k : 1.0f);   // values up to lim times k stay far from overflow
+    if (d.V <= 64 && d.top <= 16) { k_logprobs_short<T, 16, 4><<<blocks(16), 256, 0, s>>>(d, lim); return; }
+    if (d.V <= 256 && d.top <= 16) { k_logprobs_short<T, 16, 16><<<blocks(16), 256, 0, s>>>(d, lim); return; }
+    if (d.V <= kShort) { k_logprobs_short<T, 64, 16><<<blocks(4), 256, 0, s>>>(d, lim); return; }
     const Reading r = reading<T>(d.rows, d.V);
-    const float k = kLog2e / d.temperature, lim = 1e30f / (k > 1.0f ? k : 1.0f);
     if (r.waves == 1) k_logprobs_long<T, 1, false><<<blocks(4), 256, 0, s>>>(d, lim, 0);
     else if (r.parts == 1) k_logprobs_long<T, 4, false><<<blocks(1), 256, 0, s>>>(d, lim, 0);
     else {
