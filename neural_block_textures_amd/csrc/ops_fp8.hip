@@ -220,7 +220,7 @@ template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_qua
 // here, so that four of a lane's results are neighbours in C's row.
 //
 // A block of four waves makes a TM x TN tile of C, a quarter each. The tiles of A and B come 64 columns at a time straight
-// into LDS (a stage; four of them in turn), two stages ahead of the registers that the products are fed from, which are themselves
+// into LDS (a stage; kStages of them in turn), stages ahead of the registers that the products are fed from, which are themselves
 // one stage ahead of the products: one barrier a stage, and no product waits for a load of its own stage. In LDS a row is 64 bytes, and the 16-byte
 // piece c of row r lies at c ^ swizzle(r), which spreads any 8 or 16 rows' pieces over all banks.
 constexpr int kStages = 4;
@@ -234,6 +234,12 @@ __device__ __forceinline__ void to_lds16(uint32_t to, uint32_t off, const uint8_
 }
 __device__ __forceinline__ void to_lds4(uint32_t to, uint32_t off, const uint8_t* base) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(to), "v"(off), "s"(base) : "memory");
+}
+
+// until at most n of the wave's loads are on their way
+template <int n> __device__ __forceinline__ void wait_loads() {
+    static_assert(n < 64, "the counter has 6 bits");
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (n & 15) | ((n >> 4) << 14));
 }
 
 struct MatmulArgs {
@@ -253,19 +259,17 @@ template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds_
     constexpr int kStage = (TM + TN) * 64;
     __shared__ alignas(16) uint8_t lds[kStages * kStage + 2 * 4 * (TM + TN)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // Blocks are dealt to the 8 XCDs in turn, each with an L2 of its own: every XCD takes a run of tiles, which it walks in
-    // columns of up to 8 rows, so that neighbours share their operands there.
-    int tile = blockIdx.x;
-    const int tiles = d.tiles_m * d.tiles_n;
-    {
-        const int each = tiles / 8, rest = tiles % 8, x = tile % 8;
-        tile = x * each + (x < rest ? x : rest) + tile / 8;
-    }
+    // Blocks are dealt to the 8 XCDs in turn, each with an L2 of its own: every XCD takes a run of parts and tiles, which it walks in
+    // columns of up to 8 rows, so that neighbours share their operands there (256 x 256 x 65536 in 64 parts without it: 15.5 us, every operand read twice).
+    const int tiles = d.tiles_m * d.tiles_n, each = gridDim.x / 8, rest = gridDim.x % 8, xcd = blockIdx.x % 8;
+    int tile = xcd * each + (xcd < rest ? xcd : rest) + blockIdx.x / 8;
+    const int part = kParts ? tile / tiles : 0;
+    tile -= part * tiles;
     const int group = tile / (8 * d.tiles_n), first = group * 8, high = d.tiles_m - first < 8 ? d.tiles_m - first : 8;
     const int tm = first + (tile - group * 8 * d.tiles_n) % high, tn = (tile - group * 8 * d.tiles_n) / high;
     const long long m0 = (long long)tm * TM, n0 = (long long)tn * TN;
     const int rows_m = d.M - m0 < TM ? (int)(d.M - m0) : TM, rows_n = d.N - n0 < TN ? (int)(d.N - n0) : TN;   // rows past the end read the last one
-    const int block0 = kParts ? blockIdx.y * d.split_blocks : 0;
+    const int block0 = part * d.split_blocks;
     const int blocks = kParts && d.blocks - block0 > d.split_blocks ? d.split_blocks : d.blocks - block0;
 
     // what this lane loads: pieces of rows of A (the first TM / 64 loads of a wave) and of B
@@ -320,17 +324,17 @@ template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds_
         for (int i = 0; i < RN; i++) nb[i] = at[TM + wn + 32 * i + r32];
     };
     v16f acc[RM][RN] = {};
-    // All but the newest stage's loads have landed, in every wave; and every wave has its operands of the stage before (their products
+    // The next stage's loads have landed, in every wave (all but the newest kStages - 3 stages' have); and every wave has its operands of the stage before (their products
     // have been issued), so that the buffer they came from is free.
     const auto arrive = [&] {
         __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(0x0f70 | (kLoads & 15) | ((kLoads >> 4) << 14));
+        wait_loads<(kStages - 3) * kLoads>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
 
-    // A stage: its RM RN products and, spread evenly between them, the reads of the next stage and the loads of the third after. A wave has
+    // A stage: its RM RN products and, spread evenly between them, the reads of the next stage and the loads of the one kStages - 1 later. A wave has
     // its SIMD to itself and issues in order: what is not spread holds the products up. kByte: the block's byte of the exponents' words.
     const auto stage = [&](int s, auto set_, auto byte_, auto&& first, auto&& last) {
         constexpr int n = RM * RN, reads = 2 * (RM + RN), set = set_.value, kByte = byte_.value;
@@ -343,7 +347,7 @@ template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds_
 #pragma unroll
             for (int p = q * reads / n; p < (q + 1) * reads / n; p++) fetch(s + 1, set ^ 1, p);
 #pragma unroll
-            for (int p = q * kLoads / n; p < (q + 1) * kLoads / n; p++) load(s + 3, p);
+            for (int p = q * kLoads / n; p < (q + 1) * kLoads / n; p++) load(s + kStages - 1, p);
             if (q == n - 1) last();
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -358,9 +362,10 @@ template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds_
 
     load_exps(0);
 #pragma unroll
-    for (int i = 0; i < 3 * kLoads; i++) load(i / kLoads, i % kLoads);
-    __builtin_amdgcn_s_waitcnt(0x0f70);
-    arrive();
+    for (int i = 0; i < (kStages - 1) * kLoads; i++) load(i / kLoads, i % kLoads);
+    wait_loads<(kStages - 2) * kLoads>();                  // the exponents and stage 0
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int p = 0; p < 2 * (RM + RN); p++) fetch(0, 0, p);
     fetch_exps(0);
@@ -390,9 +395,9 @@ template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds_
 #pragma unroll
         for (int i = 0; i < RN; i++) eb[i] = (unsigned)eb[i] >> 8;
     }
-    __builtin_amdgcn_s_waitcnt(0x0f70);                    // loads past the end must not land after the block has gone
+    wait_loads<0>();                                       // loads past the end must not land after the block has gone
 
-    C* const quarter = (C*)d.c + (kParts ? (long long)blockIdx.y * d.M * d.N : 0) + (m0 + wm) * d.ldc + n0 + wn;
+    C* const quarter = (C*)d.c + (long long)part * d.M * d.N + (m0 + wm) * d.ldc + n0 + wn;
     const int left_m = rows_m - wm, left_n = rows_n - wn;
     const auto put = [&](C* to, const auto& run, int m, int n, auto guard) {
         constexpr int R = sizeof(run) / sizeof(C);
@@ -644,7 +649,7 @@ template <class C> static void run_few(const ntc_fp8_matmul_desc* d, hipStream_t
 
 template <int T, class C> static void launch_matmul(const MatmulArgs& A, int parts, hipStream_t s) {
     const unsigned tiles = (unsigned)(A.tiles_m * A.tiles_n);
-    if (parts > 1) k_fp8_matmul<T, T, float, true><<<dim3(tiles, parts), 256, 0, s>>>(A);
+    if (parts > 1) k_fp8_matmul<T, T, float, true><<<tiles * parts, 256, 0, s>>>(A);
     else k_fp8_matmul<T, T, C, false><<<tiles, 256, 0, s>>>(A);
 }
 
@@ -667,7 +672,7 @@ template <class C> static void run_matmul(const ntc_fp8_matmul_desc* d, hipStrea
     A.split_blocks = p.split_blocks;
     A.c = p.parts > 1 ? d->workspace : d->c;
     A.ldc = p.parts > 1 ? d->N : d->ldc;
-    if (p.tile == 256) launch_matmul<256, C>(A, p.parts, s);
+    if (p.tile == 256) launch_matmul<256, C>(A, 1, s);
     else launch_matmul<128, C>(A, p.parts, s);
     if (p.parts > 1) k_fp8_join<C><<<(unsigned)((d->M * d->N + 255) / 256), 256, 0, s>>>((const float*)d->workspace, p.parts, d->M * d->N, d->N, d->ldc, (C*)d->c);
 }
