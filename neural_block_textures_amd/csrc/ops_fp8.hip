@@ -253,7 +253,7 @@ struct MatmulArgs {
     int split_blocks;         // blocks of one part of the sum, a multiple of 4
 };
 
-template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) k_fp8_matmul(MatmulArgs d) {
+template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds__(256, TM > 128 ? 1 : TM > 64 ? 2 : 4) k_fp8_matmul(MatmulArgs d) {
     constexpr int RM = TM / 64, RN = TN / 64;              // 32-row tiles of a wave
     constexpr int kLoads = (TM + TN) / 64;                 // 1 KiB loads a wave and stage
     constexpr int kStage = (TM + TN) * 64;
@@ -284,9 +284,10 @@ template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds_
     }
     const uint8_t* ebase_a = d.ae + (m0 >> d.a_shift) * d.estride + block0;
     const uint8_t* ebase_b = d.be + (n0 >> d.b_shift) * d.estride + block0;
-    uint32_t eoff[kLoads / 4];
+    constexpr int kExpLoads = (TM + TN + 255) / 256;
+    uint32_t eoff[kExpLoads];
 #pragma unroll
-    for (int i = 0; i < kLoads / 4; i++) {                 // exponents of 64 rows: the blocks' words of A, then of B
+    for (int i = 0; i < kExpLoads; i++) {                  // exponents of 64 rows: the blocks' words of A, then of B
         const int at = 64 * (4 * i + wave), r = at < TM ? at + lane : at - TM + lane, rows = at < TM ? rows_m : rows_n;
         eoff[i] = (uint32_t)((r < rows ? r : rows - 1) >> (at < TM ? d.a_shift : d.b_shift)) * (uint32_t)d.estride;
     }
@@ -299,9 +300,9 @@ template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds_
     const auto load_exps = [&](int g) {                    // a word of four blocks' exponents for each row, two groups in turn
         const int b = 4 * g < blocks ? 4 * g : 4 * ((blocks - 1) / 4);
 #pragma unroll
-        for (int i = 0; i < kLoads / 4; i++) {
+        for (int i = 0; i < kExpLoads; i++) {
             const int at = 64 * (4 * i + wave);
-            to_lds4(lds0 + kStages * kStage + (g & 1) * 4 * (TM + TN) + 4 * at, eoff[i], (at < TM ? ebase_a : ebase_b) + b);
+            if ((TM + TN) % 256 == 0 || at < TM + TN) to_lds4(lds0 + kStages * kStage + (g & 1) * 4 * (TM + TN) + 4 * at, eoff[i], (at < TM ? ebase_a : ebase_b) + b);
         }
     };
 
@@ -399,11 +400,11 @@ template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds_
 
     C* const quarter = (C*)d.c + (long long)part * d.M * d.N + (m0 + wm) * d.ldc + n0 + wn;
     const int left_m = rows_m - wm, left_n = rows_n - wn;
+    // kGuard 0: the tile is whole; 1: its rows may end; 2: its columns too
     const auto put = [&](C* to, const auto& run, int m, int n, auto guard) {
         constexpr int R = sizeof(run) / sizeof(C);
-        if (!guard.value) { *(LooseRun<C, R>*)to = *(const LooseRun<C, R>*)&run; return; }
-        if (m >= left_m) return;
-        if (n + R <= left_n) *(LooseRun<C, R>*)to = *(const LooseRun<C, R>*)&run;
+        if (guard.value && m >= left_m) return;
+        if (guard.value < 2 || n + R <= left_n) *(LooseRun<C, R>*)to = *(const LooseRun<C, R>*)&run;
         else for (int k = 0; k < R; k++) if (n + k < left_n) to[k] = run.v[k];
     };
     const auto store = [&](auto guard) {
@@ -445,8 +446,9 @@ template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds_
     }
     };
     // (one branch for the whole tile: a guard at every store of a full one is 5% of the largest product)
-    if (rows_m == TM && rows_n == TN) store(std::false_type());
-    else store(std::true_type());
+    if (rows_n < TN) store(std::integral_constant<int, 2>());
+    else if (rows_m < TM) store(std::integral_constant<int, 1>());
+    else store(std::integral_constant<int, 0>());
 }
 
 // Few rows of A: bound by the bytes of B. A block takes 16 rows of B, its waves a share of the columns each, straight from memory into the
@@ -476,14 +478,21 @@ template <class A> __device__ __forceinline__ v8i to_codes(const Run<A, 8> (&x)[
     return r;
 }
 constexpr int kFewWaves = 8;
-template <class A, int kM, class C> __global__ void __launch_bounds__(64 * kFewWaves) k_fp8_few(FewArgs d) {
+// kM x kN tiles of 16 x 16: a wave converts (or reads) a block of A's columns once for kN tiles of B.
+template <class A, int kM, int kN, class C> __global__ void __launch_bounds__(64 * kFewWaves) k_fp8_few(FewArgs d) {
     constexpr bool kFp8 = std::is_same_v<A, uint8_t>;
-    constexpr int kAhead = kM == 1 ? (sizeof(A) == 4 ? 2 : 4) : kM == 2 && sizeof(A) < 4 ? 2 : 1;    // blocks of columns in flight: as many as the registers hold
-    __shared__ float sums[kFewWaves][kM][16][17];
+    constexpr int kRegs = kM * (kFp8 ? 8 : 8 * (int)sizeof(A)) + kN * 8;                       // registers of a block of columns in flight
+    constexpr int kAhead = kRegs > 64 ? 1 : kRegs > 32 ? 2 : 4;
+    __shared__ float sums[kFewWaves][kM * kN][16][17];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const long long n0 = (long long)blockIdx.x * 16, n = n0 + r < d.N ? n0 + r : d.N - 1;
-    const uint8_t* b = d.b + n * d.stride + 32 * g;
-    const uint8_t* be = d.be + (n >> d.b_shift) * d.estride;
+    const long long n0 = (long long)blockIdx.x * (16 * kN);
+    const uint8_t *b[kN], *be[kN];
+#pragma unroll
+    for (int i = 0; i < kN; i++) {
+        const long long n = n0 + 16 * i + r < d.N ? n0 + 16 * i + r : d.N - 1;
+        b[i] = d.b + n * d.stride + 32 * g;
+        be[i] = d.be + (n >> d.b_shift) * d.estride;
+    }
     const A* a[kM];
     const uint8_t* ae[kM];
 #pragma unroll
@@ -492,10 +501,14 @@ template <class A, int kM, class C> __global__ void __launch_bounds__(64 * kFewW
         a[i] = (const A*)d.a + (long long)m * (kFp8 ? d.stride : d.a_stride) + 32 * g;
         ae[i] = kFp8 ? d.ae + (long long)(m >> d.a_shift) * d.estride : nullptr;
     }
-    v4f acc[kM] = {};
+    const auto codes = [](const uint8_t* p) {
+        const uint4 x = *(const uint4*)p, y = *(const uint4*)(p + 16);
+        return v8i{ (int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w };
+    };
+    v4f acc[kM][kN] = {};
     for (int k0 = wave; k0 < d.blocks; k0 += kFewWaves * kAhead) {
-        v8i w[kAhead];
-        int we[kAhead];
+        v8i w[kAhead][kN];
+        int we[kAhead][kN];
         std::conditional_t<kFp8, v8i, Run<A, 8>[4]> x[kAhead][kM];
         int xe[kAhead][kM];
         // A's first, so that they are converted while B's are on the way
@@ -506,8 +519,7 @@ template <class A, int kM, class C> __global__ void __launch_bounds__(64 * kFewW
 #pragma unroll
             for (int i = 0; i < kM; i++) {
                 if constexpr (kFp8) {
-                    const uint4 s = *(const uint4*)(a[i] + 128ll * k), t = *(const uint4*)(a[i] + 128ll * k + 16);
-                    x[u][i] = v8i{ (int)s.x, (int)s.y, (int)s.z, (int)s.w, (int)t.x, (int)t.y, (int)t.z, (int)t.w };
+                    x[u][i] = codes(a[i] + 128ll * k);
                     xe[u][i] = ae[i][k];
                 } else {
                     const int left = d.K - 128 * k - 32 * g;   // values of this lane's 32 that are there
@@ -526,9 +538,11 @@ template <class A, int kM, class C> __global__ void __launch_bounds__(64 * kFewW
         for (int u = 0; u < kAhead; u++) {
             const int k = k0 + kFewWaves * u;
             if (k >= d.blocks) break;
-            const uint4 p = *(const uint4*)(b + 128ll * k), q = *(const uint4*)(b + 128ll * k + 16);
-            w[u] = v8i{ (int)p.x, (int)p.y, (int)p.z, (int)p.w, (int)q.x, (int)q.y, (int)q.z, (int)q.w };
-            we[u] = be[k];
+#pragma unroll
+            for (int i = 0; i < kN; i++) {
+                w[u][i] = codes(b[i] + 128ll * k);
+                we[u][i] = be[i][k];
+            }
         }
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
@@ -538,24 +552,28 @@ template <class A, int kM, class C> __global__ void __launch_bounds__(64 * kFewW
                 v8i code;
                 if constexpr (kFp8) code = x[u][i];
                 else code = to_codes<A>(x[u][i], xe[u][i]);
-                acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[u], code, acc[i], 0, 0, 0, we[u], 0, xe[u][i]);
+#pragma unroll
+                for (int j = 0; j < kN; j++) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[u][j], code, acc[i][j], 0, 0, 0, we[u][j], 0, xe[u][i]);
             }
         }
     }
 #pragma unroll
     for (int i = 0; i < kM; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) sums[wave][i][r][4 * g + j] = acc[i][j];
+        for (int j = 0; j < kN; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) sums[wave][i * kN + j][r][4 * g + q] = acc[i][j][q];
     __syncthreads();
-    for (int at = threadIdx.x; at < kM * 256; at += 64 * kFewWaves) {
-        const int m = at >> 4, c = at & 15;
+    for (int at = threadIdx.x; at < kM * kN * 256; at += 64 * kFewWaves) {
+        const int n = at % (16 * kN), m = at / (16 * kN);
         float s = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kFewWaves; w++) s += sums[w][m >> 4][m & 15][c];
-        if (m < d.M && n0 + c < d.N) ((C*)d.c)[m * d.ldc + n0 + c] = (C)s;
+        for (int w = 0; w < kFewWaves; w++) s += sums[w][(m >> 4) * kN + (n >> 4)][m & 15][n & 15];
+        if (m < d.M && n0 + n < d.N) ((C*)d.c)[m * d.ldc + n0 + n] = (C)s;
     }
 }
-constexpr int kFewRows = 64;
+// Up to 32 rows, floats up to 16 (64 rows by 4096 x 4096: 20 us so, 16.7 in tiles; 32 rows as floats 17.5, taken to 8 bits before 14.4).
+constexpr int kFewRows = 32, kFloatRows = 16;
 
 // The parts of a split sum, added in a fixed order: a block takes 256 results, four a lane, each of its four waves every fourth part.
 template <class C> __global__ void __launch_bounds__(256) k_fp8_join(const float* parts, int n_parts, long long size, long long N, long long ldc, C* c) {
@@ -587,18 +605,21 @@ template <class C> __global__ void __launch_bounds__(256) k_fp8_join(const float
     for (int k = 0; k < 4; k++) if (at + k < size) c[(at + k) / N * ldc + (at + k) % N] = o.v[k];
 }
 
-// How a product is divided: tiles of 256 x 256 where they fill the chip (256 CUs, one each), else of 128 x 128 (two to a CU); and the sum into parts
-// of at least 8 blocks of columns where even those leave CUs idle.
+// How a product is divided. Tiles of 256 x 256 (one to a CU) where they fill the chip and the sum is long enough for what they cost to begin and end
+// (8192 x 8192 x 512: 51 us against 59 in tiles of 128; 65536 x 256 x 256: 14.6 against 12.7); of 128 x 128 (two) where there are more than 128
+// (1003 x 2077 x 1500: 8.1 against 9.7 in tiles of 64); else of 64 x 64 (1000 x 1000 x 1000: 4.8 against 7.0, 512 x 4096 x 4096: 16.8 against 18.4).
+// Long sums of few such tiles go into parts of at least 16 blocks of columns, which a second launch adds (256 x 256 x 65536: 15.9 against 198;
+// 1024 x 1024 x 8192: 23.0 against 27.9; but 256 x 4096 x 4096: 16.6 against 10.3).
 struct Plan { int tile, parts, split_blocks; };
 static Plan plan_of(int64_t M, int64_t N, int64_t K) {
     const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    const auto tiles_of = [&](int64_t t) { return up(M, t) * up(N, t); };
     const int64_t blocks = up(K, 128);
-    Plan p = { 256, 1, (int)blocks };
-    if (up(M, 256) * up(N, 256) < 200) p.tile = 128;
-    const int64_t tiles = up(M, p.tile) * up(N, p.tile);
-    if (p.tile == 128 && tiles <= 128 && blocks >= 16) {
-        int64_t parts = 256 / tiles;
-        if (parts > blocks / 8) parts = blocks / 8;
+    Plan p = { tiles_of(256) >= 200 && blocks >= 4 ? 256 : tiles_of(128) > 128 ? 128 : 64, 1, (int)blocks };
+    const int64_t tiles = tiles_of(p.tile);
+    if (p.tile == 64 && tiles <= 256 && blocks >= 48) {
+        int64_t parts = 512 / tiles;
+        if (parts > blocks / 16) parts = blocks / 16;
         p.split_blocks = (int)(up(up(blocks, parts), 4) * 4);
         p.parts = (int)up(blocks, p.split_blocks);
     }
@@ -630,21 +651,21 @@ extern "C" size_t ntc_op_fp8_matmul_workspace(int64_t M, int64_t N, int64_t K, i
     const Plan p = plan_of(M, N, K);
     return p.parts > 1 ? (size_t)p.parts * M * N * 4 : 0;
 }
-extern "C" int64_t ntc_op_fp8_matmul_float_rows(void) { return kFewRows; }
+extern "C" int64_t ntc_op_fp8_matmul_float_rows(void) { return kFloatRows; }
 
-template <class A, class C> static void launch_few(const FewArgs& F, hipStream_t s) {
-    const unsigned blocks = (unsigned)((F.N + 15) / 16);
-    if (F.M <= 16) k_fp8_few<A, 1, C><<<blocks, 64 * kFewWaves, 0, s>>>(F);
-    else if (F.M <= 32) k_fp8_few<A, 2, C><<<blocks, 64 * kFewWaves, 0, s>>>(F);
-    else k_fp8_few<A, 4, C><<<blocks, 64 * kFewWaves, 0, s>>>(F);
+template <class A, int kM, class C> static void launch_few(const FewArgs& F, hipStream_t s) {
+    // two tiles of B a wave where that still leaves a block to each CU
+    if (F.N >= 32 * 256) k_fp8_few<A, kM, 2, C><<<(unsigned)((F.N + 31) / 32), 64 * kFewWaves, 0, s>>>(F);
+    else k_fp8_few<A, kM, 1, C><<<(unsigned)((F.N + 15) / 16), 64 * kFewWaves, 0, s>>>(F);
 }
 template <class C> static void run_few(const ntc_fp8_matmul_desc* d, hipStream_t s) {
     const FewArgs F = { d->a, d->a_exps, d->b, d->b_exps, d->c, d->N, d->a_stride, d->ldc, (int)d->M, (int)d->K, (int)((d->K + 127) / 128), (int)ntc_fp8_code_stride(d->K),
                         (int)ntc_fp8_exp_stride(d->K), d->a_block_rows == 128 ? 7 : 0, d->b_block_rows == 128 ? 7 : 0 };
-    if (d->a_type == NTC_FP8) launch_few<uint8_t, C>(F, s);
-    else if (d->a_type == NTC_F32) launch_few<f32, C>(F, s);
-    else if (d->a_type == NTC_BF16) launch_few<bf16, C>(F, s);
-    else launch_few<f16, C>(F, s);
+    if (d->a_type == NTC_F32) launch_few<f32, 1, C>(F, s);
+    else if (d->a_type == NTC_BF16) launch_few<bf16, 1, C>(F, s);
+    else if (d->a_type == NTC_F16) launch_few<f16, 1, C>(F, s);
+    else if (d->M <= 16) launch_few<uint8_t, 1, C>(F, s);
+    else launch_few<uint8_t, 2, C>(F, s);
 }
 
 template <int T, class C> static void launch_matmul(const MatmulArgs& A, int parts, hipStream_t s) {
@@ -673,7 +694,8 @@ template <class C> static void run_matmul(const ntc_fp8_matmul_desc* d, hipStrea
     A.c = p.parts > 1 ? d->workspace : d->c;
     A.ldc = p.parts > 1 ? d->N : d->ldc;
     if (p.tile == 256) launch_matmul<256, C>(A, 1, s);
-    else launch_matmul<128, C>(A, p.parts, s);
+    else if (p.tile == 128) launch_matmul<128, C>(A, p.parts, s);
+    else launch_matmul<64, C>(A, p.parts, s);
     if (p.parts > 1) k_fp8_join<C><<<(unsigned)((d->M * d->N + 255) / 256), 256, 0, s>>>((const float*)d->workspace, p.parts, d->M * d->N, d->N, d->ldc, (C*)d->c);
 }
 
@@ -681,7 +703,7 @@ extern "C" int ntc_op_fp8_matmul(const ntc_fp8_matmul_desc* d, void* stream, cha
     if (!d) return refuse(why, cap, "no description");
     if (d->M < 0 || d->N < 0 || d->K < 0) return refuse(why, cap, "sizes are not negative");
     if (d->a_type < 0 || d->a_type > NTC_FP8) return refuse(why, cap, "A is 8-bit codes, or 32-bit floats, bfloat16 or float16");
-    if (d->a_type != NTC_FP8 && d->M > kFewRows) return refuse(why, cap, "A of more than 64 rows is given in 8 bits");
+    if (d->a_type != NTC_FP8 && d->M > kFloatRows) return refuse(why, cap, "A of more than 16 rows is given in 8 bits");
     if (d->a_type != NTC_FP8 && d->a_stride < 0) return refuse(why, cap, "strides are not negative");
     if (d->c_type < 0 || d->c_type > 2) return refuse(why, cap, "C is 32-bit floats, bfloat16 or float16");
     if ((d->a_block_rows != 1 && d->a_block_rows != 128) || (d->b_block_rows != 1 && d->b_block_rows != 128)) return refuse(why, cap, "blocks are 1 x 128 or 128 x 128");
