@@ -34,17 +34,31 @@ __device__ __forceinline__ float read_lane(float x, int l) { return __uint_as_fl
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }   // one instruction, 1 ulp; 2^-inf = 0
 __device__ __forceinline__ float fast_log2(float x) { return __builtin_amdgcn_logf(x); }
 
-// Reductions over aligned groups of 16 lanes (rotations within a row of the vector registers) and of 64 (rows swapped on the
-// way): every lane gets the result, and no shared memory is used.
-template <int kRor> __device__ __forceinline__ uint32_t rotate16(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + kRor, 0xf, 0xf, false); }
-template <class V, class F> __device__ __forceinline__ V reduce16(V x, F f) {
-    const auto turn = [](V v, auto n) { return __builtin_bit_cast(V, rotate16<n.value>(__builtin_bit_cast(uint32_t, v))); };
-    x = f(x, turn(x, std::integral_constant<int, 8>()));
-    x = f(x, turn(x, std::integral_constant<int, 4>()));
-    x = f(x, turn(x, std::integral_constant<int, 2>()));
-    return f(x, turn(x, std::integral_constant<int, 1>()));
+// Reductions over aligned groups of 4, 8, 16, 32 and 64 lanes: every lane gets the result, and no shared memory is used (lanes
+// exchanged within a row of 16 on the way into the instruction, rows swapped). f is commutative and associative.
+template <int kCtrl, class V> __device__ __forceinline__ V exchange(V x) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kCtrl, 0xf, 0xf, false));
 }
-// of lanes l and l ^ 16, then l ^ 32
+template <int kGroup, class V, class F> __device__ __forceinline__ V reduce(V x, F f) {
+    x = f(x, exchange<0xb1>(x));                             // lane ^ 1
+    x = f(x, exchange<0x4e>(x));                             // lane ^ 2
+    if constexpr (kGroup >= 8) x = f(x, exchange<0x141>(x)); // the other four of eight, mirrored
+    if constexpr (kGroup >= 16) x = f(x, exchange<0x140>(x));
+    if constexpr (kGroup >= 32) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, x);
+        const auto p = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+        x = f(__builtin_bit_cast(V, (uint32_t)p[0]), __builtin_bit_cast(V, (uint32_t)p[1]));
+    }
+    if constexpr (kGroup >= 64) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, x);
+        const auto p = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+        x = f(__builtin_bit_cast(V, (uint32_t)p[0]), __builtin_bit_cast(V, (uint32_t)p[1]));
+    }
+    return x;
+}
+template <class V, class F> __device__ __forceinline__ V reduce16(V x, F f) { return reduce<16>(x, f); }
+template <class V, class F> __device__ __forceinline__ V reduce64(V x, F f) { return reduce<64>(x, f); }
+// of lanes l, l ^ 16, l ^ 32 and l ^ 48
 template <class V, class F> __device__ __forceinline__ V reduce_rows(V x, F f) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x);
     const auto p = __builtin_amdgcn_permlane16_swap(b, b, false, false);
@@ -52,11 +66,6 @@ template <class V, class F> __device__ __forceinline__ V reduce_rows(V x, F f) {
     const uint32_t c = __builtin_bit_cast(uint32_t, x);
     const auto q = __builtin_amdgcn_permlane32_swap(c, c, false, false);
     return f(__builtin_bit_cast(V, (uint32_t)q[0]), __builtin_bit_cast(V, (uint32_t)q[1]));
-}
-template <class V, class F> __device__ __forceinline__ V reduce64(V x, F f) { return reduce_rows(reduce16(x, f), f); }
-template <int kGroup, class V, class F> __device__ __forceinline__ V reduce(V x, F f) {
-    if constexpr (kGroup == 16) return reduce16(x, f);
-    else return reduce64(x, f);
 }
 
 // ---------------------------------------------------------------- refusals

@@ -64,25 +64,42 @@ __device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_floa
 
 __device__ __forceinline__ uint32_t above(uint32_t a, uint32_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint32_t below(uint32_t a, uint32_t b) { return a < b ? a : b; }
-// A lane's three largest keys, in order (0: none).
+// A lane's three best keys, in order (0: none). 16-bit types: the index is in the key.
 struct Three {
-    uint32_t a, b, c;
+    uint32_t a = 0, b = 0, c = 0;
     __device__ __forceinline__ static uint32_t middle(uint32_t x, uint32_t y, uint32_t z) { return above(below(x, y), below(above(x, y), z)); }   // one instruction
-    __device__ __forceinline__ void add(uint32_t k) { c = middle(b, c, k); b = middle(a, b, k); a = above(a, k); }
+    __device__ __forceinline__ void add(uint32_t k, uint32_t) { c = middle(b, c, k); b = middle(a, b, k); a = above(a, k); }
+    __device__ __forceinline__ void next() { a = b; b = c; c = 0; }
+};
+// With the index beside the key; added in ascending order, so that the first of equals stays ahead.
+struct ThreePlaced {
+    uint32_t a = 0, b = 0, c = 0, ia = ~0u, ib = ~0u, ic = ~0u;
+    __device__ __forceinline__ void add(uint32_t k, uint32_t i) {
+        const bool pa = k > a, pb = k > b, pc = k > c;
+        c = pb ? b : pc ? k : c;
+        ic = pb ? ib : pc ? i : ic;
+        b = pa ? a : pb ? k : b;
+        ib = pa ? ia : pb ? i : ib;
+        a = pa ? k : a;
+        ia = pa ? i : ia;
+    }
+    __device__ __forceinline__ void next() { a = b; b = c; c = 0; ia = ib; ib = ic; ic = ~0u; }
 };
 
-// A group of kGroup lanes holds a row in registers, kEach neighbouring values a lane: the largest, then the sums, then the alternatives one by
-// one, from the lanes' three largest. A 16-bit type's float has 13 low bits to spare, which take the index (of a row of at most
-// 1024, from the top down): one word orders values and indices both. A 32-bit value's index is found in a second reduction.
-// Bound by instructions: 262144 rows of 256 bf16 values with 4 alternatives take twice what their bytes do.
+// A group of kGroup lanes holds a row in registers, 16 neighbouring values a lane: the largest, then the sums, then the alternatives one by
+// one, from the lanes' three best, through LDS to whole runs of the results. A 16-bit type's float has 13 low bits to spare, which take the
+// index (of a row of at most 1024, from the top down): one word orders values and indices both. A 32-bit value's index is found in a second
+// reduction. Bound by instructions: 262144 rows of 256 bf16 values with 4 alternatives take half again what their bytes do.
 constexpr int kShort = 1024;                                 // the longest such row
-template <class T, int kGroup, int kEach> __global__ void __launch_bounds__(256) k_logprobs_short(ntc_logprobs_desc d, float lim) {
-    constexpr int kVec = 16 / (int)sizeof(T) < kEach ? 16 / (int)sizeof(T) : kEach;
+template <class T, int kGroup> __global__ void __launch_bounds__(256) k_logprobs_short(ntc_logprobs_desc d, float lim) {
+    constexpr int kEach = 16, kVec = 16 / (int)sizeof(T), kRows = 256 / kGroup;
+    constexpr bool kPlaced = sizeof(T) == 4;
     constexpr uint32_t kMask = ~0x1fffu;
     static_assert(kGroup * kEach <= kShort, "indices of 10 bits");
-    const int in = threadIdx.x % kGroup;
-    const long long row = (long long)blockIdx.x * (256 / kGroup) + threadIdx.x / kGroup;
-    if (row >= d.rows) return;                              // whole groups
+    __shared__ uint32_t keys[kRows][NTC_MAX_TOP], places[kPlaced ? kRows : 1][NTC_MAX_TOP];
+    __shared__ float2 stat[kRows];
+    const int in = threadIdx.x % kGroup, own = threadIdx.x / kGroup;
+    const long long first = (long long)blockIdx.x * kRows, row = first + own < d.rows ? first + own : d.rows - 1;   // past the end the last row again, not written
     long long outer, inner;
     const T* x = row_of<T>(d, row, outer, inner);
     const int V = (int)d.V, at = in * kEach;
@@ -90,8 +107,21 @@ template <class T, int kGroup, int kEach> __global__ void __launch_bounds__(256)
     float v[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; i += kVec) {
-        if (at + i + kVec <= V) { const auto r = *(const LooseRun<T, kVec>*)(x + at + i); for (int j = 0; j < kVec; j++) v[i + j] = (float)r.v[j]; }
-        else for (int j = 0; j < kVec; j++) v[i + j] = at + i + j < V ? (float)x[at + i + j] : -NTC_INF;
+        const int left = V - at - i;                         // of this vector's values
+        if (left >= kVec) {
+            const auto r = *(const LooseRun<T, kVec>*)(x + at + i);
+#pragma unroll
+            for (int j = 0; j < kVec; j++) v[i + j] = (float)r.v[j];
+        } else if (left > 0) {
+            T r[kVec];
+#pragma unroll
+            for (int j = 0; j < kVec; j++) r[j] = x[at + i + (j < left ? j : 0)];
+#pragma unroll
+            for (int j = 0; j < kVec; j++) v[i + j] = j < left ? (float)r[j] : -NTC_INF;
+        } else {
+#pragma unroll
+            for (int j = 0; j < kVec; j++) v[i + j] = -NTC_INF;
+        }
     }
     const auto larger = [](float a, float b) { return fmaxf(a, b); };
     const auto sum = [](float a, float b) { return a + b; };
@@ -124,7 +154,7 @@ template <class T, int kGroup, int kEach> __global__ void __launch_bounds__(256)
     t = reduce<kGroup>(t, sum);
     const bool none = s == 0.0f;
     const float log_s = fast_log2(s);
-    if (in == 0) write_row(d, row, x, token_of(d, outer, inner), mm, log_s, t / s, none, inv_t);
+    if (in == 0 && first + own < d.rows) write_row(d, row, x, token_of(d, outer, inner), mm, log_s, t / s, none, inv_t);
     if (!d.top) return;
     if (__ballot(s != s)) {                                  // a NaN somewhere (or +inf): in the order it counts as -inf
 #pragma unroll
@@ -134,50 +164,55 @@ template <class T, int kGroup, int kEach> __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int j = 0; j < kEach; j++) {
         key[j] = order_key(v[j]);
-        if constexpr (sizeof(T) == 2) key[j] = ((key[j] & kMask) | (uint32_t)(kShort - 1 - at)) - j;   // (at is a multiple of kEach: no borrow)
+        if constexpr (!kPlaced) key[j] = ((key[j] & kMask) | (uint32_t)(kShort - 1 - at)) - j;   // (at is a multiple of 16: no borrow)
     }
     if (V < kGroup * kEach) {
         asm volatile("");                                    // (a branch, not selections that every row would make)
 #pragma unroll
         for (int j = 0; j < kEach; j++) key[j] = at + j < V ? key[j] : 0;   // below every key of a value
     }
-    uint32_t mine = 0, mine_at = 0, last = 0, last_at = 0;
-    Three best = { 0, 0, 0 };
-    if constexpr (sizeof(T) == 2) {
+    std::conditional_t<kPlaced, ThreePlaced, Three> best;
 #pragma unroll
-        for (int j = 0; j < kEach; j++) best.add(key[j]);
-    }
+    for (int j = 0; j < kEach; j++) best.add(key[j], (uint32_t)(at + j));
     for (int r = 0; r < d.top; r++) {
-        if constexpr (sizeof(T) == 2) {
-            last = reduce<kGroup>(best.a, above);
-            const bool took = best.a == last;
-            best = { took ? best.b : best.a, took ? best.c : best.b, took ? 0 : best.c };
-            if (__ballot(took && best.a == 0 && r + 1 < d.top)) {   // a lane has given its three: again from those below the last
-                asm volatile("");
-                best = { 0, 0, 0 };
-#pragma unroll
-                for (int j = 0; j < kEach; j++) best.add(key[j] < last ? key[j] : 0);
-            }
-        } else {
-            // open are those below the last, and those equal to it past its index; ascending j: the first of equals stays
-            uint32_t high = 0, place = 0xffffffffu;
+        const uint32_t last = reduce<kGroup>(best.a, above);
+        uint32_t place = 0;
+        bool took = best.a == last;
+        if constexpr (kPlaced) {
+            place = reduce<kGroup>(took ? best.ia : ~0u, below);
+            took = took && best.ia == place;
+            if (in == 0) places[own][r] = place;
+        }
+        if (in == 0) keys[own][r] = last;
+        if (took) best.next();
+        if (__ballot(took && best.a == 0 && r + 1 < d.top)) {   // a lane has given its three: again from those that come after the last
+            asm volatile("");
+            best = {};
 #pragma unroll
             for (int j = 0; j < kEach; j++) {
-                const bool open = r == 0 || key[j] < last || (key[j] == last && (uint32_t)(at + j) > last_at);
-                if (open && at + j < V && (key[j] > high || place == 0xffffffffu)) { high = key[j]; place = (uint32_t)(at + j); }
+                const bool open = key[j] < last || (kPlaced && key[j] == last && (uint32_t)(at + j) > place);
+                best.add(open ? key[j] : 0, (uint32_t)(at + j));
             }
-            last = reduce<kGroup>(place == 0xffffffffu ? 0u : high, above);
-            last_at = reduce<kGroup>(high == last ? place : 0xffffffffu, below);
         }
-        if (in == r) { mine = last; mine_at = last_at; }
     }
-    if (in < d.top) {
-        if constexpr (sizeof(T) == 2) {
-            mine_at = kShort - 1 - (mine & (kShort - 1));
-            mine = mine & 0x80000000u ? mine & kMask : mine | ~kMask;
+    if (in == 0) stat[own] = { none ? NTC_INF : mm, log_s };
+    // a wave writes what its own rows found: its lanes' LDS operations are in order
+    __builtin_amdgcn_wave_barrier();
+    const int wave_row = (threadIdx.x >> 6) * (64 / kGroup);
+    for (int e = lane_id(); e < 64 / kGroup * d.top; e += 64) {
+        const int rl = wave_row + e / d.top, r = e % d.top;
+        if (first + rl >= d.rows) break;
+        uint32_t found = keys[rl][r], place = 0;
+        if constexpr (kPlaced) place = places[rl][r];
+        else {
+            place = kShort - 1 - (found & (kShort - 1));
+            found = found & 0x80000000u ? found & kMask : found | ~kMask;
         }
-        d.top_ids[row * d.top + in] = mine_at;
-        d.top_logprobs[row * d.top + in] = none ? -NTC_INF : log_prob(key_value(mine), mm, inv_t, log_s);
+        const float2 st = stat[rl];
+        const long long to = (first + rl) * d.top + r;
+        d.top_ids[to] = place;
+        // (a NaN in the row has made log_s NaN, which swallows what stands for it here)
+        d.top_logprobs[to] = st.x == NTC_INF && !(st.y != st.y) ? -NTC_INF : log_prob(key_value(found), st.x, inv_t, st.y);
     }
 }
 
@@ -437,8 +472,13 @@ template <class T> __global__ void __launch_bounds__(256) k_logprobs_grad(ntc_lo
     if (tops && lane >= 1 && lane <= d.top) { place = (int)d.top_ids[row * d.top + lane - 1]; extra = d.g_top[row * d.top + lane - 1]; }
     float all = reduce64(extra, [](float p, float q) { return p + q; });
     if (out) all = __builtin_nanf("");
+    // a token that is an alternative too gets both at once: they may nearly cancel
+    const bool twice = lane && place >= 0 && place == t;
+    const bool moved = __ballot(twice) != 0;
+    if (twice) extra += glp;
+    if (lane == 0 && moved) place = -1;
     extra *= inv_t;
-    const float na = -all * inv_t, nh = -gh * inv_t;
+    const float na = -all * inv_t * 0x1p-24f, nh = -gh * inv_t * 0x1p-24f;
 #pragma unroll
     for (int c = 0; c < kGradVecs; c++) {
         const int base = begin + c * kChunk, at = base + lane * kVec;
@@ -450,7 +490,8 @@ template <class T> __global__ void __launch_bounds__(256) k_logprobs_grad(ntc_lo
         float g[kVec];
 #pragma unroll
         for (int j = 0; j < kVec; j++) {
-            const float lp = ((float)r[j] - m) * k - log_s, p = fast_exp2(lp);
+            // (the exponential's instruction gives 0 for what is below 2^-126: probabilities are taken times 2^24)
+            const float lp = ((float)r[j] - m) * k - log_s, p = fast_exp2(lp + 24.0f);
             g[j] = p * __builtin_fmaf(nh, __builtin_fmaf(kLn2, fmaxf(lp, -160.0f), H), na);
         }
         unsigned long long here = __ballot(place >= base && place < base + kChunk);
@@ -488,9 +529,11 @@ template <class T> static Reading reading(int64_t rows, int64_t V) {
 template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s) {
     const auto blocks = [&](int per) { return (unsigned)((d.rows + per - 1) / per); };
     const float k = kLog2e / d.temperature, lim = 1e30f / (k > 1.0f ? k : 1.0f);   // values up to lim times k stay far from overflow
-    if (d.V <= 64 && d.top <= 16) { k_logprobs_short<T, 16, 4><<<blocks(16), 256, 0, s>>>(d, lim); return; }
-    if (d.V <= 256 && d.top <= 16) { k_logprobs_short<T, 16, 16><<<blocks(16), 256, 0, s>>>(d, lim); return; }
-    if (d.V <= kShort) { k_logprobs_short<T, 64, 16><<<blocks(4), 256, 0, s>>>(d, lim); return; }
+    if (d.V <= 64) { k_logprobs_short<T, 4><<<blocks(64), 256, 0, s>>>(d, lim); return; }
+    if (d.V <= 128) { k_logprobs_short<T, 8><<<blocks(32), 256, 0, s>>>(d, lim); return; }
+    if (d.V <= 256) { k_logprobs_short<T, 16><<<blocks(16), 256, 0, s>>>(d, lim); return; }
+    if (d.V <= 512) { k_logprobs_short<T, 32><<<blocks(8), 256, 0, s>>>(d, lim); return; }
+    if (d.V <= kShort) { k_logprobs_short<T, 64><<<blocks(4), 256, 0, s>>>(d, lim); return; }
     const Reading r = reading<T>(d.rows, d.V);
     if (r.waves == 1) k_logprobs_long<T, 1, false><<<blocks(4), 256, 0, s>>>(d, lim, 0);
     else if (r.parts == 1) k_logprobs_long<T, 4, false><<<blocks(1), 256, 0, s>>>(d, lim, 0);

@@ -104,7 +104,7 @@ def whole_numbers(seed, R, K, rows):
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 16, 128), (2, 64, 64), (5, 300, 200), (16, 256, 1024), (17, 33, 129), (64, 64, 640), (100, 130, 384), (128, 128, 128), (129, 257, 513),
-                                   (256, 256, 256), (300, 700, 1100), (512, 260, 96), (1000, 512, 512), (7, 4097, 2000), (260, 250, 9000), (1, 5000, 700), (40, 48, 20000)])
+                                   (256, 256, 256), (300, 700, 1100), (512, 260, 96), (1000, 512, 512), (7, 4097, 2000), (260, 250, 9000), (1, 5000, 700), (40, 48, 20000), (20, 9000, 300), (1500, 1500, 300), (3601, 3590, 520)])
 @pytest.mark.parametrize("rows", [(1, 128), (1, 1), (128, 1)])
 def test_products_of_whole_numbers_are_exact(M, N, K, rows):
     print("matmul", M, N, K, rows, flush=True)

@@ -106,6 +106,21 @@ def test_sizes(N, V, top, dtype):
     check(*make(N, V, dtype), top, T=0.7 if V % 2 else 1.3)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [16, 17, 47, 64, 65, 128, 129, 200, 257, 512, 513, 1024])
+def test_short_rows_with_many_alternatives(V, dtype):
+    """Groups of every size, more rows than a block takes and not a multiple of it, alternatives that one lane holds most of."""
+    print("logprobs short", V, dtype, flush=True)
+    x, t = make(149, V, dtype, seed=V)
+    x[1] = torch.arange(V, device="cuda").to(dtype)             # the best are all at the end, neighbours
+    x[2] = -torch.arange(V, device="cuda").to(dtype)
+    x[3, : min(V, 16)] += 50
+    x[4, V // 2:] = -math.inf
+    x[5, ::5] = math.nan
+    for top in (0, 1, 5, min(32, V)):
+        check(x, t, top, T=0.9)
+
+
 @pytest.mark.parametrize("N,V", [(1100, 2048), (1030, 5000), (520, 20001), (300, 40000), (40, 100000), (9, 200003)])
 def test_more_rows(N, V):
     print("logprobs rows", N, V, flush=True)
