@@ -217,23 +217,53 @@ template <class T, int kGroup> __global__ void __launch_bounds__(256) k_logprobs
 }
 
 // ---------------------------------------------------------------- long rows
-// The best K values of what a wave has read, in its lanes 0 to K - 1: value and index, in order; empty places are (-inf, kNoIndex).
-constexpr int kNoIndex = 0x7fffffff;
-struct Best {
-    float v;
-    int i;
-    __device__ __forceinline__ void clear() { v = -NTC_INF; i = kNoIndex; }
-    // (w, j), the same in all lanes, to its place
-    __device__ __forceinline__ void insert(float w, int j) {
-        const bool keeps = v > w || (v == w && i < j);
-        const int at = __builtin_popcountll(__ballot(keeps));
-        const float uv = __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x138, 0xf, 0xf, false));   // lane l gets lane l - 1's
-        const int ui = __builtin_amdgcn_update_dpp(0, i, 0x138, 0xf, 0xf, false);
-        const int l = lane_id();
-        v = l < at ? v : l == at ? w : uv;
-        i = l < at ? i : l == at ? j : ui;
+// The best values of what a wave has read: up to 64 candidates in LDS that its chunks add to; full, they are put in order (each counts
+// those before it) and the first `top` stay. Empty places of a finished list are (-inf, kNoIndex).
+constexpr int kNoIndex = 0x7fffffff, kCandidates = 64;
+struct Best { float v; int i; };
+struct Candidates {
+    float* v;
+    int* i;
+    int n;                                                   // the same in all lanes
+    __device__ __forceinline__ void put_in_order(int top) {
+        const int lane = lane_id();
+        __builtin_amdgcn_wave_barrier();                     // (a wave's LDS operations are in order)
+        const float w = lane < n ? v[lane] : -NTC_INF;
+        const int j = lane < n ? i[lane] : kNoIndex;
+        const uint32_t key = lane < n ? order_key(w) : 0;
+        const unsigned long long mine = (unsigned long long)key << 32 | (uint32_t)~j;
+        int before = 0;
+        for (int l = 0; l < n; l += 4) {                     // (lanes past n come after all others)
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const unsigned long long other = (unsigned long long)(uint32_t)__builtin_amdgcn_readlane(key, l + u) << 32 | (uint32_t)__builtin_amdgcn_readlane(~j, l + u);
+                before += other > mine;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (lane < n && before < top) { v[before] = w; i[before] = j; }
+        n = n < top ? n : top;
+        __builtin_amdgcn_wave_barrier();
+    }
+    // lanes of `ask` add (w, j); returns those that found no place
+    __device__ __forceinline__ unsigned long long add(unsigned long long ask, float w, int j) {
+        const int at = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(ask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ask, 0u));
+        const bool mine = ask >> lane_id() & 1;
+        if (mine && at < kCandidates) { v[at] = w; i[at] = j; }
+        const unsigned long long rest = __ballot(mine && at >= kCandidates);
+        n += __builtin_popcountll(ask) - __builtin_popcountll(rest);
+        return rest;
     }
 };
+// A bound that the K-th largest of 64 lanes' values reaches, within a 2^-10 of its size: its highest bits, one by one.
+__device__ __forceinline__ float kth_largest(float x, int k) {
+    const uint32_t key = order_key(x != x ? -NTC_INF : x);
+    uint32_t t = 0;
+#pragma unroll
+    for (uint32_t bit = 1u << 31; bit >= 1u << 13; bit >>= 1)
+        if (__builtin_popcountll(__ballot(key >= (t | bit))) >= k) t |= bit;
+    return t <= 0x007fffffu ? -NTC_INF : key_value(t);
+}
 
 // The best of up to 64 lists in LDS (list p's values at v + p stride, indices at i + p stride): each lane holds the head of one, the
 // best head of all is taken and its lane moves on.
@@ -242,8 +272,7 @@ __device__ __forceinline__ Best merge(const float* v, const int* i, int stride, 
     int at = lane * stride, left = lane < lists ? top : 0;
     float hv = left ? v[at] : -NTC_INF;
     int hi = left ? i[at] : kNoIndex;
-    Best best;
-    best.clear();
+    Best best = { -NTC_INF, kNoIndex };
     for (int r = 0; r < top; r++) {
         const float bv = reduce64(hv, [](float p, float q) { return fmaxf(p, q); });
         const int bi = (int)reduce64((uint32_t)(hv == bv ? hi : kNoIndex), [](uint32_t p, uint32_t q) { return p < q ? p : q; });
@@ -264,18 +293,20 @@ template <class T> struct Long { static constexpr int kVec = 16 / (int)sizeof(T)
 // A wave's share of a row: chunks first, first + step, .. below `end` (chunks of kChunk values, the last one ragged).
 // The sums are each lane's own, on a floor that only rises: exp2(x k - m k) is one fused operation and an exponential, with m held
 // within lim so that neither product overflows. A row whose values all lie below -lim, or reach past lim, or hold NaN ends with s = 0, infinite or
-// NaN and is read again by scan_again(). Values enter the list of the best only where their lane's largest of a chunk passes the list's last.
-template <class T> __device__ __forceinline__ void scan(const T* x, int V, int first, int step, int end, float k, float lim, int top, Soft& a, Best& best) {
+// NaN and is read again by scan_again(). Values become candidates where their lane's largest of a chunk passes what `top` values are known to
+// reach: in the wave's own list, or in that of another wave of the row (bar: as an integer that orders; only ever raised).
+template <class T> __device__ __forceinline__ void scan(const T* x, int V, int first, int step, int end, float k, float lim, int top, Soft& a, Candidates& list, uint32_t* bar) {
     using L = Long<T>;
     const int lane = lane_id();
     a = { -lim, 0.0f, 0.0f };
-    best.clear();
-    float mk = -lim * k, last = -NTC_INF;
+    float mk = -lim * k;
+    float reach = -NTC_INF, pass = -NTC_INF;                 // candidates are >= reach and, since the list's are of earlier indices, > pass
     bool fresh = true;
     for (int c = first; c < end; c += step) {
         float v[L::kRun];
         const int base = c * L::kChunk;
         const int at0 = base + lane * L::kVec;
+        const uint32_t others = top && bar ? *(volatile uint32_t*)bar : 0;
         if (base + L::kChunk <= V) {
 #pragma unroll
             for (int i = 0; i < L::kVecs; i++) {
@@ -306,31 +337,36 @@ template <class T> __device__ __forceinline__ void scan(const T* x, int V, int f
             a.t = __builtin_fmaf(e, fmaxf(d, -1e30f), a.t);
         }
         if (!top) continue;
-        float least = last;                                  // the list's last value; only larger ones can pass it later in the row
-        if (fresh) {
-            // the first chunk would enter the list value by value: start from the K-th largest of the lanes' largest, which K values reach
-            float w = cm;
-            for (int r = 0; r < top; r++) {
-                least = reduce64(w, [](float p, float q) { return fmaxf(p, q); });
-                const int who = __builtin_ctzll(__ballot(w == least) | 1ull << 63);
-                w = lane == who ? -NTC_INF : w;
-            }
-        }
-        if (__ballot(fresh ? cm >= least : cm > least)) {
+        if (others > 0x007fffffu) reach = fmaxf(reach, key_value(others));
+        if (fresh) reach = fmaxf(reach, kth_largest(cm, top));   // at least `top` values of the first chunk reach it
+        if (__ballot(cm >= reach && cm > pass)) {
+            bool some = false;
 #pragma unroll
             for (int j = 0; j < L::kRun; j++) {
-                unsigned long long ask = __ballot(v[j] >= least && v[j] > -NTC_INF);
+                unsigned long long ask = __ballot(v[j] >= reach && v[j] > pass);
                 while (ask) {
-                    const int l = __builtin_ctzll(ask);
-                    best.insert(read_lane(v[j], l), base + (j / L::kVec) * 64 * L::kVec + l * L::kVec + j % L::kVec);
-                    least = fmaxf(least, read_lane(best.v, top - 1));
-                    ask &= ask - 1;
-                    ask &= __ballot(v[j] >= least);
+                    some = true;
+                    ask = list.add(ask, v[j], base + (j / L::kVec) * 64 * L::kVec + lane * L::kVec + j % L::kVec);
+                    if (list.n == kCandidates) {
+                        list.put_in_order(top);
+                        reach = fmaxf(reach, list.v[top - 1]);
+                        ask &= __ballot(v[j] >= reach);
+                    }
                 }
             }
-            last = read_lane(best.v, top - 1);
+            if (some && (fresh || list.n >= top + 16)) {
+                list.put_in_order(top);
+                if (list.n == top) {                         // its last may only be passed, by later indices
+                    pass = fmaxf(pass, list.v[top - 1]);
+                    if (bar && lane == 0) atomicMax(bar, order_key(pass));
+                }
+            }
         }
         fresh = false;
+    }
+    if (top) {
+        list.put_in_order(top);
+        if (lane >= list.n && lane < top) { list.v[lane] = -NTC_INF; list.i[lane] = kNoIndex; }
     }
     if (a.s == 0.0f) return;                                 // (nothing above the floor: its m k has no meaning)
     // the sums were taken on the rounded m k: to those on m itself
@@ -394,27 +430,34 @@ template <class T> __device__ __forceinline__ void finish(const ntc_logprobs_des
 // kWaves waves (of a block of 4) read a row; with kParts a block reads the part blockIdx.y of a row and leaves its sums and list in the workspace.
 template <class T, int kWaves, bool kParts> __global__ void __launch_bounds__(256) k_logprobs_long(ntc_logprobs_desc d, float lim, int part_chunks) {
     __shared__ Soft soft[4];
-    __shared__ float list_v[4][NTC_MAX_TOP];
-    __shared__ int list_i[4][NTC_MAX_TOP];
+    __shared__ float list_v[4][kCandidates];
+    __shared__ int list_i[4][kCandidates];
+    __shared__ uint32_t bar;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id();
     const long long row = (long long)blockIdx.x * (4 / kWaves) + wave / kWaves;
     if (row >= d.rows) return;                               // (kWaves 1: a wave on its own; else whole blocks)
+    if (kWaves > 1) {
+        if (threadIdx.x == 0) bar = 0;
+        __syncthreads();
+    }
     long long outer, inner;
     const T* x = row_of<T>(d, row, outer, inner);
     const float k = kLog2e / d.temperature;
     const int V = (int)d.V, chunks = (V + Long<T>::kChunk - 1) / Long<T>::kChunk;
     const int begin = kParts ? (int)blockIdx.y * part_chunks : 0, end = kParts && begin + part_chunks < chunks ? begin + part_chunks : chunks;
     Soft a;
-    Best best;
-    scan(x, V, begin + wave % kWaves, kWaves, end, k, lim, d.top, a, best);
+    Candidates list = { list_v[wave], list_i[wave], 0 };
+    scan(x, V, begin + wave % kWaves, kWaves, end, k, lim, d.top, a, list, kWaves > 1 ? &bar : nullptr);
     a = join_lanes(a, k);
+    Best best = { -NTC_INF, kNoIndex };
     if (kWaves > 1) {
         if (lane == 0) soft[wave] = a;
-        if (lane < d.top) { list_v[wave][lane] = best.v; list_i[wave][lane] = best.i; }
         __syncthreads();
         if (wave) return;
         for (int w = 1; w < kWaves; w++) soft_join(a, soft[w], k);
-        if (d.top) best = merge(list_v[0], list_i[0], NTC_MAX_TOP, kWaves, d.top);
+        if (d.top) best = merge(list_v[0], list_i[0], kCandidates, kWaves, d.top);
+    } else if (lane < d.top) {
+        best = { list.v[lane], list.i[lane] };
     }
     if (!kParts) { finish(d, row, x, token_of(d, outer, inner), a, best); return; }
     const int parts = gridDim.y;
@@ -439,8 +482,7 @@ template <class T> __global__ void __launch_bounds__(256) k_logprobs_join(ntc_lo
     Soft a = { kLowest, 0.0f, 0.0f };
     if (lane < parts) a = { all[lane * size], all[lane * size + 1], all[lane * size + 2] };
     a = join_lanes(a, k);
-    Best best;
-    best.clear();
+    Best best = { -NTC_INF, kNoIndex };
     if (d.top) best = merge(all + 4, (const int*)all + 4 + d.top, size, parts, d.top);
     finish(d, row, x, token_of(d, outer, inner), a, best);
 }
