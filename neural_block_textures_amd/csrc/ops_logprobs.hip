@@ -221,12 +221,14 @@ template <class T, int kGroup> __global__ void __launch_bounds__(256) k_logprobs
 // those before it) and the first `top` stay. Empty places of a finished list are (-inf, kNoIndex).
 constexpr int kNoIndex = 0x7fffffff, kCandidates = 64;
 struct Best { float v; int i; };
+__device__ __forceinline__ unsigned long long place_key(float w, int j) { return (unsigned long long)order_key(w) << 32 | (uint32_t)~j; }   // larger: comes first
 struct Candidates {
     float* v;
     int* i;
-    int n;                                                   // the same in all lanes
+    int n = 0, ordered = 0;                                  // the same in all lanes; the first `ordered` are in order
     __device__ __forceinline__ void put_in_order(int top) {
         const int lane = lane_id();
+        if (n == ordered) return;
         __builtin_amdgcn_wave_barrier();                     // (a wave's LDS operations are in order)
         const float w = lane < n ? v[lane] : -NTC_INF;
         const int j = lane < n ? i[lane] : kNoIndex;
@@ -242,7 +244,7 @@ struct Candidates {
         }
         __builtin_amdgcn_wave_barrier();
         if (lane < n && before < top) { v[before] = w; i[before] = j; }
-        n = n < top ? n : top;
+        n = ordered = n < top ? n : top;
         __builtin_amdgcn_wave_barrier();
     }
     // lanes of `ask` add (w, j); returns those that found no place
@@ -265,42 +267,80 @@ __device__ __forceinline__ float kth_largest(float x, int k) {
     return t <= 0x007fffffu ? -NTC_INF : key_value(t);
 }
 
-// The best of up to 64 lists in LDS (list p's values at v + p stride, indices at i + p stride): each lane holds the head of one, the
-// best head of all is taken and its lane moves on.
-__device__ __forceinline__ Best merge(const float* v, const int* i, int stride, int lists, int top) {
-    const int lane = lane_id();
-    int at = lane * stride, left = lane < lists ? top : 0;
-    float hv = left ? v[at] : -NTC_INF;
-    int hi = left ? i[at] : kNoIndex;
-    Best best = { -NTC_INF, kNoIndex };
-    for (int r = 0; r < top; r++) {
-        const float bv = reduce64(hv, [](float p, float q) { return fmaxf(p, q); });
-        const int bi = (int)reduce64((uint32_t)(hv == bv ? hi : kNoIndex), [](uint32_t p, uint32_t q) { return p < q ? p : q; });
-        if (lane == r) { best.v = bv; best.i = bi; }
-        if (hv == bv && hi == bi && left) {
-            at++;
-            left--;
-            hv = left ? v[at] : -NTC_INF;
-            hi = left ? i[at] : kNoIndex;
+// The best of up to 64 lists in LDS (list p's values at v + p stride, indices at i + p stride, in order): all lists' first, then all second ones,
+// as many ranks at a time as fit 64 lanes, until a rank has nothing that comes before the `top` values found so far. `list` is empty.
+__device__ __forceinline__ Best merge(Candidates& list, const float* v, const int* i, int stride, int lists, int top) {
+    const int lane = lane_id(), ranks = 64 / lists, p = lane % lists, r0 = lane / lists;
+    unsigned long long bar = 0;                              // (every value's key is above 0)
+    for (int r = r0; __ballot(r < top && r0 < ranks); r += ranks) {
+        const bool in = r < top && r0 < ranks;
+        const float w = in ? v[p * stride + r] : -NTC_INF;
+        const int j = in ? i[p * stride + r] : kNoIndex;
+        unsigned long long ask = __ballot(j != kNoIndex && place_key(w, j) > bar);
+        if (!ask) break;
+        while (ask) {
+            ask = list.add(ask, w, j);
+            if (list.n < kCandidates) break;
+            list.put_in_order(top);
+            bar = place_key(list.v[top - 1], list.i[top - 1]);
+            ask &= __ballot(place_key(w, j) > bar);
+        }
+        if (list.n >= top + 16) {
+            list.put_in_order(top);
+            bar = place_key(list.v[top - 1], list.i[top - 1]);
         }
     }
-    return best;
+    list.put_in_order(top);
+    return lane < list.n ? Best{ list.v[lane], list.i[lane] } : Best{ -NTC_INF, kNoIndex };
 }
 
 // What a lane reads at a time: kRun values in vectors of 16 bytes.
+// A lane's value of another lane (0 where there is none): rows of 16 shifted, or a row's last lane to those after.
+template <int kCtrl, int kRows = 0xf> __device__ __forceinline__ uint32_t before(uint32_t x) { return __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false); }
+
 template <class T> struct Long { static constexpr int kVec = 16 / (int)sizeof(T), kVecs = 2, kRun = kVec * kVecs, kChunk = 64 * kRun; };
+
+// Adds all values of a chunk that reach `least`, in ascending order of index, if the list has room for them: each lane's places
+// from a prefix sum over the lanes, of both vectors at once.
+template <int kRun> __device__ __forceinline__ bool add_run(Candidates& list, const float (&v)[kRun], float least, int base) {
+    constexpr int kVec = kRun / 2;
+    uint32_t low = 0, high = 0;
+#pragma unroll
+    for (int j = 0; j < kVec; j++) { low += v[j] >= least; high += v[kVec + j] >= least; }
+    const uint32_t own = low | high << 16;
+    uint32_t x = own;
+    x += before<0x111>(x);
+    x += before<0x112>(x);
+    x += before<0x114>(x);
+    x += before<0x118>(x);                                   // within rows of 16 lanes
+    x += before<0x142, 0xa>(x);                              // the last lane's of row 0 to row 1, of 2 to 3
+    x += before<0x143, 0xc>(x);                              // lane 31's to rows 2 and 3
+    const uint32_t total = __builtin_amdgcn_readlane(x, 63);
+    const int n = list.n + (int)(total & 0xffffu) + (int)(total >> 16);
+    if (n > kCandidates) return false;
+    x -= own;
+    int at = list.n + (int)(x & 0xffffu), at1 = list.n + (int)(total & 0xffffu) + (int)(x >> 16);
+    base += lane_id() * kVec;
+#pragma unroll
+    for (int j = 0; j < kVec; j++) if (v[j] >= least) { list.v[at] = v[j]; list.i[at++] = base + j; }
+#pragma unroll
+    for (int j = 0; j < kVec; j++) if (v[kVec + j] >= least) { list.v[at1] = v[kVec + j]; list.i[at1++] = base + 64 * kVec + j; }
+    list.n = n;
+    return true;
+}
 
 // A wave's share of a row: chunks first, first + step, .. below `end` (chunks of kChunk values, the last one ragged).
 // The sums are each lane's own, on a floor that only rises: exp2(x k - m k) is one fused operation and an exponential, with m held
 // within lim so that neither product overflows. A row whose values all lie below -lim, or reach past lim, or hold NaN ends with s = 0, infinite or
 // NaN and is read again by scan_again(). Values become candidates where their lane's largest of a chunk passes what `top` values are known to
-// reach: in the wave's own list, or in that of another wave of the row (bar: as an integer that orders; only ever raised).
+// reach: its own, or those of another wave of the row (bar: as an integer that orders; only ever raised).
+constexpr uint32_t kLowestKey = 0x00800000u;                 // kLowest as an integer that orders
 template <class T> __device__ __forceinline__ void scan(const T* x, int V, int first, int step, int end, float k, float lim, int top, Soft& a, Candidates& list, uint32_t* bar) {
     using L = Long<T>;
     const int lane = lane_id();
     a = { -lim, 0.0f, 0.0f };
     float mk = -lim * k;
-    float reach = -NTC_INF, pass = -NTC_INF;                 // candidates are >= reach and, since the list's are of earlier indices, > pass
+    float least = kLowest;                                   // the least value that a candidate may have
     bool fresh = true;
     for (int c = first; c < end; c += step) {
         float v[L::kRun];
@@ -337,32 +377,34 @@ template <class T> __device__ __forceinline__ void scan(const T* x, int V, int f
             a.t = __builtin_fmaf(e, fmaxf(d, -1e30f), a.t);
         }
         if (!top) continue;
-        if (others > 0x007fffffu) reach = fmaxf(reach, key_value(others));
-        if (fresh) reach = fmaxf(reach, kth_largest(cm, top));   // at least `top` values of the first chunk reach it
-        if (__ballot(cm >= reach && cm > pass)) {
-            bool some = false;
+        least = fmaxf(least, key_value(others > kLowestKey ? others : kLowestKey));
+        if (fresh) {
+            least = fmaxf(least, kth_largest(cm, top));      // at least `top` values of the first chunk reach it
+            if (bar && lane == 0) atomicMax(bar, order_key(least));
+        }
+        fresh = false;
+        const unsigned long long lanes = __ballot(cm >= least);
+        if (!lanes) continue;
+        if (!(__builtin_popcountll(lanes) > 4 && add_run(list, v, least, base))) {
 #pragma unroll
             for (int j = 0; j < L::kRun; j++) {
-                unsigned long long ask = __ballot(v[j] >= reach && v[j] > pass);
+                unsigned long long ask = __ballot(v[j] >= least);
                 while (ask) {
-                    some = true;
                     ask = list.add(ask, v[j], base + (j / L::kVec) * 64 * L::kVec + lane * L::kVec + j % L::kVec);
                     if (list.n == kCandidates) {
                         list.put_in_order(top);
-                        reach = fmaxf(reach, list.v[top - 1]);
-                        ask &= __ballot(v[j] >= reach);
+                        least = fmaxf(least, list.v[top - 1]);
+                        ask &= __ballot(v[j] >= least);
                     }
                 }
             }
-            if (some && (fresh || list.n >= top + 16)) {
-                list.put_in_order(top);
-                if (list.n == top) {                         // its last may only be passed, by later indices
-                    pass = fmaxf(pass, list.v[top - 1]);
-                    if (bar && lane == 0) atomicMax(bar, order_key(pass));
-                }
-            }
         }
-        fresh = false;
+        if (list.n >= top + 16) {                            // its last may only be passed, by later indices
+            list.put_in_order(top);
+            const uint32_t next = order_key(list.v[top - 1]) + 1;
+            least = fmaxf(least, key_value(next));
+            if (bar && lane == 0) atomicMax(bar, next - 1);
+        }
     }
     if (top) {
         list.put_in_order(top);
@@ -430,8 +472,9 @@ template <class T> __device__ __forceinline__ void finish(const ntc_logprobs_des
 // kWaves waves (of a block of 4) read a row; with kParts a block reads the part blockIdx.y of a row and leaves its sums and list in the workspace.
 template <class T, int kWaves, bool kParts> __global__ void __launch_bounds__(256) k_logprobs_long(ntc_logprobs_desc d, float lim, int part_chunks) {
     __shared__ Soft soft[4];
-    __shared__ float list_v[4][kCandidates];
-    __shared__ int list_i[4][kCandidates];
+    constexpr int kLists = kWaves > 1 ? 5 : 4;               // (the last: of all waves)
+    __shared__ float list_v[kLists][kCandidates];
+    __shared__ int list_i[kLists][kCandidates];
     __shared__ uint32_t bar;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id();
     const long long row = (long long)blockIdx.x * (4 / kWaves) + wave / kWaves;
@@ -446,7 +489,7 @@ template <class T, int kWaves, bool kParts> __global__ void __launch_bounds__(25
     const int V = (int)d.V, chunks = (V + Long<T>::kChunk - 1) / Long<T>::kChunk;
     const int begin = kParts ? (int)blockIdx.y * part_chunks : 0, end = kParts && begin + part_chunks < chunks ? begin + part_chunks : chunks;
     Soft a;
-    Candidates list = { list_v[wave], list_i[wave], 0 };
+    Candidates list = { list_v[wave], list_i[wave] };
     scan(x, V, begin + wave % kWaves, kWaves, end, k, lim, d.top, a, list, kWaves > 1 ? &bar : nullptr);
     a = join_lanes(a, k);
     Best best = { -NTC_INF, kNoIndex };
@@ -455,7 +498,10 @@ template <class T, int kWaves, bool kParts> __global__ void __launch_bounds__(25
         __syncthreads();
         if (wave) return;
         for (int w = 1; w < kWaves; w++) soft_join(a, soft[w], k);
-        if (d.top) best = merge(list_v[0], list_i[0], kCandidates, kWaves, d.top);
+        if (d.top) {
+            Candidates all = { list_v[kLists - 1], list_i[kLists - 1] };
+            best = merge(all, list_v[0], list_i[0], kCandidates, kWaves, d.top);
+        }
     } else if (lane < d.top) {
         best = { list.v[lane], list.i[lane] };
     }
@@ -469,7 +515,8 @@ template <class T, int kWaves, bool kParts> __global__ void __launch_bounds__(25
 // Joins a row's parts: part p's sums and list in lane p.
 constexpr int kMostParts = 64;
 template <class T> __global__ void __launch_bounds__(256) k_logprobs_join(ntc_logprobs_desc d, int parts) {
-    __shared__ float all[kMostParts * (4 + 2 * NTC_MAX_TOP)];
+    __shared__ float all[kMostParts * (4 + 2 * NTC_MAX_TOP)], list_v[kCandidates];
+    __shared__ int list_i[kCandidates];
     const long long row = blockIdx.x;
     const int lane = lane_id(), size = 4 + 2 * d.top;
     const float* from = (const float*)d.workspace + row * parts * size;
@@ -483,7 +530,8 @@ template <class T> __global__ void __launch_bounds__(256) k_logprobs_join(ntc_lo
     if (lane < parts) a = { all[lane * size], all[lane * size + 1], all[lane * size + 2] };
     a = join_lanes(a, k);
     Best best = { -NTC_INF, kNoIndex };
-    if (d.top) best = merge(all + 4, (const int*)all + 4 + d.top, size, parts, d.top);
+    Candidates list = { list_v, list_i };
+    if (d.top) best = merge(list, all + 4, (const int*)all + 4 + d.top, size, parts, d.top);
     finish(d, row, x, token_of(d, outer, inner), a, best);
 }
 
@@ -553,11 +601,15 @@ template <class T> __global__ void __launch_bounds__(256) k_logprobs_grad(ntc_lo
     }
 }
 
-// How long rows are read: waves a row, and blocks a row where there are few rows.
+// How long rows are read: waves a row, and blocks a row where there are few rows. A wave to a row puts alternatives in order once, not four
+// times, and joins nothing, but needs rows for every SIMD and leaves them unevenly done (bf16, one wave against four: 5000 x 10000 21.0 against 28.0 us,
+// with 32 alternatives 51 against 75; 16384 x 20000 129 against 149; 2500 x 30000 with 4 44.6 against 41.1; 8190 x 50001 168 against 162, with 16
+// 196 against 234; float32 with 4 4096 x 30000 89 against 96, 8192 x 50000 323 against 279; 1500 x 20000 18.8 against 14.8).
 struct Reading { int waves, parts, part_chunks; };
-template <class T> static Reading reading(int64_t rows, int64_t V) {
+template <class T> static Reading reading(int64_t rows, int64_t V, int top) {
     const int64_t chunks = (V + Long<T>::kChunk - 1) / Long<T>::kChunk;
-    Reading r = { rows >= 2048 && chunks <= 8 ? 1 : 4, 1, (int)chunks };
+    const bool one = rows >= 4096 ? chunks <= 32 || (top >= 4 && (sizeof(T) == 2 || chunks <= 64)) : rows >= 2048 && chunks <= 16;
+    Reading r = { one ? 1 : 4, 1, (int)chunks };
     if (r.waves == 4 && rows < 512 && chunks > 8) {
         int64_t parts = 1024 / rows;
         if (parts > kMostParts) parts = kMostParts;
@@ -576,7 +628,7 @@ template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s
     if (d.V <= 256) { k_logprobs_short<T, 16><<<blocks(16), 256, 0, s>>>(d, lim); return; }
     if (d.V <= 512) { k_logprobs_short<T, 32><<<blocks(8), 256, 0, s>>>(d, lim); return; }
     if (d.V <= kShort) { k_logprobs_short<T, 64><<<blocks(4), 256, 0, s>>>(d, lim); return; }
-    const Reading r = reading<T>(d.rows, d.V);
+    const Reading r = reading<T>(d.rows, d.V, d.top);
     if (r.waves == 1) k_logprobs_long<T, 1, false><<<blocks(4), 256, 0, s>>>(d, lim, 0);
     else if (r.parts == 1) k_logprobs_long<T, 4, false><<<blocks(1), 256, 0, s>>>(d, lim, 0);
     else {
@@ -586,7 +638,7 @@ template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s
 }
 template <class T> static size_t workspace(int64_t rows, int64_t V, int top) {
     if (V <= kShort) return 0;
-    const Reading r = reading<T>(rows, V);
+    const Reading r = reading<T>(rows, V, top);
     return r.parts == 1 ? 0 : (size_t)rows * r.parts * (4 + 2 * top) * 4;
 }
 template <class T> static void backward(const ntc_logprobs_desc& d, hipStream_t s) {
