@@ -262,7 +262,7 @@ template <int kBits, bool kMaster> __global__ void __launch_bounds__(kAdamTPB) k
 
 __global__ void __launch_bounds__(256) k_adamw_moments(const uint8_t* cm, const uint8_t* cv, const uint8_t* me, const uint8_t* ve, long long n, float* om,
                                                        float* ov) {
-    const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    const long long at = (block_number() * 256 + threadIdx.x) * 4;
     if (at >= n) return;
     float m[4], v[4];
     decode_block(*(const uint32_t*)(cm + at), *(const uint32_t*)(cv + at), me[at >> 8], ve[at >> 8], m, v);
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(256) k_adamw_moments(const uint8_t* cm, const 
     *(Run<float, 4>*)(ov + at) = q;
 }
 __global__ void __launch_bounds__(256) k_adamw_encode(const float* im, const float* iv, long long n, uint8_t* cm, uint8_t* cv, uint8_t* me, uint8_t* ve) {
-    const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;    // whole waves: n is a multiple of 256
+    const long long at = (block_number() * 256 + threadIdx.x) * 4;    // whole waves: n is a multiple of 256
     if (at >= n) return;
     const auto r = *(const Run<float, 4>*)(im + at), q = *(const Run<float, 4>*)(iv + at);
     float m[4], v[4];
@@ -358,13 +358,13 @@ extern "C" int ntc_op_adamw_moments(const void* cm, const void* cv, const uint8_
                                     size_t cap) {
     if (const int r = check_state(cm, cv, me, ve, m, v, n, why, cap)) return r;
     if (!n) return 0;
-    k_adamw_moments<<<(unsigned)((n + 1023) / 1024), 256, 0, (hipStream_t)stream>>>((const uint8_t*)cm, (const uint8_t*)cv, me, ve, n, m, v);
+    k_adamw_moments<<<grid_of((n + 1023) / 1024), 256, 0, (hipStream_t)stream>>>((const uint8_t*)cm, (const uint8_t*)cv, me, ve, n, m, v);
     return launched(why, cap);
 }
 
 extern "C" int ntc_op_adamw_encode(const float* m, const float* v, int64_t n, void* cm, void* cv, uint8_t* me, uint8_t* ve, void* stream, char* why, size_t cap) {
     if (const int r = check_state(cm, cv, me, ve, m, v, n, why, cap)) return r;
     if (!n) return 0;
-    k_adamw_encode<<<(unsigned)((n + 1023) / 1024), 256, 0, (hipStream_t)stream>>>(m, v, n, (uint8_t*)cm, (uint8_t*)cv, me, ve);
+    k_adamw_encode<<<grid_of((n + 1023) / 1024), 256, 0, (hipStream_t)stream>>>(m, v, n, (uint8_t*)cm, (uint8_t*)cv, me, ve);
     return launched(why, cap);
 }

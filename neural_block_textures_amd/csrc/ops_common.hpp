@@ -68,6 +68,11 @@ template <class V, class F> __device__ __forceinline__ V reduce_rows(V x, F f) {
     return f(__builtin_bit_cast(V, (uint32_t)q[0]), __builtin_bit_cast(V, (uint32_t)q[1]));
 }
 
+// ---------------------------------------------------------------- launches
+// A grid of n blocks and a block's number in it: a dimension's threads have to stay below 2^32. (Numbers may pass n.)
+inline dim3 grid_of(int64_t n) { return n <= 1 << 22 ? dim3((unsigned)n) : dim3(1u << 22, (unsigned)((n + (1 << 22) - 1) >> 22)); }
+__device__ __forceinline__ long long block_number() { return blockIdx.x + (long long)blockIdx.y * gridDim.x; }
+
 // ---------------------------------------------------------------- refusals
 inline int refuse(char* why, size_t cap, const char* text) {
     if (why && cap) snprintf(why, cap, "%s", text);

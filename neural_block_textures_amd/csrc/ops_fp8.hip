@@ -485,7 +485,7 @@ template <class A, int kM, int kN, class C> __global__ void __launch_bounds__(64
     constexpr int kAhead = kRegs > 64 ? 1 : kRegs > 32 ? 2 : 4;
     __shared__ float sums[kFewWaves][kM * kN][16][17];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const long long n0 = (long long)blockIdx.x * (16 * kN);
+    const long long n0 = block_number() * (16 * kN);
     const uint8_t *b[kN], *be[kN];
 #pragma unroll
     for (int i = 0; i < kN; i++) {
@@ -637,7 +637,7 @@ extern "C" int ntc_op_fp8_quantize(const ntc_fp8_quantize_desc* d, void* stream,
     if (d->block_rows != 1 && d->block_rows != 128) return refuse(why, cap, "blocks are 1 x 128 or 128 x 128");
     if (!d->codes && !d->codes_t) return refuse(why, cap, "nothing to write");
     const int64_t gy = (d->R + 127) / 128, gx = (d->K + 127) / 128;
-    if (gy > 65535 || gx > 0x7fffffff) return refuse(why, cap, "at most 65535 * 128 rows");
+    if (gy > 65535 || gx >= 1 << 24) return refuse(why, cap, "at most 65535 * 128 rows, and fewer than 2^31 columns");
     if (!gx || !gy) return 0;
     if (!d->x || (d->codes && !d->exps) || (d->codes_t && !d->exps_t)) return refuse(why, cap, "a null pointer");
     const auto go = [&](auto kernel) { kernel<<<dim3((unsigned)gx, (unsigned)gy), 256, 0, (hipStream_t)stream>>>(*d); };
@@ -655,8 +655,8 @@ extern "C" int64_t ntc_op_fp8_matmul_float_rows(void) { return kFloatRows; }
 
 template <class A, int kM, class C> static void launch_few(const FewArgs& F, hipStream_t s) {
     // two tiles of B a wave where that still leaves a block to each CU
-    if (F.N >= 32 * 256) k_fp8_few<A, kM, 2, C><<<(unsigned)((F.N + 31) / 32), 64 * kFewWaves, 0, s>>>(F);
-    else k_fp8_few<A, kM, 1, C><<<(unsigned)((F.N + 15) / 16), 64 * kFewWaves, 0, s>>>(F);
+    if (F.N >= 32 * 256) k_fp8_few<A, kM, 2, C><<<grid_of((F.N + 31) / 32), 64 * kFewWaves, 0, s>>>(F);
+    else k_fp8_few<A, kM, 1, C><<<grid_of((F.N + 15) / 16), 64 * kFewWaves, 0, s>>>(F);
 }
 template <class C> static void run_few(const ntc_fp8_matmul_desc* d, hipStream_t s) {
     const FewArgs F = { d->a, d->a_exps, d->b, d->b_exps, d->c, d->N, d->a_stride, d->ldc, (int)d->M, (int)d->K, (int)((d->K + 127) / 128), (int)ntc_fp8_code_stride(d->K),
@@ -708,8 +708,8 @@ extern "C" int ntc_op_fp8_matmul(const ntc_fp8_matmul_desc* d, void* stream, cha
     if (d->c_type < 0 || d->c_type > 2) return refuse(why, cap, "C is 32-bit floats, bfloat16 or float16");
     if ((d->a_block_rows != 1 && d->a_block_rows != 128) || (d->b_block_rows != 1 && d->b_block_rows != 128)) return refuse(why, cap, "blocks are 1 x 128 or 128 x 128");
     if (d->ldc < d->N) return refuse(why, cap, "C's rows overlap");
-    if (d->K > 1 << 23 || d->M > (int64_t)1 << 36 || d->N > (int64_t)1 << 36 || (d->M + 127) / 128 * ((d->N + 127) / 128) > 0x7fffffff)
-        return refuse(why, cap, "K at most 2^23, and fewer than 2^31 tiles of 128 x 128");
+    if (d->K > 1 << 23 || d->M > (int64_t)1 << 36 || d->N > (int64_t)1 << 36 || (d->M + 127) / 128 * ((d->N + 127) / 128) >= 1 << 24)
+        return refuse(why, cap, "K at most 2^23, and fewer than 2^24 tiles of 128 x 128");
     if (!d->M || !d->N) return 0;
     if (!d->K) return refuse(why, cap, "K is at least 1");
     const bool codes = d->a_type == NTC_FP8;

@@ -99,7 +99,7 @@ template <class T, int kGroup> __global__ void __launch_bounds__(256) k_logprobs
     __shared__ uint32_t keys[kRows][NTC_MAX_TOP], places[kPlaced ? kRows : 1][NTC_MAX_TOP];
     __shared__ float2 stat[kRows];
     const int in = threadIdx.x % kGroup, own = threadIdx.x / kGroup;
-    const long long first = (long long)blockIdx.x * kRows, row = first + own < d.rows ? first + own : d.rows - 1;   // past the end the last row again, not written
+    const long long first = block_number() * kRows, row = first + own < d.rows ? first + own : d.rows - 1;   // past the end the last row again, not written
     long long outer, inner;
     const T* x = row_of<T>(d, row, outer, inner);
     const int V = (int)d.V, at = in * kEach;
@@ -477,7 +477,7 @@ template <class T, int kWaves, bool kParts> __global__ void __launch_bounds__(25
     __shared__ int list_i[kLists][kCandidates];
     __shared__ uint32_t bar;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id();
-    const long long row = (long long)blockIdx.x * (4 / kWaves) + wave / kWaves;
+    const long long row = (kParts ? blockIdx.x : block_number()) * (4 / kWaves) + wave / kWaves;
     if (row >= d.rows) return;                               // (kWaves 1: a wave on its own; else whole blocks)
     if (kWaves > 1) {
         if (threadIdx.x == 0) bar = 0;
@@ -542,7 +542,7 @@ constexpr int kGradVecs = 2;
 template <class T> __global__ void __launch_bounds__(256) k_logprobs_grad(ntc_logprobs_desc d, int row_chunks) {
     constexpr int kVec = 16 / (int)sizeof(T), kChunk = 64 * kVec;
     const int lane = lane_id();
-    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), row = unit / row_chunks;
+    const long long unit = block_number() * 4 + (threadIdx.x >> 6), row = unit / row_chunks;
     if (row >= d.rows) return;
     const int V = (int)d.V, begin = (int)(unit % row_chunks) * (kGradVecs * kChunk);
     long long outer, inner;
@@ -621,7 +621,7 @@ template <class T> static Reading reading(int64_t rows, int64_t V, int top) {
 }
 
 template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s) {
-    const auto blocks = [&](int per) { return (unsigned)((d.rows + per - 1) / per); };
+    const auto blocks = [&](int per) { return grid_of((d.rows + per - 1) / per); };
     const float k = kLog2e / d.temperature, lim = 1e30f / (k > 1.0f ? k : 1.0f);   // values up to lim times k stay far from overflow
     if (d.V <= 64) { k_logprobs_short<T, 4><<<blocks(64), 256, 0, s>>>(d, lim); return; }
     if (d.V <= 128) { k_logprobs_short<T, 8><<<blocks(32), 256, 0, s>>>(d, lim); return; }
@@ -644,13 +644,13 @@ template <class T> static size_t workspace(int64_t rows, int64_t V, int top) {
 template <class T> static void backward(const ntc_logprobs_desc& d, hipStream_t s) {
     constexpr int kVec = 16 / (int)sizeof(T);
     const int64_t row_chunks = (d.V + 64 * kVec * kGradVecs - 1) / (64 * kVec * kGradVecs);
-    k_logprobs_grad<T><<<(unsigned)((d.rows * row_chunks + 3) / 4), 256, 0, s>>>(d, (int)row_chunks);
+    k_logprobs_grad<T><<<grid_of((d.rows * row_chunks + 3) / 4), 256, 0, s>>>(d, (int)row_chunks);
 }
 
 static int check(const ntc_logprobs_desc* d, bool backward, char* why, size_t cap) {
     if (!d) return refuse(why, cap, "no description");
     if (d->rows < 0 || d->V < 1 || d->inner_rows < 1) return refuse(why, cap, "rows >= 0, inner_rows >= 1 and V >= 1 are needed");
-    if (d->V > 0x7fffffff || d->rows > 0x7fffffff) return refuse(why, cap, "at most 2^31 - 1 rows and values of a row");
+    if (d->V > 0x7fff0000 || d->rows > 0x7fffffff) return refuse(why, cap, "fewer than 2^31 rows, and at most 2^31 - 2^16 values of a row");
     if (d->dtype < 0 || d->dtype > 2) return refuse(why, cap, "logits are 32-bit floats, bfloat16 or float16");
     if (d->token_bytes != 4 && d->token_bytes != 8) return refuse(why, cap, "tokens are 32- or 64-bit integers");
     if (d->top < 0 || d->top > NTC_MAX_TOP || d->top > d->V) return refuse(why, cap, "top is 0 to 32 and at most V");

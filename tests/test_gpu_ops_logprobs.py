@@ -188,6 +188,43 @@ def test_strides(V, dtype):
     check(whole.view(3, 5, 1, V + 9)[..., :V], tokens[:, :5, None], 1)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,V", [(2049, 3001), (4100, 9001), (500, 9001), (1300, 6000)])
+def test_rows_in_order_and_in_ties(N, V, dtype):
+    """Rows whose best come last, first, all at once or from few values, for one wave a row, four, and blocks a row."""
+    print("logprobs order", N, V, dtype, flush=True)
+    x, t = make(N, V, dtype, seed=V)
+    up = torch.linspace(-8, 8, V, device="cuda")
+    x[:64] = up.to(dtype)
+    x[64:128] = -up.to(dtype)
+    x[128:192] = (up * 64).round().remainder(7).to(dtype)
+    x[192:256] = 100 + x[192:256] / 64                                # (a 16-bit type has few values there)
+    x[256:300, : V // 2] = -math.inf
+    x[300:310, 40:] = -math.inf
+    x[310:320, 7:] = -math.inf                                        # fewer values than alternatives
+    x[320:330, -3:] = 50
+    for top in (1, 8, 32):
+        check(x, t, top, grad=False)
+
+
+def test_more_rows_than_threads_of_a_grid():
+    print("logprobs 2^26 rows", flush=True)
+    N, V = 2 ** 26 + 77, 2
+    x = torch.zeros((N, V), dtype=torch.float16, device="cuda")
+    t = torch.zeros(N, dtype=torch.int32, device="cuda")
+    few = torch.cat([torch.arange(50), torch.arange(N - 120, N)]).cuda()
+    src, few_t = make(len(few), V, torch.float16, seed=4)
+    x[few], t[few] = src, few_t.int()
+    x.requires_grad_(True)
+    r = ops().token_logprobs(x, t)
+    r.logprob.backward(torch.ones(N, device="cuda"))
+    one = torch.ones(len(few), device="cuda")
+    w = reference(src, few_t, 0, 1.0, -100, (one, 0 * one, torch.zeros((len(few), 0), device="cuda")))
+    close(r.logprob[few], w["logprob"], 4 * U * w["logprob"].abs() + 65 * U, "logprob")
+    close(x.grad[few], w["dx"], w["dx_err"] + w["dx"].abs() * HALF[torch.float16] * 1.01 + F16_TINY, "dx")
+    assert bool((r.logprob[50:-120] == r.logprob[50]).all()) and bool((x.grad[50:-120, 0] == 0.5).all())
+
+
 def test_rows_past_32_bit_offsets():
     print("logprobs far rows", flush=True)
     V, step = 1001, 2 ** 30 + 12345
