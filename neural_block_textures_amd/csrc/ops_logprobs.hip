@@ -44,10 +44,20 @@ template <class T> __device__ __forceinline__ const T* row_of(const ntc_logprobs
     }
     return (const T*)d.logits + outer * d.outer_stride + inner * d.inner_stride;
 }
-// The results of a row but its alternatives, from its softmax with the largest value m (kLowest or less: see none).
-template <class T> __device__ __forceinline__ void write_row(const ntc_logprobs_desc& d, long long row, const T* x, long long t, float m, float log_s, float ratio, bool none, float inv_t) {
+// Row first + own: first is the same in all lanes.
+template <class T> __device__ __forceinline__ const T* row_of(const ntc_logprobs_desc& d, long long first, int own) {
+    if (d.inner_rows < d.rows) {
+        long long outer, inner;
+        return row_of<T>(d, first + own, outer, inner);
+    }
+    return (const T*)d.logits + first * d.inner_stride + own * d.inner_stride;
+}
+// What stands at a row's token: 0 where there is none.
+template <class T> __device__ __forceinline__ float value_at(const ntc_logprobs_desc& d, const T* x, long long t) { return t != d.ignore_index && t >= 0 && t < d.V ? (float)x[t] : 0.0f; }
+// The results of a row but its alternatives, from its softmax with the largest value m (kLowest or less: see none) and the token's value.
+__device__ __forceinline__ void write_row(const ntc_logprobs_desc& d, long long row, float at_token, long long t, float m, float log_s, float ratio, bool none, float inv_t) {
     float lp = 0.0f;
-    if (t != d.ignore_index) lp = t < 0 || t >= d.V ? __builtin_nanf("") : none ? -NTC_INF : log_prob((float)x[t], m, inv_t, log_s);
+    if (t != d.ignore_index) lp = t < 0 || t >= d.V ? __builtin_nanf("") : none ? -NTC_INF : log_prob(at_token, m, inv_t, log_s);
     d.logprob[row] = lp;
     d.entropy[row] = none ? 0.0f : kLn2 * (log_s - ratio);
     d.stats[2 * row] = none ? -NTC_INF : m;
@@ -62,17 +72,34 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 __device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 
+// The same for 16-bit types, two to a word, as signed 16-bit integers: a magnitude or its negative.
+template <class T> struct Half {
+    typedef short s2 __attribute__((ext_vector_type(2)));
+    static constexpr int kInf = type_code<T> == NTC_BF16 ? 0x7f80 : 0x7c00, kNone = -0x8000;   // larger magnitudes are NaN; no value's key
+    static __device__ __forceinline__ s2 order(uint32_t w) {
+        const s2 x = __builtin_bit_cast(s2, w), sign = x >> (short)15;
+        return __builtin_bit_cast(s2, (w & 0x7fff7fffu) ^ __builtin_bit_cast(uint32_t, sign)) - sign;
+    }
+    static __device__ __forceinline__ float value(int k) {
+        const uint16_t h = (uint16_t)(k < 0 ? -k | 0x8000 : k);
+        return (float)__builtin_bit_cast(T, h);
+    }
+};
+
 __device__ __forceinline__ uint32_t above(uint32_t a, uint32_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint32_t below(uint32_t a, uint32_t b) { return a < b ? a : b; }
-// A lane's three best keys, in order (0: none). 16-bit types: the index is in the key.
+__device__ __forceinline__ int above(int a, int b) { return a > b ? a : b; }
+__device__ __forceinline__ int below(int a, int b) { return a < b ? a : b; }
+// A lane's three best keys, in order. 16-bit types: the index is in the key.
+constexpr int kNoKey = (int)0x80000000;
 struct Three {
-    uint32_t a = 0, b = 0, c = 0;
-    __device__ __forceinline__ static uint32_t middle(uint32_t x, uint32_t y, uint32_t z) { return above(below(x, y), below(above(x, y), z)); }   // one instruction
-    __device__ __forceinline__ void add(uint32_t k, uint32_t) { c = middle(b, c, k); b = middle(a, b, k); a = above(a, k); }
-    __device__ __forceinline__ void next() { a = b; b = c; c = 0; }
+    int a = kNoKey, b = kNoKey, c = kNoKey;
+    __device__ __forceinline__ static int middle(int x, int y, int z) { return above(below(x, y), below(above(x, y), z)); }   // one instruction
+    __device__ __forceinline__ void add(int k) { c = middle(b, c, k); b = middle(a, b, k); a = above(a, k); }
+    __device__ __forceinline__ void next() { a = b; b = c; c = kNoKey; }
 };
 // With the index beside the key; added in ascending order, so that the first of equals stays ahead.
-struct ThreePlaced {
+struct ThreePlaced {                                          // (0: none)
     uint32_t a = 0, b = 0, c = 0, ia = ~0u, ib = ~0u, ic = ~0u;
     __device__ __forceinline__ void add(uint32_t k, uint32_t i) {
         const bool pa = k > a, pb = k > b, pc = k > c;
@@ -87,24 +114,36 @@ struct ThreePlaced {
 };
 
 // A group of kGroup lanes holds a row in registers, 16 neighbouring values a lane: the largest, then the sums, then the alternatives one by
-// one, from the lanes' three best, through LDS to whole runs of the results. A 16-bit type's float has 13 low bits to spare, which take the
-// index (of a row of at most 1024, from the top down): one word orders values and indices both. A 32-bit value's index is found in a second
-// reduction. Bound by instructions: 262144 rows of 256 bf16 values with 4 alternatives take half again what their bytes do.
+// one, from the lanes' three best, through LDS to whole runs of the results. A 16-bit value's key is ordered two at a time and leaves half a
+// word to its index (from the top down, in a row of at most 1024): one word orders values and indices both. A 32-bit value's index is found in
+// a second reduction.
 constexpr int kShort = 1024;                                 // the longest such row
-template <class T, int kGroup> __global__ void __launch_bounds__(256) k_logprobs_short(ntc_logprobs_desc d, float lim) {
+template <class T, int kGroup> __global__ void __launch_bounds__(256) k_logprobs_short(ntc_logprobs_desc d, float lim, float k, float inv_t) {
     constexpr int kEach = 16, kVec = 16 / (int)sizeof(T), kRows = 256 / kGroup;
     constexpr bool kPlaced = sizeof(T) == 4;
-    constexpr uint32_t kMask = ~0x1fffu;
     static_assert(kGroup * kEach <= kShort, "indices of 10 bits");
+    using H = Half<T>;
+    using s2 = typename H::s2;
     __shared__ uint32_t keys[kRows][NTC_MAX_TOP], places[kPlaced ? kRows : 1][NTC_MAX_TOP];
-    __shared__ float2 stat[kRows];
+    __shared__ Soft stat[kRows];
     const int in = threadIdx.x % kGroup, own = threadIdx.x / kGroup;
-    const long long first = block_number() * kRows, row = first + own < d.rows ? first + own : d.rows - 1;   // past the end the last row again, not written
-    long long outer, inner;
-    const T* x = row_of<T>(d, row, outer, inner);
+    const long long first = block_number() * kRows;
+    if (first >= d.rows) return;
+    const int last_row = d.rows - first < kRows ? (int)(d.rows - first) - 1 : kRows - 1;   // of this block; past it the same again, not written
+    // A row's lanes have its sums, but what is written of rows is left to one lane each, once all have theirs: what it needs is asked for now.
+    long long token = 0;
+    float at_token = 0.0f;
+    const T* token_row = nullptr;
+    if ((int)threadIdx.x <= last_row) {
+        long long outer, inner;
+        token_row = row_of<T>(d, first + threadIdx.x, outer, inner);
+        token = token_of(d, outer, inner);
+    }
+    const T* x = row_of<T>(d, first, own < last_row ? own : last_row);
     const int V = (int)d.V, at = in * kEach;
-    const float inv_t = 1.0f / d.temperature, k = kLog2e / d.temperature;
     float v[kEach];
+    s2 pair[kEach / 2], least = { 0, 0 };                    // keys of 16-bit values, and the least of the whole vectors'
+    bool odd = false;                                        // an infinity or a NaN
 #pragma unroll
     for (int i = 0; i < kEach; i += kVec) {
         const int left = V - at - i;                         // of this vector's values
@@ -112,32 +151,88 @@ template <class T, int kGroup> __global__ void __launch_bounds__(256) k_logprobs
             const auto r = *(const LooseRun<T, kVec>*)(x + at + i);
 #pragma unroll
             for (int j = 0; j < kVec; j++) v[i + j] = (float)r.v[j];
-        } else if (left > 0) {
+            if constexpr (!kPlaced) {
+                const uint4 w = __builtin_bit_cast(uint4, r);
+                const uint32_t words[4] = { w.x, w.y, w.z, w.w };
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    pair[i / 2 + q] = H::order(words[q]);
+                    least = __builtin_elementwise_min(least, pair[i / 2 + q]);
+                }
+            }
+        } else {
             T r[kVec];
 #pragma unroll
-            for (int j = 0; j < kVec; j++) r[j] = x[at + i + (j < left ? j : 0)];
+            for (int j = 0; j < kVec; j++) r[j] = (T)0.0f;
+            if (left > 0)
 #pragma unroll
-            for (int j = 0; j < kVec; j++) v[i + j] = j < left ? (float)r[j] : -NTC_INF;
-        } else {
+                for (int j = 0; j < kVec; j++) r[j] = x[at + i + (j < left ? j : 0)];
 #pragma unroll
-            for (int j = 0; j < kVec; j++) v[i + j] = -NTC_INF;
+            for (int j = 0; j < kVec; j++) {
+                v[i + j] = j < left ? (float)r[j] : kPlaced ? -NTC_INF : -lim;
+                odd |= !(v[i + j] > -NTC_INF);
+            }
+            if constexpr (!kPlaced) {
+#pragma unroll
+                for (int j = 0; j < kVec; j++) {
+                    const short key = H::order((uint32_t)__builtin_bit_cast(uint16_t, r[j]))[0];
+                    pair[(i + j) / 2][j & 1] = j < left ? key : (short)H::kNone;
+                }
+            }
         }
     }
     const auto larger = [](float a, float b) { return fmaxf(a, b); };
     const auto sum = [](float a, float b) { return a + b; };
-    float m = v[0];
+    float m;
+    if constexpr (kPlaced) {
+        m = v[0];
 #pragma unroll
-    for (int j = 1; j < kEach; j++) m = fmaxf(m, v[j]);
-    m = reduce<kGroup>(m, larger);
+        for (int j = 1; j < kEach; j++) m = fmaxf(m, v[j]);
+        m = reduce<kGroup>(m, larger);
+    } else {
+        const auto most = [&] {
+            s2 p = pair[0];
+#pragma unroll
+            for (int q = 1; q < kEach / 2; q++) p = __builtin_elementwise_max(p, pair[q]);
+            return above((int)p[0], (int)p[1]);
+        };
+        int top = most();
+        odd |= top >= H::kInf || below((int)least[0], (int)least[1]) <= -H::kInf;
+        odd = __ballot(odd) != 0;
+        if (odd) {                                           // a NaN counts as -inf in the order
+            asm volatile("");                                // (a branch, not selections that every row would make)
+#pragma unroll
+            for (int q = 0; q < kEach / 2; q++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int c = pair[q][h];
+                    pair[q][h] = (short)(c > H::kInf || (c < -H::kInf && c != H::kNone) ? -H::kInf : c);
+                }
+            top = most();
+        }
+        top = reduce<kGroup>(top, [](int a, int b) { return above(a, b); });
+        m = H::value(top);
+    }
+    if (token_row) at_token = value_at(d, token_row, token);
     const float mm = m == -NTC_INF ? 0.0f : m;              // nothing left: every exponential is 0
     float s = 0.0f, t = 0.0f;
-    if (__ballot(!(fabsf(mm) <= lim)) == 0) {               // on products, which do not overflow here: one operation fewer a value
-        const float mk = mm * k, off = __builtin_fmaf(mm, k, -mk);   // (the exponents are this much too large)
+    const float mk = mm * k, off = __builtin_fmaf(mm, k, -mk);
+    // on products, which do not overflow here (one operation fewer a value than on differences); the exponents are `off` too large
+    if (__ballot(!(fabsf(mm) <= 0.5f * lim)) == 0) {
+        if (!kPlaced && !odd) {
 #pragma unroll
-        for (int j = 0; j < kEach; j++) {
-            const float q = __builtin_fmaf(v[j], k, -mk), e = fast_exp2(q);
-            s += e;
-            t = __builtin_fmaf(e, fmaxf(q, -1e30f), t);
+            for (int j = 0; j < kEach; j++) {
+                const float q = __builtin_fmaf(v[j], k, -mk), e = fast_exp2(q);
+                s += e;
+                t = __builtin_fmaf(e, q, t);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kEach; j++) {
+                const float q = __builtin_fmaf(v[j], k, -mk), e = fast_exp2(q);
+                s += e;
+                t = __builtin_fmaf(e, fmaxf(q, -1e30f), t);  // (an e of 0 may have q = -inf)
+            }
         }
         const float f = fast_exp2(-off);
         t = f * __builtin_fmaf(-s, off, t);
@@ -145,74 +240,88 @@ template <class T, int kGroup> __global__ void __launch_bounds__(256) k_logprobs
     } else {
 #pragma unroll
         for (int j = 0; j < kEach; j++) {
-            const float q = (v[j] - mm) * k, e = fast_exp2(q);
+            const float q = ((at + j < V ? v[j] : -NTC_INF) - mm) * k, e = fast_exp2(q);
             s += e;
             t = __builtin_fmaf(e, fmaxf(q, -1e30f), t);
         }
     }
     s = reduce<kGroup>(s, sum);
     t = reduce<kGroup>(t, sum);
-    const bool none = s == 0.0f;
-    const float log_s = fast_log2(s);
-    if (in == 0 && first + own < d.rows) write_row(d, row, x, token_of(d, outer, inner), mm, log_s, t / s, none, inv_t);
-    if (!d.top) return;
-    if (__ballot(s != s)) {                                  // a NaN somewhere (or +inf): in the order it counts as -inf
-#pragma unroll
-        for (int j = 0; j < kEach; j++) v[j] = v[j] != v[j] ? -NTC_INF : v[j];
-    }
-    uint32_t key[kEach];
-#pragma unroll
-    for (int j = 0; j < kEach; j++) {
-        key[j] = order_key(v[j]);
-        if constexpr (!kPlaced) key[j] = ((key[j] & kMask) | (uint32_t)(kShort - 1 - at)) - j;   // (at is a multiple of 16: no borrow)
-    }
-    if (V < kGroup * kEach) {
-        asm volatile("");                                    // (a branch, not selections that every row would make)
-#pragma unroll
-        for (int j = 0; j < kEach; j++) key[j] = at + j < V ? key[j] : 0;   // below every key of a value
-    }
-    std::conditional_t<kPlaced, ThreePlaced, Three> best;
-#pragma unroll
-    for (int j = 0; j < kEach; j++) best.add(key[j], (uint32_t)(at + j));
-    for (int r = 0; r < d.top; r++) {
-        const uint32_t last = reduce<kGroup>(best.a, above);
-        uint32_t place = 0;
-        bool took = best.a == last;
+    if (in == 0) stat[own] = { mm, s, t };
+    if (d.top) {
         if constexpr (kPlaced) {
-            place = reduce<kGroup>(took ? best.ia : ~0u, below);
-            took = took && best.ia == place;
-            if (in == 0) places[own][r] = place;
-        }
-        if (in == 0) keys[own][r] = last;
-        if (took) best.next();
-        if (__ballot(took && best.a == 0 && r + 1 < d.top)) {   // a lane has given its three: again from those that come after the last
-            asm volatile("");
-            best = {};
+            if (__ballot(s != s)) {                              // a NaN somewhere (or +inf): in the order it counts as -inf
 #pragma unroll
-            for (int j = 0; j < kEach; j++) {
-                const bool open = key[j] < last || (kPlaced && key[j] == last && (uint32_t)(at + j) > place);
-                best.add(open ? key[j] : 0, (uint32_t)(at + j));
+                for (int j = 0; j < kEach; j++) v[j] = v[j] != v[j] ? -NTC_INF : v[j];
+            }
+            uint32_t key[kEach];
+#pragma unroll
+            for (int j = 0; j < kEach; j++) key[j] = order_key(v[j]);
+            if (V < kGroup * kEach) {
+                asm volatile("");
+#pragma unroll
+                for (int j = 0; j < kEach; j++) key[j] = at + j < V ? key[j] : 0;   // below every key of a value
+            }
+            ThreePlaced best;
+#pragma unroll
+            for (int j = 0; j < kEach; j++) best.add(key[j], (uint32_t)(at + j));
+            for (int r = 0; r < d.top; r++) {
+                const uint32_t last = reduce<kGroup>(best.a, [](uint32_t a, uint32_t b) { return above(a, b); });
+                const uint32_t place = reduce<kGroup>(best.a == last ? best.ia : ~0u, [](uint32_t a, uint32_t b) { return below(a, b); });
+                const bool took = best.a == last && best.ia == place;
+                if (in == 0) { keys[own][r] = last; places[own][r] = place; }
+                if (took) best.next();
+                if (__ballot(took && best.a == 0 && r + 1 < d.top)) {   // a lane has given its three: again from those that come after the last
+                    asm volatile("");
+                    best = {};
+#pragma unroll
+                    for (int j = 0; j < kEach; j++) {
+                        const bool open = key[j] < last || (key[j] == last && (uint32_t)(at + j) > place);
+                        best.add(open ? key[j] : 0, (uint32_t)(at + j));
+                    }
+                }
+            }
+        } else {
+            // Values in the upper half, the index from the top down in the lower one: its last four bits now, the lane's once the three are known.
+            const auto key = [&](int j) { return (int)__builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, pair[j / 2]), (uint32_t)(15 - j), j & 1 ? 0x07060100u : 0x05040100u); };
+            const int lane_bits = kShort - kEach - at;
+            Three best;
+#pragma unroll
+            for (int j = 0; j < kEach; j++) best.add(key(j));
+            best.a |= lane_bits; best.b |= lane_bits; best.c |= lane_bits;
+            for (int r = 0; r < d.top; r++) {
+                const int last = reduce<kGroup>(best.a, [](int a, int b) { return above(a, b); });
+                const bool took = best.a == last;
+                if (in == 0) keys[own][r] = (uint32_t)last;
+                if (took) best.next();
+                if (__ballot(took && best.a >> 16 == H::kNone && r + 1 < d.top)) {
+                    int bits = lane_bits;
+                    asm volatile("" : "+v"(bits));               // (else the comparisons' words would be made for every row)
+                    best = {};
+#pragma unroll
+                    for (int j = 0; j < kEach; j++) best.add((key(j) | bits) < last ? key(j) : kNoKey);
+                    best.a |= lane_bits; best.b |= lane_bits; best.c |= lane_bits;
+                }
             }
         }
     }
-    if (in == 0) stat[own] = { none ? NTC_INF : mm, log_s };
-    // a wave writes what its own rows found: its lanes' LDS operations are in order
-    __builtin_amdgcn_wave_barrier();
-    const int wave_row = (threadIdx.x >> 6) * (64 / kGroup);
-    for (int e = lane_id(); e < 64 / kGroup * d.top; e += 64) {
-        const int rl = wave_row + e / d.top, r = e % d.top;
-        if (first + rl >= d.rows) break;
-        uint32_t found = keys[rl][r], place = 0;
-        if constexpr (kPlaced) place = places[rl][r];
-        else {
-            place = kShort - 1 - (found & (kShort - 1));
-            found = found & 0x80000000u ? found & kMask : found | ~kMask;
-        }
-        const float2 st = stat[rl];
-        const long long to = (first + rl) * d.top + r;
-        d.top_ids[to] = place;
-        // (a NaN in the row has made log_s NaN, which swallows what stands for it here)
-        d.top_logprobs[to] = st.x == NTC_INF && !(st.y != st.y) ? -NTC_INF : log_prob(key_value(found), st.x, inv_t, st.y);
+    __syncthreads();
+    if ((int)threadIdx.x <= last_row) {
+        const Soft a = stat[threadIdx.x];
+        write_row(d, first + threadIdx.x, at_token, token, a.m, fast_log2(a.s), a.t * __builtin_amdgcn_rcpf(a.s), a.s == 0.0f, inv_t);
+    }
+    // alternatives by the other waves first
+    for (int e = threadIdx.x ^ 192; e < (last_row + 1) * d.top; e += 256) {
+        const int own = e / d.top, r = e % d.top;
+        const uint32_t found = keys[own][r];
+        uint32_t place;
+        float w;
+        if constexpr (kPlaced) { place = places[own][r]; w = key_value(found); }
+        else { place = kShort - 1 - (found & (kShort - 1)); w = H::value((int)found >> 16); }
+        const Soft a = stat[own];
+        d.top_ids[first * d.top + e] = place;
+        // (a NaN in the row has made the sum NaN, which swallows what stands for it here)
+        d.top_logprobs[first * d.top + e] = a.s == 0.0f ? -NTC_INF : log_prob(w, a.m, inv_t, fast_log2(a.s));
     }
 }
 
@@ -450,7 +559,7 @@ template <class T> __device__ __forceinline__ void finish(const ntc_logprobs_des
     if (!plain_sum(a.s)) a = scan_again(x, V, k);
     const bool none = a.s == 0.0f;
     const float log_s = fast_log2(a.s);
-    if (lane == 0) write_row(d, row, x, t, a.m, log_s, a.t / a.s, none, inv_t);
+    if (lane == 0) write_row(d, row, value_at(d, x, t), t, a.m, log_s, a.t / a.s, none, inv_t);
     if (!d.top) return;
     int have = __builtin_popcountll(__ballot(lane < d.top && best.i != kNoIndex));
     for (int i = 0; have < d.top && i < V; i += 64) {
@@ -623,11 +732,11 @@ template <class T> static Reading reading(int64_t rows, int64_t V, int top) {
 template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s) {
     const auto blocks = [&](int per) { return grid_of((d.rows + per - 1) / per); };
     const float k = kLog2e / d.temperature, lim = 1e30f / (k > 1.0f ? k : 1.0f);   // values up to lim times k stay far from overflow
-    if (d.V <= 64) { k_logprobs_short<T, 4><<<blocks(64), 256, 0, s>>>(d, lim); return; }
-    if (d.V <= 128) { k_logprobs_short<T, 8><<<blocks(32), 256, 0, s>>>(d, lim); return; }
-    if (d.V <= 256) { k_logprobs_short<T, 16><<<blocks(16), 256, 0, s>>>(d, lim); return; }
-    if (d.V <= 512) { k_logprobs_short<T, 32><<<blocks(8), 256, 0, s>>>(d, lim); return; }
-    if (d.V <= kShort) { k_logprobs_short<T, 64><<<blocks(4), 256, 0, s>>>(d, lim); return; }
+    if (d.V <= 64) { k_logprobs_short<T, 4><<<blocks(64), 256, 0, s>>>(d, lim, k, 1.0f / d.temperature); return; }
+    if (d.V <= 128) { k_logprobs_short<T, 8><<<blocks(32), 256, 0, s>>>(d, lim, k, 1.0f / d.temperature); return; }
+    if (d.V <= 256) { k_logprobs_short<T, 16><<<blocks(16), 256, 0, s>>>(d, lim, k, 1.0f / d.temperature); return; }
+    if (d.V <= 512) { k_logprobs_short<T, 32><<<blocks(8), 256, 0, s>>>(d, lim, k, 1.0f / d.temperature); return; }
+    if (d.V <= kShort) { k_logprobs_short<T, 64><<<blocks(4), 256, 0, s>>>(d, lim, k, 1.0f / d.temperature); return; }
     const Reading r = reading<T>(d.rows, d.V, d.top);
     if (r.waves == 1) k_logprobs_long<T, 1, false><<<blocks(4), 256, 0, s>>>(d, lim, 0);
     else if (r.parts == 1) k_logprobs_long<T, 4, false><<<blocks(1), 256, 0, s>>>(d, lim, 0);
