@@ -7,14 +7,14 @@
 namespace ntc_ops {
 
 constexpr int kAdamTPB = 256, kLane = 4, kWaveBlocks = 4;    // a wave's 4 blocks of 256 values, 4 a lane
-constexpr int kBatch = 160;                                   // tensors of one launch: their gradients travel as arguments
+constexpr int kBatch = 400, kRates = 16;                      // tensors of one launch, and different steps among them: gradients travel as arguments (of at most 4 KiB)
 constexpr uint32_t kNsAdam = 5;                               // stream of the counter noise (1 to 4: the ES trainer's)
 static_assert(kAdamTPB / 64 * kWaveBlocks * NTC_STATE_BLOCK == NTC_ADAMW_CHUNK, "a block of threads is a chunk");
 
 struct AdamGrads {
     const void* g[kBatch];
-    float rate[kBatch], root[kBatch];        // lr / (1 - b1^c), 1 / sqrt(1 - b2^c)
-    uint8_t type[kBatch];
+    float rate[kRates], root[kRates];        // lr / (1 - b1^c), 1 / sqrt(1 - b2^c)
+    uint8_t kind[kBatch];                    // the gradient's type, and 4 times its place among the rates
 };
 struct AdamArgs {
     const ntc_adamw_tensor* tensors;
@@ -27,40 +27,28 @@ struct AdamArgs {
     float b1, nb1, b2, nb2, eps, keep;
     uint64_t head;
 };
+static_assert(sizeof(AdamGrads) + sizeof(AdamArgs) <= 4096, "arguments of a launch");
 
 // Four values from position i of a buffer of type `type` (uniform over the block) as floats: whole runs where all four are
-// there and aligned, else one by one; 0 past the end.
-__device__ __forceinline__ void load4(float (&o)[4], const void* p, int type, long long i, long long n, bool aligned) {
-    if (type == NTC_F32) {
-        const float* q = (const float*)p + i;
-        if (aligned && i + 4 <= n) { const auto r = *(const Run<float, 4>*)q; for (int j = 0; j < 4; j++) o[j] = r.v[j]; }
-        else for (int j = 0; j < 4; j++) o[j] = i + j < n ? q[j] : 0.0f;
-    } else if (type == NTC_BF16) {
-        const bf16* q = (const bf16*)p + i;
-        if (aligned && i + 4 <= n) { const auto r = *(const Run<bf16, 4>*)q; for (int j = 0; j < 4; j++) o[j] = (float)r.v[j]; }
-        else for (int j = 0; j < 4; j++) o[j] = i + j < n ? (float)q[j] : 0.0f;
-    } else {
-        const f16* q = (const f16*)p + i;
-        if (aligned && i + 4 <= n) { const auto r = *(const Run<f16, 4>*)q; for (int j = 0; j < 4; j++) o[j] = (float)r.v[j]; }
-        else for (int j = 0; j < 4; j++) o[j] = i + j < n ? (float)q[j] : 0.0f;
-    }
+// there, else one by one; 0 past the end.
+template <class T> __device__ __forceinline__ void load4_of(float (&o)[4], const T* q, long long left) {
+    if (left >= 4) { const auto r = *(const LooseRun<T, 4>*)q; for (int j = 0; j < 4; j++) o[j] = (float)r.v[j]; }
+    else for (int j = 0; j < 4; j++) o[j] = j < left ? (float)q[j] : 0.0f;
 }
-__device__ __forceinline__ void store4(const float (&o)[4], void* p, int type, long long i, long long n, bool aligned) {
-    if (type == NTC_F32) {
-        float* q = (float*)p + i;
-        if (aligned && i + 4 <= n) { Run<float, 4> r; for (int j = 0; j < 4; j++) r.v[j] = o[j]; *(Run<float, 4>*)q = r; }
-        else for (int j = 0; j < 4; j++) if (i + j < n) q[j] = o[j];
-    } else if (type == NTC_BF16) {
-        bf16* q = (bf16*)p + i;
-        if (aligned && i + 4 <= n) { Run<bf16, 4> r; for (int j = 0; j < 4; j++) r.v[j] = (bf16)o[j]; *(Run<bf16, 4>*)q = r; }
-        else for (int j = 0; j < 4; j++) if (i + j < n) q[j] = (bf16)o[j];
-    } else {
-        f16* q = (f16*)p + i;
-        if (aligned && i + 4 <= n) { Run<f16, 4> r; for (int j = 0; j < 4; j++) r.v[j] = (f16)o[j]; *(Run<f16, 4>*)q = r; }
-        else for (int j = 0; j < 4; j++) if (i + j < n) q[j] = (f16)o[j];
-    }
+template <class T> __device__ __forceinline__ void store4_of(const float (&o)[4], T* q, long long left) {
+    if (left >= 4) { LooseRun<T, 4> r; for (int j = 0; j < 4; j++) r.v[j] = (T)o[j]; *(LooseRun<T, 4>*)q = r; }
+    else for (int j = 0; j < 4; j++) if (j < left) q[j] = (T)o[j];
 }
-__device__ __forceinline__ bool aligned4(const void* p, int type) { return ((uintptr_t)p & (type == NTC_F32 ? 15 : 7)) == 0; }
+__device__ __forceinline__ void load4(float (&o)[4], const void* p, int type, long long i, long long n) {
+    if (type == NTC_F32) load4_of(o, (const float*)p + i, n - i);
+    else if (type == NTC_BF16) load4_of(o, (const bf16*)p + i, n - i);
+    else load4_of(o, (const f16*)p + i, n - i);
+}
+__device__ __forceinline__ void store4(const float (&o)[4], void* p, int type, long long i, long long n) {
+    if (type == NTC_F32) store4_of(o, (float*)p + i, n - i);
+    else if (type == NTC_BF16) store4_of(o, (bf16*)p + i, n - i);
+    else store4_of(o, (f16*)p + i, n - i);
+}
 
 // 2^(b - 127), b from 0 to 254
 __device__ __forceinline__ float power_of(int b) { return __uint_as_float(b > 0 ? (uint32_t)b << 23 : 1u << 22); }
@@ -135,27 +123,32 @@ __device__ __forceinline__ void random16(uint64_t at, uint32_t (&rm)[4], uint32_
     }
 }
 
-// A wave's blocks of a chunk that lies whole in its tensor and on aligned addresses: everything is read first, so that the memory has
-// four blocks' requests at once; kG32, kP32: the gradient and the tensor are 32-bit.
+// A wave's blocks that lie whole in its tensor (all four, or `count`): everything is read first, so that the memory has four blocks' requests at
+// once; kG32, kP32: the gradient and the tensor are 32-bit. They may lie at any element's address.
+template <class R, int kSize> struct __attribute__((packed, aligned(kSize))) Loose { R v; };
 struct __attribute__((packed)) LooseWord { uint32_t v; };
-template <bool k32> struct Raw { using type = std::conditional_t<k32, uint4, uint2>; };
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <bool k32> struct Raw { using type = std::conditional_t<k32, u32x4, u32x2>; };
 template <bool k32> __device__ __forceinline__ void widen(float (&o)[4], const typename Raw<k32>::type& r, int type) {
     if constexpr (k32) { const auto f = __builtin_bit_cast(Run<float, 4>, r); for (int j = 0; j < 4; j++) o[j] = f.v[j]; }
     else if (type == NTC_BF16) { const auto f = __builtin_bit_cast(Run<bf16, 4>, r); for (int j = 0; j < 4; j++) o[j] = (float)f.v[j]; }
     else { const auto f = __builtin_bit_cast(Run<f16, 4>, r); for (int j = 0; j < 4; j++) o[j] = (float)f.v[j]; }
 }
 template <bool k32> __device__ __forceinline__ typename Raw<k32>::type narrow(const float (&p)[4], int type) {
-    if constexpr (k32) { Run<float, 4> f; for (int j = 0; j < 4; j++) f.v[j] = p[j]; return __builtin_bit_cast(uint4, f); }
-    else if (type == NTC_BF16) { Run<bf16, 4> f; for (int j = 0; j < 4; j++) f.v[j] = (bf16)p[j]; return __builtin_bit_cast(uint2, f); }
-    else { Run<f16, 4> f; for (int j = 0; j < 4; j++) f.v[j] = (f16)p[j]; return __builtin_bit_cast(uint2, f); }
+    if constexpr (k32) { Run<float, 4> f; for (int j = 0; j < 4; j++) f.v[j] = p[j]; return __builtin_bit_cast(u32x4, f); }
+    else if (type == NTC_BF16) { Run<bf16, 4> f; for (int j = 0; j < 4; j++) f.v[j] = (bf16)p[j]; return __builtin_bit_cast(u32x2, f); }
+    else { Run<f16, 4> f; for (int j = 0; j < 4; j++) f.v[j] = (f16)p[j]; return __builtin_bit_cast(u32x2, f); }
 }
-template <int kBits, bool kMaster, bool kG32, bool kP32> __device__ __forceinline__ void whole_chunk(const AdamArgs& A, const ntc_adamw_tensor& T, const void* g_ptr, int gt, float rate,
-                                                                                                     float root, long long i0) {
+template <int kBits, bool kMaster, bool kG32, bool kP32, bool kAll> __device__ __forceinline__ void whole_blocks(const AdamArgs& A, const ntc_adamw_tensor& T, const void* g_ptr, int gt, float rate,
+                                                                                                                 float root, long long i0, int count) {
     using GR = typename Raw<kG32>::type;
     using PR = typename Raw<kP32>::type;
+    using GL = Loose<GR, kG32 ? 4 : 2>;
+    using PL = Loose<PR, kP32 ? 4 : 2>;
     using SR = std::conditional_t<kBits == 8, uint32_t, float4>;
-    const GR* gp = (const GR*)((const uint8_t*)g_ptr + i0 * (kG32 ? 4 : 2));
-    PR* pp = (PR*)((uint8_t*)T.param + i0 * (kP32 ? 4 : 2));
+    const GL* gp = (const GL*)((const uint8_t*)g_ptr + i0 * (kG32 ? 4 : 2));
+    PL* pp = (PL*)((uint8_t*)T.param + i0 * (kP32 ? 4 : 2));
     const long long at = T.state_offset + i0;
     SR* mp = (SR*)((uint8_t*)A.m + at * (kBits / 8));
     SR* vp = (SR*)((uint8_t*)A.v + at * (kBits / 8));
@@ -167,20 +160,26 @@ template <int kBits, bool kMaster, bool kG32, bool kP32> __device__ __forceinlin
     uint32_t me = 0, ve = 0;
 #pragma unroll
     for (int u = 0; u < kWaveBlocks; u++) {
-        g[u] = gp[64 * u];
+        if (!kAll && u >= count) break;
+        g[u] = gp[64 * u].v;
         if (kMaster) w[u] = wp[64 * u];
-        else p[u] = pp[64 * u];
+        else p[u] = pp[64 * u].v;
         m[u] = mp[64 * u];
         v[u] = vp[64 * u];
     }
-    if constexpr (kBits == 8) {                              // a wave's four blocks' exponents are a word, at any byte
+    if constexpr (kBits == 8 && kAll) {                      // a wave's four blocks' exponents are a word, at any byte
         me = __builtin_amdgcn_readfirstlane(((const LooseWord*)(A.me + (at >> 8)))->v);
         ve = __builtin_amdgcn_readfirstlane(((const LooseWord*)(A.ve + (at >> 8)))->v);
+    } else if constexpr (kBits == 8) {
+        const int lane = threadIdx.x & 63;                   // lane u the exponents of block u
+        const uint32_t em = lane < count ? A.me[(at >> 8) + lane] : 0, ev = lane < count ? A.ve[(at >> 8) + lane] : 0;
+        for (int u = 0; u < kWaveBlocks; u++) { me |= __builtin_amdgcn_readlane(em, u) << (8 * u); ve |= __builtin_amdgcn_readlane(ev, u) << (8 * u); }
     }
     uint32_t new_me = 0, new_ve = 0;
     uint64_t noise = A.head + (uint64_t)(at >> 1) * ntc_hip::kPhi64;
 #pragma unroll
     for (int u = 0; u < kWaveBlocks; u++) {
+        if (!kAll && u >= count) break;
         float gf[4], pf[4], mf[4], vf[4];
         widen<kG32>(gf, g[u], gt);
         if (kMaster) { pf[0] = w[u].x; pf[1] = w[u].y; pf[2] = w[u].z; pf[3] = w[u].w; }
@@ -201,9 +200,15 @@ template <int kBits, bool kMaster, bool kG32, bool kP32> __device__ __forceinlin
             vp[64 * u] = float4{ vf[0], vf[1], vf[2], vf[3] };
         }
         if (kMaster) wp[64 * u] = float4{ pf[0], pf[1], pf[2], pf[3] };
-        pp[64 * u] = narrow<kP32>(pf, T.param_type);
+        pp[64 * u].v = narrow<kP32>(pf, T.param_type);
     }
-    if (kBits == 8 && (threadIdx.x & 63) == 0) {
+    if (kBits == 8 && !kAll) {
+        const int lane = threadIdx.x & 63;
+        if (lane < count) {
+            A.me[(at >> 8) + lane] = (uint8_t)(new_me >> (8 * lane));
+            A.ve[(at >> 8) + lane] = (uint8_t)(new_ve >> (8 * lane));
+        }
+    } else if (kBits == 8 && (threadIdx.x & 63) == 0) {
         ((LooseWord*)(A.me + (at >> 8)))->v = new_me;
         ((LooseWord*)(A.ve + (at >> 8)))->v = new_ve;
     }
@@ -216,25 +221,25 @@ template <int kBits, bool kMaster> __global__ void __launch_bounds__(kAdamTPB) k
     const void* g_ptr = G.g[gi];
     if (!g_ptr) return;
     const ntc_adamw_tensor T = A.tensors[ti];
-    const float rate = G.rate[gi], root = G.root[gi];
-    const int gt = G.type[gi];
-    const bool g_al = aligned4(g_ptr, gt), p_al = aligned4(T.param, T.param_type);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const long long base = (chunk - T.first_chunk) * NTC_ADAMW_CHUNK + wave * (kWaveBlocks * NTC_STATE_BLOCK) + lane * kLane;
-    if ((chunk - T.first_chunk + 1) * NTC_ADAMW_CHUNK <= T.numel && g_al && p_al) {
-        const bool g32 = gt == NTC_F32, p32 = T.param_type == NTC_F32;
-        if (g32) p32 ? whole_chunk<kBits, kMaster, true, true>(A, T, g_ptr, gt, rate, root, base) : whole_chunk<kBits, kMaster, true, false>(A, T, g_ptr, gt, rate, root, base);
-        else p32 ? whole_chunk<kBits, kMaster, false, true>(A, T, g_ptr, gt, rate, root, base) : whole_chunk<kBits, kMaster, false, false>(A, T, g_ptr, gt, rate, root, base);
-        return;
-    }
-#pragma unroll 1
-    for (int u = 0; u < kWaveBlocks; u++) {
-        const long long i = base + u * NTC_STATE_BLOCK, at = T.state_offset + i;
-        if (i - lane * kLane >= T.numel) break;              // the whole block lies past the end
+    const int kind = G.kind[gi], gt = kind & 3;
+    const float rate = G.rate[kind >> 2], root = G.root[kind >> 2];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const long long wave_base = (chunk - T.first_chunk) * NTC_ADAMW_CHUNK + wave * (kWaveBlocks * NTC_STATE_BLOCK), base = wave_base + lane * kLane;
+    const long long blocks = (T.numel - wave_base) >> 8;     // whole ones from here on
+    const bool g32 = gt == NTC_F32, p32 = T.param_type == NTC_F32;
+    const auto whole = [&](auto all, int count) {
+        if (g32) p32 ? whole_blocks<kBits, kMaster, true, true, all.value>(A, T, g_ptr, gt, rate, root, base, count) : whole_blocks<kBits, kMaster, true, false, all.value>(A, T, g_ptr, gt, rate, root, base, count);
+        else p32 ? whole_blocks<kBits, kMaster, false, true, all.value>(A, T, g_ptr, gt, rate, root, base, count) : whole_blocks<kBits, kMaster, false, false, all.value>(A, T, g_ptr, gt, rate, root, base, count);
+    };
+    if (blocks >= kWaveBlocks) { whole(std::true_type(), kWaveBlocks); return; }
+    if (blocks > 0) whole(std::false_type(), (int)blocks);
+    // the tensor's last, ragged block
+    const long long i = base + (blocks > 0 ? blocks : 0) * NTC_STATE_BLOCK, at = T.state_offset + i;
+    if (i - lane * kLane < T.numel) {
         float g[4], p[4], m[4], v[4];
-        load4(g, g_ptr, gt, i, T.numel, g_al);
+        load4(g, g_ptr, gt, i, T.numel);
         if (kMaster) { const auto r = *(const Run<float, 4>*)(A.master + at); for (int j = 0; j < 4; j++) p[j] = r.v[j]; }
-        else load4(p, T.param, T.param_type, i, T.numel, p_al);
+        else load4(p, T.param, T.param_type, i, T.numel);
         if (kBits == 8) {
             decode_block(*(const uint32_t*)((const uint8_t*)A.m + at), *(const uint32_t*)((const uint8_t*)A.v + at), A.me[at >> 8], A.ve[at >> 8], m, v);
         } else {
@@ -256,7 +261,7 @@ template <int kBits, bool kMaster> __global__ void __launch_bounds__(kAdamTPB) k
             *(Run<float, 4>*)((float*)A.v + at) = q;
         }
         if (kMaster) { Run<float, 4> r; for (int j = 0; j < 4; j++) r.v[j] = p[j]; *(Run<float, 4>*)(A.master + at) = r; }
-        store4(p, T.param, T.param_type, i, T.numel, p_al);
+        store4(p, T.param, T.param_type, i, T.numel);
     }
 }
 
@@ -318,23 +323,26 @@ extern "C" int ntc_op_adamw(const ntc_adamw_desc* d, void* stream, char* why, si
     A.eps = (float)d->eps;
     A.keep = (float)(1.0 - d->lr * d->weight_decay);
     A.head = ntc_hip::noise_head(d->seed, kNsAdam, d->calls, 0);
-    int32_t last = -1;
-    float rate = 0, root = 0;
-    for (int64_t t0 = 0; t0 < d->n; t0 += kBatch) {
-        const int64_t t1 = t0 + kBatch < d->n ? t0 + kBatch : d->n;
+    for (int64_t t0 = 0, t1; t0 < d->n; t0 = t1) {
         AdamGrads G;
+        int32_t steps[kRates];
+        int rates = 0;
         bool any = false;
-        for (int64_t t = t0; t < t1; t++) {
-            if (d->grads[t] && d->steps[t] != last) {     // (nearly always all tensors are at the same step)
-                last = d->steps[t];
-                rate = (float)(d->lr / (1.0 - pow(d->beta1, last)));
-                root = (float)(1.0 / sqrt(1.0 - pow(d->beta2, last)));
+        for (t1 = t0; t1 < d->n && t1 - t0 < kBatch; t1++) {
+            int r = 0;
+            if (d->grads[t1]) {                           // (nearly always all tensors are at the same step)
+                while (r < rates && steps[r] != d->steps[t1]) r++;
+                if (r == kRates) break;
+                if (r == rates) {
+                    steps[r] = d->steps[t1];
+                    G.rate[r] = (float)(d->lr / (1.0 - pow(d->beta1, steps[r])));
+                    G.root[r] = (float)(1.0 / sqrt(1.0 - pow(d->beta2, steps[r])));
+                    rates++;
+                }
+                any = true;
             }
-            G.g[t - t0] = d->grads[t];
-            G.rate[t - t0] = rate;
-            G.root[t - t0] = root;
-            G.type[t - t0] = (uint8_t)d->grad_types[t];
-            any |= d->grads[t] != nullptr;
+            G.g[t1 - t0] = d->grads[t1];
+            G.kind[t1 - t0] = (uint8_t)(d->grad_types[t1] | r << 2);
         }
         const int64_t blocks = d->first_chunk[t1] - d->first_chunk[t0];
         if (!any || !blocks) continue;

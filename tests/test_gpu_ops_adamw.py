@@ -103,6 +103,25 @@ def test_more_tensors_than_a_launch_takes():
     assert opt.steps[3] == 0 and opt.steps[4] == 1
 
 
+def test_tensors_at_many_different_steps():
+    sizes = [(k * 53) % 700 + 1 for k in range(120)]
+    params = tensors(sizes, torch.float32, 1)
+    opt = ops().AdamW(params, **HYPER)
+    zero = torch.zeros(1, device="cuda")
+    state = opt.state_dict()
+    state["step"] = [3 * (k % 23) for k in range(len(sizes))]      # (more of them than a launch takes)
+    opt.load_state_dict(state)
+    p0, grads = [p.clone() for p in params], tensors(sizes, torch.float32, 2)
+    grads[0] = grads[50] = None
+    opt.step(grads)
+    for k, (p, q, g) in enumerate(zip(params, p0, grads)):
+        if g is None:
+            assert torch.equal(p, q)
+            continue
+        w, _, _, up = step64(q, g, zero, zero, 3 * (k % 23) + 1, **HYPER)
+        near(p, w, up.abs() * 12 * U + 3 * U * q.abs().double(), k)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_a_tensor_without_gradient_keeps_its_state_and_step(bits):
     params = tensors([300, 700], torch.float32, 1)
