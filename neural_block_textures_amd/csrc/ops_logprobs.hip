@@ -64,6 +64,23 @@ __device__ __forceinline__ void write_row(const ntc_logprobs_desc& d, long long 
     d.stats[2 * row + 1] = log_s;
 }
 
+// Sixteen bytes of a row at its ragged end: the `left` values (fewer than a run) from x[at] on, zeros after them, and their store.
+typedef unsigned __int128 Bits;
+template <class T> __device__ __forceinline__ Bits last_run(const T* x, int V, int at, int left) {
+    constexpr int kVec = 16 / (int)sizeof(T);
+    if (V >= kVec) return __builtin_bit_cast(Bits, *(const LooseRun<T, kVec>*)(x + V - kVec)) >> (8 * (int)sizeof(T) * (kVec - left));
+    LooseRun<T, kVec> r = {};
+    for (int j = 0; j < kVec; j++) if (j < left) r.v[j] = x[at + j];
+    return __builtin_bit_cast(Bits, r);
+}
+template <class T> __device__ __forceinline__ void store_last(T* to, Bits w, int left) {
+    uint8_t* p = (uint8_t*)to;
+    const int bytes = left * (int)sizeof(T);
+    if (bytes & 8) { *(LooseRun<uint16_t, 4>*)p = __builtin_bit_cast(LooseRun<uint16_t, 4>, (uint64_t)w); p += 8; w >>= 64; }
+    if (bytes & 4) { *(LooseRun<uint16_t, 2>*)p = __builtin_bit_cast(LooseRun<uint16_t, 2>, (uint32_t)w); p += 4; w >>= 32; }
+    if (bytes & 2) *(uint16_t*)p = (uint16_t)w;
+}
+
 // ---------------------------------------------------------------- short rows
 // Integers that order as floats do (-0 as 0), and back.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -177,16 +194,9 @@ template <class T, int kGroup, bool kSorted> __global__ void __launch_bounds__(2
                 }
             }
         } else {
-            typedef unsigned __int128 Bits;
             Bits w = 0, inside = 0;                          // this lane's values, and ones where there are any
-            if (left > 0 && V >= kVec) {                     // from the row's last whole vector
-                const int past = 8 * (int)sizeof(T) * (kVec - left);
-                w = __builtin_bit_cast(Bits, *(const LooseRun<T, kVec>*)(x + V - kVec)) >> past;
-                inside = ~(Bits)0 >> past;
-            } else if (left > 0) {
-                LooseRun<T, kVec> r = {};
-                for (int j = 0; j < kVec; j++) if (j < left) r.v[j] = x[at + i + j];
-                w = __builtin_bit_cast(Bits, r);
+            if (left > 0) {
+                w = last_run(x, V, at + i, left);
                 inside = ~(Bits)0 >> (8 * (int)sizeof(T) * (kVec - left));
             }
             const auto r = __builtin_bit_cast(LooseRun<T, kVec>, w);
@@ -524,9 +534,15 @@ template <class T> __device__ __forceinline__ void scan(const T* x, int V, int f
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < L::kVecs; i++)
+            for (int i = 0; i < L::kVecs; i++) {
+                const int at = at0 + i * 64 * L::kVec, left = V - at;
+                Bits w = 0;
+                if (left >= L::kVec) w = __builtin_bit_cast(Bits, *(const LooseRun<T, L::kVec>*)(x + at));
+                else if (left > 0) w = last_run(x, V, at, left);
+                const auto r = __builtin_bit_cast(LooseRun<T, L::kVec>, w);
 #pragma unroll
-                for (int j = 0; j < L::kVec; j++) { const int p = at0 + i * 64 * L::kVec + j; v[i * L::kVec + j] = p < V ? (float)x[p] : -NTC_INF; }
+                for (int j = 0; j < L::kVec; j++) v[i * L::kVec + j] = j < left ? (float)r.v[j] : -NTC_INF;
+            }
         }
         float cm = v[0];
 #pragma unroll
@@ -744,7 +760,7 @@ template <class T> __global__ void __launch_bounds__(256) k_logprobs_grad(ntc_lo
         T r[kVec];
         const bool full = at + kVec <= V;
         if (full) { const auto q = *(const LooseRun<T, kVec>*)(x + at); for (int j = 0; j < kVec; j++) r[j] = q.v[j]; }
-        else for (int j = 0; j < kVec; j++) r[j] = at + j < V ? x[at + j] : (T)0.0f;
+        else { const auto q = __builtin_bit_cast(LooseRun<T, kVec>, at < V ? last_run(x, V, at, V - at) : (Bits)0); for (int j = 0; j < kVec; j++) r[j] = q.v[j]; }
         float g[kVec];
 #pragma unroll
         for (int j = 0; j < kVec; j++) {
@@ -765,20 +781,93 @@ template <class T> __global__ void __launch_bounds__(256) k_logprobs_grad(ntc_lo
 #pragma unroll
         for (int j = 0; j < kVec; j++) o.v[j] = (T)(none ? 0.0f : g[j]);
         if (full) *(LooseRun<T, kVec>*)(dx + at) = o;
-        else for (int j = 0; j < kVec; j++) if (at + j < V) dx[at + j] = o.v[j];
+        else if (at < V) store_last(dx + at, __builtin_bit_cast(Bits, o), V - at);
+    }
+}
+
+// Short rows: a group of kGroup lanes holds a row, 16 values a lane, as forward. The places that get more are a lane's each, and are added
+// where the group has laid its gradients in LDS.
+template <class T, int kGroup> __global__ void __launch_bounds__(256) k_logprobs_grad_short(ntc_logprobs_desc d, float k, float inv_t) {
+    constexpr int kEach = 16, kVec = 16 / (int)sizeof(T), kRows = 256 / kGroup;
+    __shared__ float4 laid[kEach / 4][256];
+    const int in = threadIdx.x % kGroup, own = threadIdx.x / kGroup;
+    const long long first = block_number() * kRows;
+    if (first >= d.rows) return;
+    const long long row = first + own < d.rows ? first + own : d.rows - 1;   // past the end the last row again, not written
+    const int V = (int)d.V, at = in * kEach;
+    long long outer, inner;
+    const T* x = row_of<T>(d, row, outer, inner);
+    LooseRun<T, kVec> r[kEach / kVec];
+#pragma unroll
+    for (int i = 0; i < kEach / kVec; i++) {
+        const int left = V - at - i * kVec;
+        r[i] = {};
+        if (left >= kVec) r[i] = *(const LooseRun<T, kVec>*)(x + at + i * kVec);
+        else if (left > 0) r[i] = __builtin_bit_cast(LooseRun<T, kVec>, last_run(x, V, at + i * kVec, left));
+    }
+    const float m = d.stats[2 * row], log_s = d.stats[2 * row + 1], H = d.entropy[row];
+    const long long t = token_of(d, outer, inner);
+    const bool none = m == -NTC_INF, ignored = t == d.ignore_index, out = !ignored && (t < 0 || t >= d.V);
+    const float glp = d.g_logprob && !ignored ? d.g_logprob[row] : 0.0f;
+    const float gh = d.g_entropy ? d.g_entropy[row] : 0.0f;
+    const int tops = d.g_top ? d.top : 0;
+    float all = 0.0f;
+    for (int e = in; e < tops; e += kGroup) all += d.g_top[row * d.top + e];
+    all = reduce<kGroup>(all, [](float p, float q) { return p + q; }) + glp;
+    if (out) all = __builtin_nanf("");
+    const float na = -all * inv_t * 0x1p-24f, nh = -gh * inv_t * 0x1p-24f;
+    float g[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; j++) {
+        const float lp = ((float)r[j / kVec].v[j % kVec] - m) * k - log_s, p = fast_exp2(lp + 24.0f);   // (times 2^24, as below)
+        g[j] = p * __builtin_fmaf(nh, __builtin_fmaf(kLn2, fmaxf(lp, -160.0f), H), na);
+    }
+#pragma unroll
+    for (int q = 0; q < kEach / 4; q++) laid[q][threadIdx.x] = float4{ g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3] };
+    __builtin_amdgcn_wave_barrier();                         // (a wave's LDS operations are in order)
+    const auto add = [&](int place, float extra) {
+        float* to = (float*)&laid[(place % kEach) / 4][own * kGroup + place / kEach] + place % 4;
+        *to += extra * inv_t;
+    };
+    bool joined = out || ignored;                            // the token, where it is an alternative too, is added with it: the two may nearly cancel
+    for (int e0 = 0; e0 < tops; e0 += kGroup) {
+        const int e = e0 + in;
+        const long long id = e < tops ? d.top_ids[row * d.top + e] : -1;
+        const int place = id < V ? (int)id : -1;
+        const bool both = place >= 0 && place == t && !ignored;
+        if (place >= 0) add(place, d.g_top[row * d.top + e] + (both ? glp : 0.0f));
+        const unsigned long long found = __ballot(both) >> (lane_id() & ~(kGroup - 1));
+        joined |= (kGroup == 64 ? found : found & ((1ull << (kGroup % 64)) - 1)) != 0;
+    }
+    if (in == 0 && !joined) add((int)t, glp);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int q = 0; q < kEach / 4; q++) { const float4 o = laid[q][threadIdx.x]; g[4 * q] = o.x; g[4 * q + 1] = o.y; g[4 * q + 2] = o.z; g[4 * q + 3] = o.w; }
+    if (first + own >= d.rows) return;
+    T* dx = (T*)d.dlogits + row * d.V + at;
+#pragma unroll
+    for (int i = 0; i < kEach / kVec; i++) {
+        const int left = V - at - i * kVec;
+        LooseRun<T, kVec> o;
+#pragma unroll
+        for (int j = 0; j < kVec; j++) o.v[j] = (T)(none ? 0.0f : g[i * kVec + j]);
+        if (left >= kVec) *(LooseRun<T, kVec>*)(dx + i * kVec) = o;
+        else if (left > 0) store_last(dx + i * kVec, __builtin_bit_cast(Bits, o), left);
     }
 }
 
 // How long rows are read: waves a row, and blocks a row where there are few rows. A wave to a row puts alternatives in order once, not four
 // times, and joins nothing, but needs rows for every SIMD and leaves them unevenly done (bf16, one wave against four: 5000 x 10000 21.0 against 28.0 us,
 // with 32 alternatives 51 against 75; 16384 x 20000 129 against 149; 2500 x 30000 with 4 44.6 against 41.1; 8190 x 50001 168 against 162, with 16
-// 196 against 234; float32 with 4 4096 x 30000 89 against 96, 8192 x 50000 323 against 279; 1500 x 20000 18.8 against 14.8).
+// 196 against 234; float32 with 4 4096 x 30000 89 against 96, 8192 x 50000 323 against 279; 1500 x 20000 18.8 against 14.8). Blocks to a row cost a
+// second launch (1 x 131072 4.9 against 16 us, with 4 9.8 against 27; 100 x 24000 with 4 10.1 against 12.3; 1 x 9000 5.1 against 4.0; 500 x 24000 9.5
+// against 7.8).
 struct Reading { int waves, parts, part_chunks; };
 template <class T> static Reading reading(int64_t rows, int64_t V, int top) {
     const int64_t chunks = (V + Long<T>::kChunk - 1) / Long<T>::kChunk;
     const bool one = rows >= 4096 ? chunks <= 32 || (top >= 4 && (sizeof(T) == 2 || chunks <= 64)) : rows >= 2048 && chunks <= 16;
     Reading r = { one ? 1 : 4, 1, (int)chunks };
-    if (r.waves == 4 && rows < 512 && chunks > 8) {
+    if (r.waves == 4 && rows < 384 && chunks > 16) {
         int64_t parts = 1024 / rows;
         if (parts > kMostParts) parts = kMostParts;
         if (parts > chunks / 4) parts = chunks / 4;
@@ -791,6 +880,8 @@ template <class T> static Reading reading(int64_t rows, int64_t V, int top) {
 template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s) {
     const auto blocks = [&](int per) { return grid_of((d.rows + per - 1) / per); };
     const float k = kLog2e / d.temperature, lim = 1e30f / (k > 1.0f ? k : 1.0f);   // values up to lim times k stay far from overflow
+    // Up to 512 values, and 1024 of 16 bits, a row is held in registers, in the fewest lanes of 16 values (against reading it as a long one: bf16
+    // 200000 x 256 23 against 96 us, 50000 x 1000 with 4 alternatives 38 against 46; float32 100000 x 512 31 against 40, but 50000 x 1000 54 against 37).
     // Short rows of many alternatives sort each lane's values first, where that beats finding its three best again and again (bf16, with 32: 400000 x 64
     // 55 us against 79, 50000 x 1024 77 against 83; with 8 29 against 31 and 46 against 40; float32 with 16: 400000 x 64 60 against 80,
     // 100000 x 512 89 against 78).
@@ -806,7 +897,8 @@ template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s
     if (d.V <= 128) return shorts(std::integral_constant<int, 8>());
     if (d.V <= 256) return shorts(std::integral_constant<int, 16>());
     if (d.V <= 512) return shorts(std::integral_constant<int, 32>());
-    if (d.V <= kShort) return shorts(std::integral_constant<int, 64>());
+    if constexpr (sizeof(T) == 2)
+        if (d.V <= kShort) return shorts(std::integral_constant<int, 64>());
     const Reading r = reading<T>(d.rows, d.V, d.top);
     if (r.waves == 1) k_logprobs_long<T, 1, false><<<blocks(4), 256, 0, s>>>(d, lim, 0);
     else if (r.parts == 1) k_logprobs_long<T, 4, false><<<blocks(1), 256, 0, s>>>(d, lim, 0);
@@ -816,12 +908,20 @@ template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s
     }
 }
 template <class T> static size_t workspace(int64_t rows, int64_t V, int top) {
-    if (V <= kShort) return 0;
     const Reading r = reading<T>(rows, V, top);
     return r.parts == 1 ? 0 : (size_t)rows * r.parts * (4 + 2 * top) * 4;
 }
 template <class T> static void backward(const ntc_logprobs_desc& d, hipStream_t s) {
     constexpr int kVec = 16 / (int)sizeof(T);
+    const auto shorts = [&](auto group) {
+        constexpr int g = group.value;
+        k_logprobs_grad_short<T, g><<<grid_of((d.rows + 256 / g - 1) / (256 / g)), 256, 0, s>>>(d, kLog2e / d.temperature, 1.0f / d.temperature);
+    };
+    if (d.V <= 64) return shorts(std::integral_constant<int, 4>());
+    if (d.V <= 128) return shorts(std::integral_constant<int, 8>());
+    if (d.V <= 256) return shorts(std::integral_constant<int, 16>());
+    if (d.V <= 512) return shorts(std::integral_constant<int, 32>());
+    if (d.V <= kShort) return shorts(std::integral_constant<int, 64>());
     const int64_t row_chunks = (d.V + 64 * kVec * kGradVecs - 1) / (64 * kVec * kGradVecs);
     k_logprobs_grad<T><<<grid_of((d.rows * row_chunks + 3) / 4), 256, 0, s>>>(d, (int)row_chunks);
 }
