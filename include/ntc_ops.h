@@ -131,6 +131,8 @@ typedef struct ntc_fp8_quantize_desc {
     uint8_t *codes, *exps, *codes_t, *exps_t;
 } ntc_fp8_quantize_desc;
 int ntc_op_fp8_quantize(const ntc_fp8_quantize_desc* d, void* stream, char* why, size_t why_cap);
+/* Two at once, a of block_rows 1 and b of block_rows 128 (a layer's values and its weights): one launch where their types agree. */
+int ntc_op_fp8_quantize_pair(const ntc_fp8_quantize_desc* a, const ntc_fp8_quantize_desc* b, void* stream, char* why, size_t why_cap);
 
 /* C [M][N] = A [M][K] B [N][K]^T over matrices in 8 bits, summed in 32 bits, rounded once to c_type; C's rows at ldc elements.
  * (The 8-bit matrix instruction adds a block's 128 products with about 16 bits below the largest: 1.5e-5 of a result's

@@ -100,11 +100,15 @@ template <> struct Magnitude<f32> {
 // A block of 256 threads takes a 128 x 128 tile: thread t holds 8 columns (8 (t % 16) ..) of the 8 rows 8 (t / 16) .., so that a
 // row's largest is a reduction over 16 lanes, and a column's codes of 8 rows are one 8-byte word of the transposed tile. x is
 // read once for both orders. Bound by memory.
-template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_quantize(ntc_fp8_quantize_desc d) {
+template <class T> struct QuantizeSpace {
+    alignas(16) uint32_t most[4][16 * Magnitude<T>::kWords];
+    alignas(16) uint8_t tile[128 * 128];                   // transposed; word w of 8 rows of column c at w ^ (c / 8)
+};
+template <class T, bool kBlock> __device__ __forceinline__ void quantize_tile(const ntc_fp8_quantize_desc& d, long long tile_r, long long tile_c, QuantizeSpace<T>& space) {
     using Mag = Magnitude<T>;
-    __shared__ alignas(16) uint32_t most[4][16 * Mag::kWords];
-    __shared__ alignas(16) uint8_t tile[128 * 128];        // transposed; word w of 8 rows of column c at w ^ (c / 8)
-    const long long r0 = (long long)blockIdx.y * 128, c0 = (long long)blockIdx.x * 128;
+    auto& most = space.most;
+    auto& tile = space.tile;
+    const long long r0 = tile_r * 128, c0 = tile_c * 128;
     const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4, wave = threadIdx.x >> 6;
     const int rows = d.R - r0 < 128 ? (int)(d.R - r0) : 128, cols = d.K - c0 < 128 ? (int)(d.K - c0) : 128;   // of this tile
     const T* from = (const T*)d.x + (r0 + 8 * rg) * d.row_stride + c0 + 8 * cg;
@@ -154,8 +158,8 @@ template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_qua
         b = Mag::join(Mag::join(most[0][0], most[1][0]), Mag::join(most[2][0], most[3][0]));
         block_byte = exp_byte(Mag::float_bits(b));
         if (threadIdx.x == 0) {
-            if (d.codes) put_exp(d.exps + blockIdx.y * exp_stride, blockIdx.x, block_byte, last_c, exp_stride);
-            if (d.codes_t) put_exp(d.exps_t + blockIdx.x * exp_stride_t, blockIdx.y, block_byte, last_r, exp_stride_t);
+            if (d.codes) put_exp(d.exps + tile_r * exp_stride, tile_c, block_byte, last_c, exp_stride);
+            if (d.codes_t) put_exp(d.exps_t + tile_c * exp_stride_t, tile_r, block_byte, last_r, exp_stride_t);
         }
     }
     if (d.codes) {
@@ -167,7 +171,7 @@ template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_qua
                 uint32_t b = Mag::of(x[i]);
                 b = reduce16(b, Mag::join);
                 byte = exp_byte(Mag::float_bits(b));
-                if (cg == 0 && 8 * rg + i < rows) put_exp(d.exps + (r0 + 8 * rg + i) * exp_stride, blockIdx.x, byte, last_c, exp_stride);
+                if (cg == 0 && 8 * rg + i < rows) put_exp(d.exps + (r0 + 8 * rg + i) * exp_stride, tile_c, byte, last_c, exp_stride);
             }
             const float s = power_of(254 - byte);
             uint2 o;
@@ -197,7 +201,7 @@ template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_qua
         if (!kBlock) {
             const int c = 8 * cg + j;
             byte = exp_byte(Mag::column_bits(col, j));
-            if (rg == 0 && c < cols) put_exp(d.exps_t + (c0 + c) * exp_stride_t, blockIdx.y, byte, last_r, exp_stride_t);
+            if (rg == 0 && c < cols) put_exp(d.exps_t + (c0 + c) * exp_stride_t, tile_r, byte, last_r, exp_stride_t);
         }
         const float s = power_of(254 - byte);
         uint2 o;
@@ -212,6 +216,18 @@ template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_qua
         const uint4 v = *(const uint4*)(tile + 128 * c + 8 * ((2 * part) ^ (g & 14)));
         if (c < cols) *(uint4*)(d.codes_t + (c0 + c) * code_stride_t + r0 + 16 * part) = g & 1 ? uint4{ v.z, v.w, v.x, v.y } : v;
     }
+}
+
+template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_quantize(ntc_fp8_quantize_desc d) {
+    __shared__ QuantizeSpace<T> space;
+    quantize_tile<T, kBlock>(d, blockIdx.y, blockIdx.x, space);
+}
+// Two matrices, the first in blocks of 1 x 128, the second of 128 x 128 (a layer's values and its weights): a launch less.
+template <class T> __global__ void __launch_bounds__(256) k_fp8_quantize_pair(ntc_fp8_quantize_desc a, ntc_fp8_quantize_desc b, uint32_t tiles_a, uint32_t across_a, uint32_t across_b) {
+    __shared__ QuantizeSpace<T> space;
+    const uint32_t tile = blockIdx.x;
+    if (tile < tiles_a) quantize_tile<T, false>(a, tile / across_a, tile % across_a, space);
+    else quantize_tile<T, true>(b, (tile - tiles_a) / across_b, (tile - tiles_a) % across_b, space);
 }
 
 // ---------------------------------------------------------------- products
@@ -630,19 +646,37 @@ static Plan plan_of(int64_t M, int64_t N, int64_t K) {
 
 using namespace ntc_ops;
 
-extern "C" int ntc_op_fp8_quantize(const ntc_fp8_quantize_desc* d, void* stream, char* why, size_t cap) {
+static int check_quantize(const ntc_fp8_quantize_desc* d, char* why, size_t cap) {
     if (!d) return refuse(why, cap, "no description");
     if (d->R < 0 || d->K < 0 || d->row_stride < 0) return refuse(why, cap, "sizes and strides are not negative");
     if (d->dtype < 0 || d->dtype > 2) return refuse(why, cap, "x is 32-bit floats, bfloat16 or float16");
     if (d->block_rows != 1 && d->block_rows != 128) return refuse(why, cap, "blocks are 1 x 128 or 128 x 128");
     if (!d->codes && !d->codes_t) return refuse(why, cap, "nothing to write");
-    const int64_t gy = (d->R + 127) / 128, gx = (d->K + 127) / 128;
-    if (gy > 65535 || gx >= 1 << 24) return refuse(why, cap, "at most 65535 * 128 rows, and fewer than 2^31 columns");
-    if (!gx || !gy) return 0;
-    if (!d->x || (d->codes && !d->exps) || (d->codes_t && !d->exps_t)) return refuse(why, cap, "a null pointer");
-    const auto go = [&](auto kernel) { kernel<<<dim3((unsigned)gx, (unsigned)gy), 256, 0, (hipStream_t)stream>>>(*d); };
+    if ((d->R + 127) / 128 > 65535 || (d->K + 127) / 128 >= 1 << 24) return refuse(why, cap, "at most 65535 * 128 rows, and fewer than 2^31 columns");
+    if (d->R && d->K && (!d->x || (d->codes && !d->exps) || (d->codes_t && !d->exps_t))) return refuse(why, cap, "a null pointer");
+    return 0;
+}
+
+extern "C" int ntc_op_fp8_quantize(const ntc_fp8_quantize_desc* d, void* stream, char* why, size_t cap) {
+    if (const int r = check_quantize(d, why, cap)) return r;
+    if (!d->R || !d->K) return 0;
+    const auto go = [&](auto kernel) { kernel<<<dim3((unsigned)((d->K + 127) / 128), (unsigned)((d->R + 127) / 128)), 256, 0, (hipStream_t)stream>>>(*d); };
     if (d->block_rows == 128) d->dtype == NTC_F32 ? go(k_fp8_quantize<f32, true>) : d->dtype == NTC_BF16 ? go(k_fp8_quantize<bf16, true>) : go(k_fp8_quantize<f16, true>);
     else d->dtype == NTC_F32 ? go(k_fp8_quantize<f32, false>) : d->dtype == NTC_BF16 ? go(k_fp8_quantize<bf16, false>) : go(k_fp8_quantize<f16, false>);
+    return launched(why, cap);
+}
+
+extern "C" int ntc_op_fp8_quantize_pair(const ntc_fp8_quantize_desc* a, const ntc_fp8_quantize_desc* b, void* stream, char* why, size_t cap) {
+    if (const int r = check_quantize(a, why, cap)) return r;
+    if (const int r = check_quantize(b, why, cap)) return r;
+    if (a->block_rows != 1 || b->block_rows != 128) return refuse(why, cap, "a pair's blocks are 1 x 128 and 128 x 128");
+    const int64_t across_a = (a->K + 127) / 128, across_b = (b->K + 127) / 128, tiles_a = (a->R + 127) / 128 * across_a, tiles_b = (b->R + 127) / 128 * across_b;
+    if (!tiles_a || !tiles_b || a->dtype != b->dtype || tiles_a + tiles_b >= 1 << 24) {
+        if (const int r = ntc_op_fp8_quantize(a, stream, why, cap)) return r;
+        return ntc_op_fp8_quantize(b, stream, why, cap);
+    }
+    const auto go = [&](auto kernel) { kernel<<<(unsigned)(tiles_a + tiles_b), 256, 0, (hipStream_t)stream>>>(*a, *b, (uint32_t)tiles_a, (uint32_t)across_a, (uint32_t)across_b); };
+    a->dtype == NTC_F32 ? go(k_fp8_quantize_pair<f32>) : a->dtype == NTC_BF16 ? go(k_fp8_quantize_pair<bf16>) : go(k_fp8_quantize_pair<f16>);
     return launched(why, cap);
 }
 

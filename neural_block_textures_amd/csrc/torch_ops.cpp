@@ -171,16 +171,40 @@ py::tuple token_logprobs(const Tensor& logits, Tensor tokens, int64_t top, doubl
 // ---------------------------------------------------------------- 8-bit floating point in blocks
 int64_t blocks_of(int64_t n, int64_t b) { return (n + b - 1) / b; }
 
-// A matrix in 8 bits inside one buffer: codes, then exponents.
+// A matrix in 8 bits inside a buffer, from `at` on: codes, then exponents, then up to a multiple of 16 bytes.
 struct Held {
     Tensor buffer;
-    int64_t R = 0, K = 0, block = 1;
-    uint8_t* codes() const { return (uint8_t*)buffer.data_ptr(); }
-    uint8_t* exps() const { return codes() + R * ntc_fp8_code_stride(K); }
+    int64_t R = 0, K = 0, block = 1, at = 0;
+    uint8_t* codes() const { return buffer.defined() ? (uint8_t*)buffer.data_ptr() + at : nullptr; }
+    uint8_t* exps() const { return buffer.defined() ? codes() + R * ntc_fp8_code_stride(K) : nullptr; }
+    int64_t size() const { return (R * ntc_fp8_code_stride(K) + blocks_of(R, block) * ntc_fp8_exp_stride(K) + 15) / 16 * 16; }
     Held() = default;
-    Held(int64_t r, int64_t k, int64_t b, const Tensor& like) : R(r), K(k), block(b) { buffer = bytes(r * ntc_fp8_code_stride(k) + blocks_of(r, b) * ntc_fp8_exp_stride(k), like); }
+    Held(int64_t r, int64_t k, int64_t b) : R(r), K(k), block(b) {}
+    Held(int64_t r, int64_t k, int64_t b, const Tensor& like) : Held(r, k, b) { buffer = bytes(size(), like); }
 };
+// One buffer for two of them, or for those that are wanted.
+Tensor hold(Held& a, bool want_a, Held& b, bool want_b, const Tensor& like) {
+    if (!want_a && !want_b) return {};
+    const Tensor buffer = bytes((want_a ? a.size() : 0) + (want_b ? b.size() : 0), like);
+    b.at = want_a ? a.size() : 0;
+    if (want_a) a.buffer = buffer;
+    if (want_b) b.buffer = buffer;
+    return buffer;
+}
 
+ntc_fp8_quantize_desc quantize_desc(const Tensor& x, int64_t block, const Held& plain, const Held& transposed) {
+    return { x.const_data_ptr(), x.size(0), x.size(1), x.stride(0), type_of(x), (int32_t)block, plain.codes(), plain.exps(), transposed.codes(), transposed.exps() };
+}
+void run_quantize(const Tensor& x, const Held& plain, const Held& transposed) {
+    if (!x.numel()) return;
+    const ntc_fp8_quantize_desc d = quantize_desc(x, plain.block, plain, transposed);
+    call(x.device(), [&](void* s, char* why, size_t cap) { return ntc_op_fp8_quantize(&d, s, why, cap); });
+}
+void run_quantize_pair(const Tensor& x, const Held& xq, const Held& xt, const Tensor& w, const Held& wq, const Held& wt) {
+    if (!x.numel() || !w.numel()) { run_quantize(x, xq, xt); run_quantize(w, wq, wt); return; }
+    const ntc_fp8_quantize_desc a = quantize_desc(x, 1, xq, xt), b = quantize_desc(w, 128, wq, wt);
+    call(x.device(), [&](void* s, char* why, size_t cap) { return ntc_op_fp8_quantize_pair(&a, &b, s, why, cap); });
+}
 void run_quantize(const Tensor& x, int64_t block, uint8_t* codes, uint8_t* exps, uint8_t* codes_t, uint8_t* exps_t) {
     if (!x.numel()) return;
     const ntc_fp8_quantize_desc d = { x.const_data_ptr(), x.size(0), x.size(1), x.stride(0), type_of(x), (int32_t)block, codes, exps, codes_t, exps_t };
@@ -213,7 +237,10 @@ py::tuple quantize(const Tensor& x_, int64_t block, bool plain, bool transposed)
     if (plain) q = make(R, K);
     if (transposed) t = make(K, R);
     const auto at_ = [](const Tensor& b) { return b.defined() ? (uint8_t*)b.data_ptr() : nullptr; };
-    run_quantize(x, block, at_(q.first), at_(q.second), at_(t.first), at_(t.second));
+    if (x.numel()) {
+        const ntc_fp8_quantize_desc d = { x.const_data_ptr(), R, K, x.stride(0), type_of(x), (int32_t)block, at_(q.first), at_(q.second), at_(t.first), at_(t.second) };
+        call(x.device(), [&](void* s, char* why, size_t cap) { return ntc_op_fp8_quantize(&d, s, why, cap); });
+    }
     return py::make_tuple(plain ? py::cast(q) : py::none(), transposed ? py::cast(t) : py::none());
 }
 
@@ -242,38 +269,38 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w) {
         const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
         const bool need_x = x.requires_grad(), need_w = w.requires_grad();
-        const Held xq(M, K, 1, x), wq(N, K, 128, x);
-        const Held xt = need_w ? Held(K, M, 1, x) : Held(), wt = need_x ? Held(K, N, 128, x) : Held();
-        run_quantize(x, 1, xq.codes(), xq.exps(), need_w ? xt.codes() : nullptr, need_w ? xt.exps() : nullptr);
-        run_quantize(w, 128, wq.codes(), wq.exps(), need_x ? wt.codes() : nullptr, need_x ? wt.exps() : nullptr);
+        Held xq(M, K, 1), wq(N, K, 128), xt(K, M, 1), wt(K, N, 128);
+        hold(xq, true, wq, true, x);
+        const Tensor kept = hold(xt, need_w, wt, need_x, x);
+        run_quantize_pair(x, xq, xt, w, wq, wt);
         const Tensor y = matrix(M, N, x.scalar_type(), x);
         run_matmul(operand(xq), operand(wq), K, y);
-        ctx->save_for_backward({ xt.buffer, wt.buffer });
-        ctx->saved_data["M"] = M;
-        ctx->saved_data["N"] = N;
-        ctx->saved_data["K"] = K;
-        ctx->saved_data["x"] = (int64_t)x.scalar_type();
-        ctx->saved_data["w"] = (int64_t)w.scalar_type();
+        ctx->save_for_backward({ kept });
+        ctx->saved_data["call"] = std::vector<int64_t>{ M, N, K, need_x, need_w, (int64_t)x.scalar_type(), (int64_t)w.scalar_type() };
         ctx->set_materialize_grads(false);
         return y;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
         if (!g[0].defined()) return { Tensor(), Tensor() };
         const auto saved = ctx->get_saved_variables();
-        const int64_t M = ctx->saved_data["M"].toInt(), N = ctx->saved_data["N"].toInt(), K = ctx->saved_data["K"].toInt();
-        const bool need_x = saved[1].defined(), need_w = saved[0].defined();
+        const std::vector<int64_t> of = ctx->saved_data["call"].toIntVector();
+        const int64_t M = of[0], N = of[1], K = of[2];
+        const bool need_x = of[3], need_w = of[4];
         const Tensor dy = rows_contiguous(g[0]);
-        const Held dq = need_x ? Held(M, N, 1, dy) : Held(), dt = need_w ? Held(N, M, 1, dy) : Held();
-        run_quantize(dy, 1, need_x ? dq.codes() : nullptr, need_x ? dq.exps() : nullptr, need_w ? dt.codes() : nullptr, need_w ? dt.exps() : nullptr);
+        Held dq(M, N, 1), dt(N, M, 1), xt(K, M, 1), wt(K, N, 128);
+        hold(dq, need_x, dt, need_w, dy);
+        if (need_w) xt.buffer = saved[0];
+        if (need_x) wt.buffer = saved[0];
+        wt.at = need_w ? xt.size() : 0;
+        run_quantize(dy, dq, dt);
         Tensor dx, dw;
-        const auto held = [](const Tensor& b, int64_t r, int64_t k, int64_t block) { Held h; h.buffer = b; h.R = r; h.K = k; h.block = block; return h; };
         if (need_x) {
-            dx = matrix(M, K, (at::ScalarType)ctx->saved_data["x"].toInt(), dy);
-            run_matmul(operand(dq), operand(held(saved[1], K, N, 128)), N, dx);
+            dx = matrix(M, K, (at::ScalarType)of[5], dy);
+            run_matmul(operand(dq), operand(wt), N, dx);
         }
         if (need_w) {
-            dw = matrix(N, K, (at::ScalarType)ctx->saved_data["w"].toInt(), dy);
-            run_matmul(operand(dt), operand(held(saved[0], K, M, 1)), M, dw);
+            dw = matrix(N, K, (at::ScalarType)of[6], dy);
+            run_matmul(operand(dt), operand(xt), M, dw);
         }
         return { once(dx, "fp8_linear"), once(dw, "fp8_linear") };
     }
@@ -299,9 +326,9 @@ Tensor linear(const Tensor& x, const Tensor& w) {
     const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad());
     const Tensor x2 = rows_contiguous(as_rows(x)), w2 = rows_contiguous(w);
     if (grad) return like_rows(LinearNode::apply(x2, w2), x);
-    const Held xq(x2.size(0), x2.size(1), 1, x2), wq(w2.size(0), w2.size(1), 128, x2);
-    run_quantize(x2, 1, xq.codes(), xq.exps(), nullptr, nullptr);
-    run_quantize(w2, 128, wq.codes(), wq.exps(), nullptr, nullptr);
+    Held xq(x2.size(0), x2.size(1), 1), wq(w2.size(0), w2.size(1), 128);
+    hold(xq, true, wq, true, x2);
+    run_quantize_pair(x2, xq, {}, w2, wq, {});
     const Tensor y = matrix(x2.size(0), w2.size(0), x.scalar_type(), x2);
     run_matmul(operand(xq), operand(wq), x2.size(1), y);
     return like_rows(y, x);
@@ -319,7 +346,7 @@ Tensor linear_fp8(const Tensor& x, const Tensor& codes, const Tensor& exps, int6
         run_matmul({ x2.const_data_ptr(), nullptr, M, x2.stride(0), type_of(x2), 1 }, b, K, y);
     } else {
         const Held xq(M, K, 1, x2);
-        run_quantize(x2, 1, xq.codes(), xq.exps(), nullptr, nullptr);
+        run_quantize(x2, xq, {});
         run_matmul(operand(xq), b, K, y);
     }
     return like_rows(y, x);

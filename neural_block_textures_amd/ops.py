@@ -64,6 +64,7 @@ def library() -> C.CDLL:
             "ntc_op_adamw_moments": (C.c_int, [_P, _P, _P, _P, _L, _P, _P] + tail),
             "ntc_op_adamw_encode": (C.c_int, [_P, _P, _L, _P, _P, _P, _P] + tail),
             "ntc_op_fp8_quantize": (C.c_int, [_P] + tail),
+            "ntc_op_fp8_quantize_pair": (C.c_int, [_P, _P] + tail),
             "ntc_op_fp8_matmul_workspace": (C.c_size_t, [_L, _L, _L, _I]),
             "ntc_op_fp8_matmul": (C.c_int, [_P] + tail),
             "ntc_op_fp8_matmul_float_rows": (_L, []),

@@ -69,6 +69,26 @@ def test_quantize(R, K, dtype):
     assert same(o.fp8_quantize(x, 128).values(), o.fp8_quantize_t(x, 128).values().t())
 
 
+@pytest.mark.parametrize("dtypes", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16), (torch.float32, torch.float32), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (3, 300, 127), (129, 5, 513), (260, 390, 1000)])
+def test_quantize_pair(M, N, K, dtypes):
+    """Two matrices at once hold what each alone does."""
+    import ctypes as C
+    o = ops()
+    x, w = randn(M, M, K).to(dtypes[0]), randn(N, N, K).to(dtypes[1])
+    want = [*o.fp8_quantize_both(x, 1), *o.fp8_quantize_both(w, 128)]
+    got = [o.Fp8Tensor(torch.full_like(q.codes, 77), torch.full_like(q.exps, 77), q.shape, q.block_rows) for q in want]
+    descs = []
+    for v, (q, t), rows in ((x, got[:2], 1), (w, got[2:], 128)):
+        code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[v.dtype]
+        descs.append(o.QuantizeDesc(v.data_ptr(), v.shape[0], K, K, code, rows, q.codes.data_ptr(), q.exps.data_ptr(), t.codes.data_ptr(), t.exps.data_ptr()))
+    why = C.create_string_buffer(200)
+    rc = o.library().ntc_op_fp8_quantize_pair(C.byref(descs[0]), C.byref(descs[1]), torch.cuda.current_stream().cuda_stream, why, 200)
+    assert rc == 0, why.value
+    for a, b in zip(got, want):
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.exps, b.exps)
+
+
 def test_quantize_at_the_ends():
     """Amax at and beside 448 scales, ties, subnormal codes, zeros, tiny and huge blocks, infinities and NaN."""
     x = torch.zeros(12, 256, device="cuda")

@@ -109,6 +109,20 @@ def test_quantize_refusals(kw, reason):
     assert rc == 1 and reason in why, why
 
 
+def test_quantize_pair_refusals():
+    d, e = O.QuantizeDesc(), O.QuantizeDesc()
+    for q, rows in ((d, 1), (e, 128)):
+        for k, v in {"x": 1 << 20, "R": 4, "K": 4, "row_stride": 4, "block_rows": rows, "codes": 1 << 20, "exps": 1 << 20}.items():
+            setattr(q, k, v)
+    call = O.library().ntc_op_fp8_quantize_pair
+    for a, b, reason in ((d, d, "pair's blocks"), (e, d, "pair's blocks")):
+        rc, why = refused(call, C.byref(a), C.byref(b))
+        assert rc == 1 and reason in why, why
+    e.exps = None
+    rc, why = refused(call, C.byref(d), C.byref(e))
+    assert rc == 1 and "null" in why, why
+
+
 @pytest.mark.parametrize("kw,reason", [({"M": -1}, "not negative"), ({"c_type": 3}, "C is"), ({"a_block_rows": 2}, "blocks are"), ({"b_block_rows": 0}, "blocks are"),
                                        ({"ldc": 3}, "overlap"), ({"b": None}, "null"), ({"c": None}, "null"), ({"a_exps": None}, "null"), ({"a_type": 4}, "A is")])
 def test_matmul_refusals(kw, reason):
