@@ -15,11 +15,23 @@ __device__ __forceinline__ int exp_byte(uint32_t most) {
     const int e = (int)(most >> 23) - 8 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0);
     return e < 0 ? 0 : e;
 }
-__device__ __forceinline__ uint32_t to_fp8x4(float a, float b, float c, float d) {
-    uint32_t r = 0;
-    r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, r, false);
-    r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
-    return r;
+// Four values to codes of a block whose scale is 2^(byte - 127); the instruction divides by the power itself.
+template <class T> __device__ __forceinline__ uint32_t to_codes4(T a, T b, T c, T d, float scale) {
+    typedef short s2 __attribute__((ext_vector_type(2)));
+    s2 r = { 0, 0 };
+    if constexpr (std::is_same_v<T, bf16>) {
+        typedef __bf16 two __attribute__((ext_vector_type(2)));
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, two{ a, b }, scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, two{ c, d }, scale, true);
+    } else if constexpr (std::is_same_v<T, f16>) {
+        typedef _Float16 two __attribute__((ext_vector_type(2)));
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, two{ a, b }, scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, two{ c, d }, scale, true);
+    } else {
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
+    }
+    return __builtin_bit_cast(uint32_t, r);
 }
 
 // Largest magnitudes of finite values, as integers that order like them: 16-bit types two to a word, so that one instruction
@@ -47,28 +59,32 @@ template <class T> struct Magnitude {                       // bf16 and f16
         const uint16_t h = (uint16_t)max_word(m & 0xffffu, m >> 16);
         return __float_as_uint((float)__builtin_bit_cast(T, h));
     }
-    // of eight columns over eight rows, two columns to a word; and the float bits of column j of them
+    // of eight rows of eight values, two to a word; non-finite ones as 0
     static constexpr int kWords = 4;
-    static __device__ __forceinline__ void columns(const Run<T, 8> (&x)[8], uint32_t (&m)[kWords]) {
-        uint32_t w[8][4], any = 0;
+    static __device__ __forceinline__ void all(const Run<T, 8> (&x)[8], uint32_t (&m)[8][kWords]) {
+        uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const uint4 v = __builtin_bit_cast(uint4, x[i]);
-            w[i][0] = v.x & 0x7fff7fffu; w[i][1] = v.y & 0x7fff7fffu; w[i][2] = v.z & 0x7fff7fffu; w[i][3] = v.w & 0x7fff7fffu;
-        }
+            m[i][0] = v.x & 0x7fff7fffu; m[i][1] = v.y & 0x7fff7fffu; m[i][2] = v.z & 0x7fff7fffu; m[i][3] = v.w & 0x7fff7fffu;
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            m[q] = w[0][q];
-#pragma unroll
-            for (int i = 1; i < 8; i++) m[q] = max_pair(m[q], w[i][q]);
-            any = max_pair(any, m[q]);
+            for (int q = 0; q < 4; q++) any = max_pair(any, m[i][q]);
         }
         if (__builtin_expect(__ballot(max_word(any & 0xffffu, any >> 16) >= kInf) != 0, 0)) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                m[q] = 0;
-                for (int i = 0; i < 8; i++) m[q] = max_pair(m[q], ((w[i][q] & 0xffffu) >= kInf ? 0u : w[i][q] & 0xffffu) | (w[i][q] >> 16 >= kInf ? 0u : w[i][q] & 0xffff0000u));
-            }
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) m[i][q] = ((m[i][q] & 0xffffu) >= kInf ? 0u : m[i][q] & 0xffffu) | (m[i][q] >> 16 >= kInf ? 0u : m[i][q] & 0xffff0000u);
+        }
+    }
+    // the float bits of each row's largest over 16 lanes, two rows to a word on the way
+    static __device__ __forceinline__ void rows(const uint32_t (&m)[8][kWords], uint32_t (&bits)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const uint32_t a = max_pair(max_pair(m[i][0], m[i][1]), max_pair(m[i][2], m[i][3])), b = max_pair(max_pair(m[i + 1][0], m[i + 1][1]), max_pair(m[i + 1][2], m[i + 1][3]));
+            const uint32_t both = reduce16(max_pair(__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(b, a, 0x07060302u)), max_pair);
+            bits[i] = float_bits(both & 0xffffu);
+            bits[i + 1] = float_bits(both >> 16);
         }
     }
     static __device__ __forceinline__ uint32_t column_bits(const uint32_t (&m)[kWords], int j) { return float_bits(j & 1 ? m[j >> 1] >> 16 : m[j >> 1] & 0xffffu); }
@@ -86,11 +102,19 @@ template <> struct Magnitude<f32> {
     }
     static __device__ __forceinline__ uint32_t float_bits(uint32_t m) { return m; }
     static constexpr int kWords = 8;
-    static __device__ __forceinline__ void columns(const Run<float, 8> (&x)[8], uint32_t (&m)[kWords]) {
+    static __device__ __forceinline__ void all(const Run<float, 8> (&x)[8], uint32_t (&m)[8][kWords]) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            m[j] = 0;
-            for (int i = 0; i < 8; i++) m[j] = max_word(m[j], one(x[i].v[j]));
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) m[i][j] = one(x[i].v[j]);
+    }
+    static __device__ __forceinline__ void rows(const uint32_t (&m)[8][kWords], uint32_t (&bits)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            uint32_t a = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) a = max_word(a, m[i][j]);
+            bits[i] = reduce16(a, max_word);
         }
     }
     static __device__ __forceinline__ uint32_t column_bits(const uint32_t (&m)[kWords], int j) { return m[j]; }
@@ -128,6 +152,12 @@ template <class T, bool kBlock> __device__ __forceinline__ void quantize_tile(co
                 const auto v = *(const LooseRun<T, 8>*)(tile0 + (8 * rg + i < rows ? 8 * rg + i : rows - 1) * d.row_stride + 8 * cg);
                 for (int j = 0; j < 8; j++) x[i].v[j] = v.v[j];
             }
+        } else if (left > 0 && sizeof(T) == 2 && d.K >= 8) {  // from the last eight of the row
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const auto v = *(const LooseRun<T, 8>*)((const T*)d.x + (r0 + (8 * rg + i < rows ? 8 * rg + i : rows - 1)) * d.row_stride + d.K - 8);
+                if constexpr (sizeof(T) == 2) x[i] = __builtin_bit_cast(Run<T, 8>, __builtin_bit_cast(unsigned __int128, v) >> (16 * (8 - left)));
+            }
         } else if (left > 0) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -142,16 +172,21 @@ template <class T, bool kBlock> __device__ __forceinline__ void quantize_tile(co
     }
     const long long code_stride = ntc_fp8_code_stride(d.K), exp_stride = ntc_fp8_exp_stride(d.K), code_stride_t = ntc_fp8_code_stride(d.R), exp_stride_t = ntc_fp8_exp_stride(d.R);
     // a row of exponents is written by the tile that has its block; the last one also clears what follows
+    const bool last_c = c0 + 128 >= d.K, last_r = r0 + 128 >= d.R;
     const auto put_exp = [](uint8_t* row, long long at, int byte, bool last, long long stride) {
         row[at] = (uint8_t)byte;
         if (last) for (long long k = at + 1; k < stride; k++) row[k] = 0;
     };
-    const bool last_c = c0 + 128 >= d.K, last_r = r0 + 128 >= d.R;
+    const auto byte_of = [](uint64_t packed, int i) { return (int)((packed >> (8 * i)) & 255); };
+    uint32_t mag[8][Mag::kWords];
+    Mag::all(x, mag);
     int block_byte = 0;
     if (kBlock) {
         uint32_t b = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) b = Mag::join(b, Mag::of(x[i]));
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int q = 0; q < Mag::kWords; q++) b = Mag::join(b, mag[i][q]);
         b = reduce64(b, Mag::join);
         if ((threadIdx.x & 63) == 0) most[wave][0] = b;
         __syncthreads();
@@ -164,28 +199,32 @@ template <class T, bool kBlock> __device__ __forceinline__ void quantize_tile(co
     }
     if (d.codes) {
         uint8_t* to = d.codes + (r0 + 8 * rg) * code_stride + c0 + 8 * cg;
+        uint32_t bits[8];
+        uint64_t bytes = 0;
+        if (!kBlock) Mag::rows(mag, bits);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            int byte = block_byte;
-            if (!kBlock) {
-                uint32_t b = Mag::of(x[i]);
-                b = reduce16(b, Mag::join);
-                byte = exp_byte(Mag::float_bits(b));
-                if (cg == 0 && 8 * rg + i < rows) put_exp(d.exps + (r0 + 8 * rg + i) * exp_stride, tile_c, byte, last_c, exp_stride);
-            }
-            const float s = power_of(254 - byte);
+            const int byte = kBlock ? block_byte : exp_byte(bits[i]);
+            bytes |= (uint64_t)byte << (8 * i);
+            const float s = power_of(byte);
             uint2 o;
-            o.x = to_fp8x4((float)x[i].v[0] * s, (float)x[i].v[1] * s, (float)x[i].v[2] * s, (float)x[i].v[3] * s);
-            o.y = to_fp8x4((float)x[i].v[4] * s, (float)x[i].v[5] * s, (float)x[i].v[6] * s, (float)x[i].v[7] * s);
+            o.x = to_codes4(x[i].v[0], x[i].v[1], x[i].v[2], x[i].v[3], s);
+            o.y = to_codes4(x[i].v[4], x[i].v[5], x[i].v[6], x[i].v[7], s);
             if (8 * rg + i < rows) *(uint2*)(to + i * code_stride) = o;
         }
+        // lane i of the row group's 16 has row i's exponent to write
+        if (!kBlock && cg < 8 && 8 * rg + cg < rows) put_exp(d.exps + (r0 + 8 * rg + cg) * exp_stride, tile_c, byte_of(bytes, cg), last_c, exp_stride);
     }
     if (!d.codes_t) return;
     uint32_t col[Mag::kWords];
     if (!kBlock) {
-        Mag::columns(x, col);
 #pragma unroll
-        for (int q = 0; q < Mag::kWords; q++) col[q] = reduce_rows(col[q], Mag::join);
+        for (int q = 0; q < Mag::kWords; q++) {
+            col[q] = mag[0][q];
+#pragma unroll
+            for (int i = 1; i < 8; i++) col[q] = Mag::join(col[q], mag[i][q]);
+            col[q] = reduce_rows(col[q], Mag::join);
+        }
         if ((threadIdx.x & 48) == 0)
 #pragma unroll
             for (int q = 0; q < Mag::kWords; q++) most[wave][Mag::kWords * cg + q] = col[q];
@@ -195,20 +234,18 @@ template <class T, bool kBlock> __device__ __forceinline__ void quantize_tile(co
 #pragma unroll
             for (int q = 0; q < Mag::kWords; q++) col[q] = Mag::join(col[q], most[w][Mag::kWords * cg + q]);
     }
+    uint64_t bytes = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        int byte = block_byte;
-        if (!kBlock) {
-            const int c = 8 * cg + j;
-            byte = exp_byte(Mag::column_bits(col, j));
-            if (rg == 0 && c < cols) put_exp(d.exps_t + (c0 + c) * exp_stride_t, tile_r, byte, last_r, exp_stride_t);
-        }
-        const float s = power_of(254 - byte);
+        const int byte = kBlock ? block_byte : exp_byte(Mag::column_bits(col, j));
+        bytes |= (uint64_t)byte << (8 * j);
+        const float s = power_of(byte);
         uint2 o;
-        o.x = to_fp8x4((float)x[0].v[j] * s, (float)x[1].v[j] * s, (float)x[2].v[j] * s, (float)x[3].v[j] * s);
-        o.y = to_fp8x4((float)x[4].v[j] * s, (float)x[5].v[j] * s, (float)x[6].v[j] * s, (float)x[7].v[j] * s);
+        o.x = to_codes4(x[0].v[j], x[1].v[j], x[2].v[j], x[3].v[j], s);
+        o.y = to_codes4(x[4].v[j], x[5].v[j], x[6].v[j], x[7].v[j], s);
         *(uint2*)(tile + 128 * (8 * cg + j) + 8 * (rg ^ cg)) = o;
     }
+    if (!kBlock && rg < 8 && 8 * cg + rg < cols) put_exp(d.exps_t + (c0 + 8 * cg + rg) * exp_stride_t, tile_r, byte_of(bytes, rg), last_r, exp_stride_t);
     __syncthreads();
 #pragma unroll
     for (int p = 0; p < 4; p++) {
@@ -484,12 +521,12 @@ template <class A> __device__ __forceinline__ v8i to_codes(const Run<A, 8> (&x)[
 #pragma unroll
     for (int i = 0; i < 4; i++) m = Mag::join(m, Mag::of(x[i]));
     byte = exp_byte(reduce_rows(Mag::float_bits(m), [](uint32_t p, uint32_t q) { return p > q ? p : q; }));
-    const float s = power_of(254 - byte);
+    const float s = power_of(byte);
     v8i r;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        r[2 * i] = (int)to_fp8x4((float)x[i].v[0] * s, (float)x[i].v[1] * s, (float)x[i].v[2] * s, (float)x[i].v[3] * s);
-        r[2 * i + 1] = (int)to_fp8x4((float)x[i].v[4] * s, (float)x[i].v[5] * s, (float)x[i].v[6] * s, (float)x[i].v[7] * s);
+        r[2 * i] = (int)to_codes4(x[i].v[0], x[i].v[1], x[i].v[2], x[i].v[3], s);
+        r[2 * i + 1] = (int)to_codes4(x[i].v[4], x[i].v[5], x[i].v[6], x[i].v[7], s);
     }
     return r;
 }
