@@ -123,7 +123,9 @@ template <> struct Magnitude<f32> {
 // ---------------------------------------------------------------- to 8 bits
 // A block of 256 threads takes a 128 x 128 tile: thread t holds 8 columns (8 (t % 16) ..) of the 8 rows 8 (t / 16) .., so that a
 // row's largest is a reduction over 16 lanes, and a column's codes of 8 rows are one 8-byte word of the transposed tile. x is
-// read once for both orders. Bound by memory.
+// read once for both orders. Bound by memory where it is large (bf16 8192 x 8192, 1 x 128 blocks: 34.6 us, 5.8 TB/s; both orders 51), by the tile's own
+// latency where it is not (128 x 128, both orders: 4.6 us; 4096 x 4096 15.8 us, 4.2 TB/s: loads, largest values, codes and stores of all tiles
+// go in step).
 template <class T> struct QuantizeSpace {
     alignas(16) uint32_t most[4][16 * Magnitude<T>::kWords];
     alignas(16) uint8_t tile[128 * 128];                   // transposed; word w of 8 rows of column c at w ^ (c / 8)
@@ -276,6 +278,10 @@ template <class T> __global__ void __launch_bounds__(256) k_fp8_quantize_pair(nt
 // into LDS (a stage; kStages of them in turn), stages ahead of the registers that the products are fed from, which are themselves
 // one stage ahead of the products: one barrier a stage, and no product waits for a load of its own stage. In LDS a row is 64 bytes, and the 16-byte
 // piece c of row r lies at c ^ swizzle(r), which spreads any 8 or 16 rows' pieces over all banks.
+//
+// Bound by the matrix instructions and the power they draw (8192 x 8192 x 8192: 421 us, 2.61 PFLOP/s; 483 us where twenty follow each other; the instructions alone, from registers, 3.8 PFLOP/s on random
+// data and 4.9 on zeros; the library's product with one scale for a matrix 3.05). 256 x 256 tiles read each operand byte from LDS half as often as 128 x
+// 128 ones, and the four waves' SIMDs hold nothing else.
 constexpr int kStages = 4;
 __device__ __forceinline__ int swizzle(int r) { return ((r >> 1) & 3) ^ ((r >> 3) & 1); }
 
@@ -504,7 +510,8 @@ template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds_
     else store(std::integral_constant<int, 0>());
 }
 
-// Few rows of A: bound by the bytes of B. A block takes 16 rows of B, its waves a share of the columns each, straight from memory into the
+// Few rows of A: bound by the bytes of B (one row by 4096 x 4096 5.9 us, 2.9 TB/s and mostly the launch and the first loads; by 8192 x 4096 8.1 us,
+// 4.2 TB/s). A block takes 16 rows of B, its waves a share of the columns each, straight from memory into the
 // operands' registers (v_mfma_scale_f32_16x16x128: lane l holds 32 bytes of row l % 16 at k = 32 (l / 16); result i is (first operand's row
 // 4 (l / 16) + i, second's row l % 16)), and the waves' sums are added in LDS, in order. A's rows are kM tiles of 16 (past the end the last row
 // again); floats are taken to 8 bits here, each wave what it needs, which saves a launch: a row's block is 32 values in each of 4 lanes.
@@ -625,8 +632,11 @@ template <class A, int kM, int kN, class C> __global__ void __launch_bounds__(64
         if (m < d.M && n0 + n < d.N) ((C*)d.c)[m * d.ldc + n0 + n] = (C)s;
     }
 }
-// Up to 32 rows, floats up to 16 (64 rows by 4096 x 4096: 20 us so, 16.7 in tiles; 32 rows as floats 17.5, taken to 8 bits before 14.4).
-constexpr int kFewRows = 32, kFloatRows = 16;
+// Up to 16 rows, which may be floats (17 rows as floats 9.5 us by 4096 x 4096 and 23.0 by 12000 x 4096, taken to 8 bits before 11.3 and 21.7; 32 rows
+// 13.5 and 28.3 against 13.5 and 25.8); up to 32 while B's pairs of tiles are at most one to a CU (32 rows by 8192 x 4096: 15.7 us so, 19.4 in tiles of
+// 64 x 64; by 12000 x 4096 25.8 and 19.8; by 12000 x 12000 62 and 33). More rows go into tiles (64 by 4096 x 4096: 19.4 us so, 17.6 in tiles).
+constexpr int kFloatRows = 16;
+static bool few_rows(int64_t M, int64_t N) { return M <= 16 || (M <= 32 && N <= 32 * 256); }
 
 // The parts of a split sum, added in a fixed order: a block takes 256 results, four a lane, each of its four waves every fourth part.
 template <class C> __global__ void __launch_bounds__(256) k_fp8_join(const float* parts, int n_parts, long long size, long long N, long long ldc, C* c) {
@@ -718,14 +728,14 @@ extern "C" int ntc_op_fp8_quantize_pair(const ntc_fp8_quantize_desc* a, const nt
 }
 
 extern "C" size_t ntc_op_fp8_matmul_workspace(int64_t M, int64_t N, int64_t K, int32_t) {
-    if (M <= kFewRows || N < 1 || K < 1) return 0;
+    if (M < 1 || N < 1 || K < 1 || few_rows(M, N)) return 0;
     const Plan p = plan_of(M, N, K);
     return p.parts > 1 ? (size_t)p.parts * M * N * 4 : 0;
 }
 extern "C" int64_t ntc_op_fp8_matmul_float_rows(void) { return kFloatRows; }
 
 template <class A, int kM, class C> static void launch_few(const FewArgs& F, hipStream_t s) {
-    // two tiles of B a wave where that still leaves a block to each CU
+    // two tiles of B a wave where that still leaves a block to each CU (one row by 8192 x 4096: 8.1 us against 10.1; 4096 x 4096: 7.7 against 5.9)
     if (F.N >= 32 * 256) k_fp8_few<A, kM, 2, C><<<grid_of((F.N + 31) / 32), 64 * kFewWaves, 0, s>>>(F);
     else k_fp8_few<A, kM, 1, C><<<grid_of((F.N + 15) / 16), 64 * kFewWaves, 0, s>>>(F);
 }
@@ -789,7 +799,7 @@ extern "C" int ntc_op_fp8_matmul(const ntc_fp8_matmul_desc* d, void* stream, cha
         return refuse(why, cap, "codes start at multiples of 16 bytes, exponents of 4");
     if (!d->workspace && ntc_op_fp8_matmul_workspace(d->M, d->N, d->K, d->a_type)) return refuse(why, cap, "a null workspace");
     const hipStream_t s = (hipStream_t)stream;
-    if (d->M <= kFewRows) {
+    if (few_rows(d->M, d->N)) {
         d->c_type == NTC_F32 ? run_few<f32>(d, s) : d->c_type == NTC_BF16 ? run_few<bf16>(d, s) : run_few<f16>(d, s);
         return launched(why, cap);
     }
