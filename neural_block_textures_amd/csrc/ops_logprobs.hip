@@ -135,7 +135,7 @@ struct ThreePlaced {                                          // (0: none)
 // word to its index (from the top down, in a row of at most 1024): one word orders values and indices both. A 32-bit value's index is found in
 // a second reduction. What is written of rows is left to one lane a row (and one an alternative), since a wave's instructions cost as much for 4 rows
 // as for 64. Bound by vector instructions (358 a wave with 4 alternatives): 262144 rows of 256 bf16 values 42 us with 4 alternatives, 3.6 TB/s; 400000
-// x 64 14.3 us without, at the rate of their bytes. A row's values are read once, and in registers no pass over them is repeated.
+// x 64 14.3 us without, at the rate of their bytes.
 constexpr int kShort = 1024;                                 // the longest such row
 // Sixteen values in descending order: exchanges of pairs, halves merged odd with even.
 template <class K> __device__ __forceinline__ void sort16(K (&a)[16]) {
