@@ -4,7 +4,10 @@
 
 #include <dlfcn.h>
 #include <hip/hiprtc.h>
+#include <limits.h>
+#include <link.h>
 #include <stdlib.h>
+#include <string.h>
 #include <sys/stat.h>
 #include <unistd.h>
 
@@ -30,12 +33,44 @@ namespace {
 std::mutex g_mu;
 std::map<std::string, JitModuleSet*> g_sets;    // "device|cache key" -> loaded set (kept until the process ends)
 
+// Whether the compiler behind hipRTC (libamd_comgr, loaded by name) knows the options that this library is built with. A program that loaded
+// another ROCm's libraries first (torch brings its own) gets that one's, older or newer, and an option that a compiler does not know ends the
+// process. The one in use is asked for its installation's version; without an answer it counts as another one.
+bool compiler_of_the_build() {
+    std::vector<std::string> found;
+    dl_iterate_phdr([](dl_phdr_info* info, size_t, void* to) {
+        if (info->dlpi_name && strstr(info->dlpi_name, "libamd_comgr")) ((std::vector<std::string>*)to)->push_back(info->dlpi_name);
+        return 0;
+    }, &found);
+    const auto directory = [](const std::string& file) {
+        char real[PATH_MAX];
+        if (!realpath(file.c_str(), real)) return std::string();
+        const std::string r = real;
+        return r.substr(0, r.rfind('/'));
+    };
+    if (found.empty()) {                                    // hipRTC loads the one beside it
+        Dl_info info{};
+        if (!dladdr((void*)&hiprtcCompileProgram, &info) || !info.dli_fname) return false;
+        const std::string file = directory(info.dli_fname) + "/libamd_comgr.so.3";
+        if (!dlopen(file.c_str(), RTLD_LAZY)) return false;
+        found.push_back(file);
+    }
+    for (const auto& file : found) {
+        std::ifstream f(directory(file) + "/../.info/version");
+        int major = 0, minor = 0;
+        char dot = 0;
+        if (!(f >> major >> dot >> minor) || major * 100 + minor < HIP_VERSION_MAJOR * 100 + HIP_VERSION_MINOR) return false;
+    }
+    return true;
+}
+
 // The compiler options of the library's own build (build.py) for the two groups of kernels: every
 // fused multiply-add written out, no packed FP32, matrix results straight into VGPRs; the matrix-core
 // kernels also with relaxed NaN handling and the IEEE mode bit off.
 std::vector<std::string> options(const std::string& arch, const std::string& csrc, bool pop) {
     std::vector<std::string> o = { "--offload-arch=" + arch, "-O3", "-std=c++17", "-ffp-contract=off", "-I" + csrc,
-                                   "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-mllvm", "-amdgpu-mfma-vgpr-form" };
+                                   "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops" };
+    if (compiler_of_the_build()) { o.push_back("-mllvm"); o.push_back("-amdgpu-mfma-vgpr-form"); }   // (registers only: the same results without)
     if (pop) { o.push_back("-fno-honor-nans"); o.push_back("-mno-amdgpu-ieee"); }
     return o;
 }
