@@ -104,7 +104,7 @@ int ntc_op_adamw(const ntc_adamw_desc* d, void* stream, char* why, size_t why_ca
 /* The values that an 8-bit state stands for: count (a multiple of 256) values of m and of v as 32-bit floats. */
 int ntc_op_adamw_moments(const void* exp_avg, const void* exp_avg_sq, const uint8_t* exp_avg_exp, const uint8_t* exp_avg_sq_exp,
                          int64_t count, float* m, float* v, void* stream, char* why, size_t why_cap);
-/* The nearest 8-bit state to count (a multiple of 256) values of m and v. */
+/* The nearest 8-bit state to count (a multiple of 256) values of m and v (a v below 0, or -0, counts as 0). */
 int ntc_op_adamw_encode(const float* m, const float* v, int64_t count, void* exp_avg, void* exp_avg_sq, uint8_t* exp_avg_exp,
                         uint8_t* exp_avg_sq_exp, void* stream, char* why, size_t why_cap);
 

@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(256) k_adamw_encode(const float* im, const flo
     if (at >= n) return;
     const auto r = *(const Run<float, 4>*)(im + at), q = *(const Run<float, 4>*)(iv + at);
     float m[4], v[4];
-    for (int j = 0; j < 4; j++) { m[j] = r.v[j]; v[j] = q.v[j]; }
+    for (int j = 0; j < 4; j++) { m[j] = r.v[j]; v[j] = q.v[j] <= 0.0f ? 0.0f : q.v[j]; }   // (v has no sign: a set bit would reach into the next code)
     const uint32_t half[4] = { 32768, 32768, 32768, 32768 };
     const Codes c = encode_block(m, v, half, half);
     *(uint32_t*)(cm + at) = c.m;

@@ -293,6 +293,21 @@ def test_set_moments_rounds_to_nearest():
     near(b, v.double(), v.double() / 16 * 1.0001 + 2.0 ** -33, "v")
 
 
+@pytest.mark.parametrize("at", [0, 1, 2, 3])
+def test_set_moments_takes_a_v_without_sign(at):
+    """-0 and values below 0 count as 0, and the codes beside them (four to a word) are what they are without."""
+    opt = ops().AdamW([torch.zeros(512, device="cuda")], state_bits=8)
+    m, v = torch.randn(512, generator=gen(4), device="cuda"), 0.25 + torch.rand(512, generator=gen(5), device="cuda")
+    clean, signed = v.clone(), v.clone()
+    clean[at::4] = 0.0
+    signed[at::8], signed[at + 4::8] = -0.0, -0.125
+    opt.set_moments(m, clean)
+    wanted = [t.clone() for t in opt.moments()]
+    opt.set_moments(m, signed)
+    assert all(torch.equal(a, b) for a, b in zip(opt.moments(), wanted))
+
+
+
 def test_more_than_2_31_values():
     print("adamw large", flush=True)
     n = 2 ** 31 + 1000
