@@ -6,6 +6,7 @@
 #include <torch/extension.h>
 
 #include <cmath>
+#include <cstring>
 #include <optional>
 #include <vector>
 
@@ -357,7 +358,9 @@ Tensor linear_fp8(const Tensor& x, const Tensor& codes, const Tensor& exps, int6
 struct AdamwPlan {
     std::vector<Tensor> params;
     std::vector<const void*> pointers;
-    Tensor table, chunk_tensor;
+    Tensor tables;                                          // on the device: the tensors, then each chunk's
+    const ntc_adamw_tensor* table = nullptr;
+    const int32_t* chunk_tensor = nullptr;
     std::vector<int64_t> first_chunk, offsets;
     std::vector<int32_t> steps;
     int64_t size = 0, calls = 0;
@@ -385,9 +388,14 @@ struct AdamwPlan {
         std::sort(spans.begin(), spans.end());
         for (size_t i = 1; i < spans.size(); i++) TORCH_CHECK_VALUE(spans[i - 1].second <= spans[i].first, "parameters overlap");
         const c10::DeviceGuard guard(params[0].device());
-        const auto up = [&](void* p, size_t n) { return at::from_blob(p, { (int64_t)n }, at::kByte).to(params[0].device()); };
-        table = up(rows.data(), rows.size() * sizeof(rows[0]));
-        chunk_tensor = up(of_chunk.data(), of_chunk.size() * sizeof(of_chunk[0]));
+        // one copy to the device for both: it waits, and costs more than what it moves
+        const size_t rows_size = rows.size() * sizeof(rows[0]), chunks_size = of_chunk.size() * sizeof(of_chunk[0]);
+        std::vector<uint8_t> both(rows_size + chunks_size);
+        std::memcpy(both.data(), rows.data(), rows_size);
+        if (chunks_size) std::memcpy(both.data() + rows_size, of_chunk.data(), chunks_size);
+        tables = at::from_blob(both.data(), { (int64_t)both.size() }, at::kByte).to(params[0].device());
+        table = (const ntc_adamw_tensor*)tables.const_data_ptr();
+        chunk_tensor = (const int32_t*)((const uint8_t*)tables.const_data_ptr() + rows_size);
         steps.resize(params.size());
     }
 
@@ -413,8 +421,8 @@ struct AdamwPlan {
         }
         const auto at_ = [](const optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; };
         ntc_adamw_desc d = {};
-        d.tensors = (const ntc_adamw_tensor*)table.const_data_ptr();
-        d.chunk_tensor = (const int32_t*)chunk_tensor.const_data_ptr();
+        d.tensors = table;
+        d.chunk_tensor = chunk_tensor;
         d.first_chunk = first_chunk.data();
         d.grads = g.data();
         d.grad_types = types.data();
