@@ -257,9 +257,12 @@ template <class T, bool kBlock> __device__ __forceinline__ void quantize_tile(co
     }
 }
 
+constexpr int kGridRows = 1 << 15;                           // of tiles, in a grid's second dimension; more go into its third
 template <class T, bool kBlock> __global__ void __launch_bounds__(256) k_fp8_quantize(ntc_fp8_quantize_desc d) {
     __shared__ QuantizeSpace<T> space;
-    quantize_tile<T, kBlock>(d, blockIdx.y, blockIdx.x, space);
+    const long long tile_r = blockIdx.y + (long long)blockIdx.z * kGridRows;
+    if (tile_r * 128 >= d.R) return;
+    quantize_tile<T, kBlock>(d, tile_r, blockIdx.x, space);
 }
 // Two matrices, the first in blocks of 1 x 128, the second of 128 x 128 (a layer's values and its weights): a launch less.
 template <class T> __global__ void __launch_bounds__(256) k_fp8_quantize_pair(ntc_fp8_quantize_desc a, ntc_fp8_quantize_desc b, uint32_t tiles_a, uint32_t across_a, uint32_t across_b) {
@@ -699,7 +702,7 @@ static int check_quantize(const ntc_fp8_quantize_desc* d, char* why, size_t cap)
     if (d->dtype < 0 || d->dtype > 2) return refuse(why, cap, "x is 32-bit floats, bfloat16 or float16");
     if (d->block_rows != 1 && d->block_rows != 128) return refuse(why, cap, "blocks are 1 x 128 or 128 x 128");
     if (!d->codes && !d->codes_t) return refuse(why, cap, "nothing to write");
-    if ((d->R + 127) / 128 > 65535 || (d->K + 127) / 128 >= 1 << 24) return refuse(why, cap, "at most 65535 * 128 rows, and fewer than 2^31 columns");
+    if (d->R > (int64_t)1 << 36 || (d->K + 127) / 128 >= 1 << 24) return refuse(why, cap, "at most 2^36 rows, and fewer than 2^31 columns");
     if (d->R && d->K && (!d->x || (d->codes && !d->exps) || (d->codes_t && !d->exps_t))) return refuse(why, cap, "a null pointer");
     return 0;
 }
@@ -707,7 +710,9 @@ static int check_quantize(const ntc_fp8_quantize_desc* d, char* why, size_t cap)
 extern "C" int ntc_op_fp8_quantize(const ntc_fp8_quantize_desc* d, void* stream, char* why, size_t cap) {
     if (const int r = check_quantize(d, why, cap)) return r;
     if (!d->R || !d->K) return 0;
-    const auto go = [&](auto kernel) { kernel<<<dim3((unsigned)((d->K + 127) / 128), (unsigned)((d->R + 127) / 128)), 256, 0, (hipStream_t)stream>>>(*d); };
+    const int64_t down = (d->R + 127) / 128;
+    const dim3 grid((unsigned)((d->K + 127) / 128), (unsigned)(down < kGridRows ? down : kGridRows), (unsigned)((down + kGridRows - 1) / kGridRows));
+    const auto go = [&](auto kernel) { kernel<<<grid, 256, 0, (hipStream_t)stream>>>(*d); };
     if (d->block_rows == 128) d->dtype == NTC_F32 ? go(k_fp8_quantize<f32, true>) : d->dtype == NTC_BF16 ? go(k_fp8_quantize<bf16, true>) : go(k_fp8_quantize<f16, true>);
     else d->dtype == NTC_F32 ? go(k_fp8_quantize<f32, false>) : d->dtype == NTC_BF16 ? go(k_fp8_quantize<bf16, false>) : go(k_fp8_quantize<f16, false>);
     return launched(why, cap);

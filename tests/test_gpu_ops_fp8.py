@@ -268,3 +268,29 @@ def test_products_past_32_bit_offsets():
     b = ops().fp8_quantize(torch.ones((N, K), device="cuda"), 128)
     y = ops().fp8_matmul(a, b, torch.float32)
     assert (y[0] == 128).all() and (y[-1] == K).all() and not y[1:-1].any()
+
+
+@pytest.mark.parametrize("rows", [1, 128])
+def test_more_rows_than_a_grid_dimension_takes(rows):
+    """A row's codes are its own block's, wherever it lies: the ends and the middle of 9 million rows as matrices of their own."""
+    R, K, step = 9_000_001, 5, 128 * 2 ** 15
+    print("quantize", R, K, rows, flush=True)
+    x = randn(21, R, K).to(torch.bfloat16)
+    q, t = ops().fp8_quantize_both(x, rows)
+    for a in (0, step - 256, step, 2 * step - 128, 2 * step, R // 128 * 128):
+        b = min(R, a + 512)
+        one, other = ops().fp8_quantize_both(x[a:b], rows)
+        assert torch.equal(q.codes[a:b], one.codes), a
+        assert torch.equal(q.exps[a // rows:(b + rows - 1) // rows], one.exps), a
+        assert torch.equal(t.codes[:, a:b], other.codes[:, :b - a]), a
+        n = (b - a + 127) // 128
+        assert torch.equal(t.exps[:, a // 128:a // 128 + n], other.exps[:, :n]), a
+
+
+def test_an_inference_layer_of_more_rows_than_2_23():
+    R, K, N = 2 ** 23 + 77, 16, 16
+    print("linear", R, K, N, flush=True)
+    x, w = randn(22, R, K).to(torch.bfloat16), ops().fp8_quantize(randn(23, N, K).to(torch.bfloat16), 128)
+    y = ops().fp8_linear(x, w)
+    for a in (0, 2 ** 22 - 64, 2 ** 23 - 100, R - 300):
+        assert torch.equal(y[a:a + 300], ops().fp8_linear(x[a:a + 300], w)[:300]), a
