@@ -27,8 +27,8 @@ __device__ __forceinline__ void soft_join(Soft& a, Soft b, float k) {
     a.t += b.t;
 }
 
-// log p of one value, in nats: not through (x - m) k, which overflows for a mask of the lowest value
-__device__ __forceinline__ float log_prob(float x, float m, float inv_t, float log_s) { return (x - m) * inv_t - kLn2 * log_s; }
+// log p of one value, in nats: not through (x - m) k, which overflows for a mask of the lowest value, and on halves, since the difference itself may
+__device__ __forceinline__ float log_prob(float x, float m, float inv_t, float log_s) { return 2.0f * ((0.5f * x - 0.5f * m) * inv_t) - kLn2 * log_s; }
 
 __device__ __forceinline__ long long token_of(const ntc_logprobs_desc& d, long long outer, long long inner) {
     const long long at = outer * d.token_outer_stride + inner * d.token_inner_stride;
