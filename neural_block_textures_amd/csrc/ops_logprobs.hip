@@ -617,7 +617,9 @@ template <class T> __device__ __forceinline__ Soft scan_again(const T* x, int V,
     a.t = reduce64(a.t, sum);
     return a;
 }
-__device__ __forceinline__ bool plain_sum(float s) { return s > 0.0f && s < NTC_INF; }
+// Whether a joined sum is that of an ordinary row: its largest value adds 1, and there are fewer than 2^31. (Less: all lie below the floor, and what is
+// small beside them has been lost; more: they reach past lim, and the second sum may have overflowed first.)
+__device__ __forceinline__ bool plain_sum(float s) { return s > 0.5f && s < 0x1p40f; }
 
 __device__ __forceinline__ Soft join_lanes(Soft a, float k) {
     const auto sum = [](float p, float q) { return p + q; };

@@ -1,4 +1,5 @@
-"""token_logprobs where its arithmetic has its ends: values at both ends of the type. A call holds rows of one kind only, so that no other row of a wave sends them down a more careful path. Definitions
+"""token_logprobs where its arithmetic has its ends: values at both ends of the type, and
+temperatures far from 1. A call holds rows of one kind only, so that no other row of a wave sends them down a more careful path. Definitions
 and tolerances are those of test_gpu_ops_logprobs.py, of which what no longer fits a result's type is infinite."""
 import math
 
@@ -40,6 +41,21 @@ SHORT = [5, 33, 64, 100, 256, 300, 512, 1000]          # groups of 4 to 64 lanes
 
 def fits(value, dtype):
     return abs(value) <= torch.finfo(dtype).max
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [2000, 9001])
+def test_temperatures_of_long_rows(V, dtype):
+    """From nearly one symbol to nearly all alike; what is past a row's end counts nowhere."""
+    print("logprobs temperatures", V, dtype, flush=True)
+    x, t = make(70, V, dtype, seed=V + 1)
+    wide = (x.float() * (1e37 if fits(1e38, dtype) else 1e4)).to(dtype)
+    wide = torch.where(torch.isfinite(wide), wide, torch.zeros_like(wide))
+    for T in (1e-30, 1e-10, 1e-3, 1e3, 1e10, 1e25):
+        check(x.clone(), t, min(4, V), T=T)
+    for T in (1e30, 1e34, 1e36, 2.0 ** 120):
+        check(x.clone(), t, min(4, V), T=T, grad=False)
+        check(wide.clone(), t, min(4, V), T=T, grad=False)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
