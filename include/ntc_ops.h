@@ -38,14 +38,14 @@ typedef struct ntc_logprobs_desc {
     int64_t ignore_index;
     int32_t dtype, token_bytes;
     int32_t top;
-    float temperature;
+    float temperature;    /* from 2^-127 to 2^120 */
     float* logprob;       /* [rows] */
     float* entropy;       /* [rows] */
     float* stats;         /* [rows][2] */
     int64_t* top_ids;     /* [rows][top] */
     float* top_logprobs;  /* [rows][top] */
     void* workspace;
-    /* backward only: gradients of the outputs (null: none), each row's at a stride of 0 or 1 rows */
+    /* backward only: gradients of the outputs (null: none), laid out as these are */
     const float* g_logprob;
     const float* g_entropy;
     const float* g_top;   /* [rows][top] */

@@ -1,4 +1,6 @@
 // Token log probabilities with entropy and the best alternatives, and their gradient (include/ntc_ops.h).
+#include <string.h>
+
 #include "ops_common.hpp"
 
 namespace ntc_ops {
@@ -151,7 +153,12 @@ template <class K> __device__ __forceinline__ void sort16(K (&a)[16]) {
                     a[j + k] = x > y ? y : x;
                 }
 }
-template <class T, int kGroup, bool kSorted> __global__ void __launch_bounds__(256) k_logprobs_short(ntc_logprobs_desc d, float lim, float k, float inv_t) {
+//
+// The sums are taken on products x k - m k, one operation fewer a value than on differences, where these stay exact: |m k| up to `most` = 2^24 (its
+// rounding, which every exponent is off by, is then at most 1/2 and is taken out again; past 2^31 it would be beyond an exponential's range), k from 2^-60
+// on (what is past a row's end stands as -lim, and exp2(-lim k) has to be 0; `most` is -1 for smaller ones), and no product that overflows to an infinity
+// whose e of 0 would give 0 * inf: values below -lim (`low`: that as a 16-bit key) go with the infinities and NaN.
+template <class T, int kGroup, bool kSorted> __global__ void __launch_bounds__(256) k_logprobs_short(ntc_logprobs_desc d, float lim, int low, float most, float k, float inv_t) {
     constexpr int kEach = 16, kVec = 16 / (int)sizeof(T), kRows = 256 / kGroup;
     constexpr bool kPlaced = sizeof(T) == 4;
     static_assert(kGroup * kEach <= kShort, "indices of 10 bits");
@@ -178,7 +185,7 @@ template <class T, int kGroup, bool kSorted> __global__ void __launch_bounds__(2
     const int V = (int)d.V, at = in * kEach;
     float v[kEach];
     s2 pair[kEach / 2], least = { 0, 0 };                    // keys of 16-bit values, and the least of the whole vectors'
-    bool odd = false;                                        // a 16-bit infinity or NaN
+    bool odd = false;                                        // a 16-bit value below -lim, infinity or NaN
 #pragma unroll
     for (int i = 0; i < kEach; i += kVec) {
         const int left = V - at - i;                         // of this vector's values
@@ -231,7 +238,7 @@ template <class T, int kGroup, bool kSorted> __global__ void __launch_bounds__(2
             return above((int)p[0], (int)p[1]);
         };
         int top = most();
-        odd = top >= H::kInf || below((int)least[0], (int)least[1]) <= -H::kInf;
+        odd = top >= H::kInf || below((int)least[0], (int)least[1]) <= -low;
         odd = __ballot(odd) != 0;
         if (odd) {                                           // a NaN counts as -inf in the order
             asm volatile("");                                // (a branch, not selections that every row would make)
@@ -251,8 +258,7 @@ template <class T, int kGroup, bool kSorted> __global__ void __launch_bounds__(2
     const float mm = m == -NTC_INF ? 0.0f : m;              // nothing left: every exponential is 0
     float s = 0.0f, t = 0.0f;
     const float mk = mm * k, off = __builtin_fmaf(mm, k, -mk);
-    // on products, which do not overflow here (one operation fewer a value than on differences); the exponents are `off` too large
-    if (__ballot(!(fabsf(mm) <= 0.5f * lim)) == 0) {
+    if (__ballot(!(fabsf(mk) <= most)) == 0) {              // the exponents are `off` too large
         if (!kPlaced && !odd) {
 #pragma unroll
             for (int j = 0; j < kEach; j++) {
@@ -887,6 +893,10 @@ template <class T> static Reading reading(int64_t rows, int64_t V, int top) {
 template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s) {
     const auto blocks = [&](int per) { return grid_of((d.rows + per - 1) / per); };
     const float k = kLog2e / d.temperature, lim = 1e30f / (k > 1.0f ? k : 1.0f);   // values up to lim times k stay far from overflow
+    const float most = k >= 0x1p-60f ? 0x1p24f : -1.0f;
+    uint32_t bits;
+    memcpy(&bits, &lim, 4);
+    const int low = type_code<T> == NTC_BF16 ? (int)(bits >> 16) : lim > 65504.0f ? 0x7c00 : 0;   // lim as such a type's bits (float16: its infinity's, or every row is looked at)
     // Up to 512 values, and 1024 of 16 bits, a row is held in registers, in the fewest lanes of 16 values (against reading it as a long one: bf16
     // 200000 x 256 23 against 96 us, 50000 x 1000 with 4 alternatives 38 against 46; float32 100000 x 512 31 against 40, but 50000 x 1000 54 against 37).
     // Short rows of many alternatives sort each lane's values first, where that beats finding its three best again and again (bf16, with 32: 400000 x 64
@@ -897,8 +907,8 @@ template <class T> static void forward(const ntc_logprobs_desc& d, hipStream_t s
         const dim3 grid = blocks(256 / g);
         constexpr int from = sizeof(T) == 4 ? (g > 12 ? g : 12) : g > 16 ? g / 2 : 8;
         if constexpr (from <= NTC_MAX_TOP)
-            if (d.top >= from) { k_logprobs_short<T, g, true><<<grid, 256, 0, s>>>(d, lim, k, 1.0f / d.temperature); return; }
-        k_logprobs_short<T, g, false><<<grid, 256, 0, s>>>(d, lim, k, 1.0f / d.temperature);
+            if (d.top >= from) { k_logprobs_short<T, g, true><<<grid, 256, 0, s>>>(d, lim, low, most, k, 1.0f / d.temperature); return; }
+        k_logprobs_short<T, g, false><<<grid, 256, 0, s>>>(d, lim, low, most, k, 1.0f / d.temperature);
     };
     if (d.V <= 64) return shorts(std::integral_constant<int, 4>());
     if (d.V <= 128) return shorts(std::integral_constant<int, 8>());
@@ -940,7 +950,8 @@ static int check(const ntc_logprobs_desc* d, bool backward, char* why, size_t ca
     if (d->dtype < 0 || d->dtype > 2) return refuse(why, cap, "logits are 32-bit floats, bfloat16 or float16");
     if (d->token_bytes != 4 && d->token_bytes != 8) return refuse(why, cap, "tokens are 32- or 64-bit integers");
     if (d->top < 0 || d->top > NTC_MAX_TOP || d->top > d->V) return refuse(why, cap, "top is 0 to 32 and at most V");
-    if (!(d->temperature > 0.0f) || d->temperature > 3e38f) return refuse(why, cap, "temperature is positive and finite");
+    // (below, 1 / T is infinite; above, differences of logits that overflow would still have an exponential)
+    if (!(d->temperature >= 0x1p-127f && d->temperature <= 0x1p120f)) return refuse(why, cap, "temperature is from 2^-127 to 2^120");
     if (d->rows == 0) return 0;
     if (!d->logits || !d->tokens || !d->stats || !d->entropy) return refuse(why, cap, "a null pointer");
     if (!backward && (!d->logprob || (d->top && (!d->top_ids || !d->top_logprobs)))) return refuse(why, cap, "a null pointer");

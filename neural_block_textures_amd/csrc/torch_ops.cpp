@@ -159,7 +159,7 @@ py::tuple token_logprobs(const Tensor& logits, Tensor tokens, int64_t top, doubl
     const int64_t V = logits.size(-1);
     TORCH_CHECK_VALUE(V >= 1 && (V == 1 || logits.stride(-1) == 1), "a row of logits must hold at least one value, contiguous");
     TORCH_CHECK_VALUE(top >= 0 && top <= std::min<int64_t>(NTC_MAX_TOP, V), "top is 0 to ", std::min<int64_t>(NTC_MAX_TOP, V), ", not ", top);
-    TORCH_CHECK_VALUE(temperature > 0 && temperature < 3e38, "temperature must be positive and finite, not ", temperature);
+    TORCH_CHECK_VALUE(temperature >= 0x1p-127 && temperature <= 0x1p120, "temperature must be from 2^-127 to 2^120, not ", temperature);
     if (tokens.dim() > 2) tokens = tokens.contiguous();
     if (logits.requires_grad() && at::GradMode::is_enabled()) {
         auto r = LogprobsNode::apply(logits, tokens, top, temperature, ignore);

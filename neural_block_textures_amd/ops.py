@@ -101,7 +101,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
     most probable symbols in descending order, equal ones by ascending index.
 
     logits [.., V]: float32, bfloat16 or float16, a row's values contiguous, rows at any two strides (a [batch, time, V] tensor's
-    [:, :-1] as it lies). tokens [..]: int32 or int64. A token equal to ignore_index has logprob 0 and no gradient;
+    [:, :-1] as it lies). tokens [..]: int32 or int64. temperature: 2^-127 to 2^120. A token equal to ignore_index has logprob 0 and no gradient;
     another one outside [0, V) has logprob NaN. -inf masks a symbol; a row with nothing left has log probabilities -inf, entropy 0
     and gradient 0; a NaN or +inf makes its row's results NaN (ids then order NaN as -inf). logprob, entropy and top_logprobs are
     differentiable in logits (once); log probabilities and sums are 32-bit, dlogits is rounded once to the logits' type.

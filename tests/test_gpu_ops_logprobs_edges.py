@@ -1,8 +1,6 @@
-"""token_logprobs where its arithmetic has its ends: values at both ends of the type, and
+"""token_logprobs where short rows' arithmetic has its ends: large finite logits, masks of the type's lowest value beside ordinary ones, and
 temperatures far from 1. A call holds rows of one kind only, so that no other row of a wave sends them down a more careful path. Definitions
 and tolerances are those of test_gpu_ops_logprobs.py, of which what no longer fits a result's type is infinite."""
-import math
-
 import pytest
 import torch
 
@@ -44,8 +42,46 @@ def fits(value, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V", [2000, 9001])
-def test_temperatures_of_long_rows(V, dtype):
+@pytest.mark.parametrize("V", SHORT + [2000])
+def test_large_values(V, dtype):
+    """Rows of one value, all but one, and neighbours of it: log V where all are equal, whatever their size."""
+    print("logprobs large", V, dtype, flush=True)
+    n = 70
+    t = torch.arange(n, device="cuda") % V
+    for size in (5e4, 1e7, 1e8, 1e9, 1e10, 1e15, 1e25, 1e35):
+        for value in (size, -size):
+            if not fits(value, dtype):
+                continue
+            same = torch.full((n, V), value, device="cuda").to(dtype)
+            one = same.clone()
+            one[:, V // 2] = 0
+            close = same.clone()
+            close[:, ::3] = torch.nextafter(close[:, ::3].float(), torch.zeros((), device="cuda")).to(dtype)
+            for T in (0.1, 1.0, 1.3):
+                for x in (same, one, close):
+                    check(x.clone(), t, min(4, V), T=T)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", SHORT + [2000])
+def test_masks_of_the_lowest_value_alone(V, dtype):
+    """A third and all but three symbols masked by finite values; no infinity or NaN anywhere."""
+    print("logprobs lowest", V, dtype, flush=True)
+    for low in (torch.finfo(dtype).min, -1e9, -1e30, -3e38):
+        if not fits(low, dtype):
+            continue
+        some, t = make(70, V, dtype, seed=V)
+        some[:, ::3] = low
+        few = torch.full_like(some, low)
+        few[:, [0, V // 2, V - 1]] = torch.tensor([0.5, 2.0, 1.0], device="cuda", dtype=dtype)
+        for T in (0.25, 1.0, 2.0):
+            for x in (some, few):
+                check(x.clone(), t, min(5, V), T=T)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", SHORT + [2000, 9001])
+def test_temperatures(V, dtype):
     """From nearly one symbol to nearly all alike; what is past a row's end counts nowhere."""
     print("logprobs temperatures", V, dtype, flush=True)
     x, t = make(70, V, dtype, seed=V + 1)
@@ -68,5 +104,14 @@ def test_both_ends_of_the_type(V, dtype):
     x[:, V // 3] = big
     x[1::2, 0] = 0
     t = torch.arange(70, device="cuda") % V
-    for T in (1.0, 10.0):
+    for T in (1.0, 10.0, 1e20):
         check(x.clone(), t, min(3, V), T=T)
+    for T in (1e36, 2.0 ** 120):
+        check(x.clone(), t, min(3, V), T=T, grad=False)
+
+
+def test_temperatures_out_of_range():
+    x, t = make(4, 33, torch.float32)
+    for T in (2.0 ** -128, 2.0 ** 121, 1e38):
+        with pytest.raises(ValueError, match="temperature must be from"):
+            ops().token_logprobs(x, t, temperature=T)
