@@ -15,6 +15,10 @@
 extern "C" {
 #endif
 
+/* Where this library finds the runtime's hipStreamSynchronize: a program in which two HIP runtimes may be loaded compares it with its own. Streams,
+ * and the order of work on them, are one runtime's; a stream of another is none that these calls can take. */
+const void* ntc_op_runtime(void);
+
 enum { NTC_F32 = 0, NTC_BF16 = 1, NTC_F16 = 2 };     /* element types */
 enum { NTC_MAX_TOP = 32 };                           /* alternatives of ntc_op_token_logprobs */
 enum { NTC_STATE_BLOCK = 256 };                      /* values that share one scale of an 8-bit optimizer state */

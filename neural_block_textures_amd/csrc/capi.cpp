@@ -178,6 +178,7 @@ size_t ntc_abi_sizeof(const char* name) {
     if (n == "ntc_fp8_matmul_desc") return sizeof(ntc_fp8_matmul_desc);
     return 0;
 }
+const void* ntc_op_runtime(void) { return (const void*)&hipStreamSynchronize; }
 long long ntc_trainer_nparams(const ntc_trainer* t) { return t->t.im->P; }
 long long ntc_trainer_nz(const ntc_trainer* t) { return (long long)t->t.im->nz; }
 void* ntc_trainer_stream(const ntc_trainer* t) { return (void*)t->t.im->stream; }

@@ -5,6 +5,8 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <dlfcn.h>
+
 #include <cmath>
 #include <cstring>
 #include <optional>
@@ -34,6 +36,19 @@ template <class F> void call(const c10::Device& device, F entry) {
     const int rc = entry((void*)c10::hip::getCurrentHIPStream(device.index()).stream(), why, sizeof(why));
     TORCH_CHECK_VALUE(rc != 1, why);
     TORCH_CHECK(rc == 0, why);
+}
+
+// The files of the HIP runtimes that the kernels' library and torch use. They name theirs differently, so that both end up in a process that loads
+// the library first, and torch's streams are not the library's then.
+std::pair<std::string, std::string> runtimes() {
+    const auto file = [](const void* p) {
+        Dl_info info{};
+        return p && dladdr(p, &info) && info.dli_fname ? std::string(info.dli_fname) : std::string();
+    };
+    const void* torchs = dlsym(dlopen(nullptr, RTLD_LAZY), "hipStreamSynchronize");   // (what is in the global scope comes before a library's own)
+    if (!torchs)
+        if (void* c10 = dlopen("libc10_hip.so", RTLD_NOLOAD | RTLD_LAZY)) torchs = dlsym(c10, "hipStreamSynchronize");
+    return { file(ntc_op_runtime()), file(torchs) };
 }
 
 Tensor bytes(int64_t n, const Tensor& like) { return at::empty({ n }, like.options().dtype(at::kByte).requires_grad(false)); }
@@ -467,6 +482,7 @@ void adamw_encode(const Tensor& m, const Tensor& v, const Tensor& cm, const Tens
 
 PYBIND11_MODULE(_ops, m) {
     m.doc() = "The operators of ops.py on torch tensors";
+    m.def("runtimes", &runtimes);
     m.def("token_logprobs", &token_logprobs);
     m.def("quantize", &quantize);
     m.def("matmul", [](const Tensor& ac, const Tensor& ae, int64_t M, int64_t ka, int64_t a_block, const Tensor& bc, const Tensor& be, int64_t N, int64_t kb, int64_t b_block, py::object type) {

@@ -5,7 +5,8 @@
     fp8_quantize(x), fp8_matmul(a, b)         8-bit floating point with a power-of-two scale for each block of 128
     fp8_linear(x, w)                          a layer in it, for training or, with weights laid out once, for inference
 
-Tensors are on the GPU; work is enqueued on torch's current stream and nothing waits. Arguments that an operator does not
+Tensors are on the GPU; work is enqueued on torch's current stream and nothing waits. torch, or this module, has to be imported before
+libntc_hip.so is loaded (by the first Trainer), so that both use one HIP runtime; the other order raises. Arguments that an operator does not
 take raise ValueError, errors of the runtime RuntimeError. There is no fallback: the kernels are libntc_hip.so's.
 """
 from __future__ import annotations
@@ -83,6 +84,10 @@ def _binding():
         if not os.path.exists(os.path.join(trainer.PKG, "_ops.so")):
             raise RuntimeError("_ops.so is not built; run `python -m neural_block_textures_amd.build` (or __graft_entry__.build()) first")
         from . import _ops
+        ours, torchs = _ops.runtimes()
+        if ours != torchs:
+            raise RuntimeError(f"two HIP runtimes are loaded, {ours} and torch's {torchs}, and a stream of one is none of the other: import torch (or "
+                               "neural_block_textures_amd.ops) before the first use of neural_block_textures_amd.trainer")
         _bound = _ops
     return _bound
 
