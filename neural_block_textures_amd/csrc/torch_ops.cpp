@@ -29,6 +29,11 @@ void floats(const char* name, const Tensor& t) {
     TORCH_CHECK_VALUE(type_of(t) >= 0, name, " is ", t.scalar_type(), "; it can be float32, bfloat16, float16");
 }
 
+// Forward-mode derivatives are not there either: a tangent would be dropped without a word.
+void no_tangent(const char* name, const Tensor& t) {
+    TORCH_CHECK_VALUE(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), name, " has a tangent; there is no forward-mode derivative");
+}
+
 // One entry point on a device's current stream: a refusal is a ValueError, an error of the runtime a RuntimeError.
 template <class F> void call(const c10::Device& device, F entry) {
     const c10::DeviceGuard guard(device);
@@ -167,6 +172,7 @@ struct LogprobsNode : torch::autograd::Function<LogprobsNode> {
 
 py::tuple token_logprobs(const Tensor& logits, Tensor tokens, int64_t top, double temperature, int64_t ignore) {
     floats("logits", logits);
+    no_tangent("logits", logits);
     on_gpu("tokens", tokens);
     TORCH_CHECK_VALUE(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt, "tokens is ", tokens.scalar_type(), "; it can be int64, int32");
     TORCH_CHECK_VALUE(logits.dim() >= 1 && tokens.sizes() == logits.sizes().slice(0, logits.dim() - 1) && tokens.device() == logits.device(),
@@ -337,6 +343,8 @@ Tensor like_rows(const Tensor& y, const Tensor& x) {
 Tensor linear(const Tensor& x, const Tensor& w) {
     floats("x", x);
     floats("w", w);
+    no_tangent("x", x);
+    no_tangent("w", w);
     TORCH_CHECK_VALUE(x.dim() >= 1, "x must have at least one axis");
     TORCH_CHECK_VALUE(w.dim() == 2 && w.size(1) == x.size(-1) && w.device() == x.device(), "w ", w.sizes(), " must be a matrix with x's ", x.size(-1), " columns, on its device");
     const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad());
@@ -352,6 +360,7 @@ Tensor linear(const Tensor& x, const Tensor& w) {
 
 Tensor linear_fp8(const Tensor& x, const Tensor& codes, const Tensor& exps, int64_t N, int64_t K, int64_t block) {
     floats("x", x);
+    no_tangent("x", x);
     const Operand b = given("w", codes, exps, N, K, block);
     TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == K && x.device() == codes.device(), "x ", x.sizes(), " must have w's ", K, " columns, on its device");
     TORCH_CHECK_VALUE(!(x.requires_grad() && at::GradMode::is_enabled()), "w in 8 bits is for inference: give the weights themselves for a gradient");

@@ -7,7 +7,7 @@
 
 Tensors are on the GPU; work is enqueued on torch's current stream and nothing waits. torch, or this module, has to be imported before
 libntc_hip.so is loaded (by the first Trainer), so that both use one HIP runtime; the other order raises. Arguments that an operator does not
-take raise ValueError, errors of the runtime RuntimeError. There is no fallback: the kernels are libntc_hip.so's.
+take (tensors with a forward-mode tangent among them) raise ValueError, errors of the runtime RuntimeError. There is no fallback: the kernels are libntc_hip.so's.
 """
 from __future__ import annotations
 
