@@ -105,12 +105,20 @@ __device__ __forceinline__ void decode_block(uint32_t cm, uint32_t cv, int me, i
 }
 
 // ---------------------------------------------------------------- the step
-// Four values of one tensor. The division and the root are the hardware's, an ulp each: a 2^-22 of the update, where p keeps 2^-24 of itself.
-__device__ __forceinline__ void update(const AdamArgs& A, float rate, float root, const float (&g)[4], float (&p)[4], float (&m)[4], float (&v)[4]) {
+// Four values of one tensor. The division and the root are the hardware's, an ulp each: a 2^-22 of the update, where p keeps 2^-24 of itself. They take a
+// subnormal number as 0, which eps hides unless it is small. `kSmall`, it is: small v are taken 2^64 times and the sum 2^24 times as large (2^28 bf16 values
+// with an 8-bit state 531 us against 507; with 32-bit state the same).
+template <bool kSmall> __device__ __forceinline__ void update(const AdamArgs& A, float rate, float root, const float (&g)[4], float (&p)[4], float (&m)[4], float (&v)[4]) {
     for (int j = 0; j < 4; j++) {
         m[j] = m[j] * A.b1 + g[j] * A.nb1;
         v[j] = v[j] * A.b2 + (g[j] * g[j]) * A.nb2;
-        p[j] = p[j] * A.keep - rate * (m[j] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[j]) * root + A.eps));
+        if (kSmall) {
+            const bool low = v[j] < 0x1p-96f;
+            const float below = __builtin_amdgcn_sqrtf(low ? v[j] * 0x1p64f : v[j]) * (low ? root * 0x1p-32f : root) + A.eps;
+            p[j] = p[j] * A.keep - rate * (m[j] * __builtin_amdgcn_rcpf(below * 0x1p24f) * 0x1p24f);
+        } else {
+            p[j] = p[j] * A.keep - rate * (m[j] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[j]) * root + A.eps));
+        }
     }
 }
 __device__ __forceinline__ void random16(uint64_t at, uint32_t (&rm)[4], uint32_t (&rv)[4]) {   // at: head + (position / 2) phi
@@ -140,7 +148,7 @@ template <bool k32> __device__ __forceinline__ typename Raw<k32>::type narrow(co
     else if (type == NTC_BF16) { Run<bf16, 4> f; for (int j = 0; j < 4; j++) f.v[j] = (bf16)p[j]; return __builtin_bit_cast(u32x2, f); }
     else { Run<f16, 4> f; for (int j = 0; j < 4; j++) f.v[j] = (f16)p[j]; return __builtin_bit_cast(u32x2, f); }
 }
-template <int kBits, bool kMaster, bool kG32, bool kP32, bool kAll> __device__ __forceinline__ void whole_blocks(const AdamArgs& A, const ntc_adamw_tensor& T, const void* g_ptr, int gt, float rate,
+template <int kBits, bool kMaster, bool kSmall, bool kG32, bool kP32, bool kAll> __device__ __forceinline__ void whole_blocks(const AdamArgs& A, const ntc_adamw_tensor& T, const void* g_ptr, int gt, float rate,
                                                                                                                  float root, long long i0, int count) {
     using GR = typename Raw<kG32>::type;
     using PR = typename Raw<kP32>::type;
@@ -186,7 +194,7 @@ template <int kBits, bool kMaster, bool kG32, bool kP32, bool kAll> __device__ _
         else widen<kP32>(pf, p[u], T.param_type);
         if constexpr (kBits == 8) decode_block(m[u], v[u], (me >> (8 * u)) & 255, (ve >> (8 * u)) & 255, mf, vf);
         else { mf[0] = m[u].x; mf[1] = m[u].y; mf[2] = m[u].z; mf[3] = m[u].w; vf[0] = v[u].x; vf[1] = v[u].y; vf[2] = v[u].z; vf[3] = v[u].w; }
-        update(A, rate, root, gf, pf, mf, vf);
+        update<kSmall>(A, rate, root, gf, pf, mf, vf);
         if constexpr (kBits == 8) {
             uint32_t rm[4], rv[4];
             random16(noise + (uint64_t)(128 * u) * ntc_hip::kPhi64, rm, rv);
@@ -218,7 +226,7 @@ template <int kBits, bool kMaster, bool kG32, bool kP32, bool kAll> __device__ _
 // state and no copy, 2.7 GB: 543 us, 5.0 TB/s). A block takes 4096 values of one tensor, a wave 1024 of them, 256 (a block of an 8-bit state) at a
 // time: blocks never span tensors, whose pointers are one lookup each, and small tensors (240 of 1 to 400000 values, 24 us; six of a small decoder, 4)
 // cost a launch between them, not one each.
-template <int kBits, bool kMaster> __global__ void __launch_bounds__(kAdamTPB) k_adamw(AdamArgs A, AdamGrads G) {
+template <int kBits, bool kMaster, bool kSmall> __global__ void __launch_bounds__(kAdamTPB) k_adamw(AdamArgs A, AdamGrads G) {
     const long long chunk = A.chunk0 + blockIdx.x;
     const int ti = A.chunk_tensor[chunk], gi = ti - A.tensor0;
     const void* g_ptr = G.g[gi];
@@ -231,8 +239,8 @@ template <int kBits, bool kMaster> __global__ void __launch_bounds__(kAdamTPB) k
     const long long blocks = (T.numel - wave_base) >> 8;     // whole ones from here on
     const bool g32 = gt == NTC_F32, p32 = T.param_type == NTC_F32;
     const auto whole = [&](auto all, int count) {
-        if (g32) p32 ? whole_blocks<kBits, kMaster, true, true, all.value>(A, T, g_ptr, gt, rate, root, base, count) : whole_blocks<kBits, kMaster, true, false, all.value>(A, T, g_ptr, gt, rate, root, base, count);
-        else p32 ? whole_blocks<kBits, kMaster, false, true, all.value>(A, T, g_ptr, gt, rate, root, base, count) : whole_blocks<kBits, kMaster, false, false, all.value>(A, T, g_ptr, gt, rate, root, base, count);
+        if (g32) p32 ? whole_blocks<kBits, kMaster, kSmall, true, true, all.value>(A, T, g_ptr, gt, rate, root, base, count) : whole_blocks<kBits, kMaster, kSmall, true, false, all.value>(A, T, g_ptr, gt, rate, root, base, count);
+        else p32 ? whole_blocks<kBits, kMaster, kSmall, false, true, all.value>(A, T, g_ptr, gt, rate, root, base, count) : whole_blocks<kBits, kMaster, kSmall, false, false, all.value>(A, T, g_ptr, gt, rate, root, base, count);
     };
     if (blocks >= kWaveBlocks) { whole(std::true_type(), kWaveBlocks); return; }
     if (blocks > 0) whole(std::false_type(), (int)blocks);
@@ -249,7 +257,7 @@ template <int kBits, bool kMaster> __global__ void __launch_bounds__(kAdamTPB) k
             const auto r = *(const Run<float, 4>*)((const float*)A.m + at), q = *(const Run<float, 4>*)((const float*)A.v + at);
             for (int j = 0; j < 4; j++) { m[j] = r.v[j]; v[j] = q.v[j]; }
         }
-        update(A, rate, root, g, p, m, v);
+        update<kSmall>(A, rate, root, g, p, m, v);
         if (kBits == 8) {
             uint32_t rm[4], rv[4];
             random16(A.head + (uint64_t)(at >> 1) * ntc_hip::kPhi64, rm, rv);
@@ -330,7 +338,7 @@ extern "C" int ntc_op_adamw(const ntc_adamw_desc* d, void* stream, char* why, si
         AdamGrads G;
         int32_t steps[kRates];
         int rates = 0;
-        bool any = false;
+        bool any = false, small = false;
         for (t1 = t0; t1 < d->n && t1 - t0 < kBatch; t1++) {
             int r = 0;
             if (d->grads[t1]) {                           // (nearly always all tensors are at the same step)
@@ -340,6 +348,8 @@ extern "C" int ntc_op_adamw(const ntc_adamw_desc* d, void* stream, char* why, si
                     steps[r] = d->steps[t1];
                     G.rate[r] = (float)(d->lr / (1.0 - pow(d->beta1, steps[r])));
                     G.root[r] = (float)(1.0 / sqrt(1.0 - pow(d->beta2, steps[r])));
+                    // a lost root of up to 2^-63 and its correction, against half a unit of eps
+                    small = small || !(A.eps >= 0x1p-39f * G.root[r]);
                     rates++;
                 }
                 any = true;
@@ -352,8 +362,12 @@ extern "C" int ntc_op_adamw(const ntc_adamw_desc* d, void* stream, char* why, si
         A.chunk0 = d->first_chunk[t0];
         A.tensor0 = (int)t0;
         const auto go = [&](auto kernel) { kernel<<<(unsigned)blocks, kAdamTPB, 0, (hipStream_t)stream>>>(A, G); };
-        if (d->state_bits == 8) d->master ? go(k_adamw<8, true>) : go(k_adamw<8, false>);
-        else d->master ? go(k_adamw<32, true>) : go(k_adamw<32, false>);
+        const auto with = [&](auto is_small) {
+            constexpr bool s = is_small.value;
+            if (d->state_bits == 8) d->master ? go(k_adamw<8, true, s>) : go(k_adamw<8, false, s>);
+            else d->master ? go(k_adamw<32, true, s>) : go(k_adamw<32, false, s>);
+        };
+        small ? with(std::true_type()) : with(std::false_type());
         if (const int r = launched(why, cap)) return r;
     }
     return 0;

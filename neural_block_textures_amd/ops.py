@@ -125,7 +125,7 @@ class AdamW:
     state_bits 8 holds the averages m and v in one byte each with a power of two for each 256 values (2.03 bytes a weight
     for both against 8), stochastically rounded from `seed`, the step and the position, so that runs repeat bit for bit: rounded to nearest,
     averages that move by 0.1% a step would stand still between values 6 to 12% apart. A gradient that is not
-    finite turns its block of 256 to NaN.
+    finite turns its block of 256 to NaN. With eps 0 a weight whose gradients have all been 0 becomes NaN, as the formula's 0 / 0 is.
 
     The state is flat: tensor i's starts at offsets[i], a multiple of 256. A tensor whose gradient is None is left alone, its
     step count with it.
