@@ -382,6 +382,8 @@ Tensor linear_fp8(const Tensor& x, const Tensor& codes, const Tensor& exps, int6
 struct AdamwPlan {
     std::vector<Tensor> params;
     std::vector<const void*> pointers;
+    std::vector<int64_t> numels;
+    std::vector<int32_t> kinds;
     Tensor tables;                                          // on the device: the tensors, then each chunk's
     const ntc_adamw_tensor* table = nullptr;
     const int32_t* chunk_tensor = nullptr;
@@ -405,6 +407,8 @@ struct AdamwPlan {
             rows.push_back({ (void*)at, n, size, type_of(t), (int32_t)first_chunk.back() });
             of_chunk.insert(of_chunk.end(), (size_t)chunks, (int32_t)pointers.size());
             pointers.push_back((const void*)at);
+            numels.push_back(n);
+            kinds.push_back(type_of(t));
             offsets.push_back(size);
             size += blocks_of(n, NTC_STATE_BLOCK) * NTC_STATE_BLOCK;
             first_chunk.push_back(first_chunk.back() + chunks);
@@ -433,7 +437,9 @@ struct AdamwPlan {
         std::vector<int32_t> types(n, 0), next(steps);
         const auto device = params[0].device();
         for (size_t i = 0; i < n; i++) {
-            TORCH_CHECK_VALUE(params[i].const_data_ptr() == pointers[i], "a parameter has moved to other memory since the optimizer was made");
+            const Tensor& p = params[i];
+            TORCH_CHECK_VALUE(p.const_data_ptr() == pointers[i], "a parameter has moved to other memory since the optimizer was made");
+            TORCH_CHECK_VALUE(p.numel() == numels[i] && type_of(p) == kinds[i] && p.is_contiguous(), "a parameter has another size, type or layout than when the optimizer was made");
             const Tensor& t = given ? ((*given)[i] ? *(*given)[i] : undefined) : params[i].grad();
             if (!t.defined()) continue;
             types[i] = type_of(t);
