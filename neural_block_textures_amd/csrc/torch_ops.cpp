@@ -378,6 +378,19 @@ Tensor linear_fp8(const Tensor& x, const Tensor& codes, const Tensor& exps, int6
 }
 
 // ---------------------------------------------------------------- AdamW
+void state_tensor(const char* name, const Tensor& t, at::ScalarType type, int64_t n, const c10::Device& device) {
+    TORCH_CHECK_VALUE(t.defined() && t.device() == device && t.scalar_type() == type && t.numel() == n && t.is_contiguous(), name, " must be ", n, " contiguous values of ", type, " on ", device);
+}
+// Of n values in 32 bits, or in 8 with their exponents (undefined otherwise).
+void state_tensors(const Tensor& m, const Tensor& v, const Tensor& me, const Tensor& ve, int64_t bits, int64_t n, const c10::Device& device) {
+    const auto type = bits == 8 ? at::kByte : at::kFloat;
+    state_tensor("exp_avg", m, type, n, device);
+    state_tensor("exp_avg_sq", v, type, n, device);
+    if (bits != 8) return;
+    state_tensor("exp_avg_exp", me, at::kByte, n / NTC_STATE_BLOCK, device);
+    state_tensor("exp_avg_sq_exp", ve, at::kByte, n / NTC_STATE_BLOCK, device);
+}
+
 // The tensors of an optimizer, and what their step needs beside its state.
 struct AdamwPlan {
     std::vector<Tensor> params;
@@ -436,6 +449,8 @@ struct AdamwPlan {
         std::vector<const void*> g(n, nullptr);
         std::vector<int32_t> types(n, 0), next(steps);
         const auto device = params[0].device();
+        state_tensors(m, v, me ? *me : undefined, ve ? *ve : undefined, bits, size, device);
+        if (master) state_tensor("master", *master, at::kFloat, size, device);
         for (size_t i = 0; i < n; i++) {
             const Tensor& p = params[i];
             TORCH_CHECK_VALUE(p.const_data_ptr() == pointers[i], "a parameter has moved to other memory since the optimizer was made");
@@ -480,6 +495,9 @@ struct AdamwPlan {
 };
 
 std::pair<Tensor, Tensor> adamw_moments(const Tensor& m, const Tensor& v, const Tensor& me, const Tensor& ve) {
+    on_gpu("exp_avg", m);
+    TORCH_CHECK_VALUE(m.numel() % NTC_STATE_BLOCK == 0, "a state is a multiple of 256 values");
+    state_tensors(m, v, me, ve, 8, m.numel(), m.device());
     const Tensor a = at::empty(m.sizes(), m.options().dtype(at::kFloat)), b = at::empty(m.sizes(), m.options().dtype(at::kFloat));
     call(m.device(), [&](void* s, char* why, size_t cap) {
         return ntc_op_adamw_moments(m.const_data_ptr(), v.const_data_ptr(), (const uint8_t*)me.const_data_ptr(), (const uint8_t*)ve.const_data_ptr(), m.numel(), a.mutable_data_ptr<float>(),
@@ -488,6 +506,10 @@ std::pair<Tensor, Tensor> adamw_moments(const Tensor& m, const Tensor& v, const 
     return { a, b };
 }
 void adamw_encode(const Tensor& m, const Tensor& v, const Tensor& cm, const Tensor& cv, const Tensor& me, const Tensor& ve) {
+    on_gpu("m", m);
+    state_tensor("m", m, at::kFloat, m.numel(), m.device());
+    state_tensor("v", v, at::kFloat, m.numel(), m.device());
+    state_tensors(cm, cv, me, ve, 8, m.numel(), m.device());
     call(m.device(), [&](void* s, char* why, size_t cap) {
         return ntc_op_adamw_encode(m.const_data_ptr<float>(), v.const_data_ptr<float>(), m.numel(), cm.data_ptr(), cv.data_ptr(), (uint8_t*)me.data_ptr(), (uint8_t*)ve.data_ptr(), s, why, cap);
     });

@@ -27,3 +27,24 @@ def test_a_parameter_that_has_changed_in_place(change):
     q.data = whole                                            # as it was
     opt.step([torch.ones(7, device="cuda"), torch.ones(40, 50, device="cuda")])
     assert opt.calls == 1 and (whole != 0).all()
+
+
+@pytest.mark.parametrize("bits,name", [(32, "exp_avg"), (32, "exp_avg_sq"), (8, "exp_avg"), (8, "exp_avg_sq"), (8, "exp_avg_exp"), (8, "exp_avg_sq_exp"), (32, "master"), (8, "master")])
+def test_a_state_that_is_not_the_optimizers(bits, name):
+    p = torch.ones(1000, device="cuda")
+    opt = ops.AdamW([p], state_bits=bits, master=True)
+    kept = getattr(opt, name)
+    wrong = [kept[:len(kept) // 2], kept.to(torch.int32), kept.cpu(), torch.cat([kept, kept])[::2]]
+    for t in wrong:
+        setattr(opt, name, t)
+        with pytest.raises(ValueError, match=f"{name} must be"):
+            opt.step([torch.ones_like(p)])
+        if bits == 8 and name != "master":
+            with pytest.raises(ValueError, match="must be"):
+                opt.moments()
+            with pytest.raises(ValueError, match="must be"):
+                opt.set_moments(torch.zeros(1024, device="cuda"), torch.zeros(1024, device="cuda"))
+    assert opt.calls == 0 and (p == 1).all()
+    setattr(opt, name, kept)
+    opt.step([torch.ones_like(p)])
+    assert (p != 1).all()
