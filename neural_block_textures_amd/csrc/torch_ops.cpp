@@ -487,7 +487,8 @@ struct AdamwPlan {
         d.calls = (uint32_t)(calls + 1);
         d.state_bits = (int32_t)bits;
         call(device, [&](void* s, char* why, size_t cap) { return ntc_op_adamw(&d, s, why, cap); });
-        for (Tensor& t : params) if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();     // (changed in place, behind autograd's back)
+        for (size_t i = 0; i < n; i++)                       // (changed in place, behind autograd's back; those left alone have not changed)
+            if (g[i] && !params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();
         steps = next;
         calls++;
     }
