@@ -72,6 +72,7 @@ struct Rows { int64_t rows, inner, outer_stride, inner_stride; };
 Rows rows_of(const Tensor& t, int64_t lead, const char* name) {
     if (lead == 0) return { 1, 1, 0, 0 };
     if (lead == 1) return { t.size(0), std::max<int64_t>(1, t.size(0)), 0, t.stride(0) };
+    for (int64_t a = 0; a < lead; a++) if (t.size(a) == 0) return { 0, 1, 0, 0 };
     // axes but the last one joined into one stride
     int64_t outer = 1, stride = 0;
     for (int64_t a = lead - 2; a >= 0; a--) {
