@@ -311,9 +311,10 @@ extern "C" int ntc_op_adamw(const ntc_adamw_desc* d, void* stream, char* why, si
     if (!(d->beta1 >= 0.0 && d->beta1 < 1.0) || !(d->beta2 >= 0.0 && d->beta2 < 1.0)) return refuse(why, cap, "betas are in [0, 1)");
     if (!(d->lr >= 0.0) || !(d->eps >= 0.0) || !(d->weight_decay >= 0.0)) return refuse(why, cap, "lr, eps and weight_decay are not negative");
     if (d->n == 0) return 0;
-    if (!d->tensors || !d->chunk_tensor || !d->first_chunk || !d->grads || !d->grad_types || !d->steps || !d->exp_avg || !d->exp_avg_sq)
-        return refuse(why, cap, "a null pointer");
-    if (d->state_bits == 8 && (!d->exp_avg_exp || !d->exp_avg_sq_exp)) return refuse(why, cap, "8-bit states have exponents");
+    if (!d->first_chunk || !d->grads || !d->grad_types || !d->steps) return refuse(why, cap, "a null pointer");
+    const bool values = d->first_chunk[d->n] > d->first_chunk[0];          // (tensors of no values have no state either)
+    if (values && (!d->tensors || !d->chunk_tensor || !d->exp_avg || !d->exp_avg_sq)) return refuse(why, cap, "a null pointer");
+    if (values && d->state_bits == 8 && (!d->exp_avg_exp || !d->exp_avg_sq_exp)) return refuse(why, cap, "8-bit states have exponents");
     for (int64_t i = 0; i < d->n; i++) {
         if (d->grads[i] && d->steps[i] < 1) return refuse(why, cap, "steps count from 1");
         if (d->grad_types[i] < 0 || d->grad_types[i] > 2) return refuse(why, cap, "gradients are 32-bit floats, bfloat16 or float16");

@@ -29,3 +29,11 @@ def test_fp8_linear(shape, K, N, dtype):
     assert dx.shape == x.shape and dw.shape == w.shape and not dx.any() and not dw.any()
     z = ops.fp8_linear(x.detach(), ops.fp8_quantize(w.detach(), 128))
     assert z.shape == y.shape and not z.any()
+
+
+def test_optimizer_of_nothing():
+    for bits in (8, 32):
+        p = torch.zeros((0, 4), device="cuda")
+        opt = ops.AdamW([p], state_bits=bits, master=True)
+        opt.step([torch.zeros((0, 4), device="cuda")])
+        assert opt.calls == 1 and opt.moments()[0].numel() == 0

@@ -16,3 +16,12 @@ def test_temperatures_out_of_range(T):
 @pytest.mark.parametrize("T", [2.0 ** -127, 1.0, 2.0 ** 120])
 def test_temperatures_in_range(T):
     assert refused(O.library().ntc_op_token_logprobs, C.byref(logprobs(temperature=T, rows=0))) == (0, "")
+
+
+def test_a_step_of_tensors_without_values():
+    d = O.AdamwDesc()
+    held = {"first_chunk": (C.c_int64 * 3)(0, 0, 0), "grads": (C.c_void_p * 2)(1 << 20, None), "grad_types": (C.c_int32 * 2)(0, 0), "steps": (C.c_int32 * 2)(1, 1)}
+    for k, v in held.items():
+        setattr(d, k, C.addressof(v))
+    d.n, d.state_bits, d.beta1, d.beta2 = 2, 8, 0.9, 0.9
+    assert refused(O.library().ntc_op_adamw, C.byref(d)) == (0, "")
