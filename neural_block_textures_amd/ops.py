@@ -198,19 +198,27 @@ class AdamW:
                 "exp_avg_sq_exp": self.exp_avg_sq_exp, "master": self.master}
 
     def load_state_dict(self, state: dict) -> None:
-        """Copies a state_dict()'s contents. `step` may be one number for all tensors, `calls` is the largest step where it is absent,
-        and the 32-bit copy is taken from the tensors where `master` is absent."""
-        steps = np.broadcast_to(np.asarray(state["step"], np.int32), (len(self.params),)).tolist()
+        """Copies a state_dict()'s contents; one that does not fit changes nothing. `step` may be one number for all tensors, `calls` is the
+        largest step where it is absent, and the 32-bit copy is taken from the tensors where `master` is absent."""
+        steps = np.asarray(state["step"])
+        if steps.shape not in ((), (1,), (len(self.params),)) or not ((steps >= 0) & (steps < 2 ** 31 - 1) & (steps == np.floor(steps))).all():
+            raise ValueError(f"step must be one count from 0 on, or {len(self.params)}")
+        steps = np.broadcast_to(steps, (len(self.params),)).astype(np.int32).tolist()
+        calls = int(state.get("calls", max(steps)))
+        if calls < 0:
+            raise ValueError(f"calls must be a count from 0 on, not {calls}")
         names = ["exp_avg", "exp_avg_sq"] + (["exp_avg_exp", "exp_avg_sq_exp"] if self.state_bits == 8 else [])
-        for name in names + (["master"] if self.master is not None and state.get("master") is not None else []):
+        names += ["master"] if self.master is not None and state.get("master") is not None else []
+        for name in names:
             mine, other = getattr(self, name), state.get(name)
             if other is None or other.shape != mine.shape or other.dtype != mine.dtype:
                 raise ValueError(f"{name} must be {mine.dtype} of {mine.numel()} values")
-            mine.copy_(other)
+        for name in names:
+            getattr(self, name).copy_(state[name])
         if self.master is not None and state.get("master") is None:
             self.sync_master()
         self._plan.steps = steps
-        self._plan.calls = int(state.get("calls", max(steps)))
+        self._plan.calls = calls
 
 
 # ---------------------------------------------------------------- 8-bit floating point in blocks
