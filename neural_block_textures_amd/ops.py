@@ -140,6 +140,8 @@ class AdamW:
             raise ValueError(f"states are held in 8 or 32 bits, not {state_bits}")
         if lr < 0 or eps < 0 or weight_decay < 0 or not all(0 <= b < 1 for b in betas):
             raise ValueError("lr, eps and weight_decay must not be negative, betas in [0, 1)")
+        if not 0 <= seed < 2 ** 64:
+            raise ValueError(f"seed must be from 0 to 2^64 - 1, not {seed}")
         self._plan = _binding().AdamwPlan(self.params)
         self.lr, self.betas, self.eps, self.weight_decay = lr, tuple(betas), eps, weight_decay
         self.state_bits, self.seed = state_bits, seed
@@ -195,11 +197,12 @@ class AdamW:
 
     def state_dict(self) -> dict:
         return {"step": list(self._plan.steps), "calls": self.calls, "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq, "exp_avg_exp": self.exp_avg_exp,
-                "exp_avg_sq_exp": self.exp_avg_sq_exp, "master": self.master}
+                "exp_avg_sq_exp": self.exp_avg_sq_exp, "master": self.master, "seed": self.seed}
 
     def load_state_dict(self, state: dict) -> None:
         """Copies a state_dict()'s contents; one that does not fit changes nothing. `step` may be one number for all tensors, `calls` is the
-        largest step where it is absent, and the 32-bit copy is taken from the tensors where `master` is absent."""
+        largest step where it is absent, the 32-bit copy is taken from the tensors where `master` is absent, and the optimizer's own seed
+        stays where `seed` is absent (a run goes on bit for bit on its first one's)."""
         steps = np.asarray(state["step"])
         if steps.shape not in ((), (1,), (len(self.params),)) or not ((steps >= 0) & (steps < 2 ** 31 - 1) & (steps == np.floor(steps))).all():
             raise ValueError(f"step must be one count from 0 on, or {len(self.params)}")
@@ -207,6 +210,9 @@ class AdamW:
         calls = int(state.get("calls", max(steps)))
         if calls < 0:
             raise ValueError(f"calls must be a count from 0 on, not {calls}")
+        seed = int(state.get("seed", self.seed))
+        if not 0 <= seed < 2 ** 64:
+            raise ValueError(f"seed must be from 0 to 2^64 - 1, not {seed}")
         names = ["exp_avg", "exp_avg_sq"] + (["exp_avg_exp", "exp_avg_sq_exp"] if self.state_bits == 8 else [])
         names += ["master"] if self.master is not None and state.get("master") is not None else []
         for name in names:
@@ -219,6 +225,7 @@ class AdamW:
             self.sync_master()
         self._plan.steps = steps
         self._plan.calls = calls
+        self.seed = seed
 
 
 # ---------------------------------------------------------------- 8-bit floating point in blocks
