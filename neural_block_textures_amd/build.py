@@ -4,10 +4,12 @@
 
 Every translation unit is compiled for gfx950 with FMA contraction off (the kernels write each
 fused multiply-add explicitly) and without packed-FP32 instructions; objects are rebuilt in
-parallel and linked into neural_block_textures_amd/libntc_hip.so.
+parallel and linked into neural_block_textures_amd/libntc_hip.so. The operators' torch binding (_ops.so) is built where
+torch is installed; the library needs no torch.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -81,7 +83,10 @@ def build(verbose: bool = False, jobs: int = 4) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"linking libntc_hip.so failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
-    build_torch(verbose)
+    if importlib.util.find_spec("torch") is None:
+        print("torch is not installed: its binding of the operators (_ops.so) is left out", file=sys.stderr)
+    else:
+        build_torch(verbose)
     return LIB
 
 
