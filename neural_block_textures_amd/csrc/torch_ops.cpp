@@ -288,17 +288,27 @@ Tensor matmul(const Tensor& ac, const Tensor& ae, int64_t M, int64_t ka, int64_t
     return c;
 }
 
+// Rows that one product may sum over (a multiple of its blocks): the weights' gradient of more is the sum of several, in 32 bits.
+constexpr int64_t kMostSum = 1 << 23;
+
 struct LinearNode : torch::autograd::Function<LinearNode> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w) {
         const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
         const bool need_x = x.requires_grad(), need_w = w.requires_grad();
         Held xq(M, K, 1), wq(N, K, 128), xt(K, M, 1), wt(K, N, 128);
         hold(xq, true, wq, true, x);
-        const Tensor kept = hold(xt, need_w, wt, need_x, x);
+        const bool parts = need_w && M > kMostSum;
+        const Tensor kept = hold(xt, need_w && !parts, wt, need_x, x);
         run_quantize_pair(x, xq, xt, w, wq, wt);
+        torch::autograd::variable_list saved = { kept };
+        for (int64_t m = 0; parts && m < M; m += kMostSum) {
+            const Held t(K, std::min(kMostSum, M - m), 1, x);
+            run_quantize(x.narrow(0, m, t.K), {}, t);
+            saved.push_back(t.buffer);
+        }
         const Tensor y = matrix(M, N, x.scalar_type(), x);
         run_matmul(operand(xq), operand(wq), K, y);
-        ctx->save_for_backward({ kept });
+        ctx->save_for_backward(saved);
         ctx->saved_data["call"] = std::vector<int64_t>{ M, N, K, need_x, need_w, (int64_t)x.scalar_type(), (int64_t)w.scalar_type() };
         ctx->set_materialize_grads(false);
         return y;
@@ -311,17 +321,29 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         const bool need_x = of[3], need_w = of[4];
         const Tensor dy = rows_contiguous(g[0]);
         Held dq(M, N, 1), dt(N, M, 1), xt(K, M, 1), wt(K, N, 128);
-        hold(dq, need_x, dt, need_w, dy);
-        if (need_w) xt.buffer = saved[0];
+        const bool parts = need_w && M > kMostSum;
+        hold(dq, need_x, dt, need_w && !parts, dy);
+        if (need_w && !parts) xt.buffer = saved[0];
         if (need_x) wt.buffer = saved[0];
-        wt.at = need_w ? xt.size() : 0;
-        run_quantize(dy, dq, dt);
+        wt.at = xt.buffer.defined() ? xt.size() : 0;
+        if (need_x || !parts) run_quantize(dy, dq, dt);
         Tensor dx, dw;
         if (need_x) {
             dx = matrix(M, K, (at::ScalarType)of[5], dy);
             run_matmul(operand(dq), operand(wt), N, dx);
         }
-        if (need_w) {
+        if (parts) {
+            for (int64_t m = 0; m < M; m += kMostSum) {
+                Held part(K, std::min(kMostSum, M - m), 1);
+                part.buffer = saved[1 + m / kMostSum];
+                const Held t(N, part.K, 1, dy);
+                run_quantize(dy.narrow(0, m, part.K), {}, t);
+                const Tensor sum = matrix(N, K, at::kFloat, dy);
+                run_matmul(operand(t), operand(part), part.K, sum);
+                if (m) dw += sum; else dw = sum;
+            }
+            dw = dw.to((at::ScalarType)of[6]);
+        } else if (need_w) {
             dw = matrix(N, K, (at::ScalarType)of[6], dy);
             run_matmul(operand(dt), operand(xt), M, dw);
         }

@@ -271,7 +271,7 @@ def fp8_quantize_both(x: torch.Tensor, block_rows: int = 1):
 
 def fp8_matmul(a: Fp8Tensor, b: Fp8Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """a [M, K] times b [N, K] transposed, summed in 32 bits and rounded once to dtype (bfloat16, float16 or float32; the 8-bit matrix
-    instructions are good to 1.5e-5 of a result's magnitude, so float32 holds no more than that)."""
+    instructions are good to 1.5e-5 of a result's magnitude, so float32 holds no more than that). K is at most 2^23."""
     for name, t in (("a", a), ("b", b)):
         if not isinstance(t, Fp8Tensor):
             raise ValueError(f"{name} must be an Fp8Tensor")
