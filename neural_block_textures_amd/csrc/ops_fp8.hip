@@ -292,10 +292,10 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_
 // 16 (4) bytes a lane from base + off to LDS at `to` + 16 (4) lane: `to` is the same in all lanes. Nothing waits for it but a vmcnt
 // of the caller's; the compiler's own waits only become stricter by loads that it does not count.
 __device__ __forceinline__ void to_lds16(uint32_t to, uint32_t off, const uint8_t* base) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(to), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(to), "v"(off), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void to_lds4(uint32_t to, uint32_t off, const uint8_t* base) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(to), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(to), "v"(off), "s"(base) : "memory", "m0");
 }
 
 // until at most n of the wave's loads are on their way
