@@ -756,8 +756,9 @@ template <class C> static void run_few(const ntc_fp8_matmul_desc* d, hipStream_t
 
 template <int T, class C> static void launch_matmul(const MatmulArgs& A, int parts, hipStream_t s) {
     const unsigned tiles = (unsigned)(A.tiles_m * A.tiles_n);
-    if (parts > 1) k_fp8_matmul<T, T, float, true><<<tiles * parts, 256, 0, s>>>(A);
-    else k_fp8_matmul<T, T, C, false><<<tiles, 256, 0, s>>>(A);
+    if constexpr (T == 64)
+        if (parts > 1) { k_fp8_matmul<T, T, float, true><<<tiles * parts, 256, 0, s>>>(A); return; }
+    k_fp8_matmul<T, T, C, false><<<tiles, 256, 0, s>>>(A);
 }
 
 template <class C> static void run_matmul(const ntc_fp8_matmul_desc* d, hipStream_t s) {
@@ -780,7 +781,7 @@ template <class C> static void run_matmul(const ntc_fp8_matmul_desc* d, hipStrea
     A.c = p.parts > 1 ? d->workspace : d->c;
     A.ldc = p.parts > 1 ? d->N : d->ldc;
     if (p.tile == 256) launch_matmul<256, C>(A, 1, s);
-    else if (p.tile == 128) launch_matmul<128, C>(A, p.parts, s);
+    else if (p.tile == 128) launch_matmul<128, C>(A, 1, s);
     else launch_matmul<64, C>(A, p.parts, s);
     if (p.parts > 1) k_fp8_join<C><<<(unsigned)((d->M * d->N + 255) / 256), 256, 0, s>>>((const float*)d->workspace, p.parts, d->M * d->N, d->N, d->ldc, (C*)d->c);
 }
