@@ -480,10 +480,10 @@ __device__ __forceinline__ Best merge(Candidates& list, const float* v, const in
     return lane < list.n ? Best{ list.v[lane], list.i[lane] } : Best{ -NTC_INF, kNoIndex };
 }
 
-// What a lane reads at a time: kRun values in vectors of 16 bytes.
 // A lane's value of another lane (0 where there is none): rows of 16 shifted, or a row's last lane to those after.
 template <int kCtrl, int kRows = 0xf> __device__ __forceinline__ uint32_t before(uint32_t x) { return __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false); }
 
+// What a lane reads at a time: kRun values in vectors of 16 bytes.
 template <class T> struct Long { static constexpr int kVec = 16 / (int)sizeof(T), kVecs = 2, kRun = kVec * kVecs, kChunk = 64 * kRun; };
 
 // Adds all values of a chunk that reach `least`, in ascending order of index, if the list has room for them: each lane's places

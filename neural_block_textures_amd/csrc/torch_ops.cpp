@@ -228,11 +228,6 @@ void run_quantize_pair(const Tensor& x, const Held& xq, const Held& xt, const Te
     const ntc_fp8_quantize_desc a = quantize_desc(x, 1, xq, xt), b = quantize_desc(w, 128, wq, wt);
     call(x.device(), [&](void* s, char* why, size_t cap) { return ntc_op_fp8_quantize_pair(&a, &b, s, why, cap); });
 }
-void run_quantize(const Tensor& x, int64_t block, uint8_t* codes, uint8_t* exps, uint8_t* codes_t, uint8_t* exps_t) {
-    if (!x.numel()) return;
-    const ntc_fp8_quantize_desc d = { x.const_data_ptr(), x.size(0), x.size(1), x.stride(0), type_of(x), (int32_t)block, codes, exps, codes_t, exps_t };
-    call(x.device(), [&](void* s, char* why, size_t cap) { return ntc_op_fp8_quantize(&d, s, why, cap); });
-}
 Tensor rows_contiguous(const Tensor& x) { return (x.size(1) > 1 && x.stride(1) != 1) || x.stride(0) < 0 ? x.contiguous() : x; }
 
 struct Operand { const void* p; const uint8_t* exps; int64_t rows, stride; int type, block; };
