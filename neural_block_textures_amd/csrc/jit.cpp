@@ -59,7 +59,7 @@ bool compiler_of_the_build() {
         std::ifstream f(directory(file) + "/../.info/version");
         int major = 0, minor = 0;
         char dot = 0;
-        if (!(f >> major >> dot >> minor) || major * 100 + minor < HIP_VERSION_MAJOR * 100 + HIP_VERSION_MINOR) return false;
+        if (!(f >> major >> dot >> minor) || major != HIP_VERSION_MAJOR || minor != HIP_VERSION_MINOR) return false;
     }
     return true;
 }
