@@ -674,8 +674,9 @@ template <class C> __global__ void __launch_bounds__(256) k_fp8_join(const float
 // How a product is divided. Tiles of 256 x 256 (one to a CU) where they fill the chip and the sum is long enough for what they cost to begin and end
 // (8192 x 8192 x 512: 51 us against 59 in tiles of 128; 65536 x 256 x 256: 14.6 against 12.7); of 128 x 128 (two) where there are more than 128
 // (1003 x 2077 x 1500: 8.1 against 9.7 in tiles of 64); else of 64 x 64 (1000 x 1000 x 1000: 4.8 against 7.0, 512 x 4096 x 4096: 16.8 against 18.4).
-// Long sums of few such tiles go into parts of at least 16 blocks of columns, which a second launch adds (256 x 256 x 65536: 15.9 against 198;
-// 1024 x 1024 x 8192: 23.0 against 27.9; but 256 x 4096 x 4096: 16.6 against 10.3).
+// Long sums of few such tiles go into parts of at least 16 blocks of columns, which a second launch adds, from 48 blocks on (256 x 256 x 65536: 15.9
+// against 198; 1024 x 1024 x 8192: 23.0 against 27.9; 64 x 4096 x 8192: 12.5 against 27.2, x 6144 12.5 against 11.5; with 32 blocks 64 x 4096 x 4096 9.3
+// against 8.7, 256 x 4096 x 4096 16.5 against 10.3, 64 x 1024 x 4096 8.0 against 8.6).
 struct Plan { int tile, parts, split_blocks; };
 static Plan plan_of(int64_t M, int64_t N, int64_t K) {
     const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
