@@ -34,6 +34,14 @@ __device__ __forceinline__ float read_lane(float x, int l) { return __uint_as_fl
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }   // one instruction, 1 ulp; 2^-inf = 0
 __device__ __forceinline__ float fast_log2(float x) { return __builtin_amdgcn_logf(x); }
 
+// Between a wave's accesses to shared memory of which some lanes read what others wrote: the hardware keeps them in order by itself, the
+// compiler does only across a fence (it takes a wave barrier alone for something that touches no memory). No instruction comes of it.
+__device__ __forceinline__ void wave_shared() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Reductions over aligned groups of 4, 8, 16, 32 and 64 lanes: every lane gets the result, and no shared memory is used (lanes
 // exchanged within a row of 16 on the way into the instruction, rows swapped). f is commutative and associative.
 template <int kCtrl, class V> __device__ __forceinline__ V exchange(V x) {

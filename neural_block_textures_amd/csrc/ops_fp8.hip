@@ -486,12 +486,14 @@ template <int TM, int TN, class C, bool kParts> __global__ void __launch_bounds_
                     for (int k = 0; k < 4; k++) o.v[k] = (C)acc[i][j][4 * q + k];
                     *(Run<C, 4>*)(own + r32 * kRow + 16 * ((4 * j + q) ^ (r32 & (kPieces - 1))) + 8 * half) = o;
                 }
+            wave_shared();
 #pragma unroll
             for (int p = 0; p < 32 * kPieces / 64; p++) {
                 const int r = p * (64 / kPieces) + lane / kPieces, piece = lane % kPieces;
                 const Run<C, 8> x = *(const Run<C, 8>*)(own + r * kRow + 16 * (piece ^ (r & (kPieces - 1))));
                 put(quarter + (32 * i + r) * d.ldc + 8 * piece, x, 32 * i + r, 8 * piece, guard);
             }
+            wave_shared();
         }
     } else {
 #pragma unroll

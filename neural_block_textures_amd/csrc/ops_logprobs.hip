@@ -415,7 +415,7 @@ struct Candidates {
     __device__ __forceinline__ void put_in_order(int top) {
         const int lane = lane_id();
         if (n == ordered) return;
-        __builtin_amdgcn_wave_barrier();                     // (a wave's LDS operations are in order)
+        wave_shared();
         const float w = lane < n ? v[lane] : -NTC_INF;
         const int j = lane < n ? i[lane] : kNoIndex;
         const uint32_t key = lane < n ? order_key(w) : 0;
@@ -428,10 +428,10 @@ struct Candidates {
                 before += other > mine;
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_shared();
         if (lane < n && before < top) { v[before] = w; i[before] = j; }
         n = ordered = n < top ? n : top;
-        __builtin_amdgcn_wave_barrier();
+        wave_shared();
     }
     // lanes of `ask` add (w, j); returns those that found no place
     __device__ __forceinline__ unsigned long long add(unsigned long long ask, float w, int j) {
@@ -864,7 +864,7 @@ template <class T, int kGroup> __global__ void __launch_bounds__(256) k_logprobs
     }
 #pragma unroll
     for (int q = 0; q < kEach / 4; q++) laid[q][threadIdx.x] = float4{ g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3] };
-    __builtin_amdgcn_wave_barrier();                         // (a wave's LDS operations are in order)
+    wave_shared();
     const auto add = [&](int place, float extra) {
         float* to = (float*)&laid[(place % kEach) / 4][own * kGroup + place / kEach] + place % 4;
         *to += extra * inv_t;
@@ -880,7 +880,7 @@ template <class T, int kGroup> __global__ void __launch_bounds__(256) k_logprobs
         joined |= (kGroup == 64 ? found : found & ((1ull << (kGroup % 64)) - 1)) != 0;
     }
     if (in == 0 && !joined) add((int)t, glp);
-    __builtin_amdgcn_wave_barrier();
+    wave_shared();
 #pragma unroll
     for (int q = 0; q < kEach / 4; q++) { const float4 o = laid[q][threadIdx.x]; g[4 * q] = o.x; g[4 * q + 1] = o.y; g[4 * q + 2] = o.z; g[4 * q + 3] = o.w; }
     if (first + own >= d.rows) return;
