@@ -68,6 +68,7 @@ int ntc_op_token_logprobs_backward(const ntc_logprobs_desc* d, void* stream, cha
  *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
  *   p = p (1 - lr weight_decay) - lr / (1 - b1^c) * m / (sqrt(v / (1 - b2^c)) + eps)
  * in 32-bit arithmetic, p rounded once to its type (the 32-bit copy in `master`, where there is one, is what is updated then).
+ * The gradients' addresses, the rates that follow from the step counts, and `calls` are arguments of the launch: a captured graph repeats them.
  *
  * The state is flat: tensor i's values are at state_offset (a multiple of NTC_STATE_BLOCK) in exp_avg, exp_avg_sq and master;
  * the values between a tensor's end and the next multiple are 0. With state_bits 8 each block of 256 values has

@@ -174,7 +174,8 @@ class AdamW:
 
     def step(self, grads=None) -> None:
         """One step from `grads` (one tensor or None for each parameter, of its shape, any of the three types), or from the
-        parameters' .grad. A gradient that is not contiguous is copied first."""
+        parameters' .grad. A gradient that is not contiguous is copied first. In a captured graph a replay is this same step again: the same
+        step count, rates and random bits, and not counted."""
         self._plan.step(grads, self.exp_avg, self.exp_avg_sq, self.exp_avg_exp, self.exp_avg_sq_exp, self.master, self.state_bits, self.lr, *self.betas,
                         self.eps, self.weight_decay, self.seed)
 
@@ -283,7 +284,8 @@ def fp8_linear(x: torch.Tensor, w) -> torch.Tensor:
 
     With w a tensor the layer is differentiable (once) in both: dx = q(dy) q(w) and dw = q(dy)^T q(x) with their
     operands in blocks along each product's own sum. With w an Fp8Tensor (fp8_quantize(w, 128), laid out once) it is for inference;
-    few rows of x are then taken to 8 bits inside the product.
+    few rows of x are then taken to 8 bits inside the product. Sums are the 8-bit matrix instruction's, good to 1.5e-5 of a result's magnitude:
+    a 32-bit y holds no more than that.
     """
     if isinstance(w, Fp8Tensor):
         return _binding().linear_fp8(x, w.codes, w.exps, *w.shape, w.block_rows)
