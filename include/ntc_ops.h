@@ -143,7 +143,7 @@ int ntc_op_fp8_quantize_pair(const ntc_fp8_quantize_desc* a, const ntc_fp8_quant
  * (The 8-bit matrix instruction adds a block's 128 products with about 16 bits below the largest: 1.5e-5 of a result's
  * magnitude, far below a 16-bit result's rounding, and what a 32-bit result is good to.)
  * With a_type not NTC_FP8, A is a matrix of floats (rows at a_stride elements) that is taken to 8 bits on the way, in
- * blocks of 1 x 128: a_exps is not used then. workspace: ntc_op_fp8_matmul_workspace() bytes. */
+ * blocks of 1 x 128: a_exps is not used then. K is at most 2^23. workspace: ntc_op_fp8_matmul_workspace() bytes. */
 enum { NTC_FP8 = 3 };
 typedef struct ntc_fp8_matmul_desc {
     const void* a;

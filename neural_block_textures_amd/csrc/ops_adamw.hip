@@ -223,7 +223,7 @@ template <int kBits, bool kMaster, bool kSmall, bool kG32, bool kP32, bool kAll>
 }
 
 // One pass over everything: memory bounds it (2^28 bf16 values with a 32-bit copy and state, 7.5 GB: 1406 us, 5.3 TB/s, where a copy reaches 5.0; 8-bit
-// state and no copy, 2.7 GB: 543 us, 5.0 TB/s). A block takes 4096 values of one tensor, a wave 1024 of them, 256 (a block of an 8-bit state) at a
+// state and no copy, 2.7 GB: 507 us where many follow each other, 5.3 TB/s, 555 over the first twenty). A block takes 4096 values of one tensor, a wave 1024 of them, 256 (a block of an 8-bit state) at a
 // time: blocks never span tensors, whose pointers are one lookup each, and small tensors (240 of 1 to 400000 values, 24 us; six of a small decoder, 4)
 // cost a launch between them, not one each.
 template <int kBits, bool kMaster, bool kSmall> __global__ void __launch_bounds__(kAdamTPB) k_adamw(AdamArgs A, AdamGrads G) {

@@ -282,7 +282,7 @@ template <class T> __global__ void __launch_bounds__(256) k_fp8_quantize_pair(nt
 // one stage ahead of the products: one barrier a stage, and no product waits for a load of its own stage. In LDS a row is 64 bytes, and the 16-byte
 // piece c of row r lies at c ^ swizzle(r), which spreads any 8 or 16 rows' pieces over all banks.
 //
-// Bound by the matrix instructions and the power they draw (8192 x 8192 x 8192: 421 us, 2.61 PFLOP/s; 483 us where twenty follow each other; the instructions alone, from registers, 3.8 PFLOP/s on random
+// Bound by the matrix instructions and the power they draw (8192 x 8192 x 8192: 416 us alone, 2.64 PFLOP/s, 500 to 515 for the first five in a row, 402 where hundreds follow; the instructions alone, from registers, 3.8 PFLOP/s on random
 // data and 4.9 on zeros; the library's product with one scale for a matrix 3.05). 256 x 256 tiles read each operand byte from LDS half as often as 128 x
 // 128 ones, and the four waves' SIMDs hold nothing else.
 constexpr int kStages = 4;

@@ -136,7 +136,7 @@ struct ThreePlaced {                                          // (0: none)
 // one, from the lanes' three best, through LDS to whole runs of the results. A 16-bit value's key is ordered two at a time and leaves half a
 // word to its index (from the top down, in a row of at most 1024): one word orders values and indices both. A 32-bit value's index is found in
 // a second reduction. What is written of rows is left to one lane a row (and one an alternative), since a wave's instructions cost as much for 4 rows
-// as for 64. Bound by vector instructions (358 a wave with 4 alternatives): 262144 rows of 256 bf16 values 42 us with 4 alternatives, 3.6 TB/s; 400000
+// as for 64. Bound by vector instructions (359 a wave with 4 alternatives): 262144 rows of 256 bf16 values 42 us with 4 alternatives, 3.6 TB/s; 400000
 // x 64 14.3 us without, at the rate of their bytes.
 constexpr int kShort = 1024;                                 // the longest such row
 // Sixteen values in descending order: exchanges of pairs, halves merged odd with even.
@@ -690,8 +690,9 @@ template <class T> __device__ __forceinline__ void finish(const ntc_logprobs_des
     }
 }
 
-// Memory bounds it where rows are many and alternatives few (bf16 4096 x 131072 with 16: 214 us, 5.0 TB/s; 8190 x 50001 without: 162 us, 5.1 TB/s), the
-// two launches and the dependent steps of one wave's search where rows are few (1 x 131072: 4.9 us, with 8 alternatives 10.9).
+// Memory bounds it where rows are many and alternatives few (bf16 4096 x 131072 with 16: 215 us, 5.0 TB/s; 8190 x 50001 without: 162 us, 5.1 TB/s), the
+// two launches and the dependent steps of one wave's search where rows are few (1 x 131072: 4.9 us; with 8 alternatives 10.9, the 6 more being a bound
+// from 19 ballots, one wave's ranking of candidates lane by lane, and two merges in series).
 // kWaves waves (of a block of 4) read a row; with kParts a block reads the part blockIdx.y of a row and leaves its sums and list in the workspace.
 template <class T, int kWaves, bool kParts> __global__ void __launch_bounds__(256) k_logprobs_long(ntc_logprobs_desc d, float lim, int part_chunks) {
     __shared__ Soft soft[4];

@@ -285,7 +285,7 @@ def fp8_linear(x: torch.Tensor, w) -> torch.Tensor:
     With w a tensor the layer is differentiable (once) in both: dx = q(dy) q(w) and dw = q(dy)^T q(x) with their
     operands in blocks along each product's own sum. With w an Fp8Tensor (fp8_quantize(w, 128), laid out once) it is for inference;
     few rows of x are then taken to 8 bits inside the product. Sums are the 8-bit matrix instruction's, good to 1.5e-5 of a result's magnitude:
-    a 32-bit y holds no more than that.
+    a 32-bit y holds no more than that. K is at most 2^23 (and N, for a gradient in x); rows may be any number.
     """
     if isinstance(w, Fp8Tensor):
         return _binding().linear_fp8(x, w.codes, w.exps, *w.shape, w.block_rows)
