@@ -138,8 +138,8 @@ class AdamW:
             raise ValueError("no parameters")
         if state_bits not in (8, 32):
             raise ValueError(f"states are held in 8 or 32 bits, not {state_bits}")
-        if lr < 0 or eps < 0 or weight_decay < 0 or not all(0 <= b < 1 for b in betas):
-            raise ValueError("lr, eps and weight_decay must not be negative, betas in [0, 1)")
+        if not (lr >= 0 and eps >= 0 and weight_decay >= 0) or len(betas) != 2 or not all(0 <= b < 1 for b in betas):
+            raise ValueError("lr, eps and weight_decay must not be negative, the two betas in [0, 1)")
         if not 0 <= seed < 2 ** 64:
             raise ValueError(f"seed must be from 0 to 2^64 - 1, not {seed}")
         self._plan = _binding().AdamwPlan(self.params)

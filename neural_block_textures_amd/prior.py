@@ -99,6 +99,8 @@ class Prior:
 
 def fit(sym: torch.Tensor, alphabet: int, steps: int = 300, hidden: int = 256, batch: int = 16384, lr: float = 2e-3, state_bits: int = 8, seed: int = 1):
     """(Prior, Contexts) trained on symbols [H, W, C] that are on the GPU."""
+    if steps < 0 or hidden < 1 or batch < 1 or not sym.numel():
+        raise ValueError(f"steps from 0 on, hidden units and a batch from 1 on, and symbols are needed, not {steps}, {hidden}, {batch} and {list(sym.shape)}")
     ctx = Contexts(sym, alphabet)
     prior = Prior(ctx.width, hidden, alphabet, seed, sym.device)
     opt = ops.AdamW(prior.parameters(), lr=lr, weight_decay=0.01, state_bits=state_bits, master=True, seed=seed)
