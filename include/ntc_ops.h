@@ -1,6 +1,7 @@
 /* C ABI of the operators a learned prior over a texture's symbols is made of, exported by libntc_hip.so:
- * token log probabilities with their gradient, an AdamW step over many tensors, and matrix products in
- * 8-bit floating point with a power-of-two scale for each block of 128.
+ * token log probabilities with their gradient, an AdamW step over many tensors, matrix products in
+ * 8-bit floating point with a power-of-two scale for each block of 128, and what a sequence model's blocks have beside them: layer norm,
+ * rotary positions of several axes, and causal attention, with their gradients.
  *
  * Every pointer is a device pointer unless its comment says host; every launch goes to `stream` (a hipStream_t;
  * null is the default stream) of the current device, and no call waits, allocates or copies. A call returns 0, or
@@ -162,6 +163,94 @@ size_t ntc_op_fp8_matmul_workspace(int64_t M, int64_t N, int64_t K, int32_t a_ty
 int ntc_op_fp8_matmul(const ntc_fp8_matmul_desc* d, void* stream, char* why, size_t why_cap);
 /* The rows of A up to which it may be given as floats. */
 int64_t ntc_op_fp8_matmul_float_rows(void);
+
+/* ---------------------------------------------------------------- layer norm
+ * Rows of C values, contiguous, at x_stride (dy_stride) elements; results are contiguous. With mean and variance (over C) of a row in 32 bits,
+ *   h = (x - mean) / sqrt(variance + eps),  y = h weight + bias   (null: 1 and 0),
+ * rounded once to x's type. weight and bias are of x's type or float32, both alike. stats (2 floats a row: mean and 1 / sqrt) is what the backward pass needs; null
+ * where there is none. Backward, with t = dy weight:
+ *   dx = (t - mean t - h mean(t h)) / sqrt(variance + eps),  dweight = sum over rows of dy h,  dbias = sum over rows of dy
+ * (each may be null); the sums are 32-bit, in an order that depends on the sizes alone. A row with a value that is not finite is NaN.
+ * workspace: ntc_op_layer_norm_workspace() bytes of any contents, for dweight and dbias. */
+typedef struct ntc_layer_norm_desc {
+    const void* x;
+    const void* weight;
+    const void* bias;
+    void* y;
+    float* stats;          /* [rows][2], at a multiple of 8 bytes */
+    int64_t rows, C;
+    int64_t x_stride, dy_stride;
+    int32_t dtype, weight_type;
+    float eps;
+    /* backward only */
+    const void* dy;
+    void* dx;              /* [rows][C] */
+    void* dweight;         /* [C], of weight_type */
+    void* dbias;
+    void* workspace;
+} ntc_layer_norm_desc;
+int ntc_op_layer_norm(const ntc_layer_norm_desc* d, void* stream, char* why, size_t why_cap);
+size_t ntc_op_layer_norm_workspace(int64_t rows, int64_t C);
+int ntc_op_layer_norm_backward(const ntc_layer_norm_desc* d, void* stream, char* why, size_t why_cap);
+
+/* ---------------------------------------------------------------- rotary positions of several axes
+ * Up to two tensors (queries and keys) of tokens x heads x head_dim elements, a head's contiguous, tokens and heads at any strides; results are
+ * contiguous [tokens][heads][head_dim]. A token has a position (an integer) on each of `axes` axes; axis m turns sections[m] pairs of a head's elements, in
+ * order: pair p of all P is elements p and p + P, or with `interleaved` 2p and 2p + 1; elements from 2 P on stay as they are. The angle of an axis's pair j is its position times
+ * base^(-j / sections[m]), or with one_ladder, of pair p, base^(-p / P). (a, b) becomes (a cos - b sin, a sin + b cos); with `backward` the
+ * sine's sign is changed, which is the gradient. Frequencies are good to 2^-57 and angles are fractions of a turn in 64 bits, however far the position; sines, cosines and sums are 32-bit, rounded once. */
+enum { NTC_ROTARY_AXES = 8, NTC_ROTARY_PAIRS = 128 };
+typedef struct ntc_rotary_desc {
+    const void* positions;                 /* [tokens] rows of `axes` integers, at position_stride elements */
+    int64_t position_stride, tokens;
+    const void* x[2];
+    void* y[2];
+    int64_t token_stride[2], head_stride[2];
+    int32_t heads[2];                      /* 0: no such tensor */
+    int32_t head_dim, axes, position_bytes, dtype, one_ladder, interleaved, backward;
+    int32_t sections[NTC_ROTARY_AXES];
+    double base;
+} ntc_rotary_desc;
+int ntc_op_rotary(const ntc_rotary_desc* d, void* stream, char* why, size_t why_cap);
+
+/* ---------------------------------------------------------------- attention
+ * Sequences of queries against keys and values, bfloat16 or float16, heads of head_dim elements (a multiple of 8, up to 128); q_heads is a
+ * multiple of k_heads, and query head h reads key head h / (q_heads / k_heads). For query i and key j of a sequence of Lq and Lk,
+ *   s = scale q_i k_j,  where causal: j <= i + Lk - Lq,  p = softmax over the keys that are left,  o_i = sum_j p_j v_j;
+ * a query that has none left has o = 0 and lse = -inf. What the backward pass needs, null where there is none: lse (natural log sum exp s), [query rows][q_heads], and o_rest, what o's
+ * rounding left (times 2^11 for float16), without which sum dO o is too coarse beside the differences dO v - D below.
+ *
+ * Rows: with cu_q (device, `sequences` + 1 ends, the first 0, ascending) sequence b's queries are rows cu_q[b] .. cu_q[b + 1] of q_rows; rows behind the last
+ * sequence have o = 0 and no gradient. Without, each sequence has q_rows / sequences, in turn. Keys and values alike, with cu_k and k_rows. With
+ * k_lens (device) a sequence has k_lens[b] keys, the first of those rows; the others are not read. Numbers that leave their rows are cut off at the rows' ends: wrong ones give wrong
+ * results, and no access out of bounds. A row of q is at q_row_stride elements from the one before it, within a sequence and, with cu_q, from one sequence to the next; without, sequences are
+ * at q_batch_stride. All starts and strides are multiples of 8 elements (16 bytes); rows are at most 2^22 apart, heads 2^20. o, dq, dk and dv are contiguous [rows][heads][head_dim].
+ *
+ * Scores, the softmax's maximum and sum and all sums of products are 32-bit; the probabilities, and backwards their gradients, are rounded to the operands' type for the products
+ * that follow. With D = sum dO o (o before its rounding), dS = p (dO v - D): dv = sum p dO, dq = scale sum dS k, dk = scale sum dS q, the last two over the group's heads.
+ * A query that sees a key or value that is not finite is NaN where the formula is; other queries of its sequence may be as well (0 times infinity).
+ * workspace: ntc_op_attention_workspace() bytes (backward 0 or 1), any contents, at a multiple of 16 bytes. */
+typedef struct ntc_attention_desc {
+    const void *q, *k, *v;
+    void* o;
+    void* o_rest;                          /* like o */
+    float* lse;
+    const int32_t *cu_q, *cu_k, *k_lens;
+    int64_t sequences, q_rows, k_rows;
+    int64_t q_row_stride, q_head_stride, q_batch_stride;
+    int64_t k_row_stride, k_head_stride, k_batch_stride;
+    int64_t v_row_stride, v_head_stride, v_batch_stride;
+    int32_t q_heads, k_heads, head_dim, dtype, causal;
+    float scale;                           /* above 0 */
+    void* workspace;
+    /* backward only */
+    const void* d_o;                       /* rows and heads at the strides below */
+    int64_t do_row_stride, do_head_stride, do_batch_stride;
+    void *dq, *dk, *dv;                    /* null: not wanted */
+} ntc_attention_desc;
+size_t ntc_op_attention_workspace(const ntc_attention_desc* d, int32_t backward);
+int ntc_op_attention(const ntc_attention_desc* d, void* stream, char* why, size_t why_cap);
+int ntc_op_attention_backward(const ntc_attention_desc* d, void* stream, char* why, size_t why_cap);
 
 #ifdef __cplusplus
 }

@@ -176,6 +176,9 @@ size_t ntc_abi_sizeof(const char* name) {
     if (n == "ntc_adamw_tensor") return sizeof(ntc_adamw_tensor);
     if (n == "ntc_fp8_quantize_desc") return sizeof(ntc_fp8_quantize_desc);
     if (n == "ntc_fp8_matmul_desc") return sizeof(ntc_fp8_matmul_desc);
+    if (n == "ntc_layer_norm_desc") return sizeof(ntc_layer_norm_desc);
+    if (n == "ntc_rotary_desc") return sizeof(ntc_rotary_desc);
+    if (n == "ntc_attention_desc") return sizeof(ntc_attention_desc);
     return 0;
 }
 const void* ntc_op_runtime(void) { return (const void*)&hipStreamSynchronize; }

@@ -1,0 +1,676 @@
+// Attention over packed sequences, and its gradients (include/ntc_ops.h: ntc_op_attention).
+//
+// Forward, for a sequence's queries i and keys j: s = c q_i k_j (c = scale log2 e), p = 2^(s - m), o = sum p v / sum p, keys taken 64 at a time with a
+// running m and sum (rows are rescaled where a maximum rises by more than 2^8). Backward: p = 2^(s - lse), dS = p (dO v - D).
+// The query heads that share a key head are rows of one matrix: row r of a sequence is query r / G, head r % G of the G. So keys and values are read
+// once for all of them, single tokens fill a tile, and the gradients of shared heads are sums over rows like any other.
+//
+// Matrix products are 32 x 32 x 16. A lane holds one column of a result and 16 of its rows, and 8 neighbouring values of one row of an operand.
+// Scores are made transposed (keys x queries): a lane's column is a query, its maximum and sum are the lane's own (and its other half's), and the scores, rounded, are at once the
+// second operand of the product that sums over keys; which keys stand at which place of that sum does not matter as long as the other
+// operand has them in the same order: 8 places of half h are keys 4 h .. 4 h + 3 and 8 + 4 h .. 8 + 4 h + 3 of sixteen. That operand
+// (values or keys, transposed) comes from LDS by the transposing read, four keys of a column at a time. The keys' and values' gradients go the same way with
+// queries and keys exchanged. No score leaves a register.
+#include "ops_common.hpp"
+
+namespace ntc_ops {
+namespace {
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+template <class T> __device__ __forceinline__ v16f product(v4u a, v4u b, v16f c) {
+    if constexpr (std::is_same_v<T, bf16>) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typedef T v2 __attribute__((ext_vector_type(2)));
+    const v2 x = { (T)a, (T)b };
+    return __builtin_bit_cast(uint32_t, x);
+}
+// c and both halves of x
+template <class T> __device__ __forceinline__ float add2(uint32_t x, float c) {
+    typedef T v2 __attribute__((ext_vector_type(2)));
+    const v2 one = { (T)1.f, (T)1.f };
+    if constexpr (std::is_same_v<T, bf16>) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, x), one, c, false);
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, x), one, c, false);
+}
+// of lanes l and l ^ 32
+__device__ __forceinline__ float other_half(float x) {
+    const uint32_t b = __float_as_uint(x);
+    const auto p = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __uint_as_float(lane_id() < 32 ? (uint32_t)p[1] : (uint32_t)p[0]);
+}
+
+struct Operand3 { const char* p; long long row, head, batch; };    // strides in bytes
+struct AttentionArgs {
+    Operand3 q, k, v, d_o;
+    void *out, *rest, *dq, *dk, *dv;
+    float *lse, *delta, *extent;
+    const int *cu_q, *cu_k, *k_lens;
+    long long q_rows, k_rows;
+    int sequences, q_each, k_each;     // rows of a sequence where there are no ends
+    int q_heads, k_heads, group, D, causal;
+    unsigned group_magic;              // ceil(2^32 / group): x / group is the high word of the product with it where x group < 2^32; 0 for 1
+    int tiles, tiles_each;             // tiles of rows (or keys) in all, and of each sequence where there are no ends
+    float scale, c;                    // c: scale log2 e
+};
+
+constexpr int kRows = 128, kKeys = 64, kExtents = 256;
+
+// ---------------------------------------------------------------- which rows
+struct Span { int b; long long row; int n; long long start; };     // sequence, its first row in all, its rows, the byte where they start
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long long cut(long long x, long long lo, long long hi) { return x < lo ? lo : x > hi ? hi : x; }
+
+// Tile t of all, to its sequence and its number there. With ends, sequence b's tiles are numbered from e_b units / size + b on, which leaves each at least as many numbers as
+// it has tiles, and none shared: the largest b whose first number is at most t, by 64 probes at once. Rows behind the last sequence are one more.
+template <int kSize> __device__ __forceinline__ int find_sequence(const int* cu, int sequences, int tiles_each, int units, int t, int& tile) {
+    if (!cu) { const int b = t / tiles_each; tile = t - b * tiles_each; return b; }
+    const auto first = [&](int b) { const long long e = b ? cu[b] : 0; return (int)cut(e * units / kSize, 0, 1 << 30) + b; };
+    int lo = 0, hi = sequences;
+    while (lo < hi) {
+        const int step = (hi - lo + 63) / 64, probe = lo + (lane_id() + 1) * step;
+        const bool at_most = probe <= hi && first(probe <= hi ? probe : hi) <= t;
+        lo += __builtin_popcountll(__ballot(at_most)) * step;
+        hi = lo + step - 1 < hi ? lo + step - 1 : hi;
+    }
+    lo = uniform(lo < sequences ? lo : sequences);
+    tile = t - uniform(first(lo));
+    return lo;
+}
+__device__ __forceinline__ Span span_of(const int* cu, int sequences, int each, long long rows, int b, const Operand3& x) {
+    if (!cu) return { b, (long long)b * each, b < sequences ? each : 0, b * x.batch };
+    const long long first = b ? cut(cu[b], 0, rows) : 0, end = b < sequences ? cut(cu[b + 1], first, rows) : rows;
+    return { b, first, (int)(end - first), first * x.row };
+}
+// (keys that a sequence has, of those that it has room for)
+__device__ __forceinline__ int keys_of(const AttentionArgs& d, const Span& k) {
+    if (k.b >= d.sequences) return 0;
+    return d.k_lens ? (int)cut(d.k_lens[k.b], 0, k.n) : k.n;
+}
+
+// ---------------------------------------------------------------- shared memory
+// Rows of kPitch bytes; the 16-byte piece c of row r lies at c ^ spread(r): 16 rows' pieces of one number are in different banks, and so are four rows'
+// pieces of four neighbouring numbers, which a transposing read takes.
+template <int kD> struct Tile {
+    static constexpr int kPitch = kD <= 32 ? 64 : kD <= 64 ? 128 : 256, kPieces = kPitch / 16, kLines = 256 / kPitch;
+    static __device__ __forceinline__ int spread(int r) { return (((r & 3) / kLines) << 2 | ((r >> 2) & 3)) & (kPieces - 1); }
+};
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
+// 16 (4) bytes a lane from base + off to LDS at `to` + 16 (4) lane: `to` is the same in all lanes. Nothing waits for it but a vmcnt of the caller's.
+__device__ __forceinline__ void to_lds16(uint32_t to, uint32_t off, const char* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(to), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void to_lds4(uint32_t to, uint32_t off, const char* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(to), "v"(off), "s"(base) : "memory", "m0");
+}
+// All of the wave's loads have landed, and every wave is here.
+__device__ __forceinline__ void arrive() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0070);                    // vmcnt 0, lgkmcnt 0
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// 8 neighbouring values of row `row` (of 32) of the tile at `at`: columns 16 step + 8 half on
+template <int kD> __device__ __forceinline__ v4u row_piece(const char* at, int row, int half, int step) {
+    using L = Tile<kD>;
+    return *(const v4u*)(at + row * L::kPitch + (((2 * step + half) ^ L::spread(row)) << 4));
+}
+// of 16 rows from `first` on, 8 rows of column 32 tile + lane % 32: rows 4 half .. and 8 + 4 half ..
+template <int kD> __device__ __forceinline__ v4u column_piece(const char* at, int first, int tile) {
+    using L = Tile<kD>;
+    const int lane = lane_id(), i = lane & 15, half = lane >> 5;
+    v2u r[2];
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+        const int row = 8 * b + 4 * half + (i >> 2), piece = 4 * tile + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+        const char* p = at + (first + row) * L::kPitch + ((piece ^ L::spread(row)) << 4) + 8 * (i & 1);
+        r[b] = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)p));
+    }
+    return v4u{ r[0].x, r[0].y, r[1].x, r[1].y };
+}
+// rows of a matrix into a tile of kTile rows: each wave of four takes a quarter. row_off(r): the byte offset of row r (of kTile) from `base`.
+template <int kD, int kTile, class F> __device__ __forceinline__ void load_tile(uint32_t to, const char* base, int D, F row_off) {
+    using L = Tile<kD>;
+    constexpr int kEach = kTile * L::kPieces / 256;        // loads a wave
+    const int wave = uniform(threadIdx.x >> 6), lane = lane_id();
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        const int slot = (wave * kEach + i) * 64 + lane, r = slot / L::kPieces;
+        int piece = (slot % L::kPieces) ^ L::spread(r);
+        if (L::kPieces * 8 > kD || kD != D) piece = 8 * piece < D ? piece : 0;      // past a head's end: any values of the row
+        to_lds16(to + 1024 * (wave * kEach + i), row_off(r) + 16 * piece, base);
+    }
+}
+
+// ---------------------------------------------------------------- rows in registers
+// A row of a group's matrix: query and head, from a tile's first row
+struct Row { int i, g; };
+__device__ __forceinline__ Row row_at(const AttentionArgs& d, int i0, int g0, int x) {   // x rows after row (i0, g0), x + g0 < 2^16
+    const int y = g0 + x, q = d.group_magic ? (int)__umulhi((unsigned)y, d.group_magic) : y;
+    return { i0 + q, y - q * d.group };
+}
+// the lane's row as an operand: columns 16 step + 8 half .., 0 past D
+template <int kD> __device__ __forceinline__ void load_row(v4u (&x)[kD / 16], const char* p, bool live, int D) {
+    const int half = lane_id() >> 5;
+#pragma unroll
+    for (int s = 0; s < kD / 16; s++) {
+        const int col = 16 * s + 8 * half;
+        x[s] = live && col < D ? *(const v4u*)(p + 2 * col) : v4u{};
+    }
+}
+template <class T> constexpr float kRest = std::is_same_v<T, f16> ? 2048.f : 1.f;   // what a result's rounding leaves is held times this: as large as the result
+// a transposed result (32 kTiles columns of the lane's row) to memory, times f; with kRests what its rounding left
+template <class T, int kD, bool kRests = false> __device__ __forceinline__ void store_row(char* p, const v16f (&x)[kD / 32], float f, bool live, int D) {
+    const int half = lane_id() >> 5;
+#pragma unroll
+    for (int t = 0; t < kD / 32; t++)
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float y[2] = { x[t][8 * a + 2 * i] * f, x[t][8 * a + 2 * i + 1] * f };
+                if constexpr (kRests) for (float& z : y) z = (z - (float)(T)z) * kRest<T>;
+                w[i] = pack2<T>(y[0], y[1]);
+            }
+            const auto lo = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), hi = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+            const int col = 32 * t + 16 * a + 8 * half;
+            if (live && col < D) *(v4u*)(p + 2 * col) = v4u{ (uint32_t)lo[0], (uint32_t)hi[0], (uint32_t)lo[1], (uint32_t)hi[1] };
+        }
+}
+// result register r of the lane is row 8 (r / 4) + 4 half + r % 4
+__device__ __forceinline__ constexpr int result_row(int r) { return 8 * (r / 4) + r % 4; }
+template <class T> __device__ __forceinline__ v4u packed(const v16f& x, int half16) {
+    return v4u{ pack2<T>(x[8 * half16], x[8 * half16 + 1]), pack2<T>(x[8 * half16 + 2], x[8 * half16 + 3]), pack2<T>(x[8 * half16 + 4], x[8 * half16 + 5]),
+                pack2<T>(x[8 * half16 + 6], x[8 * half16 + 7]) };
+}
+
+// ---------------------------------------------------------------- forward
+template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention(AttentionArgs d) {
+    using L = Tile<kD>;
+    constexpr int kTile = kKeys * L::kPitch;
+    __shared__ alignas(1024) char lds[4 * kTile];          // keys, values; two of each
+    const long long id = block_number();
+    const int head = (int)(id % d.k_heads);
+    const long long t_ = id / d.k_heads;
+    if (t_ >= d.tiles) return;
+    int tile;
+    const int b = find_sequence<kRows>(d.cu_q, d.sequences, d.tiles_each, d.group, d.tiles - 1 - (int)t_, tile);   // (a sequence's last rows, which see most keys, first)
+    const Span qs = span_of(d.cu_q, d.sequences, d.q_each, d.q_rows, b, d.q);
+    const long long rows = (long long)qs.n * d.group;
+    if (tile < 0 || (long long)tile * kRows >= rows) return;
+    const int kb = b < d.sequences ? b : 0;
+    Span ks = span_of(d.cu_k, d.sequences, d.k_each, d.k_rows, kb, d.k);
+    const int Lk = b < d.sequences ? keys_of(d, ks) : 0, off = Lk - qs.n;
+    const long long v_start = d.cu_k ? ks.row * d.v.row : ks.b * d.v.batch;
+
+    const int lane = lane_id(), wave = uniform(threadIdx.x >> 6), column = lane & 31, half = lane >> 5;
+    const int r0 = tile * kRows + 32 * wave, i0 = r0 / d.group, g0 = r0 - i0 * d.group;
+    const Row row = row_at(d, i0, g0, column);
+    const bool live = row.i < qs.n;
+    v4u q[kD / 16];
+    load_row<kD>(q, d.q.p + qs.start + row.i * d.q.row + (head * d.group + row.g) * d.q.head, live, d.D);
+    const int last = d.causal ? (row.i + off < Lk - 1 ? row.i + off : Lk - 1) : Lk - 1;                           // the last key that the lane's query sees
+    const int wave_first = d.causal ? (i0 + off < Lk - 1 ? i0 + off : Lk - 1) : Lk - 1;                           // ... that each of the wave's does
+    const int i_wave = (r0 + 31) / d.group, i_block = (int)(((long long)tile * kRows + kRows - 1) / d.group);
+    const int wave_last = d.causal ? (i_wave + off < Lk - 1 ? i_wave + off : Lk - 1) : Lk - 1;
+    const int block_last = d.causal ? (i_block + off < Lk - 1 ? i_block + off : Lk - 1) : Lk - 1;
+    const int stages = block_last < 0 ? 0 : block_last / kKeys + 1;
+
+    const char *kp = d.k.p + ks.start + head * d.k.head, *vp = d.v.p + v_start + head * d.v.head;
+    const uint32_t lds0 = lds_address(lds);
+    const auto load = [&](int s) {
+        const int k0 = s * kKeys, n = Lk - k0;             // rows past the end read the last one
+        const char *kb_ = kp + k0 * d.k.row, *vb_ = vp + k0 * d.v.row;
+        load_tile<kD, kKeys>(lds0 + (s & 1) * 2 * kTile, kb_, d.D, [&](int r) { return (uint32_t)(r < n ? r : n - 1) * (uint32_t)d.k.row; });
+        load_tile<kD, kKeys>(lds0 + (s & 1) * 2 * kTile + kTile, vb_, d.D, [&](int r) { return (uint32_t)(r < n ? r : n - 1) * (uint32_t)d.v.row; });
+    };
+    v16f o[kD / 32] = {};
+    // Two sums of the probabilities: as rounded, by which the result is divided (what rounding adds to all values alike is then in both), and as they are, for lse.
+    float m = -NTC_INF, l = 0, exact = 0;
+    if (stages) load(0);
+    for (int s = 0; s < stages; s++) {
+        arrive();
+        if (s + 1 < stages) load(s + 1);
+        const int k0 = s * kKeys;
+        if (k0 > wave_last) continue;
+        const char *kt = lds + (s & 1) * 2 * kTile, *vt = kt + kTile;
+        v16f x[2] = {};
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < kD / 16; i++) x[j] = product<T>(row_piece<kD>(kt + 32 * j * L::kPitch, column, half, i), q[i], x[j]);
+        if (k0 + kKeys - 1 > wave_first) {
+            const int seen = last - k0 - 4 * half;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) x[j][r] = 32 * j + result_row(r) <= seen ? x[j][r] : -NTC_INF;
+        }
+        float most = x[0][0];
+#pragma unroll
+        for (int r = 1; r < 32; r++) most = __builtin_fmaxf(most, x[r / 16][r % 16]);
+        most = __builtin_fmaxf(most, other_half(most));
+        const bool rises = most * d.c > m * d.c + 8.f;     // (m is -inf at first)
+        if (__any(rises)) {
+            const float next = rises ? most : m, by = m == next ? 1.f : fast_exp2((m - next) * d.c);
+            m = next;
+            l *= by;
+            exact *= by;
+#pragma unroll
+            for (int t = 0; t < kD / 32; t++) o[t] *= by;
+        }
+        const float mc = m == -NTC_INF ? 0.f : m * d.c;
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) x[j][r] = fast_exp2(__builtin_fmaf(x[j][r], d.c, -mc));
+        if (d.lse) {
+#pragma unroll
+            for (int r = 0; r < 32; r++) exact += x[r / 16][r % 16];
+        }
+#pragma unroll
+        for (int h = 0; h < 4; h++) {
+            const v4u p = packed<T>(x[h / 2], h & 1);
+            l = add2<T>(p.w, add2<T>(p.z, add2<T>(p.y, add2<T>(p.x, l))));
+#pragma unroll
+            for (int t = 0; t < kD / 32; t++) o[t] = product<T>(column_piece<kD>(vt, 16 * h, t), p, o[t]);
+        }
+    }
+    l += other_half(l);
+    exact += other_half(exact);
+    const long long at = (qs.row + row.i) * d.q_heads + head * d.group + row.g;
+    const float f = l == 0 ? 0.f : 1.f / l;
+    store_row<T, kD>((char*)d.out + at * d.D * 2, o, f, live, d.D);
+    if (d.rest) store_row<T, kD, true>((char*)d.rest + at * d.D * 2, o, f, live, d.D);
+    if (d.lse && live && half == 0) d.lse[at] = exact == 0 ? -NTC_INF : (m * d.c + fast_log2(exact)) * kLn2;
+}
+
+// ---------------------------------------------------------------- backward
+// float16: the score's gradients, and probabilities of long rows, leave its range. They are multiplied by powers of two: probabilities by 2^14, the score's
+// gradients by the largest that keeps 2 D max|dO| max|v|, which they cannot pass, within 2^15. Largest values of 256 blocks' shares, joined by whoever reads them.
+template <class T> __global__ void __launch_bounds__(256) k_attention_extent(AttentionArgs d) {
+    __shared__ float parts[2][4];
+    float of_v = 0, of_do = 0;
+    const int pieces = d.D / 8;
+    const auto largest = [&](const char* p, float& to) {
+        typedef T v8 __attribute__((ext_vector_type(8)));
+        const v8 x = *(const v8*)p;
+#pragma unroll
+        for (int i = 0; i < 8; i++) to = __builtin_fmaxf(to, __builtin_fabsf((float)x[i]));
+    };
+    for (int t = blockIdx.x; t < d.tiles; t += gridDim.x) {
+        int tile;
+        const int b = find_sequence<kRows>(d.cu_k, d.sequences, d.tiles_each, 1, t, tile);
+        if (b >= d.sequences) continue;
+        const Span ks = span_of(d.cu_k, d.sequences, d.k_each, d.k_rows, b, d.v);
+        const int first = tile * kRows, n = tile < 0 ? 0 : keys_of(d, ks) - first;
+        const int all = (n < kRows ? n : kRows) * d.k_heads * pieces;
+        for (int x = threadIdx.x; x < all; x += 256) {
+            const int piece = x % pieces, y = x / pieces, h = y % d.k_heads, r = y / d.k_heads;
+            largest(d.v.p + ks.start + (first + r) * d.v.row + h * d.v.head + piece * 16, of_v);
+        }
+    }
+    const long long rows = d.cu_q ? cut(d.cu_q[d.sequences], 0, d.q_rows) : d.q_rows, all = rows * d.q_heads * pieces;
+    for (long long x = blockIdx.x * 256ll + threadIdx.x; x < all; x += gridDim.x * 256ll) {
+        const int piece = (int)(x % pieces);
+        const long long y = x / pieces, r = y / d.q_heads;
+        const int h = (int)(y % d.q_heads);
+        const long long start = d.cu_q ? r * d.d_o.row : r / d.q_each * d.d_o.batch + r % d.q_each * d.d_o.row;
+        largest(d.d_o.p + start + h * d.d_o.head + piece * 16, of_do);
+    }
+    const auto most = [](float a, float b) { return __builtin_fmaxf(a, b); };
+    of_v = reduce64(of_v, most);
+    of_do = reduce64(of_do, most);
+    if (lane_id() == 0) { parts[0][threadIdx.x >> 6] = of_v; parts[1][threadIdx.x >> 6] = of_do; }
+    __syncthreads();
+    if (threadIdx.x < 2) d.extent[threadIdx.x * kExtents + blockIdx.x] = most(most(parts[threadIdx.x][0], parts[threadIdx.x][1]), most(parts[threadIdx.x][2], parts[threadIdx.x][3]));
+}
+// The power of two for the scores' gradients, as an exponent.
+template <class T> __device__ __forceinline__ int gradient_exponent(const AttentionArgs& d) {
+    if constexpr (!std::is_same_v<T, f16>) return 0;
+    float most[2] = {};
+#pragma unroll
+    for (int w = 0; w < 2; w++)
+#pragma unroll
+        for (int i = 0; i < kExtents / 64; i++) most[w] = __builtin_fmaxf(most[w], d.extent[w * kExtents + 64 * i + lane_id()]);
+    const auto larger = [](float a, float b) { return __builtin_fmaxf(a, b); };
+    const float bound = 2.f * d.D * reduce64(most[0], larger) * reduce64(most[1], larger);
+    if (!(bound > 0) || bound > 3e38f) return 0;
+    const int e = 14 - (int)((__float_as_uint(bound) >> 23) - 127);
+    return uniform(e < -60 ? -60 : e > 60 ? 60 : e);
+}
+__device__ __forceinline__ float two_to(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }
+template <class T> constexpr int kShift = std::is_same_v<T, f16> ? 14 : 0;      // probabilities are held times 2^kShift
+
+// A row's dS add up to 0; rounded, they do not quite, and neither where the sum dO o is that of rounded probabilities. What they add up to, times a vector that is near
+// all keys, is taken off: the error of dq is then one of the keys' differences from it, and keys with much in common keep their gradients' precision. The vector
+// is the mean of the first stage's keys, left in shared memory meanwhile.
+template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention_dq(AttentionArgs d) {
+    using L = Tile<kD>;
+    constexpr int kTile = kKeys * L::kPitch;
+    __shared__ alignas(1024) char lds[4 * kTile];
+    __shared__ alignas(16) float mean[kD];
+    const long long id = block_number();
+    const int head = (int)(id % d.k_heads);
+    const long long t_ = id / d.k_heads;
+    if (t_ >= d.tiles) return;
+    int tile;
+    const int b = find_sequence<kRows>(d.cu_q, d.sequences, d.tiles_each, d.group, d.tiles - 1 - (int)t_, tile);
+    const Span qs = span_of(d.cu_q, d.sequences, d.q_each, d.q_rows, b, d.q);
+    const long long rows = (long long)qs.n * d.group;
+    if (tile < 0 || (long long)tile * kRows >= rows) return;
+    const int kb = b < d.sequences ? b : 0;
+    Span ks = span_of(d.cu_k, d.sequences, d.k_each, d.k_rows, kb, d.k);
+    const int Lk = b < d.sequences ? keys_of(d, ks) : 0, off = Lk - qs.n;
+    const long long v_start = d.cu_k ? ks.row * d.v.row : ks.b * d.v.batch, do_start = d.cu_q ? qs.row * d.d_o.row : qs.b * d.d_o.batch;
+
+    const int lane = lane_id(), wave = uniform(threadIdx.x >> 6), column = lane & 31, half = lane >> 5;
+    const int r0 = tile * kRows + 32 * wave, i0 = r0 / d.group, g0 = r0 - i0 * d.group;
+    const Row row = row_at(d, i0, g0, column);
+    const bool live = row.i < qs.n;
+    const int h = head * d.group + row.g;
+    const long long at = (qs.row + row.i) * d.q_heads + h;
+    v4u q[kD / 16], g[kD / 16];
+    float delta = 0;
+    {
+        v4u o[kD / 16], rest[kD / 16];
+        load_row<kD>(o, (const char*)d.out + at * d.D * 2, live, d.D);
+        load_row<kD>(rest, (const char*)d.rest + at * d.D * 2, live, d.D);
+        load_row<kD>(g, d.d_o.p + do_start + row.i * d.d_o.row + h * d.d_o.head, live, d.D);
+        typedef T v8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+        for (int s = 0; s < kD / 16; s++) {
+            const v8 a = __builtin_bit_cast(v8, o[s]), r = __builtin_bit_cast(v8, rest[s]), c = __builtin_bit_cast(v8, g[s]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) delta = __builtin_fmaf(__builtin_fmaf((float)r[i], 1 / kRest<T>, (float)a[i]), (float)c[i], delta);
+        }
+    }
+    load_row<kD>(q, d.q.p + qs.start + row.i * d.q.row + h * d.q.head, live, d.D);
+    delta += other_half(delta);
+    if (live && half == 0) d.delta[at] = delta;
+    const int e = gradient_exponent<T>(d);
+    const float up = two_to(e), lse = live ? d.lse[at] * kLog2e : 0.f, delta_up = delta * up;
+    const int last = d.causal ? (row.i + off < Lk - 1 ? row.i + off : Lk - 1) : Lk - 1;
+    const int wave_first = d.causal ? (i0 + off < Lk - 1 ? i0 + off : Lk - 1) : Lk - 1;
+    const int i_wave = (r0 + 31) / d.group, i_block = (int)(((long long)tile * kRows + kRows - 1) / d.group);
+    const int wave_last = d.causal ? (i_wave + off < Lk - 1 ? i_wave + off : Lk - 1) : Lk - 1;
+    const int block_last = d.causal ? (i_block + off < Lk - 1 ? i_block + off : Lk - 1) : Lk - 1;
+    const int stages = block_last < 0 ? 0 : block_last / kKeys + 1;
+
+    const char *kp = d.k.p + ks.start + head * d.k.head, *vp = d.v.p + v_start + head * d.v.head;
+    const uint32_t lds0 = lds_address(lds);
+    const auto load = [&](int s) {
+        const int k0 = s * kKeys, n = Lk - k0;
+        const char *kb_ = kp + k0 * d.k.row, *vb_ = vp + k0 * d.v.row;
+        load_tile<kD, kKeys>(lds0 + (s & 1) * 2 * kTile, kb_, d.D, [&](int r) { return (uint32_t)(r < n ? r : n - 1) * (uint32_t)d.k.row; });
+        load_tile<kD, kKeys>(lds0 + (s & 1) * 2 * kTile + kTile, vb_, d.D, [&](int r) { return (uint32_t)(r < n ? r : n - 1) * (uint32_t)d.v.row; });
+    };
+    v16f dq[kD / 32] = {};
+    float sum = 0;
+    if (stages) load(0);
+    for (int s = 0; s < stages; s++) {
+        arrive();
+        if (s + 1 < stages) load(s + 1);
+        const char *kt = lds + (s & 1) * 2 * kTile, *vt = kt + kTile;
+        if (s == 0 && wave == 0) {
+            const uint32_t one = pack2<T>(1.f, 1.f);
+#pragma unroll
+            for (int t = 0; t < kD / 32; t++) {
+                v16f x = {};
+#pragma unroll
+                for (int a = 0; a < kKeys / 16; a++) x = product<T>(column_piece<kD>(kt, 16 * a, t), v4u{ one, one, one, one }, x);
+#pragma unroll
+                for (int r = 0; r < 16; r++) if (column == 0) mean[32 * t + result_row(r) + 4 * half] = x[r] * (1.f / kKeys);
+            }
+        }
+        if (s * kKeys > wave_last) continue;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int k0 = s * kKeys + 32 * j;
+            v16f x = {}, y = {};
+#pragma unroll
+            for (int i = 0; i < kD / 16; i++) x = product<T>(row_piece<kD>(kt + 32 * j * L::kPitch, column, half, i), q[i], x);
+#pragma unroll
+            for (int i = 0; i < kD / 16; i++) y = product<T>(row_piece<kD>(vt + 32 * j * L::kPitch, column, half, i), g[i], y);
+#pragma unroll
+            for (int r = 0; r < 16; r++) x[r] = fast_exp2(__builtin_fmaf(x[r], d.c, -lse)) * __builtin_fmaf(y[r], up, -delta_up);
+            if (k0 + 31 > wave_first) {
+                const int seen = last - k0 - 4 * half;
+#pragma unroll
+                for (int r = 0; r < 16; r++) x[r] = result_row(r) <= seen ? x[r] : 0.f;
+            }
+#pragma unroll
+            for (int a = 0; a < 2; a++) {
+                const v4u p = packed<T>(x, a);
+                sum = add2<T>(p.w, add2<T>(p.z, add2<T>(p.y, add2<T>(p.x, sum))));
+#pragma unroll
+                for (int t = 0; t < kD / 32; t++) dq[t] = product<T>(column_piece<kD>(kt, 32 * j + 16 * a, t), p, dq[t]);
+            }
+        }
+    }
+    if (stages) {
+        __syncthreads();
+        sum += other_half(sum);
+#pragma unroll
+        for (int t = 0; t < kD / 32; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) dq[t][r] = __builtin_fmaf(-sum, mean[32 * t + result_row(r) + 4 * half], dq[t][r]);
+    }
+    store_row<T, kD>((char*)d.dq + at * d.D * 2, dq, d.scale * two_to(-e), live && d.dq, d.D);
+}
+
+template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 2) k_attention_dkv(AttentionArgs d) {
+    using L = Tile<kD>;
+    constexpr int kStep = 64, kTile = kStep * L::kPitch, kStage = 2 * kTile + 8 * kStep;
+    __shared__ alignas(1024) char lds[2 * kStage];         // queries, gradients, log sums and deltas of kStep rows; two of each
+    const long long id = block_number();
+    const int head = (int)(id % d.k_heads);
+    const long long t_ = id / d.k_heads;
+    if (t_ >= d.tiles) return;
+    int tile;
+    const int b = find_sequence<kRows>(d.cu_k, d.sequences, d.tiles_each, 1, (int)t_, tile);                      // (a sequence's first keys, which most queries see, first)
+    const Span ks = span_of(d.cu_k, d.sequences, d.k_each, d.k_rows, b, d.k);
+    if (tile < 0 || (long long)tile * kRows >= ks.n) return;
+    const bool none = b >= d.sequences;
+    const int Lk = none ? 0 : keys_of(d, ks);
+    Span qs = span_of(d.cu_q, d.sequences, d.q_each, d.q_rows, none ? 0 : b, d.q);
+    if (none) qs.n = 0;
+    const int off = Lk - qs.n;
+    const long long v_start = d.cu_k ? ks.row * d.v.row : ks.b * d.v.batch, do_start = d.cu_q ? qs.row * d.d_o.row : qs.b * d.d_o.batch;
+
+    const int lane = lane_id(), wave = uniform(threadIdx.x >> 6), column = lane & 31, half = lane >> 5;
+    const int k0 = tile * kRows + 32 * wave, key = k0 + column;
+    const bool held = key < ks.n, live = key < Lk;
+    v4u k[kD / 16], v[kD / 16];
+    load_row<kD>(k, d.k.p + ks.start + key * d.k.row + head * d.k.head, live, d.D);
+    load_row<kD>(v, d.v.p + v_start + key * d.v.row + head * d.v.head, live, d.D);
+    const int e = gradient_exponent<T>(d);
+    const float up = two_to(e);
+
+    // Row r sees key j where r >= (j - off) G: the lane's first row, the wave's first whole one, and where the block starts
+    const int rows = qs.n * d.group;
+    const auto first_row = [&](int j) { return d.causal && j > off ? (j - off) * d.group : 0; };
+    const int lane_first = live ? first_row(key) : 1 << 30, wave_first = k0 + 31 < Lk ? first_row(k0 + 31) : 1 << 30, wave_start = first_row(k0);
+    const int stages = tile * kRows < Lk ? (rows + kStep - 1) / kStep : 0, start = stages ? first_row(tile * kRows) / kStep : 0;
+
+    const char *qp = d.q.p + qs.start + head * d.group * d.q.head, *gp = d.d_o.p + do_start + head * d.group * d.d_o.head;
+    const long long at0 = qs.row * d.q_heads + head * d.group;
+    const uint32_t lds0 = lds_address(lds);
+    const auto load = [&](int s) {
+        const int r0 = s * kStep, n = rows - r0, i0 = r0 / d.group, g0 = r0 - i0 * d.group;
+        const uint32_t to = lds0 + (s & 1) * kStage;
+        const auto place = [&](int r, long long row, long long head_) {
+            const Row x = row_at(d, 0, g0, r < n ? r : n - 1);
+            return (uint32_t)x.i * (uint32_t)row + (uint32_t)x.g * (uint32_t)head_;
+        };
+        load_tile<kD, kStep>(to, qp + i0 * d.q.row, d.D, [&](int r) { return place(r, d.q.row, d.q.head); });
+        load_tile<kD, kStep>(to + kTile, gp + i0 * d.d_o.row, d.D, [&](int r) { return place(r, d.d_o.row, d.d_o.head); });
+        if (wave < 2) to_lds4(to + 2 * kTile + 4 * kStep * wave, place(lane, 4ll * d.q_heads, 4), (const char*)((wave ? d.delta : d.lse) + at0 + (long long)i0 * d.q_heads));
+    };
+    v16f dk[kD / 32] = {}, dv[kD / 32] = {};
+    if (start < stages) load(start);
+    for (int s = start; s < stages; s++) {
+        arrive();
+        if (s + 1 < stages) load(s + 1);
+        const char *qt = lds + (s & 1) * kStage, *gt = qt + kTile;
+        const float* sums = (const float*)(gt + kTile);
+        if (s * kStep + kStep <= wave_start) continue;
+#pragma unroll
+        for (int j = 0; j < kStep / 32; j++) {
+            const int r0 = s * kStep + 32 * j;
+            v16f x = {}, y = {};
+#pragma unroll
+            for (int i = 0; i < kD / 16; i++) x = product<T>(row_piece<kD>(qt + 32 * j * L::kPitch, column, half, i), k[i], x);
+#pragma unroll
+            for (int i = 0; i < kD / 16; i++) y = product<T>(row_piece<kD>(gt + 32 * j * L::kPitch, column, half, i), v[i], y);
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int row = 32 * j + result_row(r) + 4 * half;
+                x[r] = fast_exp2(__builtin_fmaf(x[r], d.c, -__builtin_fmaf(sums[row], kLog2e, -(float)kShift<T>)));
+                y[r] = x[r] * __builtin_fmaf(y[r], up * two_to(-kShift<T>), -(sums[kStep + row] * (up * two_to(-kShift<T>))));
+            }
+            if (r0 < wave_first || r0 + 32 > rows) {
+                const int lo = lane_first - r0 - 4 * half, hi = rows - r0 - 4 * half;
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const bool seen = result_row(r) >= lo && result_row(r) < hi;
+                    x[r] = seen ? x[r] : 0.f;
+                    y[r] = seen ? y[r] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < 2; a++) {
+                const v4u p = packed<T>(x, a), z = packed<T>(y, a);
+#pragma unroll
+                for (int t = 0; t < kD / 32; t++) {
+                    dv[t] = product<T>(column_piece<kD>(gt, 32 * j + 16 * a, t), p, dv[t]);
+                    dk[t] = product<T>(column_piece<kD>(qt, 32 * j + 16 * a, t), z, dk[t]);
+                }
+            }
+        }
+    }
+    if (!live) {
+#pragma unroll
+        for (int t = 0; t < kD / 32; t++) { dk[t] = v16f{}; dv[t] = v16f{}; }
+    }
+    const long long at = (ks.row + key) * d.k_heads + head;
+    store_row<T, kD>((char*)d.dk + at * d.D * 2, dk, d.scale * two_to(-e), held && d.dk, d.D);
+    store_row<T, kD>((char*)d.dv + at * d.D * 2, dv, two_to(-kShift<T>), held && d.dv, d.D);
+}
+
+// ---------------------------------------------------------------- launches
+const char* wrong(const ntc_attention_desc* d, bool back) {
+    if (!d) return "no description";
+    if (d->sequences < 0 || d->q_rows < 0 || d->k_rows < 0 || d->sequences >= 1 << 30) return "sequences and rows from 0 on are needed, fewer than 2^30 sequences";
+    if (d->dtype != NTC_BF16 && d->dtype != NTC_F16) return "queries, keys and values are bfloat16 or float16";
+    if (d->head_dim < 8 || d->head_dim > 128 || d->head_dim % 8) return "a head has a multiple of 8 elements, up to 128";
+    if (d->k_heads < 1 || d->q_heads < 1 || d->q_heads % d->k_heads || d->q_heads / d->k_heads > 1024 || d->q_heads > 65536) return "query heads must be 1 to 1024 times the key heads, at most 65536";
+    if (!(d->scale > 0) || !(d->scale < 1e30f)) return "scale must be a number above 0";
+    if (d->q_rows * (d->q_heads / d->k_heads) >= (int64_t)1 << 30 || d->k_rows >= (int64_t)1 << 30) return "fewer than 2^30 keys, and queries times a group's heads, are needed";
+    if (!d->cu_q && d->sequences && d->q_rows % d->sequences) return "without ends every sequence has as many queries";
+    if (!d->cu_k && d->sequences && d->k_rows % d->sequences) return "without ends every sequence has as many keys";
+    if (!d->sequences && ((d->q_rows && !d->cu_q) || (d->k_rows && !d->cu_k))) return "rows without a sequence";
+    const int64_t* s = &d->q_row_stride;
+    for (int i = 0; i < 9; i++) if (s[i] < 0 || s[i] % 8 || (i % 3 == 0 && s[i] > 1 << 22) || (i % 3 == 1 && s[i] > 1 << 20)) return "strides are multiples of 8 elements from 0 on, of rows at most 2^22, of heads 2^20";
+    if (back) {
+        const int64_t* t = &d->do_row_stride;
+        for (int i = 0; i < 3; i++) if (t[i] < 0 || t[i] % 8 || (i == 0 && t[i] > 1 << 22) || (i == 1 && t[i] > 1 << 20)) return "strides are multiples of 8 elements from 0 on, of rows at most 2^22, of heads 2^20";
+    }
+    if (d->q_rows && (!d->q || !d->o || (back && (!d->d_o || !d->lse || !d->o_rest || !d->workspace)))) return "null pointer";
+    if (d->k_rows && (!d->k || !d->v)) return "null pointer";
+    uintptr_t all = (uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->o | (uintptr_t)d->o_rest | (uintptr_t)d->workspace;
+    if (back) all |= (uintptr_t)d->d_o | (uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv;
+    if (all % 16) return "operands, results and the workspace start at a multiple of 16 bytes";
+    return nullptr;
+}
+AttentionArgs args_of(const ntc_attention_desc* d) {
+    AttentionArgs a = {};
+    a.q = { (const char*)d->q, 2 * d->q_row_stride, 2 * d->q_head_stride, 2 * d->q_batch_stride };
+    a.k = { (const char*)d->k, 2 * d->k_row_stride, 2 * d->k_head_stride, 2 * d->k_batch_stride };
+    a.v = { (const char*)d->v, 2 * d->v_row_stride, 2 * d->v_head_stride, 2 * d->v_batch_stride };
+    a.d_o = { (const char*)d->d_o, 2 * d->do_row_stride, 2 * d->do_head_stride, 2 * d->do_batch_stride };
+    a.out = d->o; a.rest = d->o_rest; a.dq = d->dq; a.dk = d->dk; a.dv = d->dv;
+    a.lse = d->lse;
+    a.cu_q = d->cu_q; a.cu_k = d->cu_k; a.k_lens = d->k_lens;
+    a.q_rows = d->q_rows; a.k_rows = d->k_rows;
+    a.sequences = (int)d->sequences;
+    a.q_each = d->sequences ? (int)(d->q_rows / d->sequences) : 0;
+    a.k_each = d->sequences ? (int)(d->k_rows / d->sequences) : 0;
+    a.q_heads = d->q_heads; a.k_heads = d->k_heads; a.group = d->q_heads / d->k_heads; a.D = d->head_dim; a.causal = d->causal != 0;
+    a.group_magic = a.group > 1 ? (unsigned)((((uint64_t)1 << 32) + a.group - 1) / a.group) : 0;
+    a.scale = d->scale;
+    a.c = d->scale * kLog2e;
+    return a;
+}
+// tiles of `size` of rows that lie in sequences (each at most a tile more than its share, one more for what is behind the last)
+void set_tiles(AttentionArgs& a, bool ends, int64_t each, int64_t rows, int64_t size) {
+    a.tiles_each = (int)((each + size - 1) / size);
+    a.tiles = (int)(ends ? rows / size + a.sequences + 1 : (int64_t)a.tiles_each * a.sequences);
+}
+template <class F> void with_head(int dtype, int D, F f) {
+    const auto go = [&](auto t) {
+        if (D <= 32) f(t, std::integral_constant<int, 32>{});
+        else if (D <= 64) f(t, std::integral_constant<int, 64>{});
+        else if (D <= 96) f(t, std::integral_constant<int, 96>{});
+        else f(t, std::integral_constant<int, 128>{});
+    };
+    if (dtype == NTC_BF16) go(bf16{});
+    else go(f16{});
+}
+size_t rounded(size_t n) { return (n + 15) / 16 * 16; }
+
+}  // namespace
+}  // namespace ntc_ops
+
+using namespace ntc_ops;
+
+extern "C" {
+
+size_t ntc_op_attention_workspace(const ntc_attention_desc* d, int32_t backward) {
+    if (!d || !backward || d->q_rows < 1) return 0;
+    return rounded((size_t)d->q_rows * d->q_heads * 4) + 2 * kExtents * 4;
+}
+
+int ntc_op_attention(const ntc_attention_desc* d, void* stream, char* why, size_t cap) {
+    if (const char* w = wrong(d, false)) return refuse(why, cap, w);
+    if (!d->q_rows) return 0;
+    AttentionArgs a = args_of(d);
+    set_tiles(a, d->cu_q, (int64_t)a.q_each * a.group, a.q_rows * a.group, kRows);
+    const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads);
+    with_head(d->dtype, d->head_dim, [&](auto t, auto h) { k_attention<decltype(t), h.value><<<grid, 256, 0, (hipStream_t)stream>>>(a); });
+    return launched(why, cap);
+}
+
+int ntc_op_attention_backward(const ntc_attention_desc* d, void* stream, char* why, size_t cap) {
+    if (const char* w = wrong(d, true)) return refuse(why, cap, w);
+    const hipStream_t s = (hipStream_t)stream;
+    AttentionArgs a = args_of(d);
+    a.delta = (float*)d->workspace;
+    a.extent = (float*)((char*)d->workspace + rounded((size_t)d->q_rows * d->q_heads * 4));
+    if (d->q_rows) {
+        if (d->dtype == NTC_F16) {
+            set_tiles(a, d->cu_k, a.k_each, a.k_rows, kRows);
+            k_attention_extent<f16><<<kExtents, 256, 0, s>>>(a);
+        }
+        set_tiles(a, d->cu_q, (int64_t)a.q_each * a.group, a.q_rows * a.group, kRows);
+        const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads);
+        with_head(d->dtype, d->head_dim, [&](auto t, auto h) { k_attention_dq<decltype(t), h.value><<<grid, 256, 0, s>>>(a); });
+        if (const int rc = launched(why, cap)) return rc;
+    }
+    if (!d->k_rows || (!d->dk && !d->dv)) return 0;
+    set_tiles(a, d->cu_k, a.k_each, a.k_rows, kRows);
+    const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads);
+    with_head(d->dtype, d->head_dim, [&](auto t, auto h) { k_attention_dkv<decltype(t), h.value><<<grid, 256, 0, s>>>(a); });
+    return launched(why, cap);
+}
+
+}  // extern "C"

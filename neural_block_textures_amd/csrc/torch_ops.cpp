@@ -534,6 +534,343 @@ void adamw_encode(const Tensor& m, const Tensor& v, const Tensor& cm, const Tens
     });
 }
 
+// An autograd function takes a tensor that may be absent as an optional one.
+optional<Tensor> given_or_none(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
+
+// ---------------------------------------------------------------- layer norm
+// x's axes but the last `keep` ones as rows at one stride (a copy where they lie at several).
+struct Flat { Tensor t; int64_t rows, stride; };
+Flat flat(const Tensor& x, int64_t keep) {
+    const int64_t lead = x.dim() - keep;
+    int64_t rows = 1, stride = 0;
+    bool one = true;
+    for (int64_t a = lead - 1; a >= 0; a--) {
+        if (x.size(a) != 1) {
+            if (rows == 1) stride = x.stride(a);
+            else one = one && x.stride(a) == stride * rows;
+        }
+        rows *= x.size(a);
+    }
+    if (one || !rows) return { x, rows, stride };
+    const Tensor c = x.contiguous();
+    int64_t inner = 1;
+    for (int64_t a = lead; a < x.dim(); a++) inner *= x.size(a);
+    return { c, rows, inner };
+}
+
+ntc_layer_norm_desc norm_desc(const Flat& x, const Tensor& w, const Tensor& b, double eps) {
+    ntc_layer_norm_desc d = {};
+    d.x = x.t.const_data_ptr();
+    d.weight = w.defined() ? w.const_data_ptr() : nullptr;
+    d.bias = b.defined() ? b.const_data_ptr() : nullptr;
+    d.rows = x.rows;
+    d.C = x.t.size(-1);
+    d.x_stride = x.stride;
+    d.dtype = type_of(x.t);
+    d.weight_type = w.defined() ? type_of(w) : b.defined() ? type_of(b) : d.dtype;
+    d.eps = (float)eps;
+    return d;
+}
+Tensor norm_forward(const Flat& x, const Tensor& w, const Tensor& b, double eps, const Tensor& stats) {
+    const Tensor y = at::empty(x.t.sizes(), x.t.options().requires_grad(false));
+    ntc_layer_norm_desc d = norm_desc(x, w, b, eps);
+    d.y = y.mutable_data_ptr();
+    d.stats = stats.defined() ? stats.mutable_data_ptr<float>() : nullptr;
+    call(x.t.device(), [&](void* s, char* why, size_t cap) { return ntc_op_layer_norm(&d, s, why, cap); });
+    return y;
+}
+Tensor last_contiguous(const Tensor& x) { return x.size(-1) > 1 && x.stride(-1) != 1 ? x.contiguous() : x; }
+
+struct NormNode : torch::autograd::Function<NormNode> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const optional<Tensor>& w_, const optional<Tensor>& b_, double eps) {
+        const Tensor w = w_ ? *w_ : Tensor(), b = b_ ? *b_ : Tensor();
+        const Flat f = flat(x, 1);
+        const Tensor stats = at::empty({ f.rows, 2 }, x.options().dtype(at::kFloat).requires_grad(false));
+        const Tensor y = norm_forward(f, w, b, eps, stats);
+        ctx->save_for_backward({ x, w, b, stats });
+        ctx->saved_data["call"] = std::vector<int64_t>{ x.requires_grad(), w.defined() && w.requires_grad(), b.defined() && b.requires_grad() };
+        ctx->saved_data["eps"] = eps;
+        ctx->set_materialize_grads(false);
+        return y;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+        if (!g[0].defined()) return { Tensor(), Tensor(), Tensor(), Tensor() };
+        const auto saved = ctx->get_saved_variables();
+        const std::vector<int64_t> need = ctx->saved_data["call"].toIntVector();
+        const Tensor &w = saved[1], &b = saved[2];
+        const Flat x = flat(saved[0], 1), dy = flat(last_contiguous(g[0]), 1);
+        ntc_layer_norm_desc d = norm_desc(x, w, b, ctx->saved_data["eps"].toDouble());
+        const Tensor dx = need[0] ? at::empty(x.t.sizes(), x.t.options().requires_grad(false)) : Tensor();
+        const auto like = [](const Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false)); };
+        const Tensor dw = need[1] ? like(w) : Tensor(), db = need[2] ? like(b) : Tensor();
+        const auto at_ = [](const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; };
+        const size_t size = need[1] || need[2] ? ntc_op_layer_norm_workspace(d.rows, d.C) : 0;
+        const Tensor work = size ? bytes((int64_t)size, dy.t) : Tensor();
+        d.stats = saved[3].data_ptr<float>();
+        d.dy = dy.t.const_data_ptr();
+        d.dy_stride = dy.stride;
+        d.dx = at_(dx);
+        d.dweight = at_(dw);
+        d.dbias = at_(db);
+        d.workspace = at_(work);
+        call(dy.t.device(), [&](void* s, char* why, size_t cap) { return ntc_op_layer_norm_backward(&d, s, why, cap); });
+        return { once(dx, "layer_norm"), once(dw, "layer_norm"), once(db, "layer_norm"), Tensor() };
+    }
+};
+
+Tensor layer_norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, double eps) {
+    floats("x", x);
+    no_tangent("x", x);
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x must have a last axis of at least one value");
+    const auto vector = [&](const char* name, const optional<Tensor>& t) {
+        if (!t) return Tensor();
+        floats(name, *t);
+        no_tangent(name, *t);
+        TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == x.size(-1) && t->device() == x.device(), name, " ", t->sizes(), " must hold x's ", x.size(-1), " columns, on its device");
+        TORCH_CHECK_VALUE(t->scalar_type() == x.scalar_type() || t->scalar_type() == at::kFloat, name, " is ", t->scalar_type(), "; it can be x's ", x.scalar_type(), " or float32");
+        return t->contiguous();
+    };
+    const Tensor w = vector("weight", weight), b = vector("bias", bias);
+    TORCH_CHECK_VALUE(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(), "weight and bias must be of one type, not ", w.defined() ? w.scalar_type() : at::kFloat, " and ",
+                      b.defined() ? b.scalar_type() : at::kFloat);
+    TORCH_CHECK_VALUE(eps >= 0 && eps <= 3e38, "eps must be a number from 0 on, not ", eps);
+    const Tensor rows = last_contiguous(x);
+    if (at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()))) return NormNode::apply(rows, given_or_none(w), given_or_none(b), eps);
+    return norm_forward(flat(rows, 1), w, b, eps, {});
+}
+
+// ---------------------------------------------------------------- rotary positions of several axes
+struct Turn { std::vector<int64_t> sections; double base; bool one_ladder, interleaved; };
+std::vector<Tensor> rotary_run(const Tensor& positions, const std::vector<Tensor>& x, const Turn& turn, bool backward) {
+    const Flat p = flat(positions, 1);
+    std::vector<Flat> f;                                   // (kept until the launch)
+    std::vector<Tensor> y;
+    ntc_rotary_desc d = {};
+    for (size_t t = 0; t < x.size(); t++) {
+        f.push_back(flat(last_contiguous(x[t]), 2));
+        y.push_back(at::empty(x[t].sizes(), x[t].options().requires_grad(false)));
+        d.x[t] = f[t].t.const_data_ptr();
+        d.y[t] = y[t].mutable_data_ptr();
+        d.token_stride[t] = f[t].stride;
+        d.head_stride[t] = f[t].t.stride(-2);
+        d.heads[t] = (int32_t)x[t].size(-2);
+    }
+    d.positions = p.t.const_data_ptr();
+    d.position_stride = p.stride;
+    d.position_bytes = (int32_t)p.t.element_size();
+    d.tokens = p.rows;
+    d.head_dim = (int32_t)x[0].size(-1);
+    d.axes = (int32_t)turn.sections.size();
+    d.dtype = type_of(x[0]);
+    d.one_ladder = turn.one_ladder;
+    d.interleaved = turn.interleaved;
+    d.backward = backward;
+    for (size_t a = 0; a < turn.sections.size(); a++) d.sections[a] = (int32_t)turn.sections[a];
+    d.base = turn.base;
+    call(x[0].device(), [&](void* s, char* why, size_t cap) { return ntc_op_rotary(&d, s, why, cap); });
+    return y;
+}
+
+struct RotaryNode : torch::autograd::Function<RotaryNode> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const optional<Tensor>& k, const Tensor& positions, const std::vector<int64_t>& sections,
+                                                  double base, bool one_ladder, bool interleaved) {
+        const Turn turn = { sections, base, one_ladder, interleaved };
+        ctx->save_for_backward({ positions });
+        ctx->saved_data["sections"] = sections;
+        ctx->saved_data["base"] = base;
+        ctx->saved_data["one_ladder"] = one_ladder;
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->set_materialize_grads(false);
+        return rotary_run(positions, k ? std::vector<Tensor>{ q, *k } : std::vector<Tensor>{ q }, turn, false);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+        const Turn turn = { ctx->saved_data["sections"].toIntVector(), ctx->saved_data["base"].toDouble(), ctx->saved_data["one_ladder"].toBool(), ctx->saved_data["interleaved"].toBool() };
+        std::vector<Tensor> given;
+        for (const Tensor& t : g) if (t.defined()) given.push_back(t);
+        torch::autograd::variable_list out(7);
+        if (given.empty()) return out;
+        const std::vector<Tensor> turned = rotary_run(ctx->get_saved_variables()[0], given, turn, true);
+        for (size_t t = 0, n = 0; t < g.size(); t++) if (g[t].defined()) out[t] = once(turned[n++], "rotary");
+        return out;
+    }
+};
+
+py::tuple rotary(const Tensor& positions_, const Tensor& q, const optional<Tensor>& k, const std::vector<int64_t>& sections, double base, bool one_ladder, bool interleaved) {
+    on_gpu("positions", positions_);
+    TORCH_CHECK_VALUE(positions_.scalar_type() == at::kLong || positions_.scalar_type() == at::kInt, "positions is ", positions_.scalar_type(), "; it can be int64, int32");
+    TORCH_CHECK_VALUE(positions_.dim() >= 1 && positions_.size(-1) == (int64_t)sections.size() && !sections.empty() && sections.size() <= NTC_ROTARY_AXES, "positions ", positions_.sizes(),
+                      " must have a last axis with a number for each of 1 to ", (int)NTC_ROTARY_AXES, " sections, not ", sections.size());
+    const auto check = [&](const char* name, const Tensor& x) {
+        floats(name, x);
+        no_tangent(name, x);
+        TORCH_CHECK_VALUE(x.dim() == positions_.dim() + 1 && x.sizes().slice(0, x.dim() - 2) == positions_.sizes().slice(0, x.dim() - 2) && x.device() == positions_.device(), name, " ", x.sizes(),
+                          " must have the positions' ", positions_.sizes(), " leading axes, then heads and their elements, on their device");
+        TORCH_CHECK_VALUE(x.size(-2) <= 1 << 19, name, " has more than 2^19 heads");
+    };
+    check("q", q);
+    if (k) {
+        check("k", *k);
+        TORCH_CHECK_VALUE(k->scalar_type() == q.scalar_type() && k->size(-1) == q.size(-1), "q and k must have one type and as wide heads, not ", q.scalar_type(), " ", q.size(-1), " and ",
+                          k->scalar_type(), " ", k->size(-1));
+    }
+    int64_t pairs = 0;
+    for (const int64_t n : sections) {
+        TORCH_CHECK_VALUE(n >= 0 && n <= NTC_ROTARY_PAIRS, "a section has 0 to ", (int)NTC_ROTARY_PAIRS, " pairs, not ", n);
+        pairs += n;
+    }
+    TORCH_CHECK_VALUE(pairs >= 1 && pairs <= NTC_ROTARY_PAIRS && 2 * pairs <= q.size(-1) && q.size(-1) % 2 == 0 && q.size(-1) <= 65536, "sections of ", pairs, " pairs in all: 1 to ",
+                      (int)NTC_ROTARY_PAIRS, " are needed, within heads of an even number of at most 65536 elements, not ", q.size(-1));
+    TORCH_CHECK_VALUE(base >= 1 && base <= 1e300, "base must be a number from 1 on, not ", base);
+    const Tensor positions = last_contiguous(positions_);
+    const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || (k && k->requires_grad()));
+    const std::vector<Tensor> y = grad ? RotaryNode::apply(q, k, positions, sections, base, one_ladder, interleaved)
+                                       : rotary_run(positions, k ? std::vector<Tensor>{ q, *k } : std::vector<Tensor>{ q }, { sections, base, one_ladder, interleaved }, false);
+    return k ? py::make_tuple(y[0], y[1]) : py::make_tuple(y[0]);
+}
+
+// ---------------------------------------------------------------- attention
+struct Strides { int64_t row, head, batch; };
+Strides strides_of(const Tensor& x) {
+    const auto stride = [&](int64_t a) { return x.size(a) == 1 ? 0 : x.stride(a); };
+    return { stride(x.dim() - 3), stride(x.dim() - 2), x.dim() == 4 ? stride(0) : 0 };
+}
+// As the kernels read it: heads contiguous, everything at multiples of 16 bytes, rows no further apart than 2^22 elements, heads than 2^20; a copy where it is not.
+Tensor readable(const Tensor& x) {
+    const Strides s = strides_of(x);
+    const bool ok = x.stride(-1) == 1 && s.row % 8 == 0 && s.head % 8 == 0 && s.batch % 8 == 0 && s.row <= 1 << 22 && s.head <= 1 << 20 && (uintptr_t)x.const_data_ptr() % 16 == 0;
+    return ok ? x : x.is_contiguous() ? x.clone(at::MemoryFormat::Contiguous) : x.contiguous();
+}
+
+struct Attend { bool causal; double scale; int64_t sequences; };
+ntc_attention_desc attention_desc(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k, const Tensor& k_lens, const Attend& how) {
+    ntc_attention_desc d = {};
+    d.q = q.const_data_ptr();
+    d.k = k.const_data_ptr();
+    d.v = v.const_data_ptr();
+    const auto ints = [](const Tensor& t) { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; };
+    d.cu_q = ints(cu_q);
+    d.cu_k = ints(cu_k);
+    d.k_lens = ints(k_lens);
+    const auto rows = [](const Tensor& t) { return t.dim() == 4 ? t.size(0) * t.size(1) : t.size(0); };
+    d.sequences = how.sequences;
+    d.q_rows = rows(q);
+    d.k_rows = rows(k);
+    const Strides sq = strides_of(q), sk = strides_of(k), sv = strides_of(v);
+    d.q_row_stride = sq.row; d.q_head_stride = sq.head; d.q_batch_stride = sq.batch;
+    d.k_row_stride = sk.row; d.k_head_stride = sk.head; d.k_batch_stride = sk.batch;
+    d.v_row_stride = sv.row; d.v_head_stride = sv.head; d.v_batch_stride = sv.batch;
+    d.q_heads = (int32_t)q.size(-2);
+    d.k_heads = (int32_t)k.size(-2);
+    d.head_dim = (int32_t)q.size(-1);
+    d.dtype = type_of(q);
+    d.causal = how.causal;
+    d.scale = (float)how.scale;
+    return d;
+}
+Tensor attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k, const Tensor& k_lens, const Attend& how, const Tensor& lse, const Tensor& rest) {
+    ntc_attention_desc d = attention_desc(q, k, v, cu_q, cu_k, k_lens, how);
+    const Tensor o = at::empty(q.sizes(), q.options().requires_grad(false));
+    d.o = o.mutable_data_ptr();
+    d.o_rest = rest.defined() ? rest.mutable_data_ptr() : nullptr;
+    d.lse = lse.defined() ? lse.mutable_data_ptr<float>() : nullptr;
+    const size_t size = ntc_op_attention_workspace(&d, 0);
+    const Tensor work = size ? bytes((int64_t)size, q) : Tensor();
+    d.workspace = size ? work.mutable_data_ptr() : nullptr;
+    call(q.device(), [&](void* s, char* why, size_t cap) { return ntc_op_attention(&d, s, why, cap); });
+    return o;
+}
+
+struct AttentionNode : torch::autograd::Function<AttentionNode> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, const optional<Tensor>& ends_q, const optional<Tensor>& ends_k,
+                          const optional<Tensor>& lens, bool causal, double scale, int64_t sequences) {
+        const Tensor cu_q = ends_q ? *ends_q : Tensor(), cu_k = ends_k ? *ends_k : Tensor(), k_lens = lens ? *lens : Tensor();
+        const Tensor q = readable(q_), k = readable(k_), v = readable(v_);
+        const Tensor lse = at::empty({ q.numel() / q.size(-1) }, q.options().dtype(at::kFloat).requires_grad(false));
+        const Tensor rest = at::empty(q.sizes(), q.options().requires_grad(false));
+        const Tensor o = attention_forward(q, k, v, cu_q, cu_k, k_lens, { causal, scale, sequences }, lse, rest);
+        ctx->save_for_backward({ q, k, v, o, lse, cu_q, cu_k, k_lens, rest });
+        ctx->saved_data["causal"] = causal;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["sequences"] = sequences;
+        ctx->saved_data["need"] = std::vector<int64_t>{ q_.requires_grad(), k_.requires_grad(), v_.requires_grad() };
+        ctx->set_materialize_grads(false);
+        return o;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        torch::autograd::variable_list out(9);
+        if (!grads[0].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        const std::vector<int64_t> need = ctx->saved_data["need"].toIntVector();
+        const Tensor g = readable(grads[0]);
+        ntc_attention_desc d = attention_desc(saved[0], saved[1], saved[2], saved[5], saved[6], saved[7],
+                                              { ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["sequences"].toInt() });
+        const Strides s = strides_of(g);
+        d.o = saved[3].data_ptr();
+        d.lse = saved[4].data_ptr<float>();
+        d.o_rest = saved[8].data_ptr();
+        d.d_o = g.const_data_ptr();
+        d.do_row_stride = s.row; d.do_head_stride = s.head; d.do_batch_stride = s.batch;
+        Tensor made[3];
+        for (int i = 0; i < 3; i++) if (need[i]) made[i] = at::empty(saved[i].sizes(), saved[i].options().requires_grad(false));
+        const auto at_ = [](const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; };
+        d.dq = at_(made[0]);
+        d.dk = at_(made[1]);
+        d.dv = at_(made[2]);
+        const size_t size = ntc_op_attention_workspace(&d, 1);
+        const Tensor work = size ? bytes((int64_t)size, g) : Tensor();
+        d.workspace = at_(work);
+        call(g.device(), [&](void* s_, char* why, size_t cap) { return ntc_op_attention_backward(&d, s_, why, cap); });
+        for (int i = 0; i < 3; i++) out[i] = once(made[i], "attention");
+        return out;
+    }
+};
+
+Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, const optional<double>& scale_, const optional<Tensor>& cu_q, const optional<Tensor>& cu_k, const optional<Tensor>& k_lens) {
+    const auto check = [&](const char* name, const Tensor& t) {
+        on_gpu(name, t);
+        TORCH_CHECK_VALUE(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, name, " is ", t.scalar_type(), "; it can be bfloat16, float16");
+        no_tangent(name, t);
+        TORCH_CHECK_VALUE(t.dim() == 3 || t.dim() == 4, name, " ", t.sizes(), " must be [rows, heads, elements], or [sequences, rows, heads, elements]");
+        TORCH_CHECK_VALUE(t.device() == q.device() && t.scalar_type() == q.scalar_type(), name, " must have q's type, on its device");
+    };
+    check("q", q);
+    check("k", k);
+    check("v", v);
+    const int64_t D = q.size(-1), Hq = q.size(-2), Hk = k.size(-2);
+    TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(-1) == D, "k ", k.sizes(), " and v ", v.sizes(), " must have one shape, and heads as wide as q's ", D);
+    TORCH_CHECK_VALUE(D >= 8 && D <= 128 && D % 8 == 0, "a head has a multiple of 8 elements, up to 128, not ", D);
+    TORCH_CHECK_VALUE(Hk >= 1 && Hq >= 1 && Hq % Hk == 0 && Hq / Hk <= 1024 && Hq <= 65536, "q's ", Hq, " heads must be 1 to 1024 times the ", Hk, " of k and v, at most 65536");
+    const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)D);
+    TORCH_CHECK_VALUE((float)scale > 0 && scale < 1e30, "scale must be a number above 0, not ", scale);
+    int64_t sequences = -1;
+    const auto agree = [&](const char* name, int64_t n) {
+        TORCH_CHECK_VALUE(sequences < 0 || n == sequences, name, " is of ", n, " sequences, others of ", sequences);
+        sequences = n;
+    };
+    const auto ints = [&](const char* name, const Tensor& t) {
+        on_gpu(name, t);
+        TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == 1 && t.device() == q.device(), name, " must be a vector of int32 on q's device");
+        return t.contiguous();
+    };
+    const auto ends = [&](const char* name, const char* of, const Tensor& x, const optional<Tensor>& t) {
+        if (!t) { agree(of, x.dim() == 4 ? x.size(0) : 1); return Tensor(); }
+        TORCH_CHECK_VALUE(x.dim() == 3, name, " goes with ", of, " as [rows, heads, elements]");
+        const Tensor e = ints(name, *t);
+        TORCH_CHECK_VALUE(e.size(0) >= 1, name, " must hold a 0 and each sequence's end");
+        agree(name, e.size(0) - 1);
+        return e;
+    };
+    const Tensor eq = ends("cu_q", "q", q, cu_q), ek = ends("cu_k", "k", k, cu_k);
+    Tensor lens;
+    if (k_lens) {
+        lens = ints("k_lens", *k_lens);
+        agree("k_lens", lens.size(0));
+    }
+    if (!sequences && !eq.defined() && q.dim() == 4) TORCH_CHECK_VALUE(!ek.defined() || !k.numel(), "rows of k without a sequence");
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) return AttentionNode::apply(q, k, v, given_or_none(eq), given_or_none(ek), given_or_none(lens), causal, scale, sequences);
+    return attention_forward(readable(q), readable(k), readable(v), eq, ek, lens, { causal, scale, sequences }, {}, {});
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ops, m) {
@@ -546,6 +883,9 @@ PYBIND11_MODULE(_ops, m) {
     });
     m.def("linear", &linear);
     m.def("linear_fp8", &linear_fp8);
+    m.def("layer_norm", &layer_norm);
+    m.def("rotary", &rotary);
+    m.def("attention", &attention);
     m.def("adamw_moments", &adamw_moments);
     m.def("adamw_encode", &adamw_encode);
     py::class_<AdamwPlan>(m, "AdamwPlan")

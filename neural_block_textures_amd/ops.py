@@ -4,6 +4,9 @@
     AdamW(params, state_bits=32 or 8).step()  one step over many tensors
     fp8_quantize(x), fp8_matmul(a, b)         8-bit floating point with a power-of-two scale for each block of 128
     fp8_linear(x, w)                          a layer in it, for training or, with weights laid out once, for inference
+    layer_norm(x, weight, bias)               rows to mean 0 and variance 1; differentiable, weight and bias too
+    rotary(positions, q, k, sections=...)     rotary positions of several axes; differentiable
+    attention(q, k, v, cu_q=..., cu_k=...)    causal attention over packed sequences or a cache, grouped heads; differentiable
 
 Tensors are on the GPU; work is enqueued on torch's current stream and nothing waits. torch, or this module, has to be imported before
 libntc_hip.so is loaded (by the first Trainer), so that both use one HIP runtime; the other order raises. Arguments that an operator does not
@@ -48,6 +51,25 @@ class MatmulDesc(C.Structure):
                 ("ldc", _L), ("a_type", _I), ("a_block_rows", _I), ("b_block_rows", _I), ("c_type", _I)]
 
 
+class LayerNormDesc(C.Structure):
+    _fields_ = [("x", _P), ("weight", _P), ("bias", _P), ("y", _P), ("stats", _P), ("rows", _L), ("C", _L), ("x_stride", _L), ("dy_stride", _L), ("dtype", _I),
+                ("weight_type", _I), ("eps", C.c_float), ("dy", _P), ("dx", _P), ("dweight", _P), ("dbias", _P), ("workspace", _P)]
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [("positions", _P), ("position_stride", _L), ("tokens", _L), ("x", _P * 2), ("y", _P * 2), ("token_stride", _L * 2), ("head_stride", _L * 2),
+                ("heads", _I * 2), ("head_dim", _I), ("axes", _I), ("position_bytes", _I), ("dtype", _I), ("one_ladder", _I), ("interleaved", _I), ("backward", _I),
+                ("sections", _I * 8), ("base", C.c_double)]
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("o", _P), ("o_rest", _P), ("lse", _P), ("cu_q", _P), ("cu_k", _P), ("k_lens", _P), ("sequences", _L), ("q_rows", _L), ("k_rows", _L),
+                ("q_row_stride", _L), ("q_head_stride", _L), ("q_batch_stride", _L), ("k_row_stride", _L), ("k_head_stride", _L), ("k_batch_stride", _L),
+                ("v_row_stride", _L), ("v_head_stride", _L), ("v_batch_stride", _L), ("q_heads", _I), ("k_heads", _I), ("head_dim", _I), ("dtype", _I), ("causal", _I),
+                ("scale", C.c_float), ("workspace", _P), ("d_o", _P), ("do_row_stride", _L), ("do_head_stride", _L), ("do_batch_stride", _L), ("dq", _P), ("dk", _P),
+                ("dv", _P)]
+
+
 _TENSOR = np.dtype([("param", np.uint64), ("numel", np.int64), ("state_offset", np.int64), ("param_type", np.int32), ("first_chunk", np.int32)])
 _lib = _bound = None
 
@@ -69,6 +91,13 @@ def library() -> C.CDLL:
             "ntc_op_fp8_matmul_workspace": (C.c_size_t, [_L, _L, _L, _I]),
             "ntc_op_fp8_matmul": (C.c_int, [_P] + tail),
             "ntc_op_fp8_matmul_float_rows": (_L, []),
+            "ntc_op_layer_norm": (C.c_int, [_P] + tail),
+            "ntc_op_layer_norm_workspace": (C.c_size_t, [_L, _L]),
+            "ntc_op_layer_norm_backward": (C.c_int, [_P] + tail),
+            "ntc_op_rotary": (C.c_int, [_P] + tail),
+            "ntc_op_attention_workspace": (C.c_size_t, [_P, _I]),
+            "ntc_op_attention": (C.c_int, [_P] + tail),
+            "ntc_op_attention_backward": (C.c_int, [_P] + tail),
         }
         for name, (res, args) in sig.items():
             fn = getattr(lib, name)
@@ -291,3 +320,44 @@ def fp8_linear(x: torch.Tensor, w) -> torch.Tensor:
     if isinstance(w, Fp8Tensor):
         return _binding().linear_fp8(x, w.codes, w.exps, *w.shape, w.block_rows)
     return _binding().linear(x, w)
+
+
+# ---------------------------------------------------------------- the blocks of a sequence model
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean) / sqrt(variance + eps) * weight + bias over x's last axis, in x's type.
+
+    x [.., C]: float32, bfloat16 or float16 (copied first where a row's values are not contiguous or rows lie at several strides). weight and bias [C]:
+    of x's type or float32, both alike, or None. Differentiable (once) in all three. Statistics and sums are 32-bit, the weight's and bias's gradients over the rows too,
+    in an order that depends on the sizes alone; a row with a value that is not finite is NaN.
+    """
+    return _binding().layer_norm(x, weight, bias, eps)
+
+
+def rotary(positions: torch.Tensor, q: torch.Tensor, k: Optional[torch.Tensor] = None, *, sections, base: float = 10000.0, one_ladder: bool = False,
+           interleaved: bool = False):
+    """q, or (q, k), with pairs of each head's elements turned by angles that grow with the token's positions.
+
+    positions [.., axes]: int32 or int64, a token's place on each of 1 to 8 axes (time, row, column, channel). q and k [.., heads, elements]: float32, bfloat16 or float16, any
+    strides. sections: how many pairs of a head each axis turns, 128 in all at most; pair p of P is elements p and p + P, or with `interleaved` 2p and 2p + 1, and elements from 2 P on
+    stay as they are. Axis a's pair j turns by its position times base^(-j / sections[a]); with one_ladder pair p by its axis's position times base^(-p / P).
+    Angles keep the frequencies' 57 bits however far a position is; sines, cosines and sums are 32-bit, rounded once. Differentiable (once) in q and k.
+    """
+    out = _binding().rotary(positions, q, k, list(sections), base, one_ladder, interleaved)
+    return out[0] if k is None else out
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = True, scale: Optional[float] = None, cu_q: Optional[torch.Tensor] = None,
+              cu_k: Optional[torch.Tensor] = None, k_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale q k^T) v for each sequence and head, in q's type and shape. With `causal` query i of a sequence of Lq queries and Lk keys sees keys up to
+    i + Lk - Lq: the last query sees all of them. A query that sees none has 0, and no gradient.
+
+    q [sequences, rows, heads, elements], or packed [rows, heads, elements] with cu_q (int32 [sequences + 1] on the GPU: 0 and each sequence's end, ascending; without it one
+    sequence). k and v alike, with cu_k; their heads divide q's, and query head h reads key head h // (q's heads / k's). k_lens (int32 [sequences]): how many of its
+    rows of k and v a sequence has, as with a cache that has room; the rest are not read. Rows behind the last end have 0. scale: 1 / sqrt(elements) where it is None.
+
+    bfloat16 or float16, 8 to 128 elements a head (a multiple of 8), any strides (copied first where heads are not contiguous, or not at multiples of 16 bytes). Differentiable (once) in
+    q, k and v. Scores, the softmax and sums are 32-bit; probabilities, and backwards the scores' gradients, are rounded to the tensors' type for the products that
+    follow. Nothing is added by atomics: results repeat bit for bit. Lengths are read on the GPU: numbers that leave the tensors are cut off there, and give wrong results, not an error. A key or
+    value that is not finite makes the queries that see it NaN where the formula does, and possibly others of its sequence.
+    """
+    return _binding().attention(q, k, v, causal, scale, cu_q, cu_k, k_lens)
