@@ -56,6 +56,9 @@ struct AttentionArgs {
     int sequences, q_each, k_each;     // rows of a sequence where there are no ends
     int q_heads, k_heads, group, D, causal;
     unsigned group_magic;              // ceil(2^32 / group): x / group is the high word of the product with it where x group < 2^32; 0 for 1
+    int parts;                         // of a sequence's keys (backward: of its rows), joined by a second launch; their sums:
+    float* part_sums;                  // forward [parts][q_rows][q_heads][D]; backward dk's [parts][k_rows][k_heads][D], then dv's
+    float4* part_stats;                // forward [parts][q_rows][q_heads]: m c, both sums of probabilities
     int tiles, tiles_each;             // tiles of rows (or keys) in all, and of each sequence where there are no ends
     float scale, c;                    // c: scale log2 e
 };
@@ -186,6 +189,17 @@ template <class T, int kD, bool kRests = false> __device__ __forceinline__ void 
             if (live && col < D) *(v4u*)(p + 2 * col) = v4u{ (uint32_t)lo[0], (uint32_t)hi[0], (uint32_t)lo[1], (uint32_t)hi[1] };
         }
 }
+// ... as it is, in 32 bits
+template <int kD> __device__ __forceinline__ void store_floats(float* p, const v16f (&x)[kD / 32], bool live, int D) {
+    const int half = lane_id() >> 5;
+#pragma unroll
+    for (int t = 0; t < kD / 32; t++)
+#pragma unroll
+        for (int a = 0; a < 4; a++) {
+            const int col = 32 * t + 8 * a + 4 * half;
+            if (live && col < D) *(float4*)(p + col) = make_float4(x[t][4 * a], x[t][4 * a + 1], x[t][4 * a + 2], x[t][4 * a + 3]);
+        }
+}
 // result register r of the lane is row 8 (r / 4) + 4 half + r % 4
 __device__ __forceinline__ constexpr int result_row(int r) { return 8 * (r / 4) + r % 4; }
 template <class T> __device__ __forceinline__ v4u packed(const v16f& x, int half16) {
@@ -199,8 +213,8 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     constexpr int kTile = kKeys * L::kPitch;
     __shared__ alignas(1024) char lds[4 * kTile];          // keys, values; two of each
     const long long id = block_number();
-    const int head = (int)(id % d.k_heads);
-    const long long t_ = id / d.k_heads;
+    const int head = (int)(id % d.k_heads), part = (int)(id / d.k_heads % d.parts);
+    const long long t_ = id / d.k_heads / d.parts;
     if (t_ >= d.tiles) return;
     int tile;
     const int b = find_sequence<kRows>(d.cu_q, d.sequences, d.tiles_each, d.group, d.tiles - 1 - (int)t_, tile);   // (a sequence's last rows, which see most keys, first)
@@ -223,7 +237,8 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     const int i_wave = (r0 + 31) / d.group, i_block = (int)(((long long)tile * kRows + kRows - 1) / d.group);
     const int wave_last = d.causal ? (i_wave + off < Lk - 1 ? i_wave + off : Lk - 1) : Lk - 1;
     const int block_last = d.causal ? (i_block + off < Lk - 1 ? i_block + off : Lk - 1) : Lk - 1;
-    const int stages = block_last < 0 ? 0 : block_last / kKeys + 1;
+    const int all = block_last < 0 ? 0 : block_last / kKeys + 1;
+    const int begin = (int)((long long)all * part / d.parts), stages = (int)((long long)all * (part + 1) / d.parts);
 
     const char *kp = d.k.p + ks.start + head * d.k.head, *vp = d.v.p + v_start + head * d.v.head;
     const uint32_t lds0 = lds_address(lds);
@@ -236,8 +251,8 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     v16f o[kD / 32] = {};
     // Two sums of the probabilities: as rounded, by which the result is divided (what rounding adds to all values alike is then in both), and as they are, for lse.
     float m = -NTC_INF, l = 0, exact = 0;
-    if (stages) load(0);
-    for (int s = 0; s < stages; s++) {
+    if (begin < stages) load(begin);
+    for (int s = begin; s < stages; s++) {
         arrive();
         if (s + 1 < stages) load(s + 1);
         const int k0 = s * kKeys;
@@ -288,10 +303,57 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     l += other_half(l);
     exact += other_half(exact);
     const long long at = (qs.row + row.i) * d.q_heads + head * d.group + row.g;
+    if (d.parts > 1) {
+        const long long own = (long long)part * d.q_rows * d.q_heads + at;
+        store_floats<kD>(d.part_sums + own * d.D, o, live, d.D);
+        if (live && half == 0) d.part_stats[own] = make_float4(m * d.c, l, exact, 0.f);
+        return;
+    }
     const float f = l == 0 ? 0.f : 1.f / l;
     store_row<T, kD>((char*)d.out + at * d.D * 2, o, f, live, d.D);
     if (d.rest) store_row<T, kD, true>((char*)d.rest + at * d.D * 2, o, f, live, d.D);
     if (d.lse && live && half == 0) d.lse[at] = exact == 0 ? -NTC_INF : (m * d.c + fast_log2(exact)) * kLn2;
+}
+
+// The parts of a row, joined by a wave: a lane takes a part's statistics first, then eight columns of every 64 / kPieces-th part.
+template <class T, int kPieces> __global__ void __launch_bounds__(256) k_attention_join(AttentionArgs d) {
+    constexpr int kGroups = 64 / kPieces;
+    const int lane = lane_id(), piece = lane % kPieces, group = lane / kPieces, col = 8 * piece;
+    const long long rows = d.q_rows * d.q_heads, row = block_number() * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const float4 st = lane < d.parts ? d.part_stats[lane * rows + row] : make_float4(-NTC_INF, 0.f, 0.f, 0.f);
+    const auto larger = [](float a, float b) { return __builtin_fmaxf(a, b); };
+    const auto add = [](float a, float b) { return a + b; };
+    const float m = reduce64(st.x, larger), by = st.x == m ? 1.f : fast_exp2(st.x - m);                          // (no key at all: m is -inf, and what the part has is 0)
+    const float l = reduce64(st.y * by, add), exact = reduce64(st.z * by, add);
+    float sum[8] = {};
+#pragma unroll 4
+    for (int p0 = 0; p0 < d.parts; p0 += kGroups) {
+        const int p = p0 + group;
+        const float w = __shfl(by, p & 63);
+        if (p >= d.parts || col >= d.D) continue;
+        const float4 *of = (const float4*)(d.part_sums + (p * rows + row) * d.D + col), a = of[0], b = of[1];
+        const float v[8] = { a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w };
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum[i] = __builtin_fmaf(v[i], w, sum[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int g = kPieces; g < 64; g *= 2) sum[i] += __shfl_xor(sum[i], g);
+    if (group || col >= d.D) return;
+    const float f = l == 0 ? 0.f : 1.f / l;
+    uint32_t out[4], rest[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float y0 = sum[2 * i] * f, y1 = sum[2 * i + 1] * f;
+        out[i] = pack2<T>(y0, y1);
+        rest[i] = pack2<T>((y0 - (float)(T)y0) * kRest<T>, (y1 - (float)(T)y1) * kRest<T>);
+    }
+    const long long at = 2 * (row * d.D + col);
+    *(v4u*)((char*)d.out + at) = v4u{ out[0], out[1], out[2], out[3] };
+    if (d.rest) *(v4u*)((char*)d.rest + at) = v4u{ rest[0], rest[1], rest[2], rest[3] };
+    if (d.lse && col == 0) d.lse[row] = exact == 0 ? -NTC_INF : (m + fast_log2(exact)) * kLn2;
 }
 
 // ---------------------------------------------------------------- backward
@@ -468,13 +530,13 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     store_row<T, kD>((char*)d.dq + at * d.D * 2, dq, d.scale * two_to(-e), live && d.dq, d.D);
 }
 
-template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 2) k_attention_dkv(AttentionArgs d) {
+template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention_dkv(AttentionArgs d) {
     using L = Tile<kD>;
     constexpr int kStep = 64, kTile = kStep * L::kPitch, kStage = 2 * kTile + 8 * kStep;
     __shared__ alignas(1024) char lds[2 * kStage];         // queries, gradients, log sums and deltas of kStep rows; two of each
     const long long id = block_number();
-    const int head = (int)(id % d.k_heads);
-    const long long t_ = id / d.k_heads;
+    const int head = (int)(id % d.k_heads), part = (int)(id / d.k_heads % d.parts);
+    const long long t_ = id / d.k_heads / d.parts;
     if (t_ >= d.tiles) return;
     int tile;
     const int b = find_sequence<kRows>(d.cu_k, d.sequences, d.tiles_each, 1, (int)t_, tile);                      // (a sequence's first keys, which most queries see, first)
@@ -493,14 +555,15 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
     v4u k[kD / 16], v[kD / 16];
     load_row<kD>(k, d.k.p + ks.start + key * d.k.row + head * d.k.head, live, d.D);
     load_row<kD>(v, d.v.p + v_start + key * d.v.row + head * d.v.head, live, d.D);
-    const int e = gradient_exponent<T>(d);
+    const int e = qs.n ? gradient_exponent<T>(d) : 0;      // (without queries nothing has left it)
     const float up = two_to(e);
 
     // Row r sees key j where r >= (j - off) G: the lane's first row, the wave's first whole one, and where the block starts
     const int rows = qs.n * d.group;
     const auto first_row = [&](int j) { return d.causal && j > off ? (j - off) * d.group : 0; };
     const int lane_first = live ? first_row(key) : 1 << 30, wave_first = k0 + 31 < Lk ? first_row(k0 + 31) : 1 << 30, wave_start = first_row(k0);
-    const int stages = tile * kRows < Lk ? (rows + kStep - 1) / kStep : 0, start = stages ? first_row(tile * kRows) / kStep : 0;
+    const int end = tile * kRows < Lk ? (rows + kStep - 1) / kStep : 0, first = end ? first_row(tile * kRows) / kStep : 0, all = end > first ? end - first : 0;
+    const int start = first + (int)((long long)all * part / d.parts), stages = first + (int)((long long)all * (part + 1) / d.parts);
 
     const char *qp = d.q.p + qs.start + head * d.group * d.q.head, *gp = d.d_o.p + do_start + head * d.group * d.d_o.head;
     const long long at0 = qs.row * d.q_heads + head * d.group;
@@ -563,12 +626,41 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
         for (int t = 0; t < kD / 32; t++) { dk[t] = v16f{}; dv[t] = v16f{}; }
     }
     const long long at = (ks.row + key) * d.k_heads + head;
+    if (d.parts > 1) {
+        const long long each = d.k_rows * d.k_heads;
+        store_floats<kD>(d.part_sums + (part * each + at) * d.D, dk, held, d.D);
+        store_floats<kD>(d.part_sums + ((d.parts + part) * each + at) * d.D, dv, held, d.D);
+        return;
+    }
     store_row<T, kD>((char*)d.dk + at * d.D * 2, dk, d.scale * two_to(-e), held && d.dk, d.D);
     store_row<T, kD>((char*)d.dv + at * d.D * 2, dv, two_to(-kShift<T>), held && d.dv, d.D);
 }
 
+// The parts of dk (dv: second half of the grid) added up: eight columns to a thread.
+template <class T> __global__ void __launch_bounds__(256) k_attention_sum(AttentionArgs d) {
+    const long long n = d.k_rows * d.k_heads * d.D / 8, x = block_number() * 256 + threadIdx.x;
+    const float f = d.scale * two_to(-gradient_exponent<T>(d));
+    if (x >= 2 * n) return;
+    const int which = x >= n;
+    const long long at = 8 * (which ? x - n : x);
+    char* to = (char*)(which ? d.dv : d.dk);
+    if (!to) return;
+    float sum[8] = {};
+#pragma unroll 4
+    for (int p = 0; p < d.parts; p++) {
+        const float4 *of = (const float4*)(d.part_sums + 8 * n * (which * d.parts + p) + at), a = of[0], b = of[1];
+        const float v[8] = { a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w };
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum[i] += v[i];
+    }
+    uint32_t out[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) out[i] = pack2<T>(sum[2 * i] * (which ? two_to(-kShift<T>) : f), sum[2 * i + 1] * (which ? two_to(-kShift<T>) : f));
+    *(v4u*)(to + 2 * at) = v4u{ out[0], out[1], out[2], out[3] };
+}
+
 // ---------------------------------------------------------------- launches
-const char* wrong(const ntc_attention_desc* d, bool back) {
+const char* wrong_sizes(const ntc_attention_desc* d) {
     if (!d) return "no description";
     if (d->sequences < 0 || d->q_rows < 0 || d->k_rows < 0 || d->sequences >= 1 << 30) return "sequences and rows from 0 on are needed, fewer than 2^30 sequences";
     if (d->dtype != NTC_BF16 && d->dtype != NTC_F16) return "queries, keys and values are bfloat16 or float16";
@@ -579,6 +671,10 @@ const char* wrong(const ntc_attention_desc* d, bool back) {
     if (!d->cu_q && d->sequences && d->q_rows % d->sequences) return "without ends every sequence has as many queries";
     if (!d->cu_k && d->sequences && d->k_rows % d->sequences) return "without ends every sequence has as many keys";
     if (!d->sequences && ((d->q_rows && !d->cu_q) || (d->k_rows && !d->cu_k))) return "rows without a sequence";
+    return nullptr;
+}
+const char* wrong(const ntc_attention_desc* d, bool back) {
+    if (const char* w = wrong_sizes(d)) return w;
     const int64_t* s = &d->q_row_stride;
     for (int i = 0; i < 9; i++) if (s[i] < 0 || s[i] % 8 || (i % 3 == 0 && s[i] > 1 << 22) || (i % 3 == 1 && s[i] > 1 << 20)) return "strides are multiples of 8 elements from 0 on, of rows at most 2^22, of heads 2^20";
     if (back) {
@@ -607,6 +703,7 @@ AttentionArgs args_of(const ntc_attention_desc* d) {
     a.k_each = d->sequences ? (int)(d->k_rows / d->sequences) : 0;
     a.q_heads = d->q_heads; a.k_heads = d->k_heads; a.group = d->q_heads / d->k_heads; a.D = d->head_dim; a.causal = d->causal != 0;
     a.group_magic = a.group > 1 ? (unsigned)((((uint64_t)1 << 32) + a.group - 1) / a.group) : 0;
+    a.parts = 1;
     a.scale = d->scale;
     a.c = d->scale * kLog2e;
     return a;
@@ -616,6 +713,8 @@ void set_tiles(AttentionArgs& a, bool ends, int64_t each, int64_t rows, int64_t 
     a.tiles_each = (int)((each + size - 1) / size);
     a.tiles = (int)(ends ? rows / size + a.sequences + 1 : (int64_t)a.tiles_each * a.sequences);
 }
+void set_row_tiles(AttentionArgs& a) { set_tiles(a, a.cu_q, (int64_t)a.q_each * a.group, a.q_rows * a.group, kRows); }
+void set_key_tiles(AttentionArgs& a) { set_tiles(a, a.cu_k, a.k_each, a.k_rows, kRows); }
 template <class F> void with_head(int dtype, int D, F f) {
     const auto go = [&](auto t) {
         if (D <= 32) f(t, std::integral_constant<int, 32>{});
@@ -628,6 +727,28 @@ template <class F> void with_head(int dtype, int D, F f) {
 }
 size_t rounded(size_t n) { return (n + 15) / 16 * 16; }
 
+// Parts of a sum. Without parts the longest sum holds the card up where tiles are few; with them their 32-bit results are written and read once more. In us: `each` a stage,
+// two blocks to a compute unit at a time, stages of all blocks (half of them where causal and long on both sides) spread over these and then the longest block's own; 5 for the second launch, 4 TB/s for what the parts write and read.
+int parts_of(int64_t blocks, int64_t stages, float each, bool half, int64_t part_bytes) {
+    int best = 1;
+    float least = 0;
+    for (int p = 1; p <= 64 && p <= stages; p *= 2) {
+        const float busy = (float)blocks * stages / 512 * (half ? 0.5f : 1.f), longest = (float)((stages + p - 1) / p);
+        const float cost = each * (busy > longest ? busy + 0.5f * longest : longest + 0.5f * busy) + (p > 1 ? 5.f + 2.f * p * part_bytes / 4e6f : 0.f);
+        if (p == 1 || cost < least) { best = p; least = cost; }
+    }
+    return best;
+}
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int forward_parts(const AttentionArgs& a) {
+    const int64_t keys = a.sequences ? ceil_div(a.k_rows, a.sequences) : 0, queries = a.sequences ? a.q_rows / a.sequences : 0;
+    return parts_of((int64_t)a.tiles * a.k_heads, ceil_div(keys, kKeys), 0.4f + 0.006f * a.D, a.causal && 2 * queries > keys, a.q_rows * a.q_heads * a.D * 4);
+}
+int backward_parts(const AttentionArgs& a) {
+    const int64_t keys = a.sequences ? ceil_div(a.k_rows, a.sequences) : 0, queries = a.sequences ? a.q_rows / a.sequences : 0;
+    return parts_of((int64_t)a.tiles * a.k_heads, ceil_div(queries * a.group, 64), 0.5f + 0.015f * a.D, a.causal && 2 * keys > queries, a.k_rows * a.k_heads * a.D * 8);
+}
+
 }  // namespace
 }  // namespace ntc_ops
 
@@ -636,17 +757,40 @@ using namespace ntc_ops;
 extern "C" {
 
 size_t ntc_op_attention_workspace(const ntc_attention_desc* d, int32_t backward) {
-    if (!d || !backward || d->q_rows < 1) return 0;
-    return rounded((size_t)d->q_rows * d->q_heads * 4) + 2 * kExtents * 4;
+    if (wrong_sizes(d)) return 0;
+    AttentionArgs a = args_of(d);
+    if (!backward) {
+        if (!d->q_rows) return 0;
+        set_row_tiles(a);
+        const int parts = forward_parts(a);
+        return parts > 1 ? (size_t)parts * d->q_rows * d->q_heads * (16 + 4 * (size_t)d->head_dim) : 0;
+    }
+    size_t n = d->q_rows ? rounded((size_t)d->q_rows * d->q_heads * 4) + 2 * kExtents * 4 : 0;
+    if (d->k_rows) {
+        set_key_tiles(a);
+        const int parts = backward_parts(a);
+        if (parts > 1) n += (size_t)parts * d->k_rows * d->k_heads * d->head_dim * 8;
+    }
+    return n;
 }
 
 int ntc_op_attention(const ntc_attention_desc* d, void* stream, char* why, size_t cap) {
     if (const char* w = wrong(d, false)) return refuse(why, cap, w);
     if (!d->q_rows) return 0;
     AttentionArgs a = args_of(d);
-    set_tiles(a, d->cu_q, (int64_t)a.q_each * a.group, a.q_rows * a.group, kRows);
-    const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads);
-    with_head(d->dtype, d->head_dim, [&](auto t, auto h) { k_attention<decltype(t), h.value><<<grid, 256, 0, (hipStream_t)stream>>>(a); });
+    const hipStream_t s = (hipStream_t)stream;
+    set_row_tiles(a);
+    a.parts = forward_parts(a);
+    if (a.parts > 1) {
+        if (!d->workspace) return refuse(why, cap, "null workspace");
+        a.part_stats = (float4*)d->workspace;
+        a.part_sums = (float*)(a.part_stats + (size_t)a.parts * d->q_rows * d->q_heads);
+    }
+    const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads * a.parts);
+    with_head(d->dtype, d->head_dim, [&](auto t, auto h) {
+        k_attention<decltype(t), h.value><<<grid, 256, 0, s>>>(a);
+        if (a.parts > 1) k_attention_join<decltype(t), h.value == 96 ? 16 : h.value / 8><<<grid_of(ceil_div(d->q_rows * d->q_heads, 4)), 256, 0, s>>>(a);
+    });
     return launched(why, cap);
 }
 
@@ -656,20 +800,25 @@ int ntc_op_attention_backward(const ntc_attention_desc* d, void* stream, char* w
     AttentionArgs a = args_of(d);
     a.delta = (float*)d->workspace;
     a.extent = (float*)((char*)d->workspace + rounded((size_t)d->q_rows * d->q_heads * 4));
+    a.part_sums = d->q_rows ? a.extent + 2 * kExtents : (float*)d->workspace;
     if (d->q_rows) {
         if (d->dtype == NTC_F16) {
-            set_tiles(a, d->cu_k, a.k_each, a.k_rows, kRows);
+            set_key_tiles(a);
             k_attention_extent<f16><<<kExtents, 256, 0, s>>>(a);
         }
-        set_tiles(a, d->cu_q, (int64_t)a.q_each * a.group, a.q_rows * a.group, kRows);
+        set_row_tiles(a);
         const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads);
         with_head(d->dtype, d->head_dim, [&](auto t, auto h) { k_attention_dq<decltype(t), h.value><<<grid, 256, 0, s>>>(a); });
         if (const int rc = launched(why, cap)) return rc;
     }
     if (!d->k_rows || (!d->dk && !d->dv)) return 0;
-    set_tiles(a, d->cu_k, a.k_each, a.k_rows, kRows);
-    const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads);
-    with_head(d->dtype, d->head_dim, [&](auto t, auto h) { k_attention_dkv<decltype(t), h.value><<<grid, 256, 0, s>>>(a); });
+    set_key_tiles(a);
+    a.parts = d->q_rows ? backward_parts(a) : 1;
+    const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads * a.parts);
+    with_head(d->dtype, d->head_dim, [&](auto t, auto h) {
+        k_attention_dkv<decltype(t), h.value><<<grid, 256, 0, s>>>(a);
+        if (a.parts > 1) k_attention_sum<decltype(t)><<<grid_of(ceil_div(d->k_rows * d->k_heads * (d->head_dim / 4), 256)), 256, 0, s>>>(a);
+    });
     return launched(why, cap);
 }
 

@@ -2,7 +2,7 @@
 //
 // With mu and s the mean and 1 / sqrt(variance + eps) of a row, h = (x - mu) s and y = h w + b; backwards, with t = g w,
 //   dx = s (t - mean t - h mean(t h)),   dw = sum over rows of g h,   db = sum over rows of g.
-// A row is read once and kept in registers: 8 to 64 lanes of a wave, four waves or sixteen to a row, 8 to 32 values a lane. The variance is
+// A row is read once and kept in registers: 8 to 64 lanes of a wave, or two to sixteen waves to a row, 8 or 16 values a lane, the next row on its way meanwhile. The variance is
 // taken on differences from the mean, in a second pass over the registers. Backwards a block walks through many rows and adds up its
 // columns' dw and db on the way; a second, small launch adds the blocks' sums, in order, so that results repeat bit for bit.
 //
@@ -22,18 +22,43 @@ struct NormArgs {
     float eps;
 };
 
-template <class T> __device__ __forceinline__ float weight_at(const void* w, int f32, int c) { return f32 ? ((const float*)w)[c] : (float)((const T*)w)[c]; }
-
-// kN values from p on, those past the first n as 0
-template <class T, int kN> __device__ __forceinline__ void load_values(const T* p, int n, float* v) {
-    if (n >= kN) {
-        const auto r = *(const LooseRun<T, kN>*)p;
+// 16 bytes of a row, as they lie
+struct Words { uint32_t w[4]; };
+template <class T> constexpr int kRunOf = 16 / (int)sizeof(T);
+template <class T> __device__ __forceinline__ float value(const Words& x, int i) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(x.w[i]);
+    else if constexpr (std::is_same_v<T, bf16>) return __uint_as_float(i & 1 ? x.w[i / 2] & 0xffff0000u : x.w[i / 2] << 16);
+    else return (float)__builtin_bit_cast(T, (uint16_t)(x.w[i / 2] >> 16 * (i & 1)));
+}
+// The values from p on, of which n are the row's. `past`: what follows the row may be read as well (another row does); values past n are any then, else 0.
+template <class T> __device__ __forceinline__ Words load_run(const T* p, int n, bool past) {
+    constexpr int kN = kRunOf<T>;
+    if (n >= kN || (past && n > 0)) return __builtin_bit_cast(Words, *(const LooseRun<T, kN>*)p);
+    Words r = {};
 #pragma unroll
-        for (int i = 0; i < kN; i++) v[i] = (float)r.v[i];
-    } else {
+    for (int i = 0; i < kN; i++)
+        if (i < n) {
+            if constexpr (sizeof(T) == 4) r.w[i] = __float_as_uint(p[i]);
+            else r.w[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[i]) << 16 * (i & 1);
+        }
+    return r;
+}
+// kN values of a weight's type W (32-bit ones in two runs where the row's are 16-bit)
+template <class W, int kN> __device__ __forceinline__ void load_values(const W* p, int n, float* v) {
 #pragma unroll
-        for (int i = 0; i < kN; i++) v[i] = i < n ? (float)p[i] : 0.f;
+    for (int k = 0; k < kN; k += kRunOf<W>) {
+        const Words r = load_run<W>(p + k, n - k, false);
+#pragma unroll
+        for (int i = 0; i < kRunOf<W>; i++) v[k + i] = value<W>(r, i);
     }
+}
+// (weights and biases: null stands for `none`)
+template <class T, int kN> __device__ __forceinline__ void load_weights(const void* w, int f32_, int c, int C, float none, float* v) {
+    if (!w) {
+#pragma unroll
+        for (int i = 0; i < kN; i++) v[i] = none;
+    } else if (f32_) load_values<float, kN>((const float*)w + c, C - c, v);
+    else load_values<T, kN>((const T*)w + c, C - c, v);
 }
 template <class T, int kN> __device__ __forceinline__ void store_values(T* p, int n, const float* v) {
     if (n >= kN) {
@@ -62,7 +87,7 @@ template <int kLanes, int kWaves> __device__ __forceinline__ float row_sum(float
 
 // kLanes lanes of a wave (kWaves = 1) or kWaves whole waves to a row, kValues values a lane in runs of 16 bytes.
 template <class T, int kLanes, int kWaves, int kValues> struct Shape {
-    static constexpr int kRun = 16 / (int)sizeof(T), kRuns = kValues / kRun, kThreads = kWaves > 1 ? 64 * kWaves : 256, kGroup = kLanes * kWaves, kGroups = kThreads / kGroup;
+    static constexpr int kRun = kRunOf<T>, kRuns = kValues / kRun, kThreads = kWaves > 1 ? 64 * kWaves : 256, kGroup = kLanes * kWaves, kGroups = kThreads / kGroup;
     static __device__ __forceinline__ int column(int run) { return (run * kGroup + (int)threadIdx.x % kGroup) * kRun; }
 };
 
@@ -72,24 +97,31 @@ template <class T, int kLanes, int kWaves, int kValues> __global__ void __launch
     __shared__ float sums[2][kWaves];
     float w[kValues], b[kValues];
 #pragma unroll
-    for (int r = 0; r < kRuns; r++)
-#pragma unroll
-        for (int i = 0; i < kRun; i++) {
-            const int c = S::column(r) + i;
-            w[r * kRun + i] = d.w && c < d.C ? weight_at<T>(d.w, d.w_f32, c) : 1.f;
-            b[r * kRun + i] = d.b && c < d.C ? weight_at<T>(d.b, d.w_f32, c) : 0.f;
-        }
+    for (int r = 0; r < kRuns; r++) {
+        load_weights<T, kRun>(d.w, d.w_f32, S::column(r), d.C, 1.f, w + r * kRun);
+        load_weights<T, kRun>(d.b, d.w_f32, S::column(r), d.C, 0.f, b + r * kRun);
+    }
     const float inv = 1.f / (float)d.C;
-    const long long step = (long long)gridDim.x * S::kGroups;
-    for (long long first = (long long)blockIdx.x * S::kGroups; first < d.rows; first += step) {
-        const long long row = first + threadIdx.x / S::kGroup;
+    const long long step = (long long)gridDim.x * S::kGroups, own = (long long)blockIdx.x * S::kGroups + threadIdx.x / S::kGroup;
+    const bool apart = d.x_stride >= d.C;
+    Words next[kRuns];                                     // of the row after this one, on its way meanwhile
+    const auto load = [&](long long row) {
+        const T* x = (const T*)d.x + row * d.x_stride;
+#pragma unroll
+        for (int r = 0; r < kRuns; r++) next[r] = load_run<T>(x + S::column(r), row < d.rows ? d.C - S::column(r) : 0, apart && row + 1 < d.rows);
+    };
+    load(own);
+    for (long long first = (long long)blockIdx.x * S::kGroups, row = own; first < d.rows; first += step, row += step) {
         const bool live = row < d.rows;
-        const T* x = (const T*)d.x + (live ? row : first) * d.x_stride;
         float v[kValues], sum = 0, square = 0;
 #pragma unroll
-        for (int r = 0; r < kRuns; r++) load_values<T, kRun>(x + S::column(r), d.C - S::column(r), v + r * kRun);
+        for (int r = 0; r < kRuns; r++)
 #pragma unroll
-        for (int i = 0; i < kValues; i++) sum += v[i];
+            for (int i = 0; i < kRun; i++) {
+                v[r * kRun + i] = S::column(r) + i < d.C ? value<T>(next[r], i) : 0.f;
+                sum += v[r * kRun + i];
+            }
+        if (first + step < d.rows) load(row + step);
         const float mean = row_sum<kLanes, kWaves>(sum, sums[0]) * inv;
 #pragma unroll
         for (int r = 0; r < kRuns; r++)
@@ -121,40 +153,47 @@ template <class T, int kLanes, int kWaves, int kValues> __global__ void __launch
     __shared__ float joined[S::kGroups > 1 ? S::kGroups * S::kGroup * kValues : 1];
     float w[kValues], dw[kValues] = {}, db[kValues] = {};
 #pragma unroll
-    for (int r = 0; r < kRuns; r++)
-#pragma unroll
-        for (int i = 0; i < kRun; i++) {
-            const int c = S::column(r) + i;
-            w[r * kRun + i] = d.w && c < d.C ? weight_at<T>(d.w, d.w_f32, c) : 1.f;
-        }
+    for (int r = 0; r < kRuns; r++) load_weights<T, kRun>(d.w, d.w_f32, S::column(r), d.C, 1.f, w + r * kRun);
     const float inv = 1.f / (float)d.C;
-    const long long step = (long long)gridDim.x * S::kGroups;
-    int turn = 0;
-    for (long long first = (long long)blockIdx.x * S::kGroups; first < d.rows; first += step, turn ^= 2) {
-        const long long row = first + threadIdx.x / S::kGroup;
-        const bool live = row < d.rows;
-        const long long at = live ? row : first;
-        const T *x = (const T*)d.x + at * d.x_stride, *dy = (const T*)d.dy + at * d.dy_stride;
-        const float2 st = *(const float2*)(d.stats + 2 * at);
-        float h[kValues], g[kValues], a = 0, c = 0;
+    const long long step = (long long)gridDim.x * S::kGroups, own = (long long)blockIdx.x * S::kGroups + threadIdx.x / S::kGroup;
+    const bool apart = d.x_stride >= d.C && d.dy_stride >= d.C;
+    Words next_x[kRuns], next_g[kRuns];
+    float2 next_st;
+    const auto load = [&](long long row) {
+        const T *x = (const T*)d.x + row * d.x_stride, *dy = (const T*)d.dy + row * d.dy_stride;
 #pragma unroll
         for (int r = 0; r < kRuns; r++) {
-            const int n = live ? d.C - S::column(r) : 0;
-            load_values<T, kRun>(x + S::column(r), n, h + r * kRun);
-            load_values<T, kRun>(dy + S::column(r), n, g + r * kRun);
+            const int n = row < d.rows ? d.C - S::column(r) : 0;
+            const bool past = apart && row + 1 < d.rows;
+            next_x[r] = load_run<T>(x + S::column(r), n, past);
+            next_g[r] = load_run<T>(dy + S::column(r), n, past);
         }
+        next_st = row < d.rows ? *(const float2*)(d.stats + 2 * row) : make_float2(0.f, 0.f);
+    };
+    load(own);
+    int turn = 0;
+    for (long long first = (long long)blockIdx.x * S::kGroups, row = own; first < d.rows; first += step, row += step, turn ^= 2) {
+        const bool live = row < d.rows;
+        const float2 st = next_st;
+        float h[kValues], g[kValues], a = 0, c = 0;
 #pragma unroll
         for (int r = 0; r < kRuns; r++)
 #pragma unroll
             for (int i = 0; i < kRun; i++) {
                 const int k = r * kRun + i;
-                h[k] = live && S::column(r) + i < d.C ? (h[k] - st.x) * st.y : 0.f;
-                dw[k] = __builtin_fmaf(g[k], h[k], dw[k]);
-                db[k] += g[k];
-                g[k] *= w[k];
-                a += g[k];
-                c = __builtin_fmaf(g[k], h[k], c);
+                const bool in = live && S::column(r) + i < d.C;
+                h[k] = in ? (value<T>(next_x[r], i) - st.x) * st.y : 0.f;
+                g[k] = in ? value<T>(next_g[r], i) : 0.f;
             }
+        if (first + step < d.rows) load(row + step);
+#pragma unroll
+        for (int k = 0; k < kValues; k++) {
+            dw[k] = __builtin_fmaf(g[k], h[k], dw[k]);
+            db[k] += g[k];
+            g[k] *= w[k];
+            a += g[k];
+            c = __builtin_fmaf(g[k], h[k], c);
+        }
         if (!d.dx) continue;
         a = row_sum<kLanes, kWaves>(a, sums[turn]) * inv;
         c = row_sum<kLanes, kWaves>(c, sums[turn + 1]) * inv;
@@ -202,40 +241,73 @@ template <class T, int kLanes, int kWaves, int kValues> __global__ void __launch
 // Rows that no block holds: read three times (backward: twice), the later times from the caches.
 constexpr int kWide = 1024;
 __device__ __forceinline__ float block_sum(float x, float* at) { return row_sum<64, kWide / 64>(x, at); }
+template <class T, class F> __device__ __forceinline__ void for_runs(int C, F f) {       // f(first column of a run, its columns)
+    for (int c = threadIdx.x * kRunOf<T>; c < C; c += kWide * kRunOf<T>) f(c, C - c);
+}
 template <class T> __global__ void __launch_bounds__(kWide) k_norm_wide(NormArgs d) {
     __shared__ float sums[2][kWide / 64];
+    constexpr int kRun = kRunOf<T>;
     const float inv = 1.f / (float)d.C;
     for (long long row = blockIdx.x; row < d.rows; row += gridDim.x) {
         const T* x = (const T*)d.x + row * d.x_stride;
         float sum = 0, square = 0;
-        for (int c = threadIdx.x; c < d.C; c += kWide) sum += (float)x[c];
+        for_runs<T>(d.C, [&](int c, int n) {
+            const Words r = load_run<T>(x + c, n, false);
+#pragma unroll
+            for (int i = 0; i < kRun; i++) sum += value<T>(r, i);
+        });
         const float mean = block_sum(sum, sums[0]) * inv;
-        for (int c = threadIdx.x; c < d.C; c += kWide) { const float z = (float)x[c] - mean; square = __builtin_fmaf(z, z, square); }
+        for_runs<T>(d.C, [&](int c, int n) {
+            const Words r = load_run<T>(x + c, n, false);
+#pragma unroll
+            for (int i = 0; i < kRun; i++) { const float z = i < n ? value<T>(r, i) - mean : 0.f; square = __builtin_fmaf(z, z, square); }
+        });
         const float s = 1.f / __builtin_sqrtf(block_sum(square, sums[1]) * inv + d.eps);
-        for (int c = threadIdx.x; c < d.C; c += kWide)
-            ((T*)d.y)[row * d.C + c] = (T)__builtin_fmaf(((float)x[c] - mean) * s, d.w ? weight_at<T>(d.w, d.w_f32, c) : 1.f, d.b ? weight_at<T>(d.b, d.w_f32, c) : 0.f);
+        for_runs<T>(d.C, [&](int c, int n) {
+            const Words r = load_run<T>(x + c, n, false);
+            float w[kRun], b[kRun], o[kRun];
+            load_weights<T, kRun>(d.w, d.w_f32, c, d.C, 1.f, w);
+            load_weights<T, kRun>(d.b, d.w_f32, c, d.C, 0.f, b);
+#pragma unroll
+            for (int i = 0; i < kRun; i++) o[i] = __builtin_fmaf((value<T>(r, i) - mean) * s, w[i], b[i]);
+            store_values<T, kRun>((T*)d.y + row * d.C + c, n, o);
+        });
         if (d.stats && threadIdx.x == 0) *(float2*)(d.stats + 2 * row) = make_float2(mean, s);
     }
 }
 template <class T> __global__ void __launch_bounds__(kWide) k_norm_wide_back(NormArgs d) {
     __shared__ float sums[4][kWide / 64];
+    constexpr int kRun = kRunOf<T>;
     const float inv = 1.f / (float)d.C;
     int turn = 0;
     for (long long row = blockIdx.x; row < d.rows; row += gridDim.x, turn ^= 2) {
         const T *x = (const T*)d.x + row * d.x_stride, *dy = (const T*)d.dy + row * d.dy_stride;
         const float2 st = *(const float2*)(d.stats + 2 * row);
+        const auto run = [&](int c, int n, float* t, float* h) {
+            const Words rx = load_run<T>(x + c, n, false), rg = load_run<T>(dy + c, n, false);
+            load_weights<T, kRun>(d.w, d.w_f32, c, d.C, 1.f, t);
+#pragma unroll
+            for (int i = 0; i < kRun; i++) {
+                t[i] = i < n ? t[i] * value<T>(rg, i) : 0.f;
+                h[i] = i < n ? (value<T>(rx, i) - st.x) * st.y : 0.f;
+            }
+        };
         float a = 0, b = 0;
-        for (int c = threadIdx.x; c < d.C; c += kWide) {
-            const float t = (float)dy[c] * (d.w ? weight_at<T>(d.w, d.w_f32, c) : 1.f);
-            a += t;
-            b = __builtin_fmaf(t, ((float)x[c] - st.x) * st.y, b);
-        }
+        for_runs<T>(d.C, [&](int c, int n) {
+            float t[kRun], h[kRun];
+            run(c, n, t, h);
+#pragma unroll
+            for (int i = 0; i < kRun; i++) { a += t[i]; b = __builtin_fmaf(t[i], h[i], b); }
+        });
         a = block_sum(a, sums[turn]) * inv;
         b = block_sum(b, sums[turn + 1]) * inv;
-        for (int c = threadIdx.x; c < d.C; c += kWide) {
-            const float t = (float)dy[c] * (d.w ? weight_at<T>(d.w, d.w_f32, c) : 1.f);
-            ((T*)d.dx)[row * d.C + c] = (T)(st.y * (t - a - ((float)x[c] - st.x) * st.y * b));
-        }
+        for_runs<T>(d.C, [&](int c, int n) {
+            float t[kRun], h[kRun];
+            run(c, n, t, h);
+#pragma unroll
+            for (int i = 0; i < kRun; i++) t[i] = st.y * (t[i] - a - h[i] * b);
+            store_values<T, kRun>((T*)d.dx + row * d.C + c, n, t);
+        });
     }
 }
 // ... and their columns' sums: 256 columns and a run of rows to a block.
@@ -259,6 +331,7 @@ template <class W> __global__ void __launch_bounds__(1024) k_norm_join(const flo
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
     float sum = 0;
     if (c < 2 * C)
+#pragma unroll 8
         for (int p = k; p < blocks; p += 32) sum += parts[(long long)p * 2 * C + c];
     part[k][threadIdx.x & 31] = sum;
     __syncthreads();
@@ -279,19 +352,21 @@ Plan plan_of(int64_t C) {
     if (C <= 256) return { 32, 1, 8 };
     if (C <= 512) return { 64, 1, 8 };
     if (C <= 1024) return { 64, 1, 16 };
-    if (C <= 2048) return { 64, 1, 32 };
+    if (C <= 2048) return { 64, 2, 16 };
     if (C <= 4096) return { 64, 4, 16 };
-    if (C <= 8192) return { 64, 4, 32 };
+    if (C <= 8192) return { 64, 8, 16 };
     if (C <= 16384) return { 64, 16, 16 };
-    if (C <= 32768) return { 64, 16, 32 };
     return { 0, 0, 0 };
 }
+// (Backwards a lane also keeps its columns' sums: sixteen waves' registers do not hold sixteen values.)
+Plan back_plan_of(int64_t C) { return C <= 8192 ? plan_of(C) : Plan{ 0, 0, 0 }; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t groups_of(const Plan& p) { return p.waves > 1 ? 1 : 256 / p.lanes; }
 template <class T, class F> void with_shape(const Plan& p, F f) {
     const auto go = [&](auto l, auto w, auto v) { f(Shape<T, l.value, w.value, v.value>{}, l, w, v); };
 #define NTC_SHAPE(L, W, V) if (p.lanes == L && p.waves == W && p.values == V) return go(std::integral_constant<int, L>{}, std::integral_constant<int, W>{}, std::integral_constant<int, V>{})
-    NTC_SHAPE(8, 1, 8); NTC_SHAPE(16, 1, 8); NTC_SHAPE(32, 1, 8); NTC_SHAPE(64, 1, 8); NTC_SHAPE(64, 1, 16); NTC_SHAPE(64, 1, 32);
-    NTC_SHAPE(64, 4, 16); NTC_SHAPE(64, 4, 32); NTC_SHAPE(64, 16, 16); NTC_SHAPE(64, 16, 32);
+    NTC_SHAPE(8, 1, 8); NTC_SHAPE(16, 1, 8); NTC_SHAPE(32, 1, 8); NTC_SHAPE(64, 1, 8); NTC_SHAPE(64, 1, 16);
+    NTC_SHAPE(64, 2, 16); NTC_SHAPE(64, 4, 16); NTC_SHAPE(64, 8, 16); NTC_SHAPE(64, 16, 16);
 #undef NTC_SHAPE
 }
 template <class F> void with_type(int t, F f) {
@@ -301,9 +376,9 @@ template <class F> void with_type(int t, F f) {
 }
 // Blocks that walk through the rows backwards, each with sums of its own.
 int64_t back_blocks(int64_t rows, int64_t C) {
-    const Plan p = plan_of(C);
+    const Plan p = back_plan_of(C);
     if (!p.lanes) return rows < 64 ? rows : 64;
-    const int64_t n = (rows + groups_of(p) - 1) / groups_of(p), most = p.waves > 4 ? 256 : p.waves > 1 ? 512 : 1024;
+    const int64_t n = ceil_div(rows, groups_of(p)), most = p.waves > 4 ? 256 : p.waves > 2 ? 512 : 1024;
     return n < most ? n : most;
 }
 
@@ -344,8 +419,8 @@ int ntc_op_layer_norm(const ntc_layer_norm_desc* d, void* stream, char* why, siz
     const hipStream_t s = (hipStream_t)stream;
     with_type(d->dtype, [&](auto t) {
         using T = decltype(t);
-        const int64_t n = p.lanes ? (a.rows + groups_of(p) - 1) / groups_of(p) : a.rows;
-        const unsigned grid = (unsigned)(n < 4096 ? n : 4096);
+        const int64_t n = p.lanes ? ceil_div(a.rows, groups_of(p)) : a.rows;
+        const unsigned grid = (unsigned)ceil_div(n, ceil_div(n, p.waves > 4 ? 1024 : 3072));     // as many as the card holds at once, each with as many rows
         if (!p.lanes) k_norm_wide<T><<<grid, kWide, 0, s>>>(a);
         else with_shape<T>(p, [&](auto shape, auto l, auto w, auto v) { k_norm<T, l.value, w.value, v.value><<<grid, decltype(shape)::kThreads, 0, s>>>(a); });
     });
@@ -362,11 +437,13 @@ int ntc_op_layer_norm_backward(const ntc_layer_norm_desc* d, void* stream, char*
     const int64_t blocks = back_blocks(d->rows, d->C);
     if (sums) a.parts = (float*)d->workspace;
     if (d->rows && (sums || d->dx)) {
-        const Plan p = plan_of(d->C);
+        const Plan p = back_plan_of(d->C);
         with_type(d->dtype, [&](auto t) {
             using T = decltype(t);
             if (p.lanes) {
-                with_shape<T>(p, [&](auto shape, auto l, auto w, auto v) { k_norm_back<T, l.value, w.value, v.value><<<(unsigned)blocks, decltype(shape)::kThreads, 0, s>>>(a); });
+                with_shape<T>(p, [&](auto shape, auto l, auto w, auto v) {
+                    if constexpr (w.value < 16) k_norm_back<T, l.value, w.value, v.value><<<(unsigned)blocks, decltype(shape)::kThreads, 0, s>>>(a);
+                });
             } else {
                 if (a.dx) k_norm_wide_back<T><<<(unsigned)(a.rows < 4096 ? a.rows : 4096), kWide, 0, s>>>(a);
                 if (sums) k_norm_wide_columns<T><<<dim3((unsigned)((a.C + 255) / 256), (unsigned)blocks), 256, 0, s>>>(a);

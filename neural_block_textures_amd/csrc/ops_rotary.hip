@@ -6,8 +6,8 @@
 // for: the angle is off by no more than the frequency is, 2^-57 of it. Its quarters of a turn are its top bits, and sine and cosine come from their
 // power series on the rest, to 2^-23.
 //
-// A thread takes a token's run of pairs, makes their sines and cosines once, and turns that run in several heads of queries and
-// keys. Bound by memory: every value is read and written once.
+// A block takes a few tokens: their sines and cosines are made once, into shared memory, and serve all heads of queries and keys, whose elements
+// are then read and written in the order in which they lie. Bound by memory: every value is read and written once.
 #include <math.h>
 
 #include "ops_common.hpp"
@@ -15,7 +15,7 @@
 namespace ntc_ops {
 namespace {
 
-constexpr int kMostPairs = 128, kMostAxes = 8;
+constexpr int kMostPairs = 128, kMostAxes = 8, kTable = 1024;
 
 struct RotaryArgs {
     const void* positions;
@@ -25,10 +25,11 @@ struct RotaryArgs {
     long long token_stride[2], head_stride[2];
     int heads[2];
     int head_dim, pairs, backward;
-    int units, turned_units;          // runs of a head, and those of them that are turned
-    int heads_each, head_groups;
+    int units, turned_units;              // runs of a head, and those of them that are turned
+    int block_tokens, block_heads, head_blocks;
+    unsigned unit_magic, head_magic, pair_magic;   // ceil(2^32 / n), 0 for 1: of units, of a block's heads, of pairs
     unsigned long long turn[kMostPairs];  // f / 2 pi, in units of 2^-64
-    uint8_t axis[kMostPairs];
+    int axis[kMostPairs];
 };
 
 // cos and sin of a 64-bit fraction of a turn
@@ -43,63 +44,88 @@ __device__ __forceinline__ void cos_sin(unsigned long long t, float& c, float& s
     s = quarter & 2 ? -b : b;
 }
 
+// kRun elements as one access to any element's address. (As integers: the compiler stores a structure of 16-bit floats in pieces of 2 to 8 bytes, and 65536 tokens of 16 heads then take 45 us.)
+template <int kBytes> struct Piece;
+template <> struct Piece<16> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct Piece<8> { typedef uint32_t type __attribute__((ext_vector_type(2), aligned(2))); };
+template <> struct Piece<4> { typedef uint32_t type __attribute__((aligned(2))); };
+template <> struct Piece<2> { typedef uint16_t type; };
+template <class T, int kRun> using PieceOf = typename Piece<kRun * (int)sizeof(T)>::type;
+
+// x / n for x n < 2^32
+__device__ __forceinline__ int quotient(int x, unsigned magic) { return magic ? (int)__umulhi((unsigned)x, magic) : x; }
+
 // kRun elements in one access; kBeside: a pair's elements lie beside each other, else half of what is turned apart.
 template <class T, int kRun, bool kBeside, class P> __global__ void __launch_bounds__(256) k_rotary(RotaryArgs d) {
     constexpr int kPairs = kBeside ? kRun / 2 : kRun;
-    const long long id = block_number() * 256 + threadIdx.x;
-    const int unit = (int)(id % d.units);
-    const long long rest = id / d.units;
-    const int group = (int)(rest % d.head_groups);
-    const long long token = rest / d.head_groups;
-    if (token >= d.tokens) return;
-    const int all = d.heads[0] + d.heads[1], h0 = group * d.heads_each, h1 = h0 + d.heads_each < all ? h0 + d.heads_each : all;
-    const bool turned = unit < d.turned_units;
-    float c[kPairs], s[kPairs];
-    if (turned) {
-        const P* pos = (const P*)d.positions + token * d.position_stride;
+    __shared__ alignas(16) float cosines[kTable], sines[kTable];     // [tokens][pairs]
+    const long long block = block_number();
+    const int group = (int)(block % d.head_blocks);
+    const long long first = block / d.head_blocks * d.block_tokens;
+    if (first >= d.tokens) return;
+    const int tokens = d.tokens - first < d.block_tokens ? (int)(d.tokens - first) : d.block_tokens;
+    const int all = d.heads[0] + d.heads[1], h0 = group * d.block_heads, heads = h0 + d.block_heads < all ? d.block_heads : all - h0, items = tokens * d.block_heads * d.units;
+    using R = Run<T, kRun>;
+    using W = PieceOf<T, kRun>;
+    const auto load = [](const T* p) { return __builtin_bit_cast(R, *(const W*)p); };
+    const auto store = [](T* p, const R& r) { *(W*)p = __builtin_bit_cast(W, r); };
+    constexpr int kBatch = 4;                              // runs whose loads are on their way together
+    R lo[kBatch], hi[kBatch];
+    T* to[kBatch];
+    int angle[kBatch];                                     // of the first pair in the table; -1: not turned, -2: no run
+    const auto fetch = [&](int i0) {
 #pragma unroll
-        for (int i = 0; i < kPairs; i++) {
-            const int p = unit * kPairs + i;
-            cos_sin((unsigned long long)(long long)pos[d.axis[p]] * d.turn[p], c[i], s[i]);
-            if (d.backward) s[i] = -s[i];
+        for (int n = 0; n < kBatch; n++) {
+            const int i = i0 + 256 * n, row = quotient(i, d.unit_magic), unit = i - row * d.units, t = quotient(row, d.head_magic), own = row - t * d.block_heads;
+            const int which = h0 + own >= d.heads[0], h = which ? h0 + own - d.heads[0] : h0 + own;
+            const bool turned = unit < d.turned_units;
+            const int at = turned ? unit * kRun : 2 * d.pairs + (unit - d.turned_units) * kRun;
+            angle[n] = i >= items || own >= heads ? -2 : turned ? t * d.pairs + unit * kPairs : -1;
+            to[n] = (T*)d.y[which] + ((first + t) * d.heads[which] + h) * d.head_dim + at;
+            if (angle[n] == -2) continue;
+            const T* x = (const T*)d.x[which] + (first + t) * d.token_stride[which] + h * d.head_stride[which] + at;
+            lo[n] = load(x);
+            if (!kBeside && turned) hi[n] = load(x + d.pairs);
         }
+    };
+    fetch(threadIdx.x);                                    // (on their way while the table is made)
+    for (int i = threadIdx.x; i < tokens * d.pairs; i += 256) {
+        const int t = quotient(i, d.pair_magic), p = i - t * d.pairs;
+        const long long at = (long long)((const P*)d.positions)[(first + t) * d.position_stride + d.axis[p]];
+        float c, s;
+        cos_sin((unsigned long long)at * d.turn[p], c, s);
+        cosines[i] = c;
+        sines[i] = d.backward ? -s : s;
     }
-    const int first = turned ? unit * (kBeside ? kRun : kPairs) : 2 * d.pairs + (unit - d.turned_units) * kRun;
-    for (int h = h0; h < h1; h++) {
-        const int t = h >= d.heads[0], own = t ? h - d.heads[0] : h;
-        const T* x = (const T*)d.x[t] + token * d.token_stride[t] + own * d.head_stride[t] + first;
-        T* y = (T*)d.y[t] + (token * d.heads[t] + own) * d.head_dim + first;
-        using R = LooseRun<T, kRun>;
-        if (!turned) { *(R*)y = *(const R*)x; continue; }
-        if constexpr (kBeside) {
-            const R in = *(const R*)x;
-            R out;
+    __syncthreads();
+    for (int i0 = threadIdx.x;;) {
 #pragma unroll
-            for (int i = 0; i < kPairs; i++) {
-                const float a = (float)in.v[2 * i], b = (float)in.v[2 * i + 1];
-                out.v[2 * i] = (T)__builtin_fmaf(a, c[i], -(b * s[i]));
-                out.v[2 * i + 1] = (T)__builtin_fmaf(a, s[i], b * c[i]);
-            }
-            *(R*)y = out;
-        } else {
-            const R lo = *(const R*)x, hi = *(const R*)(x + d.pairs);
-            R a2, b2;
+        for (int n = 0; n < kBatch; n++) {
+            if (angle[n] == -2) continue;
+            if (angle[n] == -1) { store(to[n], lo[n]); continue; }
+            float c[kPairs], s[kPairs];
 #pragma unroll
-            for (int i = 0; i < kPairs; i++) {
-                const float a = (float)lo.v[i], b = (float)hi.v[i];
-                a2.v[i] = (T)__builtin_fmaf(a, c[i], -(b * s[i]));
-                b2.v[i] = (T)__builtin_fmaf(a, s[i], b * c[i]);
+            for (int k = 0; k < kPairs; k++) { c[k] = cosines[angle[n] + k]; s[k] = sines[angle[n] + k]; }
+            R out, out2;
+#pragma unroll
+            for (int k = 0; k < kPairs; k++) {
+                const float a = (float)(kBeside ? lo[n].v[2 * k] : lo[n].v[k]), b = (float)(kBeside ? lo[n].v[2 * k + 1] : hi[n].v[k]);
+                const T a2 = (T)__builtin_fmaf(a, c[k], -(b * s[k])), b2 = (T)__builtin_fmaf(a, s[k], b * c[k]);
+                if constexpr (kBeside) { out.v[2 * k] = a2; out.v[2 * k + 1] = b2; }
+                else { out.v[k] = a2; out2.v[k] = b2; }
             }
-            *(R*)y = a2;
-            *(R*)(y + d.pairs) = b2;
+            store(to[n], out);
+            if constexpr (!kBeside) store(to[n] + d.pairs, out2);
         }
+        if ((i0 += 256 * kBatch) >= items) break;
+        fetch(i0);
     }
 }
 
 const char* wrong(const ntc_rotary_desc* d) {
     if (!d) return "no description";
     if (d->tokens < 0 || d->heads[0] < 0 || d->heads[1] < 0 || (int64_t)d->heads[0] + d->heads[1] > 1 << 20) return "tokens and heads from 0 on, at most 2^20 heads, are needed";
-    if (d->head_dim < 2 || d->head_dim > 1 << 16 || d->head_dim % 2) return "a head has 2 to 65536 elements, an even number";
+    if (d->head_dim < 2 || d->head_dim > 1 << 14 || d->head_dim % 2) return "a head has 2 to 16384 elements, an even number";
     if (d->axes < 1 || d->axes > kMostAxes) return "positions have 1 to 8 axes";
     int64_t pairs = 0;
     for (int a = 0; a < d->axes; a++) {
@@ -142,7 +168,7 @@ extern "C" int ntc_op_rotary(const ntc_rotary_desc* d, void* stream, char* why, 
         if (!d->one_ladder && d->sections[m]) { f = 1; ratio = powl(d->base, -1.0L / d->sections[m]); }
         for (int j = 0; j < d->sections[m]; j++, p++, f *= ratio) {
             a.turn[p] = (unsigned long long)(f * (0x1p64L / 6.283185307179586476925286766559005768L) + 0.5L);
-            a.axis[p] = (uint8_t)m;
+            a.axis[p] = m;
         }
     }
     // The widest access, up to 16 bytes, that divides what is turned and what is not. (Rows may start at any element.)
@@ -151,13 +177,21 @@ extern "C" int ntc_op_rotary(const ntc_rotary_desc* d, void* stream, char* why, 
     const bool beside = d->interleaved != 0;                   // (runs have 2 elements at least then: heads are even)
     a.turned_units = d->interleaved ? 2 * a.pairs / run : a.pairs / run;
     a.units = a.turned_units + (d->head_dim - 2 * a.pairs) / run;
-    // Heads that share a thread's sines: as many as leave 2^19 threads (a card full of them); then a quarter of the work is theirs and not the sines'.
-    const int64_t each = a.tokens * a.units;
-    int64_t groups = ((1 << 19) + each - 1) / each;
-    if (groups > heads) groups = heads;
-    a.heads_each = (int)((heads + groups - 1) / groups);
-    a.head_groups = (heads + a.heads_each - 1) / a.heads_each;
-    const dim3 grid = grid_of((each * a.head_groups + 255) / 256);
+    // Tokens of a block: as many as give each thread four runs, where the table holds them; heads of one token in several blocks where tokens are few.
+    const auto magic = [](int n) { return n > 1 ? (unsigned)((((uint64_t)1 << 32) + n - 1) / n) : 0u; };
+    constexpr int kItems = 1024;
+    const int row = heads * a.units;
+    a.block_tokens = kItems / row < 1 ? 1 : kItems / row;
+    if (a.block_tokens > kTable / a.pairs) a.block_tokens = kTable / a.pairs;
+    while (a.block_tokens > 1 && d->tokens / a.block_tokens < 512) a.block_tokens /= 2;
+    a.block_heads = heads;
+    while (a.block_heads > 1 && a.block_tokens * a.block_heads * a.units > kItems) a.block_heads = (a.block_heads + 1) / 2;
+    while (a.block_tokens == 1 && a.block_heads > 1 && a.block_heads * a.units > 256 && d->tokens * ((heads + a.block_heads - 1) / a.block_heads) < 512) a.block_heads = (a.block_heads + 1) / 2;
+    a.head_blocks = (heads + a.block_heads - 1) / a.block_heads;
+    a.unit_magic = magic(a.units);
+    a.head_magic = magic(a.block_heads);
+    a.pair_magic = magic(a.pairs);
+    const dim3 grid = grid_of((d->tokens + a.block_tokens - 1) / a.block_tokens * a.head_blocks);
     const hipStream_t s = (hipStream_t)stream;
     const auto with = [&](auto type, auto run_, auto beside_, auto position) { k_rotary<decltype(type), run_.value, beside_.value, decltype(position)><<<grid, 256, 0, s>>>(a); };
     const auto with_position = [&](auto type, auto run_, auto beside_) { d->position_bytes == 8 ? with(type, run_, beside_, (int64_t)0) : with(type, run_, beside_, (int32_t)0); };

@@ -718,8 +718,8 @@ py::tuple rotary(const Tensor& positions_, const Tensor& q, const optional<Tenso
         TORCH_CHECK_VALUE(n >= 0 && n <= NTC_ROTARY_PAIRS, "a section has 0 to ", (int)NTC_ROTARY_PAIRS, " pairs, not ", n);
         pairs += n;
     }
-    TORCH_CHECK_VALUE(pairs >= 1 && pairs <= NTC_ROTARY_PAIRS && 2 * pairs <= q.size(-1) && q.size(-1) % 2 == 0 && q.size(-1) <= 65536, "sections of ", pairs, " pairs in all: 1 to ",
-                      (int)NTC_ROTARY_PAIRS, " are needed, within heads of an even number of at most 65536 elements, not ", q.size(-1));
+    TORCH_CHECK_VALUE(pairs >= 1 && pairs <= NTC_ROTARY_PAIRS && 2 * pairs <= q.size(-1) && q.size(-1) % 2 == 0 && q.size(-1) <= 16384, "sections of ", pairs, " pairs in all: 1 to ",
+                      (int)NTC_ROTARY_PAIRS, " are needed, within heads of an even number of at most 16384 elements, not ", q.size(-1));
     TORCH_CHECK_VALUE(base >= 1 && base <= 1e300, "base must be a number from 1 on, not ", base);
     const Tensor positions = last_contiguous(positions_);
     const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || (k && k->requires_grad()));

@@ -258,6 +258,8 @@ def test_no_sequences_no_keys():
     q, k = torch.randn(5, 2, 16, device="cuda").half(), torch.randn(7, 2, 16, device="cuda").half()
     got = run(q, k, k.clone(), torch.ones_like(q), cu_q=on_gpu([0]), cu_k=on_gpu([0]))     # every row is behind the last sequence
     assert all(not x.any() for x in got.values())
+    got = run(q[:0].detach(), k.detach(), k.detach().clone(), torch.ones_like(q[:0]))     # no queries
+    assert not got["dk"].any() and not got["dv"].any() and got["dk"].shape == k.shape
     got = run(q, k[:0], k[:0].clone(), torch.ones_like(q))
     assert not got["o"].any() and not got["dq"].any()
 
