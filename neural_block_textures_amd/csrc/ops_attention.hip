@@ -98,8 +98,9 @@ __device__ __forceinline__ int keys_of(const AttentionArgs& d, const Span& k) {
 }
 
 // ---------------------------------------------------------------- shared memory
-// Rows of kPitch bytes; the 16-byte piece c of row r lies at c ^ spread(r): 16 rows' pieces of one number are in different banks, and so are four rows'
-// pieces of four neighbouring numbers, which a transposing read takes.
+// Rows of kPitch bytes; the 16-byte piece c of row r lies at c ^ spread(r). 64 banks give 256 bytes a clock: 16 rows' pieces of one number are in different
+// banks, and so are four rows' pieces of four neighbouring numbers, which a transposing read takes from 32 lanes (both measured without conflicts; a spread over eight rows takes twice
+// as long). What depends on the lane is made once; the rest is constant offsets.
 template <int kD> struct Tile {
     static constexpr int kPitch = kD <= 32 ? 64 : kD <= 64 ? 128 : 256, kPieces = kPitch / 16, kLines = 256 / kPitch;
     static __device__ __forceinline__ int spread(int r) { return (((r & 3) / kLines) << 2 | ((r >> 2) & 3)) & (kPieces - 1); }
@@ -121,37 +122,75 @@ __device__ __forceinline__ void arrive() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// 8 neighbouring values of row `row` (of 32) of the tile at `at`: columns 16 step + 8 half on
-template <int kD> __device__ __forceinline__ v4u row_piece(const char* at, int row, int half, int step) {
+typedef __attribute__((address_space(3))) const char* Shared;
+// A wave's places in a tile: of its lane's row as an operand, and of the columns of 16 rows.
+template <int kD> struct Places {
     using L = Tile<kD>;
-    return *(const v4u*)(at + row * L::kPitch + (((2 * step + half) ^ L::spread(row)) << 4));
-}
-// of 16 rows from `first` on, 8 rows of column 32 tile + lane % 32: rows 4 half .. and 8 + 4 half ..
-template <int kD> __device__ __forceinline__ v4u column_piece(const char* at, int first, int tile) {
-    using L = Tile<kD>;
-    const int lane = lane_id(), i = lane & 15, half = lane >> 5;
-    v2u r[2];
+    uint32_t row[kD / 16], column[kD / 32][2];
+    __device__ __forceinline__ Places(uint32_t tile) {
+        const int lane = lane_id(), half = lane >> 5, r = lane & 31, i = lane & 15;
 #pragma unroll
-    for (int b = 0; b < 2; b++) {
-        const int row = 8 * b + 4 * half + (i >> 2), piece = 4 * tile + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-        const char* p = at + (first + row) * L::kPitch + ((piece ^ L::spread(row)) << 4) + 8 * (i & 1);
-        r[b] = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)p));
-    }
-    return v4u{ r[0].x, r[0].y, r[1].x, r[1].y };
-}
-// rows of a matrix into a tile of kTile rows: each wave of four takes a quarter. row_off(r): the byte offset of row r (of kTile) from `base`.
-template <int kD, int kTile, class F> __device__ __forceinline__ void load_tile(uint32_t to, const char* base, int D, F row_off) {
-    using L = Tile<kD>;
-    constexpr int kEach = kTile * L::kPieces / 256;        // loads a wave
-    const int wave = uniform(threadIdx.x >> 6), lane = lane_id();
+        for (int s = 0; s < kD / 16; s++) row[s] = tile + r * L::kPitch + (((2 * s + half) ^ L::spread(r)) << 4);
 #pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        const int slot = (wave * kEach + i) * 64 + lane, r = slot / L::kPieces;
-        int piece = (slot % L::kPieces) ^ L::spread(r);
-        if (L::kPieces * 8 > kD || kD != D) piece = 8 * piece < D ? piece : 0;      // past a head's end: any values of the row
-        to_lds16(to + 1024 * (wave * kEach + i), row_off(r) + 16 * piece, base);
+        for (int t = 0; t < kD / 32; t++)
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const int k = 8 * b + 4 * half + (i >> 2), piece = 4 * t + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+                column[t][b] = tile + k * L::kPitch + ((piece ^ L::spread(k)) << 4) + 8 * (i & 1);
+            }
     }
-}
+    // columns 16 step + 8 half on of the lane's row of 32, from row `first`, of the tile `at` bytes on
+    __device__ __forceinline__ v4u row_piece(int at, int first, int step) const {
+        return *(__attribute__((address_space(3))) const v4u*)((Shared)row[step] + (at + first * L::kPitch));
+    }
+    // of 16 rows from `first` on, 8 rows of column 32 tile + lane % 32: rows 4 half .. and 8 + 4 half ..
+    __device__ __forceinline__ v4u column_piece(int at, int first, int tile) const {
+        v2u r[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+            r[b] = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)((Shared)column[tile][b] + (at + first * L::kPitch))));
+        return v4u{ r[0].x, r[0].y, r[1].x, r[1].y };
+    }
+    // between two buffers whose addresses differ in one bit
+    __device__ __forceinline__ void toggle_rows(int bit) {
+#pragma unroll
+        for (uint32_t& x : row) x ^= bit;
+    }
+    __device__ __forceinline__ void toggle_columns(int bit) {
+#pragma unroll
+        for (auto& x : column) { x[0] ^= bit; x[1] ^= bit; }
+    }
+};
+// Rows of a matrix into a tile of kTile rows: each wave of four takes a quarter, 16 bytes a lane and load. The lane's row in the tile and its piece's byte there, of load i:
+template <int kD, int kTile> struct Loads {
+    using L = Tile<kD>;
+    static constexpr int kEach = kTile * L::kPieces / 256;                 // loads a wave
+    static __device__ __forceinline__ int slot(int i) { return (uniform(threadIdx.x >> 6) * kEach + i) * 64 + lane_id(); }
+    static __device__ __forceinline__ int row(int i) { return slot(i) / L::kPieces; }
+    static __device__ __forceinline__ int byte(int i, int D) {
+        const int piece = (slot(i) % L::kPieces) ^ L::spread(row(i));
+        return 16 * (8 * piece < D ? piece : 0);                           // past a head's end: any values of the row
+    }
+    // offset(i): of load i from `base`
+    template <class F> static __device__ __forceinline__ void run(uint32_t to, const char* base, F offset) {
+#pragma unroll
+        for (int i = 0; i < kEach; i++) to_lds16(to + 1024 * (uniform(threadIdx.x >> 6) * kEach + i), offset(i), base);
+    }
+};
+// ... of consecutive rows `stride` bytes apart, `n` of them there (past the end the last one again)
+template <int kD, int kTile> struct RowLoads : Loads<kD, kTile> {
+    using B = Loads<kD, kTile>;
+    uint32_t off[B::kEach];
+    int stride, D;
+    __device__ __forceinline__ RowLoads(long long stride_, int D_) : stride((int)stride_), D(D_) {
+#pragma unroll
+        for (int i = 0; i < B::kEach; i++) off[i] = (uint32_t)B::row(i) * (uint32_t)stride + B::byte(i, D);
+    }
+    __device__ __forceinline__ void load(uint32_t to, const char* base, int n) const {
+        if (n >= kTile) B::run(to, base, [&](int i) { return off[i]; });
+        else B::run(to, base, [&](int i) { const int r = B::row(i); return (uint32_t)(r < n ? r : n - 1) * (uint32_t)stride + B::byte(i, D); });
+    }
+};
 
 // ---------------------------------------------------------------- rows in registers
 // A row of a group's matrix: query and head, from a tile's first row
@@ -208,10 +247,10 @@ template <class T> __device__ __forceinline__ v4u packed(const v16f& x, int half
 }
 
 // ---------------------------------------------------------------- forward
-template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention(AttentionArgs d) {
+template <class T, int kD, bool kStats> __global__ void __launch_bounds__(256, 2) k_attention(AttentionArgs d) {
     using L = Tile<kD>;
     constexpr int kTile = kKeys * L::kPitch;
-    __shared__ alignas(1024) char lds[4 * kTile];          // keys, values; two of each
+    __shared__ alignas(2 * kTile) char lds[4 * kTile];     // keys, values; two of each
     const long long id = block_number();
     const int head = (int)(id % d.k_heads), part = (int)(id / d.k_heads % d.parts);
     const long long t_ = id / d.k_heads / d.parts;
@@ -240,66 +279,130 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     const int all = block_last < 0 ? 0 : block_last / kKeys + 1;
     const int begin = (int)((long long)all * part / d.parts), stages = (int)((long long)all * (part + 1) / d.parts);
 
+    // A stage is 64 keys. While its probabilities are made and summed up with the values, the next stage's scores are: products and the exponentials between them are
+    // in an order that keeps both kinds of unit busy (a wave issues in order), with operands on their way two products ahead. Keys are loaded two stages ahead, values one.
     const char *kp = d.k.p + ks.start + head * d.k.head, *vp = d.v.p + v_start + head * d.v.head;
     const uint32_t lds0 = lds_address(lds);
-    const auto load = [&](int s) {
-        const int k0 = s * kKeys, n = Lk - k0;             // rows past the end read the last one
-        const char *kb_ = kp + k0 * d.k.row, *vb_ = vp + k0 * d.v.row;
-        load_tile<kD, kKeys>(lds0 + (s & 1) * 2 * kTile, kb_, d.D, [&](int r) { return (uint32_t)(r < n ? r : n - 1) * (uint32_t)d.k.row; });
-        load_tile<kD, kKeys>(lds0 + (s & 1) * 2 * kTile + kTile, vb_, d.D, [&](int r) { return (uint32_t)(r < n ? r : n - 1) * (uint32_t)d.v.row; });
-    };
-    v16f o[kD / 32] = {};
+    const RowLoads<kD, kKeys> key_loads(d.k.row, d.D), value_loads(d.v.row, d.D);
+    const auto load_keys = [&](int s) { key_loads.load(lds0 + ((s - begin) & 1) * kTile, kp + (long long)s * kKeys * d.k.row, Lk - s * kKeys); };
+    const auto load_values = [&](int s) { value_loads.load(lds0 + (2 + ((s - begin) & 1)) * kTile, vp + (long long)s * kKeys * d.v.row, Lk - s * kKeys); };
+    constexpr int kScores = 2 * (kD / 16), kSums = 4 * (kD / 32);          // products of a stage
+    const int full = wave_first < 0 ? 0 : (wave_first + 1) / kKeys;        // stages whose keys all of the wave's queries see
+    const int own = wave_last < 0 ? 0 : wave_last / kKeys + 1, own_end = own < stages ? own : stages;
+    Places<kD> places(lds0);
+    const auto key_piece = [&](int at, int n) { return places.row_piece(at, 32 * (n & 1), n >> 1); };
+    const auto value_piece = [&](int at, int n) { return places.column_piece(2 * kTile + at, 16 * (n / (kD / 32)), n % (kD / 32)); };
+    const auto hide = [&](v16f& x, int j, int r, int s) { x[r] = 32 * j + result_row(r) <= last - s * kKeys - 4 * half ? x[r] : -NTC_INF; };
+
+    v16f o[kD / 32] = {}, even[2], odd[2];                 // sums; scores of stages in turn
     // Two sums of the probabilities: as rounded, by which the result is divided (what rounding adds to all values alike is then in both), and as they are, for lse.
-    float m = -NTC_INF, l = 0, exact = 0;
-    if (begin < stages) load(begin);
-    for (int s = begin; s < stages; s++) {
-        arrive();
-        if (s + 1 < stages) load(s + 1);
-        const int k0 = s * kKeys;
-        if (k0 > wave_last) continue;
-        const char *kt = lds + (s & 1) * 2 * kTile, *vt = kt + kTile;
-        v16f x[2] = {};
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int i = 0; i < kD / 16; i++) x[j] = product<T>(row_piece<kD>(kt + 32 * j * L::kPitch, column, half, i), q[i], x[j]);
-        if (k0 + kKeys - 1 > wave_first) {
-            const int seen = last - k0 - 4 * half;
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) x[j][r] = 32 * j + result_row(r) <= seen ? x[j][r] : -NTC_INF;
-        }
-        float most = x[0][0];
-#pragma unroll
-        for (int r = 1; r < 32; r++) most = __builtin_fmaxf(most, x[r / 16][r % 16]);
+    float m = -NTC_INF, l = 0, exact = 0, most = -NTC_INF;
+    const auto stage = [&](int s, v16f (&x)[2], v16f (&z)[2], auto key_at_, auto value_at_, auto masks_, auto more_) {
+        constexpr bool kMasks = masks_.value, kMore = more_.value;         // of the next stage, whose scores z will be: they are masked, it is there
+        constexpr int kKeyAt = key_at_.value, kValueAt = value_at_.value;  // where the next stage's keys and this one's values are, from their places
+        v4u kf[3], vf[3];
+        if constexpr (kMore) { kf[0] = key_piece(kKeyAt, 0); kf[1] = key_piece(kKeyAt, 1); }
         most = __builtin_fmaxf(most, other_half(most));
         const bool rises = most * d.c > m * d.c + 8.f;     // (m is -inf at first)
         if (__any(rises)) {
             const float next = rises ? most : m, by = m == next ? 1.f : fast_exp2((m - next) * d.c);
             m = next;
             l *= by;
-            exact *= by;
+            if constexpr (kStats) exact *= by;
 #pragma unroll
             for (int t = 0; t < kD / 32; t++) o[t] *= by;
         }
         const float mc = m == -NTC_INF ? 0.f : m * d.c;
+        uint32_t p[16];
+        const auto exponentials = [&](int e) {             // of a pair
+            const float a = fast_exp2(__builtin_fmaf(x[e / 8][2 * e % 16], d.c, -mc)), b = fast_exp2(__builtin_fmaf(x[e / 8][2 * e % 16 + 1], d.c, -mc));
+            if constexpr (kStats) exact += a + b;
+            p[e] = pack2<T>(a, b);
+            l = add2<T>(p[e], l);
+        };
+        if constexpr (kMore) {
+            z[0] = z[1] = v16f{};
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+            for (int n = 0; n < kScores; n++) {
+                z[n & 1] = product<T>(kf[n % 3], q[n >> 1], z[n & 1]);
+                if (n + 2 < kScores) kf[(n + 2) % 3] = key_piece(kKeyAt, n + 2);
+                else vf[n + 2 - kScores] = value_piece(kValueAt, n + 2 - kScores);
+                if (n < kScores - 2) {
 #pragma unroll
-            for (int r = 0; r < 16; r++) x[j][r] = fast_exp2(__builtin_fmaf(x[j][r], d.c, -mc));
-        if (d.lse) {
+                    for (int e = 16 * n / (kScores - 2); e < 16 * (n + 1) / (kScores - 2); e++) exponentials(e);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            vf[0] = value_piece(kValueAt, 0);
+            vf[1] = value_piece(kValueAt, 1);
 #pragma unroll
-            for (int r = 0; r < 32; r++) exact += x[r / 16][r % 16];
+            for (int e = 0; e < 16; e++) exponentials(e);
         }
+        most = -NTC_INF;
 #pragma unroll
-        for (int h = 0; h < 4; h++) {
-            const v4u p = packed<T>(x[h / 2], h & 1);
-            l = add2<T>(p.w, add2<T>(p.z, add2<T>(p.y, add2<T>(p.x, l))));
+        for (int n = 0; n < kSums; n++) {
+            const int t = n % (kD / 32), h = n / (kD / 32);
+            o[t] = product<T>(vf[n % 3], v4u{ p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3] }, o[t]);
+            if (n + 2 < kSums) vf[(n + 2) % 3] = value_piece(kValueAt, n + 2);
+            if constexpr (kMore) {
 #pragma unroll
-            for (int t = 0; t < kD / 32; t++) o[t] = product<T>(column_piece<kD>(vt, 16 * h, t), p, o[t]);
+                for (int e = 32 * n / kSums; e < 32 * (n + 1) / kSums; e++) {
+                    if constexpr (kMasks) hide(z[e / 16], e / 16, e % 16, s + 1);
+                    most = __builtin_fmaxf(most, z[e / 16][e % 16]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        asm volatile("" : "+v"(most), "+v"(l));            // (made here: the compiler would sink them behind the next barrier, between nothing)
+    };
+    if (begin < stages) {
+        load_keys(begin);
+        arrive();
+        load_values(begin);
+        if (begin + 1 < stages) load_keys(begin + 1);
+        if (begin < own_end) {
+            even[0] = even[1] = v16f{};
+#pragma unroll
+            for (int n = 0; n < kScores; n++) even[n & 1] = product<T>(key_piece(0, n), q[n >> 1], even[n & 1]);
+            if (begin >= full) {
+#pragma unroll
+                for (int e = 0; e < 32; e++) hide(even[e / 16], e / 16, e % 16, begin);
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e++) most = __builtin_fmaxf(most, even[e / 16][e % 16]);
         }
     }
+    const auto step = [&](int s) {
+        arrive();
+        if (s + 1 < stages) load_values(s + 1);
+        if (s + 2 < stages) load_keys(s + 2);
+    };
+    const auto turn = [&] {                                // what was odd is even now
+        even[0] = odd[0];
+        even[1] = odd[1];
+        places.toggle_rows(kTile);
+        places.toggle_columns(kTile);
+    };
+    // (loops of their own, for the compiler: one loop over all kinds of stages moves the sums between registers each time)
+    using Here = std::integral_constant<int, 0>;
+    using There = std::integral_constant<int, kTile>;
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    int s = begin;
+    const int end = full < own_end ? full : own_end;
+    for (; s + 2 < end; s += 2) {
+        step(s);
+        stage(s, even, odd, There{}, Here{}, no, yes);
+        step(s + 1);
+        stage(s + 1, odd, even, Here{}, There{}, no, yes);
+    }
+    places.toggle_rows(kTile);
+    if (s + 1 < end) { step(s); stage(s, even, odd, Here{}, Here{}, no, yes); turn(); s++; }
+    for (; s + 1 < own_end; s++) { step(s); stage(s, even, odd, Here{}, Here{}, yes, yes); turn(); }
+    if (s < own_end) { step(s); stage(s, even, odd, Here{}, Here{}, no, no); s++; }
+    for (; s < stages; s++) step(s);
     l += other_half(l);
     exact += other_half(exact);
     const long long at = (qs.row + row.i) * d.q_heads + head * d.group + row.g;
@@ -312,7 +415,7 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     const float f = l == 0 ? 0.f : 1.f / l;
     store_row<T, kD>((char*)d.out + at * d.D * 2, o, f, live, d.D);
     if (d.rest) store_row<T, kD, true>((char*)d.rest + at * d.D * 2, o, f, live, d.D);
-    if (d.lse && live && half == 0) d.lse[at] = exact == 0 ? -NTC_INF : (m * d.c + fast_log2(exact)) * kLn2;
+    if (kStats && live && half == 0) d.lse[at] = exact == 0 ? -NTC_INF : (m * d.c + fast_log2(exact)) * kLn2;
 }
 
 // The parts of a row, joined by a wave: a lane takes a part's statistics first, then eight columns of every 64 / kPieces-th part.
@@ -419,8 +522,8 @@ template <class T> constexpr int kShift = std::is_same_v<T, f16> ? 14 : 0;      
 template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention_dq(AttentionArgs d) {
     using L = Tile<kD>;
     constexpr int kTile = kKeys * L::kPitch;
-    __shared__ alignas(1024) char lds[4 * kTile];
-    __shared__ alignas(16) float mean[kD];
+    __shared__ alignas(2 * kTile) char lds[4 * kTile + 4 * kD];   // keys, values; two of each, and the mean
+    float* const mean = (float*)(lds + 4 * kTile);
     const long long id = block_number();
     const int head = (int)(id % d.k_heads);
     const long long t_ = id / d.k_heads;
@@ -470,26 +573,26 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
 
     const char *kp = d.k.p + ks.start + head * d.k.head, *vp = d.v.p + v_start + head * d.v.head;
     const uint32_t lds0 = lds_address(lds);
+    const RowLoads<kD, kKeys> key_loads(d.k.row, d.D), value_loads(d.v.row, d.D);
     const auto load = [&](int s) {
-        const int k0 = s * kKeys, n = Lk - k0;
-        const char *kb_ = kp + k0 * d.k.row, *vb_ = vp + k0 * d.v.row;
-        load_tile<kD, kKeys>(lds0 + (s & 1) * 2 * kTile, kb_, d.D, [&](int r) { return (uint32_t)(r < n ? r : n - 1) * (uint32_t)d.k.row; });
-        load_tile<kD, kKeys>(lds0 + (s & 1) * 2 * kTile + kTile, vb_, d.D, [&](int r) { return (uint32_t)(r < n ? r : n - 1) * (uint32_t)d.v.row; });
+        key_loads.load(lds0 + (s & 1) * kTile, kp + (long long)s * kKeys * d.k.row, Lk - s * kKeys);
+        value_loads.load(lds0 + (2 + (s & 1)) * kTile, vp + (long long)s * kKeys * d.v.row, Lk - s * kKeys);
     };
+    const Places<kD> places(lds0);
     v16f dq[kD / 32] = {};
     float sum = 0;
     if (stages) load(0);
     for (int s = 0; s < stages; s++) {
         arrive();
         if (s + 1 < stages) load(s + 1);
-        const char *kt = lds + (s & 1) * 2 * kTile, *vt = kt + kTile;
+        const int at = (s & 1) * kTile;
         if (s == 0 && wave == 0) {
             const uint32_t one = pack2<T>(1.f, 1.f);
 #pragma unroll
             for (int t = 0; t < kD / 32; t++) {
                 v16f x = {};
 #pragma unroll
-                for (int a = 0; a < kKeys / 16; a++) x = product<T>(column_piece<kD>(kt, 16 * a, t), v4u{ one, one, one, one }, x);
+                for (int a = 0; a < kKeys / 16; a++) x = product<T>(places.column_piece(at, 16 * a, t), v4u{ one, one, one, one }, x);
 #pragma unroll
                 for (int r = 0; r < 16; r++) if (column == 0) mean[32 * t + result_row(r) + 4 * half] = x[r] * (1.f / kKeys);
             }
@@ -500,9 +603,9 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
             const int k0 = s * kKeys + 32 * j;
             v16f x = {}, y = {};
 #pragma unroll
-            for (int i = 0; i < kD / 16; i++) x = product<T>(row_piece<kD>(kt + 32 * j * L::kPitch, column, half, i), q[i], x);
+            for (int i = 0; i < kD / 16; i++) x = product<T>(places.row_piece(at, 32 * j, i), q[i], x);
 #pragma unroll
-            for (int i = 0; i < kD / 16; i++) y = product<T>(row_piece<kD>(vt + 32 * j * L::kPitch, column, half, i), g[i], y);
+            for (int i = 0; i < kD / 16; i++) y = product<T>(places.row_piece(at + 2 * kTile, 32 * j, i), g[i], y);
 #pragma unroll
             for (int r = 0; r < 16; r++) x[r] = fast_exp2(__builtin_fmaf(x[r], d.c, -lse)) * __builtin_fmaf(y[r], up, -delta_up);
             if (k0 + 31 > wave_first) {
@@ -515,7 +618,7 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
                 const v4u p = packed<T>(x, a);
                 sum = add2<T>(p.w, add2<T>(p.z, add2<T>(p.y, add2<T>(p.x, sum))));
 #pragma unroll
-                for (int t = 0; t < kD / 32; t++) dq[t] = product<T>(column_piece<kD>(kt, 32 * j + 16 * a, t), p, dq[t]);
+                for (int t = 0; t < kD / 32; t++) dq[t] = product<T>(places.column_piece(at, 32 * j + 16 * a, t), p, dq[t]);
             }
         }
     }
@@ -532,8 +635,8 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
 
 template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention_dkv(AttentionArgs d) {
     using L = Tile<kD>;
-    constexpr int kStep = 64, kTile = kStep * L::kPitch, kStage = 2 * kTile + 8 * kStep;
-    __shared__ alignas(1024) char lds[2 * kStage];         // queries, gradients, log sums and deltas of kStep rows; two of each
+    constexpr int kStep = 64, kTile = kStep * L::kPitch;
+    __shared__ alignas(2 * kTile) char lds[4 * kTile + 16 * kStep];        // queries, gradients, then log sums and deltas of kStep rows; two of each
     const long long id = block_number();
     const int head = (int)(id % d.k_heads), part = (int)(id / d.k_heads % d.parts);
     const long long t_ = id / d.k_heads / d.parts;
@@ -568,33 +671,35 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     const char *qp = d.q.p + qs.start + head * d.group * d.q.head, *gp = d.d_o.p + do_start + head * d.group * d.d_o.head;
     const long long at0 = qs.row * d.q_heads + head * d.group;
     const uint32_t lds0 = lds_address(lds);
+    using RowsLoad = Loads<kD, kStep>;
     const auto load = [&](int s) {
         const int r0 = s * kStep, n = rows - r0, i0 = r0 / d.group, g0 = r0 - i0 * d.group;
-        const uint32_t to = lds0 + (s & 1) * kStage;
+        const uint32_t to = lds0 + (s & 1) * kTile;
         const auto place = [&](int r, long long row, long long head_) {
             const Row x = row_at(d, 0, g0, r < n ? r : n - 1);
             return (uint32_t)x.i * (uint32_t)row + (uint32_t)x.g * (uint32_t)head_;
         };
-        load_tile<kD, kStep>(to, qp + i0 * d.q.row, d.D, [&](int r) { return place(r, d.q.row, d.q.head); });
-        load_tile<kD, kStep>(to + kTile, gp + i0 * d.d_o.row, d.D, [&](int r) { return place(r, d.d_o.row, d.d_o.head); });
-        if (wave < 2) to_lds4(to + 2 * kTile + 4 * kStep * wave, place(lane, 4ll * d.q_heads, 4), (const char*)((wave ? d.delta : d.lse) + at0 + (long long)i0 * d.q_heads));
+        RowsLoad::run(to, qp + i0 * d.q.row, [&](int i) { return place(RowsLoad::row(i), d.q.row, d.q.head) + RowsLoad::byte(i, d.D); });
+        RowsLoad::run(to + 2 * kTile, gp + i0 * d.d_o.row, [&](int i) { return place(RowsLoad::row(i), d.d_o.row, d.d_o.head) + RowsLoad::byte(i, d.D); });
+        if (wave < 2) to_lds4(lds0 + 4 * kTile + (s & 1) * 8 * kStep + 4 * kStep * wave, place(lane, 4ll * d.q_heads, 4), (const char*)((wave ? d.delta : d.lse) + at0 + (long long)i0 * d.q_heads));
     };
+    const Places<kD> places(lds0);
     v16f dk[kD / 32] = {}, dv[kD / 32] = {};
     if (start < stages) load(start);
     for (int s = start; s < stages; s++) {
         arrive();
         if (s + 1 < stages) load(s + 1);
-        const char *qt = lds + (s & 1) * kStage, *gt = qt + kTile;
-        const float* sums = (const float*)(gt + kTile);
+        const int at = (s & 1) * kTile;
+        const float* sums = (const float*)(lds + 4 * kTile + (s & 1) * 8 * kStep);
         if (s * kStep + kStep <= wave_start) continue;
 #pragma unroll
         for (int j = 0; j < kStep / 32; j++) {
             const int r0 = s * kStep + 32 * j;
             v16f x = {}, y = {};
 #pragma unroll
-            for (int i = 0; i < kD / 16; i++) x = product<T>(row_piece<kD>(qt + 32 * j * L::kPitch, column, half, i), k[i], x);
+            for (int i = 0; i < kD / 16; i++) x = product<T>(places.row_piece(at, 32 * j, i), k[i], x);
 #pragma unroll
-            for (int i = 0; i < kD / 16; i++) y = product<T>(row_piece<kD>(gt + 32 * j * L::kPitch, column, half, i), v[i], y);
+            for (int i = 0; i < kD / 16; i++) y = product<T>(places.row_piece(at + 2 * kTile, 32 * j, i), v[i], y);
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int row = 32 * j + result_row(r) + 4 * half;
@@ -615,8 +720,8 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
                 const v4u p = packed<T>(x, a), z = packed<T>(y, a);
 #pragma unroll
                 for (int t = 0; t < kD / 32; t++) {
-                    dv[t] = product<T>(column_piece<kD>(gt, 32 * j + 16 * a, t), p, dv[t]);
-                    dk[t] = product<T>(column_piece<kD>(qt, 32 * j + 16 * a, t), z, dk[t]);
+                    dv[t] = product<T>(places.column_piece(at + 2 * kTile, 32 * j + 16 * a, t), p, dv[t]);
+                    dk[t] = product<T>(places.column_piece(at, 32 * j + 16 * a, t), z, dk[t]);
                 }
             }
         }
@@ -788,7 +893,8 @@ int ntc_op_attention(const ntc_attention_desc* d, void* stream, char* why, size_
     }
     const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads * a.parts);
     with_head(d->dtype, d->head_dim, [&](auto t, auto h) {
-        k_attention<decltype(t), h.value><<<grid, 256, 0, s>>>(a);
+        if (a.lse) k_attention<decltype(t), h.value, true><<<grid, 256, 0, s>>>(a);
+        else k_attention<decltype(t), h.value, false><<<grid, 256, 0, s>>>(a);
         if (a.parts > 1) k_attention_join<decltype(t), h.value == 96 ? 16 : h.value / 8><<<grid_of(ceil_div(d->q_rows * d->q_heads, 4)), 256, 0, s>>>(a);
     });
     return launched(why, cap);
