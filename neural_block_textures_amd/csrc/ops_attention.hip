@@ -12,6 +12,9 @@
 // (values or keys, transposed) comes from LDS by the transposing read, four keys of a column at a time. The keys' and values' gradients go the same way with
 // queries and keys exchanged. No score leaves a register.
 #include "ops_common.hpp"
+#ifndef NTC_P
+#define NTC_P 32
+#endif
 
 namespace ntc_ops {
 namespace {
@@ -50,7 +53,7 @@ struct Operand3 { const char* p; long long row, head, batch; };    // strides in
 struct AttentionArgs {
     Operand3 q, k, v, d_o;
     void *out, *rest, *dq, *dk, *dv;
-    float *lse, *delta, *extent;
+    float *lse, *log_sums, *deltas, *extent;   // backward [q_rows][q_heads]: log2 sum exp less kShift, dO o times the scores' power of two over 2^kShift
     const int *cu_q, *cu_k, *k_lens;
     long long q_rows, k_rows;
     int sequences, q_each, k_each;     // rows of a sequence where there are no ends
@@ -58,7 +61,7 @@ struct AttentionArgs {
     unsigned group_magic;              // ceil(2^32 / group): x / group is the high word of the product with it where x group < 2^32; 0 for 1
     int parts;                         // of a sequence's keys (backward: of its rows), joined by a second launch; their sums:
     float* part_sums;                  // forward [parts][q_rows][q_heads][D]; backward dk's [parts][k_rows][k_heads][D], then dv's
-    float4* part_stats;                // forward [parts][q_rows][q_heads]: m c, both sums of probabilities
+    float2* part_stats;                // forward [parts][q_rows][q_heads]: m c and the sum of probabilities
     int tiles, tiles_each;             // tiles of rows (or keys) in all, and of each sequence where there are no ends
     float scale, c;                    // c: scale log2 e
 };
@@ -247,7 +250,7 @@ template <class T> __device__ __forceinline__ v4u packed(const v16f& x, int half
 }
 
 // ---------------------------------------------------------------- forward
-template <class T, int kD, bool kStats> __global__ void __launch_bounds__(256, 2) k_attention(AttentionArgs d) {
+template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 : kD <= 64 ? 3 : 2) k_attention(AttentionArgs d) {
     using L = Tile<kD>;
     constexpr int kTile = kKeys * L::kPitch;
     __shared__ alignas(2 * kTile) char lds[4 * kTile];     // keys, values; two of each
@@ -286,7 +289,7 @@ template <class T, int kD, bool kStats> __global__ void __launch_bounds__(256, 2
     const RowLoads<kD, kKeys> key_loads(d.k.row, d.D), value_loads(d.v.row, d.D);
     const auto load_keys = [&](int s) { key_loads.load(lds0 + ((s - begin) & 1) * kTile, kp + (long long)s * kKeys * d.k.row, Lk - s * kKeys); };
     const auto load_values = [&](int s) { value_loads.load(lds0 + (2 + ((s - begin) & 1)) * kTile, vp + (long long)s * kKeys * d.v.row, Lk - s * kKeys); };
-    constexpr int kScores = 2 * (kD / 16), kSums = 4 * (kD / 32);          // products of a stage
+    constexpr int kScores = 2 * (kD / 16), kSums = 4 * (kD / 32), kAhead = kD <= 32 ? 2 : kD <= 64 ? 3 : 4;      // products of a stage, and how many operands come ahead of theirs
     const int full = wave_first < 0 ? 0 : (wave_first + 1) / kKeys;        // stages whose keys all of the wave's queries see
     const int own = wave_last < 0 ? 0 : wave_last / kKeys + 1, own_end = own < stages ? own : stages;
     Places<kD> places(lds0);
@@ -295,28 +298,31 @@ template <class T, int kD, bool kStats> __global__ void __launch_bounds__(256, 2
     const auto hide = [&](v16f& x, int j, int r, int s) { x[r] = 32 * j + result_row(r) <= last - s * kKeys - 4 * half ? x[r] : -NTC_INF; };
 
     v16f o[kD / 32] = {}, even[2], odd[2];                 // sums; scores of stages in turn
-    // Two sums of the probabilities: as rounded, by which the result is divided (what rounding adds to all values alike is then in both), and as they are, for lse.
-    float m = -NTC_INF, l = 0, exact = 0, most = -NTC_INF;
+    // l: the sum of the probabilities as they are rounded, so that what rounding does to all values alike is in the products and in what they are divided by. (lse takes it too: it is off by
+    // half a step at most, a probability's own rounding, and by that over the root of the keys as a rule.)
+    float m = -NTC_INF, l = 0, most = -NTC_INF;
     const auto stage = [&](int s, v16f (&x)[2], v16f (&z)[2], auto key_at_, auto value_at_, auto masks_, auto more_) {
         constexpr bool kMasks = masks_.value, kMore = more_.value;         // of the next stage, whose scores z will be: they are masked, it is there
         constexpr int kKeyAt = key_at_.value, kValueAt = value_at_.value;  // where the next stage's keys and this one's values are, from their places
-        v4u kf[3], vf[3];
-        if constexpr (kMore) { kf[0] = key_piece(kKeyAt, 0); kf[1] = key_piece(kKeyAt, 1); }
+        v4u f[kAhead + 1];
+        if constexpr (kMore) {
+#pragma unroll
+            for (int n = 0; n < kAhead; n++) f[n] = key_piece(kKeyAt, n);
+        }
         most = __builtin_fmaxf(most, other_half(most));
         const bool rises = most * d.c > m * d.c + 8.f;     // (m is -inf at first)
         if (__any(rises)) {
             const float next = rises ? most : m, by = m == next ? 1.f : fast_exp2((m - next) * d.c);
             m = next;
             l *= by;
-            if constexpr (kStats) exact *= by;
 #pragma unroll
             for (int t = 0; t < kD / 32; t++) o[t] *= by;
         }
         const float mc = m == -NTC_INF ? 0.f : m * d.c;
         uint32_t p[16];
+        constexpr int kFirst = 10;                         // pairs of exponentials that lie between the next scores' products; the others lie between the sums'
         const auto exponentials = [&](int e) {             // of a pair
             const float a = fast_exp2(__builtin_fmaf(x[e / 8][2 * e % 16], d.c, -mc)), b = fast_exp2(__builtin_fmaf(x[e / 8][2 * e % 16 + 1], d.c, -mc));
-            if constexpr (kStats) exact += a + b;
             p[e] = pack2<T>(a, b);
             l = add2<T>(p[e], l);
         };
@@ -325,18 +331,15 @@ template <class T, int kD, bool kStats> __global__ void __launch_bounds__(256, 2
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int n = 0; n < kScores; n++) {
-                z[n & 1] = product<T>(kf[n % 3], q[n >> 1], z[n & 1]);
-                if (n + 2 < kScores) kf[(n + 2) % 3] = key_piece(kKeyAt, n + 2);
-                else vf[n + 2 - kScores] = value_piece(kValueAt, n + 2 - kScores);
-                if (n < kScores - 2) {
+                z[n & 1] = product<T>(f[n % (kAhead + 1)], q[n >> 1], z[n & 1]);
+                f[(n + kAhead) % (kAhead + 1)] = n + kAhead < kScores ? key_piece(kKeyAt, n + kAhead) : value_piece(kValueAt, n + kAhead - kScores);
 #pragma unroll
-                    for (int e = 16 * n / (kScores - 2); e < 16 * (n + 1) / (kScores - 2); e++) exponentials(e);
-                }
+                for (int e = kFirst * n / kScores; e < kFirst * (n + 1) / kScores; e++) exponentials(e);
                 __builtin_amdgcn_sched_barrier(0);
             }
         } else {
-            vf[0] = value_piece(kValueAt, 0);
-            vf[1] = value_piece(kValueAt, 1);
+#pragma unroll
+            for (int n = 0; n < kAhead; n++) f[(n + kScores) % (kAhead + 1)] = value_piece(kValueAt, n);
 #pragma unroll
             for (int e = 0; e < 16; e++) exponentials(e);
         }
@@ -344,9 +347,13 @@ template <class T, int kD, bool kStats> __global__ void __launch_bounds__(256, 2
 #pragma unroll
         for (int n = 0; n < kSums; n++) {
             const int t = n % (kD / 32), h = n / (kD / 32);
-            o[t] = product<T>(vf[n % 3], v4u{ p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3] }, o[t]);
-            if (n + 2 < kSums) vf[(n + 2) % 3] = value_piece(kValueAt, n + 2);
+            o[t] = product<T>(f[(n + kScores) % (kAhead + 1)], v4u{ p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3] }, o[t]);
+            if (n + kAhead < kSums) f[(n + kAhead + kScores) % (kAhead + 1)] = value_piece(kValueAt, n + kAhead);
             if constexpr (kMore) {
+                // (the rest of them, due a quarter of the products before theirs)
+                constexpr int kRest = 16 - kFirst, kBy = kSums / 2 + kSums / 8;
+#pragma unroll
+                for (int e = kFirst + kRest * n / kBy; e < 16 && e < kFirst + kRest * (n + 1) / kBy; e++) exponentials(e);
 #pragma unroll
                 for (int e = 32 * n / kSums; e < 32 * (n + 1) / kSums; e++) {
                     if constexpr (kMasks) hide(z[e / 16], e / 16, e % 16, s + 1);
@@ -404,18 +411,17 @@ template <class T, int kD, bool kStats> __global__ void __launch_bounds__(256, 2
     if (s < own_end) { step(s); stage(s, even, odd, Here{}, Here{}, no, no); s++; }
     for (; s < stages; s++) step(s);
     l += other_half(l);
-    exact += other_half(exact);
     const long long at = (qs.row + row.i) * d.q_heads + head * d.group + row.g;
     if (d.parts > 1) {
         const long long own = (long long)part * d.q_rows * d.q_heads + at;
         store_floats<kD>(d.part_sums + own * d.D, o, live, d.D);
-        if (live && half == 0) d.part_stats[own] = make_float4(m * d.c, l, exact, 0.f);
+        if (live && half == 0) d.part_stats[own] = make_float2(m * d.c, l);
         return;
     }
     const float f = l == 0 ? 0.f : 1.f / l;
     store_row<T, kD>((char*)d.out + at * d.D * 2, o, f, live, d.D);
     if (d.rest) store_row<T, kD, true>((char*)d.rest + at * d.D * 2, o, f, live, d.D);
-    if (kStats && live && half == 0) d.lse[at] = exact == 0 ? -NTC_INF : (m * d.c + fast_log2(exact)) * kLn2;
+    if (d.lse && live && half == 0) d.lse[at] = l == 0 ? -NTC_INF : (m * d.c + fast_log2(l)) * kLn2;
 }
 
 // The parts of a row, joined by a wave: a lane takes a part's statistics first, then eight columns of every 64 / kPieces-th part.
@@ -424,11 +430,11 @@ template <class T, int kPieces> __global__ void __launch_bounds__(256) k_attenti
     const int lane = lane_id(), piece = lane % kPieces, group = lane / kPieces, col = 8 * piece;
     const long long rows = d.q_rows * d.q_heads, row = block_number() * 4 + (threadIdx.x >> 6);
     if (row >= rows) return;
-    const float4 st = lane < d.parts ? d.part_stats[lane * rows + row] : make_float4(-NTC_INF, 0.f, 0.f, 0.f);
+    const float2 st = lane < d.parts ? d.part_stats[lane * rows + row] : make_float2(-NTC_INF, 0.f);
     const auto larger = [](float a, float b) { return __builtin_fmaxf(a, b); };
     const auto add = [](float a, float b) { return a + b; };
     const float m = reduce64(st.x, larger), by = st.x == m ? 1.f : fast_exp2(st.x - m);                          // (no key at all: m is -inf, and what the part has is 0)
-    const float l = reduce64(st.y * by, add), exact = reduce64(st.z * by, add);
+    const float l = reduce64(st.y * by, add);
     float sum[8] = {};
 #pragma unroll 4
     for (int p0 = 0; p0 < d.parts; p0 += kGroups) {
@@ -456,7 +462,7 @@ template <class T, int kPieces> __global__ void __launch_bounds__(256) k_attenti
     const long long at = 2 * (row * d.D + col);
     *(v4u*)((char*)d.out + at) = v4u{ out[0], out[1], out[2], out[3] };
     if (d.rest) *(v4u*)((char*)d.rest + at) = v4u{ rest[0], rest[1], rest[2], rest[3] };
-    if (d.lse && col == 0) d.lse[row] = exact == 0 ? -NTC_INF : (m + fast_log2(exact)) * kLn2;
+    if (d.lse && col == 0) d.lse[row] = l == 0 ? -NTC_INF : (m + fast_log2(l)) * kLn2;
 }
 
 // ---------------------------------------------------------------- backward
@@ -561,9 +567,12 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     }
     load_row<kD>(q, d.q.p + qs.start + row.i * d.q.row + h * d.q.head, live, d.D);
     delta += other_half(delta);
-    if (live && half == 0) d.delta[at] = delta;
     const int e = gradient_exponent<T>(d);
     const float up = two_to(e), lse = live ? d.lse[at] * kLog2e : 0.f, delta_up = delta * up;
+    if (live && half == 0) {                               // as the keys' and values' gradients take them
+        d.log_sums[at] = lse - kShift<T>;
+        d.deltas[at] = delta_up * two_to(-kShift<T>);
+    }
     const int last = d.causal ? (row.i + off < Lk - 1 ? row.i + off : Lk - 1) : Lk - 1;
     const int wave_first = d.causal ? (i0 + off < Lk - 1 ? i0 + off : Lk - 1) : Lk - 1;
     const int i_wave = (r0 + 31) / d.group, i_block = (int)(((long long)tile * kRows + kRows - 1) / d.group);
@@ -633,10 +642,12 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     store_row<T, kD>((char*)d.dq + at * d.D * 2, dq, d.scale * two_to(-e), live && d.dq, d.D);
 }
 
-template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention_dkv(AttentionArgs d) {
+// Keys and values of 32 columns a wave stay in registers, rows come 64 at a time, in steps of 32. While a step's probabilities and gradients are made and summed up with its
+// rows' columns, the next step's scores are. With heads of 128 a wave has its SIMD to itself (320 registers): the order of its instructions is what keeps the units busy.
+template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : kD > 32 ? 2 : 3) k_attention_dkv(AttentionArgs d) {
     using L = Tile<kD>;
-    constexpr int kStep = 64, kTile = kStep * L::kPitch;
-    __shared__ alignas(2 * kTile) char lds[4 * kTile + 16 * kStep];        // queries, gradients, then log sums and deltas of kStep rows; two of each
+    constexpr int kStep = 64, kTile = kStep * L::kPitch, kBuffer = 2 * kTile, kBuffers = 3;
+    __shared__ alignas(16) char lds[kBuffers * (kBuffer + 8 * kStep)];     // queries and gradients of kStep rows, three of each; then their log sums and deltas
     const long long id = block_number();
     const int head = (int)(id % d.k_heads), part = (int)(id / d.k_heads % d.parts);
     const long long t_ = id / d.k_heads / d.parts;
@@ -659,70 +670,172 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     load_row<kD>(k, d.k.p + ks.start + key * d.k.row + head * d.k.head, live, d.D);
     load_row<kD>(v, d.v.p + v_start + key * d.v.row + head * d.v.head, live, d.D);
     const int e = qs.n ? gradient_exponent<T>(d) : 0;      // (without queries nothing has left it)
-    const float up = two_to(e);
+    const float up = two_to(e) * two_to(-kShift<T>);
 
-    // Row r sees key j where r >= (j - off) G: the lane's first row, the wave's first whole one, and where the block starts
+    // Row r sees key j where r >= (j - off) G: the lane's first row, the wave's first whole one, and where wave and block start
     const int rows = qs.n * d.group;
     const auto first_row = [&](int j) { return d.causal && j > off ? (j - off) * d.group : 0; };
-    const int lane_first = live ? first_row(key) : 1 << 30, wave_first = k0 + 31 < Lk ? first_row(k0 + 31) : 1 << 30, wave_start = first_row(k0);
+    const int lane_first = live ? first_row(key) : 1 << 30, wave_first = k0 + 31 < Lk ? first_row(k0 + 31) : 1 << 30;
     const int end = tile * kRows < Lk ? (rows + kStep - 1) / kStep : 0, first = end ? first_row(tile * kRows) / kStep : 0, all = end > first ? end - first : 0;
     const int start = first + (int)((long long)all * part / d.parts), stages = first + (int)((long long)all * (part + 1) / d.parts);
+    const int wave_start = k0 < Lk ? first_row(k0) / kStep : stages, own = wave_start > start ? wave_start : start;
 
     const char *qp = d.q.p + qs.start + head * d.group * d.q.head, *gp = d.d_o.p + do_start + head * d.group * d.d_o.head;
     const long long at0 = qs.row * d.q_heads + head * d.group;
     const uint32_t lds0 = lds_address(lds);
     using RowsLoad = Loads<kD, kStep>;
+    // a row's place: x rows after head g0 of a query
+    const auto place = [&](int g0, int x, long long row, long long head_) {
+        const Row r = row_at(d, 0, g0, x);
+        return (uint32_t)r.i * (uint32_t)row + (uint32_t)r.g * (uint32_t)head_;
+    };
+    const bool whole = kStep % d.group == 0;               // every stage starts with a query: its rows' places are the same each time
+    uint32_t q_off[RowsLoad::kEach], g_off[RowsLoad::kEach], sum_off;
+#pragma unroll
+    for (int i = 0; i < RowsLoad::kEach; i++) {
+        q_off[i] = place(0, RowsLoad::row(i), d.q.row, d.q.head) + RowsLoad::byte(i, d.D);
+        g_off[i] = place(0, RowsLoad::row(i), d.d_o.row, d.d_o.head) + RowsLoad::byte(i, d.D);
+    }
+    sum_off = place(0, lane, 4ll * d.q_heads, 4);
+    int to_buffer = 0;                                     // of the next load
     const auto load = [&](int s) {
         const int r0 = s * kStep, n = rows - r0, i0 = r0 / d.group, g0 = r0 - i0 * d.group;
-        const uint32_t to = lds0 + (s & 1) * kTile;
-        const auto place = [&](int r, long long row, long long head_) {
-            const Row x = row_at(d, 0, g0, r < n ? r : n - 1);
-            return (uint32_t)x.i * (uint32_t)row + (uint32_t)x.g * (uint32_t)head_;
-        };
-        RowsLoad::run(to, qp + i0 * d.q.row, [&](int i) { return place(RowsLoad::row(i), d.q.row, d.q.head) + RowsLoad::byte(i, d.D); });
-        RowsLoad::run(to + 2 * kTile, gp + i0 * d.d_o.row, [&](int i) { return place(RowsLoad::row(i), d.d_o.row, d.d_o.head) + RowsLoad::byte(i, d.D); });
-        if (wave < 2) to_lds4(lds0 + 4 * kTile + (s & 1) * 8 * kStep + 4 * kStep * wave, place(lane, 4ll * d.q_heads, 4), (const char*)((wave ? d.delta : d.lse) + at0 + (long long)i0 * d.q_heads));
+        const uint32_t to = lds0 + to_buffer * kBuffer, to_sums = lds0 + kBuffers * kBuffer + to_buffer * 8 * kStep + 4 * kStep * wave;
+        const char *qb = qp + i0 * d.q.row, *gb = gp + i0 * d.d_o.row, *sums = (const char*)((wave ? d.deltas : d.log_sums) + at0 + (long long)i0 * d.q_heads);
+        if (whole && n >= kStep) {
+            RowsLoad::run(to, qb, [&](int i) { return q_off[i]; });
+            RowsLoad::run(to + kTile, gb, [&](int i) { return g_off[i]; });
+            if (wave < 2) to_lds4(to_sums, sum_off, sums);
+        } else {                                           // past the end the last one again
+            const auto row = [&](int r) { return r < n ? r : n - 1; };
+            RowsLoad::run(to, qb, [&](int i) { return place(g0, row(RowsLoad::row(i)), d.q.row, d.q.head) + RowsLoad::byte(i, d.D); });
+            RowsLoad::run(to + kTile, gb, [&](int i) { return place(g0, row(RowsLoad::row(i)), d.d_o.row, d.d_o.head) + RowsLoad::byte(i, d.D); });
+            if (wave < 2) to_lds4(to_sums, place(g0, row(lane), 4ll * d.q_heads, 4), sums);
+        }
+        to_buffer = to_buffer == kBuffers - 1 ? 0 : to_buffer + 1;
     };
-    const Places<kD> places(lds0);
-    v16f dk[kD / 32] = {}, dv[kD / 32] = {};
-    if (start < stages) load(start);
-    for (int s = start; s < stages; s++) {
+
+    Places<kD> places(lds0);                               // rows: of the buffer of the next step; columns and sums: of this one's
+    uint32_t at_sums = lds0 + kBuffers * kBuffer + 16 * half;
+    constexpr int kScores = 2 * (kD / 16), kSums = 4 * (kD / 32), kAhead = 3;
+    constexpr bool kNext = kD > NTC_P;                     // the next step's scores are made between this one's exponentials (not where these outweigh the products: several waves take turns then)
+    const auto row_piece = [&](int j, int n) { return places.row_piece((n & 1) * kTile, 32 * j, n >> 1); };                 // queries and gradients in turn
+    const auto column_piece = [&](int j, int n) {                                                                          // gradients for dv, then queries for dk
+        const int m = n % (kSums / 2);
+        return places.column_piece(n < kSums / 2 ? kTile : 0, 32 * j + 16 * (m / (kD / 32)), m % (kD / 32));
+    };
+    typedef float v4f __attribute__((ext_vector_type(4)));
+    const auto sums_of = [&](int which, int j, int a) { return *(__attribute__((address_space(3))) const v4f*)((Shared)at_sums + (4 * kStep * which + 128 * j + 32 * a)); };
+    v16f dk[kD / 32] = {}, dv[kD / 32] = {}, x, y;         // x, y: scores and dO v of the step
+    const auto scores = [&](int j, v16f& to_x, v16f& to_y) {
+        to_x = to_y = v16f{};
+#pragma unroll
+        for (int n = 0; n < kScores; n++) {
+            if (n & 1) to_y = product<T>(row_piece(j, n), v[n >> 1], to_y);
+            else to_x = product<T>(row_piece(j, n), k[n >> 1], to_x);
+        }
+    };
+    // step j of the stage from row r0 on; the next step's rows are the places' rows from row 32 `next` on
+    const auto step = [&](int r0, auto j_, auto masks_) {
+        constexpr int j = j_.value, next = 1 - j;
+        constexpr bool kMasks = masks_.value;
+        v4u f[kAhead + 1];
+        v4f sum[4], delta[4];
+        v16f p, x2 = {}, y2 = {};
+        const int lo = lane_first - r0 - 32 * j - 4 * half, hi = rows - r0 - 32 * j - 4 * half;
+        const auto seen = [&](int r) { return result_row(r) >= lo && result_row(r) < hi; };
+        v4u pp[2], zz[2];
+        if constexpr (kNext) {
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) f[i] = row_piece(next, i);
+        } else scores(j, x, y);
+#pragma unroll
+        for (int a = 0; a < 4; a++) sum[a] = sums_of(0, j, a);
+#pragma unroll
+        for (int a = 0; a < 4; a++) delta[a] = sums_of(1, j, a);
+        if constexpr (kNext) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < kScores; n++) {
+            if (!kNext) f[(n + kAhead) % (kAhead + 1)] = n + kAhead < kScores ? v4u{} : column_piece(j, n + kAhead - kScores);
+            else if (n & 1) y2 = product<T>(f[n % (kAhead + 1)], v[n >> 1], y2);
+            else x2 = product<T>(f[n % (kAhead + 1)], k[n >> 1], x2);
+            if (kNext) f[(n + kAhead) % (kAhead + 1)] = n + kAhead < kScores ? row_piece(next, n + kAhead) : column_piece(j, n + kAhead - kScores);
+#pragma unroll
+            for (int r = 16 * n / kScores; r < 16 * (n + 1) / kScores; r++) {
+                p[r] = fast_exp2(__builtin_fmaf(x[r], d.c, -sum[r / 4][r % 4]));
+                if constexpr (kMasks) p[r] = seen(r) ? p[r] : 0.f;
+                if (r % 8 == 7) pp[r / 8] = packed<T>(p, r / 8);
+            }
+            if constexpr (kNext) __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int n = 0; n < kSums; n++) {
+            const int m = n % (kSums / 2), t = m % (kD / 32), a = m / (kD / 32);
+            if (n < kSums / 2) dv[t] = product<T>(f[(n + kScores) % (kAhead + 1)], pp[a], dv[t]);
+            else dk[t] = product<T>(f[(n + kScores) % (kAhead + 1)], zz[a], dk[t]);
+            if (n + kAhead < kSums) f[(n + kAhead + kScores) % (kAhead + 1)] = column_piece(j, n + kAhead);
+            if (n < kSums / 2) {
+#pragma unroll
+                for (int r = 16 * n / (kSums / 2); r < 16 * (n + 1) / (kSums / 2); r++) {
+                    p[r] = p[r] * __builtin_fmaf(y[r], up, -delta[r / 4][r % 4]);
+                    if constexpr (kMasks) p[r] = seen(r) ? p[r] : 0.f;
+                    if (r % 8 == 7) zz[r / 8] = packed<T>(p, r / 8);
+                }
+            }
+            if constexpr (kNext) __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (kNext) { x = x2; y = y2; }
+    };
+    int buffer = 0;
+    const auto stage = [&](int s, auto masks) {
+        using First = std::integral_constant<int, 0>;
+        using Second = std::integral_constant<int, 1>;
+        step(s * kStep, First{}, masks);
+        const int on = buffer == kBuffers - 1 ? -(kBuffers - 1) : 1;
+        if constexpr (!kNext) step(s * kStep, Second{}, masks);
+#pragma unroll
+        for (uint32_t& at : places.row) at += on * kBuffer;
+        if constexpr (kNext) step(s * kStep, Second{}, masks);
+#pragma unroll
+        for (auto& at : places.column) { at[0] += on * kBuffer; at[1] += on * kBuffer; }
+        at_sums += on * 8 * kStep;
+        buffer += on;
+    };
+    // a stage's rows are free once every wave is past it, which the next but one's barrier says: three buffers
+    const auto turn = [&](int s) {
         arrive();
-        if (s + 1 < stages) load(s + 1);
-        const int at = (s & 1) * kTile;
-        const float* sums = (const float*)(lds + 4 * kTile + (s & 1) * 8 * kStep);
-        if (s * kStep + kStep <= wave_start) continue;
+        if (s + 2 < stages) load(s + 2);
+    };
+    if (start < stages) {
+        load(start);
+        if (start + 1 < stages) load(start + 1);
+    }
+    int s = start;
+    for (; s < own && s < stages; s++) {                   // (no row of these sees a key of the wave)
+        turn(s);
+        const int on = buffer == kBuffers - 1 ? -(kBuffers - 1) : 1;
 #pragma unroll
-        for (int j = 0; j < kStep / 32; j++) {
-            const int r0 = s * kStep + 32 * j;
-            v16f x = {}, y = {};
+        for (uint32_t& at : places.row) at += on * kBuffer;
 #pragma unroll
-            for (int i = 0; i < kD / 16; i++) x = product<T>(places.row_piece(at, 32 * j, i), k[i], x);
-#pragma unroll
-            for (int i = 0; i < kD / 16; i++) y = product<T>(places.row_piece(at + 2 * kTile, 32 * j, i), v[i], y);
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int row = 32 * j + result_row(r) + 4 * half;
-                x[r] = fast_exp2(__builtin_fmaf(x[r], d.c, -__builtin_fmaf(sums[row], kLog2e, -(float)kShift<T>)));
-                y[r] = x[r] * __builtin_fmaf(y[r], up * two_to(-kShift<T>), -(sums[kStep + row] * (up * two_to(-kShift<T>))));
+        for (auto& at : places.column) { at[0] += on * kBuffer; at[1] += on * kBuffer; }
+        at_sums += on * 8 * kStep;
+        buffer += on;
+    }
+    if (s < stages) {
+        turn(s);
+        if constexpr (kNext) scores(0, x, y);
+        const int clear = (wave_first + kStep - 1) / kStep, tail = rows / kStep;          // stages from `clear` up to `tail` need no mask
+        bool arrived = true;
+        while (s < stages) {
+            for (; s < stages && (s < clear || s >= tail); s++) {
+                if (!arrived) turn(s);
+                arrived = false;
+                stage(s, std::true_type{});
             }
-            if (r0 < wave_first || r0 + 32 > rows) {
-                const int lo = lane_first - r0 - 4 * half, hi = rows - r0 - 4 * half;
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const bool seen = result_row(r) >= lo && result_row(r) < hi;
-                    x[r] = seen ? x[r] : 0.f;
-                    y[r] = seen ? y[r] : 0.f;
-                }
-            }
-#pragma unroll
-            for (int a = 0; a < 2; a++) {
-                const v4u p = packed<T>(x, a), z = packed<T>(y, a);
-#pragma unroll
-                for (int t = 0; t < kD / 32; t++) {
-                    dv[t] = product<T>(places.column_piece(at + 2 * kTile, 32 * j + 16 * a, t), p, dv[t]);
-                    dk[t] = product<T>(places.column_piece(at, 32 * j + 16 * a, t), z, dk[t]);
-                }
+            for (; s < stages && s >= clear && s < tail; s++) {
+                if (!arrived) turn(s);
+                arrived = false;
+                stage(s, std::false_type{});
             }
         }
     }
@@ -868,9 +981,9 @@ size_t ntc_op_attention_workspace(const ntc_attention_desc* d, int32_t backward)
         if (!d->q_rows) return 0;
         set_row_tiles(a);
         const int parts = forward_parts(a);
-        return parts > 1 ? (size_t)parts * d->q_rows * d->q_heads * (16 + 4 * (size_t)d->head_dim) : 0;
+        return parts > 1 ? (size_t)parts * d->q_rows * d->q_heads * (8 + 4 * (size_t)d->head_dim) : 0;
     }
-    size_t n = d->q_rows ? rounded((size_t)d->q_rows * d->q_heads * 4) + 2 * kExtents * 4 : 0;
+    size_t n = d->q_rows ? 2 * rounded((size_t)d->q_rows * d->q_heads * 4) + 2 * kExtents * 4 : 0;
     if (d->k_rows) {
         set_key_tiles(a);
         const int parts = backward_parts(a);
@@ -888,13 +1001,12 @@ int ntc_op_attention(const ntc_attention_desc* d, void* stream, char* why, size_
     a.parts = forward_parts(a);
     if (a.parts > 1) {
         if (!d->workspace) return refuse(why, cap, "null workspace");
-        a.part_stats = (float4*)d->workspace;
-        a.part_sums = (float*)(a.part_stats + (size_t)a.parts * d->q_rows * d->q_heads);
+        a.part_sums = (float*)d->workspace;
+        a.part_stats = (float2*)(a.part_sums + (size_t)a.parts * d->q_rows * d->q_heads * d->head_dim);
     }
     const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads * a.parts);
     with_head(d->dtype, d->head_dim, [&](auto t, auto h) {
-        if (a.lse) k_attention<decltype(t), h.value, true><<<grid, 256, 0, s>>>(a);
-        else k_attention<decltype(t), h.value, false><<<grid, 256, 0, s>>>(a);
+        k_attention<decltype(t), h.value><<<grid, 256, 0, s>>>(a);
         if (a.parts > 1) k_attention_join<decltype(t), h.value == 96 ? 16 : h.value / 8><<<grid_of(ceil_div(d->q_rows * d->q_heads, 4)), 256, 0, s>>>(a);
     });
     return launched(why, cap);
@@ -904,8 +1016,9 @@ int ntc_op_attention_backward(const ntc_attention_desc* d, void* stream, char* w
     if (const char* w = wrong(d, true)) return refuse(why, cap, w);
     const hipStream_t s = (hipStream_t)stream;
     AttentionArgs a = args_of(d);
-    a.delta = (float*)d->workspace;
-    a.extent = (float*)((char*)d->workspace + rounded((size_t)d->q_rows * d->q_heads * 4));
+    a.log_sums = (float*)d->workspace;
+    a.deltas = (float*)((char*)d->workspace + rounded((size_t)d->q_rows * d->q_heads * 4));
+    a.extent = (float*)((char*)a.deltas + rounded((size_t)d->q_rows * d->q_heads * 4));
     a.part_sums = d->q_rows ? a.extent + 2 * kExtents : (float*)d->workspace;
     if (d->q_rows) {
         if (d->dtype == NTC_F16) {
