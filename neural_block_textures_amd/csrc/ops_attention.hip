@@ -762,8 +762,8 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
             if (kNext) f[(n + kAhead) % (kAhead + 1)] = n + kAhead < kScores ? row_piece(next, n + kAhead) : column_piece(j, n + kAhead - kScores);
 #pragma unroll
             for (int r = 16 * n / kScores; r < 16 * (n + 1) / kScores; r++) {
-                p[r] = fast_exp2(__builtin_fmaf(x[r], d.c, -sum[r / 4][r % 4]));
-                if constexpr (kMasks) p[r] = seen(r) ? p[r] : 0.f;
+                const float exponent = __builtin_fmaf(x[r], d.c, -sum[r / 4][r % 4]);
+                p[r] = fast_exp2(!kMasks || seen(r) ? exponent : -NTC_INF);
                 if (r % 8 == 7) pp[r / 8] = packed<T>(p, r / 8);
             }
             if constexpr (kNext) __builtin_amdgcn_sched_barrier(0);
@@ -777,8 +777,8 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
             if (n < kSums / 2) {
 #pragma unroll
                 for (int r = 16 * n / (kSums / 2); r < 16 * (n + 1) / (kSums / 2); r++) {
-                    p[r] = p[r] * __builtin_fmaf(y[r], up, -delta[r / 4][r % 4]);
-                    if constexpr (kMasks) p[r] = seen(r) ? p[r] : 0.f;
+                    const float z = __builtin_fmaf(y[r], up, -delta[r / 4][r % 4]);
+                    p[r] *= !kMasks || seen(r) ? z : 0.f;
                     if (r % 8 == 7) zz[r / 8] = packed<T>(p, r / 8);
                 }
             }
