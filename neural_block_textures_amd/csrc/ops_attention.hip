@@ -100,6 +100,14 @@ __device__ __forceinline__ int keys_of(const AttentionArgs& d, const Span& k) {
     return d.k_lens ? (int)cut(d.k_lens[k.b], 0, k.n) : k.n;
 }
 
+// A block's key head, part and number of its tile: heads of a tile lie beside each other, so that eight heads' keys and values are in the caches of one of the 8 XCDs each, to which blocks are
+// dealt in turn. (In 32 bits: a division in 64 takes the scalar unit a thousand cycles, and there are several.)
+struct BlockPlace { int head, part; unsigned number; };
+__device__ __forceinline__ BlockPlace place_of(const AttentionArgs& d) {
+    const unsigned id = blockIdx.x + blockIdx.y * gridDim.x, rest = id / (unsigned)d.k_heads, number = d.parts == 1 ? rest : rest / (unsigned)d.parts;
+    return { (int)(id - rest * d.k_heads), (int)(rest - number * d.parts), number };
+}
+
 // ---------------------------------------------------------------- shared memory
 // Rows of kPitch bytes; the 16-byte piece c of row r lies at c ^ spread(r). 64 banks give 256 bytes a clock: 16 rows' pieces of one number are in different
 // banks, and so are four rows' pieces of four neighbouring numbers, which a transposing read takes from 32 lanes (both measured without conflicts; a spread over eight rows takes twice
@@ -254,12 +262,12 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
     using L = Tile<kD>;
     constexpr int kTile = kKeys * L::kPitch;
     __shared__ alignas(2 * kTile) char lds[4 * kTile];     // keys, values; two of each
-    const long long id = block_number();
-    const int head = (int)(id % d.k_heads), part = (int)(id / d.k_heads % d.parts);
-    const long long t_ = id / d.k_heads / d.parts;
-    if (t_ >= d.tiles) return;
+    const BlockPlace own_place = place_of(d);
+    const int head = own_place.head, part = own_place.part;
+    const unsigned number = own_place.number;
+    if (number >= (unsigned)d.tiles) return;
     int tile;
-    const int b = find_sequence<kRows>(d.cu_q, d.sequences, d.tiles_each, d.group, d.tiles - 1 - (int)t_, tile);   // (a sequence's last rows, which see most keys, first)
+    const int b = find_sequence<kRows>(d.cu_q, d.sequences, d.tiles_each, d.group, d.tiles - 1 - (int)number, tile);   // (a sequence's last rows, which see most keys, first)
     const Span qs = span_of(d.cu_q, d.sequences, d.q_each, d.q_rows, b, d.q);
     const long long rows = (long long)qs.n * d.group;
     if (tile < 0 || (long long)tile * kRows >= rows) return;
@@ -276,11 +284,11 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
     load_row<kD>(q, d.q.p + qs.start + row.i * d.q.row + (head * d.group + row.g) * d.q.head, live, d.D);
     const int last = d.causal ? (row.i + off < Lk - 1 ? row.i + off : Lk - 1) : Lk - 1;                           // the last key that the lane's query sees
     const int wave_first = d.causal ? (i0 + off < Lk - 1 ? i0 + off : Lk - 1) : Lk - 1;                           // ... that each of the wave's does
-    const int i_wave = (r0 + 31) / d.group, i_block = (int)(((long long)tile * kRows + kRows - 1) / d.group);
+    const int i_wave = (r0 + 31) / d.group, i_block = (tile * kRows + kRows - 1) / d.group;
     const int wave_last = d.causal ? (i_wave + off < Lk - 1 ? i_wave + off : Lk - 1) : Lk - 1;
     const int block_last = d.causal ? (i_block + off < Lk - 1 ? i_block + off : Lk - 1) : Lk - 1;
     const int all = block_last < 0 ? 0 : block_last / kKeys + 1;
-    const int begin = (int)((long long)all * part / d.parts), stages = (int)((long long)all * (part + 1) / d.parts);
+    const int begin = d.parts == 1 ? 0 : all * part / d.parts, stages = d.parts == 1 ? all : all * (part + 1) / d.parts;   // (2^24 stages at most, 64 parts)
 
     // A stage is 64 keys. While its probabilities are made and summed up with the values, the next stage's scores are: products and the exponentials between them are
     // in an order that keeps both kinds of unit busy (a wave issues in order), with operands on their way two products ahead. Keys are loaded two stages ahead, values one.
@@ -530,12 +538,12 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     constexpr int kTile = kKeys * L::kPitch;
     __shared__ alignas(2 * kTile) char lds[4 * kTile + 4 * kD];   // keys, values; two of each, and the mean
     float* const mean = (float*)(lds + 4 * kTile);
-    const long long id = block_number();
-    const int head = (int)(id % d.k_heads);
-    const long long t_ = id / d.k_heads;
-    if (t_ >= d.tiles) return;
+    const BlockPlace own_place = place_of(d);
+    const int head = own_place.head, part = own_place.part;
+    const unsigned number = own_place.number;
+    if (number >= (unsigned)d.tiles) return;
     int tile;
-    const int b = find_sequence<kRows>(d.cu_q, d.sequences, d.tiles_each, d.group, d.tiles - 1 - (int)t_, tile);
+    const int b = find_sequence<kRows>(d.cu_q, d.sequences, d.tiles_each, d.group, d.tiles - 1 - (int)number, tile);
     const Span qs = span_of(d.cu_q, d.sequences, d.q_each, d.q_rows, b, d.q);
     const long long rows = (long long)qs.n * d.group;
     if (tile < 0 || (long long)tile * kRows >= rows) return;
@@ -575,7 +583,7 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     }
     const int last = d.causal ? (row.i + off < Lk - 1 ? row.i + off : Lk - 1) : Lk - 1;
     const int wave_first = d.causal ? (i0 + off < Lk - 1 ? i0 + off : Lk - 1) : Lk - 1;
-    const int i_wave = (r0 + 31) / d.group, i_block = (int)(((long long)tile * kRows + kRows - 1) / d.group);
+    const int i_wave = (r0 + 31) / d.group, i_block = (tile * kRows + kRows - 1) / d.group;
     const int wave_last = d.causal ? (i_wave + off < Lk - 1 ? i_wave + off : Lk - 1) : Lk - 1;
     const int block_last = d.causal ? (i_block + off < Lk - 1 ? i_block + off : Lk - 1) : Lk - 1;
     const int stages = block_last < 0 ? 0 : block_last / kKeys + 1;
@@ -648,12 +656,12 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
     using L = Tile<kD>;
     constexpr int kStep = 64, kTile = kStep * L::kPitch, kBuffer = 2 * kTile, kBuffers = 3;
     __shared__ alignas(16) char lds[kBuffers * (kBuffer + 8 * kStep)];     // queries and gradients of kStep rows, three of each; then their log sums and deltas
-    const long long id = block_number();
-    const int head = (int)(id % d.k_heads), part = (int)(id / d.k_heads % d.parts);
-    const long long t_ = id / d.k_heads / d.parts;
-    if (t_ >= d.tiles) return;
+    const BlockPlace own_place = place_of(d);
+    const int head = own_place.head, part = own_place.part;
+    const unsigned number = own_place.number;
+    if (number >= (unsigned)d.tiles) return;
     int tile;
-    const int b = find_sequence<kRows>(d.cu_k, d.sequences, d.tiles_each, 1, (int)t_, tile);                      // (a sequence's first keys, which most queries see, first)
+    const int b = find_sequence<kRows>(d.cu_k, d.sequences, d.tiles_each, 1, (int)number, tile);                      // (a sequence's first keys, which most queries see, first)
     const Span ks = span_of(d.cu_k, d.sequences, d.k_each, d.k_rows, b, d.k);
     if (tile < 0 || (long long)tile * kRows >= ks.n) return;
     const bool none = b >= d.sequences;
@@ -677,7 +685,7 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
     const auto first_row = [&](int j) { return d.causal && j > off ? (j - off) * d.group : 0; };
     const int lane_first = live ? first_row(key) : 1 << 30, wave_first = k0 + 31 < Lk ? first_row(k0 + 31) : 1 << 30;
     const int end = tile * kRows < Lk ? (rows + kStep - 1) / kStep : 0, first = end ? first_row(tile * kRows) / kStep : 0, all = end > first ? end - first : 0;
-    const int start = first + (int)((long long)all * part / d.parts), stages = first + (int)((long long)all * (part + 1) / d.parts);
+    const int start = first + (d.parts == 1 ? 0 : all * part / d.parts), stages = first + (d.parts == 1 ? all : all * (part + 1) / d.parts);
     const int wave_start = k0 < Lk ? first_row(k0) / kStep : stages, own = wave_start > start ? wave_start : start;
 
     const char *qp = d.q.p + qs.start + head * d.group * d.q.head, *gp = d.d_o.p + do_start + head * d.group * d.d_o.head;
@@ -689,7 +697,8 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
         const Row r = row_at(d, 0, g0, x);
         return (uint32_t)r.i * (uint32_t)row + (uint32_t)r.g * (uint32_t)head_;
     };
-    const bool whole = kStep % d.group == 0;               // every stage starts with a query: its rows' places are the same each time
+    const int each = kStep / d.group;
+    const bool whole = each * d.group == kStep;            // every stage starts with a query: its rows' places are the same each time
     uint32_t q_off[RowsLoad::kEach], g_off[RowsLoad::kEach], sum_off;
 #pragma unroll
     for (int i = 0; i < RowsLoad::kEach; i++) {
@@ -699,7 +708,7 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
     sum_off = place(0, lane, 4ll * d.q_heads, 4);
     int to_buffer = 0;                                     // of the next load
     const auto load = [&](int s) {
-        const int r0 = s * kStep, n = rows - r0, i0 = r0 / d.group, g0 = r0 - i0 * d.group;
+        const int r0 = s * kStep, n = rows - r0, i0 = whole ? s * each : r0 / d.group, g0 = r0 - i0 * d.group;
         const uint32_t to = lds0 + to_buffer * kBuffer, to_sums = lds0 + kBuffers * kBuffer + to_buffer * 8 * kStep + 4 * kStep * wave;
         const char *qb = qp + i0 * d.q.row, *gb = gp + i0 * d.d_o.row, *sums = (const char*)((wave ? d.deltas : d.log_sums) + at0 + (long long)i0 * d.q_heads);
         if (whole && n >= kStep) {
@@ -943,6 +952,7 @@ template <class F> void with_head(int dtype, int D, F f) {
     if (dtype == NTC_BF16) go(bf16{});
     else go(f16{});
 }
+bool too_many(const AttentionArgs& a) { return (int64_t)a.tiles * a.k_heads * a.parts >= ((int64_t)1 << 31) - (1 << 22); }
 size_t rounded(size_t n) { return (n + 15) / 16 * 16; }
 
 // Parts of a sum. Without parts the longest sum holds the card up where tiles are few; with them their 32-bit results are written and read once more. In us: `each` a stage,
@@ -1004,6 +1014,7 @@ int ntc_op_attention(const ntc_attention_desc* d, void* stream, char* why, size_
         a.part_sums = (float*)d->workspace;
         a.part_stats = (float2*)(a.part_sums + (size_t)a.parts * d->q_rows * d->q_heads * d->head_dim);
     }
+    if (too_many(a)) return refuse(why, cap, "too many tiles of rows times heads: 2^31 at most");
     const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads * a.parts);
     with_head(d->dtype, d->head_dim, [&](auto t, auto h) {
         k_attention<decltype(t), h.value><<<grid, 256, 0, s>>>(a);
@@ -1020,6 +1031,13 @@ int ntc_op_attention_backward(const ntc_attention_desc* d, void* stream, char* w
     a.deltas = (float*)((char*)d->workspace + rounded((size_t)d->q_rows * d->q_heads * 4));
     a.extent = (float*)((char*)a.deltas + rounded((size_t)d->q_rows * d->q_heads * 4));
     a.part_sums = d->q_rows ? a.extent + 2 * kExtents : (float*)d->workspace;
+    set_key_tiles(a);
+    a.parts = d->q_rows && d->k_rows ? backward_parts(a) : 1;
+    const int parts = a.parts;
+    const bool keys_many = too_many(a);
+    a.parts = 1;
+    set_row_tiles(a);
+    if (keys_many || too_many(a)) return refuse(why, cap, "too many tiles of rows times heads: 2^31 at most");
     if (d->q_rows) {
         if (d->dtype == NTC_F16) {
             set_key_tiles(a);
@@ -1032,7 +1050,7 @@ int ntc_op_attention_backward(const ntc_attention_desc* d, void* stream, char* w
     }
     if (!d->k_rows || (!d->dk && !d->dv)) return 0;
     set_key_tiles(a);
-    a.parts = d->q_rows ? backward_parts(a) : 1;
+    a.parts = parts;
     const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads * a.parts);
     with_head(d->dtype, d->head_dim, [&](auto t, auto h) {
         k_attention_dkv<decltype(t), h.value><<<grid, 256, 0, s>>>(a);
