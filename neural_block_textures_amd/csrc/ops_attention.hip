@@ -533,7 +533,7 @@ template <class T> constexpr int kShift = std::is_same_v<T, f16> ? 14 : 0;      
 // A row's dS add up to 0; rounded, they do not quite, and neither where the sum dO o is that of rounded probabilities. What they add up to, times a vector that is near
 // all keys, is taken off: the error of dq is then one of the keys' differences from it, and keys with much in common keep their gradients' precision. The vector
 // is the mean of the first stage's keys, left in shared memory meanwhile.
-template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention_dq(AttentionArgs d) {
+template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 : 2) k_attention_dq(AttentionArgs d) {
     using L = Tile<kD>;
     constexpr int kTile = kKeys * L::kPitch;
     __shared__ alignas(2 * kTile) char lds[4 * kTile + 4 * kD];   // keys, values; two of each, and the mean
@@ -598,47 +598,124 @@ template <class T, int kD> __global__ void __launch_bounds__(256, 2) k_attention
     const Places<kD> places(lds0);
     v16f dq[kD / 32] = {};
     float sum = 0;
-    if (stages) load(0);
-    for (int s = 0; s < stages; s++) {
+    constexpr int kScores = 2 * (kD / 16), kSums = 2 * (kD / 32), kAhead = 3;
+    constexpr bool kBetween = kD <= 96;                    // (a wave's registers do not hold both halves of wider heads: 643 us where one after the other is 470)
+    // a stage at `at` in shared memory, in halves of 32 keys: the second half's scores are made between the first one's exponentials, the first one's sums between the second's
+    const auto stage = [&](int s, auto at_, auto masks_) {
+        constexpr int kAt = at_.value;
+        constexpr bool kMasks = masks_.value;
+        const auto row_piece = [&](int j, int n) { return places.row_piece(kAt + 2 * kTile * (n & 1), 32 * j, n >> 1); };        // keys and values in turn
+        const auto column_piece = [&](int j, int n) { return places.column_piece(kAt, 32 * j + 16 * (n / (kD / 32)), n % (kD / 32)); };
+        v4u p[2][2];
+        const int seen = last - s * kKeys - 4 * half;
+        const auto gradient = [&](const v16f& a, const v16f& c, int j, int r) {
+            const float exponent = __builtin_fmaf(a[r], d.c, -lse), z = __builtin_fmaf(c[r], up, -delta_up);
+            const bool in = !kMasks || 32 * j + result_row(r) <= seen;
+            return fast_exp2(in ? exponent : -NTC_INF) * (in ? z : 0.f);
+        };
+        // n of `of` parts of a half's gradients, two at a time
+        const auto gradients = [&](const v16f& a, const v16f& c, int j, int n, int of) {
+#pragma unroll
+            for (int r = 8 * n / of; r < 8 * (n + 1) / of; r++) {
+                const uint32_t w = pack2<T>(gradient(a, c, j, 2 * r), gradient(a, c, j, 2 * r + 1));
+                p[j][r / 4][r % 4] = w;
+                sum = add2<T>(w, sum);
+            }
+        };
+        v16f x = {}, y = {}, x2 = {}, y2 = {};
+        v4u f[kAhead + 1];
+#pragma unroll
+        for (int n = 0; n < kAhead; n++) f[n] = row_piece(0, n);
+        if constexpr (kD > 32) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < 2 * kScores; n++) {
+            const int m = n % kScores;
+            if (n < kScores) { if (m & 1) y = product<T>(f[n % (kAhead + 1)], g[m >> 1], y); else x = product<T>(f[n % (kAhead + 1)], q[m >> 1], x); }
+            else { if (m & 1) y2 = product<T>(f[n % (kAhead + 1)], g[m >> 1], y2); else x2 = product<T>(f[n % (kAhead + 1)], q[m >> 1], x2); }
+            const int k = n + kAhead;
+            f[k % (kAhead + 1)] = k < 2 * kScores ? row_piece(k / kScores, k % kScores) : column_piece(0, k - 2 * kScores);
+            if (n >= kScores) gradients(x, y, 0, m, kScores);
+            if constexpr (kD > 32) __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int n = 0; n < 2 * kSums; n++) {
+            const int j = n / kSums, m = n % kSums, t = m % (kD / 32), a = m / (kD / 32), k = n + kAhead;
+            dq[t] = product<T>(f[(n + 2 * kScores) % (kAhead + 1)], p[j][a], dq[t]);
+            if (k < 2 * kSums) f[(k + 2 * kScores) % (kAhead + 1)] = column_piece(k / kSums, k % kSums);
+            if (n < kSums) gradients(x2, y2, 1, n, kSums);
+            if constexpr (kD > 32) __builtin_amdgcn_sched_barrier(0);
+        }
+        asm volatile("" : "+v"(sum));
+    };
+    const auto step = [&](int s) {
         arrive();
         if (s + 1 < stages) load(s + 1);
-        const int at = (s & 1) * kTile;
-        if (s == 0 && wave == 0) {
+    };
+    const int full = wave_first < 0 ? 0 : (wave_first + 1) / kKeys, own = wave_last < 0 ? 0 : wave_last / kKeys + 1, own_end = own < stages ? own : stages, end = full < own_end ? full : own_end;
+    using Here = std::integral_constant<int, 0>;
+    using There = std::integral_constant<int, kTile>;
+    if (stages) {
+        load(0);
+        step(0);
+        if (wave == 0) {
             const uint32_t one = pack2<T>(1.f, 1.f);
 #pragma unroll
             for (int t = 0; t < kD / 32; t++) {
                 v16f x = {};
 #pragma unroll
-                for (int a = 0; a < kKeys / 16; a++) x = product<T>(places.column_piece(at, 16 * a, t), v4u{ one, one, one, one }, x);
+                for (int a = 0; a < kKeys / 16; a++) x = product<T>(places.column_piece(0, 16 * a, t), v4u{ one, one, one, one }, x);
 #pragma unroll
                 for (int r = 0; r < 16; r++) if (column == 0) mean[32 * t + result_row(r) + 4 * half] = x[r] * (1.f / kKeys);
             }
         }
-        if (s * kKeys > wave_last) continue;
+    }
+    int s = 0;
+    if constexpr (!kBetween) {
+        for (; s < own_end; s++) {
+            if (s) step(s);
+            const int at = (s & 1) * kTile;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int k0 = s * kKeys + 32 * j;
-            v16f x = {}, y = {};
+            for (int j = 0; j < 2; j++) {
+                v16f x = {}, y = {};
 #pragma unroll
-            for (int i = 0; i < kD / 16; i++) x = product<T>(places.row_piece(at, 32 * j, i), q[i], x);
+                for (int i = 0; i < kD / 16; i++) x = product<T>(places.row_piece(at, 32 * j, i), q[i], x);
 #pragma unroll
-            for (int i = 0; i < kD / 16; i++) y = product<T>(places.row_piece(at + 2 * kTile, 32 * j, i), g[i], y);
+                for (int i = 0; i < kD / 16; i++) y = product<T>(places.row_piece(at + 2 * kTile, 32 * j, i), g[i], y);
 #pragma unroll
-            for (int r = 0; r < 16; r++) x[r] = fast_exp2(__builtin_fmaf(x[r], d.c, -lse)) * __builtin_fmaf(y[r], up, -delta_up);
-            if (k0 + 31 > wave_first) {
-                const int seen = last - k0 - 4 * half;
+                for (int r = 0; r < 16; r++) x[r] = fast_exp2(__builtin_fmaf(x[r], d.c, -lse)) * __builtin_fmaf(y[r], up, -delta_up);
+                if (s * kKeys + 32 * j + 31 > wave_first) {
+                    const int seen = last - s * kKeys - 32 * j - 4 * half;
 #pragma unroll
-                for (int r = 0; r < 16; r++) x[r] = result_row(r) <= seen ? x[r] : 0.f;
-            }
+                    for (int r = 0; r < 16; r++) x[r] = result_row(r) <= seen ? x[r] : 0.f;
+                }
 #pragma unroll
-            for (int a = 0; a < 2; a++) {
-                const v4u p = packed<T>(x, a);
-                sum = add2<T>(p.w, add2<T>(p.z, add2<T>(p.y, add2<T>(p.x, sum))));
+                for (int a = 0; a < 2; a++) {
+                    const v4u p = packed<T>(x, a);
+                    sum = add2<T>(p.w, add2<T>(p.z, add2<T>(p.y, add2<T>(p.x, sum))));
 #pragma unroll
-                for (int t = 0; t < kD / 32; t++) dq[t] = product<T>(places.column_piece(at, 32 * j + 16 * a, t), p, dq[t]);
+                    for (int t = 0; t < kD / 32; t++) dq[t] = product<T>(places.column_piece(at, 32 * j + 16 * a, t), p, dq[t]);
+                }
             }
         }
+    } else {
+    for (; s + 1 < end; s += 2) {
+        if (s) step(s);
+        stage(s, Here{}, std::false_type{});
+        step(s + 1);
+        stage(s + 1, There{}, std::false_type{});
     }
+    if (s < end) {
+        if (s) step(s);
+        stage(s, Here{}, std::false_type{});
+        s++;
+    }
+    for (; s < own_end; s++) {
+        if (s) step(s);
+        if (s & 1) stage(s, There{}, std::true_type{});
+        else stage(s, Here{}, std::true_type{});
+    }
+    }
+    for (; s < stages; s++) if (s) step(s);
     if (stages) {
         __syncthreads();
         sum += other_half(sum);
