@@ -1,13 +1,18 @@
 """A learned prior over a trained latent's symbols: the bits an arithmetic coder would need for them.
 
     python -m neural_block_textures_amd.prior model.bin|model.ntcb [--steps 300] [--hidden 256] [--batch 16384] [--lr 2e-3]
-        [--state-bits 8|32] [--seed 1] [--fp32-latent]
+        [--state-bits 8|32] [--seed 1] [--fp32-latent] [--tile 0] [--layers 2] [--heads 8]
 
 The print statistics price a latent by the entropy of its histograms, each symbol on its own or against its left neighbour. Here
 a small network predicts each symbol from those before it in raster order (the texels to the left and above, and the
 texel's own earlier channels), trained on the very latent, and the sum of its log probabilities is the price. One JSON line a level: bits a
 symbol under the histogram and under the prior, the prior's own expectation (its entropy), and how often its first
 alternative, or one of its first four, is the symbol.
+
+With --tile T the model looks further than the neighbours: the plane is cut into tiles of T x T texels, a tile's symbols are a sequence in raster order, and blocks of
+layer norm, rotary positions (row, column, channel) and causal attention over the tile come between the contexts and the alphabet. Everything a symbol is
+predicted from still lies before it in the plane's raster order. Tiles of all sizes (those of the edges are smaller) are packed into one batch; TilePrior.step predicts
+symbols one at a time from the keys and values of those before them, as a decoder has to.
 
 A training step is the operators of ops.py end to end: layers in 8-bit floating point (fp8_linear), the symbols' log
 probabilities and their gradient (token_logprobs), and one AdamW step over all weights with an 8-bit state. The price is then
@@ -97,6 +102,133 @@ class Prior:
         return ops.fp8_linear(h, w[2]) + b[2]
 
 
+class TilePrior:
+    """A context's first layer, `layers` blocks of attention over a tile's earlier symbols and of two layers on each, and the alphabet's logits. Heads have
+    hidden / heads elements, a multiple of 8; their pairs turn with a symbol's row, column and channel."""
+
+    def __init__(self, width: int, hidden: int, alphabet: int, layers: int, heads: int, seed: int, device="cuda"):
+        if layers < 1 or heads < 1 or hidden % heads or hidden // heads % 8 or hidden // heads > 128:
+            raise ValueError(f"blocks and heads from 1 on are needed, heads of a multiple of 8 elements up to 128, not {layers} of {heads} in {hidden}")
+        gen = torch.Generator(device=device).manual_seed(seed)
+        self.heads, self.dim = heads, hidden // heads
+        pairs = self.dim // 2
+        self.sections = (pairs - pairs // 4 - (pairs - pairs // 4) // 2, (pairs - pairs // 4) // 2, pairs // 4)
+        part = lambda x: x.to(torch.bfloat16).requires_grad_(True)  # noqa: E731
+        matrix = lambda n, k, f=1.0: part(torch.randn((n, k), generator=gen, device=device) * (f * k ** -0.5))  # noqa: E731
+        ones, zeros = (lambda n: part(torch.ones(n, device=device))), (lambda n: part(torch.zeros(n, device=device)))
+        self.first, self.first_bias = matrix(hidden, width), zeros(hidden)
+        small = (2 * layers) ** -0.5                      # what a block adds, so that their sum keeps its size
+        self.blocks = [{"norm": ones(hidden), "norm_bias": zeros(hidden), "qkv": matrix(3 * hidden, hidden), "out": matrix(hidden, hidden, small),
+                        "norm2": ones(hidden), "norm2_bias": zeros(hidden), "up": matrix(2 * hidden, hidden), "up_bias": zeros(2 * hidden),
+                        "down": matrix(hidden, 2 * hidden, small)} for _ in range(layers)]
+        self.last_norm, self.last_norm_bias, self.last, self.last_bias = ones(hidden), zeros(hidden), matrix(alphabet, hidden), zeros(alphabet)
+
+    def parameters(self) -> list:
+        return [self.first, self.first_bias, *(p for b in self.blocks for p in b.values()), self.last_norm, self.last_norm_bias, self.last, self.last_bias]
+
+    def laid_out(self) -> dict:
+        """The matrices in 8 bits, for passes without gradients."""
+        return {id(p): ops.fp8_quantize(p.detach(), 128) for p in self.parameters() if p.dim() == 2}
+
+    def _pass(self, x, positions, attend, weights):
+        matrix = (lambda p: p) if weights is None else (lambda p: weights[id(p)])
+        h = torch.relu(ops.fp8_linear(x, matrix(self.first)) + self.first_bias)
+        for n, b in enumerate(self.blocks):
+            qkv = ops.fp8_linear(ops.layer_norm(h, b["norm"], b["norm_bias"]), matrix(b["qkv"])).view(len(h), 3 * self.heads, self.dim)
+            q, k = ops.rotary(positions, qkv[:, :self.heads], qkv[:, self.heads:2 * self.heads], sections=self.sections)
+            h = h + ops.fp8_linear(attend(n, q, k, qkv[:, 2 * self.heads:]).reshape(len(h), -1), matrix(b["out"]))
+            up = torch.relu(ops.fp8_linear(ops.layer_norm(h, b["norm2"], b["norm2_bias"]), matrix(b["up"])) + b["up_bias"])
+            h = h + ops.fp8_linear(up, matrix(b["down"]))
+        return ops.fp8_linear(ops.layer_norm(h, self.last_norm, self.last_norm_bias), matrix(self.last)) + self.last_bias
+
+    def logits(self, x: torch.Tensor, positions: torch.Tensor, ends: torch.Tensor, weights=None) -> torch.Tensor:
+        """[symbols, alphabet] for packed tiles: contexts [symbols, width], positions [symbols, 3], ends int32 [tiles + 1]."""
+        return self._pass(x, positions, lambda n, q, k, v: ops.attention(q, k, v, cu_q=ends, cu_k=ends), weights)
+
+    def cache(self, tiles: int, symbols: int) -> list:
+        """Room for the keys and values of `symbols` symbols of each of `tiles` tiles, for each block."""
+        room = lambda: torch.empty((tiles, symbols, self.heads, self.dim), dtype=torch.bfloat16, device=self.first.device)  # noqa: E731
+        return [(room(), room()) for _ in self.blocks]
+
+    def step(self, x: torch.Tensor, positions: torch.Tensor, cache: list, lens: torch.Tensor, weights=None) -> torch.Tensor:
+        """[tiles, alphabet] for one more symbol of each tile, the lens[i]-th (int32 [tiles]) of tile i; its keys and values go into the cache."""
+        each, at = torch.arange(len(x), device=x.device), lens.long()
+
+        def attend(n, q, k, v):
+            keys, values = cache[n]
+            keys[each, at], values[each, at] = k, v
+            return ops.attention(q[:, None], keys, values, k_lens=lens + 1)
+
+        return self._pass(x, positions, attend, weights)
+
+
+class Tiles:
+    """A plane's symbols tile by tile: their flat indices in raster order within each, and where each tile ends."""
+
+    def __init__(self, shape, tile: int, device):
+        H, W, C = shape
+        if tile < 1:
+            raise ValueError(f"tiles have 1 texel a side or more, not {tile}")
+        flat = torch.arange(H * W * C, device=device).view(H, W, C)
+        cut = [flat[y:y + tile, x:x + tile].reshape(-1) for y in range(0, H, tile) for x in range(0, W, tile)]
+        self.shape, self.order, self.lengths = shape, cut, [len(c) for c in cut]
+
+    def batch(self, which) -> tuple:
+        """(flat indices, positions [symbols, 3], ends) of some tiles, packed"""
+        at = torch.cat([self.order[i] for i in which])
+        _, W, C = self.shape
+        texel = at // C
+        ends = np.cumsum([0] + [self.lengths[i] for i in which], dtype=np.int32)
+        return at, torch.stack([texel // W, texel % W, at % C], 1), torch.from_numpy(ends).to(at.device)
+
+    def groups(self, symbols: int) -> list:
+        """All tiles, in runs of at most `symbols` symbols (one tile at least)."""
+        out, size = [[]], 0
+        for i, n in enumerate(self.lengths):
+            if out[-1] and size + n > symbols:
+                out.append([])
+                size = 0
+            out[-1].append(i)
+            size += n
+        return out
+
+
+def fit_tiles(sym: torch.Tensor, alphabet: int, tile: int, steps: int = 300, hidden: int = 256, layers: int = 2, heads: int = 8, batch: int = 16384, lr: float = 2e-3,
+              state_bits: int = 8, seed: int = 1):
+    """(TilePrior, Contexts, Tiles) trained on symbols [H, W, C] that are on the GPU, some `batch` symbols of whole tiles a step."""
+    if steps < 0 or hidden < 1 or batch < 1 or not sym.numel():
+        raise ValueError(f"steps from 0 on, hidden units and a batch from 1 on, and symbols are needed, not {steps}, {hidden}, {batch} and {list(sym.shape)}")
+    ctx, tiles = Contexts(sym, alphabet), Tiles(sym.shape, tile, sym.device)
+    prior = TilePrior(ctx.width, hidden, alphabet, layers, heads, seed, sym.device)
+    opt = ops.AdamW(prior.parameters(), lr=lr, weight_decay=0.01, state_bits=state_bits, master=True, seed=seed)
+    rng, flat = np.random.default_rng(seed), sym.reshape(-1)
+    count = min(len(tiles.lengths), max(1, batch // max(tiles.lengths)))
+    for step in range(steps):
+        at, positions, ends = tiles.batch(rng.choice(len(tiles.lengths), count, replace=False))
+        bits = ops.token_logprobs(prior.logits(ctx.rows(at), positions, ends), flat[at]).logprob
+        opt.zero_grad()
+        (-bits.mean()).backward()
+        opt.lr = lr * 0.5 * (1 + math.cos(math.pi * step / steps))
+        opt.step()
+    return prior, ctx, tiles
+
+
+@torch.no_grad()
+def step_logprobs(prior: TilePrior, ctx: Contexts, tiles: Tiles, sym: torch.Tensor, which) -> torch.Tensor:
+    """Log probabilities of the symbols of tiles of one size, [tiles, symbols], predicted one at a time as a decoder would."""
+    n = tiles.lengths[which[0]]
+    if any(tiles.lengths[i] != n for i in which):
+        raise ValueError("tiles of one size are needed")
+    at, positions, _ = tiles.batch(which)
+    at, positions = at.view(-1, n), positions.view(-1, n, 3)
+    flat, weights, cache = sym.reshape(-1), prior.laid_out(), prior.cache(len(at), n)
+    lens, out = torch.zeros(len(at), dtype=torch.int32, device=sym.device), []
+    for i in range(n):
+        out.append(ops.token_logprobs(prior.step(ctx.rows(at[:, i]), positions[:, i], cache, lens, weights), flat[at[:, i]]).logprob)
+        lens += 1
+    return torch.stack(out, 1)
+
+
 def fit(sym: torch.Tensor, alphabet: int, steps: int = 300, hidden: int = 256, batch: int = 16384, lr: float = 2e-3, state_bits: int = 8, seed: int = 1):
     """(Prior, Contexts) trained on symbols [H, W, C] that are on the GPU."""
     if steps < 0 or hidden < 1 or batch < 1 or not sym.numel():
@@ -117,14 +249,24 @@ def fit(sym: torch.Tensor, alphabet: int, steps: int = 300, hidden: int = 256, b
 
 
 @torch.no_grad()
-def price(prior: Prior, ctx: Contexts, sym: torch.Tensor, batch: int = 1 << 17) -> dict:
-    """The symbols' bits under the prior, its expectation of them, and how often its first one and four alternatives hold the symbol."""
+def price(prior, ctx: Contexts, sym: torch.Tensor, batch: int = 1 << 17, tiles: Tiles = None) -> dict:
+    """The symbols' bits under the prior (a TilePrior with its tiles), its expectation of them, and how often its first one and four alternatives hold the symbol."""
     flat, weights = sym.reshape(-1), prior.laid_out()
-    top = min(4, prior.weights[2].shape[0])
+    top = min(4, prior.parameters()[-1].numel())
     total = torch.zeros(4, dtype=torch.float64, device=sym.device)
-    for start in range(0, flat.numel(), batch):
-        at = torch.arange(start, min(start + batch, flat.numel()), device=sym.device)
-        r = ops.token_logprobs(prior.logits(ctx.rows(at), weights), flat[at], top=top)
+
+    def parts():
+        if tiles is None:
+            for start in range(0, flat.numel(), batch):
+                at = torch.arange(start, min(start + batch, flat.numel()), device=sym.device)
+                yield at, prior.logits(ctx.rows(at), weights)
+        else:
+            for which in tiles.groups(batch):
+                at, positions, ends = tiles.batch(which)
+                yield at, prior.logits(ctx.rows(at), positions, ends, weights)
+
+    for at, logits in parts():
+        r = ops.token_logprobs(logits, flat[at], top=top)
         hit = r.top_ids == flat[at, None]
         total += torch.stack([-r.logprob.double().sum(), r.entropy.double().sum(), hit[:, 0].double().sum(), hit.double().sum()])
     bits, expected, first, four = (total / flat.numel()).tolist()
@@ -141,11 +283,18 @@ def main(argv=None):
     ap.add_argument("--state-bits", type=int, default=8, choices=(8, 32))
     ap.add_argument("--seed", type=int, default=1)
     ap.add_argument("--fp32-latent", action="store_true", help="the stored values, not the post-hoc 8-bit grid (levels must be on a grid already)")
+    ap.add_argument("--tile", type=int, default=0, help="attention over tiles of this many texels a side (0: the neighbours alone)")
+    ap.add_argument("--layers", type=int, default=2, help="blocks of attention")
+    ap.add_argument("--heads", type=int, default=8)
     a = ap.parse_args(argv)
     for l, sym, alphabet in level_symbols(decode.load(a.model, q8=not a.fp32_latent)):
         dev = torch.from_numpy(sym).cuda()
-        prior, ctx = fit(dev, alphabet, a.steps, a.hidden, a.batch, a.lr, a.state_bits, a.seed)
-        out = {"level": l, "symbols": sym.size, "alphabet": alphabet, "histogram_bits": histogram_bits(sym), **price(prior, ctx, dev)}
+        tiles = None
+        if a.tile:
+            prior, ctx, tiles = fit_tiles(dev, alphabet, a.tile, a.steps, a.hidden, a.layers, a.heads, a.batch, a.lr, a.state_bits, a.seed)
+        else:
+            prior, ctx = fit(dev, alphabet, a.steps, a.hidden, a.batch, a.lr, a.state_bits, a.seed)
+        out = {"level": l, "symbols": sym.size, "alphabet": alphabet, "histogram_bits": histogram_bits(sym), **price(prior, ctx, dev, tiles=tiles)}
         out["saved"] = 1.0 - out["prior_bits"] / out["histogram_bits"] if out["histogram_bits"] else 0.0
         print(json.dumps(out), flush=True)
 

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from attention_reference import check, reference
+from tests.attention_reference import check, reference
 from neural_block_textures_amd import ops
 
 pytestmark = pytest.mark.gpu
