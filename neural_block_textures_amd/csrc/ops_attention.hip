@@ -531,13 +531,12 @@ __device__ __forceinline__ float two_to(int e) { return __uint_as_float((unsigne
 template <class T> constexpr int kShift = std::is_same_v<T, f16> ? 14 : 0;      // probabilities are held times 2^kShift
 
 // A row's dS add up to 0; rounded, they do not quite, and neither where the sum dO o is that of rounded probabilities. What they add up to, times a vector that is near
-// all keys, is taken off: the error of dq is then one of the keys' differences from it, and keys with much in common keep their gradients' precision. The vector
-// is the mean of the first stage's keys, left in shared memory meanwhile.
+// the row's keys, is taken off: the error of dq is then one of the keys' differences from it, and keys with much in common keep their gradients' precision. The vector
+// is the mean of the first stage's keys as the row weighs them (for a row that sees few keys, of all of them), and waits in dq's own place meanwhile.
 template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 : 2) k_attention_dq(AttentionArgs d) {
     using L = Tile<kD>;
     constexpr int kTile = kKeys * L::kPitch;
-    __shared__ alignas(2 * kTile) char lds[4 * kTile + 4 * kD];   // keys, values; two of each, and the mean
-    float* const mean = (float*)(lds + 4 * kTile);
+    __shared__ alignas(2 * kTile) char lds[4 * kTile];     // keys, values; two of each
     const BlockPlace own_place = place_of(d);
     const int head = own_place.head, part = own_place.part;
     const unsigned number = own_place.number;
@@ -657,16 +656,27 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
     if (stages) {
         load(0);
         step(0);
-        if (wave == 0) {
-            const uint32_t one = pack2<T>(1.f, 1.f);
+        if (own_end > 0 && d.dq) {
+            v16f x[2] = {};
+            float weight = 0;
 #pragma unroll
-            for (int t = 0; t < kD / 32; t++) {
-                v16f x = {};
+            for (int j = 0; j < 2; j++) {
 #pragma unroll
-                for (int a = 0; a < kKeys / 16; a++) x = product<T>(places.column_piece(0, 16 * a, t), v4u{ one, one, one, one }, x);
+                for (int i = 0; i < kD / 16; i++) x[j] = product<T>(places.row_piece(0, 32 * j, i), q[i], x[j]);
 #pragma unroll
-                for (int r = 0; r < 16; r++) if (column == 0) mean[32 * t + result_row(r) + 4 * half] = x[r] * (1.f / kKeys);
+                for (int r = 0; r < 16; r++) x[j][r] = fast_exp2(32 * j + result_row(r) <= last - 4 * half ? __builtin_fmaf(x[j][r], d.c, kShift<T> - lse) : -NTC_INF);
             }
+#pragma unroll
+            for (int h4 = 0; h4 < 4; h4++) {
+                const v4u w = packed<T>(x[h4 / 2], h4 & 1);
+                weight = add2<T>(w.w, add2<T>(w.z, add2<T>(w.y, add2<T>(w.x, weight))));
+#pragma unroll
+                for (int t = 0; t < kD / 32; t++) dq[t] = product<T>(places.column_piece(0, 16 * h4, t), w, dq[t]);
+            }
+            weight += other_half(weight);
+            store_row<T, kD>((char*)d.dq + at * d.D * 2, dq, weight > 0 ? 1.f / weight : 0.f, live, d.D);
+#pragma unroll
+            for (int t = 0; t < kD / 32; t++) dq[t] = v16f{};
         }
     }
     int s = 0;
@@ -716,13 +726,20 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
     }
     }
     for (; s < stages; s++) if (s) step(s);
-    if (stages) {
-        __syncthreads();
+    if (own_end > 0 && d.dq && live) {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");             // (the vector was written by other lanes of the wave)
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
         sum += other_half(sum);
+        typedef T v4 __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (int t = 0; t < kD / 32; t++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) dq[t][r] = __builtin_fmaf(-sum, mean[32 * t + result_row(r) + 4 * half], dq[t][r]);
+            for (int a = 0; a < 4; a++) {
+                const int col = 32 * t + 8 * a + 4 * half;
+                const v4 near = col < d.D ? *(const v4*)((const char*)d.dq + (at * d.D + col) * 2) : v4{};
+#pragma unroll
+                for (int i = 0; i < 4; i++) dq[t][4 * a + i] = __builtin_fmaf(-sum, (float)near[i], dq[t][4 * a + i]);
+            }
     }
     store_row<T, kD>((char*)d.dq + at * d.D * 2, dq, d.scale * two_to(-e), live && d.dq, d.D);
 }

@@ -4,7 +4,7 @@ With u = 2^-24, h half a step of the type, A = |q||k|^T scale: a score is a 32-b
 2 e relative and, rounded, by h. o is sum p v / sum p over rounded p, off by (2 h + 4 e) sum p|v| and its rounding. lse is that of the rounded sum, off by h, and probabilities backward by as much: dv (2 h + 4 e) sum p|dO|. dO v is off by (D + 1) u |dO||v|, the sum dO o by what o before its rounding is (with 2 h^2 |o| from
 that of what it left), and by (D + 1) u |dO||o|:
 dS by p times these and (2 h + 4 e)|dS|; dk by the sums of these with |q|, dq with |k| + |c|: it is sum dS k - (sum dS) c, the
-second 0 but for these errors, with c the mean of the first 64 keys (fewer: the last again). 32-bit sums over n rows or keys add n u of the sum of magnitudes. A value below the type's smallest normal one is off by half of its smallest step:
+second 0 but for these errors, with c a mean of the first 64 keys, as large as their largest at most. 32-bit sums over n rows or keys add n u of the sum of magnitudes. A value below the type's smallest normal one is off by half of its smallest step:
 float16's is 2^-25 of a row's largest probability forward, which is at most the row's sum (o: 2^-25 sum |v|); backward probabilities are held times 2^14 (dv: 2^-39 sum |dO|) and dS times the power of two 2^e that keeps
 B = 2 D max|dO| max|v| within 2^15: 2^e > 2^14 / B, half a step 2^-25 / 2^e < B 2^-39 (dq: scale B 2^-39 sum |k| over the keys it sees, dk alike with |q|). bfloat16 has float32's range."""
 import torch
@@ -54,7 +54,7 @@ def reference(q, k, v, do, spans, causal=True, scale=None):
             out["dv"][0][k0:k1, e] += p.T @ g
             out["dv"][1][k0:k1, e] += (p * (2 * h + 4 * err + (n * G + 8) * U)).T @ g.abs() + (2.0 ** -39 * (seen.double().T @ g.abs()) if narrow else 0)
             out["dq"][0][q0:q1, head] = scale * ds @ b
-            c = b[torch.arange(64, device="cuda").clamp_max(m - 1)].mean(0).abs()
+            c = b[:64].abs().amax(0)
             out["dq"][1][q0:q1, head] = scale * (e_ds + m * U * ds.abs()) @ (b.abs() + c)
             out["dk"][0][k0:k1, e] += scale * ds.T @ a
             out["dk"][1][k0:k1, e] += scale * (e_ds + n * G * U * ds.abs()).T @ a.abs()
