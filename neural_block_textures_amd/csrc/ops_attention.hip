@@ -197,6 +197,8 @@ template <int kD, int kTile> struct RowLoads : Loads<kD, kTile> {
 #pragma unroll
         for (int i = 0; i < B::kEach; i++) off[i] = (uint32_t)B::row(i) * (uint32_t)stride + B::byte(i, D);
     }
+    // load i of a whole tile
+    __device__ __forceinline__ void piece(uint32_t to, const char* base, int i) const { to_lds16(to + 1024 * (uniform(threadIdx.x >> 6) * B::kEach + i), off[i], base); }
     __device__ __forceinline__ void load(uint32_t to, const char* base, int n) const {
         if (n >= kTile) B::run(to, base, [&](int i) { return off[i]; });
         else B::run(to, base, [&](int i) { const int r = B::row(i); return (uint32_t)(r < n ? r : n - 1) * (uint32_t)stride + B::byte(i, D); });
@@ -297,6 +299,7 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
     const RowLoads<kD, kKeys> key_loads(d.k.row, d.D), value_loads(d.v.row, d.D);
     const auto load_keys = [&](int s) { key_loads.load(lds0 + ((s - begin) & 1) * kTile, kp + (long long)s * kKeys * d.k.row, Lk - s * kKeys); };
     const auto load_values = [&](int s) { value_loads.load(lds0 + (2 + ((s - begin) & 1)) * kTile, vp + (long long)s * kKeys * d.v.row, Lk - s * kKeys); };
+    constexpr int kPieces = 2 * Loads<kD, kKeys>::kEach;   // of both tiles' loads that a stage issues, between its first products where the tiles are whole
     constexpr int kScores = 2 * (kD / 16), kSums = 4 * (kD / 32), kAhead = kD <= 32 ? 2 : kD <= 64 ? 3 : 4;      // products of a stage, and how many operands come ahead of theirs
     const int full = wave_first < 0 ? 0 : (wave_first + 1) / kKeys;        // stages whose keys all of the wave's queries see
     const int own = wave_last < 0 ? 0 : wave_last / kKeys + 1, own_end = own < stages ? own : stages;
@@ -309,8 +312,9 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
     // l: the sum of the probabilities as they are rounded, so that what rounding does to all values alike is in the products and in what they are divided by. (lse takes it too: it is off by
     // half a step at most, a probability's own rounding, and by that over the root of the keys as a rule.)
     float m = -NTC_INF, l = 0, most = -NTC_INF;
-    const auto stage = [&](int s, v16f (&x)[2], v16f (&z)[2], auto key_at_, auto value_at_, auto masks_, auto more_) {
+    const auto stage = [&](int s, v16f (&x)[2], v16f (&z)[2], auto key_at_, auto value_at_, auto masks_, auto more_, auto loads_) {
         constexpr bool kMasks = masks_.value, kMore = more_.value;         // of the next stage, whose scores z will be: they are masked, it is there
+        constexpr bool kLoads = loads_.value;                              // the loads are this stage's own
         constexpr int kKeyAt = key_at_.value, kValueAt = value_at_.value;  // where the next stage's keys and this one's values are, from their places
         v4u f[kAhead + 1];
         if constexpr (kMore) {
@@ -327,6 +331,11 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
             for (int t = 0; t < kD / 32; t++) o[t] *= by;
         }
         const float mc = m == -NTC_INF ? 0.f : m * d.c;
+        const char *key_base = nullptr, *value_base = nullptr;
+        if constexpr (kLoads) {
+            key_base = kp + (long long)(s + 2) * kKeys * d.k.row;
+            value_base = vp + (long long)(s + 1) * kKeys * d.v.row;
+        }
         uint32_t p[16];
         constexpr int kFirst = 10;                         // pairs of exponentials that lie between the next scores' products; the others lie between the sums'
         const auto exponentials = [&](int e) {             // of a pair
@@ -341,6 +350,13 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
             for (int n = 0; n < kScores; n++) {
                 z[n & 1] = product<T>(f[n % (kAhead + 1)], q[n >> 1], z[n & 1]);
                 f[(n + kAhead) % (kAhead + 1)] = n + kAhead < kScores ? key_piece(kKeyAt, n + kAhead) : value_piece(kValueAt, n + kAhead - kScores);
+                if constexpr (kLoads) {                    // (keys where this stage's were, values where the last one's)
+#pragma unroll
+                    for (int i = kPieces * n / kScores; i < kPieces * (n + 1) / kScores; i++) {
+                        if (i % 2 == 0) key_loads.piece(lds0 + kValueAt, key_base, i / 2);
+                        else value_loads.piece(lds0 + 2 * kTile + kTile - kValueAt, value_base, i / 2);
+                    }
+                }
 #pragma unroll
                 for (int e = kFirst * n / kScores; e < kFirst * (n + 1) / kScores; e++) exponentials(e);
                 __builtin_amdgcn_sched_barrier(0);
@@ -407,16 +423,23 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
     constexpr std::false_type no{};
     int s = begin;
     const int end = full < own_end ? full : own_end;
+    const int whole = Lk / kKeys < stages ? Lk / kKeys : stages;
+    for (; s + 2 < end && s + 3 < whole; s += 2) {
+        arrive();
+        stage(s, even, odd, There{}, Here{}, no, yes, yes);
+        arrive();
+        stage(s + 1, odd, even, Here{}, There{}, no, yes, yes);
+    }
     for (; s + 2 < end; s += 2) {
         step(s);
-        stage(s, even, odd, There{}, Here{}, no, yes);
+        stage(s, even, odd, There{}, Here{}, no, yes, no);
         step(s + 1);
-        stage(s + 1, odd, even, Here{}, There{}, no, yes);
+        stage(s + 1, odd, even, Here{}, There{}, no, yes, no);
     }
     places.toggle_rows(kTile);
-    if (s + 1 < end) { step(s); stage(s, even, odd, Here{}, Here{}, no, yes); turn(); s++; }
-    for (; s + 1 < own_end; s++) { step(s); stage(s, even, odd, Here{}, Here{}, yes, yes); turn(); }
-    if (s < own_end) { step(s); stage(s, even, odd, Here{}, Here{}, no, no); s++; }
+    if (s + 1 < end) { step(s); stage(s, even, odd, Here{}, Here{}, no, yes, no); turn(); s++; }
+    for (; s + 1 < own_end; s++) { step(s); stage(s, even, odd, Here{}, Here{}, yes, yes, no); turn(); }
+    if (s < own_end) { step(s); stage(s, even, odd, Here{}, Here{}, no, no, no); s++; }
     for (; s < stages; s++) step(s);
     l += other_half(l);
     const long long at = (qs.row + row.i) * d.q_heads + head * d.group + row.g;
@@ -838,10 +861,21 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
             else to_x = product<T>(row_piece(j, n), k[n >> 1], to_x);
         }
     };
+    constexpr int kPieces = 2 * RowsLoad::kEach;           // loads of a stage, which the first step of one issues between its products where it can
     // step j of the stage from row r0 on; the next step's rows are the places' rows from row 32 `next` on
-    const auto step = [&](int r0, auto j_, auto masks_) {
+    const auto step = [&](int r0, auto j_, auto masks_, auto loads_) {
         constexpr int j = j_.value, next = 1 - j;
-        constexpr bool kMasks = masks_.value;
+        constexpr bool kMasks = masks_.value, kLoads = loads_.value;
+        uint32_t to = 0;
+        const char *qb = nullptr, *gb = nullptr;
+        if constexpr (kLoads) {
+            const int i0 = (r0 / kStep + 2) * each;
+            to = lds0 + to_buffer * kBuffer + 1024 * (wave * RowsLoad::kEach);
+            qb = qp + i0 * d.q.row;
+            gb = gp + i0 * d.d_o.row;
+            if (wave < 2) to_lds4(lds0 + kBuffers * kBuffer + to_buffer * 8 * kStep + 4 * kStep * wave, sum_off, (const char*)((wave ? d.deltas : d.log_sums) + at0 + (long long)i0 * d.q_heads));
+            to_buffer = to_buffer == kBuffers - 1 ? 0 : to_buffer + 1;
+        }
         v4u f[kAhead + 1];
         v4f sum[4], delta[4];
         v16f p, x2 = {}, y2 = {};
@@ -863,6 +897,13 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
             else if (n & 1) y2 = product<T>(f[n % (kAhead + 1)], v[n >> 1], y2);
             else x2 = product<T>(f[n % (kAhead + 1)], k[n >> 1], x2);
             if (kNext) f[(n + kAhead) % (kAhead + 1)] = n + kAhead < kScores ? row_piece(next, n + kAhead) : column_piece(j, n + kAhead - kScores);
+            if constexpr (kLoads) {
+#pragma unroll
+                for (int i = kPieces * n / kScores; i < kPieces * (n + 1) / kScores; i++) {
+                    if (i % 2 == 0) to_lds16(to + 1024 * (i / 2), q_off[i / 2], qb);
+                    else to_lds16(to + kTile + 1024 * (i / 2), g_off[i / 2], gb);
+                }
+            }
 #pragma unroll
             for (int r = 16 * n / kScores; r < 16 * (n + 1) / kScores; r++) {
                 const float exponent = __builtin_fmaf(x[r], d.c, -sum[r / 4][r % 4]);
@@ -890,15 +931,15 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
         if constexpr (kNext) { x = x2; y = y2; }
     };
     int buffer = 0;
-    const auto stage = [&](int s, auto masks) {
+    const auto stage = [&](int s, auto masks, auto loads) {
         using First = std::integral_constant<int, 0>;
         using Second = std::integral_constant<int, 1>;
-        step(s * kStep, First{}, masks);
+        step(s * kStep, First{}, masks, loads);
         const int on = buffer == kBuffers - 1 ? -(kBuffers - 1) : 1;
-        if constexpr (!kNext) step(s * kStep, Second{}, masks);
+        if constexpr (!kNext) step(s * kStep, Second{}, masks, std::false_type{});
 #pragma unroll
         for (uint32_t& at : places.row) at += on * kBuffer;
-        if constexpr (kNext) step(s * kStep, Second{}, masks);
+        if constexpr (kNext) step(s * kStep, Second{}, masks, std::false_type{});
 #pragma unroll
         for (auto& at : places.column) { at[0] += on * kBuffer; at[1] += on * kBuffer; }
         at_sums += on * 8 * kStep;
@@ -933,12 +974,19 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
             for (; s < stages && (s < clear || s >= tail); s++) {
                 if (!arrived) turn(s);
                 arrived = false;
-                stage(s, std::true_type{});
+                stage(s, std::true_type{}, std::false_type{});
+            }
+            if (whole && kNext) {
+                if (arrived && s + 2 < stages && s >= clear && s + 2 < tail) { stage(s, std::false_type{}, std::false_type{}); s++; arrived = false; }
+                for (; s + 2 < stages && s >= clear && s + 2 < tail; s++) {
+                    arrive();
+                    stage(s, std::false_type{}, std::true_type{});
+                }
             }
             for (; s < stages && s >= clear && s < tail; s++) {
                 if (!arrived) turn(s);
                 arrived = false;
-                stage(s, std::false_type{});
+                stage(s, std::false_type{}, std::false_type{});
             }
         }
     }
