@@ -561,7 +561,7 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
     constexpr int kTile = kKeys * L::kPitch;
     __shared__ alignas(2 * kTile) char lds[4 * kTile];     // keys, values; two of each
     const BlockPlace own_place = place_of(d);
-    const int head = own_place.head, part = own_place.part;
+    const int head = own_place.head;
     const unsigned number = own_place.number;
     if (number >= (unsigned)d.tiles) return;
     int tile;
@@ -1097,26 +1097,28 @@ template <class F> void with_head(int dtype, int D, F f) {
 bool too_many(const AttentionArgs& a) { return (int64_t)a.tiles * a.k_heads * a.parts >= ((int64_t)1 << 31) - (1 << 22); }
 size_t rounded(size_t n) { return (n + 15) / 16 * 16; }
 
-// Parts of a sum. Without parts the longest sum holds the card up where tiles are few; with them their 32-bit results are written and read once more. In us: `each` a stage,
-// two blocks to a compute unit at a time, stages of all blocks (half of them where causal and long on both sides) spread over these and then the longest block's own; 5 for the second launch, 4 TB/s for what the parts write and read.
-int parts_of(int64_t blocks, int64_t stages, float each, bool half, int64_t part_bytes) {
+// Parts of a sum. Without them the longest block's sum holds the card up where blocks are few; with them their 32-bit results are written and read once more. In us: `each` a
+// stage where `slots` blocks are on the card at once (a quarter less where they are not), a stage and a half to begin a block, blocks of avg stages spread over the slots; 5 for
+// the second launch, 4.5 TB/s for what the parts write and read. 8192 rows of 16 heads of 128 on 4, keys' and values' gradients: 864 us in one part, 646 in two, 667 in four, 755 in eight;
+// 16 tokens against caches of 900 to 8192 rows: 186 in one, 71 in four to sixteen, 79 in 32.
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int parts_of(int64_t blocks, int64_t stages, float slots, float each, bool half, int64_t part_bytes) {
     int best = 1;
     float least = 0;
     for (int p = 1; p <= 64 && p <= stages; p *= 2) {
-        const float busy = (float)blocks * stages / 512 * (half ? 0.5f : 1.f), longest = (float)((stages + p - 1) / p);
-        const float cost = each * (busy > longest ? busy + 0.5f * longest : longest + 0.5f * busy) + (p > 1 ? 5.f + 2.f * p * part_bytes / 4e6f : 0.f);
+        const float busy = (float)blocks * (stages * (half ? 0.5f : 1.f) + 1.5f * p) / slots, longest = 0.75f * ((float)ceil_div(stages, p) + 1.5f);
+        const float cost = each * (busy > longest ? busy : longest) + (p > 1 ? 5.f + 2.f * p * part_bytes / 4.5e6f : 0.f);
         if (p == 1 || cost < least) { best = p; least = cost; }
     }
     return best;
 }
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int forward_parts(const AttentionArgs& a) {
     const int64_t keys = a.sequences ? ceil_div(a.k_rows, a.sequences) : 0, queries = a.sequences ? a.q_rows / a.sequences : 0;
-    return parts_of((int64_t)a.tiles * a.k_heads, ceil_div(keys, kKeys), 0.4f + 0.006f * a.D, a.causal && 2 * queries > keys, a.q_rows * a.q_heads * a.D * 4);
+    return parts_of((int64_t)a.tiles * a.k_heads, ceil_div(keys, kKeys), a.D <= 32 ? 1024 : a.D <= 64 ? 768 : 512, a.D <= 64 ? 2.7f : 2.2f, a.causal && 2 * queries > keys, a.q_rows * a.q_heads * a.D * 4);
 }
 int backward_parts(const AttentionArgs& a) {
     const int64_t keys = a.sequences ? ceil_div(a.k_rows, a.sequences) : 0, queries = a.sequences ? a.q_rows / a.sequences : 0;
-    return parts_of((int64_t)a.tiles * a.k_heads, ceil_div(queries * a.group, 64), 0.5f + 0.015f * a.D, a.causal && 2 * keys > queries, a.k_rows * a.k_heads * a.D * 8);
+    return parts_of((int64_t)a.tiles * a.k_heads, ceil_div(queries * a.group, 64), a.D <= 32 ? 768 : a.D <= 64 ? 512 : 256, a.D <= 64 ? 3.f : 2.4f, a.causal && 2 * keys > queries, a.k_rows * a.k_heads * a.D * 8);
 }
 
 }  // namespace
