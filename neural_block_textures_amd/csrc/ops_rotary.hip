@@ -69,6 +69,7 @@ template <class T, int kRun, bool kBeside, class P> __global__ void __launch_bou
     using W = PieceOf<T, kRun>;
     const auto load = [](const T* p) { return __builtin_bit_cast(R, *(const W*)p); };
     const auto store = [](T* p, const R& r) { *(W*)p = __builtin_bit_cast(W, r); };
+    const int rest = d.head_dim - 2 * d.pairs;
     constexpr int kBatch = 4;                              // runs whose loads are on their way together
     R lo[kBatch], hi[kBatch];
     T* to[kBatch];
@@ -79,12 +80,18 @@ template <class T, int kRun, bool kBeside, class P> __global__ void __launch_bou
             const int i = i0 + 256 * n, row = quotient(i, d.unit_magic), unit = i - row * d.units, t = quotient(row, d.head_magic), own = row - t * d.block_heads;
             const int which = h0 + own >= d.heads[0], h = which ? h0 + own - d.heads[0] : h0 + own;
             const bool turned = unit < d.turned_units;
-            const int at = turned ? unit * kRun : 2 * d.pairs + (unit - d.turned_units) * kRun;
-            angle[n] = i >= items || own >= heads ? -2 : turned ? t * d.pairs + unit * kPairs : -1;
+            // the last run of what is turned, and of the rest, ends where these do: it lies over the one before it where they are no multiple of it (what both write is the same)
+            const int pair = unit * kPairs < d.pairs - kPairs ? unit * kPairs : d.pairs - kPairs, beyond = (unit - d.turned_units) * kRun, room = rest > kRun ? rest - kRun : 0;
+            const int at = turned ? (kBeside ? 2 * pair : pair) : 2 * d.pairs + (beyond < room ? beyond : room);
+            angle[n] = i >= items || own >= heads ? -2 : turned ? t * d.pairs + pair : -1;
             to[n] = (T*)d.y[which] + ((first + t) * d.heads[which] + h) * d.head_dim + at;
             if (angle[n] == -2) continue;
             const T* x = (const T*)d.x[which] + (first + t) * d.token_stride[which] + h * d.head_stride[which] + at;
-            lo[n] = load(x);
+            if (turned || rest >= kRun) lo[n] = load(x);
+            else {
+#pragma unroll
+                for (int k = 0; k < kRun; k++) lo[n].v[k] = k < rest ? x[k] : (T)0.f;
+            }
             if (!kBeside && turned) hi[n] = load(x + d.pairs);
         }
     };
@@ -102,7 +109,14 @@ template <class T, int kRun, bool kBeside, class P> __global__ void __launch_bou
 #pragma unroll
         for (int n = 0; n < kBatch; n++) {
             if (angle[n] == -2) continue;
-            if (angle[n] == -1) { store(to[n], lo[n]); continue; }
+            if (angle[n] == -1) {
+                if (rest >= kRun) store(to[n], lo[n]);
+                else {
+#pragma unroll
+                    for (int k = 0; k < kRun; k++) if (k < rest) to[n][k] = lo[n].v[k];
+                }
+                continue;
+            }
             float c[kPairs], s[kPairs];
 #pragma unroll
             for (int k = 0; k < kPairs; k++) { c[k] = cosines[angle[n] + k]; s[k] = sines[angle[n] + k]; }
@@ -171,12 +185,13 @@ extern "C" int ntc_op_rotary(const ntc_rotary_desc* d, void* stream, char* why, 
             a.axis[p] = m;
         }
     }
-    // The widest access, up to 16 bytes, that divides what is turned and what is not. (Rows may start at any element.)
+    // The widest access, up to 16 bytes, that what is turned holds. (Rows may start at any element.)
     int run = 16 / (int)type_size(d->dtype);
-    while ((d->interleaved ? 2 * a.pairs : a.pairs) % run || (d->head_dim - 2 * a.pairs) % run) run /= 2;
-    const bool beside = d->interleaved != 0;                   // (runs have 2 elements at least then: heads are even)
-    a.turned_units = d->interleaved ? 2 * a.pairs / run : a.pairs / run;
-    a.units = a.turned_units + (d->head_dim - 2 * a.pairs) / run;
+    const bool beside = d->interleaved != 0;                   // (pairs in one run)
+    while (run > (beside ? 2 * a.pairs : a.pairs)) run /= 2;
+    const int run_pairs = beside ? run / 2 : run;
+    a.turned_units = (a.pairs + run_pairs - 1) / run_pairs;
+    a.units = a.turned_units + (d->head_dim - 2 * a.pairs + run - 1) / run;
     // Tokens of a block: as many as give each thread four runs, where the table holds them; heads of one token in several blocks where tokens are few.
     const auto magic = [](int n) { return n > 1 ? (unsigned)((((uint64_t)1 << 32) + n - 1) / n) : 0u; };
     constexpr int kItems = 1024;

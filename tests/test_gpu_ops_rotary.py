@@ -49,7 +49,9 @@ def randn(seed, *shape):
 @pytest.mark.parametrize("N,Hq,Hk,D,sections,one_ladder,interleaved", [
     (1, 32, 8, 128, (16, 24, 24), True, False), (1, 1, 1, 2, (1,), False, True), (257, 3, 1, 64, (32,), False, False), (100, 4, 2, 80, (8, 16, 16), False, True),
     (63, 5, 5, 6, (1, 1), True, False), (40, 2, 1, 34, (3, 0, 5), False, False), (40, 2, 1, 34, (3, 0, 5), False, True), (9, 2, 2, 256, (128,), True, True), (2000, 8, 8, 32, (6, 6, 4), False, False),
-    (30, 2, 2, 24, (1, 1, 1, 1, 1, 1, 1, 1), False, False), (11, 1, 3, 70, (11, 13), True, False), (5000, 2, 0, 64, (8, 8), False, True)])
+    (30, 2, 2, 24, (1, 1, 1, 1, 1, 1, 1, 1), False, False), (11, 1, 3, 70, (11, 13), True, False), (5000, 2, 0, 64, (8, 8), False, True),
+    (300, 4, 2, 80, (4, 2, 3), True, False), (300, 4, 2, 80, (4, 2, 3), True, True), (50, 3, 1, 128, (20, 20, 23), False, False), (50, 3, 1, 128, (20, 20, 23), False, True), (20, 2, 2, 26, (3,), False, False),
+    (20, 2, 2, 18, (8,), False, False), (20, 2, 2, 18, (8,), False, True)])
 def test_sizes(N, Hq, Hk, D, sections, one_ladder, interleaved, dtype):
     print("rotary", N, Hq, Hk, D, sections, dtype, flush=True)
     t = TYPES[dtype]
