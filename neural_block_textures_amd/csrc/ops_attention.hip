@@ -12,9 +12,6 @@
 // (values or keys, transposed) comes from LDS by the transposing read, four keys of a column at a time. The keys' and values' gradients go the same way with
 // queries and keys exchanged. No score leaves a register.
 #include "ops_common.hpp"
-#ifndef NTC_P
-#define NTC_P 32
-#endif
 
 namespace ntc_ops {
 namespace {
@@ -59,8 +56,9 @@ struct AttentionArgs {
     int sequences, q_each, k_each;     // rows of a sequence where there are no ends
     int q_heads, k_heads, group, D, causal;
     unsigned group_magic;              // ceil(2^32 / group): x / group is the high word of the product with it where x group < 2^32; 0 for 1
-    int parts;                         // of a sequence's keys (backward: of its rows), joined by a second launch; their sums:
-    float* part_sums;                  // forward [parts][q_rows][q_heads][D]; backward dk's [parts][k_rows][k_heads][D], then dv's
+    int parts;                         // of a sequence's keys (dk and dv: of its rows), joined by a second launch; their sums:
+    float* part_sums;                  // forward [parts][q_rows][q_heads][D]; backward dk's [parts][k_rows][k_heads][D], then dv's; dq's [parts][q_rows][q_heads][D], then part_rests
+    float* part_rests;                 // [parts][q_rows][q_heads]: what the rounded dS add up to
     float2* part_stats;                // forward [parts][q_rows][q_heads]: m c and the sum of probabilities
     int tiles, tiles_each;             // tiles of rows (or keys) in all, and of each sequence where there are no ends
     float scale, c;                    // c: scale log2 e
@@ -556,12 +554,12 @@ template <class T> constexpr int kShift = std::is_same_v<T, f16> ? 14 : 0;      
 // A row's dS add up to 0; rounded, they do not quite, and neither where the sum dO o is that of rounded probabilities. What they add up to, times a vector that is near
 // the row's keys, is taken off: the error of dq is then one of the keys' differences from it, and keys with much in common keep their gradients' precision. The vector
 // is the mean of the first stage's keys as the row weighs them (for a row that sees few keys, of all of them), and waits in dq's own place meanwhile.
-template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 : 2) k_attention_dq(AttentionArgs d) {
+template <class T, int kD, bool kParts> __global__ void __launch_bounds__(256, kD <= 32 ? 4 : 2) k_attention_dq(AttentionArgs d) {
     using L = Tile<kD>;
     constexpr int kTile = kKeys * L::kPitch;
     __shared__ alignas(2 * kTile) char lds[4 * kTile];     // keys, values; two of each
     const BlockPlace own_place = place_of(d);
-    const int head = own_place.head;
+    const int head = own_place.head, part = kParts ? own_place.part : 0;
     const unsigned number = own_place.number;
     if (number >= (unsigned)d.tiles) return;
     int tile;
@@ -599,23 +597,24 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
     delta += other_half(delta);
     const int e = gradient_exponent<T>(d);
     const float up = two_to(e), lse = live ? d.lse[at] * kLog2e : 0.f, delta_up = delta * up;
-    if (live && half == 0) {                               // as the keys' and values' gradients take them
+    if (live && half == 0 && part == 0) {                               // as the keys' and values' gradients take them
         d.log_sums[at] = lse - kShift<T>;
         d.deltas[at] = delta_up * two_to(-kShift<T>);
     }
-    const int last = d.causal ? (row.i + off < Lk - 1 ? row.i + off : Lk - 1) : Lk - 1;
-    const int wave_first = d.causal ? (i0 + off < Lk - 1 ? i0 + off : Lk - 1) : Lk - 1;
     const int i_wave = (r0 + 31) / d.group, i_block = (tile * kRows + kRows - 1) / d.group;
-    const int wave_last = d.causal ? (i_wave + off < Lk - 1 ? i_wave + off : Lk - 1) : Lk - 1;
     const int block_last = d.causal ? (i_block + off < Lk - 1 ? i_block + off : Lk - 1) : Lk - 1;
-    const int stages = block_last < 0 ? 0 : block_last / kKeys + 1;
+    const int all_stages = block_last < 0 || !d.dq ? 0 : block_last / kKeys + 1, each_stages = kParts ? (all_stages + d.parts - 1) / d.parts : all_stages;
+    const int from = kParts ? min(part * each_stages, all_stages) : 0, stages = min(each_stages, all_stages - from), base = from * kKeys;
+    // (the part's first key is number 0 from here on)
+    const int Lp = Lk - base, top = Lp - 1, last = d.causal ? min(row.i + off - base, top) : top;
+    const int wave_first = d.causal ? min(i0 + off - base, top) : top, wave_last = d.causal ? min(i_wave + off - base, top) : top;
 
-    const char *kp = d.k.p + ks.start + head * d.k.head, *vp = d.v.p + v_start + head * d.v.head;
+    const char *kp = d.k.p + ks.start + head * d.k.head + (long long)base * d.k.row, *vp = d.v.p + v_start + head * d.v.head + (long long)base * d.v.row;
     const uint32_t lds0 = lds_address(lds);
     const RowLoads<kD, kKeys> key_loads(d.k.row, d.D), value_loads(d.v.row, d.D);
     const auto load = [&](int s) {
-        key_loads.load(lds0 + (s & 1) * kTile, kp + (long long)s * kKeys * d.k.row, Lk - s * kKeys);
-        value_loads.load(lds0 + (2 + (s & 1)) * kTile, vp + (long long)s * kKeys * d.v.row, Lk - s * kKeys);
+        key_loads.load(lds0 + (s & 1) * kTile, kp + (long long)s * kKeys * d.k.row, Lp - s * kKeys);
+        value_loads.load(lds0 + (2 + (s & 1)) * kTile, vp + (long long)s * kKeys * d.v.row, Lp - s * kKeys);
     };
     const Places<kD> places(lds0);
     v16f dq[kD / 32] = {};
@@ -679,7 +678,7 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
     if (stages) {
         load(0);
         step(0);
-        if (own_end > 0 && d.dq) {
+        if (own_end > 0 && part == 0) {
             v16f x[2] = {};
             float weight = 0;
 #pragma unroll
@@ -731,28 +730,35 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
             }
         }
     } else {
-    for (; s + 1 < end; s += 2) {
-        if (s) step(s);
-        stage(s, Here{}, std::false_type{});
-        step(s + 1);
-        stage(s + 1, There{}, std::false_type{});
-    }
-    if (s < end) {
-        if (s) step(s);
-        stage(s, Here{}, std::false_type{});
-        s++;
-    }
-    for (; s < own_end; s++) {
-        if (s) step(s);
-        if (s & 1) stage(s, There{}, std::true_type{});
-        else stage(s, Here{}, std::true_type{});
-    }
+        for (; s + 1 < end; s += 2) {
+            if (s) step(s);
+            stage(s, Here{}, std::false_type{});
+            step(s + 1);
+            stage(s + 1, There{}, std::false_type{});
+        }
+        if (s < end) {
+            if (s) step(s);
+            stage(s, Here{}, std::false_type{});
+            s++;
+        }
+        for (; s < own_end; s++) {
+            if (s) step(s);
+            if (s & 1) stage(s, There{}, std::true_type{});
+            else stage(s, Here{}, std::true_type{});
+        }
     }
     for (; s < stages; s++) if (s) step(s);
-    if (own_end > 0 && d.dq && live) {
+    sum += other_half(sum);
+    if (kParts) {
+        const long long all = d.q_rows * d.q_heads;
+        store_floats<kD>(d.part_sums + (part * all + at) * d.D, dq, live, d.D);
+        if (live && half == 0) d.part_rests[part * all + at] = sum;
+        if (own_end == 0 && part == 0) store_row<T, kD>((char*)d.dq + at * d.D * 2, dq, 0.f, live, d.D);
+        return;
+    }
+    if (own_end > 0 && live) {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");             // (the vector was written by other lanes of the wave)
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-        sum += other_half(sum);
         typedef T v4 __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (int t = 0; t < kD / 32; t++)
@@ -765,6 +771,30 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
             }
     }
     store_row<T, kD>((char*)d.dq + at * d.D * 2, dq, d.scale * two_to(-e), live && d.dq, d.D);
+}
+
+// The parts of dq added up, and what the vector near the keys takes off: eight columns to a thread.
+template <class T> __global__ void __launch_bounds__(256) k_attention_dq_join(AttentionArgs d) {
+    const long long rows = d.q_rows * d.q_heads, n = rows * d.D / 8, x = block_number() * 256 + threadIdx.x;
+    const float f = d.scale * two_to(-gradient_exponent<T>(d));
+    if (x >= n) return;
+    const long long row = x / (d.D / 8);
+    char* to = (char*)d.dq + 16 * x;
+    float sum[8] = {}, rest = 0;
+#pragma unroll 4
+    for (int p = 0; p < d.parts; p++) {
+        const float4 *of = (const float4*)(d.part_sums + 8 * (p * n + x)), a = of[0], b = of[1];
+        const float v[8] = { a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w };
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum[i] += v[i];
+        rest += d.part_rests[p * rows + row];
+    }
+    typedef T v8 __attribute__((ext_vector_type(8)));
+    const v8 near = *(const v8*)to;
+    uint32_t out[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) out[i] = pack2<T>(__builtin_fmaf(-rest, (float)near[2 * i], sum[2 * i]) * f, __builtin_fmaf(-rest, (float)near[2 * i + 1], sum[2 * i + 1]) * f);
+    *(v4u*)to = v4u{ out[0], out[1], out[2], out[3] };
 }
 
 // Keys and values of 32 columns a wave stay in registers, rows come 64 at a time, in steps of 32. While a step's probabilities and gradients are made and summed up with its
@@ -844,7 +874,7 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
     Places<kD> places(lds0);                               // rows: of the buffer of the next step; columns and sums: of this one's
     uint32_t at_sums = lds0 + kBuffers * kBuffer + 16 * half;
     constexpr int kScores = 2 * (kD / 16), kSums = 4 * (kD / 32), kAhead = 3;
-    constexpr bool kNext = kD > NTC_P;                     // the next step's scores are made between this one's exponentials (not where these outweigh the products: several waves take turns then)
+    constexpr bool kNext = kD > 32;                     // the next step's scores are made between this one's exponentials (not where these outweigh the products: several waves take turns then)
     const auto row_piece = [&](int j, int n) { return places.row_piece((n & 1) * kTile, 32 * j, n >> 1); };                 // queries and gradients in turn
     const auto column_piece = [&](int j, int n) {                                                                          // gradients for dv, then queries for dk
         const int m = n % (kSums / 2);
@@ -1098,16 +1128,17 @@ bool too_many(const AttentionArgs& a) { return (int64_t)a.tiles * a.k_heads * a.
 size_t rounded(size_t n) { return (n + 15) / 16 * 16; }
 
 // Parts of a sum. Without them the longest block's sum holds the card up where blocks are few; with them their 32-bit results are written and read once more. In us: `each` a
-// stage where `slots` blocks are on the card at once (a quarter less where they are not), a stage and a half to begin a block, blocks of avg stages spread over the slots; 5 for
-// the second launch, 4.5 TB/s for what the parts write and read. 8192 rows of 16 heads of 128 on 4, keys' and values' gradients: 864 us in one part, 646 in two, 667 in four, 755 in eight;
-// 16 tokens against caches of 900 to 8192 rows: 186 in one, 71 in four to sixteen, 79 in 32.
+// stage where `slots` blocks are on the card at once (a quarter less where they are not), a stage and a half to begin a block, blocks of avg stages spread over the slots; `join` for
+// the second launch (queries' gradients: 10 with what their parts hold twice), 4.5 TB/s for what the parts write and read. 8192 rows of 16 heads of 128 on 4, keys' and values' gradients: 864 us in one part, 646 in two, 667 in four, 755 in eight;
+// 16 tokens against caches of 900 to 8192 rows: 186 in one, 71 in four to sixteen, 79 in 32; queries'
+// gradients of 1 to 27 rows of 16 heads on 4 by 10 times 10200 to 12000 keys, all with both directions: 553 in one, 300 in parts; of ragged rows whose sums are 20 stages, 36 in one and 40 in two.
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-int parts_of(int64_t blocks, int64_t stages, float slots, float each, bool half, int64_t part_bytes) {
+int parts_of(int64_t blocks, int64_t stages, float slots, float each, bool half, int64_t part_bytes, float join = 5) {
     int best = 1;
     float least = 0;
     for (int p = 1; p <= 64 && p <= stages; p *= 2) {
         const float busy = (float)blocks * (stages * (half ? 0.5f : 1.f) + 1.5f * p) / slots, longest = 0.75f * ((float)ceil_div(stages, p) + 1.5f);
-        const float cost = each * (busy > longest ? busy : longest) + (p > 1 ? 5.f + 2.f * p * part_bytes / 4.5e6f : 0.f);
+        const float cost = each * (busy > longest ? busy : longest) + (p > 1 ? join + 2.f * p * part_bytes / 4.5e6f : 0.f);
         if (p == 1 || cost < least) { best = p; least = cost; }
     }
     return best;
@@ -1115,6 +1146,10 @@ int parts_of(int64_t blocks, int64_t stages, float slots, float each, bool half,
 int forward_parts(const AttentionArgs& a) {
     const int64_t keys = a.sequences ? ceil_div(a.k_rows, a.sequences) : 0, queries = a.sequences ? a.q_rows / a.sequences : 0;
     return parts_of((int64_t)a.tiles * a.k_heads, ceil_div(keys, kKeys), a.D <= 32 ? 1024 : a.D <= 64 ? 768 : 512, a.D <= 64 ? 2.7f : 2.2f, a.causal && 2 * queries > keys, a.q_rows * a.q_heads * a.D * 4);
+}
+int query_parts(const AttentionArgs& a) {
+    const int64_t keys = a.sequences ? ceil_div(a.k_rows, a.sequences) : 0, queries = a.sequences ? a.q_rows / a.sequences : 0;
+    return parts_of((int64_t)a.tiles * a.k_heads, ceil_div(keys, kKeys), a.D <= 32 ? 1024 : 512, a.D <= 64 ? 3.f : 3.6f, a.causal && 2 * queries > keys, a.q_rows * a.q_heads * a.D * 4, 10);
 }
 int backward_parts(const AttentionArgs& a) {
     const int64_t keys = a.sequences ? ceil_div(a.k_rows, a.sequences) : 0, queries = a.sequences ? a.q_rows / a.sequences : 0;
@@ -1137,13 +1172,15 @@ size_t ntc_op_attention_workspace(const ntc_attention_desc* d, int32_t backward)
         const int parts = forward_parts(a);
         return parts > 1 ? (size_t)parts * d->q_rows * d->q_heads * (8 + 4 * (size_t)d->head_dim) : 0;
     }
-    size_t n = d->q_rows ? 2 * rounded((size_t)d->q_rows * d->q_heads * 4) + 2 * kExtents * 4 : 0;
-    if (d->k_rows) {
+    const size_t n = d->q_rows ? 2 * rounded((size_t)d->q_rows * d->q_heads * 4) + 2 * kExtents * 4 : 0;
+    size_t of_parts = 0;                                   // (dq's are joined before dk's and dv's are made)
+    if (d->q_rows && d->k_rows) {
+        set_row_tiles(a);
+        if (const int parts = query_parts(a); parts > 1) of_parts = (size_t)parts * d->q_rows * d->q_heads * 4 * (d->head_dim + 1);
         set_key_tiles(a);
-        const int parts = backward_parts(a);
-        if (parts > 1) n += (size_t)parts * d->k_rows * d->k_heads * d->head_dim * 8;
+        if (const int parts = backward_parts(a); parts > 1) of_parts = std::max(of_parts, (size_t)parts * d->k_rows * d->k_heads * d->head_dim * 8);
     }
-    return n;
+    return n + of_parts;
 }
 
 int ntc_op_attention(const ntc_attention_desc* d, void* stream, char* why, size_t cap) {
@@ -1179,8 +1216,10 @@ int ntc_op_attention_backward(const ntc_attention_desc* d, void* stream, char* w
     a.parts = d->q_rows && d->k_rows ? backward_parts(a) : 1;
     const int parts = a.parts;
     const bool keys_many = too_many(a);
-    a.parts = 1;
     set_row_tiles(a);
+    const int q_parts = d->q_rows && d->k_rows && d->dq ? query_parts(a) : 1;
+    a.parts = q_parts;
+    a.part_rests = a.part_sums + (size_t)q_parts * d->q_rows * d->q_heads * d->head_dim;
     if (keys_many || too_many(a)) return refuse(why, cap, "too many tiles of rows times heads: 2^31 at most");
     if (d->q_rows) {
         if (d->dtype == NTC_F16) {
@@ -1188,8 +1227,12 @@ int ntc_op_attention_backward(const ntc_attention_desc* d, void* stream, char* w
             k_attention_extent<f16><<<kExtents, 256, 0, s>>>(a);
         }
         set_row_tiles(a);
-        const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads);
-        with_head(d->dtype, d->head_dim, [&](auto t, auto h) { k_attention_dq<decltype(t), h.value><<<grid, 256, 0, s>>>(a); });
+        const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads * a.parts);
+        with_head(d->dtype, d->head_dim, [&](auto t, auto h) {
+            if (a.parts == 1) { k_attention_dq<decltype(t), h.value, false><<<grid, 256, 0, s>>>(a); return; }
+            k_attention_dq<decltype(t), h.value, true><<<grid, 256, 0, s>>>(a);
+            k_attention_dq_join<decltype(t)><<<grid_of(ceil_div(d->q_rows * d->q_heads * (d->head_dim / 8), 256)), 256, 0, s>>>(a);
+        });
         if (const int rc = launched(why, cap)) return rc;
     }
     if (!d->k_rows || (!d->dk && !d->dv)) return 0;
