@@ -206,7 +206,7 @@ typedef struct ntc_rotary_desc {
     const void* x[2];
     void* y[2];
     int64_t token_stride[2], head_stride[2];
-    int32_t heads[2];                      /* 0: no such tensor */
+    int32_t heads[2];                      /* 0: no such tensor; 2^28 elements a token at most */
     int32_t head_dim, axes, position_bytes, dtype, one_ladder, interleaved, backward;
     int32_t sections[NTC_ROTARY_AXES];
     double base;

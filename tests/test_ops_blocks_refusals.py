@@ -76,7 +76,7 @@ def rotary(sections=(4,), **kw):
 @pytest.mark.parametrize("sections,kw,reason", [((4,), {"tokens": -1}, "tokens and heads"), ((4,), {"head_dim": 15}, "even number"), ((4,), {"head_dim": 0}, "even number"), ((4,), {"axes": 0}, "1 to 8 axes"),
                                                 ((4,), {"axes": 9}, "1 to 8 axes"), ((9,), {}, "pairs"), ((0,), {}, "pairs"), ((-1, 3), {}, "0 pairs or more"), ((64, 65), {"head_dim": 512}, "128 pairs"),
                                                 ((4,), {"base": 0.9}, "base"), ((4,), {"base": float("nan")}, "base"), ((4,), {"base": float("inf")}, "base"), ((4,), {"dtype": 3}, "values are"),
-                                                ((4,), {"position_bytes": 2}, "4 or 8"), ((4,), {"positions": None}, "null")])
+                                                ((4,), {"position_bytes": 2}, "4 or 8"), ((4,), {"heads": (1 << 14, 1), "head_dim": 1 << 14}, "2^28 elements"), ((4,), {"positions": None}, "null")])
 def test_rotary_refusals(sections, kw, reason):
     rc, why = refused(O.library().ntc_op_rotary, rotary(sections, **kw))
     assert rc == 1 and reason in why, why
