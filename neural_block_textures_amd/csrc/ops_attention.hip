@@ -504,32 +504,39 @@ template <class T, int kPieces> __global__ void __launch_bounds__(256) k_attenti
 template <class T> __global__ void __launch_bounds__(256) k_attention_extent(AttentionArgs d) {
     __shared__ float parts[2][4];
     float of_v = 0, of_do = 0;
-    const int pieces = d.D / 8;
-    const auto largest = [&](const char* p, float& to) {
+    const unsigned pieces = d.D / 8;
+    // of n rows that begin at `p`, all their heads: four loads of each thread on their way together
+    const auto largest = [&](const char* p, int n, const Operand3& of, unsigned heads, float& to) {
         typedef T v8 __attribute__((ext_vector_type(8)));
-        const v8 x = *(const v8*)p;
+        const unsigned all = n * heads * pieces;
+        for (unsigned x0 = threadIdx.x; x0 < all; x0 += 1024) {
+            v8 x[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) to = __builtin_fmaxf(to, __builtin_fabsf((float)x[i]));
+            for (int k = 0; k < 4; k++) {
+                const unsigned own = x0 + 256 * k < all ? x0 + 256 * k : x0, y = own / pieces, r = y / heads;
+                x[k] = *(const v8*)(p + r * of.row + (y - r * heads) * of.head + (own - y * pieces) * 16);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) to = __builtin_fmaxf(to, __builtin_fabsf((float)x[k][i]));
+        }
     };
     for (int t = blockIdx.x; t < d.tiles; t += gridDim.x) {
         int tile;
         const int b = find_sequence<kRows>(d.cu_k, d.sequences, d.tiles_each, 1, t, tile);
         if (b >= d.sequences) continue;
         const Span ks = span_of(d.cu_k, d.sequences, d.k_each, d.k_rows, b, d.v);
-        const int first = tile * kRows, n = tile < 0 ? 0 : keys_of(d, ks) - first;
-        const int all = (n < kRows ? n : kRows) * d.k_heads * pieces;
-        for (int x = threadIdx.x; x < all; x += 256) {
-            const int piece = x % pieces, y = x / pieces, h = y % d.k_heads, r = y / d.k_heads;
-            largest(d.v.p + ks.start + (first + r) * d.v.row + h * d.v.head + piece * 16, of_v);
-        }
+        const int n = tile < 0 ? 0 : keys_of(d, ks) - tile * kRows;
+        if (n > 0) largest(d.v.p + ks.start + (long long)tile * kRows * d.v.row, n < kRows ? n : kRows, d.v, d.k_heads, of_v);
     }
-    const long long rows = d.cu_q ? cut(d.cu_q[d.sequences], 0, d.q_rows) : d.q_rows, all = rows * d.q_heads * pieces;
-    for (long long x = blockIdx.x * 256ll + threadIdx.x; x < all; x += gridDim.x * 256ll) {
-        const int piece = (int)(x % pieces);
-        const long long y = x / pieces, r = y / d.q_heads;
-        const int h = (int)(y % d.q_heads);
-        const long long start = d.cu_q ? r * d.d_o.row : r / d.q_each * d.d_o.batch + r % d.q_each * d.d_o.row;
-        largest(d.d_o.p + start + h * d.d_o.head + piece * 16, of_do);
+    // (from the last block on: the first ones may have had keys)
+    constexpr int kChunk = 32;
+    const int rows = (int)(d.cu_q ? cut(d.cu_q[d.sequences], 0, d.q_rows) : d.q_each), chunks = (rows + kChunk - 1) / kChunk;
+    const long long all_chunks = d.cu_q ? chunks : (long long)chunks * d.sequences;
+    for (long long t = gridDim.x - 1 - blockIdx.x; t < all_chunks; t += gridDim.x) {
+        const int b = d.cu_q ? 0 : (int)(t / chunks), first = (int)(t - (long long)b * chunks) * kChunk;
+        largest(d.d_o.p + b * d.d_o.batch + first * d.d_o.row, rows - first < kChunk ? rows - first : kChunk, d.d_o, d.q_heads, of_do);
     }
     const auto most = [](float a, float b) { return __builtin_fmaxf(a, b); };
     of_v = reduce64(of_v, most);
