@@ -60,6 +60,7 @@ struct AttentionArgs {
     float* part_sums;                  // forward [parts][q_rows][q_heads][D]; backward dk's [parts][k_rows][k_heads][D], then dv's; dq's [parts][q_rows][q_heads][D], then part_rests
     float* part_rests;                 // [parts][q_rows][q_heads]: what the rounded dS add up to
     float2* part_stats;                // forward [parts][q_rows][q_heads]: m c and the sum of probabilities
+    int line_heads;                    // log2 of how many heads share a line of the cache (128 bytes)
     int tiles, tiles_each;             // tiles of rows (or keys) in all, and of each sequence where there are no ends
     float scale, c;                    // c: scale log2 e
 };
@@ -99,10 +100,11 @@ __device__ __forceinline__ int keys_of(const AttentionArgs& d, const Span& k) {
 }
 
 // A block's key head, part and number of its tile: heads of a tile lie beside each other, so that eight heads' keys and values are in the caches of one of the 8 XCDs each, to which blocks are
-// dealt in turn. (In 32 bits: a division in 64 takes the scalar unit a thousand cycles, and there are several.)
+// dealt in turn; heads that share a line of the cache are on one XCD (64 sequences of 600 to 1024, 8 heads of 32, both ways: 262 us, with neighbours on different ones 271). (In 32 bits: a division in 64 takes the scalar unit a thousand cycles, and there are several.)
 struct BlockPlace { int head, part; unsigned number; };
 __device__ __forceinline__ BlockPlace place_of(const AttentionArgs& d) {
-    const unsigned id = blockIdx.x + blockIdx.y * gridDim.x, rest = id / (unsigned)d.k_heads, number = d.parts == 1 ? rest : rest / (unsigned)d.parts;
+    const unsigned dealt = blockIdx.x + blockIdx.y * gridDim.x, set = (8u << d.line_heads) - 1;
+    const unsigned id = (dealt & ~set) | (dealt & 7) << d.line_heads | (dealt & set) >> 3, rest = id / (unsigned)d.k_heads, number = d.parts == 1 ? rest : rest / (unsigned)d.parts;
     return { (int)(id - rest * d.k_heads), (int)(rest - number * d.parts), number };
 }
 
@@ -1116,6 +1118,7 @@ AttentionArgs args_of(const ntc_attention_desc* d) {
     a.q_heads = d->q_heads; a.k_heads = d->k_heads; a.group = d->q_heads / d->k_heads; a.D = d->head_dim; a.causal = d->causal != 0;
     a.group_magic = a.group > 1 ? (unsigned)((((uint64_t)1 << 32) + a.group - 1) / a.group) : 0;
     a.parts = 1;
+    a.line_heads = a.k_heads % 4 == 0 && a.D <= 16 ? 2 : a.k_heads % 2 == 0 && a.D <= 32 ? 1 : 0;
     a.scale = d->scale;
     a.c = d->scale * kLog2e;
     return a;
@@ -1138,6 +1141,8 @@ template <class F> void with_head(int dtype, int D, F f) {
     else go(f16{});
 }
 bool too_many(const AttentionArgs& a) { return (int64_t)a.tiles * a.k_heads * a.parts >= ((int64_t)1 << 31) - (1 << 22); }
+// (whole sets of 8 << line_heads blocks)
+dim3 grid_for(const AttentionArgs& a) { const int64_t set = 8 << a.line_heads; return grid_of(((int64_t)a.tiles * a.k_heads * a.parts + set - 1) / set * set); }
 size_t rounded(size_t n) { return (n + 15) / 16 * 16; }
 
 // Parts of a sum. Without them the longest block's sum holds the card up where blocks are few; with them their 32-bit results are written and read once more. In us: `each` a
@@ -1209,7 +1214,7 @@ int ntc_op_attention(const ntc_attention_desc* d, void* stream, char* why, size_
         a.part_stats = (float2*)(a.part_sums + (size_t)a.parts * d->q_rows * d->q_heads * d->head_dim);
     }
     if (too_many(a)) return refuse(why, cap, "too many tiles of rows times heads: 2^31 at most");
-    const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads * a.parts);
+    const dim3 grid = grid_for(a);
     with_head(d->dtype, d->head_dim, [&](auto t, auto h) {
         k_attention<decltype(t), h.value><<<grid, 256, 0, s>>>(a);
         if (a.parts > 1) k_attention_join<decltype(t), h.value == 96 ? 16 : h.value / 8><<<grid_of(ceil_div(d->q_rows * d->q_heads, 4)), 256, 0, s>>>(a);
@@ -1240,7 +1245,7 @@ int ntc_op_attention_backward(const ntc_attention_desc* d, void* stream, char* w
             k_attention_extent<f16><<<kExtents, 256, 0, s>>>(a);
         }
         set_row_tiles(a);
-        const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads * a.parts);
+        const dim3 grid = grid_for(a);
         with_head(d->dtype, d->head_dim, [&](auto t, auto h) {
             if (a.parts == 1) { k_attention_dq<decltype(t), h.value, false><<<grid, 256, 0, s>>>(a); return; }
             k_attention_dq<decltype(t), h.value, true><<<grid, 256, 0, s>>>(a);
@@ -1251,7 +1256,7 @@ int ntc_op_attention_backward(const ntc_attention_desc* d, void* stream, char* w
     if (!d->k_rows || (!d->dk && !d->dv)) return 0;
     set_key_tiles(a);
     a.parts = parts;
-    const dim3 grid = grid_of((int64_t)a.tiles * a.k_heads * a.parts);
+    const dim3 grid = grid_for(a);
     with_head(d->dtype, d->head_dim, [&](auto t, auto h) {
         k_attention_dkv<decltype(t), h.value><<<grid, 256, 0, s>>>(a);
         if (a.parts > 1) k_attention_sum<decltype(t)><<<grid_of(ceil_div(d->k_rows * d->k_heads * (d->head_dim / 4), 256)), 256, 0, s>>>(a);
