@@ -421,7 +421,7 @@ int ntc_op_layer_norm(const ntc_layer_norm_desc* d, void* stream, char* why, siz
     with_type(d->dtype, [&](auto t) {
         using T = decltype(t);
         const int64_t n = p.lanes ? ceil_div(a.rows, groups_of(p)) : a.rows;
-        const unsigned grid = (unsigned)ceil_div(n, ceil_div(n, p.waves > 4 ? 1024 : 3072));     // as many as the card holds at once, each with as many rows
+        const unsigned grid = (unsigned)ceil_div(n, ceil_div(n, 256 * (p.waves > 4 ? 4 : 12)));     // as many blocks as the 256 compute units hold at once, each with as many rows
         if (!p.lanes) k_norm_wide<T><<<grid, kWide, 0, s>>>(a);
         else with_shape<T>(p, [&](auto shape, auto l, auto w, auto v) { k_norm<T, l.value, w.value, v.value><<<grid, decltype(shape)::kThreads, 0, s>>>(a); });
     });
