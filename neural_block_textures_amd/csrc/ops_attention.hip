@@ -567,7 +567,7 @@ template <class T> constexpr int kShift = std::is_same_v<T, f16> ? 14 : 0;      
 // A row's dS add up to 0; rounded, they do not quite, and neither where the sum dO o is that of rounded probabilities. What they add up to, times a vector that is near
 // the row's keys, is taken off: the error of dq is then one of the keys' differences from it, and keys with much in common keep their gradients' precision. The vector
 // is the mean of the first stage's keys as the row weighs them (for a row that sees few keys, of all of them), and waits in dq's own place meanwhile.
-// Rows as forward; three products for each key and row. 8192 tokens of 16 heads on 4 of 128, causal: 460 to 530 us, 780 to 900 TFLOP/s.
+// Rows as forward; three products for each key and row. 8192 tokens of 16 heads on 4 of 128, causal: 460 to 560 us, 740 to 900 TFLOP/s (the clock that a card's power leaves).
 template <class T, int kD, bool kParts> __global__ void __launch_bounds__(256, kD <= 32 ? 4 : 2) k_attention_dq(AttentionArgs d) {
     using L = Tile<kD>;
     constexpr int kTile = kKeys * L::kPitch;
@@ -634,7 +634,7 @@ template <class T, int kD, bool kParts> __global__ void __launch_bounds__(256, k
     v16f dq[kD / 32] = {};
     float sum = 0;
     constexpr int kScores = 2 * (kD / 16), kSums = 2 * (kD / 32), kAhead = 3;
-    constexpr bool kBetween = kD <= 96;                    // (a wave's registers do not hold both halves of wider heads: 643 us where one after the other is 470)
+    constexpr bool kBetween = kD <= 96;                    // (a wave's registers do not hold both halves of wider heads: 643 us where one after the other is 470; one wave to a SIMD, which has them, 595 where that is 560)
     // a stage at `at` in shared memory, in halves of 32 keys: the second half's scores are made between the first one's exponentials, the first one's sums between the second's
     const auto stage = [&](int s, auto at_, auto masks_) {
         constexpr int kAt = at_.value;
