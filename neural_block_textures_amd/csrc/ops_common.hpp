@@ -77,8 +77,11 @@ template <class V, class F> __device__ __forceinline__ V reduce_rows(V x, F f) {
 }
 
 // ---------------------------------------------------------------- launches
-// A grid of n blocks and a block's number in it: a dimension's threads have to stay below 2^32. (Numbers may pass n.)
-inline dim3 grid_of(int64_t n) { return n <= 1 << 22 ? dim3((unsigned)n) : dim3(1u << 22, (unsigned)((n + (1 << 22) - 1) >> 22)); }
+// A grid of n blocks of `threads` and a block's number in it: a dimension's threads have to stay below 2^32. (Numbers may pass n.)
+inline dim3 grid_of(int64_t n, int threads = 256) {
+    const int64_t most = (1 << 30) / threads;
+    return n <= most ? dim3((unsigned)n) : dim3((unsigned)most, (unsigned)((n + most - 1) / most));
+}
 __device__ __forceinline__ long long block_number() { return blockIdx.x + (long long)blockIdx.y * gridDim.x; }
 
 // ---------------------------------------------------------------- refusals

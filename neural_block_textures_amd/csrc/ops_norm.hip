@@ -329,7 +329,7 @@ template <class T> __global__ void __launch_bounds__(256) k_norm_wide_columns(No
 // dw and db from the blocks' sums: 32 columns to a block, 32 threads to a column.
 template <class W> __global__ void __launch_bounds__(1024) k_norm_join(const float* parts, int blocks, int C, W* dw, W* db) {
     __shared__ float part[32][33];
-    const unsigned c = blockIdx.x * 32 + (threadIdx.x & 31), all = 2u * C, k = threadIdx.x >> 5;
+    const unsigned c = (unsigned)block_number() * 32 + (threadIdx.x & 31), all = 2u * C, k = threadIdx.x >> 5;
     float sum = 0;
     if (c < all)
 #pragma unroll 8
@@ -455,7 +455,7 @@ int ntc_op_layer_norm_backward(const ntc_layer_norm_desc* d, void* stream, char*
     if (!sums) return 0;
     with_type(d->weight_type, [&](auto t) {
         using W = decltype(t);
-        k_norm_join<W><<<(unsigned)((2 * d->C + 31) / 32), 1024, 0, s>>>(a.parts, (int)(d->rows ? blocks : 0), a.C, (W*)d->dweight, (W*)d->dbias);
+        k_norm_join<W><<<grid_of((2 * d->C + 31) / 32, 1024), 1024, 0, s>>>(a.parts, (int)(d->rows ? blocks : 0), a.C, (W*)d->dweight, (W*)d->dbias);
     });
     return launched(why, cap);
 }
