@@ -446,6 +446,10 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
     if (s < own_end) { step(s); stage(s, even, odd, Here{}, Here{}, no, no, no); s++; }
     for (; s < stages; s++) step(s);
     l += other_half(l);
+    if (last < begin * kKeys) {                            // (sees none of these: whatever keys and values of other rows hold, which probabilities of 0 multiply)
+#pragma unroll
+        for (int t = 0; t < kD / 32; t++) o[t] = v16f{};
+    }
     const long long at = (qs.row + row.i) * d.q_heads + head * d.group + row.g;
     if (d.parts > 1) {
         const long long own = (long long)part * d.q_rows * d.q_heads + at;
@@ -633,6 +637,12 @@ template <class T, int kD, bool kParts> __global__ void __launch_bounds__(256, k
     const Places<kD> places(lds0);
     v16f dq[kD / 32] = {};
     float sum = 0;
+    const auto none = [&] {                                // (a row that sees no key of these: as forward)
+        if (last < 0) {
+#pragma unroll
+            for (int t = 0; t < kD / 32; t++) dq[t] = v16f{};
+        }
+    };
     constexpr int kScores = 2 * (kD / 16), kSums = 2 * (kD / 32), kAhead = 3;
     constexpr bool kBetween = kD <= 96;                    // (a wave's registers do not hold both halves of wider heads: 643 us where one after the other is 470; one wave to a SIMD, which has them, 595 where that is 560)
     // a stage at `at` in shared memory, in halves of 32 keys: the second half's scores are made between the first one's exponentials, the first one's sums between the second's
@@ -710,6 +720,7 @@ template <class T, int kD, bool kParts> __global__ void __launch_bounds__(256, k
                 for (int t = 0; t < kD / 32; t++) dq[t] = product<T>(places.column_piece(0, 16 * h4, t), w, dq[t]);
             }
             weight += other_half(weight);
+            none();
             store_row<T, kD>((char*)d.dq + at * d.D * 2, dq, weight > 0 ? 1.f / weight : 0.f, live, d.D);
 #pragma unroll
             for (int t = 0; t < kD / 32; t++) dq[t] = v16f{};
@@ -763,6 +774,7 @@ template <class T, int kD, bool kParts> __global__ void __launch_bounds__(256, k
     }
     for (; s < stages; s++) if (s) step(s);
     sum += other_half(sum);
+    none();
     if (kParts) {
         const long long all = d.q_rows * d.q_heads;
         store_floats<kD>(d.part_sums + (part * all + at) * d.D, dq, live, d.D);
