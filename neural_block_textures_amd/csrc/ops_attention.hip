@@ -59,7 +59,7 @@ struct AttentionArgs {
     int parts;                         // of a sequence's keys (dk and dv: of its rows), joined by a second launch; their sums:
     float* part_sums;                  // forward [parts][q_rows][q_heads][D]; backward dk's [parts][k_rows][k_heads][D], then dv's; dq's [parts][q_rows][q_heads][D], then part_rests
     float* part_rests;                 // [parts][q_rows][q_heads]: what the rounded dS add up to
-    float2* part_stats;                // forward [parts][q_rows][q_heads]: m c and the sum of probabilities
+    float2* part_stats;                // forward [parts][q_rows][q_heads]: m c and the sum of probabilities (-1: of keys whose scores are all -inf)
     int line_heads;                    // log2 of how many heads share a line of the cache (128 bytes)
     int tiles, tiles_each;             // tiles of rows (or keys) in all, and of each sequence where there are no ends
     float scale, c;                    // c: scale log2 e
@@ -450,17 +450,20 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
 #pragma unroll
         for (int t = 0; t < kD / 32; t++) o[t] = v16f{};
     }
+    // A row that sees no key has a sum of 0, and so has one whose scores are all -inf: that one is NaN, as its softmax is. (A part of it has a sum of -1: less than 0 together with others of its kind, 0
+    // beside a part that has more.)
+    const bool nothing = l == 0 && last >= begin * kKeys && begin < stages;
     const long long at = (qs.row + row.i) * d.q_heads + head * d.group + row.g;
     if (d.parts > 1) {
         const long long own = (long long)part * d.q_rows * d.q_heads + at;
         store_floats<kD>(d.part_sums + own * d.D, o, live, d.D);
-        if (live && half == 0) d.part_stats[own] = make_float2(m * d.c, l);
+        if (live && half == 0) d.part_stats[own] = make_float2(m * d.c, nothing ? -1.f : l);
         return;
     }
-    const float f = l == 0 ? 0.f : 1.f / l;
+    const float f = nothing ? NTC_NAN : l == 0 ? 0.f : 1.f / l;
     store_row<T, kD>((char*)d.out + at * d.D * 2, o, f, live, d.D);
     if (d.rest) store_row<T, kD, true>((char*)d.rest + at * d.D * 2, o, f, live, d.D);
-    if (d.lse && live && half == 0) d.lse[at] = l == 0 ? -NTC_INF : (m * d.c + fast_log2(l)) * kLn2;
+    if (d.lse && live && half == 0) d.lse[at] = nothing ? NTC_NAN : l == 0 ? -NTC_INF : (m * d.c + fast_log2(l)) * kLn2;
 }
 
 // The parts of a row, joined by a wave: a lane takes a part's statistics first, then eight columns of every 64 / kPieces-th part.
@@ -490,7 +493,7 @@ template <class T, int kPieces> __global__ void __launch_bounds__(256) k_attenti
 #pragma unroll
         for (int g = kPieces; g < 64; g *= 2) sum[i] += __shfl_xor(sum[i], g);
     if (group || col >= d.D) return;
-    const float f = l == 0 ? 0.f : 1.f / l;
+    const float f = l < 0 ? NTC_NAN : l == 0 ? 0.f : 1.f / l;
     uint32_t out[4], rest[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -501,7 +504,7 @@ template <class T, int kPieces> __global__ void __launch_bounds__(256) k_attenti
     const long long at = 2 * (row * d.D + col);
     *(v4u*)((char*)d.out + at) = v4u{ out[0], out[1], out[2], out[3] };
     if (d.rest) *(v4u*)((char*)d.rest + at) = v4u{ rest[0], rest[1], rest[2], rest[3] };
-    if (d.lse && col == 0) d.lse[row] = l == 0 ? -NTC_INF : (m + fast_log2(l)) * kLn2;
+    if (d.lse && col == 0) d.lse[row] = l < 0 ? NTC_NAN : l == 0 ? -NTC_INF : (m + fast_log2(l)) * kLn2;
 }
 
 // ---------------------------------------------------------------- backward

@@ -13,6 +13,7 @@ namespace ntc_ops {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;
 #define NTC_INF __builtin_inff()
+#define NTC_NAN __builtin_nanf("")
 
 // ---------------------------------------------------------------- element types
 using f32 = float;

@@ -358,6 +358,6 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     bfloat16 or float16, 8 to 128 elements a head (a multiple of 8), any strides (copied first where heads are not contiguous, or not at multiples of 16 bytes). Differentiable (once) in
     q, k and v. Scores, the softmax and sums are 32-bit; probabilities, and backwards the scores' gradients, are rounded to the tensors' type for the products that
     follow. Nothing is added by atomics: results repeat bit for bit. Lengths are read on the GPU: numbers that leave the tensors are cut off there, and give wrong results, not an error. A key or
-    value that is not finite makes the queries that see it NaN where the formula does, and possibly others of its sequence.
+    value that is not finite makes the queries that see it NaN where the formula does, and possibly any other of its sequence; a query whose scores are all -inf is NaN.
     """
     return _binding().attention(q, k, v, causal, scale, cu_q, cu_k, k_lens)
