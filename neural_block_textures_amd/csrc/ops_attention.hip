@@ -59,7 +59,7 @@ struct AttentionArgs {
     int parts;                         // of a sequence's keys (dk and dv: of its rows), joined by a second launch; their sums:
     float* part_sums;                  // forward [parts][q_rows][q_heads][D]; backward dk's [parts][k_rows][k_heads][D], then dv's; dq's [parts][q_rows][q_heads][D], then part_rests
     float* part_rests;                 // [parts][q_rows][q_heads]: what the rounded dS add up to
-    float2* part_stats;                // forward [parts][q_rows][q_heads]: m c and the sum of probabilities (-1: of keys whose scores are all -inf)
+    float2* part_stats;                // forward [parts][q_rows][q_heads]: m c (float16: less 7) and the sum of probabilities (-1: of keys whose scores are all -inf)
     int line_heads;                    // log2 of how many heads share a line of the cache (128 bytes)
     int tiles, tiles_each;             // tiles of rows (or keys) in all, and of each sequence where there are no ends
     float scale, c;                    // c: scale log2 e
@@ -264,6 +264,9 @@ template <class T> __device__ __forceinline__ v4u packed(const v16f& x, int half
 // exponentials, so that the matrix unit is fed meanwhile. Causal, of what is not masked: 8192 tokens of 16 heads on 4 of 128 in 286 to 310 us, 890 to 960 TFLOP/s; seven sequences of 300
 // to 4096 tokens, 32 heads on 8, in 373, 990 TFLOP/s, of which 297 are left when LDS reads, exponentials and loads are taken out: the matrix unit at the clock that the power leaves it, and
 // masked halves of tiles. Heads of 32 are bound by their exponentials, one for 64 multiplications. Single tokens of 32 heads on 8 against 16 caches of 900 to 8192 keys: 66 us, 4.5 TB/s.
+// float16: probabilities and their sum are held times 2^7, so that they are at most 2^15 (a maximum lags by 2^8) and those down to 2^-32 of a row's largest count: without, 60000 keys at 2^-25 of it,
+// 2e-3 of the sum, came to twice that or to nothing.
+template <class T> constexpr float kLift = std::is_same_v<T, f16> ? 7.f : 0.f;
 template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 : kD <= 64 ? 3 : 2) k_attention(AttentionArgs d) {
     using L = Tile<kD>;
     constexpr int kTile = kKeys * L::kPitch;
@@ -334,7 +337,7 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
 #pragma unroll
             for (int t = 0; t < kD / 32; t++) o[t] *= by;
         }
-        const float mc = m == -NTC_INF ? 0.f : m * d.c;
+        const float mc = (m == -NTC_INF ? 0.f : m * d.c) - kLift<T>;
         const char *key_base = nullptr, *value_base = nullptr;
         if constexpr (kLoads) {
             key_base = kp + (long long)(s + 2) * kKeys * d.k.row;
@@ -457,13 +460,13 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
     if (d.parts > 1) {
         const long long own = (long long)part * d.q_rows * d.q_heads + at;
         store_floats<kD>(d.part_sums + own * d.D, o, live, d.D);
-        if (live && half == 0) d.part_stats[own] = make_float2(m * d.c, nothing ? -1.f : l);
+        if (live && half == 0) d.part_stats[own] = make_float2(m * d.c - kLift<T>, nothing ? -1.f : l);
         return;
     }
     const float f = nothing ? NTC_NAN : l == 0 ? 0.f : 1.f / l;
     store_row<T, kD>((char*)d.out + at * d.D * 2, o, f, live, d.D);
     if (d.rest) store_row<T, kD, true>((char*)d.rest + at * d.D * 2, o, f, live, d.D);
-    if (d.lse && live && half == 0) d.lse[at] = nothing ? NTC_NAN : l == 0 ? -NTC_INF : (m * d.c + fast_log2(l)) * kLn2;
+    if (d.lse && live && half == 0) d.lse[at] = nothing ? NTC_NAN : l == 0 ? -NTC_INF : (m * d.c - kLift<T> + fast_log2(l)) * kLn2;
 }
 
 // The parts of a row, joined by a wave: a lane takes a part's statistics first, then eight columns of every 64 / kPieces-th part.
