@@ -227,7 +227,8 @@ int ntc_op_rotary(const ntc_rotary_desc* d, void* stream, char* why, size_t why_
  * at q_batch_stride. All starts and strides are multiples of 8 elements (16 bytes); rows are at most 2^22 apart, heads 2^20. o, dq, dk and dv are contiguous [rows][heads][head_dim].
  *
  * Scores, the softmax's maximum and sum and all sums of products are 32-bit; the probabilities, and backwards their gradients, are rounded to the operands' type for the products
- * that follow (float16: times 2^7, so that 2^-32 of a row's largest is half the smallest step). With D = sum dO o (o before its rounding), dS = p (dO v - D): dv = sum p dO, dq = scale sum dS k, dk = scale sum dS q, the last two over the group's heads.
+ * that follow (float16: times 2^7, so that 2^-32 of a row's largest is half the smallest step; backwards the gradients
+ * times a power of two that goes by a sequence's largest dO and v, for dq by the row's own dO). With D = sum dO o (o before its rounding), dS = p (dO v - D): dv = sum p dO, dq = scale sum dS k, dk = scale sum dS q, the last two over the group's heads.
  * A query that sees a key or value that is not finite is NaN where the formula is, and so is one all of whose scores are -inf (lse too; also where finite values' products leave 32 bits); any query of that sequence may
  * be as well (0 times infinity).
  * workspace: ntc_op_attention_workspace() bytes (backward 0 or 1), any contents, at a multiple of 16 bytes. */

@@ -50,7 +50,9 @@ struct Operand3 { const char* p; long long row, head, batch; };    // strides in
 struct AttentionArgs {
     Operand3 q, k, v, d_o;
     void *out, *rest, *dq, *dk, *dv;
-    float *lse, *log_sums, *deltas, *extent;   // backward [q_rows][q_heads]: log2 sum exp less kShift, dO o times the scores' power of two over 2^kShift
+    float *lse, *log_sums, *deltas;    // backward [q_rows][q_heads]: log2 sum exp less kShift, dO o times the sequence's power of two over 2^kShift
+    float *extents_v, *extents_do;     // float16, backward: the largest |v| and |dO| of each kExtentRows rows of a sequence
+    int v_extents, v_extents_each, do_extents, do_extents_each;    // how many in all, and of each sequence where there are no ends
     const int *cu_q, *cu_k, *k_lens;
     long long q_rows, k_rows;
     int sequences, q_each, k_each;     // rows of a sequence where there are no ends
@@ -65,7 +67,7 @@ struct AttentionArgs {
     float scale, c;                    // c: scale log2 e
 };
 
-constexpr int kRows = 128, kKeys = 64, kExtents = 256;
+constexpr int kRows = 128, kKeys = 64, kExtentRows = 32;
 
 // ---------------------------------------------------------------- which rows
 struct Span { int b; long long row; int n; long long start; };     // sequence, its first row in all, its rows, the byte where they start
@@ -74,9 +76,14 @@ __device__ __forceinline__ long long cut(long long x, long long lo, long long hi
 
 // Tile t of all, to its sequence and its number there. With ends, sequence b's tiles are numbered from e_b units / size + b on, which leaves each at least as many numbers as
 // it has tiles, and none shared: the largest b whose first number is at most t, by 64 probes at once. Rows behind the last sequence are one more.
+template <int kSize> __device__ __forceinline__ int first_tile(const int* cu, int tiles_each, int units, int b) {
+    if (!cu) return b * tiles_each;
+    const long long e = b ? cu[b] : 0;
+    return (int)cut(e * units / kSize, 0, 1 << 30) + b;
+}
 template <int kSize> __device__ __forceinline__ int find_sequence(const int* cu, int sequences, int tiles_each, int units, int t, int& tile) {
     if (!cu) { const int b = t / tiles_each; tile = t - b * tiles_each; return b; }
-    const auto first = [&](int b) { const long long e = b ? cu[b] : 0; return (int)cut(e * units / kSize, 0, 1 << 30) + b; };
+    const auto first = [&](int b) { return first_tile<kSize>(cu, tiles_each, units, b); };
     int lo = 0, hi = sequences;
     while (lo < hi) {
         const int step = (hi - lo + 63) / 64, probe = lo + (lane_id() + 1) * step;
@@ -241,15 +248,15 @@ template <class T, int kD, bool kRests = false> __device__ __forceinline__ void 
             if (live && col < D) *(v4u*)(p + 2 * col) = v4u{ (uint32_t)lo[0], (uint32_t)hi[0], (uint32_t)lo[1], (uint32_t)hi[1] };
         }
 }
-// ... as it is, in 32 bits
-template <int kD> __device__ __forceinline__ void store_floats(float* p, const v16f (&x)[kD / 32], bool live, int D) {
+// ... in 32 bits
+template <int kD> __device__ __forceinline__ void store_floats(float* p, const v16f (&x)[kD / 32], float f, bool live, int D) {
     const int half = lane_id() >> 5;
 #pragma unroll
     for (int t = 0; t < kD / 32; t++)
 #pragma unroll
         for (int a = 0; a < 4; a++) {
             const int col = 32 * t + 8 * a + 4 * half;
-            if (live && col < D) *(float4*)(p + col) = make_float4(x[t][4 * a], x[t][4 * a + 1], x[t][4 * a + 2], x[t][4 * a + 3]);
+            if (live && col < D) *(float4*)(p + col) = make_float4(x[t][4 * a] * f, x[t][4 * a + 1] * f, x[t][4 * a + 2] * f, x[t][4 * a + 3] * f);
         }
 }
 // result register r of the lane is row 8 (r / 4) + 4 half + r % 4
@@ -459,7 +466,7 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD <= 32 ? 4 :
     const long long at = (qs.row + row.i) * d.q_heads + head * d.group + row.g;
     if (d.parts > 1) {
         const long long own = (long long)part * d.q_rows * d.q_heads + at;
-        store_floats<kD>(d.part_sums + own * d.D, o, live, d.D);
+        store_floats<kD>(d.part_sums + own * d.D, o, 1.f, live, d.D);
         if (live && half == 0) d.part_stats[own] = make_float2(m * d.c - kLift<T>, nothing ? -1.f : l);
         return;
     }
@@ -512,16 +519,28 @@ template <class T, int kPieces> __global__ void __launch_bounds__(256) k_attenti
 
 // ---------------------------------------------------------------- backward
 // float16: the score's gradients, and probabilities of long rows, leave its range. They are multiplied by powers of two: probabilities by 2^14, the score's
-// gradients by the largest that keeps 2 D max|dO| max|v|, which they cannot pass, within 2^15. Largest values of 256 blocks' shares, joined by whoever reads them.
+// gradients by the largest that keeps 2 D max|dO| max|v|, which they cannot pass, within 2^15: for dq of the row's dO and its sequence's v, for dk of the sequence's both, so that what other sequences
+// hold (and for dq, other rows' dO) does not decide what is left of them. A block takes the largest value of kExtentRows rows of v (first) or dO; who needs a sequence's joins its blocks'.
 template <class T> __global__ void __launch_bounds__(256) k_attention_extent(AttentionArgs d) {
-    __shared__ float parts[2][4];
-    float of_v = 0, of_do = 0;
+    __shared__ float parts[4];
+    float to = 0;
     const unsigned pieces = d.D / 8;
-    // of n rows that begin at `p`, all their heads: four loads of each thread on their way together
-    const auto largest = [&](const char* p, int n, const Operand3& of, unsigned heads, float& to) {
+    const long long block = block_number();
+    const bool of_v = block < d.v_extents;
+    const int number = (int)(of_v ? block : block - d.v_extents);
+    if (!of_v && number >= d.do_extents) return;
+    int tile;
+    const int* cu = of_v ? d.cu_k : d.cu_q;
+    const int b = find_sequence<kExtentRows>(cu, d.sequences, of_v ? d.v_extents_each : d.do_extents_each, 1, number, tile);
+    if (b < d.sequences && tile >= 0) {
+        const Operand3& of = of_v ? d.v : d.d_o;
+        const Span span = of_v ? span_of(cu, d.sequences, d.k_each, d.k_rows, b, of) : span_of(cu, d.sequences, d.q_each, d.q_rows, b, of);
+        const unsigned heads = of_v ? d.k_heads : d.q_heads;
+        const long long left = (long long)(of_v ? keys_of(d, span) : span.n) - (long long)tile * kExtentRows;
+        const unsigned all = (unsigned)cut(left, 0, kExtentRows) * heads * pieces;
+        const char* p = of.p + span.start + (long long)tile * kExtentRows * of.row;
         typedef T v8 __attribute__((ext_vector_type(8)));
-        const unsigned all = n * heads * pieces;
-        for (unsigned x0 = threadIdx.x; x0 < all; x0 += 1024) {
+        for (unsigned x0 = threadIdx.x; x0 < all; x0 += 1024) {               // four loads of a thread on their way together
             v8 x[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -533,43 +552,27 @@ template <class T> __global__ void __launch_bounds__(256) k_attention_extent(Att
 #pragma unroll
                 for (int i = 0; i < 8; i++) to = __builtin_fmaxf(to, __builtin_fabsf((float)x[k][i]));
         }
-    };
-    for (int t = blockIdx.x; t < d.tiles; t += gridDim.x) {
-        int tile;
-        const int b = find_sequence<kRows>(d.cu_k, d.sequences, d.tiles_each, 1, t, tile);
-        if (b >= d.sequences) continue;
-        const Span ks = span_of(d.cu_k, d.sequences, d.k_each, d.k_rows, b, d.v);
-        const int n = tile < 0 ? 0 : keys_of(d, ks) - tile * kRows;
-        if (n > 0) largest(d.v.p + ks.start + (long long)tile * kRows * d.v.row, n < kRows ? n : kRows, d.v, d.k_heads, of_v);
-    }
-    // (from the last block on: the first ones may have had keys)
-    constexpr int kChunk = 32;
-    const int rows = (int)(d.cu_q ? cut(d.cu_q[d.sequences], 0, d.q_rows) : d.q_each), chunks = (rows + kChunk - 1) / kChunk;
-    const long long all_chunks = d.cu_q ? chunks : (long long)chunks * d.sequences;
-    for (long long t = gridDim.x - 1 - blockIdx.x; t < all_chunks; t += gridDim.x) {
-        const int b = d.cu_q ? 0 : (int)(t / chunks), first = (int)(t - (long long)b * chunks) * kChunk;
-        largest(d.d_o.p + b * d.d_o.batch + first * d.d_o.row, rows - first < kChunk ? rows - first : kChunk, d.d_o, d.q_heads, of_do);
     }
     const auto most = [](float a, float b) { return __builtin_fmaxf(a, b); };
-    of_v = reduce64(of_v, most);
-    of_do = reduce64(of_do, most);
-    if (lane_id() == 0) { parts[0][threadIdx.x >> 6] = of_v; parts[1][threadIdx.x >> 6] = of_do; }
+    to = reduce64(to, most);
+    if (lane_id() == 0) parts[threadIdx.x >> 6] = to;
     __syncthreads();
-    if (threadIdx.x < 2) d.extent[threadIdx.x * kExtents + blockIdx.x] = most(most(parts[threadIdx.x][0], parts[threadIdx.x][1]), most(parts[threadIdx.x][2], parts[threadIdx.x][3]));
+    if (threadIdx.x == 0) (of_v ? d.extents_v : d.extents_do)[number] = most(most(parts[0], parts[1]), most(parts[2], parts[3]));
 }
+// A sequence's largest |v| (of n rows) or |dO|
+__device__ __forceinline__ float extent_of(const float* extents, int first, int n) {
+    float most = 0;
+    for (int i = lane_id(); i < (n + kExtentRows - 1) / kExtentRows; i += 64) most = __builtin_fmaxf(most, extents[first + i]);
+    return reduce64(most, [](float a, float b) { return __builtin_fmaxf(a, b); });
+}
+__device__ __forceinline__ float extent_of_v(const AttentionArgs& d, int b, int n) { return extent_of(d.extents_v, first_tile<kExtentRows>(d.cu_k, d.v_extents_each, 1, b), n); }
+__device__ __forceinline__ float extent_of_do(const AttentionArgs& d, int b, int n) { return extent_of(d.extents_do, first_tile<kExtentRows>(d.cu_q, d.do_extents_each, 1, b), n); }
 // The power of two for the scores' gradients, as an exponent.
-template <class T> __device__ __forceinline__ int gradient_exponent(const AttentionArgs& d) {
-    if constexpr (!std::is_same_v<T, f16>) return 0;
-    float most[2] = {};
-#pragma unroll
-    for (int w = 0; w < 2; w++)
-#pragma unroll
-        for (int i = 0; i < kExtents / 64; i++) most[w] = __builtin_fmaxf(most[w], d.extent[w * kExtents + 64 * i + lane_id()]);
-    const auto larger = [](float a, float b) { return __builtin_fmaxf(a, b); };
-    const float bound = 2.f * d.D * reduce64(most[0], larger) * reduce64(most[1], larger);
+__device__ __forceinline__ int gradient_exponent(const AttentionArgs& d, float v, float d_o) {
+    const float bound = 2.f * d.D * v * d_o;
     if (!(bound > 0) || bound > 3e38f) return 0;
     const int e = 14 - (int)((__float_as_uint(bound) >> 23) - 127);
-    return uniform(e < -60 ? -60 : e > 60 ? 60 : e);
+    return e < -60 ? -60 : e > 60 ? 60 : e;
 }
 __device__ __forceinline__ float two_to(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }
 template <class T> constexpr int kShift = std::is_same_v<T, f16> ? 14 : 0;      // probabilities are held times 2^kShift
@@ -619,11 +622,25 @@ template <class T, int kD, bool kParts> __global__ void __launch_bounds__(256, k
     }
     load_row<kD>(q, d.q.p + qs.start + row.i * d.q.row + h * d.q.head, live, d.D);
     delta += other_half(delta);
-    const int e = gradient_exponent<T>(d);
-    const float up = two_to(e), lse = live ? d.lse[at] * kLog2e : 0.f, delta_up = delta * up;
+    const float lse = live ? d.lse[at] * kLog2e : 0.f;
+    int e = 0, e_sequence = 0;                             // of the row, and of its sequence
+    if constexpr (std::is_same_v<T, f16>) {
+        typedef T v8 __attribute__((ext_vector_type(8)));
+        float most = 0;
+#pragma unroll
+        for (int s = 0; s < kD / 16; s++) {
+            const v8 c = __builtin_bit_cast(v8, g[s]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) most = __builtin_fmaxf(most, __builtin_fabsf((float)c[i]));
+        }
+        const float of_v = extent_of_v(d, b, Lk);
+        e = gradient_exponent(d, of_v, __builtin_fmaxf(most, other_half(most)));
+        e_sequence = gradient_exponent(d, of_v, extent_of_do(d, b, qs.n));
+    }
+    const float lse_up = lse - (float)e;                   // (2^e goes into the exponential: its argument is off by 2^-18 then)
     if (live && half == 0 && part == 0) {                               // as the keys' and values' gradients take them
         d.log_sums[at] = lse - kShift<T>;
-        d.deltas[at] = delta_up * two_to(-kShift<T>);
+        d.deltas[at] = delta * two_to(e_sequence) * two_to(-kShift<T>);
     }
     const int i_wave = (r0 + 31) / d.group, i_block = (tile * kRows + kRows - 1) / d.group;
     const int block_last = d.causal ? (i_block + off < Lk - 1 ? i_block + off : Lk - 1) : Lk - 1;
@@ -660,7 +677,7 @@ template <class T, int kD, bool kParts> __global__ void __launch_bounds__(256, k
         v4u p[2][2];
         const int seen = last - s * kKeys - 4 * half;
         const auto gradient = [&](const v16f& a, const v16f& c, int j, int r) {
-            const float exponent = __builtin_fmaf(a[r], d.c, -lse), z = __builtin_fmaf(c[r], up, -delta_up);
+            const float exponent = __builtin_fmaf(a[r], d.c, -lse_up), z = c[r] - delta;
             const bool in = !kMasks || 32 * j + result_row(r) <= seen;
             return fast_exp2(in ? exponent : -NTC_INF) * (in ? z : 0.f);
         };
@@ -745,7 +762,7 @@ template <class T, int kD, bool kParts> __global__ void __launch_bounds__(256, k
 #pragma unroll
                 for (int i = 0; i < kD / 16; i++) y = product<T>(places.row_piece(at + 2 * kTile, 32 * j, i), g[i], y);
 #pragma unroll
-                for (int r = 0; r < 16; r++) x[r] = fast_exp2(__builtin_fmaf(x[r], d.c, -lse)) * __builtin_fmaf(y[r], up, -delta_up);
+                for (int r = 0; r < 16; r++) x[r] = fast_exp2(__builtin_fmaf(x[r], d.c, -lse_up)) * (y[r] - delta);
                 if (s * kKeys + 32 * j + 31 > wave_first) {
                     const int seen = last - s * kKeys - 32 * j - 4 * half;
 #pragma unroll
@@ -783,8 +800,8 @@ template <class T, int kD, bool kParts> __global__ void __launch_bounds__(256, k
     none();
     if (kParts) {
         const long long all = d.q_rows * d.q_heads;
-        store_floats<kD>(d.part_sums + (part * all + at) * d.D, dq, live, d.D);
-        if (live && half == 0) d.part_rests[part * all + at] = sum;
+        store_floats<kD>(d.part_sums + (part * all + at) * d.D, dq, two_to(-e), live, d.D);
+        if (live && half == 0) d.part_rests[part * all + at] = sum * two_to(-e);
         if (own_end == 0 && part == 0) store_row<T, kD>((char*)d.dq + at * d.D * 2, dq, 0.f, live, d.D);
         return;
     }
@@ -808,7 +825,6 @@ template <class T, int kD, bool kParts> __global__ void __launch_bounds__(256, k
 // The parts of dq added up, and what the vector near the keys takes off: eight columns to a thread.
 template <class T> __global__ void __launch_bounds__(256) k_attention_dq_join(AttentionArgs d) {
     const long long rows = d.q_rows * d.q_heads, n = rows * d.D / 8, x = block_number() * 256 + threadIdx.x;
-    const float f = d.scale * two_to(-gradient_exponent<T>(d));
     if (x >= n) return;
     const long long row = x / (d.D / 8);
     char* to = (char*)d.dq + 16 * x;
@@ -825,7 +841,7 @@ template <class T> __global__ void __launch_bounds__(256) k_attention_dq_join(At
     const v8 near = *(const v8*)to;
     uint32_t out[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) out[i] = pack2<T>(__builtin_fmaf(-rest, (float)near[2 * i], sum[2 * i]) * f, __builtin_fmaf(-rest, (float)near[2 * i + 1], sum[2 * i + 1]) * f);
+    for (int i = 0; i < 4; i++) out[i] = pack2<T>(__builtin_fmaf(-rest, (float)near[2 * i], sum[2 * i]) * d.scale, __builtin_fmaf(-rest, (float)near[2 * i + 1], sum[2 * i + 1]) * d.scale);
     *(v4u*)to = v4u{ out[0], out[1], out[2], out[3] };
 }
 
@@ -857,7 +873,8 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
     v4u k[kD / 16], v[kD / 16];
     load_row<kD>(k, d.k.p + ks.start + key * d.k.row + head * d.k.head, live, d.D);
     load_row<kD>(v, d.v.p + v_start + key * d.v.row + head * d.v.head, live, d.D);
-    const int e = qs.n ? gradient_exponent<T>(d) : 0;      // (without queries nothing has left it)
+    int e = 0;
+    if constexpr (std::is_same_v<T, f16>) if (qs.n) e = uniform(gradient_exponent(d, extent_of_v(d, b, Lk), extent_of_do(d, b, qs.n)));      // (without queries nothing has left them)
     const float up = two_to(e) * two_to(-kShift<T>);
 
     // Row r sees key j where r >= (j - off) G: the lane's first row, the wave's first whole one, and where wave and block start
@@ -1060,8 +1077,8 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
     const long long at = (ks.row + key) * d.k_heads + head;
     if (d.parts > 1) {
         const long long each = d.k_rows * d.k_heads;
-        store_floats<kD>(d.part_sums + (part * each + at) * d.D, dk, held, d.D);
-        store_floats<kD>(d.part_sums + ((d.parts + part) * each + at) * d.D, dv, held, d.D);
+        store_floats<kD>(d.part_sums + (part * each + at) * d.D, dk, two_to(-e), held, d.D);
+        store_floats<kD>(d.part_sums + ((d.parts + part) * each + at) * d.D, dv, 1.f, held, d.D);
         return;
     }
     store_row<T, kD>((char*)d.dk + at * d.D * 2, dk, d.scale * two_to(-e), held && d.dk, d.D);
@@ -1071,9 +1088,9 @@ template <class T, int kD> __global__ void __launch_bounds__(256, kD > 64 ? 1 : 
 // The parts of dk (dv: second half of the grid) added up: eight columns to a thread.
 template <class T> __global__ void __launch_bounds__(256) k_attention_sum(AttentionArgs d) {
     const long long n = d.k_rows * d.k_heads * d.D / 8, x = block_number() * 256 + threadIdx.x;
-    const float f = d.scale * two_to(-gradient_exponent<T>(d));
     if (x >= 2 * n) return;
     const int which = x >= n;
+    const float f = which ? two_to(-kShift<T>) : d.scale;
     const long long at = 8 * (which ? x - n : x);
     char* to = (char*)(which ? d.dv : d.dk);
     if (!to) return;
@@ -1087,7 +1104,7 @@ template <class T> __global__ void __launch_bounds__(256) k_attention_sum(Attent
     }
     uint32_t out[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) out[i] = pack2<T>(sum[2 * i] * (which ? two_to(-kShift<T>) : f), sum[2 * i + 1] * (which ? two_to(-kShift<T>) : f));
+    for (int i = 0; i < 4; i++) out[i] = pack2<T>(sum[2 * i] * f, sum[2 * i + 1] * f);
     *(v4u*)(to + 2 * at) = v4u{ out[0], out[1], out[2], out[3] };
 }
 
@@ -1142,12 +1159,17 @@ AttentionArgs args_of(const ntc_attention_desc* d) {
     return a;
 }
 // tiles of `size` of rows that lie in sequences (each at most a tile more than its share, one more for what is behind the last)
-void set_tiles(AttentionArgs& a, bool ends, int64_t each, int64_t rows, int64_t size) {
-    a.tiles_each = (int)((each + size - 1) / size);
-    a.tiles = (int)(ends ? rows / size + a.sequences + 1 : (int64_t)a.tiles_each * a.sequences);
+void set_tiles(const AttentionArgs& a, bool ends, int64_t each, int64_t rows, int64_t size, int& tiles_each, int& tiles) {
+    tiles_each = (int)((each + size - 1) / size);
+    tiles = (int)(ends ? rows / size + a.sequences + 1 : (int64_t)tiles_each * a.sequences);
 }
-void set_row_tiles(AttentionArgs& a) { set_tiles(a, a.cu_q, (int64_t)a.q_each * a.group, a.q_rows * a.group, kRows); }
-void set_key_tiles(AttentionArgs& a) { set_tiles(a, a.cu_k, a.k_each, a.k_rows, kRows); }
+void set_row_tiles(AttentionArgs& a) { set_tiles(a, a.cu_q, (int64_t)a.q_each * a.group, a.q_rows * a.group, kRows, a.tiles_each, a.tiles); }
+void set_key_tiles(AttentionArgs& a) { set_tiles(a, a.cu_k, a.k_each, a.k_rows, kRows, a.tiles_each, a.tiles); }
+void set_extents(AttentionArgs& a) {
+    set_tiles(a, a.cu_k, a.k_each, a.k_rows, kExtentRows, a.v_extents_each, a.v_extents);
+    set_tiles(a, a.cu_q, a.q_each, a.q_rows, kExtentRows, a.do_extents_each, a.do_extents);
+}
+size_t extents_size(const AttentionArgs& a) { return 4 * ((size_t)a.v_extents + a.do_extents); }
 template <class F> void with_head(int dtype, int D, F f) {
     const auto go = [&](auto t) {
         if (D <= 32) f(t, std::integral_constant<int, 32>{});
@@ -1208,7 +1230,8 @@ size_t ntc_op_attention_workspace(const ntc_attention_desc* d, int32_t backward)
         const int parts = forward_parts(a);
         return parts > 1 ? (size_t)parts * d->q_rows * d->q_heads * (8 + 4 * (size_t)d->head_dim) : 0;
     }
-    const size_t n = d->q_rows ? 2 * rounded((size_t)d->q_rows * d->q_heads * 4) + 2 * kExtents * 4 : 0;
+    if (d->dtype == NTC_F16) set_extents(a);
+    const size_t n = d->q_rows ? 2 * rounded((size_t)d->q_rows * d->q_heads * 4) + rounded(extents_size(a)) : 0;
     size_t of_parts = 0;                                   // (dq's are joined before dk's and dv's are made)
     if (d->q_rows && d->k_rows) {
         set_row_tiles(a);
@@ -1246,8 +1269,10 @@ int ntc_op_attention_backward(const ntc_attention_desc* d, void* stream, char* w
     AttentionArgs a = args_of(d);
     a.log_sums = (float*)d->workspace;
     a.deltas = (float*)((char*)d->workspace + rounded((size_t)d->q_rows * d->q_heads * 4));
-    a.extent = (float*)((char*)a.deltas + rounded((size_t)d->q_rows * d->q_heads * 4));
-    a.part_sums = d->q_rows ? a.extent + 2 * kExtents : (float*)d->workspace;
+    if (d->dtype == NTC_F16) set_extents(a);
+    a.extents_v = (float*)((char*)a.deltas + rounded((size_t)d->q_rows * d->q_heads * 4));
+    a.extents_do = a.extents_v + a.v_extents;
+    a.part_sums = d->q_rows ? (float*)((char*)a.extents_v + rounded(extents_size(a))) : (float*)d->workspace;
     set_key_tiles(a);
     a.parts = d->q_rows && d->k_rows ? backward_parts(a) : 1;
     const int parts = a.parts;
@@ -1258,11 +1283,7 @@ int ntc_op_attention_backward(const ntc_attention_desc* d, void* stream, char* w
     a.part_rests = a.part_sums + (size_t)q_parts * d->q_rows * d->q_heads * d->head_dim;
     if (keys_many || too_many(a)) return refuse(why, cap, "too many tiles of rows times heads: 2^31 at most");
     if (d->q_rows) {
-        if (d->dtype == NTC_F16) {
-            set_key_tiles(a);
-            k_attention_extent<f16><<<kExtents, 256, 0, s>>>(a);
-        }
-        set_row_tiles(a);
+        if (d->dtype == NTC_F16) k_attention_extent<f16><<<grid_of((int64_t)a.v_extents + a.do_extents), 256, 0, s>>>(a);
         const dim3 grid = grid_for(a);
         with_head(d->dtype, d->head_dim, [&](auto t, auto h) {
             if (a.parts == 1) { k_attention_dq<decltype(t), h.value, false><<<grid, 256, 0, s>>>(a); return; }
