@@ -151,8 +151,14 @@ class TilePrior:
         return [(room(), room()) for _ in self.blocks]
 
     def step(self, x: torch.Tensor, positions: torch.Tensor, cache: list, lens: torch.Tensor, weights=None) -> torch.Tensor:
-        """[tiles, alphabet] for one more symbol of each tile, the lens[i]-th (int32 [tiles]) of tile i; its keys and values go into the cache."""
-        each, at = torch.arange(len(x), device=x.device), lens.long()
+        """[tiles, alphabet] for one more symbol of each tile, the lens[i]-th (int32 [tiles]) of tile i; its keys and values go into the cache. Lengths are read on the GPU: where a tile's
+        has no room its last place is written over, and the prediction is wrong."""
+        if len(cache) != len(self.blocks) or not len(x) == len(positions) == len(lens):
+            raise ValueError(f"one context, position and length a tile and a cache for each block are needed, not {len(x)}, {len(positions)} and {len(lens)}, and {len(cache)} for {len(self.blocks)}")
+        for room in (r for pair in cache for r in pair):
+            if room.dim() != 4 or len(room) != len(x) or room.shape[1] < 1 or room.shape[1] != cache[0][0].shape[1] or room.shape[2:] != (self.heads, self.dim):
+                raise ValueError(f"the cache must be [{len(x)} tiles, symbols, {self.heads} heads, {self.dim}], not {list(room.shape)}")
+        each, at = torch.arange(len(x), device=x.device), lens.long().clamp(0, cache[0][0].shape[1] - 1)
 
         def attend(n, q, k, v):
             keys, values = cache[n]
