@@ -150,6 +150,7 @@ class TilePrior:
         room = lambda: torch.empty((tiles, symbols, self.heads, self.dim), dtype=torch.bfloat16, device=self.first.device)  # noqa: E731
         return [(room(), room()) for _ in self.blocks]
 
+    @torch.no_grad()                                      # (a cache that is written in place keeps no graph)
     def step(self, x: torch.Tensor, positions: torch.Tensor, cache: list, lens: torch.Tensor, weights=None) -> torch.Tensor:
         """[tiles, alphabet] for one more symbol of each tile, the lens[i]-th (int32 [tiles]) of tile i; its keys and values go into the cache. Lengths are read on the GPU: where a tile's
         has no room its last place is written over, and the prediction is wrong."""

@@ -25,3 +25,13 @@ def test_lengths_that_leave_the_cache(length):
             want = torch.zeros_like(changed)
             want[1, 3] = want[2, 9 if length > 0 else 0] = want[3, 9] = True
             assert torch.equal(changed, want)
+
+
+def test_no_graph_is_kept():
+    """... from step to step, where a caller has gradients on."""
+    p = prior.TilePrior(13, 64, 4, 2, 4, 1)
+    cache, lens = p.cache(2, 10), torch.zeros(2, dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        logits = p.step(torch.ones(2, 13, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 3, dtype=torch.int64, device="cuda"), cache, lens)
+        lens += 1
+    assert not logits.requires_grad and not any(room.requires_grad for pair in cache for room in pair)
