@@ -1,7 +1,7 @@
 """A learned prior over a trained latent's symbols: the bits an arithmetic coder would need for them.
 
     python -m neural_block_textures_amd.prior model.bin|model.ntcb [--steps 300] [--hidden 256] [--batch 16384] [--lr 2e-3]
-        [--state-bits 8|32] [--seed 1] [--fp32-latent] [--tile 0] [--layers 2] [--heads 8]
+        [--state-bits 8|32] [--seed 1] [--fp32-latent] [--tile 0] [--layers 2] [--heads 8] [--stepped 0]
 
 The print statistics price a latent by the entropy of its histograms, each symbol on its own or against its left neighbour. Here
 a small network predicts each symbol from those before it in raster order (the texels to the left and above, and the
@@ -12,7 +12,8 @@ alternative, or one of its first four, is the symbol.
 With --tile T the model looks further than the neighbours: the plane is cut into tiles of T x T texels, a tile's symbols are a sequence in raster order, and blocks of
 layer norm, rotary positions (row, column, channel) and causal attention over the tile come between the contexts and the alphabet. Everything a symbol is
 predicted from still lies before it in the plane's raster order. Tiles of all sizes (those of the edges are smaller) are packed into one batch; TilePrior.step predicts
-symbols one at a time from the keys and values of those before them, as a decoder has to.
+single symbols from the keys and values of those before them in their tiles. A decoder knows a symbol's neighbours in other tiles only in the plane's raster order, and raster_logprobs goes
+that way, from a plane that holds nothing else yet; with --stepped N the first N symbols' bits are given as it predicts them, beside those of the pass over whole tiles.
 
 A training step is the operators of ops.py end to end: layers in 8-bit floating point (fp8_linear), the symbols' log
 probabilities and their gradient (token_logprobs), and one AdamW step over all weights with an 8-bit state. The price is then
@@ -64,9 +65,19 @@ class Contexts:
     def __init__(self, sym: torch.Tensor, alphabet: int):
         self.H, self.W, self.C = sym.shape
         self.width = 6 * self.C + 1
-        self.values = sym.float() * (2.0 / max(1, alphabet - 1)) - 1.0
+        self.alphabet = alphabet
+        self.values = self._scaled(sym)
         self.padded = torch.zeros((self.H + 1, self.W + 2, self.C), device=sym.device)
         self.padded[1:, 1:-1] = self.values
+
+    def _scaled(self, sym):
+        return sym.float() * (2.0 / max(1, self.alphabet - 1)) - 1.0
+
+    def put(self, at: torch.Tensor, sym: torch.Tensor) -> None:
+        """Symbols that have become known, at flat indices `at`"""
+        texel, c = at // self.C, at % self.C
+        y, x = texel // self.W, texel % self.W
+        self.values[y, x, c] = self.padded[y + 1, x + 1, c] = self._scaled(sym)
 
     def rows(self, at: torch.Tensor) -> torch.Tensor:
         """[len(at), width] for symbols `at` (flat indices), in bfloat16"""
@@ -178,7 +189,7 @@ class Tiles:
             raise ValueError(f"tiles have 1 texel a side or more, not {tile}")
         flat = torch.arange(H * W * C, device=device).view(H, W, C)
         cut = [flat[y:y + tile, x:x + tile].reshape(-1) for y in range(0, H, tile) for x in range(0, W, tile)]
-        self.shape, self.order, self.lengths = shape, cut, [len(c) for c in cut]
+        self.shape, self.tile, self.order, self.lengths = shape, tile, cut, [len(c) for c in cut]
 
     def batch(self, which) -> tuple:
         """(flat indices, positions [symbols, 3], ends) of some tiles, packed"""
@@ -222,7 +233,8 @@ def fit_tiles(sym: torch.Tensor, alphabet: int, tile: int, steps: int = 300, hid
 
 @torch.no_grad()
 def step_logprobs(prior: TilePrior, ctx: Contexts, tiles: Tiles, sym: torch.Tensor, which) -> torch.Tensor:
-    """Log probabilities of the symbols of tiles of one size, [tiles, symbols], predicted one at a time as a decoder would."""
+    """Log probabilities of the symbols of tiles of one size, [tiles, symbols], predicted one at a time in all tiles together, with contexts of the finished plane: TilePrior.step against the pass
+    over whole tiles. (A decoder has no such contexts across the tiles' borders, and goes as raster_logprobs does.)"""
     n = tiles.lengths[which[0]]
     if any(tiles.lengths[i] != n for i in which):
         raise ValueError("tiles of one size are needed")
@@ -234,6 +246,41 @@ def step_logprobs(prior: TilePrior, ctx: Contexts, tiles: Tiles, sym: torch.Tens
         out.append(ops.token_logprobs(prior.step(ctx.rows(at[:, i]), positions[:, i], cache, lens, weights), flat[at[:, i]]).logprob)
         lens += 1
     return torch.stack(out, 1)
+
+
+@torch.no_grad()
+def raster_logprobs(prior: TilePrior, tiles: Tiles, sym: torch.Tensor, alphabet: int, count: int = None) -> torch.Tensor:
+    """Log probabilities of the plane's first `count` symbols (all of them where it is None), predicted one at a time in its raster order: contexts of a plane that holds the symbols before and
+    nothing else, keys and values of the symbol's own tile. A decoder that reads the symbol where this one looks it up goes the same way."""
+    H, W, C = tiles.shape
+    flat, n = sym.reshape(-1), sym.numel() if count is None else count
+    if not 0 <= n <= flat.numel():
+        raise ValueError(f"0 to {flat.numel()} symbols can be predicted, not {n}")
+    ctx, weights, across = Contexts(torch.zeros_like(sym), alphabet), prior.laid_out(), -(-W // tiles.tile)
+    cache, lens = prior.cache(across, max(tiles.lengths)), torch.zeros(across, dtype=torch.int32, device=sym.device)      # of one row of tiles, the next row's after it
+    at = torch.arange(n, device=sym.device)
+    positions, out = torch.stack([at // C // W, at // C % W, at % C], 1), torch.empty(n, device=sym.device)
+    for i in range(n):
+        if i % (tiles.tile * W * C) == 0:
+            lens.zero_()
+        one, t = slice(i, i + 1), i // C % W // tiles.tile
+        own = slice(t, t + 1)
+        logits = prior.step(ctx.rows(at[one]), positions[one], [(k[own], v[own]) for k, v in cache], lens[own], weights)
+        out[one] = ops.token_logprobs(logits, flat[one]).logprob
+        ctx.put(at[one], flat[one])
+        lens[own] += 1
+    return out
+
+
+@torch.no_grad()
+def packed_logprobs(prior: TilePrior, ctx: Contexts, tiles: Tiles, sym: torch.Tensor, batch: int = 1 << 17) -> torch.Tensor:
+    """Log probabilities of all symbols, in the plane's raster order, by passes over whole tiles"""
+    flat, weights = sym.reshape(-1), prior.laid_out()
+    out = torch.empty(flat.numel(), device=sym.device)
+    for which in tiles.groups(batch):
+        at, positions, ends = tiles.batch(which)
+        out[at] = ops.token_logprobs(prior.logits(ctx.rows(at), positions, ends, weights), flat[at]).logprob
+    return out
 
 
 def fit(sym: torch.Tensor, alphabet: int, steps: int = 300, hidden: int = 256, batch: int = 16384, lr: float = 2e-3, state_bits: int = 8, seed: int = 1):
@@ -293,7 +340,10 @@ def main(argv=None):
     ap.add_argument("--tile", type=int, default=0, help="attention over tiles of this many texels a side (0: the neighbours alone)")
     ap.add_argument("--layers", type=int, default=2, help="blocks of attention")
     ap.add_argument("--heads", type=int, default=8)
+    ap.add_argument("--stepped", type=int, default=0, help="predict a level's first so many symbols one at a time too, as a decoder has to (with --tile)")
     a = ap.parse_args(argv)
+    if a.stepped < 0 or (a.stepped and not a.tile):
+        ap.error("--stepped takes a number from 0 on, and --tile beside it")
     for l, sym, alphabet in level_symbols(decode.load(a.model, q8=not a.fp32_latent)):
         dev = torch.from_numpy(sym).cuda()
         tiles = None
@@ -303,6 +353,10 @@ def main(argv=None):
             prior, ctx = fit(dev, alphabet, a.steps, a.hidden, a.batch, a.lr, a.state_bits, a.seed)
         out = {"level": l, "symbols": sym.size, "alphabet": alphabet, "histogram_bits": histogram_bits(sym), **price(prior, ctx, dev, tiles=tiles)}
         out["saved"] = 1.0 - out["prior_bits"] / out["histogram_bits"] if out["histogram_bits"] else 0.0
+        if a.stepped:
+            n = min(a.stepped, sym.size)
+            bits = lambda x: -x.double().mean().item() / math.log(2)  # noqa: E731
+            out.update(stepped=n, stepped_bits=bits(raster_logprobs(prior, tiles, dev, alphabet, n)), packed_bits=bits(packed_logprobs(prior, ctx, tiles, dev)[:n]))
         print(json.dumps(out), flush=True)
 
 
