@@ -198,7 +198,8 @@ int ntc_op_layer_norm_backward(const ntc_layer_norm_desc* d, void* stream, char*
  * contiguous [tokens][heads][head_dim] and do not overlap what they are made from. A token has a position (an integer) on each of `axes` axes; axis m turns sections[m] pairs of a head's elements, in
  * order: pair p of all P is elements p and p + P, or with `interleaved` 2p and 2p + 1; elements from 2 P on stay as they are. The angle of an axis's pair j is its position times
  * base^(-j / sections[m]), or with one_ladder, of pair p, base^(-p / P). (a, b) becomes (a cos - b sin, a sin + b cos); with `backward` the
- * sine's sign is changed, which is the gradient. Frequencies are good to 2^-57 and angles are fractions of a turn in 64 bits, however far the position; sines, cosines and sums are 32-bit, rounded once. */
+ * sine's sign is changed, which is the gradient. Frequencies are good to 2^-57 of them and angles are fractions of a turn in 64 bits: an angle is off by no more than its position times
+ * (2^-57 of its frequency + 2^-65 of a turn). Sines, cosines and sums are 32-bit, rounded once. */
 enum { NTC_ROTARY_AXES = 8, NTC_ROTARY_PAIRS = 128 };
 typedef struct ntc_rotary_desc {
     const void* positions;                 /* [tokens] rows of `axes` integers, at position_stride elements */

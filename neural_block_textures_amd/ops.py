@@ -340,7 +340,8 @@ def rotary(positions: torch.Tensor, q: torch.Tensor, k: Optional[torch.Tensor] =
     positions [.., axes]: int32 or int64, a token's place on each of 1 to 8 axes (time, row, column, channel). q and k [.., heads, elements]: float32, bfloat16 or float16, any
     strides. sections: how many pairs of a head each axis turns, 128 in all at most; pair p of P is elements p and p + P, or with `interleaved` 2p and 2p + 1, and elements from 2 P on
     stay as they are. Axis a's pair j turns by its position times base^(-j / sections[a]); with one_ladder pair p by its axis's position times base^(-p / P).
-    Angles keep the frequencies' 57 bits however far a position is; sines, cosines and sums are 32-bit, rounded once. Differentiable (once) in q and k.
+    Angles are made in 64 bits, and off by no more than the position times (2^-57 of the frequency + 2^-65 of a turn): 2^-24 at 2^33. Sines, cosines and sums are 32-bit, rounded once.
+    Differentiable (once) in q and k.
     """
     out = _binding().rotary(positions, q, k, list(sections), base, one_ladder, interleaved)
     return out[0] if k is None else out
